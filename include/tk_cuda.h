@@ -309,6 +309,138 @@ int tk_paged_attention_async(tk_device *dev, const float *q, const float *k_cach
                              uint32_t num_heads, uint32_t head_dim, uint32_t max_blocks,
                              void *stream);
 
+/* ---- serving step over a key/value cache held in 4 bits ------------------------------------
+ * No counterpart in the reference, whose PagedAttention (src/kernels/attention.zig:51-100) reads
+ * an f32 cache with one query token per sequence and as many key heads as query heads.  One step:
+ *   tk_paged_slots      the requests' lengths -> block tables, positions and slots
+ *   tk_qk_norm_rope     norm and rotation of the step's queries and keys
+ *   tk_kv4_append       its keys and values, quantised into their slots
+ *   tk_kv4_attention    its queries over the pages
+ * Every length, page and slot is read on the device, so a step captured into a CUDA graph is
+ * replayed with other lengths: capture it with as many rows (max_tokens, tokens) as a step may
+ * have; the rows behind the last token carry position -1 and slot -1 and are left as they were.
+ * No call keeps state, allocates or waits: calls on different streams or from different threads
+ * are independent as long as they share no output and no workspace.  The _async forms take the
+ * stream as all others do; cudaStreamLegacy ((void *)1) names the legacy default stream.
+ *
+ * The cache:  codes u8 [block][kv_head][block_size][head_dim/2], even dimension in the low nibble,
+ *             scales f16 [block][kv_head][block_size][head_dim/group_size][2], (scale, offset);
+ *             value = code * scale + offset.
+ * block_size 16, 32, 64, 128 or 256; head_dim 64, 128 or 256; group_size 64 or 128, at most
+ * head_dim; num_blocks * block_size < 2^31; the four arrays on 16-byte boundaries.  A slot is
+ * block * block_size + token within the block. */
+#define TK_F32 0
+#define TK_F16 1
+#define TK_BF16 2
+
+typedef struct tk_kv4_cache {
+  uint8_t *k_codes;
+  uint8_t *v_codes;
+  uint16_t *k_scales;
+  uint16_t *v_scales;
+  uint32_t num_blocks, kv_heads, block_size, head_dim, group_size;
+} tk_kv4_cache;
+
+/* Block tables and slots of a step.  Request b has context_lens[b] tokens in the cache, in the
+ * pages of block_tables[b][0 .. ceil(context_lens[b] / block_size)), and query_lens[b] new ones
+ * (negative lengths count as 0).  Pages that the step needs are taken from
+ * free_blocks[free_range[0] .. free_range[1]) in the order of the requests and of their pages, and
+ * written into block_tables (all other entries stay).  Written:
+ *   kv_lens[b]      context_lens[b] + query_lens[b]
+ *   query_start[b]  index of the request's first token among the step's; query_start[batch]: all
+ *   positions[t], slots[t]  of the step's token t; -1, -1 from the last token to max_tokens
+ *   counts[4]       tokens of the step; pages it needs; tokens without a slot; free_range[0] plus
+ *                   the pages taken
+ * A page that the list does not have, or whose id is outside [0, num_blocks), enters the table as
+ * -1 and its tokens get slot -1, as do tokens past max_blocks pages; counts[2] counts them.
+ * Tokens past max_tokens are cut off from the last requests (kv_lens and query_start go by what
+ * remains).  The inputs are not changed: the caller moves free_range on by counts[1].  The outputs
+ * must not be the inputs.  int32 throughout. */
+int tk_paged_slots(tk_device *dev, const int32_t *context_lens, const int32_t *query_lens,
+                   const int32_t *free_blocks, const int32_t *free_range, int32_t *block_tables,
+                   int32_t *kv_lens, int32_t *query_start, int32_t *positions, int32_t *slots,
+                   int32_t *counts, uint32_t batch, uint32_t max_blocks, uint32_t block_size,
+                   uint32_t num_blocks, uint32_t max_tokens);
+int tk_paged_slots_async(tk_device *dev, const int32_t *context_lens, const int32_t *query_lens,
+                         const int32_t *free_blocks, const int32_t *free_range,
+                         int32_t *block_tables, int32_t *kv_lens, int32_t *query_start,
+                         int32_t *positions, int32_t *slots, int32_t *counts, uint32_t batch,
+                         uint32_t max_blocks, uint32_t block_size, uint32_t num_blocks,
+                         uint32_t max_tokens, void *stream);
+
+/* Norm of each head of the queries and keys, and their rotation, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight      (q_weight / k_weight NULL: y = x)
+ * then over the first rot_dim dimensions, with c, s = cos/sin_cache[position * rot_dim/2 + j]:
+ *   (y[j], y[j + rot_dim/2])  by default, (y[2j], y[2j+1]) with TK_ROPE_INTERLEAVED
+ *   (a, b) -> (a*c - b*s, b*c + a*s)
+ * q rows of q_heads * head_dim, k rows of kv_heads * head_dim, of type dtype (f32 inside, rounded
+ * once); rows are the given strides (in elements, 0: packed) apart, so q and k may be parts of one
+ * projection's rows.  The outputs may be the inputs (same pointer, same stride), else must not
+ * overlap them.  q_heads or kv_heads may be 0 (its pointers unused).  A token whose position is
+ * outside [0, max_pos) leaves its rows as they were.  head_dim even, at most 1024; rot_dim even,
+ * at most head_dim, 0 for the norm alone. */
+#define TK_ROPE_INTERLEAVED 1u
+int tk_qk_norm_rope(tk_device *dev, const void *q, const void *k, const float *q_weight,
+                    const float *k_weight, const float *cos_cache, const float *sin_cache,
+                    const int32_t *positions, void *q_out, void *k_out, uint32_t tokens,
+                    uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rot_dim,
+                    uint32_t max_pos, uint32_t q_stride, uint32_t k_stride, uint32_t q_out_stride,
+                    uint32_t k_out_stride, float eps, int dtype, uint32_t flags);
+int tk_qk_norm_rope_async(tk_device *dev, const void *q, const void *k, const float *q_weight,
+                          const float *k_weight, const float *cos_cache, const float *sin_cache,
+                          const int32_t *positions, void *q_out, void *k_out, uint32_t tokens,
+                          uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t rot_dim,
+                          uint32_t max_pos, uint32_t q_stride, uint32_t k_stride,
+                          uint32_t q_out_stride, uint32_t k_out_stride, float eps, int dtype,
+                          uint32_t flags, void *stream);
+
+/* Writes the keys and values of `tokens` tokens into their slots, quantised per group of
+ * group_size dimensions: offset = f16(min), scale = f16((max - min) / 15), code = the integer
+ * nearest to (x - offset) / scale (ties to even), in 0..15; a group of one value has scale 0.
+ * Finite values past the f16 range saturate; a group that holds an infinity or a NaN reads back as
+ * NaN.  k and v: rows of kv_heads * head_dim of type dtype, strides as above.  A token whose slot
+ * is outside the cache (-1) is not written.  The slots of a call must differ: of two tokens in one
+ * slot, parts of either may remain. */
+int tk_kv4_append(tk_device *dev, const tk_kv4_cache *cache, const void *k, const void *v,
+                  const int32_t *slots, uint32_t tokens, uint32_t k_stride, uint32_t v_stride,
+                  int dtype);
+int tk_kv4_append_async(tk_device *dev, const tk_kv4_cache *cache, const void *k, const void *v,
+                        const int32_t *slots, uint32_t tokens, uint32_t k_stride,
+                        uint32_t v_stride, int dtype, void *stream);
+/* Reads the keys and values of `tokens` slots back (code * scale + offset, rounded once to dtype);
+ * the rows of slots outside the cache stay as they were. */
+int tk_kv4_gather(tk_device *dev, const tk_kv4_cache *cache, const int32_t *slots, void *k,
+                  void *v, uint32_t tokens, uint32_t k_stride, uint32_t v_stride, int dtype);
+int tk_kv4_gather_async(tk_device *dev, const tk_kv4_cache *cache, const int32_t *slots, void *k,
+                        void *v, uint32_t tokens, uint32_t k_stride, uint32_t v_stride, int dtype,
+                        void *stream);
+
+/* Attention over the cache.  Sequence b has the query tokens query_start[b] .. query_start[b+1]
+ * (NULL: one each, tokens == batch) and kv_lens[b] tokens in the cache, its query tokens the last
+ * of them: query i of n sees the positions below kv_lens[b] - n + i + 1,
+ *   o = softmax(scale * q . K^T) V  over them, position t in page block_tables[b][t / block_size].
+ * Grouped heads: query head h reads key head h / (q_heads / kv_heads).  q and o: [tokens] rows of
+ * q_heads * head_dim of type dtype, strides in elements (0: packed); o may be q.  The sequences'
+ * ranges must not overlap; rows of no sequence are left as they were, and nothing behind a
+ * sequence's last token is read.  A query that sees nothing gives zeros.  kv_lens past max_blocks *
+ * block_size is cut there; a page whose id is outside [0, num_blocks) counts as absent.  Results do
+ * not depend on the run (fixed order of sums).
+ * workspace: tk_kv4_attention_workspace bytes of device memory on a 16-byte boundary, not
+ * initialised, for calls that do not run at the same time. */
+int tk_kv4_attention_workspace(tk_device *dev, const tk_kv4_cache *cache, uint32_t q_heads,
+                               size_t *bytes);
+int tk_kv4_attention(tk_device *dev, const tk_kv4_cache *cache, const void *q,
+                     const int32_t *block_tables, const int32_t *kv_lens,
+                     const int32_t *query_start, void *o, void *workspace, size_t workspace_bytes,
+                     uint32_t tokens, uint32_t batch, uint32_t q_heads, uint32_t max_blocks,
+                     uint32_t q_stride, uint32_t o_stride, float scale, int dtype);
+int tk_kv4_attention_async(tk_device *dev, const tk_kv4_cache *cache, const void *q,
+                           const int32_t *block_tables, const int32_t *kv_lens,
+                           const int32_t *query_start, void *o, void *workspace,
+                           size_t workspace_bytes, uint32_t tokens, uint32_t batch,
+                           uint32_t q_heads, uint32_t max_blocks, uint32_t q_stride,
+                           uint32_t o_stride, float scale, int dtype, void *stream);
+
 /* ---- sampler ----------------------------------------------------------------------------
  * Replaces the argmax shader (src/kernels/shaders.zig:889-943; the host loop of
  * src/model/llama.zig:290-303): out[0] = index of the largest of x[0..n).  Ties go to the smallest

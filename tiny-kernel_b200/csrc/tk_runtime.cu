@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -25,6 +26,7 @@
 #include "tk_decode.h"
 #include "tk_engine.h"
 #include "tk_internal.h"
+#include "tk_kv4.h"
 
 using namespace tk;
 
@@ -1290,6 +1292,309 @@ int tk_paged_attention(tk_device* d, const float* q, const float* kc, const floa
                        uint32_t heads, uint32_t head_dim, uint32_t max_blocks) {
   int st = tk_paged_attention_async(d, q, kc, vc, bt, cl, o, batch, heads, head_dim, max_blocks,
                                     nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
+// ---- serving step over the 4-bit cache (tk_kv4.cu, tk_kv4_attention.cu) --------------------------
+// The arguments are checked before the device, so that a refusal needs none.  These entry points
+// leave the calling thread's current device as they found it.
+
+namespace {
+
+struct DeviceScope {
+  int previous = -1;
+  int enter(tk_device* d) {
+    if (!d) return fail(TK_ERR_ARG, "device is NULL");
+    int now = -1;
+    TK_CUDA_TRY(cudaGetDevice(&now));
+    if (now == d->ordinal) return TK_OK;
+    TK_CUDA_TRY(cudaSetDevice(d->ordinal));
+    previous = now;
+    return TK_OK;
+  }
+  ~DeviceScope() {
+    if (previous >= 0) cudaSetDevice(previous);
+  }
+};
+
+constexpr uint32_t kMaxCount = 0x7fffffffu;
+
+int check_dtype(int dtype) {
+  if (dtype != TK_F32 && dtype != TK_F16 && dtype != TK_BF16) return fail(TK_ERR_ARG, "unknown dtype %d", dtype);
+  return TK_OK;
+}
+
+bool aligned_for(const void* p, int dtype) {
+  return (reinterpret_cast<uintptr_t>(p) & (dtype == TK_F32 ? 3u : 1u)) == 0;
+}
+
+// A stride of rows of `width` values: 0 is packed.
+int check_stride(const char* name, uint32_t stride, uint64_t width, long long* out) {
+  if (stride != 0 && stride < width)
+    return fail(TK_ERR_ARG, "%s stride %u is below the row's %llu values", name, stride, (unsigned long long)width);
+  *out = stride ? (long long)stride : (long long)width;
+  return TK_OK;
+}
+
+int check_cache(const tk_kv4_cache* c, Kv4View* view) {
+  if (!c || !c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales) return fail(TK_ERR_ARG, "NULL cache");
+  if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned16(c->k_scales) || !aligned16(c->v_scales))
+    return fail(TK_ERR_ARG, "the cache's arrays must be on 16-byte boundaries");
+  const uint32_t bs = c->block_size;
+  if (bs < 16 || bs > 256 || (bs & (bs - 1)))
+    return fail(TK_ERR_ARG, "block_size %u is none of 16, 32, 64, 128, 256", bs);
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(TK_ERR_ARG, "head_dim %u is none of 64, 128, 256", c->head_dim);
+  if ((c->group_size != 64 && c->group_size != 128) || c->group_size > c->head_dim)
+    return fail(TK_ERR_ARG, "group_size %u is not 64 or 128 within head_dim %u", c->group_size, c->head_dim);
+  if (c->kv_heads == 0 || c->kv_heads > 65535 || c->num_blocks == 0 || (uint64_t)c->num_blocks * bs > kMaxCount)
+    return fail(TK_ERR_ARG, "cache of %u blocks of %u tokens, %u heads is out of range", c->num_blocks, bs,
+                c->kv_heads);
+  int shift = 0;
+  while ((1u << shift) < bs) ++shift;
+  *view = Kv4View{c->k_codes, c->v_codes, reinterpret_cast<uint32_t*>(c->k_scales),
+                  reinterpret_cast<uint32_t*>(c->v_scales), (int)c->num_blocks, (int)c->kv_heads, shift,
+                  (int)c->head_dim, (int)c->group_size};
+  return TK_OK;
+}
+
+}  // namespace
+
+int tk_paged_slots_async(tk_device* d, const int32_t* context_lens, const int32_t* query_lens,
+                         const int32_t* free_blocks, const int32_t* free_range, int32_t* block_tables,
+                         int32_t* kv_lens, int32_t* query_start, int32_t* positions, int32_t* slots,
+                         int32_t* counts, uint32_t batch, uint32_t max_blocks, uint32_t block_size,
+                         uint32_t num_blocks, uint32_t max_tokens, void* stream) {
+  const int32_t* in[] = {context_lens, query_lens, free_blocks, free_range};
+  int32_t* out[] = {block_tables, kv_lens, query_start, positions, slots, counts};
+  for (const int32_t* i : in)
+    if (!i) return fail(TK_ERR_ARG, "NULL argument");
+  for (int o = 0; o < 6; ++o) {
+    if (!out[o]) return fail(TK_ERR_ARG, "NULL argument");
+    for (const int32_t* i : in)
+      if (out[o] == i) return fail(TK_ERR_ARG, "an output is an input");
+    for (int e = 0; e < o; ++e)
+      if (out[o] == out[e]) return fail(TK_ERR_ARG, "two outputs are the same");
+  }
+  if (block_size < 16 || block_size > 256 || (block_size & (block_size - 1)))
+    return fail(TK_ERR_ARG, "block_size %u is none of 16, 32, 64, 128, 256", block_size);
+  if (batch == 0 || batch > (1u << 24) || max_blocks == 0 || max_blocks > kMaxCount || num_blocks == 0 ||
+      (uint64_t)num_blocks * block_size > kMaxCount || max_tokens == 0 || max_tokens > kMaxCount - 8)
+    return fail(TK_ERR_ARG, "batch %u, max_blocks %u, num_blocks %u or max_tokens %u is out of range", batch,
+                max_blocks, num_blocks, max_tokens);
+  DeviceScope scope;
+  int st = scope.enter(d);
+  if (st != TK_OK) return st;
+  int shift = 0;
+  while ((1u << shift) < block_size) ++shift;
+  const SlotsParams p{context_lens, query_lens, free_blocks, free_range, block_tables, kv_lens, query_start,
+                      positions, slots, counts, (int)batch, (int)max_blocks, shift, (int)num_blocks,
+                      (int)max_tokens};
+  TK_LAUNCH(d, launch_paged_slots(p, d->sm_count, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_paged_slots(tk_device* d, const int32_t* context_lens, const int32_t* query_lens,
+                   const int32_t* free_blocks, const int32_t* free_range, int32_t* block_tables,
+                   int32_t* kv_lens, int32_t* query_start, int32_t* positions, int32_t* slots,
+                   int32_t* counts, uint32_t batch, uint32_t max_blocks, uint32_t block_size,
+                   uint32_t num_blocks, uint32_t max_tokens) {
+  int st = tk_paged_slots_async(d, context_lens, query_lens, free_blocks, free_range, block_tables, kv_lens,
+                                query_start, positions, slots, counts, batch, max_blocks, block_size,
+                                num_blocks, max_tokens, nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
+int tk_qk_norm_rope_async(tk_device* d, const void* q, const void* k, const float* q_weight,
+                          const float* k_weight, const float* cos_cache, const float* sin_cache,
+                          const int32_t* positions, void* q_out, void* k_out, uint32_t tokens, uint32_t q_heads,
+                          uint32_t kv_heads, uint32_t head_dim, uint32_t rot_dim, uint32_t max_pos,
+                          uint32_t q_stride, uint32_t k_stride, uint32_t q_out_stride, uint32_t k_out_stride,
+                          float eps, int dtype, uint32_t flags, void* stream) {
+  int st = check_dtype(dtype);
+  if (st != TK_OK) return st;
+  if (flags & ~TK_ROPE_INTERLEAVED) return fail(TK_ERR_ARG, "unknown flags 0x%x", flags);
+  if ((q_heads && (!q || !q_out)) || (kv_heads && (!k || !k_out)) || !positions ||
+      (rot_dim && (!cos_cache || !sin_cache)))
+    return fail(TK_ERR_ARG, "NULL argument");
+  if (head_dim == 0 || head_dim % 2 || head_dim > 1024 || rot_dim % 2 || rot_dim > head_dim)
+    return fail(TK_ERR_ARG, "head_dim=%u must be even and at most 1024, rot_dim=%u even and within it", head_dim,
+                rot_dim);
+  if (q_heads > 65535 || kv_heads > 65535 || q_heads + kv_heads == 0 || max_pos == 0 || max_pos > kMaxCount ||
+      (uint64_t)tokens * (q_heads + kv_heads) > kMaxCount)
+    return fail(TK_ERR_ARG, "%u tokens of %u + %u heads, %u positions are out of range", tokens, q_heads,
+                kv_heads, max_pos);
+  QkNormRopeParams p{{q, k}, {q_out, k_out}, {q_weight, k_weight}, {}, {}, {(int)q_heads, (int)kv_heads},
+                     cos_cache, sin_cache, positions, (int)tokens, (int)head_dim, (int)rot_dim, (int)max_pos,
+                     (flags & TK_ROPE_INTERLEAVED) ? 1 : 0, eps};
+  const uint32_t in[2] = {q_stride, k_stride}, out[2] = {q_out_stride, k_out_stride};
+  for (int i = 0; i < 2; ++i) {
+    const char* name = i == 0 ? "q" : "k";
+    const uint64_t width = (uint64_t)p.heads[i] * head_dim;
+    if ((st = check_stride(name, in[i], width, &p.in_stride[i])) != TK_OK) return st;
+    if ((st = check_stride(name, out[i], width, &p.out_stride[i])) != TK_OK) return st;
+    if (p.heads[i] && (!aligned_for(p.x[i], dtype) || !aligned_for(p.out[i], dtype)))
+      return fail(TK_ERR_ARG, "%s is not aligned to its type", name);
+    if (p.heads[i] && p.x[i] == p.out[i] && p.in_stride[i] != p.out_stride[i])
+      return fail(TK_ERR_ARG, "%s in place needs the same stride in and out", name);
+  }
+  if (q_heads && kv_heads && q_out == k_out) return fail(TK_ERR_ARG, "two outputs are the same");
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
+  if (tokens == 0) return TK_OK;
+  TK_LAUNCH(d, launch_qk_norm_rope(p, dtype, d->sm_count, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_qk_norm_rope(tk_device* d, const void* q, const void* k, const float* q_weight, const float* k_weight,
+                    const float* cos_cache, const float* sin_cache, const int32_t* positions, void* q_out,
+                    void* k_out, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                    uint32_t rot_dim, uint32_t max_pos, uint32_t q_stride, uint32_t k_stride,
+                    uint32_t q_out_stride, uint32_t k_out_stride, float eps, int dtype, uint32_t flags) {
+  int st = tk_qk_norm_rope_async(d, q, k, q_weight, k_weight, cos_cache, sin_cache, positions, q_out, k_out,
+                                 tokens, q_heads, kv_heads, head_dim, rot_dim, max_pos, q_stride, k_stride,
+                                 q_out_stride, k_out_stride, eps, dtype, flags, nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
+namespace {
+
+// The arguments that append and gather share.
+int check_rows(const tk_kv4_cache* cache, Kv4View* view, const void* k, const void* v, const int32_t* slots,
+               uint32_t tokens, uint32_t k_stride, uint32_t v_stride, int dtype, long long* ks, long long* vs) {
+  int st = check_cache(cache, view);
+  if (st != TK_OK) return st;
+  if ((st = check_dtype(dtype)) != TK_OK) return st;
+  if (!k || !v || !slots) return fail(TK_ERR_ARG, "NULL argument");
+  if (!aligned_for(k, dtype) || !aligned_for(v, dtype)) return fail(TK_ERR_ARG, "k or v is not aligned to its type");
+  // one thread per 8 values: the grid's limit
+  if ((uint64_t)tokens * cache->kv_heads * cache->head_dim > (1ull << 38))
+    return fail(TK_ERR_ARG, "%u tokens of %u heads are too many for one call", tokens, cache->kv_heads);
+  if (tokens > kMaxCount) return fail(TK_ERR_ARG, "%u tokens are too many for one call", tokens);
+  const uint64_t width = (uint64_t)cache->kv_heads * cache->head_dim;
+  if ((st = check_stride("k", k_stride, width, ks)) != TK_OK) return st;
+  return check_stride("v", v_stride, width, vs);
+}
+
+}  // namespace
+
+int tk_kv4_append_async(tk_device* d, const tk_kv4_cache* cache, const void* k, const void* v,
+                        const int32_t* slots, uint32_t tokens, uint32_t k_stride, uint32_t v_stride, int dtype,
+                        void* stream) {
+  Kv4View view{};
+  long long ks = 0, vs = 0;
+  int st = check_rows(cache, &view, k, v, slots, tokens, k_stride, v_stride, dtype, &ks, &vs);
+  if (st != TK_OK) return st;
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
+  if (tokens == 0) return TK_OK;
+  TK_LAUNCH(d, launch_kv4_append(view, k, v, slots, (int)tokens, ks, vs, dtype, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_kv4_append(tk_device* d, const tk_kv4_cache* cache, const void* k, const void* v, const int32_t* slots,
+                  uint32_t tokens, uint32_t k_stride, uint32_t v_stride, int dtype) {
+  int st = tk_kv4_append_async(d, cache, k, v, slots, tokens, k_stride, v_stride, dtype, nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
+int tk_kv4_gather_async(tk_device* d, const tk_kv4_cache* cache, const int32_t* slots, void* k, void* v,
+                        uint32_t tokens, uint32_t k_stride, uint32_t v_stride, int dtype, void* stream) {
+  Kv4View view{};
+  long long ks = 0, vs = 0;
+  int st = check_rows(cache, &view, k, v, slots, tokens, k_stride, v_stride, dtype, &ks, &vs);
+  if (st != TK_OK) return st;
+  if (k == v) return fail(TK_ERR_ARG, "two outputs are the same");
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
+  if (tokens == 0) return TK_OK;
+  TK_LAUNCH(d, launch_kv4_gather(view, k, v, slots, (int)tokens, ks, vs, dtype, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_kv4_gather(tk_device* d, const tk_kv4_cache* cache, const int32_t* slots, void* k, void* v,
+                  uint32_t tokens, uint32_t k_stride, uint32_t v_stride, int dtype) {
+  int st = tk_kv4_gather_async(d, cache, slots, k, v, tokens, k_stride, v_stride, dtype, nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
+namespace {
+
+int check_heads(const Kv4View& view, uint32_t q_heads) {
+  if (q_heads == 0 || q_heads > 65535 || q_heads % (uint32_t)view.kv_heads)
+    return fail(TK_ERR_ARG, "q_heads=%u must be a positive multiple of kv_heads=%d", q_heads, view.kv_heads);
+  return TK_OK;
+}
+
+}  // namespace
+
+int tk_kv4_attention_workspace(tk_device* d, const tk_kv4_cache* cache, uint32_t q_heads, size_t* bytes) {
+  if (!bytes) return fail(TK_ERR_ARG, "NULL argument");
+  Kv4View view{};
+  int st = check_cache(cache, &view);
+  if (st != TK_OK) return st;
+  if ((st = check_heads(view, q_heads)) != TK_OK) return st;
+  if (!d) return fail(TK_ERR_ARG, "device is NULL");
+  *bytes = kv4_attention_workspace(view.head_dim, d->sm_count);
+  return TK_OK;
+}
+
+int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* q, const int32_t* block_tables,
+                           const int32_t* kv_lens, const int32_t* query_start, void* o, void* workspace,
+                           size_t workspace_bytes, uint32_t tokens, uint32_t batch, uint32_t q_heads,
+                           uint32_t max_blocks, uint32_t q_stride, uint32_t o_stride, float scale, int dtype,
+                           void* stream) {
+  Kv4AttentionParams p{};
+  int st = check_cache(cache, &p.cache);
+  if (st != TK_OK) return st;
+  if ((st = check_heads(p.cache, q_heads)) != TK_OK) return st;
+  if ((st = check_dtype(dtype)) != TK_OK) return st;
+  if (!q || !block_tables || !kv_lens || !o || !workspace) return fail(TK_ERR_ARG, "NULL argument");
+  if (!aligned_for(q, dtype) || !aligned_for(o, dtype)) return fail(TK_ERR_ARG, "q or o is not aligned to its type");
+  if (!aligned16(workspace)) return fail(TK_ERR_ARG, "the workspace must be on a 16-byte boundary");
+  if (batch == 0 || batch > (1u << 24) || max_blocks == 0 || max_blocks > kMaxCount || tokens > kMaxCount ||
+      (uint64_t)tokens * q_heads > kMaxCount)
+    return fail(TK_ERR_ARG, "%u tokens of %u heads in %u sequences of %u blocks are out of range", tokens, q_heads,
+                batch, max_blocks);
+  if (!query_start && tokens != batch)
+    return fail(TK_ERR_ARG, "without query_start there is one token per sequence: %u tokens, batch %u", tokens, batch);
+  if (!std::isfinite(scale)) return fail(TK_ERR_ARG, "scale is not finite");
+  const uint64_t width = (uint64_t)q_heads * cache->head_dim;
+  if ((st = check_stride("q", q_stride, width, &p.q_stride)) != TK_OK) return st;
+  if ((st = check_stride("o", o_stride, width, &p.o_stride)) != TK_OK) return st;
+  if (q == o && p.q_stride != p.o_stride) return fail(TK_ERR_ARG, "in place needs the same stride in and out");
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
+  const size_t need = kv4_attention_workspace(p.cache.head_dim, d->sm_count);
+  if (workspace_bytes < need)
+    return fail(TK_ERR_ARG, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+  if (tokens == 0) return TK_OK;
+  p.q = q;
+  p.o = o;
+  p.block_tables = block_tables;
+  p.kv_lens = kv_lens;
+  p.query_start = query_start;
+  p.workspace = workspace;
+  p.tokens = (int)tokens;
+  p.batch = (int)batch;
+  p.q_heads = (int)q_heads;
+  p.max_blocks = (int)max_blocks;
+  p.scale = scale;
+  TK_LAUNCH(d, launch_kv4_attention(p, dtype, d->sm_count, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_kv4_attention(tk_device* d, const tk_kv4_cache* cache, const void* q, const int32_t* block_tables,
+                     const int32_t* kv_lens, const int32_t* query_start, void* o, void* workspace,
+                     size_t workspace_bytes, uint32_t tokens, uint32_t batch, uint32_t q_heads,
+                     uint32_t max_blocks, uint32_t q_stride, uint32_t o_stride, float scale, int dtype) {
+  int st = tk_kv4_attention_async(d, cache, q, block_tables, kv_lens, query_start, o, workspace, workspace_bytes,
+                                  tokens, batch, q_heads, max_blocks, q_stride, o_stride, scale, dtype, nullptr);
   if (st != TK_OK) return st;
   return sync_and_check(d, d->stream);
 }

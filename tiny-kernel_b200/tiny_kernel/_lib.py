@@ -30,6 +30,10 @@ TK_FFN_HOST_IO = 2
 TK_TP_UNIQUE_ID_BYTES = 128
 TK_Q4_0_REFERENCE_ORDER = 0
 TK_Q4_0_GGML_ORDER = 1
+TK_F32 = 0
+TK_F16 = 1
+TK_BF16 = 2
+TK_ROPE_INTERLEAVED = 1
 
 vp = C.c_void_p
 u32 = C.c_uint32
@@ -40,6 +44,13 @@ i32 = C.c_int
 class Int4MatrixC(C.Structure):
     """tk_int4_matrix: device pointers of one packed INT4 matrix."""
     _fields_ = [("w_packed", vp), ("scales", vp), ("zeros", vp)]
+
+
+class Kv4CacheC(C.Structure):
+    """tk_kv4_cache: device pointers and sizes of a 4-bit key/value cache."""
+    _fields_ = [("k_codes", vp), ("v_codes", vp), ("k_scales", vp), ("v_scales", vp),
+                ("num_blocks", u32), ("kv_heads", u32), ("block_size", u32), ("head_dim", u32),
+                ("group_size", u32)]
 
 
 # name -> (restype, argtypes); the exported surface of include/tk_cuda.h
@@ -85,6 +96,19 @@ SIGNATURES = {
     "tk_repack_q4_0": (i32, [vp, vp, vp, vp, vp, u32, u32, i32]),
     "tk_paged_attention": (i32, [vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32]),
     "tk_paged_attention_async": (i32, [vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, vp]),
+    "tk_paged_slots": (i32, [vp] * 11 + [u32] * 5),
+    "tk_paged_slots_async": (i32, [vp] * 11 + [u32] * 5 + [vp]),
+    "tk_qk_norm_rope": (i32, [vp] * 10 + [u32] * 10 + [f32, i32, u32]),
+    "tk_qk_norm_rope_async": (i32, [vp] * 10 + [u32] * 10 + [f32, i32, u32, vp]),
+    "tk_kv4_append": (i32, [vp, C.POINTER(Kv4CacheC), vp, vp, vp, u32, u32, u32, i32]),
+    "tk_kv4_append_async": (i32, [vp, C.POINTER(Kv4CacheC), vp, vp, vp, u32, u32, u32, i32, vp]),
+    "tk_kv4_gather": (i32, [vp, C.POINTER(Kv4CacheC), vp, vp, vp, u32, u32, u32, i32]),
+    "tk_kv4_gather_async": (i32, [vp, C.POINTER(Kv4CacheC), vp, vp, vp, u32, u32, u32, i32, vp]),
+    "tk_kv4_attention_workspace": (i32, [vp, C.POINTER(Kv4CacheC), u32, C.POINTER(C.c_size_t)]),
+    "tk_kv4_attention": (i32, [vp, C.POINTER(Kv4CacheC)] + [vp] * 6 + [C.c_size_t] + [u32] * 6
+                         + [f32, i32]),
+    "tk_kv4_attention_async": (i32, [vp, C.POINTER(Kv4CacheC)] + [vp] * 6 + [C.c_size_t] + [u32] * 6
+                               + [f32, i32, vp]),
     "tk_argmax": (i32, [vp, vp, u32, vp]),
     "tk_argmax_async": (i32, [vp, vp, u32, vp, vp]),
     "tk_softmax_sample": (i32, [vp, vp, vp, vp, u32, f32, f32]),

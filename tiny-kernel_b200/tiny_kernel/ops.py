@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
-from ._lib import Int4MatrixC, check
+from ._lib import Int4MatrixC, Kv4CacheC, check
 
 
 def _ptr(v) -> int:
@@ -134,6 +134,93 @@ def paged_attention(device, q, k_cache, v_cache, block_tables, context_lens, o, 
                                         _ptr(block_tables), _ptr(context_lens), _ptr(o),
                                         int(batch), int(num_heads), int(head_dim),
                                         int(max_blocks)))
+
+
+_TYPES = {"f32": _lib.TK_F32, "f16": _lib.TK_F16, "bf16": _lib.TK_BF16}
+
+
+def _dtype(dtype) -> int:
+    """A TK_* type code from "f32", "f16", "bf16" or the code itself."""
+    if isinstance(dtype, str):
+        if dtype not in _TYPES:
+            raise ValueError(f"unknown dtype {dtype!r}: f32, f16 or bf16")
+        return _TYPES[dtype]
+    return int(dtype)
+
+
+def _call(name, args, stream, sync):
+    """The synchronous entry point, or with a stream (or sync=False) the one that only queues."""
+    L = _lib.lib()
+    if sync and stream is None:
+        check(getattr(L, name)(*args))
+    else:
+        check(getattr(L, name + "_async")(*args, stream))
+
+
+def paged_slots(device, context_lens, query_lens, free_blocks, free_range, block_tables, kv_lens,
+                query_start, positions, slots, counts, batch, max_blocks, block_size, num_blocks,
+                max_tokens, stream=None, sync=True):
+    """Block tables, positions and slots of a step from the requests' lengths (int32 buffers)."""
+    _call("tk_paged_slots",
+          (_dev(device), _ptr(context_lens), _ptr(query_lens), _ptr(free_blocks), _ptr(free_range),
+           _ptr(block_tables), _ptr(kv_lens), _ptr(query_start), _ptr(positions), _ptr(slots),
+           _ptr(counts), int(batch), int(max_blocks), int(block_size), int(num_blocks),
+           int(max_tokens)), stream, sync)
+
+
+def qk_norm_rope(device, q, k, q_weight, k_weight, cos_cache, sin_cache, positions, q_out, k_out,
+                 tokens, q_heads, kv_heads, head_dim, rot_dim, max_pos, eps, dtype="f32",
+                 interleaved=False, q_stride=0, k_stride=0, q_out_stride=0, k_out_stride=0,
+                 stream=None, sync=True):
+    """Per-head norm (a None weight: none) and rotation of queries and keys at their positions."""
+    _call("tk_qk_norm_rope",
+          (_dev(device), _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), _ptr(cos_cache),
+           _ptr(sin_cache), _ptr(positions), _ptr(q_out), _ptr(k_out), int(tokens), int(q_heads),
+           int(kv_heads), int(head_dim), int(rot_dim), int(max_pos), int(q_stride), int(k_stride),
+           int(q_out_stride), int(k_out_stride), float(eps), _dtype(dtype),
+           _lib.TK_ROPE_INTERLEAVED if interleaved else 0), stream, sync)
+
+
+def kv4_cache(k_codes, v_codes, k_scales, v_scales, num_blocks, kv_heads, block_size, head_dim,
+              group_size) -> Kv4CacheC:
+    """The description of a 4-bit cache that the kv4_* calls take (the buffers stay the caller's)."""
+    return Kv4CacheC(_ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), int(num_blocks),
+                     int(kv_heads), int(block_size), int(head_dim), int(group_size))
+
+
+def kv4_append(device, cache, k, v, slots, tokens, dtype="f32", k_stride=0, v_stride=0, stream=None,
+               sync=True):
+    """Keys and values quantised into their slots (-1: not written)."""
+    _call("tk_kv4_append",
+          (_dev(device), C.byref(cache), _ptr(k), _ptr(v), _ptr(slots), int(tokens), int(k_stride),
+           int(v_stride), _dtype(dtype)), stream, sync)
+
+
+def kv4_gather(device, cache, slots, k, v, tokens, dtype="f32", k_stride=0, v_stride=0, stream=None,
+               sync=True):
+    """Keys and values of slots read back from the cache (-1: the row stays)."""
+    _call("tk_kv4_gather",
+          (_dev(device), C.byref(cache), _ptr(slots), _ptr(k), _ptr(v), int(tokens), int(k_stride),
+           int(v_stride), _dtype(dtype)), stream, sync)
+
+
+def kv4_attention_workspace(device, cache, q_heads) -> int:
+    """Bytes of the workspace that kv4_attention needs."""
+    size = C.c_size_t()
+    check(_lib.lib().tk_kv4_attention_workspace(_dev(device), C.byref(cache), int(q_heads),
+                                                C.byref(size)))
+    return size.value
+
+
+def kv4_attention(device, cache, q, block_tables, kv_lens, query_start, o, workspace,
+                  workspace_bytes, tokens, batch, q_heads, max_blocks, scale, dtype="f32",
+                  q_stride=0, o_stride=0, stream=None, sync=True):
+    """Attention of the step's queries over the 4-bit pages (query_start None: one token each)."""
+    _call("tk_kv4_attention",
+          (_dev(device), C.byref(cache), _ptr(q), _ptr(block_tables), _ptr(kv_lens),
+           _ptr(query_start), _ptr(o), _ptr(workspace), int(workspace_bytes), int(tokens),
+           int(batch), int(q_heads), int(max_blocks), int(q_stride), int(o_stride), float(scale),
+           _dtype(dtype)), stream, sync)
 
 
 def argmax(device, x, n, out):
