@@ -421,10 +421,11 @@ int tk_kv4_gather_async(tk_device *dev, const tk_kv4_cache *cache, const int32_t
  *   o = softmax(scale * q . K^T) V  over them, position t in page block_tables[b][t / block_size].
  * Grouped heads: query head h reads key head h / (q_heads / kv_heads).  q and o: [tokens] rows of
  * q_heads * head_dim of type dtype, strides in elements (0: packed); o may be q.  The sequences'
- * ranges must not overlap; rows of no sequence are left as they were, and nothing behind a
- * sequence's last token is read.  A query that sees nothing gives zeros.  kv_lens past max_blocks *
- * block_size is cut there; a page whose id is outside [0, num_blocks) counts as absent.  Results do
- * not depend on the run (fixed order of sums).
+ * ranges must not overlap; rows of no sequence are left as they were, and what the cache holds at
+ * positions that a query does not see does not matter.  A query that sees nothing gives zeros.
+ * kv_lens past max_blocks * block_size (below 2^31 - 1024) is cut there; a page whose id is outside
+ * [0, num_blocks) counts as absent.  Products and sums hold f32 precision for every dtype and do
+ * not depend on the run (fixed order); scale * q may reach 2^118.
  * workspace: tk_kv4_attention_workspace bytes of device memory on a 16-byte boundary, not
  * initialised, for calls that do not run at the same time. */
 int tk_kv4_attention_workspace(tk_device *dev, const tk_kv4_cache *cache, uint32_t q_heads,

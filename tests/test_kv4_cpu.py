@@ -87,6 +87,7 @@ GOOD_ATTENTION = dict(q=U, tables=T, kv_lens=S, start=A, o=V, ws=W, size=1 << 30
     (dict(ws=0), "NULL"), (dict(ws=W + 8), "16-byte"), (dict(q_heads=3), "q_heads=3"),
     (dict(q_heads=0), "q_heads=0"), (dict(dtype=7), "dtype 7"), (dict(batch=0), "out of range"),
     (dict(max_blocks=0), "out of range"), (dict(tokens=1 << 31), "out of range"),
+    (dict(max_blocks=1 << 27), "positions"),
     (dict(start=None), "one token per sequence"), (dict(scale=float("nan")), "scale"),
     (dict(scale=float("inf")), "scale"), (dict(qs=511), "q stride 511"), (dict(os=100), "o stride 100"),
     (dict(o=U, qs=512, os=520), "in place"), (dict(q=U + 2), "aligned"), (dict(o=V + 1, dtype=1), "aligned"),

@@ -1561,6 +1561,8 @@ int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* 
       (uint64_t)tokens * q_heads > kMaxCount)
     return fail(TK_ERR_ARG, "%u tokens of %u heads in %u sequences of %u blocks are out of range", tokens, q_heads,
                 batch, max_blocks);
+  if ((uint64_t)max_blocks * cache->block_size > kMaxCount - 1024)
+    return fail(TK_ERR_ARG, "max_blocks=%u of %u tokens: positions are out of range", max_blocks, cache->block_size);
   if (!query_start && tokens != batch)
     return fail(TK_ERR_ARG, "without query_start there is one token per sequence: %u tokens, batch %u", tokens, batch);
   if (!std::isfinite(scale)) return fail(TK_ERR_ARG, "scale is not finite");
@@ -1585,6 +1587,7 @@ int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* 
   p.q_heads = (int)q_heads;
   p.max_blocks = (int)max_blocks;
   p.scale = scale;
+  ++d->launches;  // two kernels
   TK_LAUNCH(d, launch_kv4_attention(p, dtype, d->sm_count, pick_stream(d, stream)));
   return TK_OK;
 }
