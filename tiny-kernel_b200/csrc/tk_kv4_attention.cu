@@ -6,14 +6,15 @@
 // query that sees no position gets zeros.
 //
 // The mathematics.  Scales and offsets stay out of the products (c: codes, per group of dimensions):
-//     q . k   = sum_g s_k (q . c)_g + m_k (sum q)_g
-//     sum p v = sum (p s_v) (c - 8)  +  sum p (m_v + 8 s_v)
-// so both products are f16 x f16 tensor-core products with exact codes: keys as f16 subnormals
-// (c * 2^-24, or c * 2^-20 from the high nibble, the matching queries divided by 16: one AND per two
-// codes), values as c - 8 (without the shift the sums would carry 7.5 times the weights, and a long
-// flat softmax would lose its digits against it).  f32 queries and weights are split into two f16
-// (22 bits), which take the rows g and g + 8 of the same m16n8k16 product: the heads of a group and
-// the query tokens of a sequence (rows, 8 to a tile) fill the upper half, the remainders the lower.
+//     q . k   = sum_g s_k (q . (c - 8))_g + (m_k + 8 s_k) (sum q)_g
+//     sum p v = sum (p s_v) (c - 8)       + sum p (m_v + 8 s_v)
+// (Without the shift by 8 the sums carry 7.5 times the sum of the factors, and a long flat softmax
+// loses its digits against it.)
+//   Queries against keys: integers.  A row of queries, scaled by a power of two to 30 bits, is four
+// signed 8-bit digits; the codes are bytes after one AND (and a shift for the odd dimensions); the
+// sums are exact.  The digits of 8 rows fill the 16 rows of two m16n8k32 products.
+//   Weights against values: f16.  c - 8 is exact, p s_v is split into two f16 (22 bits), which take
+// the rows g and g + 8 of one m16n8k16 product.
 // mma.sync and not tcgen05: one token of a head group is 8 rows, an eighth of tcgen05's smallest
 // tile, whose operands would also have to pass through shared memory unpacked.
 //
@@ -33,12 +34,15 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;       // rows (query token, head of the group) of a tile
-constexpr int kUnit = 16;      // tokens of a warp's step; a page holds whole units
-constexpr int kStep = kUnit * kWarps;
-constexpr int kStages = 4;
+constexpr int kUnit = 16;      // tokens that lie in one page for sure
+constexpr int kSub = 2;        // units of a warp's step
+constexpr int kTokens = kUnit * kSub;
+constexpr int kStep = kTokens * kWarps;
+constexpr int kStages = 3;
+constexpr int kTileCost = 2;   // steps that a tile costs beside its own: queries, first loads, join
 
-// Work is (sequence, key head, row tile, step of 64 tokens) in this order, cut into equal runs, one
-// per CTA (Kv4Run).  A run that ends inside a (sequence, head, tile) leaves its sums in the
+// Work is (sequence, key head, row tile, step of 128 tokens) in this order, cut into equal runs, one
+// per CTA; a tile counts kTileCost steps more than it has, before its first.  A run that ends inside a (sequence, head, tile) leaves its sums in the
 // workspace; the CTA in whose run the tile begins describes it, and a second kernel joins the parts
 // in the order of the CTAs.  A CTA has at most two parts: the end of a tile in slot 0, the beginning
 // of one in slot 1.
@@ -69,6 +73,17 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -86,9 +101,6 @@ __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
-  return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(b) << 16;
 }
 __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)w)); }
 __device__ __forceinline__ float half_hi(uint32_t w) {
@@ -111,38 +123,56 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t x) {
   return y;
 }
 
-// A stage of a warp's ring: 16 tokens of codes and pairs.  16-byte pieces are placed so that no two
-// lanes of a load meet in a bank: the keys of token x in row krow(x), piece c ^ kflip(x); the values
-// of token 4t + r in row 4r + t, piece c ^ vflip(t).
+// Two f32 as f16 (a in the low half), and what that leaves of them.
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(b), "f"(a));
+  return y;
+}
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_f16(a, b);
+  lo = pack_f16(a - half_lo(hi), b - half_hi(hi));
+}
+
+// A stage of a warp's ring: kSub units of 16 tokens' codes and pairs.  Piece c (16 bytes) of a
+// token's row lies at c ^ flip(token), so that the 8 rows of an ldmatrix and the lanes of a load of
+// keys meet in no bank.
 template <int D, int G>
 struct Stage {
   static constexpr int NG = D / G;
   static constexpr int kRowBytes = D / 2;
-  static constexpr int kPieces = D / 32;  // 16-byte pieces of a row
+  static constexpr int kPieces = D / 32;
   static constexpr int kCodes = kUnit * kRowBytes;
   static constexpr int kPairs = kUnit * NG * 4;
-  static constexpr int kBytes = 2 * (kCodes + kPairs);
-  static __device__ __forceinline__ int krow(int x) { return D == 64 ? x ^ ((x >> 2 & 1) << 1) : x; }
-  static __device__ __forceinline__ int kflip(int x) {
-    if (D == 64) return 0;
-    if (D == 128) return (x >> 2 & 1) << 1;
-    return G == 128 ? (x & 1) << 2 : (x & 1) << 1 | (x >> 2 & 1) << 2;
+  static constexpr int kUnitBytes = 2 * (kCodes + kPairs);
+  static constexpr int kBytes = kSub * kUnitBytes;
+  static __device__ __forceinline__ int flip(int x) {
+    return ((x & 1) << 2 | (x & 2) | (x >> 2 & 1)) & (kPieces - 1);
   }
-  static __device__ __forceinline__ int vflip(int t) { return D == 64 ? 0 : D == 128 ? (t >> 1) << 1 : t << 1; }
-  static __device__ __forceinline__ int key_at(int token, int byte) {
-    return krow(token) * kRowBytes + ((byte / 16 ^ kflip(token)) * 16 + byte % 16);
-  }
-  static __device__ __forceinline__ int value_at(int token, int byte) {
-    return ((token & 3) * 4 + token / 4) * kRowBytes + ((byte / 16 ^ vflip(token / 4)) * 16 + byte % 16);
+  static __device__ __forceinline__ int at(int token, int byte) {
+    return token * kRowBytes + (byte / 16 ^ flip(token)) * 16 + byte % 16;
   }
 };
+
+// The (scale, offset) pairs of group y of tokens 2t, 2t + 1, 8 + 2t, 9 + 2t of a unit.
+template <int NG>
+__device__ __forceinline__ void load_pairs(const uint8_t* pairs, int t, int y, uint32_t (&out)[4]) {
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(pairs) + 2 * t * NG + y;
+  if constexpr (NG == 1) {
+    const uint2 a = *reinterpret_cast<const uint2*>(src), b = *reinterpret_cast<const uint2*>(src + 8);
+    out[0] = a.x, out[1] = a.y, out[2] = b.x, out[3] = b.y;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[r] = src[((r & 2) * 4 + (r & 1)) * NG];
+  }
+}
 
 struct Sequence {
   int first, n;     // query tokens
   int kv;           // visible positions, at most the table's reach
   int last;         // kv_len - n: query i sees the positions below last + i + 1
   int tiles;        // row tiles
-  int steps;        // of a tile; 1 at least, so that empty contexts get their zeros
+  int steps;        // of a tile, its cost among them
 };
 __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b, int per) {
   Sequence s;
@@ -157,14 +187,14 @@ __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b,
   s.last = len - s.n;
   s.kv = (int)min((long long)len, (long long)p.max_blocks << p.cache.shift);
   s.tiles = (int)(((long long)s.n * per + kRows - 1) / kRows);
-  s.steps = max(1, (s.kv + kStep - 1) / kStep);  // kv < 2^31 - 1024
+  s.steps = kTileCost + (s.kv + kStep - 1) / kStep;  // kv < 2^31 - 1024
   return s;
 }
 
 template <int D, int G>
 __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kernel(Kv4AttentionParams p, int dtype) {
   using S = Stage<D, G>;
-  constexpr int NG = S::NG, KS = D / 16, NT = D / 8;
+  constexpr int NG = S::NG, KW = D / 32, NT = D / 8;  // KW: words of a lane's keys, 32 dimensions of the row each
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ long long s_warp[kWarps];
   __shared__ long long s_at;
@@ -221,105 +251,146 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
   float* joint = reinterpret_cast<float*>(ring);  // after the ring: 8 rows of D sums, 8 x (reference, l)
 
+  // where the lane's pieces go in a unit, and where its operands lie
+  uint32_t piece_dst[S::kCodes / 512];
+#pragma unroll
+  for (int i = 0; i < S::kCodes / 512; ++i) {
+    const int piece = i * 32 + lane;
+    piece_dst[i] = S::at(piece / S::kPieces, piece % S::kPieces * 16);
+  }
+  const uint32_t pair_dst = 2 * S::kCodes + (lane < 16 ? 0 : S::kPairs) + (lane & 15) * 16;
+  int k_at[NG];
+#pragma unroll
+  for (int y = 0; y < NG; ++y) k_at[y] = S::at(g, y * (G / 2) + t * (G / 8));
+  // ldmatrix: lanes 0-7, 8-15 the rows of tokens 0-7, 8-15 at one piece, lanes 16-31 at the next
+  const uint32_t v_row = S::kCodes + (lane & 15) * S::kRowBytes, v_piece = (lane >> 4) ^ S::flip(lane & 15);
+  const size_t page_rows = (size_t)hk << p.cache.shift;
+  const int page_mask = (1 << p.cache.shift) - 1;
+
   for (long long at = start; at < stop; ++b, offset = 0) {
     const Sequence s = sequence(p, b, per);
     const long long in_seq = (long long)s.steps * s.tiles * hk;
     while (at < stop && offset < in_seq) {
-      const int unit = (int)(offset / s.steps), s0 = (int)(offset % s.steps);
-      const int s1 = (int)min((long long)s.steps, s0 + (stop - at));
+      const int unit = (int)(offset / s.steps), c0 = (int)(offset % s.steps);
+      const int c1 = (int)min((long long)s.steps, c0 + (stop - at));
       const int head = unit / s.tiles, row0 = (unit % s.tiles) * kRows;
       const int rows = min(kRows, s.n * per - row0);
-      const bool whole = s0 == 0 && s1 == s.steps;
+      const bool whole = c0 == 0 && c1 == s.steps;
+      const int s0 = max(c0 - kTileCost, 0), s1 = max(c1 - kTileCost, 0);
       // positions that the tile's last row sees, and this lane's row
       const int see_tile = min(s.kv, s.last + (row0 + rows - 1) / per + 1);
       const int my_row = row0 + min(g, rows - 1);
       const int see = min(s.kv, s.last + my_row / per + 1);
       const int* table = p.block_tables + (size_t)b * p.max_blocks;
 
-      // ---- queue of loads ----
-      unsigned valid = 0;
-      auto page_of = [&](int step) {
-        const int pos = step * kStep + warp * kUnit;
-        return step < s1 && pos < see_tile ? __ldg(table + (pos >> p.cache.shift)) : -1;
-      };
-      auto issue = [&](int stage, int step, int page) {
-        const int pos = step * kStep + warp * kUnit;
-        const long long row = kv4_row(p.cache, page, head, pos & ((1 << p.cache.shift) - 1));
-        valid &= ~(1u << stage);
-        if (row >= 0) {
-          valid |= 1u << stage;
-          const uint32_t dst = ring_addr + stage * S::kBytes;
-          const uint8_t* kc = p.cache.k_codes + row * S::kRowBytes;
-          const uint8_t* vc = p.cache.v_codes + row * S::kRowBytes;
+      // ---- queue of loads: a unit is four runs of consecutive bytes ----
+      const size_t head_row = (size_t)head << p.cache.shift;
+      const uint8_t* k_src = p.cache.k_codes + head_row * S::kRowBytes + lane * 16;
+      const uint8_t* v_src = p.cache.v_codes + head_row * S::kRowBytes + lane * 16;
+      const uint32_t* pair_src = (lane < 16 ? p.cache.k_scales : p.cache.v_scales) + head_row * NG + (lane & 15) * 4;
+      unsigned valid = 0;  // kSub bits a stage
+      auto page_of = [&](int pos) { return pos < see_tile ? __ldg(table + (pos >> p.cache.shift)) : -1; };
+      auto issue = [&](int stage, int step, const int (&page)[kSub]) {
 #pragma unroll
-          for (int i = 0; i < S::kCodes / 512; ++i) {
-            const int piece = i * 32 + lane, token = piece / S::kPieces, byte = piece % S::kPieces * 16;
-            cp_async16(dst + S::key_at(token, byte), kc + piece * 16);
-            cp_async16(dst + S::kCodes + S::value_at(token, byte), vc + piece * 16);
-          }
-          if ((lane & 15) < 4 * NG) {
-            const uint32_t* src = (lane < 16 ? p.cache.k_scales : p.cache.v_scales) + row * NG + (lane & 15) * 4;
-            cp_async16(dst + 2 * S::kCodes + (lane < 16 ? 0 : S::kPairs) + (lane & 15) * 16, src);
+        for (int u = 0; u < kSub; ++u) {
+          const int pos = step * kStep + warp * kTokens + u * kUnit;
+          const unsigned bit = 1u << (stage * kSub + u);
+          valid &= ~bit;
+          if (step < s1 && page[u] >= 0 && page[u] < p.cache.num_blocks) {
+            valid |= bit;
+            const size_t row = (size_t)page[u] * page_rows + (pos & page_mask);
+            const uint32_t dst = ring_addr + stage * S::kBytes + u * S::kUnitBytes;
+#pragma unroll
+            for (int i = 0; i < S::kCodes / 512; ++i) {
+              cp_async16(dst + piece_dst[i], k_src + row * S::kRowBytes + i * 512);
+              cp_async16(dst + S::kCodes + piece_dst[i], v_src + row * S::kRowBytes + i * 512);
+            }
+            if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, pair_src + row * NG);
           }
         }
         cp_commit();
       };
+      int page[kSub];
+      auto look = [&](int step) {
 #pragma unroll
-      for (int i = 0; i < kStages - 1; ++i) issue(i, s0 + i, page_of(s0 + i));
-      int page_next = page_of(s0 + kStages - 1);
+        for (int u = 0; u < kSub; ++u)
+          page[u] = step < s1 ? page_of(step * kStep + warp * kTokens + u * kUnit) : -1;
+      };
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) {
+        look(s0 + i);
+        issue(i, s0 + i, page);
+      }
+      look(s0 + kStages - 1);
 
-      // ---- queries: scaled, normalised by a power of two, split ----
-      uint32_t qf[KS][4];
+      // ---- queries: scaled, as integers of 30 bits, in digits ----
+      uint32_t qd[KW][2][4];  // [..][0]: rows g, g + 8 the highest digit and the next, [1]: the lower two
       float qsum[NG], unscale;
+      int centre[NG][2];  // -8 times the sums of the upper and of the lower two digits
       {
         float q[D / 4];  // the lane's dimensions of row g: G/4 consecutive ones of each group
         const long long at_q = (long long)(s.first + my_row / per) * p.q_stride +
                                (long long)(head * per + my_row % per) * D;
         const float f = p.scale * 1.4426950408889634f;
-        float top = 0.f;
+        float top = 0.f, odd = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 4; ++i) {
           const int d = i / (G / 4) * G + t * (G / 4) + i % (G / 4);
-          q[i] = load_any(p.q, at_q + d, dtype) * f;
+          q[i] = see > 0 ? load_any(p.q, at_q + d, dtype) * f : 0.f;
           top = fmaxf(top, fabsf(q[i]));
+          odd = fmaf(q[i], 0.f, odd);  // NaN if one is not finite
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the largest becomes 2^14 .. 2^15; a row of zeros, infinities or NaN goes as it is
-        int e = 0;
-        if (top > 0.f && top < INFINITY) e = min(max(14 - ilogbf(top), -100), 120);
+        odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+        odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+        // the largest becomes 2^29 .. 2^30
+        const int e = top > 0.f && top < INFINITY ? min(29 - ilogbf(top), 120) : 0;
         const float norm = ldexpf(1.f, e);
-        unscale = ldexpf(1.f, 24 - e);
+        unscale = ldexpf(1.f, -e) + odd;
 #pragma unroll
         for (int y = 0; y < NG; ++y) {
           float sum = 0.f;
+          int upper = 0, lower = 0;
 #pragma unroll
-          for (int i = 0; i < G / 4; ++i) sum += q[y * (G / 4) + i];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          qsum[y] = sum;
-        }
+          for (int i = 0; i < G / 32; ++i) {
+            const int w = y * (G / 32) + i;
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w)
+            for (int h = 0; h < 2; ++h) {  // the even, the odd dimensions of the word
+              uint32_t d[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x[4];  // codes 2h, 2h + 4 of the word, then 2h + 1, 2h + 5 (a factor 16 up)
-            x[0] = q[8 * w + 2 * h] * norm;
-            x[1] = q[8 * w + 2 * h + 4] * norm;
-            x[2] = q[8 * w + 2 * h + 1] * norm * 0.0625f;
-            x[3] = q[8 * w + 2 * h + 5] * norm * 0.0625f;
-            __half hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              hi[i] = __float2half_rn(x[i]);
-              lo[i] = __float2half_rn(x[i] - __half2float(hi[i]));
+              for (int k = 0; k < 4; ++k) {
+                int x = __float2int_rn(q[8 * w + 2 * k + h] * norm);
+                sum += (float)x;
+                const int d0 = (int8_t)x;
+                x = (x - d0) >> 8;
+                const int d1 = (int8_t)x;
+                x = (x - d1) >> 8;
+                const int d2 = (int8_t)x;
+                x = (x - d2) >> 8;
+                upper += x * 256 + d2;
+                lower += d1 * 256 + d0;
+                d[0] |= (uint32_t)(x & 255) << (8 * k);
+                d[1] |= (uint32_t)(d2 & 255) << (8 * k);
+                d[2] |= (uint32_t)(d1 & 255) << (8 * k);
+                d[3] |= (uint32_t)(d0 & 255) << (8 * k);
+              }
+              qd[w][0][2 * h] = d[0];
+              qd[w][0][2 * h + 1] = d[1];
+              qd[w][1][2 * h] = d[2];
+              qd[w][1][2 * h + 1] = d[3];
             }
-            uint32_t(&a)[4] = qf[2 * w + h];
-            a[0] = pack2(hi[0], hi[1]);
-            a[1] = pack2(lo[0], lo[1]);
-            a[2] = pack2(hi[2], hi[3]);
-            a[3] = pack2(lo[2], lo[3]);
           }
+#pragma unroll
+          for (int off = 1; off < 4; off <<= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            upper += __shfl_xor_sync(0xffffffffu, upper, off);
+            lower += __shfl_xor_sync(0xffffffffu, lower, off);
+          }
+          qsum[y] = sum;
+          centre[y][0] = -8 * upper;
+          centre[y][1] = -8 * lower;
+        }
       }
 
       float o[NT][4], off_sum[NG], l = 0.f, ref = -INFINITY;  // weights are 2^(s - ref + 10) s_v
@@ -329,64 +400,73 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
       for (int y = 0; y < NG; ++y) off_sum[y] = 0.f;
 
       // ---- the steps ----
+      int stage = 0;
       for (int step = s0; step < s1; ++step) {
-        const int stage = (step - s0) % kStages;
         cp_wait<kStages - 2>();
         __syncwarp();
-        const bool there = valid >> stage & 1;
-        issue((stage + kStages - 1) % kStages, step + kStages - 1, page_next);
-        page_next = page_of(step + kStages);
-        if (!there) continue;
+        const unsigned there = valid >> (stage * kSub) & ((1u << kSub) - 1);
+        issue(stage == 0 ? kStages - 1 : stage - 1, step + kStages - 1, page);
+        look(step + kStages);
         const uint8_t* st = ring + stage * S::kBytes;
-        const uint32_t* kpair = reinterpret_cast<const uint32_t*>(st + 2 * S::kCodes) + 4 * t * NG;
-        const uint32_t* vpair = reinterpret_cast<const uint32_t*>(st + 2 * S::kCodes + S::kPairs) + 4 * t * NG;
-        const int left = see - (step * kStep + warp * kUnit + 4 * t);  // of the lane's 4 tokens, row g sees so many
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+        if (!there) continue;
+        int left[kSub];  // positions that row g sees from token 2t of a unit on
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+          left[u] = there >> u & 1 ? see - (step * kStep + warp * kTokens + u * kUnit + 2 * t) : 0;
 
-        // scores of tokens 4t + r
-        float sc[4] = {0.f, 0.f, 0.f, 0.f};
+        // scores of tokens 2t, 2t + 1, 8 + 2t, 9 + 2t of the units, in units of unscale
+        float sc[kSub][4], top = -INFINITY;
 #pragma unroll
-        for (int y = 0; y < NG; ++y) {
-          float c[2][4];
+        for (int u = 0; u < kSub; ++u) {
+          const uint8_t* su = st + u * S::kUnitBytes;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-            const int token = 4 * (g >> 1) + 2 * j + (g & 1);
-            uint32_t w[G / 32];
-            const uint8_t* src = st + S::key_at(token, y * (G / 2) + t * (G / 8));
-            if constexpr (G == 128)
-              *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
-            else
-              *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
+          for (int r = 0; r < 4; ++r) sc[u][r] = 0.f;
 #pragma unroll
-            for (int i = 0; i < G / 32; ++i) {
-              const int ks = y * (G / 16) + 2 * i;
-              mma16816(c[j], qf[ks], w[i] & 0x000F000Fu, w[i] & 0x00F000F0u);
-              const uint32_t v = w[i] >> 8;
-              mma16816(c[j], qf[ks + 1], v & 0x000F000Fu, v & 0x00F000F0u);
+          for (int y = 0; y < NG; ++y) {
+            uint32_t pair[4];
+            load_pairs<NG>(su + 2 * S::kCodes, t, y, pair);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t w[G / 32];
+              const uint8_t* src = su + k_at[y] + j * 8 * S::kRowBytes;
+              if constexpr (G == 128)
+                *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
+              else
+                *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
+              int c[2][4] = {};
+#pragma unroll
+              for (int i = 0; i < G / 32; ++i) {
+                const uint32_t even = w[i] & 0x0F0F0F0Fu, odd = w[i] >> 4 & 0x0F0F0F0Fu;
+                mma16832(c[0], qd[y * (G / 32) + i][0], even, odd);
+                mma16832(c[1], qd[y * (G / 32) + i][1], even, odd);
+              }
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float upper = (float)(c[0][i] * 256 + c[0][2 + i] + centre[y][0]);
+                const float lower = (float)(c[1][i] * 256 + c[1][2 + i] + centre[y][1]);
+                const float dot = fmaf(upper, 65536.f, lower);
+                const float ks = half_lo(pair[2 * j + i]), km = fmaf(ks, 8.f, half_hi(pair[2 * j + i]));
+                sc[u][2 * j + i] = fmaf(dot, ks, fmaf(qsum[y], km, sc[u][2 * j + i]));
+              }
             }
+          }
+          // reference: the row's largest s + log2 of the value scale
+          float most[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) most[r] = 5.9604645e-8f;  // 2^-24, the least f16
+#pragma unroll
+          for (int y = 0; y < NG; ++y) {
+            uint32_t pair[4];
+            load_pairs<NG>(su + 2 * S::kCodes + S::kPairs, t, y, pair);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) most[r] = fmaxf(most[r], fabsf(half_lo(pair[r])));
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const uint32_t pair = kpair[r * NG + y];
-            const float dot = c[r >> 1][r & 1] + c[r >> 1][2 + (r & 1)];
-            sc[r] += dot * unscale * half_lo(pair) + qsum[y] * half_hi(pair);
+            if ((r & 2) * 4 + (r & 1) >= left[u]) sc[u][r] = -INFINITY;
+            top = fmaxf(top, fmaf(sc[u][r], unscale, lg2(most[r])));
           }
-        }
-
-        // reference: the row's largest s + log2 of the value scale
-        float vs[NG][4], vm[NG][4], top = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float most = 5.9604645e-8f;  // 2^-24, the least f16
-#pragma unroll
-          for (int y = 0; y < NG; ++y) {
-            const uint32_t pair = r < left ? vpair[r * NG + y] : 0u;
-            vs[y][r] = half_lo(pair);
-            vm[y][r] = fmaf(vs[y][r], 8.f, half_hi(pair));
-            most = fmaxf(most, fabsf(vs[y][r]));
-          }
-          if (r >= left) sc[r] = -INFINITY;
-          top = fmaxf(top, sc[r] + lg2(most));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -405,44 +485,48 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
             o[i][3] *= f;
           }
         }
-        const float base = ref == -INFINITY ? 0.f : ref - 10.f;
-        float pr[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          pr[r] = ex2(sc[r] - base);
-          l += pr[r];
-        }
+        const float base = ref == -INFINITY ? 0.f : 10.f - ref;
 
 #pragma unroll
-        for (int y = 0; y < NG; ++y) {
-          uint32_t a[4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float w0 = pr[2 * h] * vs[y][2 * h], w1 = pr[2 * h + 1] * vs[y][2 * h + 1];
-            const __half h0 = __float2half_rn(w0), h1 = __float2half_rn(w1);
-            a[2 * h] = pack2(h0, h1);
-            a[2 * h + 1] = pack2(__float2half_rn(w0 - __half2float(h0)), __float2half_rn(w1 - __half2float(h1)));
-            off_sum[y] = fmaf(pr[2 * h], vm[y][2 * h], fmaf(pr[2 * h + 1], vm[y][2 * h + 1], off_sum[y]));
-          }
-          uint32_t w[4][G / 64];
+        for (int u = 0; u < kSub; ++u) {
+          const uint8_t* su = st + u * S::kUnitBytes;
+          float pr[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const uint8_t* src = st + S::kCodes + S::value_at(4 * t + r, y * (G / 2) + g * (G / 16));
-            if constexpr (G == 128)
-              *reinterpret_cast<uint2*>(w[r]) = *reinterpret_cast<const uint2*>(src);
-            else
-              w[r][0] = *reinterpret_cast<const uint32_t*>(src);
+            pr[r] = ex2(fmaf(sc[u][r], unscale, base));
+            l += pr[r];
           }
 #pragma unroll
-          for (int v = 0; v < G / 64; ++v)
+          for (int y = 0; y < NG; ++y) {
+            uint32_t pair[4], a[4];
+            load_pairs<NG>(su + 2 * S::kCodes + S::kPairs, t, y, pair);
+            float w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {  // byte k of the four tokens' words: dimensions 2k, 2k + 1
-              const uint32_t x = __byte_perm(w[0][v], w[1][v], k | k << 4 | (k + 4) << 8 | (k + 4) << 12);
-              const uint32_t z = __byte_perm(w[2][v], w[3][v], k | k << 4 | (k + 4) << 8 | (k + 4) << 12);
-              const int n = (y * (G / 64) + v) * 8 + 2 * k;
-              mma16816(o[n], a, codes_lo(x), codes_lo(z));
-              mma16816(o[n + 1], a, codes_hi(x), codes_hi(z));
+            for (int r = 0; r < 4; ++r) {
+              if ((r & 2) * 4 + (r & 1) >= left[u]) pair[r] = 0;  // what is not seen may be NaN
+              const float vs = half_lo(pair[r]);
+              w[r] = pr[r] * vs;
+              off_sum[y] = fmaf(pr[r], fmaf(vs, 8.f, half_hi(pair[r])), off_sum[y]);
             }
+            split_f16(w[0], w[1], a[0], a[1]);
+            split_f16(w[2], w[3], a[2], a[3]);
+#pragma unroll
+            for (int z = y * (G / 32); z < (y + 1) * (G / 32); z += 2) {  // 32 dimensions each
+              uint32_t c[4];  // of 4 dimensions: tokens 2t, 2t + 1; 8 + 2t, 9 + 2t; then of the next 32
+              ldmatrix_trans(c, ring_addr + (uint32_t)(su - ring) + v_row + (v_piece ^ z) * 16);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int n = (z + h) * 4;
+                uint32_t b0 = c[2 * h], b1 = c[2 * h + 1];
+                mma16816(o[n], a, codes_lo(b0), codes_lo(b1));
+                mma16816(o[n + 1], a, codes_hi(b0), codes_hi(b1));
+                b0 >>= 8;
+                b1 >>= 8;
+                mma16816(o[n + 2], a, codes_lo(b0), codes_lo(b1));
+                mma16816(o[n + 3], a, codes_hi(b0), codes_hi(b1));
+              }
+            }
+          }
         }
       }
       cp_wait<0>();
@@ -456,13 +540,11 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
         off_sum[y] += __shfl_xor_sync(0xffffffffu, off_sum[y], 1);
         off_sum[y] += __shfl_xor_sync(0xffffffffu, off_sum[y], 2);
 #pragma unroll
-        for (int v = 0; v < G / 64; ++v)
+        for (int z = y * (G / 32); z < (y + 1) * (G / 32); ++z)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int n = (y * (G / 64) + v) * 8 + e;
-            const int d = y * G + 8 * v + e;  // of column 0; the next column is G/8 on
-            joint[g * D + d + 2 * t * (G / 8)] = o[n][0] + o[n][2] + off_sum[y];
-            joint[g * D + d + (2 * t + 1) * (G / 8)] = o[n][1] + o[n][3] + off_sum[y];
+          for (int e = 0; e < 4; ++e) {  // columns 2t, 2t + 1: dimensions 8t + e, 8t + 4 + e of the 32
+            joint[g * D + z * 32 + 8 * t + e] = o[z * 4 + e][0] + o[z * 4 + e][2] + off_sum[y];
+            joint[g * D + z * 32 + 8 * t + 4 + e] = o[z * 4 + e][1] + o[z * 4 + e][3] + off_sum[y];
           }
       }
       if (t == 0) {
@@ -502,13 +584,13 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
           }
         }
       }
-      if (!whole && s0 == 0 && tid == 0) {  // the tile begins here: where its parts are
+      if (!whole && c0 == 0 && tid == 0) {  // the tile begins here: where its parts are
         const long long end = at + s.steps;
         parts[blockIdx.x] = Part{s.first, rows, head, (int)((end - 1) / run - blockIdx.x + 1), row0, slot, 0, 0};
       }
       __syncthreads();
-      at += s1 - s0;
-      offset += s1 - s0;
+      at += c1 - c0;
+      offset += c1 - c0;
     }
   }
 }
