@@ -595,33 +595,54 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
   }
 }
 
+// Joins the parts of the tile that begins in the run of CTA blockIdx.x.  kJoinWarps warps a row, each
+// with every kJoinWarps-th part, then in the order of the warps.
+constexpr int kJoinWarps = 4;
+
 template <int D>
-__global__ void __launch_bounds__(kRows * 32) kv4_join_kernel(Kv4AttentionParams p, int dtype) {
+__global__ void __launch_bounds__(kRows * kJoinWarps * 32) kv4_join_kernel(Kv4AttentionParams p, int dtype) {
+  __shared__ float s_sum[kRows][kJoinWarps];
+  __shared__ float s_v[kRows][kJoinWarps][D];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const Part* parts = static_cast<const Part*>(p.workspace);
   const float* sums = reinterpret_cast<const float*>(parts + gridDim.x);
   constexpr int kSlot = kRows * (D + 2);
   const Part part = parts[blockIdx.x];
-  const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (row >= part.rows || part.count == 0) return;
-  const int per = p.q_heads / p.cache.kv_heads;
+  if (part.count == 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = warp / kJoinWarps, w = warp % kJoinWarps;
   auto base = [&](int i) { return sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot; };
   float top = -INFINITY;
-  for (int i = 0; i < part.count; ++i) top = fmaxf(top, base(i)[kRows * D + 2 * row]);
+  for (int i = lane; i < part.count; i += 32) top = fmaxf(top, base(i)[kRows * D + 2 * row]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   float sum = 0.f, v[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) v[e] = 0.f;
-  for (int i = 0; i < part.count; ++i) {
+#pragma unroll 4
+  for (int i = w; i < part.count; i += kJoinWarps) {
     const float* s = base(i);
     const float r = s[kRows * D + 2 * row];
     const float f = r == -INFINITY ? 1.f : ex2(r - top);  // no reference: sums of 0, or of NaN
-    sum += s[kRows * D + 2 * row + 1] * f;
+    sum = fmaf(s[kRows * D + 2 * row + 1], f, sum);
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) v[e] += s[row * D + e * 32 + lane] * f;
+    for (int e = 0; e < D / 32; ++e) v[e] = fmaf(s[row * D + e * 32 + lane], f, v[e]);
   }
-  const int q = part.row0 + row;
-  const long long at = (long long)(part.token + q / per) * p.o_stride + (long long)(part.head * per + q % per) * D;
+  if (lane == 0) s_sum[row][w] = sum;
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) store_any(p.o, at + e * 32 + lane, dtype, sum == 0.f ? 0.f : v[e] / sum);
+  for (int e = 0; e < D / 32; ++e) s_v[row][w][e * 32 + lane] = v[e];
+  __syncthreads();
+  if (row >= part.rows) return;
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) sum += s_sum[row][i];
+  const int per = p.q_heads / p.cache.kv_heads, q = part.row0 + row;
+  const long long at = (long long)(part.token + q / per) * p.o_stride + (long long)(part.head * per + q % per) * D;
+  for (int d = w * 32 + lane; d < D; d += kJoinWarps * 32) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) x += s_v[row][i][d];
+    store_any(p.o, at + d, dtype, sum == 0.f ? 0.f : x / sum);
+  }
 }
 
 int attention_ctas(int head_dim, int sm_count) { return sm_count * (head_dim == 256 ? 2 : 3); }
@@ -629,15 +650,27 @@ int attention_ctas(int head_dim, int sm_count) { return sm_count * (head_dim == 
 template <int D, int G>
 cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStream_t st) {
   const size_t smem = (size_t)kWarps * kStages * Stage<D, G>::kBytes;
+  cudaError_t e;
   if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_attention_kernel<D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(kv4_attention_kernel<D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
   }
   const int ctas = attention_ctas(D, sm_count);
   kv4_attention_kernel<D, G><<<ctas, kThreads, smem, st>>>(p, dtype);
-  kv4_join_kernel<D><<<ctas, kRows * 32, 0, st>>>(p, dtype);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // a programmatic launch: set up while the attention runs, past its wait when that has completed
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kRows * kJoinWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, p, dtype);
 }
 
 }  // namespace
