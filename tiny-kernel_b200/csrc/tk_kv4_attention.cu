@@ -38,7 +38,10 @@ constexpr int kUnit = 16;      // tokens that lie in one page for sure
 constexpr int kSub = 2;        // units of a warp's step
 constexpr int kTokens = kUnit * kSub;
 constexpr int kStep = kTokens * kWarps;
-constexpr int kStages = 3;
+template <int D>
+constexpr int kRing = D == 256 ? 2 : 3;  // stages of a warp's ring: as many as leave 3 (2) CTAs on an SM
+constexpr int kFlush = 16;     // steps between two settings aside of the sums
+constexpr int kMinRun = 1;
 constexpr int kTileCost = 2;   // steps that a tile costs beside its own: queries, first loads, join
 
 // Work is (sequence, key head, row tile, step of 128 tokens) in this order, cut into equal runs, one
@@ -57,6 +60,31 @@ __device__ __forceinline__ float load_any(const void* base, long long i, int dty
   if (dtype == kTypeF32) return static_cast<const float*>(base)[i];
   if (dtype == kTypeF16) return __half2float(static_cast<const __half*>(base)[i]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
+}
+// 8 consecutive values of a row.
+__device__ __forceinline__ void load_row8(const void* base, long long i, int dtype, float (&v)[8]) {
+  const int size = dtype == kTypeF32 ? 4 : 2;
+  const uint8_t* src = static_cast<const uint8_t*>(base) + i * size;
+  if (reinterpret_cast<uintptr_t>(src) & 15) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = load_any(base, i + k, dtype);
+    return;
+  }
+  const uint4 x = reinterpret_cast<const uint4*>(src)[0];
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  if (dtype == kTypeF32) {
+    const uint4 z = reinterpret_cast<const uint4*>(src)[1];
+    const uint32_t w2[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]), v[4 + k] = __uint_as_float(w2[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[2 * k] = dtype == kTypeF16 ? __half2float(__ushort_as_half((unsigned short)w[k])) : __uint_as_float(w[k] << 16);
+      v[2 * k + 1] = dtype == kTypeF16 ? __half2float(__ushort_as_half((unsigned short)(w[k] >> 16)))
+                                       : __uint_as_float(w[k] & 0xFFFF0000u);
+    }
+  }
 }
 __device__ __forceinline__ void store_any(void* base, long long i, int dtype, float v) {
   if (dtype == kTypeF32)
@@ -77,6 +105,12 @@ __device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], ui
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same, the sum starting at 0.
+__device__ __forceinline__ void mma16832_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -154,19 +188,6 @@ struct Stage {
   }
 };
 
-// The (scale, offset) pairs of group y of tokens 2t, 2t + 1, 8 + 2t, 9 + 2t of a unit.
-template <int NG>
-__device__ __forceinline__ void load_pairs(const uint8_t* pairs, int t, int y, uint32_t (&out)[4]) {
-  const uint32_t* src = reinterpret_cast<const uint32_t*>(pairs) + 2 * t * NG + y;
-  if constexpr (NG == 1) {
-    const uint2 a = *reinterpret_cast<const uint2*>(src), b = *reinterpret_cast<const uint2*>(src + 8);
-    out[0] = a.x, out[1] = a.y, out[2] = b.x, out[3] = b.y;
-  } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) out[r] = src[((r & 2) * 4 + (r & 1)) * NG];
-  }
-}
-
 struct Sequence {
   int first, n;     // query tokens
   int kv;           // visible positions, at most the table's reach
@@ -191,9 +212,26 @@ __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b,
   return s;
 }
 
+// Shared memory of a CTA: the tile's queries as operands, its rows' numbers, then per warp the ring
+// and the step's scales and offsets in f32.
+template <int D, int G>
+struct Smem {
+  using S = Stage<D, G>;
+  static constexpr int kQuery = D / 32 * 32 * 32;              // [word][lane][8] digits of 32 bits
+  static constexpr int kRowWords = 1 + 3 * S::NG;              // unscale; sum, two centres a group
+  static constexpr int kRowBytes = kRows * kRowWords * 4;
+  static constexpr int kFloats = (S::NG * kUnit * 4 + kUnit) * kSub;  // [unit][k, v][group][token][2]; [unit][token]
+  static constexpr int kWarp = kRing<D> * S::kBytes + kFloats * 4;
+  static constexpr int kBytes = kQuery + kRowBytes + kWarps * kWarp;
+  static constexpr int kJoint = D + 1;  // floats of a row of sums at the end: rows fall into different banks
+  static_assert(kRows * (kJoint + 2) * 4 <= kWarp && kRowBytes % 16 == 0 && kWarp % 16 == 0, "");
+};
+
 template <int D, int G>
 __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kernel(Kv4AttentionParams p, int dtype) {
   using S = Stage<D, G>;
+  using M = Smem<D, G>;
+  constexpr int kStages = kRing<D>;
   constexpr int NG = S::NG, KW = D / 32, NT = D / 8;  // KW: words of a lane's keys, 32 dimensions of the row each
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ long long s_warp[kWarps];
@@ -204,6 +242,8 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
   Part* parts = static_cast<Part*>(p.workspace);
   float* sums = reinterpret_cast<float*>(parts + gridDim.x);
   constexpr int kSlot = kRows * (D + 2);
+  // this warp's sums of earlier steps (kFlush): [product][lane]
+  float* kept = sums + (size_t)gridDim.x * 2 * kSlot + ((size_t)blockIdx.x * kWarps + warp) * kRows * D + lane;
 
   // ---- this CTA's run ----
   const int chunk = (p.batch + kThreads - 1) / kThreads;
@@ -227,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
     if (w < warp) before += s_warp[w];
     total += s_warp[w];
   }
-  const long long run = (total + gridDim.x - 1) / gridDim.x;
+  const long long run = max((total + gridDim.x - 1) / gridDim.x, (long long)kMinRun);
   const long long start = run * blockIdx.x, stop = min(start + run, total);
   if (tid == 0) parts[blockIdx.x].count = 0;
   if (start >= stop) return;
@@ -247,9 +287,14 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
   int b = s_seq;
   long long offset = s_at;  // of the run's next step in its sequence
 
-  uint8_t* ring = smem + warp * kStages * S::kBytes;
+  uint32_t* query = reinterpret_cast<uint32_t*>(smem);
+  float* row_num = reinterpret_cast<float*>(smem + M::kQuery);
+  uint8_t* ring = smem + M::kQuery + M::kRowBytes + warp * M::kWarp;
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-  float* joint = reinterpret_cast<float*>(ring);  // after the ring: 8 rows of D sums, 8 x (reference, l)
+  float* pairs = reinterpret_cast<float*>(ring + kStages * S::kBytes);
+  constexpr int kUnitPairs = NG * kUnit * 4;      // floats of a unit's pairs
+  float* logs = pairs + kSub * kUnitPairs;        // log2 of the units' largest value scales
+  float* joint = reinterpret_cast<float*>(ring);  // after the steps: 8 rows of D sums, 8 x (reference, l)
 
   // where the lane's pieces go in a unit, and where its operands lie
   uint32_t piece_dst[S::kCodes / 512];
@@ -277,10 +322,9 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
       const int rows = min(kRows, s.n * per - row0);
       const bool whole = c0 == 0 && c1 == s.steps;
       const int s0 = max(c0 - kTileCost, 0), s1 = max(c1 - kTileCost, 0);
-      // positions that the tile's last row sees, and this lane's row
-      const int see_tile = min(s.kv, s.last + (row0 + rows - 1) / per + 1);
-      const int my_row = row0 + min(g, rows - 1);
-      const int see = min(s.kv, s.last + my_row / per + 1);
+      // positions that row r sees; the tile's last row sees most, its first least
+      auto sees = [&](int r) { return min(s.kv, s.last + (row0 + min(r, rows - 1)) / per + 1); };
+      const int see_most = sees(kRows - 1), see_least = sees(0), see = sees(g);
       const int* table = p.block_tables + (size_t)b * p.max_blocks;
 
       // ---- queue of loads: a unit is four runs of consecutive bytes ----
@@ -289,15 +333,22 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
       const uint8_t* v_src = p.cache.v_codes + head_row * S::kRowBytes + lane * 16;
       const uint32_t* pair_src = (lane < 16 ? p.cache.k_scales : p.cache.v_scales) + head_row * NG + (lane & 15) * 4;
       unsigned valid = 0;  // kSub bits a stage
-      auto page_of = [&](int pos) { return pos < see_tile ? __ldg(table + (pos >> p.cache.shift)) : -1; };
-      auto issue = [&](int stage, int step, const int (&page)[kSub]) {
+      int page[kSub];
+      auto look = [&](int step) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
           const int pos = step * kStep + warp * kTokens + u * kUnit;
+          page[u] = step < s1 && pos < see_most ? __ldg(table + (pos >> p.cache.shift)) : -1;
+        }
+      };
+      auto issue = [&](int stage, int step) {
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
           const unsigned bit = 1u << (stage * kSub + u);
           valid &= ~bit;
-          if (step < s1 && page[u] >= 0 && page[u] < p.cache.num_blocks) {
+          if (page[u] >= 0 && page[u] < p.cache.num_blocks) {
             valid |= bit;
+            const int pos = step * kStep + warp * kTokens + u * kUnit;
             const size_t row = (size_t)page[u] * page_rows + (pos & page_mask);
             const uint32_t dst = ring_addr + stage * S::kBytes + u * S::kUnitBytes;
 #pragma unroll
@@ -310,87 +361,99 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
         }
         cp_commit();
       };
-      int page[kSub];
-      auto look = [&](int step) {
-#pragma unroll
-        for (int u = 0; u < kSub; ++u)
-          page[u] = step < s1 ? page_of(step * kStep + warp * kTokens + u * kUnit) : -1;
-      };
 #pragma unroll
       for (int i = 0; i < kStages - 1; ++i) {
         look(s0 + i);
-        issue(i, s0 + i, page);
+        issue(i, s0 + i);
       }
       look(s0 + kStages - 1);
 
-      // ---- queries: scaled, as integers of 30 bits, in digits ----
-      uint32_t qd[KW][2][4];  // [..][0]: rows g, g + 8 the highest digit and the next, [1]: the lower two
-      float qsum[NG], unscale;
-      int centre[NG][2];  // -8 times the sums of the upper and of the lower two digits
-      {
-        float q[D / 4];  // the lane's dimensions of row g: G/4 consecutive ones of each group
-        const long long at_q = (long long)(s.first + my_row / per) * p.q_stride +
-                               (long long)(head * per + my_row % per) * D;
+      // ---- queries: scaled, as integers of 30 bits, in digits; 8 dimensions a thread ----
+      constexpr int LPR = D / 8;  // threads of a row
+#pragma unroll
+      for (int r0 = 0; r0 < kRows; r0 += kThreads / LPR) {
+        const int r = r0 + tid / LPR, at8 = tid % LPR;
+        if (r >= kRows) continue;  // whole warps
+        const int row = row0 + min(r, rows - 1);
+        float q[8];
+        if (sees(r) > 0)
+          load_row8(p.q, (long long)(s.first + row / per) * p.q_stride + (long long)(head * per + row % per) * D + at8 * 8,
+                    dtype, q);
+        else
+#pragma unroll
+          for (int i = 0; i < 8; ++i) q[i] = 0.f;
         const float f = p.scale * 1.4426950408889634f;
         float top = 0.f, odd = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 4; ++i) {
-          const int d = i / (G / 4) * G + t * (G / 4) + i % (G / 4);
-          q[i] = see > 0 ? load_any(p.q, at_q + d, dtype) * f : 0.f;
+        for (int i = 0; i < 8; ++i) {
+          q[i] *= f;
           top = fmaxf(top, fabsf(q[i]));
           odd = fmaf(q[i], 0.f, odd);  // NaN if one is not finite
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        odd += __shfl_xor_sync(0xffffffffu, odd, 1);
-        odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+#pragma unroll
+        for (int off = LPR / 2; off > 0; off >>= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          odd += __shfl_xor_sync(0xffffffffu, odd, off);
+        }
         // the largest becomes 2^29 .. 2^30
         const int e = top > 0.f && top < INFINITY ? min(29 - ilogbf(top), 120) : 0;
         const float norm = ldexpf(1.f, e);
-        unscale = ldexpf(1.f, -e) + odd;
+        float sum = 0.f;
+        int upper = 0, lower = 0;
+        uint32_t digits[2][4] = {};  // of the even, the odd dimensions; highest first
 #pragma unroll
-        for (int y = 0; y < NG; ++y) {
-          float sum = 0.f;
-          int upper = 0, lower = 0;
-#pragma unroll
-          for (int i = 0; i < G / 32; ++i) {
-            const int w = y * (G / 32) + i;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {  // the even, the odd dimensions of the word
-              uint32_t d[4] = {0, 0, 0, 0};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                int x = __float2int_rn(q[8 * w + 2 * k + h] * norm);
-                sum += (float)x;
-                const int d0 = (int8_t)x;
-                x = (x - d0) >> 8;
-                const int d1 = (int8_t)x;
-                x = (x - d1) >> 8;
-                const int d2 = (int8_t)x;
-                x = (x - d2) >> 8;
-                upper += x * 256 + d2;
-                lower += d1 * 256 + d0;
-                d[0] |= (uint32_t)(x & 255) << (8 * k);
-                d[1] |= (uint32_t)(d2 & 255) << (8 * k);
-                d[2] |= (uint32_t)(d1 & 255) << (8 * k);
-                d[3] |= (uint32_t)(d0 & 255) << (8 * k);
-              }
-              qd[w][0][2 * h] = d[0];
-              qd[w][0][2 * h + 1] = d[1];
-              qd[w][1][2 * h] = d[2];
-              qd[w][1][2 * h + 1] = d[3];
-            }
-          }
-#pragma unroll
-          for (int off = 1; off < 4; off <<= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            upper += __shfl_xor_sync(0xffffffffu, upper, off);
-            lower += __shfl_xor_sync(0xffffffffu, lower, off);
-          }
-          qsum[y] = sum;
-          centre[y][0] = -8 * upper;
-          centre[y][1] = -8 * lower;
+        for (int i = 0; i < 8; ++i) {
+          int x = __float2int_rn(q[i] * norm);
+          sum += (float)x;
+          const int d0 = (int8_t)x;
+          x = (x - d0) >> 8;
+          const int d1 = (int8_t)x;
+          x = (x - d1) >> 8;
+          const int d2 = (int8_t)x;
+          x = (x - d2) >> 8;
+          upper += x * 256 + d2;
+          lower += d1 * 256 + d0;
+          digits[i & 1][0] |= (uint32_t)(x & 255) << (i / 2 * 8);
+          digits[i & 1][1] |= (uint32_t)(d2 & 255) << (i / 2 * 8);
+          digits[i & 1][2] |= (uint32_t)(d1 & 255) << (i / 2 * 8);
+          digits[i & 1][3] |= (uint32_t)(d0 & 255) << (i / 2 * 8);
         }
+#pragma unroll
+        for (int off = G / 16; off > 0; off >>= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, off);
+          upper += __shfl_xor_sync(0xffffffffu, upper, off);
+          lower += __shfl_xor_sync(0xffffffffu, lower, off);
+        }
+        const int y = at8 / (G / 8), tt = at8 % (G / 8) / (G / 32), w = y * (G / 32) + at8 % (G / 32);
+        // two products, upper and lower digits; a0: row g, even; a1: row g + 8; a2, a3: odd
+        uint32_t* dst = query + (w * 32 + r * 4 + tt) * 8;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(digits[0][0], digits[0][1], digits[1][0], digits[1][1]);
+        *reinterpret_cast<uint4*>(dst + 4) = make_uint4(digits[0][2], digits[0][3], digits[1][2], digits[1][3]);
+        float* num = row_num + r * M::kRowWords;
+        if (at8 == 0) num[0] = ldexpf(1.f, -e) + odd;
+        if (at8 % (G / 8) == 0) {
+          num[1 + 3 * y] = sum;
+          num[2 + 3 * y] = __int_as_float(-8 * upper);
+          num[3 + 3 * y] = __int_as_float(-8 * lower);
+        }
+      }
+      __syncthreads();
+      uint32_t qd[KW][2][4];
+      float qsum[NG];
+      int centre[NG][2];  // -8 times the sums of the upper and of the lower digits
+#pragma unroll
+      for (int w = 0; w < KW; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 v = *reinterpret_cast<const uint4*>(query + (w * 32 + lane) * 8 + 4 * h);
+          qd[w][h][0] = v.x, qd[w][h][1] = v.y, qd[w][h][2] = v.z, qd[w][h][3] = v.w;
+        }
+      const float unscale = row_num[g * M::kRowWords];
+#pragma unroll
+      for (int y = 0; y < NG; ++y) {
+        qsum[y] = row_num[g * M::kRowWords + 1 + 3 * y];
+        centre[y][0] = __float_as_int(row_num[g * M::kRowWords + 2 + 3 * y]);
+        centre[y][1] = __float_as_int(row_num[g * M::kRowWords + 3 + 3 * y]);
       }
 
       float o[NT][4], off_sum[NG], l = 0.f, ref = -INFINITY;  // weights are 2^(s - ref + 10) s_v
@@ -398,6 +461,8 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
       for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
       for (int y = 0; y < NG; ++y) off_sum[y] = 0.f;
+      bool flushed = false;
+      int since = 0;  // steps since the sums were set aside
 
       // ---- the steps ----
       int stage = 0;
@@ -405,18 +470,39 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
         cp_wait<kStages - 2>();
         __syncwarp();
         const unsigned there = valid >> (stage * kSub) & ((1u << kSub) - 1);
-        issue(stage == 0 ? kStages - 1 : stage - 1, step + kStages - 1, page);
+        issue(stage == 0 ? kStages - 1 : stage - 1, step + kStages - 1);
         look(step + kStages);
         const uint8_t* st = ring + stage * S::kBytes;
         stage = stage == kStages - 1 ? 0 : stage + 1;
         if (!there) continue;
-        int left[kSub];  // positions that row g sees from token 2t of a unit on
+        const int pos = step * kStep + warp * kTokens;
+
+        // scales and offsets in f32, of keys by lanes 0-15, of values by lanes 16-31; 0 for what the
+        // tile does not see (it may hold anything)
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
-          left[u] = there >> u & 1 ? see - (step * kStep + warp * kTokens + u * kUnit + 2 * t) : 0;
+        for (int u = 0; u < kSub; ++u) {
+          const bool on = (there >> u & 1) && pos + u * kUnit + (lane & 15) < see_most;
+          const uint32_t* src =
+              reinterpret_cast<const uint32_t*>(st + u * S::kUnitBytes + 2 * S::kCodes + (lane < 16 ? 0 : S::kPairs)) +
+              (lane & 15) * NG;
+          float2* dst = reinterpret_cast<float2*>(pairs + u * kUnitPairs + (lane < 16 ? 0 : NG * kUnit * 2)) + (lane & 15);
+          float most = 5.9604645e-8f;  // 2^-24, the least f16
+#pragma unroll
+          for (int y = 0; y < NG; ++y) {
+            const uint32_t pair = on ? src[y] : 0u;
+            const float scale = half_lo(pair);
+            most = fmaxf(most, fabsf(scale));
+            dst[y * kUnit] = make_float2(scale, fmaf(scale, 8.f, half_hi(pair)));
+          }
+          if (lane >= 16) logs[u * kUnit + (lane & 15)] = lg2(most);
+        }
+        __syncwarp();
+        const bool masked = there != (1u << kSub) - 1 || pos + kTokens > see_least;
+        // positions that row g sees from token 2t of a unit on
+        const int left0 = there & 1 ? see - pos - 2 * t : 0, left1 = there >> 1 & 1 ? see - pos - kUnit - 2 * t : 0;
 
         // scores of tokens 2t, 2t + 1, 8 + 2t, 9 + 2t of the units, in units of unscale
-        float sc[kSub][4], top = -INFINITY;
+        float sc[kSub][4];
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
           const uint8_t* su = st + u * S::kUnitBytes;
@@ -424,8 +510,6 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
           for (int r = 0; r < 4; ++r) sc[u][r] = 0.f;
 #pragma unroll
           for (int y = 0; y < NG; ++y) {
-            uint32_t pair[4];
-            load_pairs<NG>(su + 2 * S::kCodes, t, y, pair);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               uint32_t w[G / 32];
@@ -434,40 +518,46 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
                 *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
               else
                 *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
-              int c[2][4] = {};
+              int c[2][4];
 #pragma unroll
               for (int i = 0; i < G / 32; ++i) {
                 const uint32_t even = w[i] & 0x0F0F0F0Fu, odd = w[i] >> 4 & 0x0F0F0F0Fu;
-                mma16832(c[0], qd[y * (G / 32) + i][0], even, odd);
-                mma16832(c[1], qd[y * (G / 32) + i][1], even, odd);
+                if (i == 0) {
+                  mma16832_first(c[0], qd[y * (G / 32)][0], even, odd);
+                  mma16832_first(c[1], qd[y * (G / 32)][1], even, odd);
+                } else {
+                  mma16832(c[0], qd[y * (G / 32) + i][0], even, odd);
+                  mma16832(c[1], qd[y * (G / 32) + i][1], even, odd);
+                }
               }
+              const float4 kp = *reinterpret_cast<const float4*>(pairs + u * kUnitPairs + (y * kUnit + j * 8 + 2 * t) * 2);
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
                 const float upper = (float)(c[0][i] * 256 + c[0][2 + i] + centre[y][0]);
                 const float lower = (float)(c[1][i] * 256 + c[1][2 + i] + centre[y][1]);
                 const float dot = fmaf(upper, 65536.f, lower);
-                const float ks = half_lo(pair[2 * j + i]), km = fmaf(ks, 8.f, half_hi(pair[2 * j + i]));
-                sc[u][2 * j + i] = fmaf(dot, ks, fmaf(qsum[y], km, sc[u][2 * j + i]));
+                sc[u][2 * j + i] = fmaf(dot, i ? kp.z : kp.x, fmaf(qsum[y], i ? kp.w : kp.y, sc[u][2 * j + i]));
               }
             }
           }
-          // reference: the row's largest s + log2 of the value scale
-          float most[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) most[r] = 5.9604645e-8f;  // 2^-24, the least f16
-#pragma unroll
-          for (int y = 0; y < NG; ++y) {
-            uint32_t pair[4];
-            load_pairs<NG>(su + 2 * S::kCodes + S::kPairs, t, y, pair);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) most[r] = fmaxf(most[r], fabsf(half_lo(pair[r])));
-          }
+        }
+        if (masked) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            if ((r & 2) * 4 + (r & 1) >= left[u]) sc[u][r] = -INFINITY;
-            top = fmaxf(top, fmaf(sc[u][r], unscale, lg2(most[r])));
+            if ((r & 2) * 4 + (r & 1) >= left0) sc[0][r] = -INFINITY;
+            if ((r & 2) * 4 + (r & 1) >= left1) sc[1][r] = -INFINITY;
           }
         }
+        // reference: the row's largest s + log2 of the value scale
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 lg = *reinterpret_cast<const float2*>(logs + u * kUnit + j * 8 + 2 * t);
+            top = fmaxf(top, fmaf(sc[u][2 * j], unscale, lg.x));
+            top = fmaxf(top, fmaf(sc[u][2 * j + 1], unscale, lg.y));
+          }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const bool move = top > ref + 5.f;
@@ -484,12 +574,13 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
             o[i][2] *= f;
             o[i][3] *= f;
           }
+          if (flushed)
+            for (int i = 0; i < 2 * NT; ++i) kept[i * 32] *= f;
         }
         const float base = ref == -INFINITY ? 0.f : 10.f - ref;
 
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-          const uint8_t* su = st + u * S::kUnitBytes;
           float pr[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -498,35 +589,60 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
           }
 #pragma unroll
           for (int y = 0; y < NG; ++y) {
-            uint32_t pair[4], a[4];
-            load_pairs<NG>(su + 2 * S::kCodes + S::kPairs, t, y, pair);
-            float w[4];
+            float vs[4], vm[4];
+            uint32_t a[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float4 vp =
+                  *reinterpret_cast<const float4*>(pairs + u * kUnitPairs + ((NG + y) * kUnit + j * 8 + 2 * t) * 2);
+              vs[2 * j] = vp.x, vm[2 * j] = vp.y, vs[2 * j + 1] = vp.z, vm[2 * j + 1] = vp.w;
+            }
+            if (masked) {  // what the row does not see, and another does, may be NaN
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if ((r & 2) * 4 + (r & 1) >= (u ? left1 : left0)) vs[r] = vm[r] = 0.f;
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              if ((r & 2) * 4 + (r & 1) >= left[u]) pair[r] = 0;  // what is not seen may be NaN
-              const float vs = half_lo(pair[r]);
-              w[r] = pr[r] * vs;
-              off_sum[y] = fmaf(pr[r], fmaf(vs, 8.f, half_hi(pair[r])), off_sum[y]);
+              off_sum[y] = fmaf(pr[r], vm[r], off_sum[y]);
+              vs[r] *= pr[r];
             }
-            split_f16(w[0], w[1], a[0], a[1]);
-            split_f16(w[2], w[3], a[2], a[3]);
+            split_f16(vs[0], vs[1], a[0], a[1]);
+            split_f16(vs[2], vs[3], a[2], a[3]);
 #pragma unroll
             for (int z = y * (G / 32); z < (y + 1) * (G / 32); z += 2) {  // 32 dimensions each
               uint32_t c[4];  // of 4 dimensions: tokens 2t, 2t + 1; 8 + 2t, 9 + 2t; then of the next 32
-              ldmatrix_trans(c, ring_addr + (uint32_t)(su - ring) + v_row + (v_piece ^ z) * 16);
+              ldmatrix_trans(c, ring_addr + (uint32_t)(st - ring) + u * S::kUnitBytes + v_row + (v_piece ^ z) * 16);
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int n = (z + h) * 4;
-                uint32_t b0 = c[2 * h], b1 = c[2 * h + 1];
-                mma16816(o[n], a, codes_lo(b0), codes_lo(b1));
-                mma16816(o[n + 1], a, codes_hi(b0), codes_hi(b1));
-                b0 >>= 8;
-                b1 >>= 8;
-                mma16816(o[n + 2], a, codes_lo(b0), codes_lo(b1));
-                mma16816(o[n + 3], a, codes_hi(b0), codes_hi(b1));
+                uint32_t x0 = c[2 * h], x1 = c[2 * h + 1];
+                mma16816(o[n], a, codes_lo(x0), codes_lo(x1));
+                mma16816(o[n + 1], a, codes_hi(x0), codes_hi(x1));
+                x0 >>= 8;
+                x1 >>= 8;
+                mma16816(o[n + 2], a, codes_lo(x0), codes_lo(x1));
+                mma16816(o[n + 3], a, codes_hi(x0), codes_hi(x1));
               }
             }
           }
+        }
+        // The tensor core drops what lies under the last bit of a sum, always towards 0: its sums are
+        // set aside before that adds up (f32 outputs over 8192 positions of one CTA: 2.8e-6 off).
+        if (++since == kFlush) {
+          since = 0;
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            float x = o[i][0] + o[i][2], z = o[i][1] + o[i][3];
+            if (flushed) {
+              x += kept[2 * i * 32];
+              z += kept[(2 * i + 1) * 32];
+            }
+            kept[2 * i * 32] = x;
+            kept[(2 * i + 1) * 32] = z;
+            o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+          }
+          flushed = true;
         }
       }
       cp_wait<0>();
@@ -543,32 +659,38 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
         for (int z = y * (G / 32); z < (y + 1) * (G / 32); ++z)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {  // columns 2t, 2t + 1: dimensions 8t + e, 8t + 4 + e of the 32
-            joint[g * D + z * 32 + 8 * t + e] = o[z * 4 + e][0] + o[z * 4 + e][2] + off_sum[y];
-            joint[g * D + z * 32 + 8 * t + 4 + e] = o[z * 4 + e][1] + o[z * 4 + e][3] + off_sum[y];
+            const int i = z * 4 + e;
+            float x = o[i][0] + o[i][2] + off_sum[y], w = o[i][1] + o[i][3] + off_sum[y];
+            if (flushed) {
+              x += kept[2 * i * 32];
+              w += kept[(2 * i + 1) * 32];
+            }
+            joint[g * M::kJoint + z * 32 + 8 * t + e] = x;
+            joint[g * M::kJoint + z * 32 + 8 * t + 4 + e] = w;
           }
       }
       if (t == 0) {
-        joint[kRows * D + 2 * g] = ref;
-        joint[kRows * D + 2 * g + 1] = l;
+        joint[kRows * M::kJoint + 2 * g] = ref;
+        joint[kRows * M::kJoint + 2 * g + 1] = l;
       }
       __syncthreads();
-      constexpr int kJoint = kStages * S::kBytes / 4;  // floats from warp to warp
-      const float* all = reinterpret_cast<const float*>(smem);
+      constexpr int kNext = M::kWarp / 4;  // floats from warp to warp
+      const float* all = reinterpret_cast<const float*>(smem + M::kQuery + M::kRowBytes);
       const int slot = at == start ? 0 : 1;
       float* out = sums + ((size_t)blockIdx.x * 2 + slot) * kSlot;
-      for (int i = tid; i < kRows * D; i += kThreads) {
-        const int row = i / D, d = i % D;
+#pragma unroll
+      for (int i0 = 0; i0 < kRows * D; i0 += kThreads) {
+        const int row = (i0 + tid) / D, d = (i0 + tid) % D;
+        const float* num = all + kRows * M::kJoint + 2 * row;
         float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, all[w * kJoint + kRows * D + 2 * row]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, num[w * kNext]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float r = all[w * kJoint + kRows * D + 2 * row];
-          const float f = r == -INFINITY ? 0.f : ex2(r - top);
-          const float lw = all[w * kJoint + kRows * D + 2 * row + 1];
-          // a row of NaN scores never moves its reference: its sums are NaN
-          sum += r == -INFINITY ? lw : lw * f;
-          v += r == -INFINITY ? all[w * kJoint + i] : all[w * kJoint + i] * f;
+          const float r = num[w * kNext];
+          const float f = r == -INFINITY ? 1.f : ex2(r - top);  // no reference: sums of 0, or of NaN
+          sum = fmaf(num[w * kNext + 1], f, sum);
+          v = fmaf(all[w * kNext + row * M::kJoint + d], f, v);
         }
         if (whole) {
           if (row < rows) {
@@ -577,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
                       dtype, sum == 0.f ? 0.f : v / sum);
           }
         } else {
-          out[i] = v;
+          out[row * D + d] = v;
           if (d == 0) {
             out[kRows * D + 2 * row] = top;
             out[kRows * D + 2 * row + 1] = sum;
@@ -649,7 +771,7 @@ int attention_ctas(int head_dim, int sm_count) { return sm_count * (head_dim == 
 
 template <int D, int G>
 cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStream_t st) {
-  const size_t smem = (size_t)kWarps * kStages * Stage<D, G>::kBytes;
+  const size_t smem = Smem<D, G>::kBytes;
   cudaError_t e;
   if (smem > 48 * 1024) {
     e = cudaFuncSetAttribute(kv4_attention_kernel<D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -676,7 +798,8 @@ cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStr
 }  // namespace
 
 size_t kv4_attention_workspace(int head_dim, int sm_count) {
-  return (size_t)attention_ctas(head_dim, sm_count) * (sizeof(Part) + 2 * part_bytes(head_dim));
+  return (size_t)attention_ctas(head_dim, sm_count) *
+         (sizeof(Part) + 2 * part_bytes(head_dim) + (size_t)kWarps * kRows * head_dim * sizeof(float));
 }
 
 cudaError_t launch_kv4_attention(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStream_t st) {
