@@ -10,13 +10,16 @@
 //     sum p v = sum (p s_v) (c - 8)       + sum p (m_v + 8 s_v)
 // (Without the shift by 8 the sums carry 7.5 times the sum of the factors, and a long flat softmax
 // loses its digits against it.)
-//   Queries against keys: integers.  A row of queries, scaled by a power of two to 30 bits, is four
-// signed 8-bit digits; the codes are bytes after one AND (and a shift for the odd dimensions); the
-// sums are exact.  The digits of 8 rows fill the 16 rows of two m16n8k32 products.
-//   Weights against values: f16.  c - 8 is exact, p s_v is split into two f16 (22 bits), which take
-// the rows g and g + 8 of one m16n8k16 product.
-// mma.sync and not tcgen05: one token of a head group is 8 rows, an eighth of tcgen05's smallest
-// tile, whose operands would also have to pass through shared memory unpacked.
+// Both products are taken transposed, tokens (dimensions) as the 16 rows of a product, 8 rows of
+// queries as its 8 columns, so that no part of the product is idle and a lane holds the sums of two
+// rows:  S^T = K Q^T  and  O^T = V^T P^T.
+//   Queries against keys: integers.  A row of queries, scaled by a power of two to 22 bits, is three
+// signed 8-bit digits, one m16n8k32 product each; the codes are bytes after one AND (and a shift for
+// the odd dimensions); the sums are exact.
+//   Weights against values: f16.  c - 8 is exact, p s_v is split into two f16 (22 bits), one m16n8k16
+// product each.
+// mma.sync and not tcgen05: one token of a head group is at most 8 rows, an eighth of tcgen05's
+// smallest tile, whose operands would also have to pass through shared memory unpacked.
 //
 // Softmax in base 2 with a running reference per row: w = 2^(s - r) s_v must fit f16, so r follows
 // max(s + log2 s_v) and is moved (sums rescaled) only when a weight would leave [0, 2^15].
@@ -25,6 +28,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "tk_kv4.h"
 
@@ -33,13 +37,15 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 8;       // rows (query token, head of the group) of a tile
+constexpr int kRows = 8;       // rows (query token, head of the group) of a product
 constexpr int kUnit = 16;      // tokens that lie in one page for sure
 constexpr int kSub = 2;        // units of a warp's step
 constexpr int kTokens = kUnit * kSub;
 constexpr int kStep = kTokens * kWarps;
 template <int D>
-constexpr int kRing = D == 256 ? 2 : 3;  // stages of a warp's ring: as many as leave 3 (2) CTAs on an SM
+constexpr int kRing = D == 256 ? 2 : 3;  // stages of a warp's ring
+template <int D>
+constexpr int kResident = D == 256 ? 2 : 3;  // CTAs of an SM
 constexpr int kFlush = 16;     // steps between two settings aside of the sums
 constexpr int kMinRun = 1;
 constexpr int kTileCost = 2;   // steps that a tile costs beside its own: queries, first loads, join
@@ -102,15 +108,21 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // The same, the sum starting at 0.
 __device__ __forceinline__ void mma16832_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+// An 8 x 8 matrix of f16, two neighbours of a row a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -212,27 +224,25 @@ __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b,
   return s;
 }
 
-// Shared memory of a CTA: the tile's queries as operands, its rows' numbers, then per warp the ring
-// and the step's scales and offsets in f32.
+// Shared memory of a CTA: the tile's queries as operands, its rows' numbers, then the warps' rings.
 template <int D, int G>
 struct Smem {
   using S = Stage<D, G>;
-  static constexpr int kQuery = D / 32 * 32 * 32;              // [word][lane][8] digits of 32 bits
-  static constexpr int kRowWords = 1 + 3 * S::NG;              // unscale; sum, two centres a group
+  static constexpr int kQuery = D / 32 * 32 * 32;  // [word][lane][8]: three digits of 32 bits twice, two words idle
+  static constexpr int kRowWords = 1 + 3 * S::NG;  // unscale; sum, two centres a group
   static constexpr int kRowBytes = kRows * kRowWords * 4;
-  static constexpr int kFloats = (S::NG * kUnit * 4 + kUnit) * kSub;  // [unit][k, v][group][token][2]; [unit][token]
-  static constexpr int kWarp = kRing<D> * S::kBytes + kFloats * 4;
+  static constexpr int kWarp = kRing<D> * S::kBytes;
   static constexpr int kBytes = kQuery + kRowBytes + kWarps * kWarp;
-  static constexpr int kJoint = D + 1;  // floats of a row of sums at the end: rows fall into different banks
+  static constexpr int kJoint = D + 1;  // floats of a row of sums at the end
   static_assert(kRows * (kJoint + 2) * 4 <= kWarp && kRowBytes % 16 == 0 && kWarp % 16 == 0, "");
 };
 
 template <int D, int G>
-__global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kernel(Kv4AttentionParams p, int dtype) {
+__global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(Kv4AttentionParams p, int dtype) {
   using S = Stage<D, G>;
   using M = Smem<D, G>;
   constexpr int kStages = kRing<D>;
-  constexpr int NG = S::NG, KW = D / 32, NT = D / 8;  // KW: words of a lane's keys, 32 dimensions of the row each
+  constexpr int NG = S::NG, KW = D / 32, NT = D / 16;  // KW: words of a lane's keys, 32 dimensions of the row each
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ long long s_warp[kWarps];
   __shared__ long long s_at;
@@ -291,9 +301,6 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
   float* row_num = reinterpret_cast<float*>(smem + M::kQuery);
   uint8_t* ring = smem + M::kQuery + M::kRowBytes + warp * M::kWarp;
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-  float* pairs = reinterpret_cast<float*>(ring + kStages * S::kBytes);
-  constexpr int kUnitPairs = NG * kUnit * 4;      // floats of a unit's pairs
-  float* logs = pairs + kSub * kUnitPairs;        // log2 of the units' largest value scales
   float* joint = reinterpret_cast<float*>(ring);  // after the steps: 8 rows of D sums, 8 x (reference, l)
 
   // where the lane's pieces go in a unit, and where its operands lie
@@ -309,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
   for (int y = 0; y < NG; ++y) k_at[y] = S::at(g, y * (G / 2) + t * (G / 8));
   // ldmatrix: lanes 0-7, 8-15 the rows of tokens 0-7, 8-15 at one piece, lanes 16-31 at the next
   const uint32_t v_row = S::kCodes + (lane & 15) * S::kRowBytes, v_piece = (lane >> 4) ^ S::flip(lane & 15);
-  const size_t page_rows = (size_t)hk << p.cache.shift;
+  const uint32_t page_bytes = (uint32_t)(hk << p.cache.shift) * S::kRowBytes;  // at most 2^16 heads of 2^8 rows of 2^7
   const int page_mask = (1 << p.cache.shift) - 1;
 
   for (long long at = start; at < stop; ++b, offset = 0) {
@@ -324,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
       const int s0 = max(c0 - kTileCost, 0), s1 = max(c1 - kTileCost, 0);
       // positions that row r sees; the tile's last row sees most, its first least
       auto sees = [&](int r) { return min(s.kv, s.last + (row0 + min(r, rows - 1)) / per + 1); };
-      const int see_most = sees(kRows - 1), see_least = sees(0), see = sees(g);
+      const int see_most = sees(kRows - 1), see_least = sees(0), see[2] = {sees(2 * t), sees(2 * t + 1)};
       const int* table = p.block_tables + (size_t)b * p.max_blocks;
 
       // ---- queue of loads: a unit is four runs of consecutive bytes ----
@@ -349,14 +356,14 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
           if (page[u] >= 0 && page[u] < p.cache.num_blocks) {
             valid |= bit;
             const int pos = step * kStep + warp * kTokens + u * kUnit;
-            const size_t row = (size_t)page[u] * page_rows + (pos & page_mask);
+            const size_t codes = (size_t)(uint32_t)page[u] * page_bytes + (pos & page_mask) * S::kRowBytes;
             const uint32_t dst = ring_addr + stage * S::kBytes + u * S::kUnitBytes;
 #pragma unroll
             for (int i = 0; i < S::kCodes / 512; ++i) {
-              cp_async16(dst + piece_dst[i], k_src + row * S::kRowBytes + i * 512);
-              cp_async16(dst + S::kCodes + piece_dst[i], v_src + row * S::kRowBytes + i * 512);
+              cp_async16(dst + piece_dst[i], k_src + codes + i * 512);
+              cp_async16(dst + S::kCodes + piece_dst[i], v_src + codes + i * 512);
             }
-            if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, pair_src + row * NG);
+            if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, pair_src + codes / S::kRowBytes * NG);
           }
         }
         cp_commit();
@@ -368,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
       }
       look(s0 + kStages - 1);
 
-      // ---- queries: scaled, as integers of 30 bits, in digits; 8 dimensions a thread ----
+      // ---- queries: scaled, as integers of 22 bits, in digits; 8 dimensions a thread ----
       constexpr int LPR = D / 8;  // threads of a row
 #pragma unroll
       for (int r0 = 0; r0 < kRows; r0 += kThreads / LPR) {
@@ -395,12 +402,12 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
           odd += __shfl_xor_sync(0xffffffffu, odd, off);
         }
-        // the largest becomes 2^29 .. 2^30
-        const int e = top > 0.f && top < INFINITY ? min(29 - ilogbf(top), 120) : 0;
+        // the largest becomes 2^21 .. 2^22
+        const int e = top > 0.f && top < INFINITY ? min(21 - ilogbf(top), 120) : 0;
         const float norm = ldexpf(1.f, e);
         float sum = 0.f;
         int upper = 0, lower = 0;
-        uint32_t digits[2][4] = {};  // of the even, the odd dimensions; highest first
+        uint32_t digits[3][2] = {};  // highest first; of the even, the odd dimensions
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           int x = __float2int_rn(q[i] * norm);
@@ -409,14 +416,11 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
           x = (x - d0) >> 8;
           const int d1 = (int8_t)x;
           x = (x - d1) >> 8;
-          const int d2 = (int8_t)x;
-          x = (x - d2) >> 8;
-          upper += x * 256 + d2;
-          lower += d1 * 256 + d0;
-          digits[i & 1][0] |= (uint32_t)(x & 255) << (i / 2 * 8);
-          digits[i & 1][1] |= (uint32_t)(d2 & 255) << (i / 2 * 8);
-          digits[i & 1][2] |= (uint32_t)(d1 & 255) << (i / 2 * 8);
-          digits[i & 1][3] |= (uint32_t)(d0 & 255) << (i / 2 * 8);
+          upper += x * 256 + d1;
+          lower += d0;
+          digits[0][i & 1] |= (uint32_t)(x & 255) << (i / 2 * 8);
+          digits[1][i & 1] |= (uint32_t)(d1 & 255) << (i / 2 * 8);
+          digits[2][i & 1] |= (uint32_t)(d0 & 255) << (i / 2 * 8);
         }
 #pragma unroll
         for (int off = G / 16; off > 0; off >>= 1) {
@@ -425,10 +429,9 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
           lower += __shfl_xor_sync(0xffffffffu, lower, off);
         }
         const int y = at8 / (G / 8), tt = at8 % (G / 8) / (G / 32), w = y * (G / 32) + at8 % (G / 32);
-        // two products, upper and lower digits; a0: row g, even; a1: row g + 8; a2, a3: odd
         uint32_t* dst = query + (w * 32 + r * 4 + tt) * 8;
         *reinterpret_cast<uint4*>(dst) = make_uint4(digits[0][0], digits[0][1], digits[1][0], digits[1][1]);
-        *reinterpret_cast<uint4*>(dst + 4) = make_uint4(digits[0][2], digits[0][3], digits[1][2], digits[1][3]);
+        *reinterpret_cast<uint2*>(dst + 4) = make_uint2(digits[2][0], digits[2][1]);
         float* num = row_num + r * M::kRowWords;
         if (at8 == 0) num[0] = ldexpf(1.f, -e) + odd;
         if (at8 % (G / 8) == 0) {
@@ -438,29 +441,35 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
         }
       }
       __syncthreads();
-      uint32_t qd[KW][2][4];
-      float qsum[NG];
-      int centre[NG][2];  // -8 times the sums of the upper and of the lower digits
+      uint32_t qd[KW][3][2];  // digits of row g
 #pragma unroll
-      for (int w = 0; w < KW; ++w)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 v = *reinterpret_cast<const uint4*>(query + (w * 32 + lane) * 8 + 4 * h);
-          qd[w][h][0] = v.x, qd[w][h][1] = v.y, qd[w][h][2] = v.z, qd[w][h][3] = v.w;
-        }
-      const float unscale = row_num[g * M::kRowWords];
-#pragma unroll
-      for (int y = 0; y < NG; ++y) {
-        qsum[y] = row_num[g * M::kRowWords + 1 + 3 * y];
-        centre[y][0] = __float_as_int(row_num[g * M::kRowWords + 2 + 3 * y]);
-        centre[y][1] = __float_as_int(row_num[g * M::kRowWords + 3 + 3 * y]);
+      for (int w = 0; w < KW; ++w) {
+        const uint32_t* src = query + (w * 32 + lane) * 8;
+        const uint4 v = *reinterpret_cast<const uint4*>(src);
+        const uint2 x = *reinterpret_cast<const uint2*>(src + 4);
+        qd[w][0][0] = v.x, qd[w][0][1] = v.y, qd[w][1][0] = v.z, qd[w][1][1] = v.w;
+        qd[w][2][0] = x.x, qd[w][2][1] = x.y;
       }
-
-      float o[NT][4], off_sum[NG], l = 0.f, ref = -INFINITY;  // weights are 2^(s - ref + 10) s_v
+      // of the lane's rows 2t, 2t + 1
+      float unscale[2], qsum[NG][2], off_sum[NG][2], l[2] = {0.f, 0.f};
+      float ref[2] = {-INFINITY, -INFINITY};  // weights are 2^(s - ref + 10) s_v
+      int centre[NG][2][2];                   // -8 times the sums of the upper two digits and of the lowest
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float* num = row_num + (2 * t + i) * M::kRowWords;
+        unscale[i] = num[0];
+#pragma unroll
+        for (int y = 0; y < NG; ++y) {
+          qsum[y][i] = num[1 + 3 * y];
+          centre[y][0][i] = __float_as_int(num[2 + 3 * y]);
+          centre[y][1][i] = __float_as_int(num[3 + 3 * y]);
+          off_sum[y][i] = 0.f;
+        }
+      }
+      // sums: products of 16 dimensions, 32 z + 4 g + 2 h + {0, 1} in o[2 z + h], of rows 2t, 2t + 1
+      float o[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-#pragma unroll
-      for (int y = 0; y < NG; ++y) off_sum[y] = 0.f;
       bool flushed = false;
       int since = 0;  // steps since the sums were set aside
 
@@ -477,171 +486,180 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
         if (!there) continue;
         const int pos = step * kStep + warp * kTokens;
 
-        // scales and offsets in f32, of keys by lanes 0-15, of values by lanes 16-31; 0 for what the
-        // tile does not see (it may hold anything)
-#pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-          const bool on = (there >> u & 1) && pos + u * kUnit + (lane & 15) < see_most;
-          const uint32_t* src =
-              reinterpret_cast<const uint32_t*>(st + u * S::kUnitBytes + 2 * S::kCodes + (lane < 16 ? 0 : S::kPairs)) +
-              (lane & 15) * NG;
-          float2* dst = reinterpret_cast<float2*>(pairs + u * kUnitPairs + (lane < 16 ? 0 : NG * kUnit * 2)) + (lane & 15);
-          float most = 5.9604645e-8f;  // 2^-24, the least f16
-#pragma unroll
-          for (int y = 0; y < NG; ++y) {
-            const uint32_t pair = on ? src[y] : 0u;
-            const float scale = half_lo(pair);
-            most = fmaxf(most, fabsf(scale));
-            dst[y * kUnit] = make_float2(scale, fmaf(scale, 8.f, half_hi(pair)));
-          }
-          if (lane >= 16) logs[u * kUnit + (lane & 15)] = lg2(most);
-        }
-        __syncwarp();
-        const bool masked = there != (1u << kSub) - 1 || pos + kTokens > see_least;
-        // positions that row g sees from token 2t of a unit on
-        const int left0 = there & 1 ? see - pos - 2 * t : 0, left1 = there >> 1 & 1 ? see - pos - kUnit - 2 * t : 0;
+        // Two forms of a step: one masks what a row does not see
+        auto step_of = [&](auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
 
-        // scores of tokens 2t, 2t + 1, 8 + 2t, 9 + 2t of the units, in units of unscale
-        float sc[kSub][4];
+        // scores of tokens g, g + 8 of the units against rows 2t, 2t + 1, in units of unscale
+        float sc[kSub][2][2], vs[kSub][2][NG], vm[kSub][2][NG], top[2] = {-INFINITY, -INFINITY};
+        unsigned hidden = 0;  // scores that are not seen
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
           const uint8_t* su = st + u * S::kUnitBytes;
+          const uint32_t* pairs = reinterpret_cast<const uint32_t*>(su + 2 * S::kCodes) + g * NG;
+          float lg[2];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[u][r] = 0.f;
+          for (int j = 0; j < 2; ++j) {
+            float most = 5.9604645e-8f;  // 2^-24, the least f16
+#pragma unroll
+            for (int y = 0; y < NG; ++y) {
+              const uint32_t pair = pairs[(kUnit + j * 8) * NG + y];
+              vs[u][j][y] = half_lo(pair);
+              vm[u][j][y] = fmaf(vs[u][j][y], 8.f, half_hi(pair));
+              most = fmaxf(most, fabsf(vs[u][j][y]));
+            }
+            lg[j] = lg2(most);
+            sc[u][j][0] = sc[u][j][1] = 0.f;
+          }
 #pragma unroll
           for (int y = 0; y < NG; ++y) {
+            uint32_t w[2][G / 32];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              uint32_t w[G / 32];
               const uint8_t* src = su + k_at[y] + j * 8 * S::kRowBytes;
               if constexpr (G == 128)
-                *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
+                *reinterpret_cast<uint4*>(w[j]) = *reinterpret_cast<const uint4*>(src);
               else
-                *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
-              int c[2][4];
+                *reinterpret_cast<uint2*>(w[j]) = *reinterpret_cast<const uint2*>(src);
+            }
+            int c[3][4];
 #pragma unroll
-              for (int i = 0; i < G / 32; ++i) {
-                const uint32_t even = w[i] & 0x0F0F0F0Fu, odd = w[i] >> 4 & 0x0F0F0F0Fu;
-                if (i == 0) {
-                  mma16832_first(c[0], qd[y * (G / 32)][0], even, odd);
-                  mma16832_first(c[1], qd[y * (G / 32)][1], even, odd);
-                } else {
-                  mma16832(c[0], qd[y * (G / 32) + i][0], even, odd);
-                  mma16832(c[1], qd[y * (G / 32) + i][1], even, odd);
-                }
+            for (int i = 0; i < G / 32; ++i) {
+              const uint32_t a[4] = {w[0][i] & 0x0F0F0F0Fu, w[1][i] & 0x0F0F0F0Fu, w[0][i] >> 4 & 0x0F0F0F0Fu,
+                                     w[1][i] >> 4 & 0x0F0F0F0Fu};
+#pragma unroll
+              for (int d = 0; d < 3; ++d) {
+                const uint32_t(&q)[2] = qd[y * (G / 32) + i][d];
+                if (i == 0)
+                  mma16832_first(c[d], a, q[0], q[1]);
+                else
+                  mma16832(c[d], a, q[0], q[1]);
               }
-              const float4 kp = *reinterpret_cast<const float4*>(pairs + u * kUnitPairs + (y * kUnit + j * 8 + 2 * t) * 2);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t pair = pairs[j * 8 * NG + y];
+              const float ks = half_lo(pair), km = fmaf(ks, 8.f, half_hi(pair));
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const float upper = (float)(c[0][i] * 256 + c[0][2 + i] + centre[y][0]);
-                const float lower = (float)(c[1][i] * 256 + c[1][2 + i] + centre[y][1]);
-                const float dot = fmaf(upper, 65536.f, lower);
-                sc[u][2 * j + i] = fmaf(dot, i ? kp.z : kp.x, fmaf(qsum[y], i ? kp.w : kp.y, sc[u][2 * j + i]));
+                const float upper = (float)(c[0][2 * j + i] * 256 + c[1][2 * j + i] + centre[y][0][i]);
+                const float lower = (float)(c[2][2 * j + i] + centre[y][1][i]);
+                sc[u][j][i] = fmaf(fmaf(upper, 256.f, lower), ks, fmaf(qsum[y][i], km, sc[u][j][i]));
               }
             }
           }
-        }
-        if (masked) {
+          if constexpr (kMasked) {  // of what a row does not see nothing counts, and it may be NaN
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if ((r & 2) * 4 + (r & 1) >= left0) sc[0][r] = -INFINITY;
-            if ((r & 2) * 4 + (r & 1) >= left1) sc[1][r] = -INFINITY;
+            for (int j = 0; j < 2; ++j) {
+              const int at_token = there >> u & 1 ? pos + u * kUnit + j * 8 + g : 0x7fffffff;
+              if (at_token >= see_most) {
+#pragma unroll
+                for (int y = 0; y < NG; ++y) vs[u][j][y] = vm[u][j][y] = 0.f;
+              }
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (at_token >= see[i]) {
+                  sc[u][j][i] = -INFINITY;
+                  hidden |= 1u << (4 * u + 2 * j + i);
+                }
+            }
           }
+          // reference: the row's largest s + log2 of the value scale
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) top[i] = fmaxf(top[i], fmaf(sc[u][j][i], unscale[i], lg[j]));
         }
-        // reference: the row's largest s + log2 of the value scale
-        float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
+        for (int off = 4; off < 32; off <<= 1) {
+          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+        }
+        const bool move0 = top[0] > ref[0] + 5.f, move1 = top[1] > ref[1] + 5.f;
+        if (__any_sync(0xffffffffu, move0 || move1)) {
+          const float f0 = move0 ? ex2(ref[0] - top[0]) : 1.f, f1 = move1 ? ex2(ref[1] - top[1]) : 1.f;  // 0 at first
+          if (move0) ref[0] = top[0];
+          if (move1) ref[1] = top[1];
+          l[0] *= f0;
+          l[1] *= f1;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float2 lg = *reinterpret_cast<const float2*>(logs + u * kUnit + j * 8 + 2 * t);
-            top = fmaxf(top, fmaf(sc[u][2 * j], unscale, lg.x));
-            top = fmaxf(top, fmaf(sc[u][2 * j + 1], unscale, lg.y));
+          for (int y = 0; y < NG; ++y) {
+            off_sum[y][0] *= f0;
+            off_sum[y][1] *= f1;
           }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const bool move = top > ref + 5.f;
-        if (__any_sync(0xffffffffu, move)) {
-          const float f = move ? ex2(ref - top) : 1.f;  // 0 at first
-          if (move) ref = top;
-          l *= f;
-#pragma unroll
-          for (int y = 0; y < NG; ++y) off_sum[y] *= f;
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            o[i][0] *= f;
-            o[i][1] *= f;
-            o[i][2] *= f;
-            o[i][3] *= f;
+            o[i][0] *= f0;
+            o[i][1] *= f1;
+            o[i][2] *= f0;
+            o[i][3] *= f1;
           }
           if (flushed)
-            for (int i = 0; i < 2 * NT; ++i) kept[i * 32] *= f;
+            for (int i = 0; i < 4 * NT; ++i) kept[i * 32] *= i & 1 ? f1 : f0;
         }
-        const float base = ref == -INFINITY ? 0.f : 10.f - ref;
+        const float base[2] = {ref[0] == -INFINITY ? 0.f : 10.f - ref[0], ref[1] == -INFINITY ? 0.f : 10.f - ref[1]};
 
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-          float pr[4];
+          float pr[2][2];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            pr[r] = ex2(fmaf(sc[u][r], unscale, base));
-            l += pr[r];
-          }
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              pr[j][i] = ex2(fmaf(sc[u][j][i], unscale[i], base[i]));
+              l[i] += pr[j][i];
+            }
 #pragma unroll
           for (int y = 0; y < NG; ++y) {
-            float vs[4], vm[4];
-            uint32_t a[4];
+            uint32_t hi[2], lo[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float4 vp =
-                  *reinterpret_cast<const float4*>(pairs + u * kUnitPairs + ((NG + y) * kUnit + j * 8 + 2 * t) * 2);
-              vs[2 * j] = vp.x, vm[2 * j] = vp.y, vs[2 * j + 1] = vp.z, vm[2 * j + 1] = vp.w;
-            }
-            if (masked) {  // what the row does not see, and another does, may be NaN
+              float w[2];
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if ((r & 2) * 4 + (r & 1) >= (u ? left1 : left0)) vs[r] = vm[r] = 0.f;
+              for (int i = 0; i < 2; ++i) {
+                w[i] = pr[j][i] * vs[u][j][y];
+                const float with = fmaf(pr[j][i], vm[u][j][y], off_sum[y][i]);
+                if (!(kMasked && hidden >> (4 * u + 2 * j + i) & 1))
+                  off_sum[y][i] = with;
+                else
+                  w[i] = 0.f;
+              }
+              split_f16(w[0], w[1], hi[j], lo[j]);
+              hi[j] = transpose8(hi[j]);  // tokens 8j + 2t, 8j + 2t + 1 of row g
+              lo[j] = transpose8(lo[j]);
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              off_sum[y] = fmaf(pr[r], vm[r], off_sum[y]);
-              vs[r] *= pr[r];
-            }
-            split_f16(vs[0], vs[1], a[0], a[1]);
-            split_f16(vs[2], vs[3], a[2], a[3]);
 #pragma unroll
             for (int z = y * (G / 32); z < (y + 1) * (G / 32); z += 2) {  // 32 dimensions each
               uint32_t c[4];  // of 4 dimensions: tokens 2t, 2t + 1; 8 + 2t, 9 + 2t; then of the next 32
               ldmatrix_trans(c, ring_addr + (uint32_t)(st - ring) + u * S::kUnitBytes + v_row + (v_piece ^ z) * 16);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int n = (z + h) * 4;
-                uint32_t x0 = c[2 * h], x1 = c[2 * h + 1];
-                mma16816(o[n], a, codes_lo(x0), codes_lo(x1));
-                mma16816(o[n + 1], a, codes_hi(x0), codes_hi(x1));
-                x0 >>= 8;
-                x1 >>= 8;
-                mma16816(o[n + 2], a, codes_lo(x0), codes_lo(x1));
-                mma16816(o[n + 3], a, codes_hi(x0), codes_hi(x1));
+              for (int h = 0; h < 4; ++h) {
+                uint32_t x = c[h / 2 * 2], x8 = c[h / 2 * 2 + 1];
+                if (h & 1) x >>= 8, x8 >>= 8;
+                const uint32_t a[4] = {codes_lo(x), codes_hi(x), codes_lo(x8), codes_hi(x8)};
+                mma16816(o[2 * z + h], a, hi[0], hi[1]);
+                mma16816(o[2 * z + h], a, lo[0], lo[1]);
               }
             }
           }
         }
+        };
+        if (there != (1u << kSub) - 1 || pos + kTokens > see_least)
+          step_of(std::true_type{});
+        else
+          step_of(std::false_type{});
         // The tensor core drops what lies under the last bit of a sum, always towards 0: its sums are
         // set aside before that adds up (f32 outputs over 8192 positions of one CTA: 2.8e-6 off).
         if (++since == kFlush) {
           since = 0;
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            float x = o[i][0] + o[i][2], z = o[i][1] + o[i][3];
-            if (flushed) {
-              x += kept[2 * i * 32];
-              z += kept[(2 * i + 1) * 32];
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float* x = kept + (4 * i + k) * 32;
+              *x = flushed ? *x + o[i][k] : o[i][k];
+              o[i][k] = 0.f;
             }
-            kept[2 * i * 32] = x;
-            kept[(2 * i + 1) * 32] = z;
-            o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-          }
           flushed = true;
         }
       }
@@ -649,29 +667,28 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
       __syncwarp();
 
       // ---- join the four warps ----
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
 #pragma unroll
-      for (int y = 0; y < NG; ++y) {
-        off_sum[y] += __shfl_xor_sync(0xffffffffu, off_sum[y], 1);
-        off_sum[y] += __shfl_xor_sync(0xffffffffu, off_sum[y], 2);
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int z = y * (G / 32); z < (y + 1) * (G / 32); ++z)
+        for (int off = 4; off < 32; off <<= 1) {
+          l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {  // columns 2t, 2t + 1: dimensions 8t + e, 8t + 4 + e of the 32
-            const int i = z * 4 + e;
-            float x = o[i][0] + o[i][2] + off_sum[y], w = o[i][1] + o[i][3] + off_sum[y];
-            if (flushed) {
-              x += kept[2 * i * 32];
-              w += kept[(2 * i + 1) * 32];
-            }
-            joint[g * M::kJoint + z * 32 + 8 * t + e] = x;
-            joint[g * M::kJoint + z * 32 + 8 * t + 4 + e] = w;
-          }
-      }
-      if (t == 0) {
-        joint[kRows * M::kJoint + 2 * g] = ref;
-        joint[kRows * M::kJoint + 2 * g + 1] = l;
+          for (int y = 0; y < NG; ++y) off_sum[y][i] += __shfl_xor_sync(0xffffffffu, off_sum[y][i], off);
+        }
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float x = o[i][k] + off_sum[i / (G / 16)][k & 1];
+          if (flushed) x += kept[(4 * i + k) * 32];
+          joint[(2 * t + (k & 1)) * M::kJoint + i / 2 * 32 + 4 * g + i % 2 * 2 + k / 2] = x;
+        }
+      if (g == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          joint[kRows * M::kJoint + 2 * (2 * t + i)] = ref[i];
+          joint[kRows * M::kJoint + 2 * (2 * t + i) + 1] = l[i];
+        }
       }
       __syncthreads();
       constexpr int kNext = M::kWarp / 4;  // floats from warp to warp
@@ -717,21 +734,23 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) kv4_attention_kern
   }
 }
 
-// Joins the parts of the tile that begins in the run of CTA blockIdx.x.  kJoinWarps warps a row, each
-// with every kJoinWarps-th part, then in the order of the warps.
+// Joins the parts of the tile that begins in the run of CTA blockIdx.x, kJoinRows of its rows.
+// kJoinWarps warps a row, each with every kJoinWarps-th part, then in the order of the warps.
 constexpr int kJoinWarps = 4;
+constexpr int kJoinRows = 2;
 
 template <int D>
-__global__ void __launch_bounds__(kRows * kJoinWarps * 32) kv4_join_kernel(Kv4AttentionParams p, int dtype) {
-  __shared__ float s_sum[kRows][kJoinWarps];
-  __shared__ float s_v[kRows][kJoinWarps][D];
+__global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(Kv4AttentionParams p, int dtype) {
+  __shared__ float s_sum[kJoinRows][kJoinWarps];
+  __shared__ float s_v[kJoinRows][kJoinWarps][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Part* parts = static_cast<const Part*>(p.workspace);
   const float* sums = reinterpret_cast<const float*>(parts + gridDim.x);
   constexpr int kSlot = kRows * (D + 2);
   const Part part = parts[blockIdx.x];
   if (part.count == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = warp / kJoinWarps, w = warp % kJoinWarps;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = warp / kJoinWarps, w = warp % kJoinWarps;
+  const int row = blockIdx.y * kJoinRows + r0;
   auto base = [&](int i) { return sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot; };
   float top = -INFINITY;
   for (int i = lane; i < part.count; i += 32) top = fmaxf(top, base(i)[kRows * D + 2 * row]);
@@ -749,25 +768,25 @@ __global__ void __launch_bounds__(kRows * kJoinWarps * 32) kv4_join_kernel(Kv4At
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) v[e] = fmaf(s[row * D + e * 32 + lane], f, v[e]);
   }
-  if (lane == 0) s_sum[row][w] = sum;
+  if (lane == 0) s_sum[r0][w] = sum;
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) s_v[row][w][e * 32 + lane] = v[e];
+  for (int e = 0; e < D / 32; ++e) s_v[r0][w][e * 32 + lane] = v[e];
   __syncthreads();
   if (row >= part.rows) return;
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) sum += s_sum[row][i];
+  for (int i = 0; i < kJoinWarps; ++i) sum += s_sum[r0][i];
   const int per = p.q_heads / p.cache.kv_heads, q = part.row0 + row;
   const long long at = (long long)(part.token + q / per) * p.o_stride + (long long)(part.head * per + q % per) * D;
   for (int d = w * 32 + lane; d < D; d += kJoinWarps * 32) {
     float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) x += s_v[row][i][d];
+    for (int i = 0; i < kJoinWarps; ++i) x += s_v[r0][i][d];
     store_any(p.o, at + d, dtype, sum == 0.f ? 0.f : x / sum);
   }
 }
 
-int attention_ctas(int head_dim, int sm_count) { return sm_count * (head_dim == 256 ? 2 : 3); }
+int attention_ctas(int head_dim, int sm_count) { return sm_count * (head_dim == 256 ? kResident<256> : kResident<128>); }
 
 template <int D, int G>
 cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStream_t st) {
@@ -784,8 +803,8 @@ cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStr
   if (e != cudaSuccess) return e;
   // a programmatic launch: set up while the attention runs, past its wait when that has completed
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kRows * kJoinWarps * 32);
+  cfg.gridDim = dim3((unsigned)ctas, kRows / kJoinRows);
+  cfg.blockDim = dim3(kJoinRows * kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
