@@ -43,7 +43,7 @@ constexpr int kSub = 2;        // units of a warp's step
 constexpr int kTokens = kUnit * kSub;
 constexpr int kStep = kTokens * kWarps;
 template <int D>
-constexpr int kRing = D == 256 ? 2 : 3;  // stages of a warp's ring
+constexpr int kRing = 2;  // stages of a warp's ring
 template <int D>
 constexpr int kResident = D == 256 ? 2 : 3;  // CTAs of an SM
 constexpr int kFlush = 16;     // steps between two settings aside of the sums
@@ -224,7 +224,15 @@ __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b,
   return s;
 }
 
-// Shared memory of a CTA: the tile's queries as operands, its rows' numbers, then the warps' rings.
+// The part of a tile that a run holds.
+struct Tile {
+  int b, head, rt;  // sequence, key head, row tile
+  int c0, c1;       // steps, the tile's cost among them
+  Sequence s;
+};
+
+// Shared memory of a CTA: the tile's queries as operands, its rows' numbers, the warps' rings, the
+// warps' sums at the end of a tile.
 template <int D, int G>
 struct Smem {
   using S = Stage<D, G>;
@@ -232,9 +240,11 @@ struct Smem {
   static constexpr int kRowWords = 1 + 3 * S::NG;  // unscale; sum, two centres a group
   static constexpr int kRowBytes = kRows * kRowWords * 4;
   static constexpr int kWarp = kRing<D> * S::kBytes;
-  static constexpr int kBytes = kQuery + kRowBytes + kWarps * kWarp;
-  static constexpr int kJoint = D + 1;  // floats of a row of sums at the end
-  static_assert(kRows * (kJoint + 2) * 4 <= kWarp && kRowBytes % 16 == 0 && kWarp % 16 == 0, "");
+  static constexpr int kJoint = D + 1;                     // floats of a row of sums at the end
+  static constexpr int kJointWarp = kRows * (kJoint + 2);  // and per row the reference and l
+  static constexpr int kRings = kQuery + kRowBytes, kJoints = kRings + kWarps * kWarp;
+  static constexpr int kBytes = kJoints + kWarps * kJointWarp * 4;
+  static_assert(kRowBytes % 16 == 0 && kWarp % 16 == 0, "");
 };
 
 template <int D, int G>
@@ -247,6 +257,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   __shared__ long long s_warp[kWarps];
   __shared__ long long s_at;
   __shared__ int s_seq;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing is read before the kernels before have completed
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per = p.q_heads / p.cache.kv_heads, hk = p.cache.kv_heads;
   Part* parts = static_cast<Part*>(p.workspace);
@@ -294,22 +306,27 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
     s_at = start - at;
   }
   __syncthreads();
-  int b = s_seq;
-  long long offset = s_at;  // of the run's next step in its sequence
+  Tile cur;
+  cur.b = s_seq;
+  cur.s = sequence(p, cur.b, per);
+  {
+    const long long unit = s_at / cur.s.steps;
+    cur.c0 = (int)(s_at - unit * cur.s.steps);
+    cur.head = (int)unit / cur.s.tiles;
+    cur.rt = (int)unit - cur.head * cur.s.tiles;
+  }
+  long long at = start;  // of the tile's first step here, in all work
+  cur.c1 = (int)min((long long)cur.s.steps, cur.c0 + (stop - at));
 
   uint32_t* query = reinterpret_cast<uint32_t*>(smem);
   float* row_num = reinterpret_cast<float*>(smem + M::kQuery);
-  uint8_t* ring = smem + M::kQuery + M::kRowBytes + warp * M::kWarp;
+  uint8_t* ring = smem + M::kRings + warp * M::kWarp;
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-  float* joint = reinterpret_cast<float*>(ring);  // after the steps: 8 rows of D sums, 8 x (reference, l)
+  float* joint = reinterpret_cast<float*>(smem + M::kJoints) + warp * M::kJointWarp;
 
   // where the lane's pieces go in a unit, and where its operands lie
-  uint32_t piece_dst[S::kCodes / 512];
-#pragma unroll
-  for (int i = 0; i < S::kCodes / 512; ++i) {
-    const int piece = i * 32 + lane;
-    piece_dst[i] = S::at(piece / S::kPieces, piece % S::kPieces * 16);
-  }
+  // (piece 32 i + lane lies 512 i on, at D = 256 with one bit of its place turned for odd i)
+  const uint32_t piece_dst = S::at(lane / S::kPieces, lane % S::kPieces * 16);
   const uint32_t pair_dst = 2 * S::kCodes + (lane < 16 ? 0 : S::kPairs) + (lane & 15) * 16;
   int k_at[NG];
 #pragma unroll
@@ -319,83 +336,92 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   const uint32_t page_bytes = (uint32_t)(hk << p.cache.shift) * S::kRowBytes;  // at most 2^16 heads of 2^8 rows of 2^7
   const int page_mask = (1 << p.cache.shift) - 1;
 
-  for (long long at = start; at < stop; ++b, offset = 0) {
-    const Sequence s = sequence(p, b, per);
-    const long long in_seq = (long long)s.steps * s.tiles * hk;
-    while (at < stop && offset < in_seq) {
-      const int unit = (int)(offset / s.steps), c0 = (int)(offset % s.steps);
-      const int c1 = (int)min((long long)s.steps, c0 + (stop - at));
-      const int head = unit / s.tiles, row0 = (unit % s.tiles) * kRows;
-      const int rows = min(kRows, s.n * per - row0);
-      const bool whole = c0 == 0 && c1 == s.steps;
-      const int s0 = max(c0 - kTileCost, 0), s1 = max(c1 - kTileCost, 0);
-      // positions that row r sees; the tile's last row sees most, its first least
-      auto sees = [&](int r) { return min(s.kv, s.last + (row0 + min(r, rows - 1)) / per + 1); };
-      const int see_most = sees(kRows - 1), see_least = sees(0), see[2] = {sees(2 * t), sees(2 * t + 1)};
-      const int* table = p.block_tables + (size_t)b * p.max_blocks;
-
-      // ---- queue of loads: a unit is four runs of consecutive bytes ----
-      const size_t head_row = (size_t)head << p.cache.shift;
-      const uint8_t* k_src = p.cache.k_codes + head_row * S::kRowBytes + lane * 16;
-      const uint8_t* v_src = p.cache.v_codes + head_row * S::kRowBytes + lane * 16;
-      const uint32_t* pair_src = (lane < 16 ? p.cache.k_scales : p.cache.v_scales) + head_row * NG + (lane & 15) * 4;
-      unsigned valid = 0;  // kSub bits a stage
-      int page[kSub];
-      auto look = [&](int step) {
+  // ---- queue of loads of a tile: a unit is four runs of consecutive bytes ----
+  const uint8_t *k_src, *v_src, *pair_src;
+  const int* table;
+  int s0, s1, see_most, page[kSub];
+  unsigned valid = 0;  // kSub bits a stage
+  auto look = [&](int step) {
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-          const int pos = step * kStep + warp * kTokens + u * kUnit;
-          page[u] = step < s1 && pos < see_most ? __ldg(table + (pos >> p.cache.shift)) : -1;
+    for (int u = 0; u < kSub; ++u) {
+      const int pos = step * kStep + warp * kTokens + u * kUnit;
+      page[u] = step < s1 && pos < see_most ? __ldg(table + (pos >> p.cache.shift)) : -1;
+    }
+  };
+  auto issue = [&](int stage, int step) {
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+      const unsigned bit = 1u << (stage * kSub + u);
+      valid &= ~bit;
+      if ((unsigned)page[u] < (unsigned)p.cache.num_blocks) {
+        valid |= bit;
+        const int pos = step * kStep + warp * kTokens + u * kUnit;
+        const size_t codes = (size_t)(uint32_t)page[u] * page_bytes + (pos & page_mask) * S::kRowBytes;
+        const uint32_t dst = ring_addr + stage * S::kBytes + u * S::kUnitBytes;
+        const uint32_t dst0 = dst + piece_dst, dst1 = dst + (D == 256 ? piece_dst ^ 16 : piece_dst);
+        const uint8_t *kc = k_src + codes, *vc = v_src + codes;
+#pragma unroll
+        for (int i = 0; i < S::kCodes / 512; ++i) {
+          cp_async16((i & 1 ? dst1 : dst0) + i * 512, kc + i * 512);
+          cp_async16((i & 1 ? dst1 : dst0) + S::kCodes + i * 512, vc + i * 512);
         }
-      };
-      auto issue = [&](int stage, int step) {
-#pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-          const unsigned bit = 1u << (stage * kSub + u);
-          valid &= ~bit;
-          if (page[u] >= 0 && page[u] < p.cache.num_blocks) {
-            valid |= bit;
-            const int pos = step * kStep + warp * kTokens + u * kUnit;
-            const size_t codes = (size_t)(uint32_t)page[u] * page_bytes + (pos & page_mask) * S::kRowBytes;
-            const uint32_t dst = ring_addr + stage * S::kBytes + u * S::kUnitBytes;
-#pragma unroll
-            for (int i = 0; i < S::kCodes / 512; ++i) {
-              cp_async16(dst + piece_dst[i], k_src + codes + i * 512);
-              cp_async16(dst + S::kCodes + piece_dst[i], v_src + codes + i * 512);
-            }
-            if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, pair_src + codes / S::kRowBytes * NG);
-          }
-        }
-        cp_commit();
-      };
-#pragma unroll
-      for (int i = 0; i < kStages - 1; ++i) {
-        look(s0 + i);
-        issue(i, s0 + i);
+        if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, pair_src + codes / (S::kRowBytes / NG / 4));
       }
-      look(s0 + kStages - 1);
+    }
+    cp_commit();
+  };
+  // the position after the last that row r of a tile sees; its last row sees most, its first least
+  auto sees = [&](const Tile& x, int r) {
+    const int row = x.rt * kRows + r, end = x.s.n * per - 1;
+    return min(x.s.kv, x.s.last + min(row, end) / per + 1);
+  };
+  constexpr int LPR = D / 8;                                   // threads of a row of queries, 8 dimensions each
+  constexpr int kPasses = (kRows * LPR + kThreads - 1) / kThreads;
+  float q[kPasses][8];
+  auto begin = [&](const Tile& x) {
+    const size_t head_row = (size_t)x.head << p.cache.shift;
+    k_src = p.cache.k_codes + head_row * S::kRowBytes + lane * 16;
+    v_src = p.cache.v_codes + head_row * S::kRowBytes + lane * 16;
+    pair_src = reinterpret_cast<const uint8_t*>((lane < 16 ? p.cache.k_scales : p.cache.v_scales) + head_row * NG +
+                                                (lane & 15) * 4);
+    table = p.block_tables + (size_t)x.b * p.max_blocks;
+    s0 = max(x.c0 - kTileCost, 0);
+    s1 = max(x.c1 - kTileCost, 0);
+    see_most = sees(x, kRows - 1);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      look(s0 + i);
+      issue(i, s0 + i);
+    }
+    look(s0 + kStages - 1);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * (kThreads / LPR) + tid / LPR;
+      const int row = min(x.rt * kRows + r, x.s.n * per - 1);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) q[i][k] = 0.f;
+      if (r < kRows && sees(x, r) > 0)
+        load_row8(p.q, (long long)(x.s.first + row / per) * p.q_stride + (long long)(x.head * per + row % per) * D +
+                           tid % LPR * 8, dtype, q[i]);
+    }
+  };
+  begin(cur);
+
+  for (;;) {
+      const int see_least = sees(cur, 0), see[2] = {sees(cur, 2 * t), sees(cur, 2 * t + 1)};
 
       // ---- queries: scaled, as integers of 22 bits, in digits; 8 dimensions a thread ----
-      constexpr int LPR = D / 8;  // threads of a row
 #pragma unroll
-      for (int r0 = 0; r0 < kRows; r0 += kThreads / LPR) {
-        const int r = r0 + tid / LPR, at8 = tid % LPR;
+      for (int pass = 0; pass < kPasses; ++pass) {
+        const int r = pass * (kThreads / LPR) + tid / LPR, at8 = tid % LPR;
         if (r >= kRows) continue;  // whole warps
-        const int row = row0 + min(r, rows - 1);
-        float q[8];
-        if (sees(r) > 0)
-          load_row8(p.q, (long long)(s.first + row / per) * p.q_stride + (long long)(head * per + row % per) * D + at8 * 8,
-                    dtype, q);
-        else
-#pragma unroll
-          for (int i = 0; i < 8; ++i) q[i] = 0.f;
         const float f = p.scale * 1.4426950408889634f;
         float top = 0.f, odd = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          q[i] *= f;
-          top = fmaxf(top, fabsf(q[i]));
-          odd = fmaf(q[i], 0.f, odd);  // NaN if one is not finite
+          q[pass][i] *= f;
+          top = fmaxf(top, fabsf(q[pass][i]));
+          odd = fmaf(q[pass][i], 0.f, odd);  // NaN if one is not finite
         }
 #pragma unroll
         for (int off = LPR / 2; off > 0; off >>= 1) {
@@ -410,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
         uint32_t digits[3][2] = {};  // highest first; of the even, the odd dimensions
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          int x = __float2int_rn(q[i] * norm);
+          int x = __float2int_rn(q[pass][i] * norm);
           sum += (float)x;
           const int d0 = (int8_t)x;
           x = (x - d0) >> 8;
@@ -570,13 +596,13 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 #pragma unroll
             for (int i = 0; i < 2; ++i) top[i] = fmaxf(top[i], fmaf(sc[u][j][i], unscale[i], lg[j]));
         }
+        if (__any_sync(0xffffffffu, top[0] > ref[0] + 5.f || top[1] > ref[1] + 5.f)) {
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
-          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
-        }
-        const bool move0 = top[0] > ref[0] + 5.f, move1 = top[1] > ref[1] + 5.f;
-        if (__any_sync(0xffffffffu, move0 || move1)) {
+          for (int off = 4; off < 32; off <<= 1) {
+            top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+            top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+          }
+          const bool move0 = top[0] > ref[0] + 5.f, move1 = top[1] > ref[1] + 5.f;
           const float f0 = move0 ? ex2(ref[0] - top[0]) : 1.f, f1 = move1 ? ex2(ref[1] - top[1]) : 1.f;  // 0 at first
           if (move0) ref[0] = top[0];
           if (move1) ref[1] = top[1];
@@ -690,47 +716,69 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
           joint[kRows * M::kJoint + 2 * (2 * t + i) + 1] = l[i];
         }
       }
+
+      // the next tile's first loads travel meanwhile
+      const Tile done = cur;
+      const long long done_at = at;
+      at += cur.c1 - cur.c0;
+      const bool more = at < stop;
+      if (more) {
+        cur.c0 = 0;
+        if (++cur.rt == cur.s.tiles) {
+          cur.rt = 0;
+          if (++cur.head == hk) {
+            cur.head = 0;
+            do {
+              cur.s = sequence(p, ++cur.b, per);
+            } while (cur.s.tiles == 0);
+          }
+        }
+        cur.c1 = (int)min((long long)cur.s.steps, stop - at);
+        begin(cur);
+      }
       __syncthreads();
-      constexpr int kNext = M::kWarp / 4;  // floats from warp to warp
-      const float* all = reinterpret_cast<const float*>(smem + M::kQuery + M::kRowBytes);
-      const int slot = at == start ? 0 : 1;
-      float* out = sums + ((size_t)blockIdx.x * 2 + slot) * kSlot;
-#pragma unroll
-      for (int i0 = 0; i0 < kRows * D; i0 += kThreads) {
-        const int row = (i0 + tid) / D, d = (i0 + tid) % D;
+
+      {
+        const bool whole = done.c0 == 0 && done.c1 == done.s.steps;
+        const int row0 = done.rt * kRows, rows = min(kRows, done.s.n * per - row0), slot = done_at == start ? 0 : 1;
+        constexpr int kThreadsRow = kThreads / kRows;
+        const int row = tid / kThreadsRow, d0 = tid % kThreadsRow;
+        const float* all = reinterpret_cast<const float*>(smem + M::kJoints);
         const float* num = all + kRows * M::kJoint + 2 * row;
-        float top = -INFINITY, sum = 0.f, v = 0.f;
+        float top = -INFINITY, sum = 0.f, f[kWarps];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, num[w * kNext]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, num[w * M::kJointWarp]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float r = num[w * kNext];
-          const float f = r == -INFINITY ? 1.f : ex2(r - top);  // no reference: sums of 0, or of NaN
-          sum = fmaf(num[w * kNext + 1], f, sum);
-          v = fmaf(all[w * kNext + row * M::kJoint + d], f, v);
+          const float r = num[w * M::kJointWarp];
+          f[w] = r == -INFINITY ? 1.f : ex2(r - top);  // no reference: sums of 0, or of NaN
+          sum = fmaf(num[w * M::kJointWarp + 1], f[w], sum);
         }
-        if (whole) {
-          if (row < rows) {
-            const int q = row0 + row;
-            store_any(p.o, (long long)(s.first + q / per) * p.o_stride + (long long)(head * per + q % per) * D + d,
-                      dtype, sum == 0.f ? 0.f : v / sum);
-          }
-        } else {
-          out[row * D + d] = v;
-          if (d == 0) {
-            out[kRows * D + 2 * row] = top;
-            out[kRows * D + 2 * row + 1] = sum;
-          }
+        float* out = sums + ((size_t)blockIdx.x * 2 + slot) * kSlot;
+        const int query_row = row0 + min(row, rows - 1);
+        const long long o_at = (long long)(done.s.first + query_row / per) * p.o_stride +
+                               (long long)(done.head * per + query_row % per) * D;
+#pragma unroll
+        for (int d = d0; d < D; d += kThreadsRow) {
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) v = fmaf(all[w * M::kJointWarp + row * M::kJoint + d], f[w], v);
+          if (!whole)
+            out[row * D + d] = v;
+          else if (row < rows)
+            store_any(p.o, o_at + d, dtype, sum == 0.f ? 0.f : v / sum);
+        }
+        if (!whole && d0 == 0) {
+          out[kRows * D + 2 * row] = top;
+          out[kRows * D + 2 * row + 1] = sum;
+        }
+        if (!whole && done.c0 == 0 && tid == 0) {  // the tile begins here: where its parts are
+          const long long end = done_at + done.s.steps;
+          parts[blockIdx.x] =
+              Part{done.s.first, rows, done.head, (int)((end - 1) / run - blockIdx.x + 1), row0, slot, 0, 0};
         }
       }
-      if (!whole && c0 == 0 && tid == 0) {  // the tile begins here: where its parts are
-        const long long end = at + s.steps;
-        parts[blockIdx.x] = Part{s.first, rows, head, (int)((end - 1) / run - blockIdx.x + 1), row0, slot, 0, 0};
-      }
-      __syncthreads();
-      at += c1 - c0;
-      offset += c1 - c0;
-    }
+      if (!more) break;
   }
 }
 
@@ -744,6 +792,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(K
   __shared__ float s_sum[kJoinRows][kJoinWarps];
   __shared__ float s_v[kJoinRows][kJoinWarps][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Part* parts = static_cast<const Part*>(p.workspace);
   const float* sums = reinterpret_cast<const float*>(parts + gridDim.x);
   constexpr int kSlot = kRows * (D + 2);
@@ -797,20 +846,24 @@ cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStr
                                          (int)smem);
     if (e != cudaSuccess) return e;
   }
+  // programmatic launches: a kernel is set up while the one before it runs, and passes its wait when
+  // that has completed
   const int ctas = attention_ctas(D, sm_count);
-  kv4_attention_kernel<D, G><<<ctas, kThreads, smem, st>>>(p, dtype);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  // a programmatic launch: set up while the attention runs, past its wait when that has completed
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas, kRows / kJoinRows);
-  cfg.blockDim = dim3(kJoinRows * kJoinWarps * 32);
-  cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, G>, p, dtype);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3((unsigned)ctas, kRows / kJoinRows);
+  cfg.blockDim = dim3(kJoinRows * kJoinWarps * 32);
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, p, dtype);
 }
 
