@@ -112,11 +112,14 @@ __device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], ui
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The same, the sum starting at 0.
+// The same, the sum starting at the bits of 1.5 * 2^23: read as f32 it is that plus the sum, while
+// the sum is below 2^22 (at most 256 * 15 * 128 here).
+constexpr int kSumBits = 0x4B400000;
+constexpr float kSumStart = 12582912.f;
 __device__ __forceinline__ void mma16832_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(kSumBits));
 }
 // An 8 x 8 matrix of f16, two neighbours of a row a lane, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -152,22 +155,19 @@ __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ush
 __device__ __forceinline__ float half_hi(uint32_t w) {
   return __half2float(__ushort_as_half((unsigned short)(w >> 16)));
 }
-// Two codes less 8 from bits 0-3 (codes_lo) or 4-7 (codes_hi) of the halves of x: as 1024 + c or
-// 1024 + 16 c by the bits of the exponent, then exact f16 arithmetic.
+// Two codes less 8, times 2^-9, from bits 0-3 (codes_lo) or 4-7 (codes_hi) of the halves of x: the
+// bits are the subnormals c * 2^-24 and c * 2^-20, and one f16 product and sum of them is exact.
 __device__ __forceinline__ uint32_t codes_lo(uint32_t x) {
-  x = (x & 0x000F000Fu) | 0x64006400u;
-  const uint32_t k = 0x64086408u;  // 1032
   uint32_t y;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(k));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x & 0x000F000Fu), "r"(0x78007800u), "r"(0xA400A400u));  // 2^15, -2^-6
   return y;
 }
 __device__ __forceinline__ uint32_t codes_hi(uint32_t x) {
-  x = (x & 0x00F000F0u) | 0x64006400u;
-  const uint32_t f = 0x2C002C00u, k = 0xD480D480u;  // 1/16, -72
   uint32_t y;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(f), "r"(k));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x & 0x00F000F0u), "r"(0x68006800u), "r"(0xA400A400u));  // 2^11, -2^-6
   return y;
 }
+constexpr float kCodes = 512.f;  // what undoes the 2^-9
 
 // Two f32 as f16 (a in the low half), and what that leaves of them.
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
@@ -237,7 +237,7 @@ template <int D, int G>
 struct Smem {
   using S = Stage<D, G>;
   static constexpr int kQuery = D / 32 * 32 * 32;  // [word][lane][8]: three digits of 32 bits twice, two words idle
-  static constexpr int kRowWords = 1 + 3 * S::NG;  // unscale; sum, two centres a group
+  static constexpr int kRowWords = 1 + 4 * S::NG;  // unscale; sum, three centres a group
   static constexpr int kRowBytes = kRows * kRowWords * 4;
   static constexpr int kWarp = kRing<D> * S::kBytes;
   static constexpr int kJoint = D + 1;                     // floats of a row of sums at the end
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   using S = Stage<D, G>;
   using M = Smem<D, G>;
   constexpr int kStages = kRing<D>;
-  constexpr int NG = S::NG, KW = D / 32, NT = D / 16;  // KW: words of a lane's keys, 32 dimensions of the row each
+  constexpr int NG = S::NG, NT = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ long long s_warp[kWarps];
   __shared__ long long s_at;
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   const int page_mask = (1 << p.cache.shift) - 1;
 
   // ---- queue of loads of a tile: a unit is four runs of consecutive bytes ----
-  const uint8_t *k_src, *v_src, *pair_src;
+  uint32_t head_at;  // bytes from a page's codes to the head's
   const int* table;
   int s0, s1, see_most, page[kSub];
   unsigned valid = 0;  // kSub bits a stage
@@ -356,16 +356,17 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
       if ((unsigned)page[u] < (unsigned)p.cache.num_blocks) {
         valid |= bit;
         const int pos = step * kStep + warp * kTokens + u * kUnit;
-        const size_t codes = (size_t)(uint32_t)page[u] * page_bytes + (pos & page_mask) * S::kRowBytes;
+        const size_t codes = (size_t)(uint32_t)page[u] * page_bytes + (head_at + (pos & page_mask) * S::kRowBytes);
         const uint32_t dst = ring_addr + stage * S::kBytes + u * S::kUnitBytes;
         const uint32_t dst0 = dst + piece_dst, dst1 = dst + (D == 256 ? piece_dst ^ 16 : piece_dst);
-        const uint8_t *kc = k_src + codes, *vc = v_src + codes;
+        const uint8_t *kc = p.cache.k_codes + codes + lane * 16, *vc = p.cache.v_codes + codes + lane * 16;
 #pragma unroll
         for (int i = 0; i < S::kCodes / 512; ++i) {
           cp_async16((i & 1 ? dst1 : dst0) + i * 512, kc + i * 512);
           cp_async16((i & 1 ? dst1 : dst0) + S::kCodes + i * 512, vc + i * 512);
         }
-        if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, pair_src + codes / (S::kRowBytes / NG / 4));
+        if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, reinterpret_cast<const uint8_t*>(lane < 16 ? p.cache.k_scales : p.cache.v_scales) +
+                                                              codes / (S::kRowBytes / NG / 4) + (lane & 15) * 16);
       }
     }
     cp_commit();
@@ -379,11 +380,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   constexpr int kPasses = (kRows * LPR + kThreads - 1) / kThreads;
   float q[kPasses][8];
   auto begin = [&](const Tile& x) {
-    const size_t head_row = (size_t)x.head << p.cache.shift;
-    k_src = p.cache.k_codes + head_row * S::kRowBytes + lane * 16;
-    v_src = p.cache.v_codes + head_row * S::kRowBytes + lane * 16;
-    pair_src = reinterpret_cast<const uint8_t*>((lane < 16 ? p.cache.k_scales : p.cache.v_scales) + head_row * NG +
-                                                (lane & 15) * 4);
+    head_at = (uint32_t)(x.head << p.cache.shift) * S::kRowBytes;
     table = p.block_tables + (size_t)x.b * p.max_blocks;
     s0 = max(x.c0 - kTileCost, 0);
     s1 = max(x.c1 - kTileCost, 0);
@@ -432,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
         const int e = top > 0.f && top < INFINITY ? min(21 - ilogbf(top), 120) : 0;
         const float norm = ldexpf(1.f, e);
         float sum = 0.f;
-        int upper = 0, lower = 0;
+        int sums[3] = {};  // of the digits
         uint32_t digits[3][2] = {};  // highest first; of the even, the odd dimensions
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -442,8 +439,9 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
           x = (x - d0) >> 8;
           const int d1 = (int8_t)x;
           x = (x - d1) >> 8;
-          upper += x * 256 + d1;
-          lower += d0;
+          sums[0] += x;
+          sums[1] += d1;
+          sums[2] += d0;
           digits[0][i & 1] |= (uint32_t)(x & 255) << (i / 2 * 8);
           digits[1][i & 1] |= (uint32_t)(d1 & 255) << (i / 2 * 8);
           digits[2][i & 1] |= (uint32_t)(d0 & 255) << (i / 2 * 8);
@@ -451,8 +449,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 #pragma unroll
         for (int off = G / 16; off > 0; off >>= 1) {
           sum += __shfl_xor_sync(0xffffffffu, sum, off);
-          upper += __shfl_xor_sync(0xffffffffu, upper, off);
-          lower += __shfl_xor_sync(0xffffffffu, lower, off);
+#pragma unroll
+          for (int d = 0; d < 3; ++d) sums[d] += __shfl_xor_sync(0xffffffffu, sums[d], off);
         }
         const int y = at8 / (G / 8), tt = at8 % (G / 8) / (G / 32), w = y * (G / 32) + at8 % (G / 32);
         uint32_t* dst = query + (w * 32 + r * 4 + tt) * 8;
@@ -461,34 +459,25 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
         float* num = row_num + r * M::kRowWords;
         if (at8 == 0) num[0] = ldexpf(1.f, -e) + odd;
         if (at8 % (G / 8) == 0) {
-          num[1 + 3 * y] = sum;
-          num[2 + 3 * y] = __int_as_float(-8 * upper);
-          num[3 + 3 * y] = __int_as_float(-8 * lower);
+          num[1 + 4 * y] = sum;
+#pragma unroll
+          for (int d = 0; d < 3; ++d) num[2 + 4 * y + d] = kSumStart + (float)(8 * sums[d]);
         }
       }
       __syncthreads();
-      uint32_t qd[KW][3][2];  // digits of row g
-#pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const uint32_t* src = query + (w * 32 + lane) * 8;
-        const uint4 v = *reinterpret_cast<const uint4*>(src);
-        const uint2 x = *reinterpret_cast<const uint2*>(src + 4);
-        qd[w][0][0] = v.x, qd[w][0][1] = v.y, qd[w][1][0] = v.z, qd[w][1][1] = v.w;
-        qd[w][2][0] = x.x, qd[w][2][1] = x.y;
-      }
       // of the lane's rows 2t, 2t + 1
       float unscale[2], qsum[NG][2], off_sum[NG][2], l[2] = {0.f, 0.f};
       float ref[2] = {-INFINITY, -INFINITY};  // weights are 2^(s - ref + 10) s_v
-      int centre[NG][2][2];                   // -8 times the sums of the upper two digits and of the lowest
+      float centre[NG][3][2];                 // where a digit's sum begins, and 8 times the sum of the row's digits
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float* num = row_num + (2 * t + i) * M::kRowWords;
         unscale[i] = num[0];
 #pragma unroll
         for (int y = 0; y < NG; ++y) {
-          qsum[y][i] = num[1 + 3 * y];
-          centre[y][0][i] = __float_as_int(num[2 + 3 * y]);
-          centre[y][1][i] = __float_as_int(num[3 + 3 * y]);
+          qsum[y][i] = num[1 + 4 * y];
+#pragma unroll
+          for (int d = 0; d < 3; ++d) centre[y][d][i] = num[2 + 4 * y + d];
           off_sum[y][i] = 0.f;
         }
       }
@@ -551,15 +540,19 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
             int c[3][4];
 #pragma unroll
             for (int i = 0; i < G / 32; ++i) {
+              // the digits of row g: from shared memory again, for the registers' sake
+              const uint32_t* qs = query + ((y * (G / 32) + i) * 32 + lane) * 8;
+              const uint4 q4 = *reinterpret_cast<const uint4*>(qs);
+              const uint2 q2 = *reinterpret_cast<const uint2*>(qs + 4);
+              const uint32_t qd[3][2] = {{q4.x, q4.y}, {q4.z, q4.w}, {q2.x, q2.y}};
               const uint32_t a[4] = {w[0][i] & 0x0F0F0F0Fu, w[1][i] & 0x0F0F0F0Fu, w[0][i] >> 4 & 0x0F0F0F0Fu,
                                      w[1][i] >> 4 & 0x0F0F0F0Fu};
 #pragma unroll
               for (int d = 0; d < 3; ++d) {
-                const uint32_t(&q)[2] = qd[y * (G / 32) + i][d];
                 if (i == 0)
-                  mma16832_first(c[d], a, q[0], q[1]);
+                  mma16832_first(c[d], a, qd[d][0], qd[d][1]);
                 else
-                  mma16832(c[d], a, q[0], q[1]);
+                  mma16832(c[d], a, qd[d][0], qd[d][1]);
               }
             }
 #pragma unroll
@@ -568,9 +561,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
               const float ks = half_lo(pair), km = fmaf(ks, 8.f, half_hi(pair));
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const float upper = (float)(c[0][2 * j + i] * 256 + c[1][2 * j + i] + centre[y][0][i]);
-                const float lower = (float)(c[2][2 * j + i] + centre[y][1][i]);
-                sc[u][j][i] = fmaf(fmaf(upper, 256.f, lower), ks, fmaf(qsum[y][i], km, sc[u][j][i]));
+                float dot = __int_as_float(c[0][2 * j + i]) - centre[y][0][i];  // exact, as the next two
+                dot = fmaf(dot, 256.f, __int_as_float(c[1][2 * j + i]) - centre[y][1][i]);
+                dot = fmaf(dot, 256.f, __int_as_float(c[2][2 * j + i]) - centre[y][2][i]);
+                sc[u][j][i] = fmaf(dot, ks, fmaf(qsum[y][i], km, sc[u][j][i]));
               }
             }
           }
@@ -658,14 +652,16 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
             for (int z = y * (G / 32); z < (y + 1) * (G / 32); z += 2) {  // 32 dimensions each
               uint32_t c[4];  // of 4 dimensions: tokens 2t, 2t + 1; 8 + 2t, 9 + 2t; then of the next 32
               ldmatrix_trans(c, ring_addr + (uint32_t)(st - ring) + u * S::kUnitBytes + v_row + (v_piece ^ z) * 16);
+              uint32_t a[4][4];
 #pragma unroll
               for (int h = 0; h < 4; ++h) {
                 uint32_t x = c[h / 2 * 2], x8 = c[h / 2 * 2 + 1];
                 if (h & 1) x >>= 8, x8 >>= 8;
-                const uint32_t a[4] = {codes_lo(x), codes_hi(x), codes_lo(x8), codes_hi(x8)};
-                mma16816(o[2 * z + h], a, hi[0], hi[1]);
-                mma16816(o[2 * z + h], a, lo[0], lo[1]);
+                a[h][0] = codes_lo(x), a[h][1] = codes_hi(x), a[h][2] = codes_lo(x8), a[h][3] = codes_hi(x8);
+                mma16816(o[2 * z + h], a[h], hi[0], hi[1]);
               }
+#pragma unroll
+              for (int h = 0; h < 4; ++h) mma16816(o[2 * z + h], a[h], lo[0], lo[1]);
             }
           }
         }
@@ -705,8 +701,9 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          float x = o[i][k] + off_sum[i / (G / 16)][k & 1];
+          float x = o[i][k];
           if (flushed) x += kept[(4 * i + k) * 32];
+          x = fmaf(x, kCodes, off_sum[i / (G / 16)][k & 1]);
           joint[(2 * t + (k & 1)) * M::kJoint + i / 2 * 32 + 4 * g + i % 2 * 2 + k / 2] = x;
         }
       if (g == 0) {
