@@ -147,6 +147,7 @@ struct Kv4AttentionParams {
   long long q_stride, o_stride;
   int tokens, batch, q_heads, max_blocks;
   float scale;
+  double inv_ctas;  // 1 / CTAs, set at the launch
 };
 size_t kv4_attention_workspace(int head_dim, int sm_count);
 cudaError_t launch_kv4_attention(const Kv4AttentionParams& p, int dtype, int sm_count,

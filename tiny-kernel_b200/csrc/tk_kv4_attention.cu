@@ -43,7 +43,7 @@ constexpr int kSub = 2;        // units of a warp's step
 constexpr int kTokens = kUnit * kSub;
 constexpr int kStep = kTokens * kWarps;
 template <int D>
-constexpr int kRing = 2;  // stages of a warp's ring
+constexpr int kRing = D == 256 ? 2 : 3;  // stages of a warp's ring
 template <int D>
 constexpr int kResident = D == 256 ? 2 : 3;  // CTAs of an SM
 constexpr int kFlush = 16;     // steps between two settings aside of the sums
@@ -264,8 +264,6 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   Part* parts = static_cast<Part*>(p.workspace);
   float* sums = reinterpret_cast<float*>(parts + gridDim.x);
   constexpr int kSlot = kRows * (D + 2);
-  // this warp's sums of earlier steps (kFlush): [product][lane]
-  float* kept = sums + (size_t)gridDim.x * 2 * kSlot + ((size_t)blockIdx.x * kWarps + warp) * kRows * D + lane;
 
   // ---- this CTA's run ----
   const int chunk = (p.batch + kThreads - 1) / kThreads;
@@ -289,7 +287,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
     if (w < warp) before += s_warp[w];
     total += s_warp[w];
   }
-  const long long run = max((total + gridDim.x - 1) / gridDim.x, (long long)kMinRun);
+  // (a quotient in f64, rounded up at least: 64-bit division takes as long as a load)
+  const long long run = max((long long)__dmul_ru((double)total, p.inv_ctas) + 1, (long long)kMinRun);
   const long long start = run * blockIdx.x, stop = min(start + run, total);
   if (tid == 0) parts[blockIdx.x].count = 0;
   if (start >= stop) return;
@@ -310,7 +309,9 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   cur.b = s_seq;
   cur.s = sequence(p, cur.b, per);
   {
-    const long long unit = s_at / cur.s.steps;
+    long long unit = (long long)((double)s_at / cur.s.steps);  // off by one at most
+    if (unit * cur.s.steps > s_at) --unit;
+    if ((unit + 1) * cur.s.steps <= s_at) ++unit;
     cur.c0 = (int)(s_at - unit * cur.s.steps);
     cur.head = (int)unit / cur.s.tiles;
     cur.rt = (int)unit - cur.head * cur.s.tiles;
@@ -323,6 +324,11 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   uint8_t* ring = smem + M::kRings + warp * M::kWarp;
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
   float* joint = reinterpret_cast<float*>(smem + M::kJoints) + warp * M::kJointWarp;
+  // the lane's sum o[i][k] in it: row 2t + k % 2, dimension 32 (i / 2) + 4g + 2 (i % 2) + k / 2
+  float* mine_at = joint + 2 * t * M::kJoint + 4 * g;
+  auto kept = [&](int i, int k) -> float& {
+    return mine_at[(k & 1) * M::kJoint + i / 2 * 32 + i % 2 * 2 + k / 2];
+  };
 
   // where the lane's pieces go in a unit, and where its operands lie
   // (piece 32 i + lane lies 512 i on, at D = 256 with one bit of its place turned for odd i)
@@ -335,9 +341,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   const uint32_t v_row = S::kCodes + (lane & 15) * S::kRowBytes, v_piece = (lane >> 4) ^ S::flip(lane & 15);
   const uint32_t page_bytes = (uint32_t)(hk << p.cache.shift) * S::kRowBytes;  // at most 2^16 heads of 2^8 rows of 2^7
   const int page_mask = (1 << p.cache.shift) - 1;
+  const ptrdiff_t k_to_v = p.cache.v_codes - p.cache.k_codes;
 
   // ---- queue of loads of a tile: a unit is four runs of consecutive bytes ----
-  uint32_t head_at;  // bytes from a page's codes to the head's
+  const uint8_t *k_src, *pair_src;  // of the head in page 0, and the lane's piece
   const int* table;
   int s0, s1, see_most, page[kSub];
   unsigned valid = 0;  // kSub bits a stage
@@ -356,51 +363,56 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
       if ((unsigned)page[u] < (unsigned)p.cache.num_blocks) {
         valid |= bit;
         const int pos = step * kStep + warp * kTokens + u * kUnit;
-        const size_t codes = (size_t)(uint32_t)page[u] * page_bytes + (head_at + (pos & page_mask) * S::kRowBytes);
+        const uint64_t codes = (uint64_t)(uint32_t)page[u] * page_bytes + (uint32_t)((pos & page_mask) * S::kRowBytes);
         const uint32_t dst = ring_addr + stage * S::kBytes + u * S::kUnitBytes;
         const uint32_t dst0 = dst + piece_dst, dst1 = dst + (D == 256 ? piece_dst ^ 16 : piece_dst);
-        const uint8_t *kc = p.cache.k_codes + codes + lane * 16, *vc = p.cache.v_codes + codes + lane * 16;
+        const uint8_t *kc = k_src + codes, *vc = kc + k_to_v;
 #pragma unroll
         for (int i = 0; i < S::kCodes / 512; ++i) {
           cp_async16((i & 1 ? dst1 : dst0) + i * 512, kc + i * 512);
           cp_async16((i & 1 ? dst1 : dst0) + S::kCodes + i * 512, vc + i * 512);
         }
-        if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, reinterpret_cast<const uint8_t*>(lane < 16 ? p.cache.k_scales : p.cache.v_scales) +
-                                                              codes / (S::kRowBytes / NG / 4) + (lane & 15) * 16);
+        if ((lane & 15) < 4 * NG) cp_async16(dst + pair_dst, pair_src + codes / (S::kRowBytes / NG / 4));
       }
     }
     cp_commit();
   };
+  // a row's query token of its sequence; a row is (token, head of the group)
+  auto token_of = [&](const Tile& x, int row) { return x.s.n == 1 ? 0 : row / per; };
   // the position after the last that row r of a tile sees; its last row sees most, its first least
   auto sees = [&](const Tile& x, int r) {
     const int row = x.rt * kRows + r, end = x.s.n * per - 1;
-    return min(x.s.kv, x.s.last + min(row, end) / per + 1);
+    return min(x.s.kv, x.s.last + token_of(x, min(row, end)) + 1);
   };
   constexpr int LPR = D / 8;                                   // threads of a row of queries, 8 dimensions each
   constexpr int kPasses = (kRows * LPR + kThreads - 1) / kThreads;
   float q[kPasses][8];
   auto begin = [&](const Tile& x) {
-    head_at = (uint32_t)(x.head << p.cache.shift) * S::kRowBytes;
+    const uint64_t head_at = (uint64_t)(uint32_t)(x.head << p.cache.shift) * S::kRowBytes;
+    k_src = p.cache.k_codes + head_at + lane * 16;
+    pair_src = reinterpret_cast<const uint8_t*>(lane < 16 ? p.cache.k_scales : p.cache.v_scales) +
+               head_at / (S::kRowBytes / NG / 4) + (lane & 15) * 16;
     table = p.block_tables + (size_t)x.b * p.max_blocks;
     s0 = max(x.c0 - kTileCost, 0);
     s1 = max(x.c1 - kTileCost, 0);
     see_most = sees(x, kRows - 1);
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-      look(s0 + i);
-      issue(i, s0 + i);
-    }
-    look(s0 + kStages - 1);
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * (kThreads / LPR) + tid / LPR;
       const int row = min(x.rt * kRows + r, x.s.n * per - 1);
 #pragma unroll
       for (int k = 0; k < 8; ++k) q[i][k] = 0.f;
+      const int token = token_of(x, row);
       if (r < kRows && sees(x, r) > 0)
-        load_row8(p.q, (long long)(x.s.first + row / per) * p.q_stride + (long long)(x.head * per + row % per) * D +
+        load_row8(p.q, (long long)(x.s.first + token) * p.q_stride + (long long)(x.head * per + row - token * per) * D +
                            tid % LPR * 8, dtype, q[i]);
     }
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      look(s0 + i);
+      issue(i, s0 + i);
+    }
+    look(s0 + kStages - 1);
   };
   begin(cur);
 
@@ -614,8 +626,12 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
             o[i][2] *= f0;
             o[i][3] *= f1;
           }
-          if (flushed)
-            for (int i = 0; i < 4 * NT; ++i) kept[i * 32] *= i & 1 ? f1 : f0;
+          if (flushed) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) kept(i, k) *= k & 1 ? f1 : f0;
+          }
         }
         const float base[2] = {ref[0] == -INFINITY ? 0.f : 10.f - ref[0], ref[1] == -INFINITY ? 0.f : 10.f - ref[1]};
 
@@ -671,15 +687,15 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
         else
           step_of(std::false_type{});
         // The tensor core drops what lies under the last bit of a sum, always towards 0: its sums are
-        // set aside before that adds up (f32 outputs over 8192 positions of one CTA: 2.8e-6 off).
+        // set aside, in the warp's place for the join, before that adds up (f32 outputs over 8192 positions
+        // of one CTA: 2.8e-6 off without it).
         if (++since == kFlush) {
           since = 0;
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              float* x = kept + (4 * i + k) * 32;
-              *x = flushed ? *x + o[i][k] : o[i][k];
+              kept(i, k) = flushed ? kept(i, k) + o[i][k] : o[i][k];
               o[i][k] = 0.f;
             }
           flushed = true;
@@ -702,9 +718,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float x = o[i][k];
-          if (flushed) x += kept[(4 * i + k) * 32];
-          x = fmaf(x, kCodes, off_sum[i / (G / 16)][k & 1]);
-          joint[(2 * t + (k & 1)) * M::kJoint + i / 2 * 32 + 4 * g + i % 2 * 2 + k / 2] = x;
+          if (flushed) x += kept(i, k);
+          kept(i, k) = fmaf(x, kCodes, off_sum[i / (G / 16)][k & 1]);
         }
       if (g == 0) {
 #pragma unroll
@@ -753,8 +768,9 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
         }
         float* out = sums + ((size_t)blockIdx.x * 2 + slot) * kSlot;
         const int query_row = row0 + min(row, rows - 1);
-        const long long o_at = (long long)(done.s.first + query_row / per) * p.o_stride +
-                               (long long)(done.head * per + query_row % per) * D;
+        const int token = token_of(done, query_row);
+        const long long o_at = (long long)(done.s.first + token) * p.o_stride +
+                               (long long)(done.head * per + query_row - token * per) * D;
 #pragma unroll
         for (int d = d0; d < D; d += kThreadsRow) {
           float v = 0.f;
@@ -798,25 +814,40 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(K
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = warp / kJoinWarps, w = warp % kJoinWarps;
   const int row = blockIdx.y * kJoinRows + r0;
   auto base = [&](int i) { return sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot; };
+  // the lane's part of each 32: its reference and l, then its factor
   float top = -INFINITY;
   for (int i = lane; i < part.count; i += 32) top = fmaxf(top, base(i)[kRows * D + 2 * row]);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  float sum = 0.f, v[D / 32];
+  constexpr int V = D == 64 ? 2 : 4, E = D / (32 * V);  // values of a load, loads of a row
+  float sum = 0.f, v[E][V];
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) v[e] = 0.f;
-#pragma unroll 4
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[e][k] = 0.f;
+#pragma unroll 8
   for (int i = w; i < part.count; i += kJoinWarps) {
     const float* s = base(i);
-    const float r = s[kRows * D + 2 * row];
-    const float f = r == -INFINITY ? 1.f : ex2(r - top);  // no reference: sums of 0, or of NaN
-    sum = fmaf(s[kRows * D + 2 * row + 1], f, sum);
+    const float2 num = *reinterpret_cast<const float2*>(s + kRows * D + 2 * row);
+    const float f = num.x == -INFINITY ? 1.f : ex2(num.x - top);  // no reference: sums of 0, or of NaN
+    sum = fmaf(num.y, f, sum);
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) v[e] = fmaf(s[row * D + e * 32 + lane], f, v[e]);
+    for (int e = 0; e < E; ++e) {
+      float x[V];
+      const float* src = s + row * D + (e * 32 + lane) * V;
+      if constexpr (V == 4)
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
+      else
+        *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[e][k] = fmaf(x[k], f, v[e][k]);
+    }
   }
   if (lane == 0) s_sum[r0][w] = sum;
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) s_v[r0][w][e * 32 + lane] = v[e];
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int k = 0; k < V; ++k) s_v[r0][w][(e * 32 + lane) * V + k] = v[e][k];
   __syncthreads();
   if (row >= part.rows) return;
   sum = 0.f;
@@ -835,7 +866,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(K
 int attention_ctas(int head_dim, int sm_count) { return sm_count * (head_dim == 256 ? kResident<256> : kResident<128>); }
 
 template <int D, int G>
-cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStream_t st) {
+cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t st) {
   const size_t smem = Smem<D, G>::kBytes;
   cudaError_t e;
   if (smem > 48 * 1024) {
@@ -846,6 +877,7 @@ cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStr
   // programmatic launches: a kernel is set up while the one before it runs, and passes its wait when
   // that has completed
   const int ctas = attention_ctas(D, sm_count);
+  p.inv_ctas = 1.0 / ctas;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -867,8 +899,7 @@ cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStr
 }  // namespace
 
 size_t kv4_attention_workspace(int head_dim, int sm_count) {
-  return (size_t)attention_ctas(head_dim, sm_count) *
-         (sizeof(Part) + 2 * part_bytes(head_dim) + (size_t)kWarps * kRows * head_dim * sizeof(float));
+  return (size_t)attention_ctas(head_dim, sm_count) * (sizeof(Part) + 2 * part_bytes(head_dim));
 }
 
 cudaError_t launch_kv4_attention(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStream_t st) {
