@@ -5,11 +5,33 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "tk_kv4.h"
 
 namespace tk {
 namespace {
+
+// Programmatic launches: a kernel is set up while the one before it in the stream runs; it reads
+// nothing, and no thread of it ends, before that one has completed.
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <class... P, class... A>
+cudaError_t launch(void (*kernel)(P...), long long blocks, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 
 // ---- elements ------------------------------------------------------------------------------------
 
@@ -60,38 +82,75 @@ __device__ __forceinline__ void store_f32(T* dst, bool vec, const float (&v)[E])
   }
 }
 
+// E/2 elements at src and E/2 at src + next.  vec: both on the boundary of their 8 or 16 bytes.
+template <class T, int E>
+__device__ __forceinline__ void load_halves(const T* src, int next, bool vec, float (&v)[E]) {
+  constexpr int H = E / 2;
+  using V = typename std::conditional<H * sizeof(T) == 16, uint4, uint2>::type;
+  if (vec) {
+    V raw[2] = {*reinterpret_cast<const V*>(src), *reinterpret_cast<const V*>(src + next)};
+    const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = to_f32(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = to_f32(src[(i / H) * next + i % H]);
+  }
+}
+template <class T, int E>
+__device__ __forceinline__ void store_halves(T* dst, int next, bool vec, const float (&v)[E]) {
+  constexpr int H = E / 2;
+  using V = typename std::conditional<H * sizeof(T) == 16, uint4, uint2>::type;
+  if (vec) {
+    V raw[2];
+    T* e = reinterpret_cast<T*>(raw);
+#pragma unroll
+    for (int i = 0; i < E; ++i) e[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<V*>(dst) = raw[0];
+    *reinterpret_cast<V*>(dst + next) = raw[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) dst[(i / H) * next + i % H] = from_f32<T>(v[i]);
+  }
+}
+
 // ---- block tables and slots ----------------------------------------------------------------------
 //
 // Two exclusive prefix sums over the requests (tokens, pages to take) give every token its request
 // and every page its place in the free list.  Every CTA computes the sums itself: 8 bytes a request
 // from L2, against a second launch or a wait between CTAs.  A thread owns a run of consecutive
 // requests and only the sums at the runs' starts are kept, so the batch has no limit; a token finds
-// its run by binary search and walks it.  No atomics: the last CTA writes what is per request and
-// counts the tokens without a slot on its own.
+// its run by binary search and walks it.  No atomics: one CTA (the only
+// one of a small step) writes what is per request and counts the tokens without a slot.
 constexpr int kSlotsThreads = 256;
-constexpr int kSlotsTokens = 4;  // consecutive tokens of a thread: one search, 16-byte stores
 
-__device__ __forceinline__ long long block_exclusive_scan(long long v, long long* warp_sums,
-                                                          long long* total) {
+// Exclusive sums of two values a thread; totals in all[2].
+struct SlotsSums {
+  long long tokens, pages;
+};
+__device__ __forceinline__ SlotsSums block_exclusive_scan(SlotsSums v, SlotsSums* warp_sums, SlotsSums* all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long inc = v;
+  SlotsSums inc = v;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, inc, off);
-    if (lane >= off) inc += o;
+    const long long t = __shfl_up_sync(0xffffffffu, inc.tokens, off), g = __shfl_up_sync(0xffffffffu, inc.pages, off);
+    if (lane >= off) {
+      inc.tokens += t;
+      inc.pages += g;
+    }
   }
   __syncthreads();  // the sums of an earlier scan have been read
   if (lane == 31) warp_sums[warp] = inc;
   __syncthreads();
-  long long before = 0, all = 0;
+  SlotsSums before{0, 0}, total{0, 0};
 #pragma unroll
   for (int w = 0; w < kSlotsThreads / 32; ++w) {
-    const long long s = warp_sums[w];
-    if (w < warp) before += s;
-    all += s;
+    const SlotsSums s = warp_sums[w];
+    if (w < warp) before = {before.tokens + s.tokens, before.pages + s.pages};
+    total = {total.tokens + s.tokens, total.pages + s.pages};
   }
-  *total = all;
-  return before + inc - v;
+  *all = total;
+  return {before.tokens + inc.tokens - v.tokens, before.pages + inc.pages - v.pages};
 }
 
 // The last run whose sum is at most `at`.
@@ -118,39 +177,56 @@ struct SlotsCursor {
   }
 };
 
+// TOK: consecutive tokens of a thread (4: one search and 16-byte stores for four).
+template <int TOK>
 __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(SlotsParams p) {
-  __shared__ long long s_start[kSlotsThreads], s_first[kSlotsThreads], s_warp[kSlotsThreads / 32];
+  __shared__ long long s_start[kSlotsThreads], s_first[kSlotsThreads];
+  __shared__ SlotsSums s_warp[kSlotsThreads / 32];
+  after_previous();
   const int tid = threadIdx.x;
+  const bool alone = gridDim.x == 1, requests = blockIdx.x == gridDim.x - 1;
   const int per = (p.batch + kSlotsThreads - 1) / kSlotsThreads;
-  const int r0 = min((long long)p.batch, (long long)tid * per), r1 = min(p.batch, r0 + per);
+  const int r0 = (int)min((long long)p.batch, (long long)tid * per), r1 = min(p.batch, r0 + per);
   const int begin = p.free_range[0], end = p.free_range[1];
+  const int bs1 = (1 << p.shift) - 1;
 
-  long long sum = 0, asked, taken;
-  for (int r = r0; r < r1; ++r) sum += slots_wanted(p.context_lens[r], p.query_lens[r]);
-  const long long start0 = block_exclusive_scan(sum, s_warp, &asked);
-  SlotsCursor c{r0, start0, 0, {}};
-  while (c.r < r1) {
-    c.at(p);
-    c.next(p);
+  // Both sums at once, as if all tokens had room; if they have not, the pages are summed again.
+  SlotsSums sum{0, 0}, all;
+  for (int r = r0; r < r1; ++r) {
+    const int ctx = p.context_lens[r], q = p.query_lens[r];
+    const SlotsRequest x = slots_request(ctx, q, -0x7fffffffffffll, p.shift, p.max_blocks, p.max_tokens);
+    sum.tokens += slots_wanted(ctx, q);
+    sum.pages += x.need - x.have;
   }
-  const long long first0 = block_exclusive_scan(c.first, s_warp, &taken);
+  SlotsSums at0 = block_exclusive_scan(sum, s_warp, &all);
+  const long long asked = all.tokens, start0 = at0.tokens;
+  SlotsCursor c;
+  if (asked > p.max_tokens) {
+    c = {r0, start0, 0, {}};
+    while (c.r < r1) {
+      c.at(p);
+      c.next(p);
+    }
+    at0 = block_exclusive_scan({0, c.first}, s_warp, &all);
+  }
+  const long long first0 = at0.pages, taken = all.pages;
   s_start[tid] = start0;
   s_first[tid] = first0;
   __syncthreads();
   const int tokens = (int)min(asked, (long long)p.max_tokens);
-  const int bs1 = (1 << p.shift) - 1;
 
   const bool wide = ((reinterpret_cast<uintptr_t>(p.positions) | reinterpret_cast<uintptr_t>(p.slots)) & 15) == 0;
-  for (long long t0 = ((long long)blockIdx.x * kSlotsThreads + tid) * kSlotsTokens; t0 < p.max_tokens;
-       t0 += (long long)gridDim.x * kSlotsThreads * kSlotsTokens) {
-    int pos[kSlotsTokens], slot[kSlotsTokens];
+  const int token_ctas = alone ? 1 : gridDim.x - 1;
+  for (long long t0 = ((long long)blockIdx.x * kSlotsThreads + tid) * TOK;
+       t0 < p.max_tokens && (alone || !requests); t0 += (long long)token_ctas * kSlotsThreads * TOK) {
+    int pos[TOK], slot[TOK];
     if (t0 < tokens) {
       const int run = find_run(s_start, t0);
       c = {run * per, s_start[run], s_first[run], {}};
       c.at(p);
     }
 #pragma unroll
-    for (int i = 0; i < kSlotsTokens; ++i) {
+    for (int i = 0; i < TOK; ++i) {
       const long long t = t0 + i;
       pos[i] = slot[i] = -1;
       if (t >= tokens) continue;
@@ -172,12 +248,17 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(SlotsParams 
       }
       if (id >= 0) slot[i] = (id << p.shift) + (pos[i] & bs1);
     }
-    if (wide && t0 + kSlotsTokens <= p.max_tokens) {
-      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-      *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-    } else {
+    bool stored = false;
+    if constexpr (TOK == 4) {
+      if (wide && t0 + TOK <= p.max_tokens) {
+        *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        stored = true;
+      }
+    }
+    if (!stored) {
 #pragma unroll
-      for (int i = 0; i < kSlotsTokens; ++i)
+      for (int i = 0; i < TOK; ++i)
         if (t0 + i < p.max_tokens) {
           p.positions[t0 + i] = pos[i];
           p.slots[t0 + i] = slot[i];
@@ -185,7 +266,7 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(SlotsParams 
     }
   }
 
-  if (blockIdx.x != gridDim.x - 1) return;
+  if (!requests) return;
   long long without = 0;
   c = {r0, start0, first0, {}};
   while (c.r < r1) {
@@ -201,24 +282,39 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(SlotsParams 
     without += max(0ll, (long long)q.ctx + q.q - reach);
     c.next(p);
   }
-  for (long long a = tid; a < taken; a += kSlotsThreads) {  // pages that the pool did not have
-    if (slots_new_block(p.free_blocks, begin, end, a, p.num_blocks) >= 0) continue;
-    const int run = find_run(s_first, a);
-    c = {run * per, s_start[run], s_first[run], {}};
-    c.at(p);
-    while (a >= c.first + c.req.need - c.req.have) {
-      c.next(p);
-      c.at(p);
+  constexpr int kIds = 16;  // reads in flight of a thread
+  const long long free0 = begin > 0 ? begin : 0;
+  for (long long a0 = tid; a0 < taken; a0 += kSlotsThreads * kIds) {  // pages that the pool did not have
+    int id[kIds];
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {  // read without a branch, some valid place at least
+      const long long x = free0 + a0 + i * kSlotsThreads;
+      id[i] = free0 < end ? p.free_blocks[x < end ? x : free0] : -1;
     }
-    without += slots_tokens_in(c.req, c.req.have + (int)(a - c.first), p.shift);
+#pragma unroll 1
+    for (int i = 0; i < kIds; ++i) {
+      const long long a = a0 + (long long)i * kSlotsThreads;
+      int v = id[0];
+#pragma unroll
+      for (int k = 1; k < kIds; ++k)
+        if (k == i) v = id[k];
+      if (a >= taken || (free0 + a < end && v >= 0 && v < p.num_blocks)) continue;
+      const int run = find_run(s_first, a);
+      c = {run * per, s_start[run], s_first[run], {}};
+      c.at(p);
+      while (a >= c.first + c.req.need - c.req.have) {
+        c.next(p);
+        c.at(p);
+      }
+      without += slots_tokens_in(c.req, c.req.have + (int)(a - c.first), p.shift);
+    }
   }
-  long long all;
-  block_exclusive_scan(without, s_warp, &all);
+  block_exclusive_scan({without, 0}, s_warp, &all);
   if (tid == 0) {
     p.query_start[p.batch] = tokens;
     p.counts[0] = tokens;
     p.counts[1] = (int)taken;
-    p.counts[2] = (int)all;
+    p.counts[2] = (int)all.tokens;
     const long long first = begin > 0 ? begin : 0;
     p.counts[3] = (int)max(first, min(first + taken, (long long)end));
   }
@@ -236,78 +332,123 @@ __device__ __forceinline__ QkRow qk_row(const QkNormRopeParams& p, int head) {
   return head < p.heads[0] ? QkRow{0, head} : QkRow{1, head - p.heads[0]};
 }
 
-// LPH lanes hold a head, E consecutive values each (16 or 32 bytes); the pair of a value lies
+// LPH lanes hold a head, E values each (16 or 32 bytes); a group of lanes takes HB queries or keys of
+// a token, so that weights and angles are read once and HB loads are in flight: bound by HBM.
+// HALVES (the whole head turns, by halves): a lane holds E/2 consecutive values of each half and so
+// both values of a pair, and half as many angles.  Otherwise E consecutive values; the pair of one lies
 // rot_dim / 2 values on, a multiple of E: the same place in another lane.
-template <class T, int E, int LPH>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, int vec_in, int vec_out,
-                                                           int heads_per_group) {
+template <class T, int E, int LPH, int HB, bool HALVES>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, int vec_in, int vec_out, int vec_turn) {
+  constexpr int H = E / 2, D = E * LPH;
+  after_previous();
   const int lane = threadIdx.x & 31, l = lane % LPH;
-  const int heads = p.heads[0] + p.heads[1];
-  const int parts = (heads + heads_per_group - 1) / heads_per_group;
-  const long long group = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / LPH;
-  const long long token = group / parts;
-  const int h0 = (int)(group % parts) * heads_per_group, h1 = min(heads, h0 + heads_per_group);
+  const int q_parts = (p.heads[0] + HB - 1) / HB, parts = q_parts + (p.heads[1] + HB - 1) / HB;
+  const unsigned group = (unsigned)(((long long)blockIdx.x * blockDim.x + threadIdx.x) / LPH);  // below 2^31
+  const int token = (int)(group / (unsigned)parts), part = (int)(group - (unsigned)token * parts);
+  const int which = part >= q_parts, h0 = (which ? part - q_parts : part) * HB, heads = p.heads[which];
   const int half = p.rot_dim / 2;
   const int pos = token < p.tokens ? p.positions[token] : -1;
   const bool on = pos >= 0 && pos < p.max_pos;
   if (!__any_sync(0xffffffffu, on)) return;
 
-  // what the lane's values are turned by (1, 0 past rot_dim), and the lane of their pairs
-  float c[E], s[E];
-  int src = lane;
+  float y[HB][E];
+  const T* x = static_cast<const T*>(p.x[which]) + token * p.in_stride[which] + (long long)h0 * D;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = l * E + e;
-    const int j = p.interleaved ? i / 2 : (i < half ? i : i - half);
-    const bool turned = on && i < p.rot_dim;
-    c[e] = turned ? p.cos_cache[(size_t)pos * half + j] : 1.f;
-    s[e] = turned ? p.sin_cache[(size_t)pos * half + j] : 0.f;
-    if (p.interleaved ? (i & 1) == 0 : i < half) s[e] = -s[e];
+  for (int i = 0; i < HB; ++i) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[i][e] = 0.f;
+    if (on && h0 + i < heads) {
+      if constexpr (HALVES)
+        load_halves<T, E>(x + i * D + l * H, D / 2, vec_in, y[i]);
+      else
+        load_f32<T, E>(x + i * D + l * E, vec_in, y[i]);
+    }
   }
-  if (!p.interleaved && l * E < p.rot_dim) src = l * E < half ? lane + half / E : lane - half / E;
 
-  for (int h = h0; h < h0 + heads_per_group; ++h) {  // the same count in every lane of the warp
-    const bool mine = on && h < h1;
-    const QkRow r = qk_row(p, min(h, heads - 1));
-    float y[E];
+  // what the lane's values are turned by (1, 0 past rot_dim), and the lane of their pairs
+  constexpr int A = HALVES ? H : E;
+  float c[A], s[A];
+  int src = lane;
+  const bool turned = on && (HALVES || l * E < p.rot_dim);
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = 0.f;
-    if (mine)
-      load_f32<T, E>(static_cast<const T*>(p.x[r.which]) + token * p.in_stride[r.which] +
-                         (long long)r.head * p.head_dim + l * E,
-                     vec_in, y);
-    const float* w = p.weight[r.which];
-    if (w) {
+  for (int e = 0; e < A; ++e) c[e] = 1.f, s[e] = 0.f;
+  if (turned) {
+    const int j0 = HALVES ? l * H : (p.interleaved ? l * E / 2 : (l * E < half ? l * E : l * E - half));
+    const float* cp = p.cos_cache + (size_t)pos * half + j0;
+    const float* sp = p.sin_cache + (size_t)pos * half + j0;
+    if (vec_turn && !p.interleaved) {  // on a boundary of the A values, by pairs at least
+#pragma unroll
+      for (int e = 0; e < A; e += 2) {
+        const float2 cv = __ldg(reinterpret_cast<const float2*>(cp + e)), sv = __ldg(reinterpret_cast<const float2*>(sp + e));
+        c[e] = cv.x, c[e + 1] = cv.y;
+        s[e] = sv.x, s[e + 1] = sv.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < A; ++e)
+        if (HALVES || l * E + e < p.rot_dim) {
+          c[e] = __ldg(cp + (p.interleaved ? e / 2 : e));
+          s[e] = __ldg(sp + (p.interleaved ? e / 2 : e));
+        }
+    }
+    if constexpr (!HALVES) {
+#pragma unroll
+      for (int e = 0; e < A; ++e)
+        if (p.interleaved ? (e & 1) == 0 : l * E < half) s[e] = -s[e];
+      if (!p.interleaved) src = l * E < half ? lane + half / E : lane - half / E;
+    }
+  }
+  const float* wp = p.weight[which];
+  float w[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) w[e] = wp ? __ldg(wp + (HALVES ? (e / H) * (D / 2) + l * H + e % H : l * E + e)) : 1.f;
+
+  T* out = static_cast<T*>(p.out[which]) + token * p.out_stride[which] + (long long)h0 * D;
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    if (p.weight[0] || p.weight[1]) {  // the same for all lanes: queries and keys may share a warp
       float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) ss = fmaf(y[e], y[e], ss);
+      for (int e = 0; e < E; ++e) ss = fmaf(y[i][e], y[i][e], ss);
 #pragma unroll
       for (int off = LPH / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-      const float inv = rsqrtf(ss / (float)p.head_dim + p.eps);
+      if (wp) {
+        const float inv = rsqrtf(ss / (float)D + p.eps);
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = y[e] * inv * __ldg(w + l * E + e);
+        for (int e = 0; e < E; ++e) y[i][e] = y[i][e] * inv * w[e];
+      }
     }
-    // a value past rot_dim is its own pair, with sine 0: it must not meet an infinity times 0
     float z[E];
+    if constexpr (HALVES) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float other = p.interleaved ? y[e ^ 1] : __shfl_sync(0xffffffffu, y[e], src);
-      z[e] = l * E + e < p.rot_dim ? y[e] * c[e] + other * s[e] : y[e];
+      for (int e = 0; e < H; ++e) {
+        z[e] = y[i][e] * c[e] - y[i][H + e] * s[e];
+        z[H + e] = y[i][H + e] * c[e] + y[i][e] * s[e];
+      }
+    } else {
+      // a value past rot_dim is its own pair, with sine 0: it must not meet an infinity times 0
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float other = p.interleaved ? y[i][e ^ 1] : __shfl_sync(0xffffffffu, y[i][e], src);
+        z[e] = l * E + e < p.rot_dim ? y[i][e] * c[e] + other * s[e] : y[i][e];
+      }
     }
-    if (mine)
-      store_f32<T, E>(static_cast<T*>(p.out[r.which]) + token * p.out_stride[r.which] +
-                          (long long)r.head * p.head_dim + l * E,
-                      vec_out, z);
+    if (on && h0 + i < heads) {
+      if constexpr (HALVES)
+        store_halves<T, E>(out + i * D + l * H, D / 2, vec_out, z);
+      else
+        store_f32<T, E>(out + i * D + l * E, vec_out, z);
+    }
   }
 }
 
-// Any even head_dim up to kQkMaxDim: a warp per head, the normalised row in shared memory.
-constexpr int kQkMaxDim = 1024;
+// Any even head_dim (up to 1024, for the shared memory): a warp per head, the normalised row in it.
 constexpr int kQkWarps = 4;
 
 template <class T>
 __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_any_kernel(QkNormRopeParams p) {
   extern __shared__ float s_rows[];
+  after_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = p.head_dim, half = p.rot_dim / 2;
   float* row = s_rows + warp * d;
   const int heads = p.heads[0] + p.heads[1];
@@ -347,13 +488,18 @@ __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_any_kernel(QkNormR
 
 template <class T, int E, int LPH>
 cudaError_t qk_launch_vec(const QkNormRopeParams& p, bool vec_in, bool vec_out, int sm_count, cudaStream_t st) {
-  const int heads = p.heads[0] + p.heads[1];
-  const int hpg = 1;
-  (void)sm_count;
-  const long long groups = (long long)p.tokens * ((heads + hpg - 1) / hpg);
-  const long long blocks = (groups * LPH + 255) / 256;
-  qk_norm_rope_kernel<T, E, LPH><<<(unsigned)blocks, 256, 0, st>>>(p, vec_in, vec_out, hpg);
-  return cudaGetLastError();
+  const int vec_turn = (reinterpret_cast<uintptr_t>(p.cos_cache) | reinterpret_cast<uintptr_t>(p.sin_cache)) % 8 == 0 &&
+                       p.rot_dim / 2 % 2 == 0;
+  auto blocks = [&](int hb) {
+    return ((long long)p.tokens * ((p.heads[0] + hb - 1) / hb + (p.heads[1] + hb - 1) / hb) * LPH + 255) / 256;
+  };
+  const bool halves = !p.interleaved && p.rot_dim == p.head_dim;
+  // one head a group until every SM has its 2048 threads twice over
+  if (blocks(4) < 16ll * sm_count)
+    return launch(halves ? qk_norm_rope_kernel<T, E, LPH, 1, true> : qk_norm_rope_kernel<T, E, LPH, 1, false>,
+                  blocks(1), 256, 0, st, p, (int)vec_in, (int)vec_out, vec_turn);
+  return launch(halves ? qk_norm_rope_kernel<T, E, LPH, 4, true> : qk_norm_rope_kernel<T, E, LPH, 4, false>, blocks(4),
+                256, 0, st, p, (int)vec_in, (int)vec_out, vec_turn);
 }
 
 template <class T>
@@ -374,111 +520,148 @@ cudaError_t qk_launch(const QkNormRopeParams& p, int sm_count, cudaStream_t st) 
     if (p.head_dim == 256) return qk_launch_vec<T, 8, 32>(p, vec_in, vec_out, sm_count, st);
   }
   const long long units = (long long)p.tokens * (p.heads[0] + p.heads[1]);
-  qk_norm_rope_any_kernel<T><<<(unsigned)((units + kQkWarps - 1) / kQkWarps), kQkWarps * 32,
-                               kQkWarps * p.head_dim * sizeof(float), st>>>(p);
-  return cudaGetLastError();
+  return launch(qk_norm_rope_any_kernel<T>, (units + kQkWarps - 1) / kQkWarps, kQkWarps * 32,
+                kQkWarps * p.head_dim * sizeof(float), st, p);
 }
 
 // ---- quantised writes and reads ------------------------------------------------------------------
 //
 // A group of G values: offset m = f16(min), scale s = f16((max - min) / 15), codes
 // clamp(rint((x - m) / s), 0, 15) with the true quotient rounded to the nearest, ties to even.  The
-// quotient in f32 is off by under 2e-6 (two roundings of 2^-24 of at most 15.01), so only one that
-// close to a tie is settled in 64 bits; the two 64-bit operations a group that make s round right
-// are 1/64 of the work.  8 values a lane: one 16-byte load (f16, bf16) or two (f32), one 32-bit
-// store of codes; a group is 8 or 16 lanes.
+// quotient is taken as (x - m) * (1 / s) in f32: three roundings, off by at most 3 * 2^-24 * 15.01 <
+// 3e-6; a thread that holds one within 8e-6 of a tie settles its 8 codes in 64 bits.  (IEEE divisions
+// instead of the product: 43 us for 8192 tokens of 8 heads of 128 in f32.)  8 values a lane: one
+// 16-byte load (f16, bf16) or two (f32), one 32-bit store of codes; a group is 8 or 16 lanes.  A
+// group of lanes takes HB heads of a token's keys or values, their loads in flight at once: bound
+// by HBM.
 constexpr int kKv4Lane = 8;
 
-__device__ __forceinline__ int kv4_code(float x, float m, float s) {
-  const float q = __fdiv_rn(x - m, s);
-  float c = rintf(q);
-  if (fabsf(fabsf(q - c) - 0.5f) < 4e-6f) c = (float)rint(((double)x - (double)m) / (double)s);
-  return (int)fminf(fmaxf(c, 0.f), 15.f);
+struct Kv4Lane {
+  int l, head, which, token;  // lane of the row, first head, 0 keys 1 values
+};
+template <int HB>
+__device__ __forceinline__ Kv4Lane kv4_lane(const Kv4View& c) {
+  const int log_lanes = c.head_dim == 64 ? 3 : c.head_dim == 128 ? 4 : 5;
+  const long long thread = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const unsigned unit = (unsigned)(thread >> log_lanes);  // (token, keys or values, heads): below 2^32
+  const unsigned parts = (unsigned)(c.kv_heads + HB - 1) / HB, pair = unit / parts;
+  return {(int)(thread & ((1 << log_lanes) - 1)), (int)(unit - pair * parts) * HB, (int)(pair & 1), (int)(pair >> 1)};
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4View c, const T* __restrict__ k,
-                                                         const T* __restrict__ v,
-                                                         const int* __restrict__ slots, int tokens,
-                                                         long long k_stride, long long v_stride, int vec) {
-  const int lanes = c.head_dim / kKv4Lane;  // 8, 16 or 32 lanes a row
-  const long long thread = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int l = (int)(thread % lanes);
-  long long unit = thread / lanes;  // (token, keys or values, head)
-  const int head = (int)(unit % c.kv_heads);
-  unit /= c.kv_heads;
-  const bool values = unit & 1;
-  const long long token = unit >> 1;
-  const int slot = token < tokens ? slots[token] : -1;
-  const long long row = kv4_slot_row(c, slot, head);
-  float x[kKv4Lane];
-#pragma unroll
-  for (int e = 0; e < kKv4Lane; ++e) x[e] = 0.f;
-  if (row >= 0)
-    load_f32<T, kKv4Lane>((values ? v + token * v_stride : k + token * k_stride) + head * c.head_dim +
-                              l * kKv4Lane,
-                          vec, x);
-  // min and max pass over a NaN, and an infinity has none of the two: 0 * x is 0 or NaN, and its
-  // sum makes the group's offset and scale NaN wherever a value is not finite
-  float lo = x[0], hi = x[0], odd = 0.f;
-#pragma unroll
-  for (int e = 0; e < kKv4Lane; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    odd = fmaf(x[e], 0.f, odd);
-  }
-  for (int off = c.group / kKv4Lane / 2; off > 0; off >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-    odd += __shfl_xor_sync(0xffffffffu, odd, off);
-  }
-  if (row < 0) return;
-  // finite values past f16 saturate
-  const float range = (float)(((double)hi - (double)lo) / 15.0);
-  const __half hs = __float2half_rn(fminf(range, 65504.f) + odd);
-  const __half hm = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f) + odd);
-  const float s = __half2float(hs), m = __half2float(hm);
-  uint32_t word = 0;
-  if (s > 0.f) {
-#pragma unroll
-    for (int e = 0; e < kKv4Lane; ++e) word |= (uint32_t)kv4_code(x[e], m, s) << (4 * e);
-  }
-  uint8_t* codes = values ? c.v_codes : c.k_codes;
-  uint32_t* scales = values ? c.v_scales : c.k_scales;
-  *reinterpret_cast<uint32_t*>(codes + row * (c.head_dim / 2) + l * (kKv4Lane / 2)) = word;
-  const int lane_of_group = c.group / kKv4Lane;
-  if (l % lane_of_group == 0)
-    scales[row * (c.head_dim / c.group) + l / lane_of_group] =
-        (uint32_t)__half_as_ushort(hs) | (uint32_t)__half_as_ushort(hm) << 16;
+// The lesser and the greater; NaN if one is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4View c, T* __restrict__ k, T* __restrict__ v,
-                                                         const int* __restrict__ slots, int tokens,
-                                                         long long k_stride, long long v_stride, int vec) {
-  const int lanes = c.head_dim / kKv4Lane;
-  const long long thread = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int l = (int)(thread % lanes);
-  long long unit = thread / lanes;
-  const int head = (int)(unit % c.kv_heads);
-  unit /= c.kv_heads;
-  const bool values = unit & 1;
-  const long long token = unit >> 1;
-  if (token >= tokens) return;
-  const long long row = kv4_slot_row(c, slots[token], head);
-  if (row < 0) return;
-  const uint8_t* codes = values ? c.v_codes : c.k_codes;
-  const uint32_t* scales = values ? c.v_scales : c.k_scales;
-  const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + row * (c.head_dim / 2) + l * (kKv4Lane / 2));
-  const uint32_t pair = scales[row * (c.head_dim / c.group) + l * kKv4Lane / c.group];
-  const float s = __half2float(__ushort_as_half((unsigned short)pair));
-  const float m = __half2float(__ushort_as_half((unsigned short)(pair >> 16)));
-  float x[kKv4Lane];
+template <class T, int HB>
+__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4View c, const T* k, const T* v, const int* slots,
+                                                         int tokens, long long k_stride, long long v_stride, int vec) {
+  after_previous();
+  const Kv4Lane at = kv4_lane<HB>(c);
+  const int slot = at.token < tokens ? slots[at.token] : -1;
+  const bool on = kv4_slot_row(c, slot, 0) >= 0;
+  const T* src = (at.which ? v + at.token * v_stride : k + at.token * k_stride) + at.l * kKv4Lane;
+  uint8_t* codes = at.which ? c.v_codes : c.k_codes;
+  uint32_t* scales = at.which ? c.v_scales : c.k_scales;
+  float x[HB][kKv4Lane];
 #pragma unroll
-  for (int e = 0; e < kKv4Lane; ++e) x[e] = fmaf((float)(word >> (4 * e) & 15u), s, m);
-  store_f32<T, kKv4Lane>((values ? v + token * v_stride : k + token * k_stride) + head * c.head_dim +
-                             l * kKv4Lane,
-                         vec, x);
+  for (int i = 0; i < HB; ++i) {
+#pragma unroll
+    for (int e = 0; e < kKv4Lane; ++e) x[i][e] = 0.f;
+    if (on && at.head + i < c.kv_heads)
+      load_f32<T, kKv4Lane>(src + (long long)(at.head + i) * c.head_dim, vec, x[i]);
+  }
+  const int group_lanes = c.group / kKv4Lane;
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    float lo = x[i][0], hi = x[i][0];
+#pragma unroll
+    for (int e = 1; e < kKv4Lane; ++e) {
+      lo = min_nan(lo, x[i][e]);
+      hi = max_nan(hi, x[i][e]);
+    }
+    for (int off = group_lanes / 2; off > 0; off >>= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+    }
+    if (!on || at.head + i >= c.kv_heads) continue;
+    const float odd = lo * 0.f + hi * 0.f;  // NaN when a value is not finite, else 0
+    // (max - min) / 15 rounded to f16, finite values past it saturating: in f32 when 2^-21 on either
+    // side round alike (two roundings of 2^-24), else in 64 bits
+    const float range = (hi - lo) * (1.f / 15.f);
+    __half hs = __float2half_rn(fminf(range * (1.f + 4.8e-7f), 65504.f) + odd);
+    if (__half_as_ushort(hs) != __half_as_ushort(__float2half_rn(fminf(range * (1.f - 4.8e-7f), 65504.f) + odd)))
+      hs = __float2half_rn(fminf((float)(((double)hi - (double)lo) / 15.0), 65504.f) + odd);
+    const __half hm = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f) + odd);
+    const float s = __half2float(hs), m = __half2float(hm);
+    uint32_t word = 0;
+    if (s > 0.f) {
+      const float inv = __frcp_rn(s);
+      constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: an integer in the low bits of a sum with it
+      float off_tie = 0.f;
+#pragma unroll
+      for (int e = kKv4Lane - 1; e >= 0; --e) {
+        const float d = x[i][e] - m;
+        const float t = fmaf(d, inv, kMagic);
+        off_tie = fmaxf(off_tie, fabsf(fmaf(d, inv, kMagic - t)));
+        word = word * 16u + (__float_as_uint(t) - 0x4B400000u);  // 16 * word + code
+      }
+      // near a tie, or a group whose rounded offset or scale leaves its ends past 0 .. 15
+      if (off_tie > 0.5f - 8e-6f || !((lo - m) * inv > -0.499f && (hi - m) * inv < 15.499f)) {
+        word = 0;
+#pragma unroll 1
+        for (int e = kKv4Lane - 1; e >= 0; --e) {
+          float xe = x[i][0];
+#pragma unroll
+          for (int q = 1; q < kKv4Lane; ++q)
+            if (q == e) xe = x[i][q];
+          word = word * 16u + (uint32_t)fmin(fmax(rint(((double)xe - (double)m) / (double)s), 0.0), 15.0);
+        }
+      }
+    }
+    const long long row = kv4_slot_row(c, slot, at.head + i);
+    *reinterpret_cast<uint32_t*>(codes + row * (c.head_dim / 2) + at.l * (kKv4Lane / 2)) = word;
+    if (at.l % group_lanes == 0)
+      scales[row * (c.head_dim / c.group) + at.l / group_lanes] =
+          (uint32_t)__half_as_ushort(hs) | (uint32_t)__half_as_ushort(hm) << 16;
+  }
+}
+
+template <class T, int HB>
+__global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4View c, T* k, T* v, const int* slots, int tokens,
+                                                         long long k_stride, long long v_stride, int vec) {
+  after_previous();
+  const Kv4Lane at = kv4_lane<HB>(c);
+  if (at.token >= tokens) return;
+  const int slot = slots[at.token];
+  if (kv4_slot_row(c, slot, 0) < 0) return;
+  const uint8_t* codes = at.which ? c.v_codes : c.k_codes;
+  const uint32_t* scales = at.which ? c.v_scales : c.k_scales;
+  T* dst = (at.which ? v + at.token * v_stride : k + at.token * k_stride) + at.l * kKv4Lane;
+  uint32_t word[HB], pair[HB];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    const long long row = kv4_slot_row(c, slot, min(at.head + i, c.kv_heads - 1));
+    word[i] = *reinterpret_cast<const uint32_t*>(codes + row * (c.head_dim / 2) + at.l * (kKv4Lane / 2));
+    pair[i] = scales[row * (c.head_dim / c.group) + at.l * kKv4Lane / c.group];
+  }
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    if (at.head + i >= c.kv_heads) break;
+    const float s = __half2float(__ushort_as_half((unsigned short)pair[i]));
+    const float m = __half2float(__ushort_as_half((unsigned short)(pair[i] >> 16)));
+    float x[kKv4Lane];
+#pragma unroll
+    for (int e = 0; e < kKv4Lane; ++e) x[e] = fmaf((float)(word[i] >> (4 * e) & 15u), s, m);
+    store_f32<T, kKv4Lane>(dst + (long long)(at.head + i) * c.head_dim, vec, x);
+  }
 }
 
 template <class T>
@@ -487,35 +670,47 @@ bool rows_vec(const void* k, const void* v, long long k_stride, long long v_stri
          k_stride * (long long)sizeof(T) % 16 == 0 && v_stride * (long long)sizeof(T) % 16 == 0;
 }
 
-unsigned kv4_blocks(const Kv4View& c, int tokens) {
-  return (unsigned)(((long long)tokens * 2 * c.kv_heads * (c.head_dim / kKv4Lane) + 255) / 256);
+long long kv4_blocks(const Kv4View& c, int tokens, int hb) {
+  return ((long long)tokens * 2 * ((c.kv_heads + hb - 1) / hb) * (c.head_dim / kKv4Lane) + 255) / 256;
+}
+// one head a group until every SM has its 2048 threads twice over
+constexpr int kKv4Heads = 4;
+bool kv4_batched(const Kv4View& c, int tokens, int sm_count) {
+  return kv4_blocks(c, tokens, kKv4Heads) >= 16ll * sm_count;
 }
 
 template <class T>
 cudaError_t append(const Kv4View& c, const void* k, const void* v, const int* slots, int tokens,
-                   long long k_stride, long long v_stride, cudaStream_t st) {
-  kv4_append_kernel<T><<<kv4_blocks(c, tokens), 256, 0, st>>>(
-      c, static_cast<const T*>(k), static_cast<const T*>(v), slots, tokens, k_stride, v_stride,
-      rows_vec<T>(k, v, k_stride, v_stride));
-  return cudaGetLastError();
+                   long long k_stride, long long v_stride, int sm_count, cudaStream_t st) {
+  const int vec = rows_vec<T>(k, v, k_stride, v_stride);
+  const T *kt = static_cast<const T*>(k), *vt = static_cast<const T*>(v);
+  if (kv4_batched(c, tokens, sm_count))
+    return launch(kv4_append_kernel<T, kKv4Heads>, kv4_blocks(c, tokens, kKv4Heads), 256, 0, st, c, kt, vt, slots,
+                  tokens, k_stride, v_stride, vec);
+  return launch(kv4_append_kernel<T, 1>, kv4_blocks(c, tokens, 1), 256, 0, st, c, kt, vt, slots, tokens, k_stride,
+                v_stride, vec);
 }
 
 template <class T>
 cudaError_t gather(const Kv4View& c, void* k, void* v, const int* slots, int tokens, long long k_stride,
-                   long long v_stride, cudaStream_t st) {
-  kv4_gather_kernel<T><<<kv4_blocks(c, tokens), 256, 0, st>>>(
-      c, static_cast<T*>(k), static_cast<T*>(v), slots, tokens, k_stride, v_stride,
-      rows_vec<T>(k, v, k_stride, v_stride));
-  return cudaGetLastError();
+                   long long v_stride, int sm_count, cudaStream_t st) {
+  const int vec = rows_vec<T>(k, v, k_stride, v_stride);
+  T *kt = static_cast<T*>(k), *vt = static_cast<T*>(v);
+  if (kv4_batched(c, tokens, sm_count))
+    return launch(kv4_gather_kernel<T, kKv4Heads>, kv4_blocks(c, tokens, kKv4Heads), 256, 0, st, c, kt, vt, slots,
+                  tokens, k_stride, v_stride, vec);
+  return launch(kv4_gather_kernel<T, 1>, kv4_blocks(c, tokens, 1), 256, 0, st, c, kt, vt, slots, tokens, k_stride,
+                v_stride, vec);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_slots(const SlotsParams& p, int sm_count, cudaStream_t st) {
-  const long long per = kSlotsThreads * kSlotsTokens;
-  const long long blocks = std::max(1ll, std::min((p.max_tokens + per - 1) / per, (long long)sm_count * 2));
-  paged_slots_kernel<<<(unsigned)blocks, kSlotsThreads, 0, st>>>(p);
-  return cudaGetLastError();
+  // a token a thread while that fills the SMs at most once
+  const bool few = p.max_tokens <= (long long)kSlotsThreads * sm_count;
+  const long long per = kSlotsThreads * (few ? 1 : 4);
+  const long long ctas = std::min((p.max_tokens + per - 1) / per, (long long)sm_count * 4);
+  return launch(few ? paged_slots_kernel<1> : paged_slots_kernel<4>, ctas > 1 ? ctas + 1 : 1, kSlotsThreads, 0, st, p);
 }
 
 cudaError_t launch_qk_norm_rope(const QkNormRopeParams& p, int dtype, int sm_count, cudaStream_t st) {
@@ -527,20 +722,20 @@ cudaError_t launch_qk_norm_rope(const QkNormRopeParams& p, int dtype, int sm_cou
 }
 
 cudaError_t launch_kv4_append(const Kv4View& c, const void* k, const void* v, const int* slots, int tokens,
-                              long long k_stride, long long v_stride, int dtype, cudaStream_t st) {
+                              long long k_stride, long long v_stride, int dtype, int sm_count, cudaStream_t st) {
   switch (dtype) {
-    case kTypeF32: return append<float>(c, k, v, slots, tokens, k_stride, v_stride, st);
-    case kTypeF16: return append<__half>(c, k, v, slots, tokens, k_stride, v_stride, st);
-    default: return append<__nv_bfloat16>(c, k, v, slots, tokens, k_stride, v_stride, st);
+    case kTypeF32: return append<float>(c, k, v, slots, tokens, k_stride, v_stride, sm_count, st);
+    case kTypeF16: return append<__half>(c, k, v, slots, tokens, k_stride, v_stride, sm_count, st);
+    default: return append<__nv_bfloat16>(c, k, v, slots, tokens, k_stride, v_stride, sm_count, st);
   }
 }
 
 cudaError_t launch_kv4_gather(const Kv4View& c, void* k, void* v, const int* slots, int tokens,
-                              long long k_stride, long long v_stride, int dtype, cudaStream_t st) {
+                              long long k_stride, long long v_stride, int dtype, int sm_count, cudaStream_t st) {
   switch (dtype) {
-    case kTypeF32: return gather<float>(c, k, v, slots, tokens, k_stride, v_stride, st);
-    case kTypeF16: return gather<__half>(c, k, v, slots, tokens, k_stride, v_stride, st);
-    default: return gather<__nv_bfloat16>(c, k, v, slots, tokens, k_stride, v_stride, st);
+    case kTypeF32: return gather<float>(c, k, v, slots, tokens, k_stride, v_stride, sm_count, st);
+    case kTypeF16: return gather<__half>(c, k, v, slots, tokens, k_stride, v_stride, sm_count, st);
+    default: return gather<__nv_bfloat16>(c, k, v, slots, tokens, k_stride, v_stride, sm_count, st);
   }
 }
 

@@ -131,9 +131,10 @@ cudaError_t launch_qk_norm_rope(const QkNormRopeParams& p, int dtype, int sm_cou
 // k, v: rows of kv_heads * head_dim values, stride elements apart; slots [tokens].
 cudaError_t launch_kv4_append(const Kv4View& c, const void* k, const void* v, const int* slots,
                               int tokens, long long k_stride, long long v_stride, int dtype,
-                              cudaStream_t st);
+                              int sm_count, cudaStream_t st);
 cudaError_t launch_kv4_gather(const Kv4View& c, void* k, void* v, const int* slots, int tokens,
-                              long long k_stride, long long v_stride, int dtype, cudaStream_t st);
+                              long long k_stride, long long v_stride, int dtype, int sm_count,
+                              cudaStream_t st);
 
 // tk_kv4_attention.cu
 struct Kv4AttentionParams {

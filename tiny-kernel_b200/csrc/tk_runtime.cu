@@ -1423,7 +1423,7 @@ int tk_qk_norm_rope_async(tk_device* d, const void* q, const void* k, const floa
     return fail(TK_ERR_ARG, "head_dim=%u must be even and at most 1024, rot_dim=%u even and within it", head_dim,
                 rot_dim);
   if (q_heads > 65535 || kv_heads > 65535 || q_heads + kv_heads == 0 || max_pos == 0 || max_pos > kMaxCount ||
-      (uint64_t)tokens * (q_heads + kv_heads) > kMaxCount)
+      (uint64_t)tokens * (q_heads + kv_heads) > (1u << 30))
     return fail(TK_ERR_ARG, "%u tokens of %u + %u heads, %u positions are out of range", tokens, q_heads,
                 kv_heads, max_pos);
   QkNormRopeParams p{{q, k}, {q_out, k_out}, {q_weight, k_weight}, {}, {}, {(int)q_heads, (int)kv_heads},
@@ -1470,10 +1470,8 @@ int check_rows(const tk_kv4_cache* cache, Kv4View* view, const void* k, const vo
   if ((st = check_dtype(dtype)) != TK_OK) return st;
   if (!k || !v || !slots) return fail(TK_ERR_ARG, "NULL argument");
   if (!aligned_for(k, dtype) || !aligned_for(v, dtype)) return fail(TK_ERR_ARG, "k or v is not aligned to its type");
-  // one thread per 8 values: the grid's limit
-  if ((uint64_t)tokens * cache->kv_heads * cache->head_dim > (1ull << 38))
+  if ((uint64_t)tokens * cache->kv_heads > (1u << 30))
     return fail(TK_ERR_ARG, "%u tokens of %u heads are too many for one call", tokens, cache->kv_heads);
-  if (tokens > kMaxCount) return fail(TK_ERR_ARG, "%u tokens are too many for one call", tokens);
   const uint64_t width = (uint64_t)cache->kv_heads * cache->head_dim;
   if ((st = check_stride("k", k_stride, width, ks)) != TK_OK) return st;
   return check_stride("v", v_stride, width, vs);
@@ -1491,7 +1489,8 @@ int tk_kv4_append_async(tk_device* d, const tk_kv4_cache* cache, const void* k, 
   DeviceScope scope;
   if ((st = scope.enter(d)) != TK_OK) return st;
   if (tokens == 0) return TK_OK;
-  TK_LAUNCH(d, launch_kv4_append(view, k, v, slots, (int)tokens, ks, vs, dtype, pick_stream(d, stream)));
+  TK_LAUNCH(d, launch_kv4_append(view, k, v, slots, (int)tokens, ks, vs, dtype, d->sm_count,
+                                 pick_stream(d, stream)));
   return TK_OK;
 }
 
@@ -1512,7 +1511,8 @@ int tk_kv4_gather_async(tk_device* d, const tk_kv4_cache* cache, const int32_t* 
   DeviceScope scope;
   if ((st = scope.enter(d)) != TK_OK) return st;
   if (tokens == 0) return TK_OK;
-  TK_LAUNCH(d, launch_kv4_gather(view, k, v, slots, (int)tokens, ks, vs, dtype, pick_stream(d, stream)));
+  TK_LAUNCH(d, launch_kv4_gather(view, k, v, slots, (int)tokens, ks, vs, dtype, d->sm_count,
+                                 pick_stream(d, stream)));
   return TK_OK;
 }
 

@@ -13,12 +13,13 @@ from ._lib import Int4MatrixC, Kv4CacheC, check
 
 
 def _ptr(v) -> int:
-    if v is None:
-        return None
+    if v is None or type(v) is int:
+        return v
+    at = getattr(v, "data_ptr", None)
+    if at is not None:
+        return at()
     if hasattr(v, "ptr"):
         return v.ptr
-    if hasattr(v, "data_ptr"):
-        return v.data_ptr()
     return int(v)
 
 
