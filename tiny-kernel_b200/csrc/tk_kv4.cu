@@ -19,12 +19,12 @@ __device__ __forceinline__ void after_previous() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 template <class... P, class... A>
-cudaError_t launch(void (*kernel)(P...), long long blocks, int threads, size_t smem, cudaStream_t st, A... args) {
+cudaError_t launch(void (*kernel)(P...), dim3 blocks, int threads, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.gridDim = blocks;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -48,9 +48,18 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // E consecutive elements as f32.  vec: the address is on a 16-byte boundary (E elements are 16 or
-// 32 bytes).
+// 32 bytes), 2: on a 32-byte boundary.
 template <class T, int E>
-__device__ __forceinline__ void load_f32(const T* src, bool vec, float (&v)[E]) {
+__device__ __forceinline__ void load_f32(const T* src, int vec, float (&v)[E]) {
+  if constexpr (E * sizeof(T) == 32) {
+    if (vec == 2) {
+      static_assert(sizeof(T) == 4, "");
+      asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                   : "l"(src));
+      return;
+    }
+  }
   if (vec) {
     constexpr int W = E * (int)sizeof(T) / 16;
     uint4 raw[W];
@@ -67,7 +76,15 @@ __device__ __forceinline__ void load_f32(const T* src, bool vec, float (&v)[E]) 
 
 // Rounds once, to the nearest of T.
 template <class T, int E>
-__device__ __forceinline__ void store_f32(T* dst, bool vec, const float (&v)[E]) {
+__device__ __forceinline__ void store_f32(T* dst, int vec, const float (&v)[E]) {
+  if constexpr (E * sizeof(T) == 32) {
+    if (vec == 2) {
+      asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                   "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                   : "memory");
+      return;
+    }
+  }
   if (vec) {
     constexpr int W = E * (int)sizeof(T) / 16;
     uint4 raw[W];
@@ -487,7 +504,7 @@ __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_any_kernel(QkNormR
 }
 
 template <class T, int E, int LPH>
-cudaError_t qk_launch_vec(const QkNormRopeParams& p, bool vec_in, bool vec_out, int sm_count, cudaStream_t st) {
+cudaError_t qk_launch_vec(const QkNormRopeParams& p, int vec_in, int vec_out, int sm_count, cudaStream_t st) {
   const int vec_turn = (reinterpret_cast<uintptr_t>(p.cos_cache) | reinterpret_cast<uintptr_t>(p.sin_cache)) % 8 == 0 &&
                        p.rot_dim / 2 % 2 == 0;
   auto blocks = [&](int hb) {
@@ -497,20 +514,21 @@ cudaError_t qk_launch_vec(const QkNormRopeParams& p, bool vec_in, bool vec_out, 
   // one head a group until every SM has its 2048 threads twice over
   if (blocks(4) < 16ll * sm_count)
     return launch(halves ? qk_norm_rope_kernel<T, E, LPH, 1, true> : qk_norm_rope_kernel<T, E, LPH, 1, false>,
-                  blocks(1), 256, 0, st, p, (int)vec_in, (int)vec_out, vec_turn);
-  return launch(halves ? qk_norm_rope_kernel<T, E, LPH, 4, true> : qk_norm_rope_kernel<T, E, LPH, 4, false>, blocks(4),
-                256, 0, st, p, (int)vec_in, (int)vec_out, vec_turn);
+                  dim3((unsigned)blocks(1)), 256, 0, st, p, vec_in, vec_out, vec_turn);
+  return launch(halves ? qk_norm_rope_kernel<T, E, LPH, 4, true> : qk_norm_rope_kernel<T, E, LPH, 4, false>,
+                dim3((unsigned)blocks(4)), 256, 0, st, p, vec_in, vec_out, vec_turn);
 }
 
 template <class T>
 cudaError_t qk_launch(const QkNormRopeParams& p, int sm_count, cudaStream_t st) {
   const int size = (int)sizeof(T);
-  bool vec_in = true, vec_out = true;
+  uintptr_t in = 0, out = 0;
   for (int i = 0; i < 2; ++i) {
     if (p.heads[i] == 0) continue;
-    vec_in = vec_in && reinterpret_cast<uintptr_t>(p.x[i]) % 16 == 0 && p.in_stride[i] * size % 16 == 0;
-    vec_out = vec_out && reinterpret_cast<uintptr_t>(p.out[i]) % 16 == 0 && p.out_stride[i] * size % 16 == 0;
+    in |= reinterpret_cast<uintptr_t>(p.x[i]) | (uintptr_t)(p.in_stride[i] * size);
+    out |= reinterpret_cast<uintptr_t>(p.out[i]) | (uintptr_t)(p.out_stride[i] * size);
   }
+  const int vec_in = in % 32 == 0 ? 2 : in % 16 == 0, vec_out = out % 32 == 0 ? 2 : out % 16 == 0;
   constexpr int E = 16 / (int)sizeof(T);  // 16 bytes a lane
   const int half = p.rot_dim / 2;
   const int e = p.head_dim == 256 ? 8 : E;
@@ -520,7 +538,7 @@ cudaError_t qk_launch(const QkNormRopeParams& p, int sm_count, cudaStream_t st) 
     if (p.head_dim == 256) return qk_launch_vec<T, 8, 32>(p, vec_in, vec_out, sm_count, st);
   }
   const long long units = (long long)p.tokens * (p.heads[0] + p.heads[1]);
-  return launch(qk_norm_rope_any_kernel<T>, (units + kQkWarps - 1) / kQkWarps, kQkWarps * 32,
+  return launch(qk_norm_rope_any_kernel<T>, dim3((unsigned)((units + kQkWarps - 1) / kQkWarps)), kQkWarps * 32,
                 kQkWarps * p.head_dim * sizeof(float), st, p);
 }
 
@@ -536,16 +554,16 @@ cudaError_t qk_launch(const QkNormRopeParams& p, int sm_count, cudaStream_t st) 
 // by HBM.
 constexpr int kKv4Lane = 8;
 
+// A CTA's threads are rows of consecutive tokens; blockIdx.y names the heads, of keys or of values.
 struct Kv4Lane {
   int l, head, which, token;  // lane of the row, first head, 0 keys 1 values
 };
 template <int HB>
 __device__ __forceinline__ Kv4Lane kv4_lane(const Kv4View& c) {
   const int log_lanes = c.head_dim == 64 ? 3 : c.head_dim == 128 ? 4 : 5;
-  const long long thread = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const unsigned unit = (unsigned)(thread >> log_lanes);  // (token, keys or values, heads): below 2^32
-  const unsigned parts = (unsigned)(c.kv_heads + HB - 1) / HB, pair = unit / parts;
-  return {(int)(thread & ((1 << log_lanes) - 1)), (int)(unit - pair * parts) * HB, (int)(pair & 1), (int)(pair >> 1)};
+  const int which = blockIdx.y & 1, head = (int)(blockIdx.y >> 1) * HB;
+  return {(int)threadIdx.x & ((1 << log_lanes) - 1), head, which,
+          (int)(blockIdx.x << (8 - log_lanes)) + (int)(threadIdx.x >> log_lanes)};
 }
 
 // The lesser and the greater; NaN if one is.
@@ -566,8 +584,9 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4View c, const T* k, 
   after_previous();
   const Kv4Lane at = kv4_lane<HB>(c);
   const int slot = at.token < tokens ? slots[at.token] : -1;
-  const bool on = kv4_slot_row(c, slot, 0) >= 0;
-  const T* src = (at.which ? v + at.token * v_stride : k + at.token * k_stride) + at.l * kKv4Lane;
+  const long long row0 = kv4_slot_row(c, slot, at.head);
+  const bool on = row0 >= 0;
+  const T* src = (at.which ? v + at.token * v_stride : k + at.token * k_stride) + at.head * c.head_dim + at.l * kKv4Lane;
   uint8_t* codes = at.which ? c.v_codes : c.k_codes;
   uint32_t* scales = at.which ? c.v_scales : c.k_scales;
   float x[HB][kKv4Lane];
@@ -576,9 +595,10 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4View c, const T* k, 
 #pragma unroll
     for (int e = 0; e < kKv4Lane; ++e) x[i][e] = 0.f;
     if (on && at.head + i < c.kv_heads)
-      load_f32<T, kKv4Lane>(src + (long long)(at.head + i) * c.head_dim, vec, x[i]);
+      load_f32<T, kKv4Lane>(src + i * c.head_dim, vec, x[i]);
   }
-  const int group_lanes = c.group / kKv4Lane;
+  const int log_group = c.group == 64 ? 3 : 4;  // lanes of a group
+  const int log_row = c.head_dim == 64 ? 3 : c.head_dim == 128 ? 4 : 5;
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
     float lo = x[i][0], hi = x[i][0];
@@ -587,7 +607,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4View c, const T* k, 
       lo = min_nan(lo, x[i][e]);
       hi = max_nan(hi, x[i][e]);
     }
-    for (int off = group_lanes / 2; off > 0; off >>= 1) {
+    for (int off = 1 << (log_group - 1); off > 0; off >>= 1) {
       lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
       hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
     }
@@ -626,10 +646,10 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4View c, const T* k, 
         }
       }
     }
-    const long long row = kv4_slot_row(c, slot, at.head + i);
-    *reinterpret_cast<uint32_t*>(codes + row * (c.head_dim / 2) + at.l * (kKv4Lane / 2)) = word;
-    if (at.l % group_lanes == 0)
-      scales[row * (c.head_dim / c.group) + at.l / group_lanes] =
+    const long long row = row0 + ((long long)i << c.shift);
+    reinterpret_cast<uint32_t*>(codes)[(row << log_row) + at.l] = word;
+    if ((at.l & ((1 << log_group) - 1)) == 0)
+      scales[(row << (log_row - log_group)) + (at.l >> log_group)] =
           (uint32_t)__half_as_ushort(hs) | (uint32_t)__half_as_ushort(hm) << 16;
   }
 }
@@ -640,17 +660,18 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4View c, T* k, T* v, 
   after_previous();
   const Kv4Lane at = kv4_lane<HB>(c);
   if (at.token >= tokens) return;
-  const int slot = slots[at.token];
-  if (kv4_slot_row(c, slot, 0) < 0) return;
+  const long long row0 = kv4_slot_row(c, slots[at.token], at.head);
+  if (row0 < 0) return;
   const uint8_t* codes = at.which ? c.v_codes : c.k_codes;
   const uint32_t* scales = at.which ? c.v_scales : c.k_scales;
-  T* dst = (at.which ? v + at.token * v_stride : k + at.token * k_stride) + at.l * kKv4Lane;
+  T* dst = (at.which ? v + at.token * v_stride : k + at.token * k_stride) + at.head * c.head_dim + at.l * kKv4Lane;
+  const int log_group = c.group == 64 ? 3 : 4, log_row = c.head_dim == 64 ? 3 : c.head_dim == 128 ? 4 : 5;
   uint32_t word[HB], pair[HB];
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
-    const long long row = kv4_slot_row(c, slot, min(at.head + i, c.kv_heads - 1));
-    word[i] = *reinterpret_cast<const uint32_t*>(codes + row * (c.head_dim / 2) + at.l * (kKv4Lane / 2));
-    pair[i] = scales[row * (c.head_dim / c.group) + at.l * kKv4Lane / c.group];
+    const long long row = row0 + ((long long)(min(at.head + i, c.kv_heads - 1) - at.head) << c.shift);
+    word[i] = reinterpret_cast<const uint32_t*>(codes)[(row << log_row) + at.l];
+    pair[i] = scales[(row << (log_row - log_group)) + (at.l >> log_group)];
   }
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
@@ -659,24 +680,33 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4View c, T* k, T* v, 
     const float m = __half2float(__ushort_as_half((unsigned short)(pair[i] >> 16)));
     float x[kKv4Lane];
 #pragma unroll
-    for (int e = 0; e < kKv4Lane; ++e) x[e] = fmaf((float)(word[i] >> (4 * e) & 15u), s, m);
-    store_f32<T, kKv4Lane>(dst + (long long)(at.head + i) * c.head_dim, vec, x);
+    for (int e = 0; e < kKv4Lane; ++e) {
+      // the nibble in the low bits of 1.5 * 2^23, read as f32: faster than a conversion
+      const float code = __uint_as_float((word[i] >> (4 * e) & 15u) | 0x4B400000u) - 12582912.f;
+      x[e] = fmaf(code, s, m);
+    }
+    store_f32<T, kKv4Lane>(dst + i * c.head_dim, vec, x);
   }
 }
 
+// 2: all rows on 32-byte boundaries, 1: on 16-byte boundaries.
 template <class T>
-bool rows_vec(const void* k, const void* v, long long k_stride, long long v_stride) {
-  return (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 &&
-         k_stride * (long long)sizeof(T) % 16 == 0 && v_stride * (long long)sizeof(T) % 16 == 0;
+int rows_vec(const void* k, const void* v, long long k_stride, long long v_stride) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                         (uintptr_t)(k_stride * (long long)sizeof(T)) | (uintptr_t)(v_stride * (long long)sizeof(T));
+  return bits % 32 == 0 ? 2 : bits % 16 == 0 ? 1 : 0;
 }
 
-long long kv4_blocks(const Kv4View& c, int tokens, int hb) {
-  return ((long long)tokens * 2 * ((c.kv_heads + hb - 1) / hb) * (c.head_dim / kKv4Lane) + 255) / 256;
+// Grid of HB heads a group: rows of 256 threads, (heads, keys and values).
+dim3 kv4_grid(const Kv4View& c, int tokens, int hb) {
+  const int rows = 256 / (c.head_dim / kKv4Lane);
+  return dim3((unsigned)((tokens + (long long)rows - 1) / rows), 2u * (unsigned)((c.kv_heads + hb - 1) / hb));
 }
-// one head a group until every SM has its 2048 threads twice over
+// one head a group until every SM has its 2048 threads
 constexpr int kKv4Heads = 4;
 bool kv4_batched(const Kv4View& c, int tokens, int sm_count) {
-  return kv4_blocks(c, tokens, kKv4Heads) >= 16ll * sm_count;
+  const dim3 g = kv4_grid(c, tokens, kKv4Heads);
+  return (long long)g.x * g.y >= 8ll * sm_count;
 }
 
 template <class T>
@@ -685,9 +715,9 @@ cudaError_t append(const Kv4View& c, const void* k, const void* v, const int* sl
   const int vec = rows_vec<T>(k, v, k_stride, v_stride);
   const T *kt = static_cast<const T*>(k), *vt = static_cast<const T*>(v);
   if (kv4_batched(c, tokens, sm_count))
-    return launch(kv4_append_kernel<T, kKv4Heads>, kv4_blocks(c, tokens, kKv4Heads), 256, 0, st, c, kt, vt, slots,
+    return launch(kv4_append_kernel<T, kKv4Heads>, kv4_grid(c, tokens, kKv4Heads), 256, 0, st, c, kt, vt, slots,
                   tokens, k_stride, v_stride, vec);
-  return launch(kv4_append_kernel<T, 1>, kv4_blocks(c, tokens, 1), 256, 0, st, c, kt, vt, slots, tokens, k_stride,
+  return launch(kv4_append_kernel<T, 1>, kv4_grid(c, tokens, 1), 256, 0, st, c, kt, vt, slots, tokens, k_stride,
                 v_stride, vec);
 }
 
@@ -697,9 +727,9 @@ cudaError_t gather(const Kv4View& c, void* k, void* v, const int* slots, int tok
   const int vec = rows_vec<T>(k, v, k_stride, v_stride);
   T *kt = static_cast<T*>(k), *vt = static_cast<T*>(v);
   if (kv4_batched(c, tokens, sm_count))
-    return launch(kv4_gather_kernel<T, kKv4Heads>, kv4_blocks(c, tokens, kKv4Heads), 256, 0, st, c, kt, vt, slots,
+    return launch(kv4_gather_kernel<T, kKv4Heads>, kv4_grid(c, tokens, kKv4Heads), 256, 0, st, c, kt, vt, slots,
                   tokens, k_stride, v_stride, vec);
-  return launch(kv4_gather_kernel<T, 1>, kv4_blocks(c, tokens, 1), 256, 0, st, c, kt, vt, slots, tokens, k_stride,
+  return launch(kv4_gather_kernel<T, 1>, kv4_grid(c, tokens, 1), 256, 0, st, c, kt, vt, slots, tokens, k_stride,
                 v_stride, vec);
 }
 
@@ -710,7 +740,7 @@ cudaError_t launch_paged_slots(const SlotsParams& p, int sm_count, cudaStream_t 
   const bool few = p.max_tokens <= (long long)kSlotsThreads * sm_count;
   const long long per = kSlotsThreads * (few ? 1 : 4);
   const long long ctas = std::min((p.max_tokens + per - 1) / per, (long long)sm_count * 4);
-  return launch(few ? paged_slots_kernel<1> : paged_slots_kernel<4>, ctas > 1 ? ctas + 1 : 1, kSlotsThreads, 0, st, p);
+  return launch(few ? paged_slots_kernel<1> : paged_slots_kernel<4>, dim3((unsigned)(ctas > 1 ? ctas + 1 : 1)), kSlotsThreads, 0, st, p);
 }
 
 cudaError_t launch_qk_norm_rope(const QkNormRopeParams& p, int dtype, int sm_count, cudaStream_t st) {

@@ -1348,7 +1348,7 @@ int check_cache(const tk_kv4_cache* c, Kv4View* view) {
     return fail(TK_ERR_ARG, "head_dim %u is none of 64, 128, 256", c->head_dim);
   if ((c->group_size != 64 && c->group_size != 128) || c->group_size > c->head_dim)
     return fail(TK_ERR_ARG, "group_size %u is not 64 or 128 within head_dim %u", c->group_size, c->head_dim);
-  if (c->kv_heads == 0 || c->kv_heads > 65535 || c->num_blocks == 0 || (uint64_t)c->num_blocks * bs > kMaxCount)
+  if (c->kv_heads == 0 || c->kv_heads > 4096 || c->num_blocks == 0 || (uint64_t)c->num_blocks * bs > kMaxCount)
     return fail(TK_ERR_ARG, "cache of %u blocks of %u tokens, %u heads is out of range", c->num_blocks, bs,
                 c->kv_heads);
   int shift = 0;
