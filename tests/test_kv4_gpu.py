@@ -119,6 +119,12 @@ QK = [
     (9, 4, 2, 128, 36, False, True, 0, 0),    # half of it no whole load
     (5, 4, 2, 128, 128, False, True, 1, 1),   # rows on no 16-byte boundary
     (300, 9, 3, 64, 64, False, False, 8, 0),
+    (4, 5, 2, 48, 48, False, True, 8, 0),     # lanes that hold nothing
+    (3, 5, 2, 96, 32, False, True, 0, 0),
+    (5, 2, 2, 160, 20, True, True, 0, 0),     # a lane's values turned in part
+    (2, 3, 2, 256, 256, False, True, 4, 4),
+    (700, 18, 3, 128, 128, False, True, 0, 0),  # groups of heads, the last not full
+    (800, 9, 6, 112, 56, True, False, 0, 0),
 ]
 
 

@@ -349,16 +349,23 @@ __device__ __forceinline__ QkRow qk_row(const QkNormRopeParams& p, int head) {
   return head < p.heads[0] ? QkRow{0, head} : QkRow{1, head - p.heads[0]};
 }
 
-// LPH lanes hold a head, E values each (16 or 32 bytes); a group of lanes takes HB queries or keys of
-// a token, so that weights and angles are read once and HB loads are in flight: bound by HBM.
-// HALVES (the whole head turns, by halves): a lane holds E/2 consecutive values of each half and so
-// both values of a pair, and half as many angles.  Otherwise E consecutive values; the pair of one lies
-// rot_dim / 2 values on, a multiple of E: the same place in another lane.
-template <class T, int E, int LPH, int HB, bool HALVES>
+// Up to LPH lanes hold a head, E values each (16 or 32 bytes); a group of LPH lanes takes HB queries or
+// keys of a token, so that weights and angles are read once and HB loads are in flight: bound by HBM.
+//   kHalves (the whole head turns, by halves): a lane holds E/2 consecutive values of each half, and so
+//     both values of a pair;
+//   kPairs (interleaved): E consecutive values;
+//   kPart (a part of the head turns, by halves): E consecutive values; the pair of one lies rot_dim / 2
+//     values on, a multiple of E: the same place in another lane.
+// EXACT: head_dim is E * LPH, and else less.
+enum QkMode { kHalves, kPairs, kPart };
+
+template <class T, int E, int LPH, int HB, int MODE, bool EXACT>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, int vec_in, int vec_out, int vec_turn) {
-  constexpr int H = E / 2, D = E * LPH;
+  constexpr int H = E / 2;
   after_previous();
+  const int D = EXACT ? E * LPH : p.head_dim;
   const int lane = threadIdx.x & 31, l = lane % LPH;
+  const bool holds = EXACT || l * E < D;
   const int q_parts = (p.heads[0] + HB - 1) / HB, parts = q_parts + (p.heads[1] + HB - 1) / HB;
   const unsigned group = (unsigned)(((long long)blockIdx.x * blockDim.x + threadIdx.x) / LPH);  // below 2^31
   const int token = (int)(group / (unsigned)parts), part = (int)(group - (unsigned)token * parts);
@@ -374,8 +381,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, i
   for (int i = 0; i < HB; ++i) {
 #pragma unroll
     for (int e = 0; e < E; ++e) y[i][e] = 0.f;
-    if (on && h0 + i < heads) {
-      if constexpr (HALVES)
+    if (on && holds && h0 + i < heads) {
+      if constexpr (MODE == kHalves)
         load_halves<T, E>(x + i * D + l * H, D / 2, vec_in, y[i]);
       else
         load_f32<T, E>(x + i * D + l * E, vec_in, y[i]);
@@ -383,17 +390,16 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, i
   }
 
   // what the lane's values are turned by (1, 0 past rot_dim), and the lane of their pairs
-  constexpr int A = HALVES ? H : E;
+  constexpr int A = MODE == kPart ? E : H;
   float c[A], s[A];
   int src = lane;
-  const bool turned = on && (HALVES || l * E < p.rot_dim);
 #pragma unroll
   for (int e = 0; e < A; ++e) c[e] = 1.f, s[e] = 0.f;
-  if (turned) {
-    const int j0 = HALVES ? l * H : (p.interleaved ? l * E / 2 : (l * E < half ? l * E : l * E - half));
+  if (on && holds && (MODE == kHalves || l * E < p.rot_dim)) {
+    const int j0 = MODE != kPart ? l * H : l * E < half ? l * E : l * E - half;
     const float* cp = p.cos_cache + (size_t)pos * half + j0;
     const float* sp = p.sin_cache + (size_t)pos * half + j0;
-    if (vec_turn && !p.interleaved) {  // on a boundary of the A values, by pairs at least
+    if (vec_turn && (MODE != kPairs || l * E + E <= p.rot_dim)) {  // by pairs on 8-byte boundaries
 #pragma unroll
       for (int e = 0; e < A; e += 2) {
         const float2 cv = __ldg(reinterpret_cast<const float2*>(cp + e)), sv = __ldg(reinterpret_cast<const float2*>(sp + e));
@@ -403,22 +409,23 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, i
     } else {
 #pragma unroll
       for (int e = 0; e < A; ++e)
-        if (HALVES || l * E + e < p.rot_dim) {
-          c[e] = __ldg(cp + (p.interleaved ? e / 2 : e));
-          s[e] = __ldg(sp + (p.interleaved ? e / 2 : e));
+        if (j0 + e < half) {
+          c[e] = __ldg(cp + e);
+          s[e] = __ldg(sp + e);
         }
     }
-    if constexpr (!HALVES) {
+    if constexpr (MODE == kPart) {
 #pragma unroll
       for (int e = 0; e < A; ++e)
-        if (p.interleaved ? (e & 1) == 0 : l * E < half) s[e] = -s[e];
-      if (!p.interleaved) src = l * E < half ? lane + half / E : lane - half / E;
+        if (l * E < half) s[e] = -s[e];
+      src = l * E < half ? lane + half / E : lane - half / E;
     }
   }
   const float* wp = p.weight[which];
   float w[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) w[e] = wp ? __ldg(wp + (HALVES ? (e / H) * (D / 2) + l * H + e % H : l * E + e)) : 1.f;
+  for (int e = 0; e < E; ++e)
+    w[e] = wp && holds ? __ldg(wp + (MODE == kHalves ? (e / H) * (D / 2) + l * H + e % H : l * E + e)) : 1.f;
 
   T* out = static_cast<T*>(p.out[which]) + token * p.out_stride[which] + (long long)h0 * D;
 #pragma unroll
@@ -436,22 +443,24 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, i
       }
     }
     float z[E];
-    if constexpr (HALVES) {
-#pragma unroll
-      for (int e = 0; e < H; ++e) {
-        z[e] = y[i][e] * c[e] - y[i][H + e] * s[e];
-        z[H + e] = y[i][H + e] * c[e] + y[i][e] * s[e];
-      }
-    } else {
-      // a value past rot_dim is its own pair, with sine 0: it must not meet an infinity times 0
+    if constexpr (MODE == kPart) {
+      // a value past rot_dim stays: it must not meet an infinity times 0
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float other = p.interleaved ? y[i][e ^ 1] : __shfl_sync(0xffffffffu, y[i][e], src);
-        z[e] = l * E + e < p.rot_dim ? y[i][e] * c[e] + other * s[e] : y[i][e];
+        const float other = __shfl_sync(0xffffffffu, y[i][e], src);
+        z[e] = l * E < p.rot_dim ? y[i][e] * c[e] + other * s[e] : y[i][e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < H; ++e) {
+        const int a = MODE == kHalves ? e : 2 * e, b = MODE == kHalves ? H + e : 2 * e + 1;
+        const bool stays = MODE == kPairs && l * E + a >= p.rot_dim;
+        z[a] = stays ? y[i][a] : y[i][a] * c[e] - y[i][b] * s[e];
+        z[b] = stays ? y[i][b] : y[i][b] * c[e] + y[i][a] * s[e];
       }
     }
-    if (on && h0 + i < heads) {
-      if constexpr (HALVES)
+    if (on && holds && h0 + i < heads) {
+      if constexpr (MODE == kHalves)
         store_halves<T, E>(out + i * D + l * H, D / 2, vec_out, z);
       else
         store_f32<T, E>(out + i * D + l * E, vec_out, z);
@@ -503,39 +512,58 @@ __global__ void __launch_bounds__(kQkWarps * 32) qk_norm_rope_any_kernel(QkNormR
   }
 }
 
-template <class T, int E, int LPH>
-cudaError_t qk_launch_vec(const QkNormRopeParams& p, int vec_in, int vec_out, int sm_count, cudaStream_t st) {
-  const int vec_turn = (reinterpret_cast<uintptr_t>(p.cos_cache) | reinterpret_cast<uintptr_t>(p.sin_cache)) % 8 == 0 &&
-                       p.rot_dim / 2 % 2 == 0;
+struct QkLaunch {
+  QkNormRopeParams p;
+  int vec_in, vec_out, vec_turn, sm_count;
+  cudaStream_t st;
+};
+
+template <class T, int E, int LPH, int MODE, bool EXACT>
+cudaError_t qk_launch_vec(const QkLaunch& a) {
   auto blocks = [&](int hb) {
-    return ((long long)p.tokens * ((p.heads[0] + hb - 1) / hb + (p.heads[1] + hb - 1) / hb) * LPH + 255) / 256;
+    const int parts = (a.p.heads[0] + hb - 1) / hb + (a.p.heads[1] + hb - 1) / hb;
+    return (unsigned)(((long long)a.p.tokens * parts * LPH + 255) / 256);
   };
-  const bool halves = !p.interleaved && p.rot_dim == p.head_dim;
   // one head a group until every SM has its 2048 threads twice over
-  if (blocks(4) < 16ll * sm_count)
-    return launch(halves ? qk_norm_rope_kernel<T, E, LPH, 1, true> : qk_norm_rope_kernel<T, E, LPH, 1, false>,
-                  dim3((unsigned)blocks(1)), 256, 0, st, p, vec_in, vec_out, vec_turn);
-  return launch(halves ? qk_norm_rope_kernel<T, E, LPH, 4, true> : qk_norm_rope_kernel<T, E, LPH, 4, false>,
-                dim3((unsigned)blocks(4)), 256, 0, st, p, vec_in, vec_out, vec_turn);
+  if (blocks(4) < 16ll * a.sm_count)
+    return launch(qk_norm_rope_kernel<T, E, LPH, 1, MODE, EXACT>, dim3(blocks(1)), 256, 0, a.st, a.p, a.vec_in, a.vec_out,
+                  a.vec_turn);
+  return launch(qk_norm_rope_kernel<T, E, LPH, 4, MODE, EXACT>, dim3(blocks(4)), 256, 0, a.st, a.p, a.vec_in, a.vec_out,
+                a.vec_turn);
+}
+
+template <class T, int E, int LPH>
+cudaError_t qk_launch_mode(const QkLaunch& a, int mode) {
+  const bool exact = a.p.head_dim == E * LPH;
+  if (mode == kHalves) return exact ? qk_launch_vec<T, E, LPH, kHalves, true>(a) : qk_launch_vec<T, E, LPH, kHalves, false>(a);
+  if (mode == kPairs) return exact ? qk_launch_vec<T, E, LPH, kPairs, true>(a) : qk_launch_vec<T, E, LPH, kPairs, false>(a);
+  return exact ? qk_launch_vec<T, E, LPH, kPart, true>(a) : qk_launch_vec<T, E, LPH, kPart, false>(a);
 }
 
 template <class T>
 cudaError_t qk_launch(const QkNormRopeParams& p, int sm_count, cudaStream_t st) {
-  const int size = (int)sizeof(T);
+  constexpr int S = (int)sizeof(T), E = 16 / S;  // 16 bytes a lane
   uintptr_t in = 0, out = 0;
   for (int i = 0; i < 2; ++i) {
     if (p.heads[i] == 0) continue;
-    in |= reinterpret_cast<uintptr_t>(p.x[i]) | (uintptr_t)(p.in_stride[i] * size);
-    out |= reinterpret_cast<uintptr_t>(p.out[i]) | (uintptr_t)(p.out_stride[i] * size);
+    in |= reinterpret_cast<uintptr_t>(p.x[i]) | (uintptr_t)(p.in_stride[i] * S);
+    out |= reinterpret_cast<uintptr_t>(p.out[i]) | (uintptr_t)(p.out_stride[i] * S);
   }
-  const int vec_in = in % 32 == 0 ? 2 : in % 16 == 0, vec_out = out % 32 == 0 ? 2 : out % 16 == 0;
-  constexpr int E = 16 / (int)sizeof(T);  // 16 bytes a lane
-  const int half = p.rot_dim / 2;
-  const int e = p.head_dim == 256 ? 8 : E;
-  if (p.interleaved || half % e == 0) {
-    if (p.head_dim == 64) return qk_launch_vec<T, E, 64 / E>(p, vec_in, vec_out, sm_count, st);
-    if (p.head_dim == 128) return qk_launch_vec<T, E, 128 / E>(p, vec_in, vec_out, sm_count, st);
-    if (p.head_dim == 256) return qk_launch_vec<T, 8, 32>(p, vec_in, vec_out, sm_count, st);
+  const uintptr_t heads = (uintptr_t)(p.head_dim * S);  // heads lie one after the other
+  in |= heads;
+  out |= heads;
+  QkLaunch a{p, in % 32 == 0 ? 2 : in % 16 == 0, out % 32 == 0 ? 2 : out % 16 == 0,
+             (reinterpret_cast<uintptr_t>(p.cos_cache) | reinterpret_cast<uintptr_t>(p.sin_cache)) % 8 == 0 &&
+                 p.rot_dim / 2 % 2 == 0,
+             sm_count, st};
+  const int half = p.rot_dim / 2, e = p.head_dim > 32 * E ? 8 : E;  // values of a lane
+  const int mode = p.interleaved ? kPairs : p.rot_dim == p.head_dim ? kHalves : kPart;
+  if (p.head_dim % e == 0 && p.head_dim <= 32 * e && (mode != kPart || half % e == 0)) {
+    const int lanes = p.head_dim / e;
+    if (e != E) return qk_launch_mode<T, 8, 32>(a, mode);
+    if (lanes <= 8) return qk_launch_mode<T, E, 8>(a, mode);
+    if (lanes <= 16) return qk_launch_mode<T, E, 16>(a, mode);
+    return qk_launch_mode<T, E, 32>(a, mode);
   }
   const long long units = (long long)p.tokens * (p.heads[0] + p.heads[1]);
   return launch(qk_norm_rope_any_kernel<T>, dim3((unsigned)((units + kQkWarps - 1) / kQkWarps)), kQkWarps * 32,
