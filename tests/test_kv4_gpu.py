@@ -394,6 +394,10 @@ ATTENTION = [
     ([4000], [3], 12, 4, 256, 64, 128),
     ([37] * 70, None, 4, 4, 64, 64, 16),
     ([5000] + [20] * 150, None, 8, 2, 128, 128, 16),      # one long, many short
+    ([90] + [17] * 29, [30] + [1] * 29, 4, 2, 128, 64, 16),  # one token on the mean, thirty once
+    ([260, 31, 7], [1, 0, 2], 4, 1, 64, 64, 32),          # four heads a group: one row a head
+    ([1500], [1], 3, 1, 256, 128, 16),
+    ([10, 700], None, 2, 1, 128, 64, 64),
 ]
 
 

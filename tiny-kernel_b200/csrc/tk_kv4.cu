@@ -308,14 +308,16 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(SlotsParams 
       const long long x = free0 + a0 + i * kSlotsThreads;
       id[i] = free0 < end ? p.free_blocks[x < end ? x : free0] : -1;
     }
+    const long long left = end - free0 - a0;  // of the list from this place
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kIds; ++i)
+      bad = bad || (unsigned)id[i] >= (unsigned)p.num_blocks || i * kSlotsThreads >= left;
+    if (!bad) continue;
 #pragma unroll 1
     for (int i = 0; i < kIds; ++i) {
       const long long a = a0 + (long long)i * kSlotsThreads;
-      int v = id[0];
-#pragma unroll
-      for (int k = 1; k < kIds; ++k)
-        if (k == i) v = id[k];
-      if (a >= taken || (free0 + a < end && v >= 0 && v < p.num_blocks)) continue;
+      if (a >= taken || slots_new_block(p.free_blocks, begin, end, a, p.num_blocks) >= 0) continue;
       const int run = find_run(s_first, a);
       c = {run * per, s_start[run], s_first[run], {}};
       c.at(p);

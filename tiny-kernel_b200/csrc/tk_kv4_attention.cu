@@ -18,6 +18,10 @@
 // the odd dimensions); the sums are exact.
 //   Weights against values: f16.  c - 8 is exact, p s_v is split into two f16 (22 bits), one m16n8k16
 // product each.
+//   Tiles of four rows (one token of up to four heads a group) put two digits, and both f16 parts of a
+// weight, next to each other in the 8 columns: 2 + 1 products instead of 3 + 2, and a lane has half
+// the scores (one token of a unit instead of two).  1 x 131072 and 48 x 8192 with four heads a group:
+// see attention_rows.
 // mma.sync and not tcgen05: one token of a head group is at most 8 rows, an eighth of tcgen05's
 // smallest tile, whose operands would also have to pass through shared memory unpacked.
 //
@@ -37,7 +41,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 8;       // rows (query token, head of the group) of a product
+constexpr int kCols = 8;       // columns of a product; a tile has 8 rows (query token, head of the group) or 4
 constexpr int kUnit = 16;      // tokens that lie in one page for sure
 constexpr int kSub = 2;        // units of a warp's step
 constexpr int kTokens = kUnit * kSub;
@@ -60,7 +64,7 @@ struct Part {
   int row0, slot, pad0, pad1;    // first row of the tile; the slot of the first part
 };
 
-size_t part_bytes(int head_dim) { return (size_t)kRows * (head_dim + 2) * sizeof(float); }
+size_t part_bytes(int head_dim) { return (size_t)kCols * (head_dim + 2) * sizeof(float); }
 
 __device__ __forceinline__ float load_any(const void* base, long long i, int dtype) {
   if (dtype == kTypeF32) return static_cast<const float*>(base)[i];
@@ -207,6 +211,7 @@ struct Sequence {
   int tiles;        // row tiles
   int steps;        // of a tile, its cost among them
 };
+template <int ROWS>
 __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b, int per) {
   Sequence s;
   if (p.query_start) {
@@ -219,7 +224,7 @@ __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b,
   const int len = max(p.kv_lens[b], 0);
   s.last = len - s.n;
   s.kv = (int)min((long long)len, (long long)p.max_blocks << p.cache.shift);
-  s.tiles = (int)(((long long)s.n * per + kRows - 1) / kRows);
+  s.tiles = (int)(((long long)s.n * per + ROWS - 1) / ROWS);
   s.steps = kTileCost + (s.kv + kStep - 1) / kStep;  // kv < 2^31 - 1024
   return s;
 }
@@ -233,24 +238,28 @@ struct Tile {
 
 // Shared memory of a CTA: the tile's queries as operands, its rows' numbers, the warps' rings, the
 // warps' sums at the end of a tile.
-template <int D, int G>
+template <int D, int G, int ROWS>
 struct Smem {
   using S = Stage<D, G>;
-  static constexpr int kQuery = D / 32 * 32 * 32;  // [word][lane][8]: three digits of 32 bits twice, two words idle
+  // [word][lane]: three digits of 32 bits twice, two words idle; of four rows two products' digits twice
+  static constexpr int kLaneWords = ROWS == 4 ? 4 : 8;
+  static constexpr int kQuery = D / 32 * 32 * kLaneWords * 4;
   static constexpr int kRowWords = 1 + 4 * S::NG;  // unscale; sum, three centres a group
-  static constexpr int kRowBytes = kRows * kRowWords * 4;
+  static constexpr int kRowBytes = kCols * kRowWords * 4;
   static constexpr int kWarp = kRing<D> * S::kBytes;
   static constexpr int kJoint = D + 1;                     // floats of a row of sums at the end
-  static constexpr int kJointWarp = kRows * (kJoint + 2);  // and per row the reference and l
+  static constexpr int kJointWarp = kCols * (kJoint + 2);  // and per row the reference and l
   static constexpr int kRings = kQuery + kRowBytes, kJoints = kRings + kWarps * kWarp;
   static constexpr int kBytes = kJoints + kWarps * kJointWarp * 4;
   static_assert(kRowBytes % 16 == 0 && kWarp % 16 == 0, "");
 };
 
-template <int D, int G>
+template <int D, int G, int ROWS>
 __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(Kv4AttentionParams p, int dtype) {
   using S = Stage<D, G>;
-  using M = Smem<D, G>;
+  using M = Smem<D, G, ROWS>;
+  constexpr bool kFour = ROWS == 4;
+  constexpr int J = kFour ? 1 : 2;  // tokens of a unit that a lane has scores of
   constexpr int kStages = kRing<D>;
   constexpr int NG = S::NG, NT = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -263,14 +272,14 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   const int per = p.q_heads / p.cache.kv_heads, hk = p.cache.kv_heads;
   Part* parts = static_cast<Part*>(p.workspace);
   float* sums = reinterpret_cast<float*>(parts + gridDim.x);
-  constexpr int kSlot = kRows * (D + 2);
+  constexpr int kSlot = ROWS * (D + 2);
 
   // ---- this CTA's run ----
   const int chunk = (p.batch + kThreads - 1) / kThreads;
   const int b0 = (int)min((long long)p.batch, (long long)tid * chunk), b1 = min(p.batch, b0 + chunk);
   long long mine = 0;
   for (int b = b0; b < b1; ++b) {
-    const Sequence s = sequence(p, b, per);
+    const Sequence s = sequence<ROWS>(p, b, per);
     mine += (long long)s.steps * s.tiles * hk;
   }
   long long inc = mine;
@@ -296,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
     long long at = before;
     int b = b0;
     for (;; ++b) {
-      const Sequence s = sequence(p, b, per);
+      const Sequence s = sequence<ROWS>(p, b, per);
       const long long w = (long long)s.steps * s.tiles * hk;
       if (start < at + w) break;
       at += w;
@@ -307,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   __syncthreads();
   Tile cur;
   cur.b = s_seq;
-  cur.s = sequence(p, cur.b, per);
+  cur.s = sequence<ROWS>(p, cur.b, per);
   {
     long long unit = (long long)((double)s_at / cur.s.steps);  // off by one at most
     if (unit * cur.s.steps > s_at) --unit;
@@ -324,7 +333,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   uint8_t* ring = smem + M::kRings + warp * M::kWarp;
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
   float* joint = reinterpret_cast<float*>(smem + M::kJoints) + warp * M::kJointWarp;
-  // the lane's sum o[i][k] in it: row 2t + k % 2, dimension 32 (i / 2) + 4g + 2 (i % 2) + k / 2
+  // the lane's rows, and its token of a unit (and the one 8 on)
+  const int my_row = kFour ? 2 * (t & 1) : 2 * t, my_token = kFour ? g + 8 * (t >> 1) : g;
+  const bool low = kFour && t >= 2;  // the columns of the lower digit, the lower part of a weight
+  // the lane's sum o[i][k] in it: column 2t + k % 2, dimension 32 (i / 2) + 4g + 2 (i % 2) + k / 2
   float* mine_at = joint + 2 * t * M::kJoint + 4 * g;
   auto kept = [&](int i, int k) -> float& {
     return mine_at[(k & 1) * M::kJoint + i / 2 * 32 + i % 2 * 2 + k / 2];
@@ -381,11 +393,11 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   auto token_of = [&](const Tile& x, int row) { return x.s.n == 1 ? 0 : row / per; };
   // the position after the last that row r of a tile sees; its last row sees most, its first least
   auto sees = [&](const Tile& x, int r) {
-    const int row = x.rt * kRows + r, end = x.s.n * per - 1;
+    const int row = x.rt * ROWS + r, end = x.s.n * per - 1;
     return min(x.s.kv, x.s.last + token_of(x, min(row, end)) + 1);
   };
   constexpr int LPR = D / 8;                                   // threads of a row of queries, 8 dimensions each
-  constexpr int kPasses = (kRows * LPR + kThreads - 1) / kThreads;
+  constexpr int kPasses = (ROWS * LPR + kThreads - 1) / kThreads;
   float q[kPasses][8];
   auto begin = [&](const Tile& x) {
     const uint64_t head_at = (uint64_t)(uint32_t)(x.head << p.cache.shift) * S::kRowBytes;
@@ -395,15 +407,15 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
     table = p.block_tables + (size_t)x.b * p.max_blocks;
     s0 = max(x.c0 - kTileCost, 0);
     s1 = max(x.c1 - kTileCost, 0);
-    see_most = sees(x, kRows - 1);
+    see_most = sees(x, ROWS - 1);
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * (kThreads / LPR) + tid / LPR;
-      const int row = min(x.rt * kRows + r, x.s.n * per - 1);
+      const int row = min(x.rt * ROWS + r, x.s.n * per - 1);
 #pragma unroll
       for (int k = 0; k < 8; ++k) q[i][k] = 0.f;
       const int token = token_of(x, row);
-      if (r < kRows && sees(x, r) > 0)
+      if (r < ROWS && sees(x, r) > 0)
         load_row8(p.q, (long long)(x.s.first + token) * p.q_stride + (long long)(x.head * per + row - token * per) * D +
                            tid % LPR * 8, dtype, q[i]);
     }
@@ -417,13 +429,13 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   begin(cur);
 
   for (;;) {
-      const int see_least = sees(cur, 0), see[2] = {sees(cur, 2 * t), sees(cur, 2 * t + 1)};
+      const int see_least = sees(cur, 0), see[2] = {sees(cur, my_row), sees(cur, my_row + 1)};
 
       // ---- queries: scaled, as integers of 22 bits, in digits; 8 dimensions a thread ----
 #pragma unroll
       for (int pass = 0; pass < kPasses; ++pass) {
         const int r = pass * (kThreads / LPR) + tid / LPR, at8 = tid % LPR;
-        if (r >= kRows) continue;  // whole warps
+        if (r >= ROWS) continue;  // whole warps
         const float f = p.scale * 1.4426950408889634f;
         float top = 0.f, odd = 0.f;
 #pragma unroll
@@ -465,9 +477,15 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
           for (int d = 0; d < 3; ++d) sums[d] += __shfl_xor_sync(0xffffffffu, sums[d], off);
         }
         const int y = at8 / (G / 8), tt = at8 % (G / 8) / (G / 32), w = y * (G / 32) + at8 % (G / 32);
-        uint32_t* dst = query + (w * 32 + r * 4 + tt) * 8;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(digits[0][0], digits[0][1], digits[1][0], digits[1][1]);
-        *reinterpret_cast<uint2*>(dst + 4) = make_uint2(digits[2][0], digits[2][1]);
+        uint32_t* dst = query + (w * 32 + r * 4 + tt) * M::kLaneWords;
+        if constexpr (kFour) {  // columns 0-3, 4-7: the highest digit, the next; the lowest twice
+          *reinterpret_cast<uint4*>(dst) = make_uint4(digits[0][0], digits[0][1], digits[2][0], digits[2][1]);
+          *reinterpret_cast<uint4*>(dst + 16 * M::kLaneWords) =
+              make_uint4(digits[1][0], digits[1][1], digits[2][0], digits[2][1]);
+        } else {
+          *reinterpret_cast<uint4*>(dst) = make_uint4(digits[0][0], digits[0][1], digits[1][0], digits[1][1]);
+          *reinterpret_cast<uint2*>(dst + 4) = make_uint2(digits[2][0], digits[2][1]);
+        }
         float* num = row_num + r * M::kRowWords;
         if (at8 == 0) num[0] = ldexpf(1.f, -e) + odd;
         if (at8 % (G / 8) == 0) {
@@ -477,23 +495,26 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
         }
       }
       __syncthreads();
-      // of the lane's rows 2t, 2t + 1
+      // of the lane's two rows
       float unscale[2], qsum[NG][2], off_sum[NG][2], l[2] = {0.f, 0.f};
       float ref[2] = {-INFINITY, -INFINITY};  // weights are 2^(s - ref + 10) s_v
       float centre[NG][3][2];                 // where a digit's sum begins, and 8 times the sum of the row's digits
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float* num = row_num + (2 * t + i) * M::kRowWords;
+        const float* num = row_num + (my_row + i) * M::kRowWords;
         unscale[i] = num[0];
 #pragma unroll
         for (int y = 0; y < NG; ++y) {
           qsum[y][i] = num[1 + 4 * y];
 #pragma unroll
           for (int d = 0; d < 3; ++d) centre[y][d][i] = num[2 + 4 * y + d];
+          // four rows: of the lane's own digit, at its place; exact, so that a product and sum with it is
+          if (kFour) centre[y][0][i] = low ? -256.f * num[3 + 4 * y] : -65536.f * num[2 + 4 * y];
           off_sum[y][i] = 0.f;
         }
       }
-      // sums: products of 16 dimensions, 32 z + 4 g + 2 h + {0, 1} in o[2 z + h], of rows 2t, 2t + 1
+      const float place = low ? 256.f : 65536.f;  // of the lane's digit
+      // sums: products of 16 dimensions, 32 z + 4 g + 2 h + {0, 1} in o[2 z + h], of columns 2t, 2t + 1
       float o[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -517,16 +538,16 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
         auto step_of = [&](auto masked) {
         constexpr bool kMasked = decltype(masked)::value;
 
-        // scores of tokens g, g + 8 of the units against rows 2t, 2t + 1, in units of unscale
-        float sc[kSub][2][2], vs[kSub][2][NG], vm[kSub][2][NG], top[2] = {-INFINITY, -INFINITY};
+        // scores of the lane's tokens of the units against its rows, in units of unscale
+        float sc[kSub][J][2], vs[kSub][J][NG], vm[kSub][J][NG], top[2] = {-INFINITY, -INFINITY};
         unsigned hidden = 0;  // scores that are not seen
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
           const uint8_t* su = st + u * S::kUnitBytes;
-          const uint32_t* pairs = reinterpret_cast<const uint32_t*>(su + 2 * S::kCodes) + g * NG;
-          float lg[2];
+          const uint32_t* pairs = reinterpret_cast<const uint32_t*>(su + 2 * S::kCodes) + my_token * NG;
+          float lg[J];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < J; ++j) {
             float most = 5.9604645e-8f;  // 2^-24, the least f16
 #pragma unroll
             for (int y = 0; y < NG; ++y) {
@@ -549,41 +570,60 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
               else
                 *reinterpret_cast<uint2*>(w[j]) = *reinterpret_cast<const uint2*>(src);
             }
-            int c[3][4];
+            constexpr int P = kFour ? 2 : 3;  // products
+            int c[P][4];
 #pragma unroll
             for (int i = 0; i < G / 32; ++i) {
-              // the digits of row g: from shared memory again, for the registers' sake
-              const uint32_t* qs = query + ((y * (G / 32) + i) * 32 + lane) * 8;
+              // the digits of column g: from shared memory again, for the registers' sake
+              const uint32_t* qs = query + ((y * (G / 32) + i) * 32 + lane) * M::kLaneWords;
               const uint4 q4 = *reinterpret_cast<const uint4*>(qs);
-              const uint2 q2 = *reinterpret_cast<const uint2*>(qs + 4);
-              const uint32_t qd[3][2] = {{q4.x, q4.y}, {q4.z, q4.w}, {q2.x, q2.y}};
+              uint32_t qd[P][2];
+              qd[0][0] = q4.x, qd[0][1] = q4.y, qd[1][0] = q4.z, qd[1][1] = q4.w;
+              if constexpr (!kFour) {
+                const uint2 q2 = *reinterpret_cast<const uint2*>(qs + 4);
+                qd[2][0] = q2.x, qd[2][1] = q2.y;
+              }
               const uint32_t a[4] = {w[0][i] & 0x0F0F0F0Fu, w[1][i] & 0x0F0F0F0Fu, w[0][i] >> 4 & 0x0F0F0F0Fu,
                                      w[1][i] >> 4 & 0x0F0F0F0Fu};
 #pragma unroll
-              for (int d = 0; d < 3; ++d) {
+              for (int d = 0; d < P; ++d) {
                 if (i == 0)
                   mma16832_first(c[d], a, qd[d][0], qd[d][1]);
                 else
                   mma16832(c[d], a, qd[d][0], qd[d][1]);
               }
             }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t pair = pairs[j * 8 * NG + y];
+            if constexpr (kFour) {
+              const uint32_t pair = pairs[y];
               const float ks = half_lo(pair), km = fmaf(ks, 8.f, half_hi(pair));
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                float dot = __int_as_float(c[0][2 * j + i]) - centre[y][0][i];  // exact, as the next two
-                dot = fmaf(dot, 256.f, __int_as_float(c[1][2 * j + i]) - centre[y][1][i]);
-                dot = fmaf(dot, 256.f, __int_as_float(c[2][2 * j + i]) - centre[y][2][i]);
-                sc[u][j][i] = fmaf(dot, ks, fmaf(qsum[y][i], km, sc[u][j][i]));
+                // the lane's digit of both tokens, at its place: exact.  The lane two on (mod 4) has the other
+                const float x0 = fmaf(__int_as_float(c[0][i]), place, centre[y][0][i]);
+                const float x8 = fmaf(__int_as_float(c[0][2 + i]), place, centre[y][0][i]);
+                float dot = __int_as_float(low ? c[1][2 + i] : c[1][i]) - centre[y][2][i];
+                dot += (low ? x8 : x0) + __shfl_xor_sync(0xffffffffu, low ? x0 : x8, 2);
+                sc[u][0][i] = fmaf(dot, ks, fmaf(qsum[y][i], km, sc[u][0][i]));
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < J; ++j) {
+                const uint32_t pair = pairs[j * 8 * NG + y];
+                const float ks = half_lo(pair), km = fmaf(ks, 8.f, half_hi(pair));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  float dot = __int_as_float(c[0][2 * j + i]) - centre[y][0][i];  // exact, as the next two
+                  dot = fmaf(dot, 256.f, __int_as_float(c[1][2 * j + i]) - centre[y][1][i]);
+                  dot = fmaf(dot, 256.f, __int_as_float(c[P - 1][2 * j + i]) - centre[y][2][i]);
+                  sc[u][j][i] = fmaf(dot, ks, fmaf(qsum[y][i], km, sc[u][j][i]));
+                }
               }
             }
           }
           if constexpr (kMasked) {  // of what a row does not see nothing counts, and it may be NaN
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int at_token = there >> u & 1 ? pos + u * kUnit + j * 8 + g : 0x7fffffff;
+            for (int j = 0; j < J; ++j) {
+              const int at_token = there >> u & 1 ? pos + u * kUnit + j * 8 + my_token : 0x7fffffff;
               if (at_token >= see_most) {
 #pragma unroll
                 for (int y = 0; y < NG; ++y) vs[u][j][y] = vm[u][j][y] = 0.f;
@@ -598,13 +638,13 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
           }
           // reference: the row's largest s + log2 of the value scale
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int i = 0; i < 2; ++i) top[i] = fmaxf(top[i], fmaf(sc[u][j][i], unscale[i], lg[j]));
         }
         if (__any_sync(0xffffffffu, top[0] > ref[0] + 5.f || top[1] > ref[1] + 5.f)) {
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) {
+          for (int off = kFour ? 2 : 4; off < 32; off <<= 1) {
             top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
             top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
           }
@@ -637,9 +677,9 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-          float pr[2][2];
+          float pr[J][2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               pr[j][i] = ex2(fmaf(sc[u][j][i], unscale[i], base[i]));
@@ -647,9 +687,9 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
             }
 #pragma unroll
           for (int y = 0; y < NG; ++y) {
-            uint32_t hi[2], lo[2];
+            uint32_t hi[2], lo[2];  // four rows: hi holds both parts
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < J; ++j) {
               float w[2];
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
@@ -661,8 +701,19 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
                   w[i] = 0.f;
               }
               split_f16(w[0], w[1], hi[j], lo[j]);
-              hi[j] = transpose8(hi[j]);  // tokens 8j + 2t, 8j + 2t + 1 of row g
-              lo[j] = transpose8(lo[j]);
+            }
+            if constexpr (kFour) {
+              // columns 0-3 the upper parts of tokens 0-7 (8-15), columns 4-7 the lower ones
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, low ? hi[0] : lo[0], 2);
+              const uint32_t m0 = low ? other : hi[0], m8 = low ? lo[0] : other;
+              hi[0] = transpose8(m0);
+              hi[1] = transpose8(m8);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                hi[j] = transpose8(hi[j]);  // tokens 8j + 2t, 8j + 2t + 1 of row g
+                lo[j] = transpose8(lo[j]);
+              }
             }
 #pragma unroll
             for (int z = y * (G / 32); z < (y + 1) * (G / 32); z += 2) {  // 32 dimensions each
@@ -676,8 +727,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
                 a[h][0] = codes_lo(x), a[h][1] = codes_hi(x), a[h][2] = codes_lo(x8), a[h][3] = codes_hi(x8);
                 mma16816(o[2 * z + h], a[h], hi[0], hi[1]);
               }
+              if constexpr (!kFour) {
 #pragma unroll
-              for (int h = 0; h < 4; ++h) mma16816(o[2 * z + h], a[h], lo[0], lo[1]);
+                for (int h = 0; h < 4; ++h) mma16816(o[2 * z + h], a[h], lo[0], lo[1]);
+              }
             }
           }
         }
@@ -708,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
+        for (int off = kFour ? 2 : 4; off < 32; off <<= 1) {
           l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
 #pragma unroll
           for (int y = 0; y < NG; ++y) off_sum[y][i] += __shfl_xor_sync(0xffffffffu, off_sum[y][i], off);
@@ -719,13 +772,14 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
         for (int k = 0; k < 4; ++k) {
           float x = o[i][k];
           if (flushed) x += kept(i, k);
-          kept(i, k) = fmaf(x, kCodes, off_sum[i / (G / 16)][k & 1]);
+          if (kFour) x += __shfl_xor_sync(0xffffffffu, x, 2);  // both parts
+          if (!low) kept(i, k) = fmaf(x, kCodes, off_sum[i / (G / 16)][k & 1]);
         }
-      if (g == 0) {
+      if (g == 0 && !low) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          joint[kRows * M::kJoint + 2 * (2 * t + i)] = ref[i];
-          joint[kRows * M::kJoint + 2 * (2 * t + i) + 1] = l[i];
+          joint[kCols * M::kJoint + 2 * (my_row + i)] = ref[i];
+          joint[kCols * M::kJoint + 2 * (my_row + i) + 1] = l[i];
         }
       }
 
@@ -741,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
           if (++cur.head == hk) {
             cur.head = 0;
             do {
-              cur.s = sequence(p, ++cur.b, per);
+              cur.s = sequence<ROWS>(p, ++cur.b, per);
             } while (cur.s.tiles == 0);
           }
         }
@@ -752,11 +806,11 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 
       {
         const bool whole = done.c0 == 0 && done.c1 == done.s.steps;
-        const int row0 = done.rt * kRows, rows = min(kRows, done.s.n * per - row0), slot = done_at == start ? 0 : 1;
-        constexpr int kThreadsRow = kThreads / kRows;
+        const int row0 = done.rt * ROWS, rows = min(ROWS, done.s.n * per - row0), slot = done_at == start ? 0 : 1;
+        constexpr int kThreadsRow = kThreads / ROWS;
         const int row = tid / kThreadsRow, d0 = tid % kThreadsRow;
         const float* all = reinterpret_cast<const float*>(smem + M::kJoints);
-        const float* num = all + kRows * M::kJoint + 2 * row;
+        const float* num = all + kCols * M::kJoint + 2 * row;
         float top = -INFINITY, sum = 0.f, f[kWarps];
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, num[w * M::kJointWarp]);
@@ -782,8 +836,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
             store_any(p.o, o_at + d, dtype, sum == 0.f ? 0.f : v / sum);
         }
         if (!whole && d0 == 0) {
-          out[kRows * D + 2 * row] = top;
-          out[kRows * D + 2 * row + 1] = sum;
+          out[ROWS * D + 2 * row] = top;
+          out[ROWS * D + 2 * row + 1] = sum;
         }
         if (!whole && done.c0 == 0 && tid == 0) {  // the tile begins here: where its parts are
           const long long end = done_at + done.s.steps;
@@ -800,7 +854,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 constexpr int kJoinWarps = 4;
 constexpr int kJoinRows = 2;
 
-template <int D>
+template <int D, int ROWS>
 __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(Kv4AttentionParams p, int dtype) {
   __shared__ float s_sum[kJoinRows][kJoinWarps];
   __shared__ float s_v[kJoinRows][kJoinWarps][D];
@@ -808,7 +862,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(K
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Part* parts = static_cast<const Part*>(p.workspace);
   const float* sums = reinterpret_cast<const float*>(parts + gridDim.x);
-  constexpr int kSlot = kRows * (D + 2);
+  constexpr int kSlot = ROWS * (D + 2);
   const Part part = parts[blockIdx.x];
   if (part.count == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = warp / kJoinWarps, w = warp % kJoinWarps;
@@ -816,7 +870,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(K
   auto base = [&](int i) { return sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot; };
   // the lane's part of each 32: its reference and l, then its factor
   float top = -INFINITY;
-  for (int i = lane; i < part.count; i += 32) top = fmaxf(top, base(i)[kRows * D + 2 * row]);
+  for (int i = lane; i < part.count; i += 32) top = fmaxf(top, base(i)[ROWS * D + 2 * row]);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   constexpr int V = D == 64 ? 2 : 4, E = D / (32 * V);  // values of a load, loads of a row
@@ -828,7 +882,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(K
 #pragma unroll 8
   for (int i = w; i < part.count; i += kJoinWarps) {
     const float* s = base(i);
-    const float2 num = *reinterpret_cast<const float2*>(s + kRows * D + 2 * row);
+    const float2 num = *reinterpret_cast<const float2*>(s + ROWS * D + 2 * row);
     const float f = num.x == -INFINITY ? 1.f : ex2(num.x - top);  // no reference: sums of 0, or of NaN
     sum = fmaf(num.y, f, sum);
 #pragma unroll
@@ -863,14 +917,21 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(K
   }
 }
 
+// Rows of a tile: four where a sequence has about as many (its query tokens are not known here, their
+// mean is), eight otherwise.
+int attention_rows(const Kv4AttentionParams& p) {
+  const long long per = p.q_heads / p.cache.kv_heads;
+  return p.tokens * per <= 4ll * p.batch ? 4 : 8;
+}
+
 int attention_ctas(int head_dim, int sm_count) { return sm_count * (head_dim == 256 ? kResident<256> : kResident<128>); }
 
-template <int D, int G>
+template <int D, int G, int ROWS>
 cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t st) {
-  const size_t smem = Smem<D, G>::kBytes;
+  const size_t smem = Smem<D, G, ROWS>::kBytes;
   cudaError_t e;
   if (smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(kv4_attention_kernel<D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(kv4_attention_kernel<D, G, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
   }
@@ -888,12 +949,12 @@ cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t s
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, G>, p, dtype);
+  e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, G, ROWS>, p, dtype);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3((unsigned)ctas, kRows / kJoinRows);
+  cfg.gridDim = dim3((unsigned)ctas, ROWS / kJoinRows);
   cfg.blockDim = dim3(kJoinRows * kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, p, dtype);
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, ROWS>, p, dtype);
 }
 
 }  // namespace
@@ -904,9 +965,14 @@ size_t kv4_attention_workspace(int head_dim, int sm_count) {
 
 cudaError_t launch_kv4_attention(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStream_t st) {
   const int d = p.cache.head_dim, g = p.cache.group;
-  if (d == 64) return launch<64, 64>(p, dtype, sm_count, st);
-  if (d == 128) return g == 64 ? launch<128, 64>(p, dtype, sm_count, st) : launch<128, 128>(p, dtype, sm_count, st);
-  return g == 64 ? launch<256, 64>(p, dtype, sm_count, st) : launch<256, 128>(p, dtype, sm_count, st);
+  if (attention_rows(p) == 4) {
+    if (d == 64) return launch<64, 64, 4>(p, dtype, sm_count, st);
+    if (d == 128) return g == 64 ? launch<128, 64, 4>(p, dtype, sm_count, st) : launch<128, 128, 4>(p, dtype, sm_count, st);
+    return g == 64 ? launch<256, 64, 4>(p, dtype, sm_count, st) : launch<256, 128, 4>(p, dtype, sm_count, st);
+  }
+  if (d == 64) return launch<64, 64, 8>(p, dtype, sm_count, st);
+  if (d == 128) return g == 64 ? launch<128, 64, 8>(p, dtype, sm_count, st) : launch<128, 128, 8>(p, dtype, sm_count, st);
+  return g == 64 ? launch<256, 64, 8>(p, dtype, sm_count, st) : launch<256, 128, 8>(p, dtype, sm_count, st);
 }
 
 }  // namespace tk
