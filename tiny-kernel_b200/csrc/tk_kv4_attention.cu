@@ -47,7 +47,7 @@ constexpr int kSub = 2;        // units of a warp's step
 constexpr int kTokens = kUnit * kSub;
 constexpr int kStep = kTokens * kWarps;
 template <int D>
-constexpr int kRing = D == 256 ? 2 : 3;  // stages of a warp's ring
+constexpr int kRing = 2;  // stages of a warp's ring
 template <int D>
 constexpr int kResident = D == 256 ? 2 : 3;  // CTAs of an SM
 constexpr int kFlush = 16;     // steps between two settings aside of the sums
@@ -849,15 +849,12 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   }
 }
 
-// Joins the parts of the tile that begins in the run of CTA blockIdx.x, kJoinRows of its rows.
-// kJoinWarps warps a row, each with every kJoinWarps-th part, then in the order of the warps.
-constexpr int kJoinWarps = 4;
-constexpr int kJoinRows = 2;
-
-template <int D, int ROWS>
-__global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(Kv4AttentionParams p, int dtype) {
-  __shared__ float s_sum[kJoinRows][kJoinWarps];
-  __shared__ float s_v[kJoinRows][kJoinWarps][D];
+// Joins the parts of the tile that begins in the run of CTA blockIdx.x, RC of its rows.  W warps a row,
+// each with every W-th part, then in the order of the warps.
+template <int D, int ROWS, int RC, int W>
+__global__ void __launch_bounds__(RC * W * 32) kv4_join_kernel(Kv4AttentionParams p, int dtype) {
+  __shared__ float s_num[RC][W][2];
+  __shared__ float s_v[RC][W][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Part* parts = static_cast<const Part*>(p.workspace);
@@ -865,54 +862,79 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_join_kernel(K
   constexpr int kSlot = ROWS * (D + 2);
   const Part part = parts[blockIdx.x];
   if (part.count == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = warp / kJoinWarps, w = warp % kJoinWarps;
-  const int row = blockIdx.y * kJoinRows + r0;
-  auto base = [&](int i) { return sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot; };
-  // the lane's part of each 32: its reference and l, then its factor
-  float top = -INFINITY;
-  for (int i = lane; i < part.count; i += 32) top = fmaxf(top, base(i)[ROWS * D + 2 * row]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = warp / W, w = warp % W;
+  const int row = blockIdx.y * RC + r0;
   constexpr int V = D == 64 ? 2 : 4, E = D / (32 * V);  // values of a load, loads of a row
-  float sum = 0.f, v[E][V];
+  constexpr int U = 8 / E;                              // parts in flight
+  float top = -INFINITY, sum = 0.f, v[E][V];
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int k = 0; k < V; ++k) v[e][k] = 0.f;
-#pragma unroll 8
-  for (int i = w; i < part.count; i += kJoinWarps) {
-    const float* s = base(i);
-    const float2 num = *reinterpret_cast<const float2*>(s + ROWS * D + 2 * row);
-    const float f = num.x == -INFINITY ? 1.f : ex2(num.x - top);  // no reference: sums of 0, or of NaN
-    sum = fmaf(num.y, f, sum);
+  for (int i0 = w; i0 < part.count; i0 += W * U) {
+    float2 num[U];
+    float x[U][E][V];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float x[V];
-      const float* src = s + row * D + (e * 32 + lane) * V;
-      if constexpr (V == 4)
-        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
-      else
-        *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * W, part.count - 1);  // one that counts, read again
+      const float* s = sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot;
+      num[u] = *reinterpret_cast<const float2*>(s + ROWS * D + 2 * row);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[e][k] = fmaf(x[k], f, v[e][k]);
+      for (int e = 0; e < E; ++e) {
+        const float* src = s + row * D + (e * 32 + lane) * V;
+        if constexpr (V == 4)
+          *reinterpret_cast<float4*>(x[u][e]) = *reinterpret_cast<const float4*>(src);
+        else
+          *reinterpret_cast<float2*>(x[u][e]) = *reinterpret_cast<const float2*>(src);
+      }
+    }
+    float now = top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) now = fmaxf(now, num[u].x);
+    const float f0 = top == -INFINITY ? 1.f : ex2(top - now);  // no reference: sums of 0, or of NaN
+    top = now;
+    sum *= f0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[e][k] *= f0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * W >= part.count) break;
+      const float f = num[u].x == -INFINITY ? 1.f : ex2(num[u].x - top);
+      sum = fmaf(num[u].y, f, sum);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[e][k] = fmaf(x[u][e][k], f, v[e][k]);
     }
   }
-  if (lane == 0) s_sum[r0][w] = sum;
+  if (lane == 0) {
+    s_num[r0][w][0] = top;
+    s_num[r0][w][1] = sum;
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int k = 0; k < V; ++k) s_v[r0][w][(e * 32 + lane) * V + k] = v[e][k];
   __syncthreads();
   if (row >= part.rows) return;
+  float f[W];
+  top = -INFINITY;
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) sum += s_sum[r0][i];
+  for (int i = 0; i < W; ++i) top = fmaxf(top, s_num[r0][i][0]);
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    f[i] = s_num[r0][i][0] == -INFINITY ? 1.f : ex2(s_num[r0][i][0] - top);
+    sum = fmaf(s_num[r0][i][1], f[i], sum);
+  }
   const int per = p.q_heads / p.cache.kv_heads, q = part.row0 + row;
   const long long at = (long long)(part.token + q / per) * p.o_stride + (long long)(part.head * per + q % per) * D;
-  for (int d = w * 32 + lane; d < D; d += kJoinWarps * 32) {
+  for (int d = w * 32 + lane; d < D; d += W * 32) {
     float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) x += s_v[r0][i][d];
+    for (int i = 0; i < W; ++i) x = fmaf(s_v[r0][i][d], f[i], x);
     store_any(p.o, at + d, dtype, sum == 0.f ? 0.f : x / sum);
   }
 }
@@ -951,10 +973,25 @@ cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t s
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, G, ROWS>, p, dtype);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3((unsigned)ctas, ROWS / kJoinRows);
-  cfg.blockDim = dim3(kJoinRows * kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, ROWS>, p, dtype);
+  // Parts that a tile may have, by the table's reach and the CTAs: many want more warps a row (1 x 131072,
+  // 56 parts: 3.8 us with 4, 2.3 with 8; 8 x 2000, 7 parts: 0.6 us less with 4), many tiles want fewer
+  // CTAs, most of which have nothing to do (48 x 4096: 1 us less with four rows a CTA than with two).
+  const long long tiles = ((long long)p.tokens * (p.q_heads / p.cache.kv_heads) / ROWS + p.batch) * p.cache.kv_heads;
+  const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost;
+  if (tiles <= sm_count && std::min(steps, ctas / tiles) > 16) {
+    cfg.gridDim = dim3((unsigned)ctas, ROWS / 2);
+    cfg.blockDim = dim3(2 * 8 * 32);
+    return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, ROWS, 2, 8>, p, dtype);
+  }
+  if (tiles <= sm_count) {
+    cfg.gridDim = dim3((unsigned)ctas, ROWS / 2);
+    cfg.blockDim = dim3(2 * 4 * 32);
+    return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, ROWS, 2, 4>, p, dtype);
+  }
+  cfg.gridDim = dim3((unsigned)ctas, ROWS / 4);
+  cfg.blockDim = dim3(4 * 2 * 32);
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, ROWS, 4, 2>, p, dtype);
 }
 
 }  // namespace
