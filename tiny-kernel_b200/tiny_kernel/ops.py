@@ -13,11 +13,12 @@ from ._lib import Int4MatrixC, Kv4CacheC, check
 
 
 def _ptr(v) -> int:
+    try:
+        return v.data_ptr()
+    except AttributeError:
+        pass
     if v is None or type(v) is int:
         return v
-    at = getattr(v, "data_ptr", None)
-    if at is not None:
-        return at()
     if hasattr(v, "ptr"):
         return v.ptr
     return int(v)
@@ -149,13 +150,33 @@ def _dtype(dtype) -> int:
     return int(dtype)
 
 
+_entries = {}  # name -> (synchronous entry point, queued one)
+
+
+def _number(v):
+    """An argument that ctypes did not take as it was: other kinds of numbers (numpy's)."""
+    if v is None or isinstance(v, (int, float)) or not hasattr(v, "__float__"):
+        return v
+    return int(v) if hasattr(v, "__index__") else float(v)
+
+
 def _call(name, args, stream, sync):
     """The synchronous entry point, or with a stream (or sync=False) the one that only queues."""
-    L = _lib.lib()
-    if sync and stream is None:
-        check(getattr(L, name)(*args))
+    entry = _entries.get(name)
+    if entry is None:
+        L = _lib.lib()
+        entry = _entries[name] = (getattr(L, name), getattr(L, name + "_async"))
+    if stream is None and sync:
+        fn = entry[0]
     else:
-        check(getattr(L, name + "_async")(*args, stream))
+        fn = entry[1]
+        args += (stream,)
+    try:
+        status = fn(*args)
+    except C.ArgumentError:
+        status = fn(*map(_number, args))
+    if status:
+        check(status)
 
 
 def paged_slots(device, context_lens, query_lens, free_blocks, free_range, block_tables, kv_lens,
@@ -165,8 +186,8 @@ def paged_slots(device, context_lens, query_lens, free_blocks, free_range, block
     _call("tk_paged_slots",
           (_dev(device), _ptr(context_lens), _ptr(query_lens), _ptr(free_blocks), _ptr(free_range),
            _ptr(block_tables), _ptr(kv_lens), _ptr(query_start), _ptr(positions), _ptr(slots),
-           _ptr(counts), int(batch), int(max_blocks), int(block_size), int(num_blocks),
-           int(max_tokens)), stream, sync)
+           _ptr(counts), batch, max_blocks, block_size, num_blocks,
+           max_tokens), stream, sync)
 
 
 def qk_norm_rope(device, q, k, q_weight, k_weight, cos_cache, sin_cache, positions, q_out, k_out,
@@ -176,9 +197,9 @@ def qk_norm_rope(device, q, k, q_weight, k_weight, cos_cache, sin_cache, positio
     """Per-head norm (a None weight: none) and rotation of queries and keys at their positions."""
     _call("tk_qk_norm_rope",
           (_dev(device), _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), _ptr(cos_cache),
-           _ptr(sin_cache), _ptr(positions), _ptr(q_out), _ptr(k_out), int(tokens), int(q_heads),
-           int(kv_heads), int(head_dim), int(rot_dim), int(max_pos), int(q_stride), int(k_stride),
-           int(q_out_stride), int(k_out_stride), float(eps), _dtype(dtype),
+           _ptr(sin_cache), _ptr(positions), _ptr(q_out), _ptr(k_out), tokens, q_heads,
+           kv_heads, head_dim, rot_dim, max_pos, q_stride, k_stride,
+           q_out_stride, k_out_stride, eps, _dtype(dtype),
            _lib.TK_ROPE_INTERLEAVED if interleaved else 0), stream, sync)
 
 
@@ -193,16 +214,16 @@ def kv4_append(device, cache, k, v, slots, tokens, dtype="f32", k_stride=0, v_st
                sync=True):
     """Keys and values quantised into their slots (-1: not written)."""
     _call("tk_kv4_append",
-          (_dev(device), C.byref(cache), _ptr(k), _ptr(v), _ptr(slots), int(tokens), int(k_stride),
-           int(v_stride), _dtype(dtype)), stream, sync)
+          (_dev(device), C.byref(cache), _ptr(k), _ptr(v), _ptr(slots), tokens, k_stride,
+           v_stride, _dtype(dtype)), stream, sync)
 
 
 def kv4_gather(device, cache, slots, k, v, tokens, dtype="f32", k_stride=0, v_stride=0, stream=None,
                sync=True):
     """Keys and values of slots read back from the cache (-1: the row stays)."""
     _call("tk_kv4_gather",
-          (_dev(device), C.byref(cache), _ptr(slots), _ptr(k), _ptr(v), int(tokens), int(k_stride),
-           int(v_stride), _dtype(dtype)), stream, sync)
+          (_dev(device), C.byref(cache), _ptr(slots), _ptr(k), _ptr(v), tokens, k_stride,
+           v_stride, _dtype(dtype)), stream, sync)
 
 
 def kv4_attention_workspace(device, cache, q_heads) -> int:
@@ -219,8 +240,8 @@ def kv4_attention(device, cache, q, block_tables, kv_lens, query_start, o, works
     """Attention of the step's queries over the 4-bit pages (query_start None: one token each)."""
     _call("tk_kv4_attention",
           (_dev(device), C.byref(cache), _ptr(q), _ptr(block_tables), _ptr(kv_lens),
-           _ptr(query_start), _ptr(o), _ptr(workspace), int(workspace_bytes), int(tokens),
-           int(batch), int(q_heads), int(max_blocks), int(q_stride), int(o_stride), float(scale),
+           _ptr(query_start), _ptr(o), _ptr(workspace), workspace_bytes, tokens,
+           batch, q_heads, max_blocks, q_stride, o_stride, scale,
            _dtype(dtype)), stream, sync)
 
 
