@@ -327,8 +327,8 @@ int tk_paged_attention_async(tk_device *dev, const float *q, const float *k_cach
  *             scales f16 [block][kv_head][block_size][head_dim/group_size][2], (scale, offset);
  *             value = code * scale + offset.
  * block_size 16, 32, 64, 128 or 256; head_dim 64, 128 or 256; group_size 64 or 128, at most
- * head_dim; num_blocks * block_size < 2^31; the four arrays on 16-byte boundaries.  A slot is
- * block * block_size + token within the block. */
+ * head_dim; kv_heads at most 4096; num_blocks * block_size < 2^31; the four arrays on 16-byte
+ * boundaries.  A slot is block * block_size + token within the block. */
 #define TK_F32 0
 #define TK_F16 1
 #define TK_BF16 2
@@ -424,8 +424,10 @@ int tk_kv4_gather_async(tk_device *dev, const tk_kv4_cache *cache, const int32_t
  * ranges must not overlap; rows of no sequence are left as they were, and what the cache holds at
  * positions that a query does not see does not matter.  A query that sees nothing gives zeros.
  * kv_lens past max_blocks * block_size (below 2^31 - 1024) is cut there; a page whose id is outside
- * [0, num_blocks) counts as absent.  Products and sums hold f32 precision for every dtype and do
- * not depend on the run (fixed order); scale * q may reach 2^118.
+ * [0, num_blocks) counts as absent.  For every dtype the queries enter with 22 bits of their row's
+ * largest magnitude, the weights with 22 bits, sums are f32 and do not depend on the run (fixed
+ * order).  Scores have to fit f32; a query row that holds an infinity or a NaN gives NaN.
+ * tokens * q_heads at most 2^30.
  * workspace: tk_kv4_attention_workspace bytes of device memory on a 16-byte boundary, not
  * initialised, for calls that do not run at the same time. */
 int tk_kv4_attention_workspace(tk_device *dev, const tk_kv4_cache *cache, uint32_t q_heads,

@@ -13,7 +13,8 @@ namespace tk {
 namespace {
 
 // Programmatic launches: a kernel is set up while the one before it in the stream runs; it reads
-// nothing, and no thread of it ends, before that one has completed.
+// nothing, and no thread of it ends, before that one has completed.  It reads nothing through the
+// read-only path (__ldg) either, which holds only for what no kernel writes once it has been set up.
 __device__ __forceinline__ void after_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, i
     if (vec_turn && (MODE != kPairs || l * E + E <= p.rot_dim)) {  // by pairs on 8-byte boundaries
 #pragma unroll
       for (int e = 0; e < A; e += 2) {
-        const float2 cv = __ldg(reinterpret_cast<const float2*>(cp + e)), sv = __ldg(reinterpret_cast<const float2*>(sp + e));
+        const float2 cv = *reinterpret_cast<const float2*>(cp + e), sv = *reinterpret_cast<const float2*>(sp + e);
         c[e] = cv.x, c[e + 1] = cv.y;
         s[e] = sv.x, s[e + 1] = sv.y;
       }
@@ -412,8 +413,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, i
 #pragma unroll
       for (int e = 0; e < A; ++e)
         if (j0 + e < half) {
-          c[e] = __ldg(cp + e);
-          s[e] = __ldg(sp + e);
+          c[e] = cp[e];
+          s[e] = sp[e];
         }
     }
     if constexpr (MODE == kPart) {
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p, i
   float w[E];
 #pragma unroll
   for (int e = 0; e < E; ++e)
-    w[e] = wp && holds ? __ldg(wp + (MODE == kHalves ? (e / H) * (D / 2) + l * H + e % H : l * E + e)) : 1.f;
+    w[e] = wp && holds ? wp[MODE == kHalves ? (e / H) * (D / 2) + l * H + e % H : l * E + e] : 1.f;
 
   T* out = static_cast<T*>(p.out[which]) + token * p.out_stride[which] + (long long)h0 * D;
 #pragma unroll

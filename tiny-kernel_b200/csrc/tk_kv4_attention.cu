@@ -20,10 +20,15 @@
 // product each.
 //   Tiles of four rows (one token of up to four heads a group) put two digits, and both f16 parts of a
 // weight, next to each other in the 8 columns: 2 + 1 products instead of 3 + 2, and a lane has half
-// the scores (one token of a unit instead of two).  1 x 131072 and 48 x 8192 with four heads a group:
-// see attention_rows.
-// mma.sync and not tcgen05: one token of a head group is at most 8 rows, an eighth of tcgen05's
-// smallest tile, whose operands would also have to pass through shared memory unpacked.
+// the scores (one token of a unit instead of two).
+// mma.sync and not tcgen05: one token of a head group is 1 to 8 rows, and tcgen05's operands would have
+// to pass through shared memory unpacked (384 bytes a token and head against the 132 that are read).
+//
+// What bounds it (B200, four heads a group, head dimension 128, group 128): 524288 positions take 128 us,
+// 4.5 TB/s of the 6.5 that a copy reaches.  Without its loads the same arithmetic runs at 6.4 TB/s of
+// codes, the loads without arithmetic at 5.3, and 12 warps on an SM overlap them only in part; 16 warps
+// of 128 registers spill (48 x 4096: 65 us instead of 58).  A short call is 9 us of waits one after the
+// other: lengths, block table, first pages, the end of the tile, the second kernel.
 //
 // Softmax in base 2 with a running reference per row: w = 2^(s - r) s_v must fit f16, so r follows
 // max(s + log2 s_v) and is moved (sums rescaled) only when a weight would leave [0, 2^15].
@@ -31,9 +36,11 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
+#include "tk_internal.h"
 #include "tk_kv4.h"
 
 namespace tk {
@@ -41,27 +48,28 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kCols = 8;       // columns of a product; a tile has 8 rows (query token, head of the group) or 4
-constexpr int kUnit = 16;      // tokens that lie in one page for sure
-constexpr int kSub = 2;        // units of a warp's step
+constexpr int kCols = 8;   // columns of a product; a tile has 8 rows (query token, head of the group) or 4
+constexpr int kUnit = 16;  // tokens that lie in one page for sure
+constexpr int kSub = 2;    // units of a warp's step, which share one reference and its reduction
 constexpr int kTokens = kUnit * kSub;
 constexpr int kStep = kTokens * kWarps;
+constexpr int kStages = 2;  // steps of a warp's ring: one computed, one on its way (three: 0 to 4 % slower)
 template <int D>
-constexpr int kRing = 2;  // stages of a warp's ring
-template <int D>
-constexpr int kResident = D == 256 ? 2 : 3;  // CTAs of an SM
-constexpr int kFlush = 16;     // steps between two settings aside of the sums
-constexpr int kMinRun = 1;
-constexpr int kTileCost = 2;   // steps that a tile costs beside its own: queries, first loads, join
+constexpr int kResident = D == 256 ? 2 : 3;  // CTAs of an SM: 255 or 168 registers a thread
+constexpr int kFlush = 16;                   // steps between two settings aside of the sums
+// Steps that a tile costs beside its own: queries, first loads, join (48 sequences of 64 to 8192: 65.3 us
+// with 1, 61.6 with 2, 60.6 with 3; 32 of 512: 15.2, 15.5, 17.5).
+constexpr int kTileCost = 2;
 
 // Work is (sequence, key head, row tile, step of 128 tokens) in this order, cut into equal runs, one
-// per CTA; a tile counts kTileCost steps more than it has, before its first.  A run that ends inside a (sequence, head, tile) leaves its sums in the
-// workspace; the CTA in whose run the tile begins describes it, and a second kernel joins the parts
-// in the order of the CTAs.  A CTA has at most two parts: the end of a tile in slot 0, the beginning
-// of one in slot 1.
+// per CTA; a tile counts kTileCost steps more than it has, before its first.  So long and short
+// sequences, few and many, load the SMs alike, whatever the lengths, which only the device knows.  A
+// run that ends inside a tile leaves its sums in the workspace; the CTA in whose run the tile begins
+// describes it, and a second kernel joins the parts in the order of the CTAs.  A CTA has at most two
+// parts: the end of a tile in slot 0, the beginning of one in slot 1.
 struct Part {
-  int token, rows, head, count;  // first row's query token... of the tile; parts to join (0: none)
-  int row0, slot, pad0, pad1;    // first row of the tile; the slot of the first part
+  int token, rows, head, count;  // of the tile: the sequence's first query token, rows, key head; its parts (0: none)
+  int row0, slot, pad0, pad1;    // the tile's first row; the slot of the first part
 };
 
 size_t part_bytes(int head_dim) { return (size_t)kCols * (head_dim + 2) * sizeof(float); }
@@ -246,7 +254,7 @@ struct Smem {
   static constexpr int kQuery = D / 32 * 32 * kLaneWords * 4;
   static constexpr int kRowWords = 1 + 4 * S::NG;  // unscale; sum, three centres a group
   static constexpr int kRowBytes = kCols * kRowWords * 4;
-  static constexpr int kWarp = kRing<D> * S::kBytes;
+  static constexpr int kWarp = kStages * S::kBytes;
   static constexpr int kJoint = D + 1;                     // floats of a row of sums at the end
   static constexpr int kJointWarp = kCols * (kJoint + 2);  // and per row the reference and l
   static constexpr int kRings = kQuery + kRowBytes, kJoints = kRings + kWarps * kWarp;
@@ -260,13 +268,14 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
   using M = Smem<D, G, ROWS>;
   constexpr bool kFour = ROWS == 4;
   constexpr int J = kFour ? 1 : 2;  // tokens of a unit that a lane has scores of
-  constexpr int kStages = kRing<D>;
   constexpr int NG = S::NG, NT = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ long long s_warp[kWarps];
   __shared__ long long s_at;
   __shared__ int s_seq;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing is read before the kernels before have completed
+  // Nothing is read before the kernels before have completed; and nothing through the read-only path
+  // (__ldg), which holds only for what no kernel writes once this one has been set up.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per = p.q_heads / p.cache.kv_heads, hk = p.cache.kv_heads;
@@ -297,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
     total += s_warp[w];
   }
   // (a quotient in f64, rounded up at least: 64-bit division takes as long as a load)
-  const long long run = max((long long)__dmul_ru((double)total, p.inv_ctas) + 1, (long long)kMinRun);
+  const long long run = (long long)__dmul_ru((double)total, p.inv_ctas) + 1;
   const long long start = run * blockIdx.x, stop = min(start + run, total);
   if (tid == 0) parts[blockIdx.x].count = 0;
   if (start >= stop) return;
@@ -364,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
       const int pos = step * kStep + warp * kTokens + u * kUnit;
-      page[u] = step < s1 && pos < see_most ? __ldg(table + (pos >> p.cache.shift)) : -1;
+      page[u] = step < s1 && pos < see_most ? table[pos >> p.cache.shift] : -1;
     }
   };
   auto issue = [&](int stage, int step) {
@@ -939,8 +948,9 @@ __global__ void __launch_bounds__(RC * W * 32) kv4_join_kernel(Kv4AttentionParam
   }
 }
 
-// Rows of a tile: four where a sequence has about as many (its query tokens are not known here, their
-// mean is), eight otherwise.
+// Rows of a tile: four where a sequence has as many on the mean (its own query tokens are not known
+// here), eight otherwise: with four heads a group, 48 x 4096 58 us instead of 68, 524288 128 instead of
+// 146; with eight, four-row tiles would read the cache twice.
 int attention_rows(const Kv4AttentionParams& p) {
   const long long per = p.q_heads / p.cache.kv_heads;
   return p.tokens * per <= 4ll * p.batch ? 4 : 8;
@@ -951,11 +961,17 @@ int attention_ctas(int head_dim, int sm_count) { return sm_count * (head_dim == 
 template <int D, int G, int ROWS>
 cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t st) {
   const size_t smem = Smem<D, G, ROWS>::kBytes;
-  cudaError_t e;
-  if (smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(kv4_attention_kernel<D, G, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
+  // shared memory above 48 KB is asked for once per device (and again in a new context of it)
+  constexpr int kMaxDevices = 64;
+  static std::atomic<unsigned> asked[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned gen = attr_generation(dev) + 1;
+  if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
+    e = cudaFuncSetAttribute(kv4_attention_kernel<D, G, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
   }
   // programmatic launches: a kernel is set up while the one before it runs, and passes its wait when
   // that has completed

@@ -1558,7 +1558,7 @@ int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* 
   if (!aligned_for(q, dtype) || !aligned_for(o, dtype)) return fail(TK_ERR_ARG, "q or o is not aligned to its type");
   if (!aligned16(workspace)) return fail(TK_ERR_ARG, "the workspace must be on a 16-byte boundary");
   if (batch == 0 || batch > (1u << 24) || max_blocks == 0 || max_blocks > kMaxCount || tokens > kMaxCount ||
-      (uint64_t)tokens * q_heads > kMaxCount)
+      (uint64_t)tokens * q_heads > (1u << 30))
     return fail(TK_ERR_ARG, "%u tokens of %u heads in %u sequences of %u blocks are out of range", tokens, q_heads,
                 batch, max_blocks);
   if ((uint64_t)max_blocks * cache->block_size > kMaxCount - 1024)
