@@ -638,3 +638,55 @@ def test_no_tokens_is_no_launch(torch_cuda, tkdev):
     ops.kv4_append(tkdev, cache, c.q, c.q, c.dev_args[1], 0)
     ops.kv4_attention(tkdev, cache, c.q, *c.dev_args[:2], c.dev_args[1], c.o, c.ws, c.ws_size, 0, 1, 1, c.width, 1.0)
     assert tkdev.launch_count() == before
+
+
+def test_kernel_classes(torch_cuda, tkdev):
+    """The classes over the framework's own buffers: a prompt, then one token, against the oracle."""
+    import tiny_kernel as tk
+    hq, hk, dim, bs, width, tokens = 4, 2, 64, 16, 3, 20
+    rng = np.random.default_rng(31)
+    buf = lambda x, t: tkdev.create_buffer_with_data(t, x)
+    new = lambda n, t: tkdev.create_buffer_with_data(t, np.zeros(n))
+    slots_of, qk = tk.kernels.kv4.PagedSlots.init(tkdev), tk.kernels.kv4.QKNormRoPE.init(tkdev)
+    cache = tk.kernels.kv4.KV4Cache.init(tkdev, 4, hk, bs, dim, 64)
+    angles = np.arange(width * bs)[:, None] * 10000.0 ** -(np.arange(dim // 2) / (dim // 2))
+    cos, sin = np.cos(angles).astype(np.float32), np.sin(angles).astype(np.float32)
+    w = rng.uniform(0.5, 1.5, dim).astype(np.float32)
+    tables, free = buf(np.full(width, -1), "i32"), buf([3, 1, 0], "i32")
+    held, ctx, taken = [np.zeros((0, hk, dim))] * 2, 0, 0
+    for n in (tokens, 1):
+        kv, start, pos, slots, counts = (new(m, "i32") for m in (1, 2, n, n, 4))
+        slots_of.forward(buf([ctx], "i32"), buf([n], "i32"), free, buf([taken, 3], "i32"), tables, kv, start, pos, slots,
+                         counts, bs, 4)
+        taken += int(counts.slice()[1])
+        assert pos.slice().tolist() == list(range(ctx, ctx + n)) and kv.slice().tolist() == [ctx + n]
+        q, k, v = (rng.standard_normal((n, h, dim)).astype(np.float32) for h in (hq, hk, hk))
+        qo, ko = new(q.size, "f32"), new(k.size, "f32")
+        qk.forward(buf(q, "f32"), buf(k, "f32"), buf(w, "f32"), None, buf(cos, "f32"), buf(sin, "f32"), pos, qo, ko, hq, hk,
+                   dim, dim, width * bs, 1e-5)
+        qr, kr = qo.slice().reshape(n, hq, dim).copy(), ko.slice().reshape(n, hk, dim).copy()
+        norm = np.sqrt((q.astype(np.float64) ** 2).mean(-1, keepdims=True) + 1e-5)
+        y = q / norm * w
+        a, b = y[..., :dim // 2], y[..., dim // 2:]
+        c, s = (x[ctx:ctx + n, None].astype(np.float64) for x in (cos, sin))
+        # at most 64 roundings in the sum of squares (half of it in the root) and 5 more, over sqrt(2) |y|
+        atol = 37 * 2.0**-24 * 2**0.5 * np.abs(y).max()
+        assert np.allclose(qr, np.concatenate([a * c - b * s, b * c + a * s], -1), rtol=0, atol=atol)
+        cache.append(ko, buf(v, "f32"), slots)
+        kb, vb = new(k.size, "f32"), new(k.size, "f32")
+        cache.gather(slots, kb, vb)
+        for i, x in enumerate((kr, v)):
+            held[i] = np.concatenate([held[i], oracle4.values_f64(*oracle4.quantise(x, 64))])
+        assert np.array_equal(kb.slice().reshape(k.shape), held[0][ctx:].astype(np.float32))
+        assert np.array_equal(vb.slice().reshape(v.shape), held[1][ctx:].astype(np.float32))
+        o = new(q.size, "f32")
+        cache.forward(qo, tables, kv, start, o, hq, dim ** -0.5)
+        ctx += n
+        pad = -ctx % bs
+        kp, vp = (np.pad(x, ((0, pad), (0, 0), (0, 0))).reshape(-1, bs, hk, dim).transpose(0, 2, 1, 3) for x in held)
+        want, bound = oracle4.attention_f64(qr.astype(np.float64), kp, vp, 3 * np.abs(kp).max() + 0 * kp,
+                                            3 * np.abs(vp).max() + 0 * vp, np.arange(kp.shape[0])[None], [ctx], [0, n],
+                                            dim ** -0.5, bs)
+        off = np.abs(o.slice().reshape(want.shape) - want)
+        assert (off <= bound + 2.0**-24 * np.abs(want) + 2.0**-149).all()
+    cache.deinit()

@@ -5,6 +5,7 @@ pub const cuda = @import("cuda/cuda.zig");
 pub const quantized = @import("kernels/quantized.zig");
 pub const fused = @import("kernels/fused.zig");
 pub const rmsnorm = @import("kernels/rmsnorm.zig");
+pub const kv4 = @import("kernels/kv4.zig");
 
 pub const Device = cuda.Device;
 pub const Buffer = cuda.Buffer;
