@@ -408,6 +408,101 @@ def test_attention(torch_cuda, tkdev, n, dtype):
     c.check(c.run(tkdev, c.upload()))
 
 
+# many rows a sequence, one group a head: the kernel for prompts where the queries have 16 bits
+PROMPTS = [
+    ([128], [128], 1, 1, 128, 128, 16),                      # one full tile, one step
+    ([1], [1], 40, 1, 64, 64, 16),                           # one token in all
+    ([129, 300], [129, 33], 4, 4, 64, 64, 16),               # a row and a step more than full ones
+    ([700, 130], [130, 33], 7, 1, 128, 128, 32),
+    ([1000, 17, 0, 400], [100, 17, 0, 1], 10, 2, 128, 128, 64),  # a prompt, one token, no request
+    ([50, 2, 0, 9], [60, 40, 3, 9], 8, 8, 128, 128, 16),     # queries before the first position
+    ([2500], [70], 16, 1, 64, 64, 256),                      # many CTAs to a tile
+    ([300] * 20, [40] * 20, 4, 4, 64, 64, 16),
+    ([5200] * 4, [130] * 4, 16, 16, 64, 64, 32),             # runs long enough for sums to be set aside
+    ([4600, 4300, 4400], [257, 256, 140], 10, 10, 128, 128, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", range(len(PROMPTS)))
+def test_attention_of_prompts(torch_cuda, tkdev, n, dtype):
+    if dtype == "f32" and n >= 8:
+        pytest.skip("the same kernel as shorter ones")
+    c = Case(torch_cuda, 40 + n, *PROMPTS[n], dtype)
+    c.check(c.run(tkdev, c.upload()))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_with_absent_pages_and_anything_in_masked_places(torch_cuda, tkdev, dim):
+    """Pages that are not in the cache (more than a step of them, and the whole of a sequence), and
+    NaN and infinities in scales behind the last token, in pages of nobody and in the last query's own
+    position, which only it sees."""
+    c = Case(torch_cuda, 61, [700, 2500, 40], [100, 40, 40], 4, 2, dim, dim, 16, "f16")
+    c.tables[0, 3:14] = -1
+    c.tables[1, :140] = c.blocks
+    c.tables[2, :] = [-5, 2**31 - 1, -2**31] + [-1] * (c.width - 3)
+    for part in c.parts:
+        for b, n in enumerate(c.kv_lens):
+            page = c.tables[b, n // 16]
+            if 0 <= page < c.blocks:
+                part[1][page, :, n % 16:], part[2][page, :, n % 16:] = np.nan, np.inf
+        part[1][np.setdiff1d(np.arange(c.blocks), c.tables)] = np.inf
+    o = c.run(tkdev, c.upload())
+    c.check(o)
+    assert not o[140:].any()
+    last = c.tables[0, 699 // 16]
+    c.parts[1][1][last, :, 699 % 16] = np.inf
+    c.parts[0][2][last, :, 699 % 16] = np.nan
+    p = c.run(tkdev, c.upload())
+    assert torch_cuda.isnan(p[99]).all() and torch_cuda.equal(p[:99], o[:99]) and torch_cuda.equal(p[100:], o[100:])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_prompts_in_place_strided_and_repeated(torch_cuda, tkdev, dtype):
+    """Rows of a projection apart and off the 16-byte boundary, output over the queries; the same bits
+    from run to run, and rows of no sequence left as they were."""
+    torch = torch_cuda
+    c = Case(torch, 62, [900, 333], [90, 40], 6, 2, 64, 64, 16, dtype)
+    cache = c.upload()
+    first = c.run(tkdev, cache).clone()
+    for _ in range(3):
+        assert torch.equal(c.run(tkdev, cache), first)
+    wide = torch.full((135, 6 * 64 + 3), 9.0, dtype=c.q.dtype, device="cuda")
+    wide[2:132, 1:385] = c.q.view(130, 384)
+    c.dev_args[2] = i32(torch, [2, 92, 132])
+    row = wide[:, 1:]
+    torch.cuda.synchronize()
+    ops.kv4_attention(tkdev, cache, row, *c.dev_args, row, c.ws, c.ws_size, 135, 2, 6, c.width, c.scale, dtype,
+                      q_stride=387, o_stride=387)
+    assert torch.equal(wide[2:132, 1:385], first.view(130, 384))
+    wide[2:132, 1:385] = 9
+    assert (wide == 9).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_prompts_with_scales_of_every_kind(torch_cuda, tkdev, dtype):
+    """Scales of 0, of either sign, the smallest subnormal and sizes far apart; queries of every size;
+    a row of queries with an infinity gives NaN and no other row does."""
+    c = Case(torch_cuda, 63, [600, 200], [64, 40], 2, 1, 128, 128, 16, dtype)
+    rng = np.random.default_rng(63)
+    for part in c.parts:
+        some = rng.integers(0, 8, part[1].shape)
+        part[1][some == 0] = 0
+        part[1][some == 1] *= -1
+        part[1][some == 2] = 2.0**-24
+        part[1][some == 3] *= np.float16(2.0**-9)
+        part[2][some == 2] = 0.25
+    c.q[::7] *= 1e-3
+    c.q[::11] *= 6
+    o = c.run(tkdev, c.upload()).clone()
+    c.check(o)
+    c.q[70, 1, 5] = float("inf")
+    p = c.run(tkdev, c.upload())
+    assert torch_cuda.isnan(p[70, 1]).all()
+    p[70, 1] = o[70, 1]
+    assert torch_cuda.equal(p, o)
+
+
 def test_attention_repeats_bit_for_bit(torch_cuda, tkdev):
     c = Case(torch_cuda, 3, [3000, 17, 900], [1, 4, 2], 8, 2, 128, 128, 16, "f32")
     cache = c.upload()

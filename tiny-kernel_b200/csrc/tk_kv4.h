@@ -149,6 +149,8 @@ struct Kv4AttentionParams {
   int tokens, batch, q_heads, max_blocks;
   float scale;
   double inv_ctas;  // 1 / CTAs, set at the launch
+  unsigned* err;    // the device's error word, and how long a wait of a kernel may take
+  unsigned long long timeout_ns;
 };
 size_t kv4_attention_workspace(int head_dim, int sm_count);
 cudaError_t launch_kv4_attention(const Kv4AttentionParams& p, int dtype, int sm_count,

@@ -1,0 +1,532 @@
+// tk_kv4_prompt.cu -- attention over the 4-bit cache for many query rows a key head: prompts and
+// their chunks.
+//
+// The mathematics is that of tk_kv4_attention.cu, with one group a head and queries of 16 bits, and
+// the products on tcgen05: a tile is 128 rows (query token, head of the group) against 128 tokens a
+// step.
+//   S = Q (c - 8)^T    Q as it is (f16 or bf16), the codes exact in either
+//   t = a S + b sum(q) + log2 |s_v|      a = f s_k, b = f (m_k + 8 s_k), f = scale log2 e
+//   w = 2^(t - r),  O += w sign(s_v) (c - 8),  l += w / |s_v|,  off += w (m_v + 8 s_v) / |s_v|
+// and o = (O + off) / l.  So a weight comes out of the exponential with its scale in it, ready for
+// the second product; it is split into two f16 (22 bits), two products into one accumulator.
+// s_v = 0 counts as 1 with values of 0.  The reference r of a row keeps the weights below 2^15 and is
+// moved down from there to 2^10 when one would pass; the sums are rescaled then, which is rare.
+//
+// One CTA is 256 threads, two a row: tokens 0-63 and 64-127 of a step, and half of the dimensions of
+// O.  Tensor memory: S (128 columns), over which the weights lie as f16 pairs once all of S has been
+// read, and O.  A step is one chain (unpack keys, S, weights, O), so two CTAs live on an SM, one
+// computing while the other's products run; the next step's codes travel in registers meanwhile.
+// The tensor core's sums round toward zero: O is set aside into the CTA's slot of the workspace, in
+// f32 additions, every kFlush steps.
+#include <algorithm>
+#include <atomic>
+
+#include "tk_internal.h"
+#include "tk_kv4_attention.cuh"
+#include "tk_ptx.cuh"
+
+namespace tk {
+namespace {
+
+constexpr int kRows = 128, kThreads = 256, kFlush = 16, kCtasPerSm = 2;
+constexpr uint32_t kTmemCols = 256, kTmemO = 128, kTmemLow = 64;  // S and the weights' high parts at 0
+constexpr unsigned kErrWait = 4u;                                  // a product never completed
+
+// Waits for the phase of `bar`; gives up, for good, after timeout_ns.
+__device__ __forceinline__ void wait_products(uint64_t* bar, uint32_t& phase, bool& dead, const Kv4AttentionParams& p) {
+  if (!dead && !mbar_try_wait(bar, phase)) {
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait(bar, phase))
+      if (global_timer_ns() - t0 > p.timeout_ns) {
+        atomicOr(p.err, kErrWait);
+        dead = true;
+        break;
+      }
+  }
+  phase ^= 1;
+  tcgen05_fence_after();
+}
+
+#define TK_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+#define TK_R16(r, i) TK_R4(r, i), TK_R4(r, i + 4), TK_R4(r, i + 8), TK_R4(r, i + 12)
+#define TK_V4(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3])
+// 64 (16) consecutive columns of the warp's 32 lanes, complete on return.
+__device__ __forceinline__ void tmem_load64(uint32_t at, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, "
+      "%36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, "
+      "%57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+      : TK_R16(r, 0), TK_R16(r, 16), TK_R16(r, 32), TK_R16(r, 48)
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : TK_R16(r, 0)
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(at),
+      TK_V4(r, 0), TK_V4(r, 4), TK_V4(r, 8), TK_V4(r, 12)
+      : "memory");
+}
+#undef TK_R4
+#undef TK_R16
+#undef TK_V4
+
+// Eight codes less 8 from a word of them, times m: f16, or bf16 (m = 1).  The bits 0x6400 | c are the
+// f16 1024 + c, 0x4300 | c the bf16 128 + c; both differences are exact.
+__device__ __forceinline__ uint4 codes_f16(uint32_t w, uint32_t m, uint32_t shift) {  // shift: -1032 m
+  const uint32_t w4 = w >> 4;
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = (__byte_perm(w, w4, 0x4400 + i * 0x1111) & 0x000F000Fu) | 0x64006400u;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y[i]) : "r"(x), "r"(m), "r"(shift));
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
+}
+__device__ __forceinline__ uint4 codes_bf16(uint32_t w) {
+  const uint32_t w4 = w >> 4;
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = (__byte_perm(w, w4, 0x4400 + i * 0x1111) & 0x000F000Fu) | 0x43004300u;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(y[i]) : "r"(x), "r"(0x3F803F80u), "r"(0xC308C308u));  // 1, -136
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
+}
+
+// Operands in shared memory: rows of 64 values (128 bytes), their 16-byte pieces turned by the row's
+// number; heads of 128 dimensions as two halves.  Keys and queries [half][row], values by eights of
+// tokens [token / 8][half][token % 8].
+template <int D>
+struct PromptSmem {
+  static constexpr int kOperand = kRows * D * 2;
+  static constexpr int kQ = 0, kK = kOperand, kV = 2 * kOperand, kNums = 3 * kOperand;
+  // per token a, b, log2 |s_v|, 1 / |s_v|, (m_v + 8 s_v) / |s_v|; per row sum(q), and two halves' numbers twice
+  static constexpr int kBytes = kNums + (5 * kStep + kRows + 4 * kRows) * 4 + 1024;
+};
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4AttentionParams p) {
+  using M = PromptSmem<D>;
+  constexpr int H = D / 64;          // halves of a head, 128 bytes a row
+  constexpr int dtype = BF ? kTypeBF16 : kTypeF16;
+  constexpr int kWords = D / 16;     // of codes of half a head
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t bar;
+  __shared__ uint32_t tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = p.q_heads / p.cache.kv_heads, hk = p.cache.kv_heads;
+  Part* parts = static_cast<Part*>(p.workspace);
+  float* sums = reinterpret_cast<float*>(parts + gridDim.x);
+  constexpr int kSlot = kRows * (D + 2);
+  Run r;
+  Tile cur;
+  if (!find_run<kRows, kThreads>(p, per, parts, r, cur)) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    return;
+  }
+  uint8_t* smem = dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
+  const uint32_t q_at = smem_addr(smem) + M::kQ, k_at = smem_addr(smem) + M::kK, v_at = smem_addr(smem) + M::kV;
+  float* tok_a = reinterpret_cast<float*>(smem + M::kNums);
+  float *tok_b = tok_a + kStep, *tok_l = tok_b + kStep, *tok_i = tok_l + kStep, *tok_v = tok_i + kStep;
+  float* row_sum = tok_v + kStep;
+  float *row_max = row_sum + kRows, *row_num = row_max + 2 * kRows;  // [half][row] each
+  if (tid == 0) {
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) tmem_alloc(&tmem_slot, kTmemCols);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  // Only now: a kernel that is set up early may take tensor memory before its wait, and this one's
+  // blocks have theirs.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  uint32_t phase = 0;
+  bool dead = false;
+
+  // this thread as a loader: half a token's codes (of a row's queries); as a row's: half its tokens
+  const int tok = tid >> 1, part = tid & 1;
+  const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+  const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+  const uint32_t t_s = tmem + lanes + half * 64, t_p = tmem + lanes + half * 32, t_o = tmem + lanes + kTmemO + half * (D / 2);
+  const int page_mask = (1 << p.cache.shift) - 1;
+  const float f = p.scale * 1.4426950408889634f;
+  // where a loader's pieces go: at D = 128 its half's eight, begun with the fourth in the odd lanes, so
+  // that the eight lanes of a store meet in no bank; at D = 64 four of the row's eight
+  const uint32_t piece0 = H == 2 ? part * 4 : 0;
+  auto piece = [&](uint32_t base, int c) {
+    const uint32_t i = H == 2 ? (c ^ piece0) : (uint32_t)(part * 4 + c);
+    return base + ((i ^ (uint32_t)(tok & 7)) << 4);
+  };
+  const uint32_t kq_row = (H == 2 ? part * (kRows * 128) : 0) + tok * 128;
+  const uint32_t v_row = (tok >> 3) * (H * 1024) + (H == 2 ? part * 1024 : 0) + (tok & 7) * 128;
+  auto put = [&](uint32_t at, const uint4& x) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+  };
+
+  long long at = r.start;
+  for (;;) {
+    const int end = cur.s.n * per - 1, row0 = cur.rt * kRows, rows = min(kRows, end + 1 - row0);
+    auto sees = [&](int i) { return min(cur.s.kv, cur.s.last + min(row0 + i, end) / per + 1); };
+    const int see = sees(row), see_least = sees(0), see_most = max(sees(kRows - 1), 0);
+    const int s0 = max(cur.c0 - kTileCost, 0), s1 = min(max(cur.c1 - kTileCost, 0), (see_most + kStep - 1) / kStep);
+    const int slot = at == r.start ? 0 : 1;
+    float* set_aside = sums + ((size_t)blockIdx.x * 2 + slot) * kSlot + (size_t)row * D + half * (D / 2);
+    const int* table = p.block_tables + (size_t)cur.b * p.max_blocks;
+
+    // ---- the loads of a step ----
+    int page = -1;
+    bool there = false;
+    uint32_t kw[kWords], vw[kWords], pair = 0;
+    auto look = [&](int step) {
+      const long long pos = (long long)step * kStep + tok;
+      page = step < s1 && pos < see_most ? table[pos >> p.cache.shift] : -1;
+    };
+    auto fetch = [&](int step) {
+      there = (unsigned)page < (unsigned)p.cache.num_blocks;
+      if (there) {
+        const long long at_row = kv4_row(p.cache, page, cur.head, (step * kStep + tok) & page_mask);
+        const uint4* k = reinterpret_cast<const uint4*>(p.cache.k_codes + at_row * (D / 2) + part * (D / 4));
+        const uint4* v = reinterpret_cast<const uint4*>(p.cache.v_codes + at_row * (D / 2) + part * (D / 4));
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
+          // (the odd lanes' pieces are written from the fourth on)
+          const int j = kWords == 8 ? i ^ part : i;
+          const uint4 x = k[j], y = v[j];
+          kw[4 * i] = x.x, kw[4 * i + 1] = x.y, kw[4 * i + 2] = x.z, kw[4 * i + 3] = x.w;
+          vw[4 * i] = y.x, vw[4 * i + 1] = y.y, vw[4 * i + 2] = y.z, vw[4 * i + 3] = y.w;
+        }
+        pair = (part ? p.cache.v_scales : p.cache.k_scales)[at_row];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) kw[i] = vw[i] = 0;
+        pair = 0;
+      }
+    };
+    look(s0);
+
+    // ---- queries: half a row a thread ----
+    {
+      const int i = min(row0 + tok, end), token = i / per;
+      float sum = 0.f, odd = 0.f;
+      const bool live = tok < rows && sees(tok) > 0;
+      const long long src = (long long)(cur.s.first + token) * p.q_stride + (long long)(cur.head * per + i - token * per) * D +
+                            part * (D / 2);
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        const int j = H == 2 ? c ^ (part * 4) : c;
+        if (live) {
+          float v[8];
+          load_row8(p.q, src + j * 8, dtype, v);
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (BF)
+              asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
+            else
+              w[k] = pack_f16(v[2 * k], v[2 * k + 1]);
+            sum += v[2 * k] + v[2 * k + 1];
+            odd = fmaf(v[2 * k], 0.f, fmaf(v[2 * k + 1], 0.f, odd));  // NaN if one is not finite
+          }
+          x = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        put(piece(q_at + kq_row, c), x);
+      }
+      sum += odd;
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      if (part == 0) row_sum[tok] = sum;
+    }
+    fetch(s0);
+    look(s0 + 1);
+
+    float ref = -INFINITY, l = 0.f, off = 0.f, aside_ref = 0.f;
+    bool fresh = true, pending = false, aside = false;  // O empty; products of O on their way; O in part in the slot
+    int since = 0;
+    for (int step = s0; step < s1; ++step) {
+      // ---- keys, and the tokens' numbers ----
+      float m = 1.f;
+      {
+        const float scale = half_lo(pair), offset = half_hi(pair);
+        if (part == 0) {
+          tok_a[tok] = f * scale;
+          tok_b[tok] = f * fmaf(8.f, scale, offset);
+        } else {
+          const float size = fabsf(scale), centre = fmaf(8.f, scale, offset);
+          float lg = 0.f, inv = 1.f;
+          if (!there) {
+            lg = -INFINITY;  // weights of 0
+            inv = m = 0.f;
+          } else if (size == 0.f) {
+            m = 0.f;
+          } else if (!(size < INFINITY)) {
+            inv = NAN;
+          } else {
+            lg = log2f(size);
+            inv = 1.f / size;
+            m = scale < 0.f ? -1.f : 1.f;
+          }
+          tok_l[tok] = lg;
+          tok_i[tok] = inv;
+          tok_v[tok] = there ? centre * inv : 0.f;
+        }
+        m = __shfl_sync(0xffffffffu, m, lane | 1);
+      }
+#pragma unroll
+      for (int c = 0; c < kWords; ++c)
+        put(piece(k_at + kq_row, c), BF ? codes_bf16(kw[c]) : codes_f16(kw[c], 0x3C003C00u, 0xE408E408u));
+      fence_proxy_async_smem();
+      if (pending) wait_products(&bar, phase, dead, p);
+      if (since == kFlush) {
+#pragma unroll 1
+        for (int c = 0; c < D / 2; c += 16) {
+          uint32_t o[16];
+          tmem_load16(t_o + c, o);
+          const float g = aside_ref == ref ? 1.f : ex2(aside_ref - ref);  // (neither has one yet: 1)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            set_aside[c + k] = aside ? fmaf(set_aside[c + k], g, __uint_as_float(o[k])) : __uint_as_float(o[k]);
+        }
+        aside_ref = ref;
+        aside = fresh = true;
+        since = 0;
+      }
+      tcgen05_fence_before();
+      __syncthreads();
+      if (warp == 0) {
+        if (elect_one()) {
+          tcgen05_fence_after();
+          constexpr uint32_t idesc = umma_idesc_f16(kRows, kStep) | (BF ? 1u << 7 | 1u << 10 : 0u);
+          const uint64_t a = umma_smem_desc(q_at, 16, 1024, 2), b = umma_smem_desc(k_at, 16, 1024, 2);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t d = ((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4;
+            umma_f16(tmem, a + d, b + d, idesc, kk > 0);
+          }
+          umma_commit(&bar);
+        }
+        __syncwarp();
+      }
+
+      // ---- values, and the next step's loads ----
+      {
+        const uint32_t mm = m == 0.f ? 0u : (m < 0.f ? 0xBC00BC00u : 0x3C003C00u);
+        const uint32_t shift = m == 0.f ? 0u : (m < 0.f ? 0x64086408u : 0xE408E408u);  // -1032 m
+#pragma unroll
+        for (int c = 0; c < kWords; ++c) put(piece(v_at + v_row, c), codes_f16(vw[c], mm, shift));
+        fence_proxy_async_smem();
+      }
+      fetch(step + 1);
+      look(step + 2);
+
+      // ---- scores ----
+      wait_products(&bar, phase, dead, p);
+      uint32_t t[64];
+      tmem_load64(t_s, t);
+      const float q_sum = row_sum[row];
+      const int pos0 = step * kStep + half * 64;  // below 2^31 - 1024
+      const bool masked = (long long)step * kStep + kStep > see_least;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 64; j += 4) {
+        float a[4], b[4], g[4];
+        *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(tok_a + half * 64 + j);
+        *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(tok_b + half * 64 + j);
+        *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(tok_l + half * 64 + j);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float x = fmaf(a[k], __uint_as_float(t[j + k]), fmaf(b[k], q_sum, g[k]));
+          if (masked && pos0 + j + k >= see) x = -INFINITY;
+          t[j + k] = __float_as_uint(x);
+          top = fmaxf(top, x);
+        }
+      }
+      row_max[half * kRows + row] = top;
+      tcgen05_fence_before();
+      __syncthreads();
+      tcgen05_fence_after();
+      top = fmaxf(top, row_max[(1 - half) * kRows + row]);
+      float fall = 1.f;
+      if (top - ref > 15.f || (ref == -INFINITY && top > -INFINITY)) {
+        fall = ex2(ref - (top - 10.f));
+        ref = top - 10.f;
+        l *= fall;
+        off *= fall;
+      }
+      if (!fresh && __any_sync(0xffffffffu, fall != 1.f)) {
+#pragma unroll 1
+        for (int c = 0; c < D / 2; c += 16) {
+          uint32_t o[16];
+          tmem_load16(t_o + c, o);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fall);
+          tmem_store16(t_o + c, o);
+        }
+      }
+
+      // ---- weights ----
+      const float r0 = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          float inv[4], v[4], w[4];
+          *reinterpret_cast<float4*>(inv) = *reinterpret_cast<const float4*>(tok_i + half * 64 + c * 32 + j);
+          *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(tok_v + half * 64 + c * 32 + j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            w[k] = ex2(__uint_as_float(t[c * 32 + j + k]) - r0);
+            const bool hidden = masked && pos0 + c * 32 + j + k >= see;
+            l = hidden ? l : fmaf(w[k], inv[k], l);
+            off = hidden ? off : fmaf(w[k], v[k], off);
+          }
+          split_f16(w[0], w[1], hi[j / 2], lo[j / 2]);
+          split_f16(w[2], w[3], hi[j / 2 + 1], lo[j / 2 + 1]);
+        }
+        tmem_store16(t_p + c * 16, hi);
+        tmem_store16(t_p + kTmemLow + c * 16, lo);
+      }
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncthreads();
+      if (warp == 0) {
+        if (elect_one()) {
+          tcgen05_fence_after();
+          constexpr uint32_t idesc = umma_idesc_f16(kRows, D) | 1u << 16;  // B by rows of the k dimension
+          const uint64_t b = umma_smem_desc(v_at, 1024, H * 1024, 2);
+#pragma unroll
+          for (int kk = 0; kk < kStep / 16; ++kk) {
+            const uint64_t d = b + (uint64_t)(kk * (H * 2048) >> 4);
+            umma_f16_ts(tmem + kTmemO, tmem + 8 * kk, d, idesc, !fresh || kk > 0);
+            umma_f16_ts(tmem + kTmemO, tmem + kTmemLow + 8 * kk, d, idesc, 1);
+          }
+          umma_commit(&bar);
+        }
+        __syncwarp();
+      }
+      fresh = false;
+      pending = true;
+      ++since;
+    }
+    if (pending) wait_products(&bar, phase, dead, p);
+
+    // ---- the tile's end ----
+    row_max[half * kRows + row] = l;
+    row_num[half * kRows + row] = off;
+    __syncthreads();
+    l += row_max[(1 - half) * kRows + row];
+    off += row_num[(1 - half) * kRows + row];
+    const bool whole = cur.c0 == 0 && cur.c1 == cur.s.steps;
+    const float g = aside_ref == ref ? 1.f : ex2(aside_ref - ref);  // (neither has one yet: 1)
+    const int i = min(row0 + row, end), token = i / per;
+    const long long o_at = (long long)(cur.s.first + token) * p.o_stride + (long long)(cur.head * per + i - token * per) * D +
+                           half * (D / 2);
+    const float over = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+    for (int c = 0; c < D / 2; c += 16) {
+      uint32_t o[16];
+      if (!fresh)
+        tmem_load16(t_o + c, o);
+      else
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = 0;
+      float x[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        x[k] = __uint_as_float(o[k]) + off;
+        if (aside) x[k] = fmaf(set_aside[c + k], g, x[k]);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) set_aside[c + k] = x[k];
+      } else if (row < rows) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) store_any(p.o, o_at + c + k, dtype, l == 0.f ? 0.f : x[k] * over);
+      }
+    }
+    if (!whole && half == 0) {
+      float* num = sums + ((size_t)blockIdx.x * 2 + slot) * kSlot + kRows * D + 2 * row;
+      num[0] = ref;
+      num[1] = l;
+    }
+    if (!whole && cur.c0 == 0 && tid == 0)
+      parts[blockIdx.x] = Part{cur.s.first, rows, cur.head, (int)((at + cur.s.steps - 1) / r.length - blockIdx.x + 1), row0,
+                               slot, 0, 0};
+    at += cur.c1 - cur.c0;
+    if (at >= r.stop) break;
+    next_tile<kRows>(p, per, at, r.stop, cur);
+    tcgen05_fence_before();
+    __syncthreads();  // the rows' numbers have been read
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, kTmemCols);
+}
+
+template <int D, bool BF>
+cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t st) {
+  constexpr int smem = PromptSmem<D>::kBytes, kMaxDevices = 64;
+  static std::atomic<unsigned> asked[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned gen = attr_generation(dev) + 1;
+  if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
+    e = cudaFuncSetAttribute(kv4_prompt_kernel<D, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
+  }
+  const int ctas = sm_count * kCtasPerSm;
+  p.inv_ctas = 1.0 / ctas;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, BF>, p);
+  if (e != cudaSuccess) return e;
+  cfg.dynamicSmemBytes = 0;
+  cfg.gridDim = dim3((unsigned)ctas, kRows / 8);
+  cfg.blockDim = dim3(8 * 32);
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, kRows, 8, 1>, p, dtype);
+}
+
+}  // namespace
+
+// Queries of 16 bits (one product of theirs is exact), one group a head, and on the mean enough rows
+// a sequence and key head.
+bool kv4_prompt_takes(const Kv4AttentionParams& p, int dtype) {
+  const long long per = p.q_heads / p.cache.kv_heads;
+  return dtype != kTypeF32 && p.cache.head_dim <= 128 && p.cache.group == p.cache.head_dim &&
+         p.tokens * per >= 32ll * p.batch;
+}
+
+size_t kv4_prompt_workspace(int head_dim, int sm_count) {
+  return head_dim > 128 ? 0 : attention_workspace(sm_count * kCtasPerSm, kRows, head_dim);
+}
+
+cudaError_t launch_kv4_prompt(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t st) {
+  if (p.cache.head_dim == 64)
+    return dtype == kTypeBF16 ? launch<64, true>(p, dtype, sm_count, st) : launch<64, false>(p, dtype, sm_count, st);
+  return dtype == kTypeBF16 ? launch<128, true>(p, dtype, sm_count, st) : launch<128, false>(p, dtype, sm_count, st);
+}
+
+}  // namespace tk

@@ -1587,6 +1587,8 @@ int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* 
   p.q_heads = (int)q_heads;
   p.max_blocks = (int)max_blocks;
   p.scale = scale;
+  p.err = d->err;
+  p.timeout_ns = d->timeout_ns;
   ++d->launches;  // two kernels
   TK_LAUNCH(d, launch_kv4_attention(p, dtype, d->sm_count, pick_stream(d, stream)));
   return TK_OK;
