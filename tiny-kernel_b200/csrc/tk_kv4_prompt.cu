@@ -20,6 +20,7 @@
 // f32 additions, every kFlush steps.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "tk_internal.h"
 #include "tk_kv4_attention.cuh"
@@ -103,13 +104,57 @@ __device__ __forceinline__ uint4 codes_bf16(uint32_t w) {
   return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
+__device__ __forceinline__ void add_scaled(float4& x, const float4& y, float f) {
+  x.x = fmaf(y.x, f, x.x);
+  x.y = fmaf(y.y, f, x.y);
+  x.z = fmaf(y.z, f, x.z);
+  x.w = fmaf(y.w, f, x.w);
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack_out(float a, float b) {
+  if constexpr (!BF) return pack_f16(a, b);
+  uint32_t y;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(b), "f"(a));
+  return y;
+}
+
+// Two f32 at once.
+struct Pair {
+  unsigned long long x;
+};
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y.x) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float2 values_of(Pair p) {
+  float2 y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(p.x));
+  return y;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y.x) : "l"(a.x), "l"(b.x), "l"(c.x));
+  return y;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y.x) : "l"(a.x), "l"(b.x));
+  return y;
+}
+__device__ __forceinline__ void load_pairs(const float* src, Pair (&y)[2]) {  // 4 floats on a 16-byte boundary
+  const float4 v = *reinterpret_cast<const float4*>(src);
+  y[0] = pair_of(v.x, v.y);
+  y[1] = pair_of(v.z, v.w);
+}
+
 // Operands in shared memory: rows of 64 values (128 bytes), their 16-byte pieces turned by the row's
 // number; heads of 128 dimensions as two halves.  Keys and queries [half][row], values by eights of
 // tokens [token / 8][half][token % 8].
 template <int D>
 struct PromptSmem {
   static constexpr int kOperand = kRows * D * 2;
-  static constexpr int kQ = 0, kK = kOperand, kV = 2 * kOperand, kNums = 3 * kOperand;
+  static constexpr int kQ = 0, kK = kOperand, kV = 2 * kOperand, kRaw = 3 * kOperand, kNums = kRaw + kStep * D / 2;
   // per token a, b, log2 |s_v|, 1 / |s_v|, (m_v + 8 s_v) / |s_v|; per row sum(q), and two halves' numbers twice
   static constexpr int kBytes = kNums + (5 * kStep + kRows + 4 * kRows) * 4 + 1024;
 };
@@ -136,6 +181,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
     return;
   }
   uint8_t* smem = dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
+  const uint32_t raw_at = smem_addr(smem) + M::kRaw + threadIdx.x * 16;  // the thread's codes of values, 4 KB apart
   const uint32_t q_at = smem_addr(smem) + M::kQ, k_at = smem_addr(smem) + M::kK, v_at = smem_addr(smem) + M::kV;
   float* tok_a = reinterpret_cast<float*>(smem + M::kNums);
   float *tok_b = tok_a + kStep, *tok_l = tok_b + kStep, *tok_i = tok_l + kStep, *tok_v = tok_i + kStep;
@@ -176,6 +222,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
   };
 
+  auto get = [&](uint32_t at, uint32_t* x) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+  };
+  auto copy16 = [&](uint32_t dst, const uint8_t* src, uint32_t size) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+  };
+
   long long at = r.start;
   for (;;) {
     const int end = cur.s.n * per - 1, row0 = cur.rt * kRows, rows = min(kRows, end + 1 - row0);
@@ -189,32 +242,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
     // ---- the loads of a step ----
     int page = -1;
     bool there = false;
-    uint32_t kw[kWords], vw[kWords], pair = 0;
+    uint32_t pair = 0;
     auto look = [&](int step) {
       const long long pos = (long long)step * kStep + tok;
       page = step < s1 && pos < see_most ? table[pos >> p.cache.shift] : -1;
     };
+    // Codes of values wait in the thread's place, codes of keys in its own row of the operand, whose
+    // products have completed; where nothing is there nothing is read.
     auto fetch = [&](int step) {
       there = (unsigned)page < (unsigned)p.cache.num_blocks;
-      if (there) {
-        const long long at_row = kv4_row(p.cache, page, cur.head, (step * kStep + tok) & page_mask);
-        const uint4* k = reinterpret_cast<const uint4*>(p.cache.k_codes + at_row * (D / 2) + part * (D / 4));
-        const uint4* v = reinterpret_cast<const uint4*>(p.cache.v_codes + at_row * (D / 2) + part * (D / 4));
+      const long long at_row = there ? kv4_row(p.cache, page, cur.head, (step * kStep + tok) & page_mask) : 0;
+      const long long at_code = at_row * (D / 2) + part * (D / 4);
+      const uint32_t size = there ? 16 : 0;
 #pragma unroll
-        for (int i = 0; i < kWords / 4; ++i) {
-          // (the odd lanes' pieces are written from the fourth on)
-          const int j = kWords == 8 ? i ^ part : i;
-          const uint4 x = k[j], y = v[j];
-          kw[4 * i] = x.x, kw[4 * i + 1] = x.y, kw[4 * i + 2] = x.z, kw[4 * i + 3] = x.w;
-          vw[4 * i] = y.x, vw[4 * i + 1] = y.y, vw[4 * i + 2] = y.z, vw[4 * i + 3] = y.w;
-        }
-        pair = (part ? p.cache.v_scales : p.cache.k_scales)[at_row];
-      } else {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) kw[i] = vw[i] = 0;
-        pair = 0;
+      for (int i = 0; i < kWords / 4; ++i) {
+        copy16(piece(k_at + kq_row, i), p.cache.k_codes + at_code + i * 16, size);
+        copy16(raw_at + i * (kThreads * 16), p.cache.v_codes + at_code + i * 16, size);
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      pair = there ? (part ? p.cache.v_scales : p.cache.k_scales)[at_row] : 0;
     };
+    auto fetched = [&] { asm volatile("cp.async.wait_group 0;" ::: "memory"); };
     look(s0);
 
     // ---- queries: half a row a thread ----
@@ -234,10 +282,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            if constexpr (BF)
-              asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
-            else
-              w[k] = pack_f16(v[2 * k], v[2 * k + 1]);
+            w[k] = pack_out<BF>(v[2 * k], v[2 * k + 1]);
             sum += v[2 * k] + v[2 * k + 1];
             odd = fmaf(v[2 * k], 0.f, fmaf(v[2 * k + 1], 0.f, odd));  // NaN if one is not finite
           }
@@ -249,6 +294,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       if (part == 0) row_sum[tok] = sum;
     }
+    fetched();  // the last tile's last, of nothing
     fetch(s0);
     look(s0 + 1);
 
@@ -284,9 +330,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
         }
         m = __shfl_sync(0xffffffffu, m, lane | 1);
       }
+      fetched();
+      {
+        uint32_t w[kWords];
 #pragma unroll
-      for (int c = 0; c < kWords; ++c)
-        put(piece(k_at + kq_row, c), BF ? codes_bf16(kw[c]) : codes_f16(kw[c], 0x3C003C00u, 0xE408E408u));
+        for (int i = 0; i < kWords / 4; ++i) get(piece(k_at + kq_row, i), w + 4 * i);
+        // (the odd lanes' pieces are written from the fourth on)
+#pragma unroll
+        for (int c = 0; c < kWords; ++c) {
+          const uint32_t x = kWords == 8 && part ? w[c ^ 4] : w[c];
+          put(piece(k_at + kq_row, c), BF ? codes_bf16(x) : codes_f16(x, 0x3C003C00u, 0xE408E408u));
+        }
+      }
       fence_proxy_async_smem();
       if (pending) wait_products(&bar, phase, dead, p);
       if (since == kFlush) {
@@ -296,8 +351,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
           tmem_load16(t_o + c, o);
           const float g = aside_ref == ref ? 1.f : ex2(aside_ref - ref);  // (neither has one yet: 1)
 #pragma unroll
-          for (int k = 0; k < 16; ++k)
-            set_aside[c + k] = aside ? fmaf(set_aside[c + k], g, __uint_as_float(o[k])) : __uint_as_float(o[k]);
+          for (int k = 0; k < 16; k += 4) {
+            float4 x = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
+                                   __uint_as_float(o[k + 3]));
+            if (aside) add_scaled(x, *reinterpret_cast<const float4*>(set_aside + c + k), g);
+            *reinterpret_cast<float4*>(set_aside + c + k) = x;
+          }
         }
         aside_ref = ref;
         aside = fresh = true;
@@ -325,34 +384,50 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
         const uint32_t mm = m == 0.f ? 0u : (m < 0.f ? 0xBC00BC00u : 0x3C003C00u);
         const uint32_t shift = m == 0.f ? 0u : (m < 0.f ? 0x64086408u : 0xE408E408u);  // -1032 m
 #pragma unroll
-        for (int c = 0; c < kWords; ++c) put(piece(v_at + v_row, c), codes_f16(vw[c], mm, shift));
+        for (int i = 0; i < kWords / 4; ++i) {
+          uint32_t w[4];
+          get(raw_at + (kWords == 8 ? i ^ part : i) * (kThreads * 16), w);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) put(piece(v_at + v_row, 4 * i + k), codes_f16(w[k], mm, shift));
+        }
         fence_proxy_async_smem();
       }
-      fetch(step + 1);
-      look(step + 2);
 
       // ---- scores ----
       wait_products(&bar, phase, dead, p);
+      fetch(step + 1);
+      look(step + 2);
       uint32_t t[64];
       tmem_load64(t_s, t);
       const float q_sum = row_sum[row];
       const int pos0 = step * kStep + half * 64;  // below 2^31 - 1024
       const bool masked = (long long)step * kStep + kStep > see_least;
       float top = -INFINITY;
+      auto score = [&](auto with_mask) {
+        constexpr bool kMasked = decltype(with_mask)::value;
+        const Pair q2 = pair_of(q_sum, q_sum);
 #pragma unroll
-      for (int j = 0; j < 64; j += 4) {
-        float a[4], b[4], g[4];
-        *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(tok_a + half * 64 + j);
-        *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(tok_b + half * 64 + j);
-        *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(tok_l + half * 64 + j);
+        for (int j = 0; j < 64; j += 4) {
+          Pair a[2], b[2], g[2];
+          load_pairs(tok_a + half * 64 + j, a);
+          load_pairs(tok_b + half * 64 + j, b);
+          load_pairs(tok_l + half * 64 + j, g);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float x = fmaf(a[k], __uint_as_float(t[j + k]), fmaf(b[k], q_sum, g[k]));
-          if (masked && pos0 + j + k >= see) x = -INFINITY;
-          t[j + k] = __float_as_uint(x);
-          top = fmaxf(top, x);
+          for (int k = 0; k < 2; ++k) {
+            const int i = j + 2 * k;
+            float2 x = values_of(fma2(a[k], pair_of(__uint_as_float(t[i]), __uint_as_float(t[i + 1])), fma2(b[k], q2, g[k])));
+            if (kMasked && pos0 + i >= see) x.x = -INFINITY;
+            if (kMasked && pos0 + i + 1 >= see) x.y = -INFINITY;
+            t[i] = __float_as_uint(x.x);
+            t[i + 1] = __float_as_uint(x.y);
+            top = fmaxf(top, fmaxf(x.x, x.y));
+          }
         }
-      }
+      };
+      if (masked)
+        score(std::true_type{});
+      else
+        score(std::false_type{});
       row_max[half * kRows + row] = top;
       tcgen05_fence_before();
       __syncthreads();
@@ -377,28 +452,51 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
       }
 
       // ---- weights ----
-      const float r0 = ref == -INFINITY ? 0.f : ref;
+      auto weigh = [&](auto with_mask) {
+        constexpr bool kMasked = decltype(with_mask)::value;
+        const float r0 = ref == -INFINITY ? 0.f : -ref;
+        const Pair r2 = pair_of(r0, r0);
+        Pair l2 = pair_of(l, 0.f), off2 = pair_of(off, 0.f);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t hi[16], lo[16];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          float inv[4], v[4], w[4];
-          *reinterpret_cast<float4*>(inv) = *reinterpret_cast<const float4*>(tok_i + half * 64 + c * 32 + j);
-          *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(tok_v + half * 64 + c * 32 + j);
+          for (int j = 0; j < 32; j += 4) {
+            Pair inv[2], v[2];
+            load_pairs(tok_i + half * 64 + c * 32 + j, inv);
+            load_pairs(tok_v + half * 64 + c * 32 + j, v);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            w[k] = ex2(__uint_as_float(t[c * 32 + j + k]) - r0);
-            const bool hidden = masked && pos0 + c * 32 + j + k >= see;
-            l = hidden ? l : fmaf(w[k], inv[k], l);
-            off = hidden ? off : fmaf(w[k], v[k], off);
+            for (int k = 0; k < 2; ++k) {
+              const int i = c * 32 + j + 2 * k;
+              float2 w = values_of(add2(pair_of(__uint_as_float(t[i]), __uint_as_float(t[i + 1])), r2));
+              w.x = ex2(w.x);
+              w.y = ex2(w.y);
+              const Pair w2 = pair_of(w.x, w.y);
+              if (kMasked) {  // what the numbers of hidden tokens are does not matter
+                const bool hide_x = pos0 + i >= see, hide_y = pos0 + i + 1 >= see;
+                float2 a = values_of(inv[k]), b = values_of(v[k]);
+                inv[k] = pair_of(hide_x ? 0.f : a.x, hide_y ? 0.f : a.y);
+                v[k] = pair_of(hide_x ? 0.f : b.x, hide_y ? 0.f : b.y);
+              }
+              l2 = fma2(w2, inv[k], l2);
+              off2 = fma2(w2, v[k], off2);
+              const uint32_t h = pack_f16(w.x, w.y);
+              const float2 rest = values_of(add2(w2, pair_of(-half_lo(h), -half_hi(h))));
+              hi[j / 2 + k] = h;
+              lo[j / 2 + k] = pack_f16(rest.x, rest.y);
+            }
           }
-          split_f16(w[0], w[1], hi[j / 2], lo[j / 2]);
-          split_f16(w[2], w[3], hi[j / 2 + 1], lo[j / 2 + 1]);
+          tmem_store16(t_p + c * 16, hi);
+          tmem_store16(t_p + kTmemLow + c * 16, lo);
         }
-        tmem_store16(t_p + c * 16, hi);
-        tmem_store16(t_p + kTmemLow + c * 16, lo);
-      }
+        const float2 a = values_of(l2), b = values_of(off2);
+        l = a.x + a.y;
+        off = b.x + b.y;
+      };
+      if (masked)
+        weigh(std::true_type{});
+      else
+        weigh(std::false_type{});
       tmem_st_wait();
       tcgen05_fence_before();
       __syncthreads();
@@ -443,18 +541,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
       else
 #pragma unroll
         for (int k = 0; k < 16; ++k) o[k] = 0;
-      float x[16];
+      float4 x[4];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        x[k] = __uint_as_float(o[k]) + off;
-        if (aside) x[k] = fmaf(set_aside[c + k], g, x[k]);
+      for (int k = 0; k < 4; ++k) {
+        x[k] = make_float4(__uint_as_float(o[4 * k]) + off, __uint_as_float(o[4 * k + 1]) + off,
+                           __uint_as_float(o[4 * k + 2]) + off, __uint_as_float(o[4 * k + 3]) + off);
+        float4* kept = reinterpret_cast<float4*>(set_aside + c + 4 * k);
+        if (aside) add_scaled(x[k], *kept, g);
+        if (!whole) *kept = x[k];
       }
-      if (!whole) {
+      if (whole && row < rows) {
+        if (l == 0.f) x[0] = x[1] = x[2] = x[3] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) set_aside[c + k] = x[k];
-      } else if (row < rows) {
+        for (int k = 0; k < 4; k += 2) {
+          const uint4 y = make_uint4(pack_out<BF>(x[k].x * over, x[k].y * over), pack_out<BF>(x[k].z * over, x[k].w * over),
+                                     pack_out<BF>(x[k + 1].x * over, x[k + 1].y * over),
+                                     pack_out<BF>(x[k + 1].z * over, x[k + 1].w * over));
+          uint16_t* dst = static_cast<uint16_t*>(p.o) + o_at + c + 4 * k;
+          if (reinterpret_cast<uintptr_t>(dst) % 16 == 0) {
+            *reinterpret_cast<uint4*>(dst) = y;
+          } else {
+            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int k = 0; k < 16; ++k) store_any(p.o, o_at + c + k, dtype, l == 0.f ? 0.f : x[k] * over);
+            for (int i8 = 0; i8 < 8; ++i8) dst[i8] = (uint16_t)(w[i8 / 2] >> (i8 % 2 * 16));
+          }
+        }
       }
     }
     if (!whole && half == 0) {
