@@ -33,8 +33,8 @@ constexpr int kRows = 128, kThreads = 256, kFlush = 16, kCtasPerSm = 2;
 constexpr uint32_t kTmemCols = 256, kTmemO = 128, kTmemLow = 64;  // S and the weights' high parts at 0
 constexpr unsigned kErrWait = 4u;                                  // a product never completed
 
-// Waits for the phase of `bar`; gives up, for good, after timeout_ns.
-__device__ __forceinline__ void wait_products(uint64_t* bar, uint32_t& phase, bool& dead, const Kv4AttentionParams& p) {
+// Waits, a warp together, for the phase of `bar`; gives up, for good, after timeout_ns.
+__device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t phase, bool& dead, const Kv4AttentionParams& p) {
   if (!dead && !mbar_try_wait(bar, phase)) {
     const uint64_t t0 = global_timer_ns();
     while (!mbar_try_wait(bar, phase))
@@ -44,7 +44,7 @@ __device__ __forceinline__ void wait_products(uint64_t* bar, uint32_t& phase, bo
         break;
       }
   }
-  phase ^= 1;
+  __syncwarp();
   tcgen05_fence_after();
 }
 
@@ -155,8 +155,8 @@ template <int D>
 struct PromptSmem {
   static constexpr int kOperand = kRows * D * 2;
   static constexpr int kQ = 0, kK = kOperand, kV = 2 * kOperand, kRaw = 3 * kOperand, kNums = kRaw + kStep * D / 2;
-  // per token a, b, log2 |s_v|, 1 / |s_v|, (m_v + 8 s_v) / |s_v|; per row sum(q), and two halves' numbers twice
-  static constexpr int kBytes = kNums + (5 * kStep + kRows + 4 * kRows) * 4 + 1024;
+  // per token, twice, a, b, log2 |s_v|, 1 / |s_v|, (m_v + 8 s_v) / |s_v|; per row sum(q), and two halves' numbers twice
+  static constexpr int kBytes = kNums + (2 * 5 * kStep + kRows + 4 * kRows) * 4 + 1024;
 };
 
 template <int D, bool BF>
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
   constexpr int dtype = BF ? kTypeBF16 : kTypeF16;
   constexpr int kWords = D / 16;     // of codes of half a head
   extern __shared__ uint8_t dynamic[];
-  __shared__ uint64_t bar;
+  __shared__ uint64_t bar, keys_bar, weights_bar;  // products complete; all warps' keys, weights written
   __shared__ uint32_t tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -185,10 +185,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
   const uint32_t q_at = smem_addr(smem) + M::kQ, k_at = smem_addr(smem) + M::kK, v_at = smem_addr(smem) + M::kV;
   float* tok_a = reinterpret_cast<float*>(smem + M::kNums);
   float *tok_b = tok_a + kStep, *tok_l = tok_b + kStep, *tok_i = tok_l + kStep, *tok_v = tok_i + kStep;
-  float* row_sum = tok_v + kStep;
+  float* row_sum = tok_a + 2 * 5 * kStep;
   float *row_max = row_sum + kRows, *row_num = row_max + 2 * kRows;  // [half][row] each
   if (tid == 0) {
     mbar_init(&bar, 1);
+    mbar_init(&keys_bar, kThreads / 32);
+    mbar_init(&weights_bar, kThreads / 32);
     fence_mbar_init();
   }
   if (warp == 0) tmem_alloc(&tmem_slot, kTmemCols);
@@ -199,8 +201,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
   // blocks have theirs.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = tmem_slot;
-  uint32_t phase = 0;
+  uint32_t phase = 0, step_phase = 0;  // of products; of the barriers that complete once a step
   bool dead = false;
+  auto wait_products = [&] {
+    wait_phase(&bar, phase, dead, p);
+    phase ^= 1;
+  };
+  // the warp's writes are done, for the products and the other warps
+  auto arrive = [&](uint64_t* b) {
+    tcgen05_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(b);
+  };
 
   // this thread as a loader: half a token's codes (of a row's queries); as a row's: half its tokens
   const int tok = tid >> 1, part = tid & 1;
@@ -303,12 +315,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
     int since = 0;
     for (int step = s0; step < s1; ++step) {
       // ---- keys, and the tokens' numbers ----
+      const int turn = (int)step_phase * (5 * kStep);  // a warp may be a step ahead of another
       float m = 1.f;
       {
         const float scale = half_lo(pair), offset = half_hi(pair);
         if (part == 0) {
-          tok_a[tok] = f * scale;
-          tok_b[tok] = f * fmaf(8.f, scale, offset);
+          tok_a[turn + tok] = f * scale;
+          tok_b[turn + tok] = f * fmaf(8.f, scale, offset);
         } else {
           const float size = fabsf(scale), centre = fmaf(8.f, scale, offset);
           float lg = 0.f, inv = 1.f;
@@ -324,9 +337,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
             inv = 1.f / size;
             m = scale < 0.f ? -1.f : 1.f;
           }
-          tok_l[tok] = lg;
-          tok_i[tok] = inv;
-          tok_v[tok] = there ? centre * inv : 0.f;
+          tok_l[turn + tok] = lg;
+          tok_i[turn + tok] = inv;
+          tok_v[turn + tok] = there ? centre * inv : 0.f;
         }
         m = __shfl_sync(0xffffffffu, m, lane | 1);
       }
@@ -343,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
         }
       }
       fence_proxy_async_smem();
-      if (pending) wait_products(&bar, phase, dead, p);
+      if (pending) wait_products();
       if (since == kFlush) {
 #pragma unroll 1
         for (int c = 0; c < D / 2; c += 16) {
@@ -362,11 +375,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
         aside = fresh = true;
         since = 0;
       }
-      tcgen05_fence_before();
-      __syncthreads();
+      arrive(&keys_bar);
       if (warp == 0) {
+        wait_phase(&keys_bar, step_phase, dead, p);
         if (elect_one()) {
-          tcgen05_fence_after();
           constexpr uint32_t idesc = umma_idesc_f16(kRows, kStep) | (BF ? 1u << 7 | 1u << 10 : 0u);
           const uint64_t a = umma_smem_desc(q_at, 16, 1024, 2), b = umma_smem_desc(k_at, 16, 1024, 2);
 #pragma unroll
@@ -394,7 +406,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
       }
 
       // ---- scores ----
-      wait_products(&bar, phase, dead, p);
+      wait_products();
+      wait_phase(&keys_bar, step_phase, dead, p);  // (complete: the products were issued after it)
       fetch(step + 1);
       look(step + 2);
       uint32_t t[64];
@@ -409,9 +422,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
 #pragma unroll
         for (int j = 0; j < 64; j += 4) {
           Pair a[2], b[2], g[2];
-          load_pairs(tok_a + half * 64 + j, a);
-          load_pairs(tok_b + half * 64 + j, b);
-          load_pairs(tok_l + half * 64 + j, g);
+          load_pairs(tok_a + turn + half * 64 + j, a);
+          load_pairs(tok_b + turn + half * 64 + j, b);
+          load_pairs(tok_l + turn + half * 64 + j, g);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const int i = j + 2 * k;
@@ -428,9 +441,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
         score(std::true_type{});
       else
         score(std::false_type{});
+      // the two warps of these rows: both have read S, over which the weights go
       row_max[half * kRows + row] = top;
       tcgen05_fence_before();
-      __syncthreads();
+      named_barrier(1 + (warp & 3), 64);
       tcgen05_fence_after();
       top = fmaxf(top, row_max[(1 - half) * kRows + row]);
       float fall = 1.f;
@@ -463,8 +477,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             Pair inv[2], v[2];
-            load_pairs(tok_i + half * 64 + c * 32 + j, inv);
-            load_pairs(tok_v + half * 64 + c * 32 + j, v);
+            load_pairs(tok_i + turn + half * 64 + c * 32 + j, inv);
+            load_pairs(tok_v + turn + half * 64 + c * 32 + j, v);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const int i = c * 32 + j + 2 * k;
@@ -498,11 +512,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
       else
         weigh(std::false_type{});
       tmem_st_wait();
-      tcgen05_fence_before();
-      __syncthreads();
+      arrive(&weights_bar);
       if (warp == 0) {
+        wait_phase(&weights_bar, step_phase, dead, p);
         if (elect_one()) {
-          tcgen05_fence_after();
           constexpr uint32_t idesc = umma_idesc_f16(kRows, D) | 1u << 16;  // B by rows of the k dimension
           const uint64_t b = umma_smem_desc(v_at, 1024, H * 1024, 2);
 #pragma unroll
@@ -515,11 +528,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
         }
         __syncwarp();
       }
+      step_phase ^= 1;
       fresh = false;
       pending = true;
       ++since;
     }
-    if (pending) wait_products(&bar, phase, dead, p);
+    if (pending) wait_products();
 
     // ---- the tile's end ----
     row_max[half * kRows + row] = l;
