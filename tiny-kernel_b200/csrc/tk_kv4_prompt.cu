@@ -104,6 +104,22 @@ __device__ __forceinline__ uint4 codes_bf16(uint32_t w) {
   return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
+__device__ __forceinline__ uint4 load_bits8(const uint16_t* src) {
+  if (reinterpret_cast<uintptr_t>(src) % 16 == 0) return *reinterpret_cast<const uint4*>(src);
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = src[2 * k] | (uint32_t)src[2 * k + 1] << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_bits8(uint16_t* dst, const uint4& y) {
+  if (reinterpret_cast<uintptr_t>(dst) % 16 == 0) {
+    *reinterpret_cast<uint4*>(dst) = y;
+    return;
+  }
+  const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) dst[k] = (uint16_t)(w[k / 2] >> (k % 2 * 16));
+}
 __device__ __forceinline__ void add_scaled(float4& x, const float4& y, float f) {
   x.x = fmaf(y.x, f, x.x);
   x.y = fmaf(y.y, f, x.y);
@@ -163,7 +179,6 @@ template <int D, bool BF>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4AttentionParams p) {
   using M = PromptSmem<D>;
   constexpr int H = D / 64;          // halves of a head, 128 bytes a row
-  constexpr int dtype = BF ? kTypeBF16 : kTypeF16;
   constexpr int kWords = D / 16;     // of codes of half a head
   extern __shared__ uint8_t dynamic[];
   __shared__ uint64_t bar, keys_bar, weights_bar;  // products complete; all warps' keys, weights written
@@ -248,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
     const int see = sees(row), see_least = sees(0), see_most = max(sees(kRows - 1), 0);
     const int s0 = max(cur.c0 - kTileCost, 0), s1 = min(max(cur.c1 - kTileCost, 0), (see_most + kStep - 1) / kStep);
     const int slot = at == r.start ? 0 : 1;
-    float* set_aside = sums + ((size_t)blockIdx.x * 2 + slot) * kSlot + (size_t)row * D + half * (D / 2);
+    float4* set_aside = reinterpret_cast<float4*>(sums + ((size_t)blockIdx.x * 2 + slot) * kSlot) + half * (D / 8) * kRows + row;
     const int* table = p.block_tables + (size_t)cur.b * p.max_blocks;
 
     // ---- the loads of a step ----
@@ -284,23 +299,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
       const bool live = tok < rows && sees(tok) > 0;
       const long long src = (long long)(cur.s.first + token) * p.q_stride + (long long)(cur.head * per + i - token * per) * D +
                             part * (D / 2);
+      uint4 x[D / 16];  // all under way before the first is looked at
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        const int j = H == 2 ? c ^ (part * 4) : c;
-        if (live) {
-          float v[8];
-          load_row8(p.q, src + j * 8, dtype, v);
-          uint32_t w[4];
+        x[c] = make_uint4(0, 0, 0, 0);
+        if (live) x[c] = load_bits8(static_cast<const uint16_t*>(p.q) + src + (H == 2 ? c ^ (part * 4) : c) * 8);
+      }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            w[k] = pack_out<BF>(v[2 * k], v[2 * k + 1]);
-            sum += v[2 * k] + v[2 * k + 1];
-            odd = fmaf(v[2 * k], 0.f, fmaf(v[2 * k + 1], 0.f, odd));  // NaN if one is not finite
-          }
-          x = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int c = 0; c < D / 16; ++c) {
+        const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float a = BF ? __uint_as_float(w[k] << 16) : half_lo(w[k]);
+          const float b = BF ? __uint_as_float(w[k] & 0xFFFF0000u) : half_hi(w[k]);
+          sum += a + b;
+          odd = fmaf(a, 0.f, fmaf(b, 0.f, odd));  // NaN if one is not finite
         }
-        put(piece(q_at + kq_row, c), x);
+        put(piece(q_at + kq_row, c), x[c]);
       }
       sum += odd;
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -367,8 +382,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
           for (int k = 0; k < 16; k += 4) {
             float4 x = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
                                    __uint_as_float(o[k + 3]));
-            if (aside) add_scaled(x, *reinterpret_cast<const float4*>(set_aside + c + k), g);
-            *reinterpret_cast<float4*>(set_aside + c + k) = x;
+            float4* kept = set_aside + (c + k) / 4 * kRows;
+            if (aside) add_scaled(x, *kept, g);
+            *kept = x;
           }
         }
         aside_ref = ref;
@@ -560,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
       for (int k = 0; k < 4; ++k) {
         x[k] = make_float4(__uint_as_float(o[4 * k]) + off, __uint_as_float(o[4 * k + 1]) + off,
                            __uint_as_float(o[4 * k + 2]) + off, __uint_as_float(o[4 * k + 3]) + off);
-        float4* kept = reinterpret_cast<float4*>(set_aside + c + 4 * k);
+        float4* kept = set_aside + (c / 4 + k) * kRows;
         if (aside) add_scaled(x[k], *kept, g);
         if (!whole) *kept = x[k];
       }
@@ -571,14 +587,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
           const uint4 y = make_uint4(pack_out<BF>(x[k].x * over, x[k].y * over), pack_out<BF>(x[k].z * over, x[k].w * over),
                                      pack_out<BF>(x[k + 1].x * over, x[k + 1].y * over),
                                      pack_out<BF>(x[k + 1].z * over, x[k + 1].w * over));
-          uint16_t* dst = static_cast<uint16_t*>(p.o) + o_at + c + 4 * k;
-          if (reinterpret_cast<uintptr_t>(dst) % 16 == 0) {
-            *reinterpret_cast<uint4*>(dst) = y;
-          } else {
-            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i8 = 0; i8 < 8; ++i8) dst[i8] = (uint16_t)(w[i8 / 2] >> (i8 % 2 * 16));
-          }
+          store_bits8(static_cast<uint16_t*>(p.o) + o_at + c + 4 * k, y);
         }
       }
     }
@@ -601,8 +610,55 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
   if (warp == 0) tmem_dealloc(tmem, kTmemCols);
 }
 
+// Joins the parts of the tile that begins in the run of CTA blockIdx.x: a thread a row, 32 dimensions.
 template <int D, bool BF>
-cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t st) {
+__global__ void __launch_bounds__(kRows) kv4_prompt_join_kernel(Kv4AttentionParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Part* parts = static_cast<const Part*>(p.workspace);
+  const float* sums = reinterpret_cast<const float*>(parts + gridDim.x);
+  constexpr int kSlot = kRows * (D + 2);
+  const Part part = parts[blockIdx.x];
+  const int row = threadIdx.x;
+  if (part.count == 0 || row >= part.rows) return;
+  const int d0 = blockIdx.y * 32;
+  float top = -INFINITY, sum = 0.f;
+  float4 v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < part.count; ++i) {
+    const float* s = sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot;
+    const float2 num = *reinterpret_cast<const float2*>(s + kRows * D + 2 * row);
+    float4 x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = reinterpret_cast<const float4*>(s)[(d0 / 4 + k) * kRows + row];
+    const float now = fmaxf(top, num.x);
+    const float f = top == now ? 1.f : ex2(top - now), g = num.x == now ? 1.f : ex2(num.x - now);
+    top = now;
+    sum = fmaf(num.y, g, sum * f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
+      add_scaled(v[k], x[k], g);
+    }
+  }
+  const int per = p.q_heads / p.cache.kv_heads, q = part.row0 + row;
+  const long long at = (long long)(part.token + q / per) * p.o_stride + (long long)(part.head * per + q % per) * D + d0;
+  const float over = sum == 0.f ? 0.f : 1.f / sum;
+  if (sum == 0.f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int k = 0; k < 8; k += 2)
+    store_bits8(static_cast<uint16_t*>(p.o) + at + 4 * k,
+                make_uint4(pack_out<BF>(v[k].x * over, v[k].y * over), pack_out<BF>(v[k].z * over, v[k].w * over),
+                           pack_out<BF>(v[k + 1].x * over, v[k + 1].y * over),
+                           pack_out<BF>(v[k + 1].z * over, v[k + 1].w * over)));
+}
+
+template <int D, bool BF>
+cudaError_t launch(Kv4AttentionParams p, int sm_count, cudaStream_t st) {
   constexpr int smem = PromptSmem<D>::kBytes, kMaxDevices = 64;
   static std::atomic<unsigned> asked[kMaxDevices];
   int dev = 0;
@@ -629,9 +685,9 @@ cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t s
   e = cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, BF>, p);
   if (e != cudaSuccess) return e;
   cfg.dynamicSmemBytes = 0;
-  cfg.gridDim = dim3((unsigned)ctas, kRows / 8);
-  cfg.blockDim = dim3(8 * 32);
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, kRows, 8, 1>, p, dtype);
+  cfg.gridDim = dim3((unsigned)ctas, D / 32);
+  cfg.blockDim = dim3(kRows);
+  return cudaLaunchKernelEx(&cfg, kv4_prompt_join_kernel<D, BF>, p);
 }
 
 }  // namespace
@@ -650,8 +706,8 @@ size_t kv4_prompt_workspace(int head_dim, int sm_count) {
 
 cudaError_t launch_kv4_prompt(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t st) {
   if (p.cache.head_dim == 64)
-    return dtype == kTypeBF16 ? launch<64, true>(p, dtype, sm_count, st) : launch<64, false>(p, dtype, sm_count, st);
-  return dtype == kTypeBF16 ? launch<128, true>(p, dtype, sm_count, st) : launch<128, false>(p, dtype, sm_count, st);
+    return dtype == kTypeBF16 ? launch<64, true>(p, sm_count, st) : launch<64, false>(p, sm_count, st);
+  return dtype == kTypeBF16 ? launch<128, true>(p, sm_count, st) : launch<128, false>(p, sm_count, st);
 }
 
 }  // namespace tk
