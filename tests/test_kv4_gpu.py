@@ -408,16 +408,16 @@ def test_attention(torch_cuda, tkdev, n, dtype):
     c.check(c.run(tkdev, c.upload()))
 
 
-# many rows a sequence, one group a head: the kernel for prompts where the queries have 16 bits
+# many rows a sequence, one group a head, a long table: the kernel for prompts where the queries have 16 bits
 PROMPTS = [
     ([128], [128], 1, 1, 128, 128, 16),                      # one full tile, one step
-    ([1], [1], 40, 1, 64, 64, 16),                           # one token in all
+    ([1], [1], 50, 1, 64, 64, 16),                           # one token in all
     ([129, 300], [129, 33], 4, 4, 64, 64, 16),               # a row and a step more than full ones
     ([700, 130], [130, 33], 7, 1, 128, 128, 32),
     ([1000, 17, 0, 400], [100, 17, 0, 1], 10, 2, 128, 128, 64),  # a prompt, one token, no request
-    ([50, 2, 0, 9], [60, 40, 3, 9], 8, 8, 128, 128, 16),     # queries before the first position
+    ([50, 2, 0, 9], [60, 40, 3, 9], 16, 8, 128, 128, 16),    # queries before the first position
     ([2500], [70], 16, 1, 64, 64, 256),                      # many CTAs to a tile
-    ([300] * 20, [40] * 20, 4, 4, 64, 64, 16),
+    ([300] * 20, [50] * 20, 4, 4, 64, 64, 16),
     ([5200] * 4, [130] * 4, 16, 16, 64, 64, 32),             # runs long enough for sums to be set aside
     ([4600, 4300, 4400], [257, 256, 140], 10, 10, 128, 128, 16),
 ]
@@ -428,7 +428,7 @@ PROMPTS = [
 def test_attention_of_prompts(torch_cuda, tkdev, n, dtype):
     if dtype == "f32" and n >= 8:
         pytest.skip("the same kernel as shorter ones")
-    c = Case(torch_cuda, 40 + n, *PROMPTS[n], dtype)
+    c = Case(torch_cuda, 40 + n, *PROMPTS[n], dtype, spare=6000)
     c.check(c.run(tkdev, c.upload()))
 
 
@@ -437,7 +437,7 @@ def test_prompts_with_absent_pages_and_anything_in_masked_places(torch_cuda, tkd
     """Pages that are not in the cache (more than a step of them, and the whole of a sequence), and
     NaN and infinities in scales behind the last token, in pages of nobody and in the last query's own
     position, which only it sees."""
-    c = Case(torch_cuda, 61, [700, 2500, 40], [100, 40, 40], 4, 2, dim, dim, 16, "f16")
+    c = Case(torch_cuda, 61, [700, 2500, 40], [100, 40, 40], 4, 2, dim, dim, 16, "f16", spare=6000)
     c.tables[0, 3:14] = -1
     c.tables[1, :140] = c.blocks
     c.tables[2, :] = [-5, 2**31 - 1, -2**31] + [-1] * (c.width - 3)
@@ -462,7 +462,7 @@ def test_prompts_in_place_strided_and_repeated(torch_cuda, tkdev, dtype):
     """Rows of a projection apart and off the 16-byte boundary, output over the queries; the same bits
     from run to run, and rows of no sequence left as they were."""
     torch = torch_cuda
-    c = Case(torch, 62, [900, 333], [90, 40], 6, 2, 64, 64, 16, dtype)
+    c = Case(torch, 62, [900, 333], [90, 40], 6, 2, 64, 64, 16, dtype, spare=6000)
     cache = c.upload()
     first = c.run(tkdev, cache).clone()
     for _ in range(3):
@@ -483,7 +483,7 @@ def test_prompts_in_place_strided_and_repeated(torch_cuda, tkdev, dtype):
 def test_prompts_with_scales_of_every_kind(torch_cuda, tkdev, dtype):
     """Scales of 0, of either sign, the smallest subnormal and sizes far apart; queries of every size;
     a row of queries with an infinity gives NaN and no other row does."""
-    c = Case(torch_cuda, 63, [600, 200], [64, 40], 2, 1, 128, 128, 16, dtype)
+    c = Case(torch_cuda, 63, [600, 200], [64, 40], 2, 1, 128, 128, 16, dtype, spare=6000)
     rng = np.random.default_rng(63)
     for part in c.parts:
         some = rng.integers(0, 8, part[1].shape)
@@ -722,6 +722,46 @@ def test_two_streams_with_their_own_workspaces(torch_cuda, tkdev):
             ops.kv4_attention(tkdev, cache, c.q, *c.dev_args, o, w, c.ws_size, 2, 2, 8, c.width, c.scale, stream=s.cuda_stream)
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_prompts_beside_the_gemm_and_captured(torch_cuda, tkdev):
+    """Prompts on two streams, one of them a replayed graph, and the INT4 GEMM, which takes all of an
+    SM's tensor memory, on a third: the same bits as each alone."""
+    torch = torch_cuda
+    c = Case(torch, 71, [1500, 700], [130, 64], 8, 4, 128, 128, 16, "bf16", spare=2000)
+    cache = c.upload()
+    want = c.run(tkdev, cache).clone()
+    m, k, n = 64, 1024, 2048
+    x = torch.randn(m, k, device="cuda")
+    w = torch.randint(0, 256, (k // 2, n), dtype=torch.uint8, device="cuda")
+    scales = torch.rand(k // 64, n, device="cuda").half()
+    zeros = torch.randint(0, 256, (k // 64, n // 2), dtype=torch.uint8, device="cuda")
+    y = torch.zeros(m, n, device="cuda")
+    assert ops.path(m, k, n, 64) == 2
+    torch.cuda.synchronize()
+    ops.qmatmul_int4(tkdev, x, w, scales, zeros, y, m, k, n, 64)
+    y0 = y.clone()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs, ws = [torch.zeros_like(c.q) for _ in "ab"], [torch.zeros_like(c.ws) for _ in "ab"]
+
+    def attend(i, stream):
+        ops.kv4_attention(tkdev, cache, c.q, *c.dev_args, outs[i], ws[i], c.ws_size, c.tokens, 2, 8, c.width, c.scale,
+                          "bf16", stream=stream.cuda_stream)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        attend(0, streams[0])
+        attend(0, streams[0])
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        attend(1, streams[1])
+        ops.qmatmul_int4(tkdev, x, w, scales, zeros, y, m, k, n, 64, stream=streams[2].cuda_stream, sync=False)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want) and torch.equal(y, y0)
+    tkdev.synchronize()
+    del graph
 
 
 def test_no_tokens_is_no_launch(torch_cuda, tkdev):

@@ -610,36 +610,49 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
   if (warp == 0) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the parts of the tile that begins in the run of CTA blockIdx.x: a thread a row, 32 dimensions.
+// Joins the parts of the tile that begins in the run of CTA blockIdx.x, kJoinDims dimensions of it: a
+// thread a row, four parts under way at a time.
+constexpr int kJoinDims = 16, kJoinParts = 4;
 template <int D, bool BF>
 __global__ void __launch_bounds__(kRows) kv4_prompt_join_kernel(Kv4AttentionParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Part* parts = static_cast<const Part*>(p.workspace);
   const float* sums = reinterpret_cast<const float*>(parts + gridDim.x);
-  constexpr int kSlot = kRows * (D + 2);
+  constexpr int kSlot = kRows * (D + 2), V = kJoinDims / 4;
   const Part part = parts[blockIdx.x];
   const int row = threadIdx.x;
   if (part.count == 0 || row >= part.rows) return;
-  const int d0 = blockIdx.y * 32;
+  const int d0 = blockIdx.y * kJoinDims;
   float top = -INFINITY, sum = 0.f;
-  float4 v[8];
+  float4 v[V];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < part.count; ++i) {
-    const float* s = sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot;
-    const float2 num = *reinterpret_cast<const float2*>(s + kRows * D + 2 * row);
-    float4 x[8];
+  for (int k = 0; k < V; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < part.count; i0 += kJoinParts) {
+    float2 num[kJoinParts];
+    float4 x[kJoinParts][V];
+    float now = top;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = reinterpret_cast<const float4*>(s)[(d0 / 4 + k) * kRows + row];
-    const float now = fmaxf(top, num.x);
-    const float f = top == now ? 1.f : ex2(top - now), g = num.x == now ? 1.f : ex2(num.x - now);
+    for (int u = 0; u < kJoinParts; ++u) {
+      const int i = min(i0 + u, part.count - 1);  // one that counts, read again
+      const float* s = sums + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? part.slot : 0)) * kSlot;
+      num[u] = *reinterpret_cast<const float2*>(s + kRows * D + 2 * row);
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[u][k] = reinterpret_cast<const float4*>(s)[(d0 / 4 + k) * kRows + row];
+      now = fmaxf(now, num[u].x);
+    }
+    const float f = top == now ? 1.f : ex2(top - now);  // (no reference yet: sums of 0, or of NaN)
     top = now;
-    sum = fmaf(num.y, g, sum * f);
+    sum *= f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      v[k] = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
-      add_scaled(v[k], x[k], g);
+    for (int k = 0; k < V; ++k) v[k] = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
+#pragma unroll
+    for (int u = 0; u < kJoinParts; ++u) {
+      if (i0 + u >= part.count) break;
+      const float g = num[u].x == now ? 1.f : ex2(num[u].x - now);
+      sum = fmaf(num[u].y, g, sum);
+#pragma unroll
+      for (int k = 0; k < V; ++k) add_scaled(v[k], x[u][k], g);
     }
   }
   const int per = p.q_heads / p.cache.kv_heads, q = part.row0 + row;
@@ -647,10 +660,10 @@ __global__ void __launch_bounds__(kRows) kv4_prompt_join_kernel(Kv4AttentionPara
   const float over = sum == 0.f ? 0.f : 1.f / sum;
   if (sum == 0.f) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < V; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 #pragma unroll
-  for (int k = 0; k < 8; k += 2)
+  for (int k = 0; k < V; k += 2)
     store_bits8(static_cast<uint16_t*>(p.o) + at + 4 * k,
                 make_uint4(pack_out<BF>(v[k].x * over, v[k].y * over), pack_out<BF>(v[k].z * over, v[k].w * over),
                            pack_out<BF>(v[k + 1].x * over, v[k + 1].y * over),
@@ -685,19 +698,24 @@ cudaError_t launch(Kv4AttentionParams p, int sm_count, cudaStream_t st) {
   e = cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<D, BF>, p);
   if (e != cudaSuccess) return e;
   cfg.dynamicSmemBytes = 0;
-  cfg.gridDim = dim3((unsigned)ctas, D / 32);
+  cfg.gridDim = dim3((unsigned)ctas, D / kJoinDims);
   cfg.blockDim = dim3(kRows);
   return cudaLaunchKernelEx(&cfg, kv4_prompt_join_kernel<D, BF>, p);
 }
 
 }  // namespace
 
-// Queries of 16 bits (one product of theirs is exact), one group a head, and on the mean enough rows
-// a sequence and key head.
+// Queries of 16 bits (one product with them is exact), one group a head, and on the mean enough rows a
+// sequence: against tiles of eight rows, 16 x 2000 positions with 32 rows a head take 64 us instead of
+// 53, with 48 65 instead of 73, with 128 70 instead of 168; 60000 positions 110 and 75, 111 and 106, 114
+// and 255.  A step is long, so little work in all wants more rows (one sequence of 3000, by the table's
+// reach: 48 rows 29 and 19 us, 128 rows 32 and 28, 256 rows 33 and 40).
 bool kv4_prompt_takes(const Kv4AttentionParams& p, int dtype) {
-  const long long per = p.q_heads / p.cache.kv_heads;
-  return dtype != kTypeF32 && p.cache.head_dim <= 128 && p.cache.group == p.cache.head_dim &&
-         p.tokens * per >= 32ll * p.batch;
+  if (dtype == kTypeF32 || p.cache.head_dim > 128 || p.cache.group != p.cache.head_dim) return false;
+  const long long rows = (long long)p.tokens * (p.q_heads / p.cache.kv_heads);
+  const long long tiles = (rows / kRows + p.batch) * p.cache.kv_heads;
+  const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost;
+  return rows >= 160ll * p.batch || (rows >= 48ll * p.batch && tiles * steps >= 600);
 }
 
 size_t kv4_prompt_workspace(int head_dim, int sm_count) {
