@@ -479,11 +479,12 @@ def test_prompts_in_place_strided_and_repeated(torch_cuda, tkdev, dtype):
     assert (wide == 9).all()
 
 
-@pytest.mark.parametrize("dtype", ["f16", "bf16"])
-def test_prompts_with_scales_of_every_kind(torch_cuda, tkdev, dtype):
+@pytest.mark.parametrize("dtype,group,spare", [("f16", 128, 6000), ("bf16", 128, 6000), ("f32", 128, 2),
+                                               ("f32", 64, 2), ("bf16", 64, 2)])
+def test_prompts_with_scales_of_every_kind(torch_cuda, tkdev, dtype, group, spare):
     """Scales of 0, of either sign, the smallest subnormal and sizes far apart; queries of every size;
     a row of queries with an infinity gives NaN and no other row does."""
-    c = Case(torch_cuda, 63, [600, 200], [64, 40], 2, 1, 128, 128, 16, dtype, spare=6000)
+    c = Case(torch_cuda, 63, [600, 200], [64, 40], 2, 1, 128, group, 16, dtype, spare=spare)
     rng = np.random.default_rng(63)
     for part in c.parts:
         some = rng.integers(0, 8, part[1].shape)
