@@ -134,6 +134,11 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
   return y;
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // Two f32 at once.
 struct Pair {
   unsigned long long x;
@@ -348,8 +353,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
           } else if (!(size < INFINITY)) {
             inv = NAN;
           } else {
-            lg = log2f(size);
-            inv = 1.f / size;
+            lg = lg2(size);  // (normal in f32; an error of it is one of the weight, in both sums alike)
+            inv = rcp(size);
             m = scale < 0.f ? -1.f : 1.f;
           }
           tok_l[turn + tok] = lg;
@@ -424,8 +429,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
       // ---- scores ----
       wait_products();
       wait_phase(&keys_bar, step_phase, dead, p);  // (complete: the products were issued after it)
-      fetch(step + 1);
-      look(step + 2);
       uint32_t t[64];
       tmem_load64(t_s, t);
       const float q_sum = row_sum[row];
@@ -480,6 +483,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_prompt_kernel(Kv4Att
           tmem_store16(t_o + c, o);
         }
       }
+
+      fetch(step + 1);
+      look(step + 2);
 
       // ---- weights ----
       auto weigh = [&](auto with_mask) {
