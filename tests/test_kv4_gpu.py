@@ -432,12 +432,27 @@ def test_attention_of_prompts(torch_cuda, tkdev, n, dtype):
     c.check(c.run(tkdev, c.upload()))
 
 
-@pytest.mark.parametrize("dim", [64, 128])
-def test_prompts_with_absent_pages_and_anything_in_masked_places(torch_cuda, tkdev, dim):
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 64), (128, 128), (256, 64), (256, 128)])
+def test_attention_of_prompts_in_every_form(torch_cuda, tkdev, dim, group, dtype):
+    c = Case(torch_cuda, 81, [900, 17, 0, 300], [129, 17, 0, 40], 9, 3, dim, group, 32, dtype, spare=100)
+    c.check(c.run(tkdev, c.upload()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,group,hk", [(128, 64, 20), (128, 128, 12), (256, 64, 8), (256, 128, 8)])
+def test_long_prompts_set_their_sums_aside(torch_cuda, tkdev, dim, group, hk, dtype):
+    """Runs of more steps than the sums of the tensor core are left to themselves."""
+    c = Case(torch_cuda, 82, [5000] * 3, [161] * 3, hk, hk, dim, group, 16, dtype)
+    c.check(c.run(tkdev, c.upload()))
+
+
+@pytest.mark.parametrize("dim,group,dtype", [(64, 64, "f16"), (128, 128, "f16"), (128, 64, "f32"), (256, 64, "bf16")])
+def test_prompts_with_absent_pages_and_anything_in_masked_places(torch_cuda, tkdev, dim, group, dtype):
     """Pages that are not in the cache (more than a step of them, and the whole of a sequence), and
     NaN and infinities in scales behind the last token, in pages of nobody and in the last query's own
     position, which only it sees."""
-    c = Case(torch_cuda, 61, [700, 2500, 40], [100, 40, 40], 4, 2, dim, dim, 16, "f16", spare=6000)
+    c = Case(torch_cuda, 61, [700, 2500, 40], [100, 40, 40], 4, 2, dim, group, 16, dtype, spare=6000)
     c.tables[0, 3:14] = -1
     c.tables[1, :140] = c.blocks
     c.tables[2, :] = [-5, 2**31 - 1, -2**31] + [-1] * (c.width - 3)
@@ -479,8 +494,8 @@ def test_prompts_in_place_strided_and_repeated(torch_cuda, tkdev, dtype):
     assert (wide == 9).all()
 
 
-@pytest.mark.parametrize("dtype,group,spare", [("f16", 128, 6000), ("bf16", 128, 6000), ("f32", 128, 2),
-                                               ("f32", 64, 2), ("bf16", 64, 2)])
+@pytest.mark.parametrize("dtype,group,spare", [("f16", 128, 6000), ("bf16", 128, 6000), ("f32", 128, 6000),
+                                               ("bf16", 64, 6000), ("f32", 128, 2), ("f32", 64, 2), ("bf16", 64, 2)])
 def test_prompts_with_scales_of_every_kind(torch_cuda, tkdev, dtype, group, spare):
     """Scales of 0, of either sign, the smallest subnormal and sizes far apart; queries of every size;
     a row of queries with an infinity gives NaN and no other row does."""
