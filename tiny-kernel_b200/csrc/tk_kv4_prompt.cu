@@ -1,29 +1,31 @@
 // tk_kv4_prompt.cu -- attention over the 4-bit cache for many query rows a key head: prompts and
 // their chunks.
 //
-// The mathematics is that of tk_kv4_attention.cu, with one group a head and queries of 16 bits, and
-// the products on tcgen05: a tile is 128 rows (query token, head of the group) against 128 tokens a
-// step.
-//   S = Q (c - 8)^T    Q as it is (f16 or bf16), the codes exact in either
-//   t = a S + b sum(q) + log2 |s_v|      a = f s_k, b = f (m_k + 8 s_k), f = scale log2 e
-//   w = 2^(t - r),  O += w sign(s_v) (c - 8),  l += w / |s_v|,  off += w (m_v + 8 s_v) / |s_v|
-// and o = (O + off) / l.  So a weight comes out of the exponential with its scale in it, ready for
-// the second product; it is split into two f16 (22 bits), two products into one accumulator.
-// s_v = 0 counts as 1 with values of 0.  A row's reference r keeps the weights below 2^15; when one
-// would pass, r is moved so that the largest is 2^10, and the sums are rescaled, which is rare.
+// The mathematics is that of tk_kv4_attention.cu, with the products on tcgen05: a tile is 128 rows (query
+// token, head of the group) against 64 or 128 tokens a step.  For each group of dimensions
+//   S = Q (c - 8)^T    Q as it is (f16 or bf16; f32 as two f16, 22 bits of the row's largest), the codes exact
+//   t = sum over groups of (a S + b sum(q)) + e,   a = f s_k, b = f (m_k + 8 s_k), f = scale log2 e
+//   w = 2^(t - r + log2 |s_v| - e),  O += w sign(s_v) (c - 8),  off += w (m_v + 8 s_v) / |s_v|
+// with e the largest log2 |s_v| of the token's groups; l += w / |s_v| of the first; o = (O + off) / l.  So
+// a weight comes out of the exponential with its scale in it, ready for the second product; it is split
+// into two f16 (22 bits), two products into one accumulator.  s_v = 0 counts as 1 with values of 0.  A
+// row's reference r keeps the weights below 2^15; when one would pass, r is moved so that the largest is
+// 2^10, and the sums are rescaled, which is rare.
 //
-// One CTA is 256 threads, two a row: tokens 0-63 and 64-127 of a step, and half of the dimensions of
-// O.  Tensor memory: S (128 columns), over which the weights lie as f16 pairs once all of S has been
-// read, and O.  A step is one chain (unpack keys, S, weights, O), so two CTAs live on an SM, one
+// One CTA is 256 threads, two a row: half of a step's tokens each, and half of the dimensions of O.
+// Tensor memory: S, over which the weights lie as f16 pairs once all of S has been read, and O.  A step
+// is one chain (unpack keys, S, weights, O), so two CTAs live on an SM (one at 256 dimensions), one
 // computing while the other's products run.  Warps wait for products, the two of a row for each other,
 // and one, which issues the products, for all.  The next step's codes travel meanwhile: those of keys
 // into the operand's own rows, whose products have completed.
 //   The tensor core's sums round toward zero: O is set aside into the CTA's slot of the workspace, in
-// f32 additions, every kFlush steps.
+// f32 additions, every 2048 tokens (512 of f32 queries, whose outputs would show it).  S has eight
+// products a row, sixteen of f32 queries: 2.9e-6 of the result against 1.4e-6 of f32 sums in torch (2 x
+// 256 tokens over 1500 to 4000 positions); the exact integers of smaller tiles give 0.8e-6.
 //
-// What bounds it (B200; 2 x 256 tokens over 1500 to 4000 positions, 40 + 8 heads of 128, bf16): 112 us,
-// 290 TFLOP/s with one product each (the second part of the weights is a third one); tiles of eight rows
-// on mma.sync take 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
+// What bounds it (B200; those 2 x 256 tokens, 40 + 8 heads of 128, bf16): 115 us, 280 TFLOP/s with one
+// product each (the second part of the weights is a third one); tiles of eight rows on mma.sync take 299.
+// f32: 157 and 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
 // cycle and scheduler, four warps a scheduler (128 registers, most of them scores), tensor pipe 24 %
 // busy.  Numbers of tokens for eight instead of four columns at a time: 125 us, spilled.  One f16 part of
 // a weight instead of two: 102 us, but 11 bits.
@@ -891,16 +893,19 @@ cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStr
 
 }  // namespace
 
-// Queries of 16 bits (one product with them is exact), one group a head, and on the mean enough rows a
-// sequence: against tiles of eight rows, 16 x 2000 positions with 32 rows a head take 64 us instead of
-// 53, with 48 65 instead of 73, with 128 70 instead of 168; 60000 positions 110 and 75, 111 and 106, 114
-// and 255.  A step is long, so little work in all wants more rows (one sequence of 3000, by the table's
-// reach: 48 rows 29 and 19 us, 128 rows 32 and 28, 256 rows 33 and 40).
+// On the mean enough rows a sequence.  Against tiles of eight rows, four heads a group of 128, 16 x 2000
+// positions with 32 rows take 64 us instead of 53, with 48 65 instead of 73, with 128 70 instead of 168
+// (f32: 82 and 52, 83 and 73, 94 and 168; 256 dimensions, two groups: 141 and 99, 142 and 140); 60000
+// positions 110 and 75, 111 and 106, 114 and 255.  A step is long, so little work in all wants more rows:
+// one sequence of 3000, by the table's reach, with 128 rows 32 us instead of 28, with 256 33 instead of 40
+// (f32: 41 and 28, 43 and 43; 256 dimensions: 34 and 44 with 128, 33 and 29 with 64).
 bool kv4_prompt_takes(const Kv4AttentionParams& p, int dtype) {
+  const bool wide = dtype == kTypeF32, large = p.cache.head_dim == 256;
   const long long rows = (long long)p.tokens * (p.q_heads / p.cache.kv_heads);
   const long long tiles = (rows / kRows + p.batch) * p.cache.kv_heads;
   const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost;
-  return rows >= 160ll * p.batch || (rows >= 48ll * p.batch && tiles * steps >= 600);
+  const long long few = (wide ? 256 : 160) / (large ? 2 : 1), many = wide ? 64 : 48;
+  return rows >= few * p.batch || (rows >= many * p.batch && tiles * steps >= 600);
 }
 
 size_t kv4_prompt_workspace(int head_dim, int sm_count) {
