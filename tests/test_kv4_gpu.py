@@ -670,14 +670,15 @@ class Server:
 STEPS = [[5, 0, 30], [1, 17, 1], [1, 1, 1], [3, 1, 0], [1, 40, 1]]
 
 
-@pytest.mark.parametrize("dtype,hq,hk,dim", [("f32", 4, 2, 128), ("bf16", 6, 1, 64), ("f16", 2, 2, 256)])
-def test_steps_together_and_captured(torch_cuda, tkdev, dtype, hq, hk, dim):
+@pytest.mark.parametrize("dtype,hq,hk,dim,most", [("f32", 4, 2, 128, 50), ("bf16", 6, 1, 64, 50), ("f16", 2, 2, 256, 50),
+                                                  ("bf16", 8, 2, 128, 250), ("f32", 8, 1, 256, 250)])
+def test_steps_together_and_captured(torch_cuda, tkdev, dtype, hq, hk, dim, most):
     """Prompts, then single tokens and chunks, of three requests: every step's outputs against the
     oracle over the keys and values of all steps; then the same steps as replays of one captured
     graph (on a stream of its own, with other lengths each time): the same bits."""
     torch = torch_cuda
-    plain = Server(torch, tkdev, 3, 50, hq, hk, dim, dtype)
-    graphed = Server(torch, tkdev, 3, 50, hq, hk, dim, dtype)
+    plain = Server(torch, tkdev, 3, most, hq, hk, dim, dtype)
+    graphed = Server(torch, tkdev, 3, most, hq, hk, dim, dtype)
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
@@ -719,6 +720,37 @@ def test_steps_together_and_captured(torch_cuda, tkdev, dtype, hq, hk, dim):
         plain.advance()
         graphed.advance()
     del graph
+
+
+def test_pages_past_four_gigabytes(torch_cuda, tkdev):
+    """The last pages of a cache whose codes have more than 2^32 bytes, and the first of a small one:
+    the same keys and values, the same outputs of one token and of a prompt, to the bit."""
+    torch = torch_cuda
+    hq, hk, dim, ctx, pages = 16, 8, 128, 200, 13
+    gen = torch.Generator(device="cuda").manual_seed(91)
+    draw = lambda n, h: torch.randn((n, h * dim), generator=gen, device="cuda").half()
+    k, v, q = draw(ctx, hk), draw(ctx, hk), draw(100, hq)
+    got = []
+    for blocks in (pages, 600000):
+        assert blocks == pages or blocks * hk * 16 * dim // 2 > 2**32
+        codes = [torch.empty((blocks, hk, 16, dim // 2), dtype=torch.uint8, device="cuda") for _ in "kv"]
+        pairs = [torch.empty((blocks, hk, 16, 1, 2), dtype=torch.float16, device="cuda") for _ in "kv"]
+        cache = ops.kv4_cache(*codes, *pairs, blocks, hk, 16, dim, dim)
+        table = torch.arange(blocks - pages, blocks, dtype=torch.int32, device="cuda")
+        slots = (table[:, None] * 16 + torch.arange(16, dtype=torch.int32, device="cuda")).flatten()[:ctx].contiguous()
+        size = ops.kv4_attention_workspace(tkdev, cache, hq)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        back, one, many = [torch.zeros_like(k) for _ in "kv"], torch.zeros_like(q[:1]), torch.zeros_like(q)
+        lens, start = i32(torch, [ctx]), i32(torch, [0, 100])
+        torch.cuda.synchronize()
+        ops.kv4_append(tkdev, cache, k, v, slots, ctx, "f16")
+        ops.kv4_gather(tkdev, cache, slots, *back, ctx, "f16")
+        ops.kv4_attention(tkdev, cache, q, table, lens, None, one, ws, size, 1, 1, hq, pages, dim ** -0.5, "f16")
+        ops.kv4_attention(tkdev, cache, q, table, lens, start, many, ws, size, 100, 1, hq, pages, dim ** -0.5, "f16")
+        got.append(back + [one, many])
+        del codes, pairs
+    assert all(torch.equal(x, y) for x, y in zip(*got)) and got[0][3].isfinite().all()
+    assert (got[0][0] - k).abs().max() < 0.6  # half of a fifteenth of a row's range
 
 
 def test_two_streams_with_their_own_workspaces(torch_cuda, tkdev):
