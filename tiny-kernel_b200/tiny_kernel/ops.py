@@ -13,12 +13,12 @@ from ._lib import Int4MatrixC, Kv4CacheC, check
 
 
 def _ptr(v) -> int:
+    if type(v) is int or v is None:
+        return v
     try:
         return v.data_ptr()
     except AttributeError:
         pass
-    if v is None or type(v) is int:
-        return v
     if hasattr(v, "ptr"):
         return v.ptr
     return int(v)
