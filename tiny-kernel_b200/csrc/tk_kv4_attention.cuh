@@ -13,8 +13,10 @@ namespace {
 
 constexpr int kStep = 128;  // tokens of a step
 // Steps that a tile costs beside its own: queries, first loads, join (48 sequences of 64 to 8192: 65.3 us
-// with 1, 61.6 with 2, 60.6 with 3; 32 of 512: 15.2, 15.5, 17.5).
-constexpr int kTileCost = 2;
+// with 1, 61.6 with 2, 60.6 with 3; 32 of 512: 15.2, 15.5, 17.5.  Prompts, whose steps are longer: 2 x 256
+// tokens over 1500 to 4000 positions 110, 115, 115; over themselves 33, 38, 39; 16 x 12 over 2000 65, 64, 70).
+template <int ROWS>
+constexpr int kTileCost = ROWS > 8 ? 1 : 2;
 
 // Work is (sequence, key head, row tile, step of 128 tokens) in this order, cut into equal runs, one
 // per CTA; a tile counts kTileCost steps more than it has, before its first.  So long and short
@@ -112,7 +114,7 @@ __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b,
   s.last = len - s.n;
   s.kv = (int)min((long long)len, (long long)p.max_blocks << p.cache.shift);
   s.tiles = (int)(((long long)s.n * per + ROWS - 1) / ROWS);
-  s.steps = kTileCost + (s.kv + kStep - 1) / kStep;  // kv < 2^31 - 1024
+  s.steps = kTileCost<ROWS> + (s.kv + kStep - 1) / kStep;  // kv < 2^31 - 1024
   return s;
 }
 

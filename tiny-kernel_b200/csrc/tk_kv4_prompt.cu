@@ -21,14 +21,14 @@
 //   The tensor core's sums round toward zero: O is set aside into the CTA's slot of the workspace, in
 // f32 additions, every 2048 tokens (512 of f32 queries, whose outputs would show it).  S has eight
 // products a row, sixteen of f32 queries: 2.9e-6 of the result against 1.4e-6 of f32 sums in torch (2 x
-// 256 tokens over 1500 to 4000 positions); the exact integers of smaller tiles give 0.8e-6.
+// 256 tokens over 1500 to 4000 positions); the exact integers of smaller tiles give 0.4 to 1.2e-6.
 //
-// What bounds it (B200; those 2 x 256 tokens, 40 + 8 heads of 128, bf16): 115 us, 280 TFLOP/s with one
+// What bounds it (B200; those 2 x 256 tokens, 40 + 8 heads of 128, bf16): 110 us, 295 TFLOP/s with one
 // product each (the second part of the weights is a third one); tiles of eight rows on mma.sync take 299.
-// f32: 157 and 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
+// f32: 149 and 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
 // cycle and scheduler, four warps a scheduler (128 registers, most of them scores), tensor pipe 24 %
-// busy.  Numbers of tokens for eight instead of four columns at a time: 125 us, spilled.  One f16 part of
-// a weight instead of two: 102 us, but 11 bits.
+// busy.  When a call took 118 us, numbers of tokens for eight instead of four columns at a time made it
+// 125 (spilled); when it took 112, one f16 part of a weight instead of two 102, with 11 bits.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
     auto sees = [&](int i) { return min(cur.s.kv, cur.s.last + min(row0 + i, end) / per + 1); };
     const int see = sees(row), see_least = sees(0), see_most = max(sees(kRows - 1), 0);
     constexpr int kParts = kStep / TOK;  // steps here of one of the partition's
-    const int s0 = max(cur.c0 - kTileCost, 0) * kParts;
-    const int s1 = min(max(cur.c1 - kTileCost, 0) * kParts, (see_most + TOK - 1) / TOK);
+    const int s0 = max(cur.c0 - kTileCost<kRows>, 0) * kParts;
+    const int s1 = min(max(cur.c1 - kTileCost<kRows>, 0) * kParts, (see_most + TOK - 1) / TOK);
     const int slot = at == r.start ? 0 : 1;
     // where the half's dimensions c .. c + 3 are set aside: (half * D / 8 + c / 4) * kRows + row
     float4* set_aside = reinterpret_cast<float4*>(sums + ((size_t)blockIdx.x * 2 + slot) * kSlot) + half * (D / 8) * kRows + row;
@@ -903,7 +903,7 @@ bool kv4_prompt_takes(const Kv4AttentionParams& p, int dtype) {
   const bool wide = dtype == kTypeF32, large = p.cache.head_dim == 256;
   const long long rows = (long long)p.tokens * (p.q_heads / p.cache.kv_heads);
   const long long tiles = (rows / kRows + p.batch) * p.cache.kv_heads;
-  const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost;
+  const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost<kRows>;
   const long long few = (wide ? 256 : 160) / (large ? 2 : 1), many = wide ? 64 : 48;
   return rows >= few * p.batch || (rows >= many * p.batch && tiles * steps >= 600);
 }
