@@ -37,6 +37,16 @@ int kv4_index_tokens_in(int ctx, int q, int j, int shift) {
   return slots_tokens_in(r, j, shift);
 }
 
+long long kv4_index_prompt_work(int tiles, int per, int cost, int last, int kv) {
+  return prompt_work(prompt_tiles(tiles, per, cost, last, kv));
+}
+int kv4_index_prompt_steps(int tiles, int per, int cost, int last, int kv, int tile) {
+  return prompt_steps(prompt_tiles(tiles, per, cost, last, kv), tile);
+}
+int kv4_index_prompt_find(int tiles, int per, int cost, int last, int kv, long long x, int* at) {
+  return prompt_find(prompt_tiles(tiles, per, cost, last, kv), x, at);
+}
+
 int kv4_index_new_block(const int* list, int begin, int end, long long a, int num_blocks) {
   return slots_new_block(list, begin, end, a, num_blocks);
 }

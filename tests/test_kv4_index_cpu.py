@@ -24,6 +24,9 @@ def index():
     L.kv4_index_request.argtypes, L.kv4_index_request.restype = [i, i, n, i, i, i, C.c_void_p], None
     L.kv4_index_tokens_in.argtypes = [i] * 4
     L.kv4_index_new_block.argtypes = [C.c_void_p, i, i, n, i]
+    L.kv4_index_prompt_work.argtypes, L.kv4_index_prompt_work.restype = [i] * 5, n
+    L.kv4_index_prompt_steps.argtypes = [i] * 6
+    L.kv4_index_prompt_find.argtypes = [i] * 5 + [n, C.c_void_p]
     return L
 
 
@@ -74,6 +77,39 @@ def test_pages_off_the_free_list(index):
     assert [get(-4, 2, a) for a in range(3)] == [3, -1, -1]  # a negative begin counts as 0
     assert get(5, 0, 0) == get(0, INT_MIN, 0) == get(0, 0, 0) == -1
     assert get(INT_MAX, 5, 2**40) == -1
+
+
+@pytest.mark.parametrize("per", [1, 2, 3, 5, 128, 200])
+def test_work_of_prompts(index, per):
+    """A tile's steps cover what its last row sees, by less than two steps; the sums over tiles and the
+    search for a step agree with counting one by one."""
+    at = C.c_int()
+    for n, length, reach, cost in [(1, 1, 999, 1), (1, 0, 999, 1), (200, 50, 999, 1), (300, 300, 2000, 2), (700, 700, 400, 1),
+                                   (129, 5000, 9000, 1), (257, 4000, 4096, 1), (640, 100, 999, 1), (1000, 1000, 1024, 1)]:
+        last, kv, tiles = length - n, min(length, reach), -(-n * per // 128)
+        args = (tiles, per, cost, last, kv)
+        steps = [index.kv4_index_prompt_steps(*args, t) for t in range(tiles)]
+        for t, s in enumerate(steps):
+            sees = min(kv, last + min((t + 1) * 128 - 1, n * per - 1) // per + 1)
+            assert -(-max(sees, 0) // 128) <= s - cost <= min(-(-max(sees, 0) // 128) + 1, -(-kv // 128))
+        assert index.kv4_index_prompt_work(*args) == sum(steps)
+        x = 0
+        for t, s in enumerate(steps):
+            for j in {0, s // 2, s - 1}:
+                assert index.kv4_index_prompt_find(*args, x + j, C.byref(at)) == t and at.value == j
+            x += s
+
+
+def test_work_of_the_largest_prompts(index):
+    """2^30 rows, or 2^31 positions: no overflow, and the last step lies in the last tile."""
+    at = C.c_int()
+    for n, per, kv in [(2**30, 1, 2**31 - 2048), (2**14, 2**16 - 1, 2**31 - 2048), (2**30, 1, 2**30), (1, 2**16 - 1, 1)]:
+        tiles = -(-n * per // 128)
+        args = (tiles, per, 1, kv - n, kv)
+        work, last = index.kv4_index_prompt_work(*args), index.kv4_index_prompt_steps(*args, tiles - 1)
+        assert tiles <= work <= tiles * (kv // 128 + 2)
+        assert index.kv4_index_prompt_find(*args, work - 1, C.byref(at)) == tiles - 1 and at.value == last - 1
+        assert index.kv4_index_prompt_find(*args, 0, C.byref(at)) == 0 and at.value == 0
 
 
 def test_numpy_numbers_pass_as_arguments():

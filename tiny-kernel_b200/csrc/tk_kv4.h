@@ -104,6 +104,52 @@ TK_HD int slots_new_block(const int* free_blocks, int begin, int end, long long 
   return id >= 0 && id < num_blocks ? id : -1;
 }
 
+// ---- the work of a prompt ------------------------------------------------------------------------
+
+// Tiles of 128 rows (query token, head of the group) of a sequence against steps of 128 positions: the
+// tiles of 128 tokens, `per` of them, count as many steps as the last of those tokens sees, and `cost`.
+// So the steps grow by one from each `per` tiles to the next, and their sums have a closed form.
+struct PromptTiles {
+  int tiles, per, cost;
+  int base;  // steps that the token before the first sees; negative where it sees nothing
+  int most;  // of the sequence
+};
+TK_HD PromptTiles prompt_tiles(int tiles, int per, int cost, int last, int kv) {  // last: kv_len less the query tokens
+  const int base = last > 0 ? last / 128 + (last % 128 != 0) : last / 128;
+  return {tiles, per, cost, base, kv / 128 + (kv % 128 != 0)};
+}
+TK_HD int prompt_steps(const PromptTiles& t, int tile) {
+  const int i = t.base + tile / t.per + 1;
+  return t.cost + (i < 0 ? 0 : i < t.most ? i : t.most);
+}
+// The sum of i up to x, each within 0 .. most.
+TK_HD long long prompt_sum(long long x, long long most) {
+  return x <= 0 ? 0 : x <= most ? x * (x + 1) / 2 : most * (most + 1) / 2 + (x - most) * most;
+}
+// Steps of the first n times `per` tiles.
+TK_HD long long prompt_before(const PromptTiles& t, int n) {
+  return t.per * (prompt_sum((long long)t.base + n, t.most) - prompt_sum(t.base, t.most) + (long long)t.cost * n);
+}
+TK_HD long long prompt_work(const PromptTiles& t) {
+  const int n = t.tiles / t.per, rest = t.tiles - n * t.per;
+  return prompt_before(t, n) + (rest ? (long long)rest * prompt_steps(t, n * t.per) : 0);
+}
+// The tile that step x of all (below prompt_work) lies in, and its place there.
+TK_HD int prompt_find(const PromptTiles& t, long long x, int* at) {
+  int lo = 0, hi = t.tiles / t.per;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    if (prompt_before(t, mid) <= x)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const long long rest = x - prompt_before(t, lo);
+  const int steps = prompt_steps(t, lo * t.per), i = (int)(rest / steps);
+  *at = (int)(rest - (long long)i * steps);
+  return lo * t.per + i;
+}
+
 }  // namespace tk
 
 #if defined(__CUDACC__)

@@ -252,8 +252,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
     pair_src = reinterpret_cast<const uint8_t*>(lane < 16 ? p.cache.k_scales : p.cache.v_scales) +
                head_at / (S::kRowBytes / NG / 4) + (lane & 15) * 16;
     table = p.block_tables + (size_t)x.b * p.max_blocks;
-    s0 = max(x.c0 - kTileCost<ROWS>, 0);
-    s1 = max(x.c1 - kTileCost<ROWS>, 0);
+    s0 = max(x.c0 - kTileCost, 0);
+    s1 = max(x.c1 - kTileCost, 0);
     see_most = sees(x, ROWS - 1);
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
       __syncthreads();
 
       {
-        const bool whole = done.c0 == 0 && done.c1 == done.s.steps;
+        const bool whole = done.c0 == 0 && done.c1 == done.steps;
         const int row0 = done.rt * ROWS, rows = min(ROWS, done.s.n * per - row0), slot = done_at == start ? 0 : 1;
         constexpr int kThreadsRow = kThreads / ROWS;
         const int row = tid / kThreadsRow, d0 = tid % kThreadsRow;
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
           out[ROWS * D + 2 * row + 1] = sum;
         }
         if (!whole && done.c0 == 0 && tid == 0) {  // the tile begins here: where its parts are
-          const long long end = done_at + done.s.steps;
+          const long long end = done_at + done.steps;
           parts[blockIdx.x] =
               Part{done.s.first, rows, done.head, (int)((end - 1) / run - blockIdx.x + 1), row0, slot, 0, 0};
         }
@@ -732,7 +732,7 @@ cudaError_t launch(Kv4AttentionParams p, int dtype, int sm_count, cudaStream_t s
   // 56 parts: 3.8 us with 4, 2.3 with 8; 8 x 2000, 7 parts: 0.6 us less with 4), many tiles want fewer
   // CTAs, most of which have nothing to do (48 x 4096: 1 us less with four rows a CTA than with two).
   const long long tiles = ((long long)p.tokens * (p.q_heads / p.cache.kv_heads) / ROWS + p.batch) * p.cache.kv_heads;
-  const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost<ROWS>;
+  const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost;
   if (tiles <= sm_count && std::min(steps, ctas / tiles) > 16) {
     cfg.gridDim = dim3((unsigned)ctas, ROWS / 2);
     cfg.blockDim = dim3(2 * 8 * 32);

@@ -13,10 +13,9 @@ namespace {
 
 constexpr int kStep = 128;  // tokens of a step
 // Steps that a tile costs beside its own: queries, first loads, join (48 sequences of 64 to 8192: 65.3 us
-// with 1, 61.6 with 2, 60.6 with 3; 32 of 512: 15.2, 15.5, 17.5.  Prompts, whose steps are longer: 2 x 256
-// tokens over 1500 to 4000 positions 110, 115, 115; over themselves 33, 38, 39; 16 x 12 over 2000 65, 64, 70).
-template <int ROWS>
-constexpr int kTileCost = ROWS > 8 ? 1 : 2;
+// with 1, 61.6 with 2, 60.6 with 3; 32 of 512: 15.2, 15.5, 17.5.  Prompts: 2 x 256 tokens over 1500 to
+// 4000 positions 113, 110, 116; 2048 tokens over themselves 140, 133, 133; 2 x 256 of them 34.5, 35.7, 39.4).
+constexpr int kTileCost = 2;
 
 // Work is (sequence, key head, row tile, step of 128 tokens) in this order, cut into equal runs, one
 // per CTA; a tile counts kTileCost steps more than it has, before its first.  So long and short
@@ -98,8 +97,19 @@ struct Sequence {
   int kv;           // visible positions, at most the table's reach
   int last;         // kv_len - n: query i sees the positions below last + i + 1
   int tiles;        // row tiles
-  int steps;        // of a tile, its cost among them
+  int steps;        // of a tile that sees all of it, its cost among them
 };
+// Tiles of many rows count the steps that their own rows see (32 + 8 heads of 128, 2048 tokens over
+// themselves: 133 us instead of 194, 8192: 1.44 ms instead of 2.55), smaller ones all of the sequence's.
+constexpr int kManyRows = 128;
+__device__ __forceinline__ PromptTiles prompt_of(const Sequence& s, int per) {
+  return prompt_tiles(s.tiles, per, kTileCost, s.last, s.kv);
+}
+template <int ROWS>
+__device__ __forceinline__ long long work_of(const Sequence& s, int per) {  // of a key head
+  if constexpr (ROWS == kManyRows) return prompt_work(prompt_of(s, per));
+  return (long long)s.steps * s.tiles;
+}
 template <int ROWS>
 __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b, int per) {
   Sequence s;
@@ -114,14 +124,15 @@ __device__ __forceinline__ Sequence sequence(const Kv4AttentionParams& p, int b,
   s.last = len - s.n;
   s.kv = (int)min((long long)len, (long long)p.max_blocks << p.cache.shift);
   s.tiles = (int)(((long long)s.n * per + ROWS - 1) / ROWS);
-  s.steps = kTileCost<ROWS> + (s.kv + kStep - 1) / kStep;  // kv < 2^31 - 1024
+  s.steps = kTileCost + (s.kv + kStep - 1) / kStep;  // kv < 2^31 - 1024
   return s;
 }
 
 // The part of a tile that a run holds.
 struct Tile {
   int b, head, rt;  // sequence, key head, row tile
-  int c0, c1;       // steps, the tile's cost among them
+  int steps;        // of the tile, its cost among them
+  int c0, c1;       // those of the run
   Sequence s;
 };
 
@@ -142,7 +153,7 @@ __device__ __forceinline__ bool find_run(const Kv4AttentionParams& p, int per, P
   long long mine = 0;
   for (int b = b0; b < b1; ++b) {
     const Sequence s = sequence<ROWS>(p, b, per);
-    mine += (long long)s.steps * s.tiles * hk;
+    mine += work_of<ROWS>(s, per) * hk;
   }
   long long inc = mine;
 #pragma unroll
@@ -168,7 +179,7 @@ __device__ __forceinline__ bool find_run(const Kv4AttentionParams& p, int per, P
     int b = b0;
     for (;; ++b) {
       const Sequence s = sequence<ROWS>(p, b, per);
-      const long long w = (long long)s.steps * s.tiles * hk;
+      const long long w = work_of<ROWS>(s, per) * hk;
       if (start < at + w) break;
       at += w;
     }
@@ -178,15 +189,24 @@ __device__ __forceinline__ bool find_run(const Kv4AttentionParams& p, int per, P
   __syncthreads();
   cur.b = s_seq;
   cur.s = sequence<ROWS>(p, cur.b, per);
-  {
-    long long unit = (long long)((double)s_at / cur.s.steps);  // off by one at most
-    if (unit * cur.s.steps > s_at) --unit;
-    if ((unit + 1) * cur.s.steps <= s_at) ++unit;
-    cur.c0 = (int)(s_at - unit * cur.s.steps);
+  // which head, or head and tile, by a quotient in f64, off by one at most
+  const long long of_unit = ROWS == kManyRows ? work_of<ROWS>(cur.s, per) : cur.s.steps;
+  long long unit = (long long)((double)s_at / (double)of_unit);
+  if (unit * of_unit > s_at) --unit;
+  if ((unit + 1) * of_unit <= s_at) ++unit;
+  const long long rest = s_at - unit * of_unit;
+  if constexpr (ROWS == kManyRows) {
+    const PromptTiles t = prompt_of(cur.s, per);
+    cur.head = (int)unit;
+    cur.rt = prompt_find(t, rest, &cur.c0);
+    cur.steps = prompt_steps(t, cur.rt);
+  } else {
     cur.head = (int)unit / cur.s.tiles;
     cur.rt = (int)unit - cur.head * cur.s.tiles;
+    cur.c0 = (int)rest;
+    cur.steps = cur.s.steps;
   }
-  cur.c1 = (int)min((long long)cur.s.steps, cur.c0 + (stop - start));
+  cur.c1 = (int)min((long long)cur.steps, cur.c0 + (stop - start));
   r = Run{run, start, stop};
   return true;
 }
@@ -204,7 +224,8 @@ __device__ __forceinline__ void next_tile(const Kv4AttentionParams& p, int per, 
       } while (cur.s.tiles == 0);
     }
   }
-  cur.c1 = (int)min((long long)cur.s.steps, stop - at);
+  cur.steps = ROWS == kManyRows ? prompt_steps(prompt_of(cur.s, per), cur.rt) : cur.s.steps;
+  cur.c1 = (int)min((long long)cur.steps, stop - at);
 }
 
 // Joins the parts of the tile that begins in the run of CTA blockIdx.x, RC of its rows.  W warps a row,

@@ -25,7 +25,7 @@
 //
 // What bounds it (B200; those 2 x 256 tokens, 40 + 8 heads of 128, bf16): 110 us, 295 TFLOP/s with one
 // product each (the second part of the weights is a third one); tiles of eight rows on mma.sync take 299.
-// f32: 149 and 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
+// f32: 150 and 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
 // cycle and scheduler, four warps a scheduler (128 registers, most of them scores), tensor pipe 24 %
 // busy.  When a call took 118 us, numbers of tokens for eight instead of four columns at a time made it
 // 125 (spilled); when it took 112, one f16 part of a weight instead of two 102, with 11 bits.
@@ -40,7 +40,7 @@
 namespace tk {
 namespace {
 
-constexpr int kRows = 128, kThreads = 256;
+constexpr int kRows = kManyRows, kThreads = 256;
 constexpr unsigned kErrWait = 4u;  // a product never completed
 
 // Waits, a warp together, for the phase of `bar`; gives up, for good, after timeout_ns.
@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
     auto sees = [&](int i) { return min(cur.s.kv, cur.s.last + min(row0 + i, end) / per + 1); };
     const int see = sees(row), see_least = sees(0), see_most = max(sees(kRows - 1), 0);
     constexpr int kParts = kStep / TOK;  // steps here of one of the partition's
-    const int s0 = max(cur.c0 - kTileCost<kRows>, 0) * kParts;
-    const int s1 = min(max(cur.c1 - kTileCost<kRows>, 0) * kParts, (see_most + TOK - 1) / TOK);
+    const int s0 = max(cur.c0 - kTileCost, 0) * kParts;
+    const int s1 = min(max(cur.c1 - kTileCost, 0) * kParts, (see_most + TOK - 1) / TOK);
     const int slot = at == r.start ? 0 : 1;
     // where the half's dimensions c .. c + 3 are set aside: (half * D / 8 + c / 4) * kRows + row
     float4* set_aside = reinterpret_cast<float4*>(sums + ((size_t)blockIdx.x * 2 + slot) * kSlot) + half * (D / 8) * kRows + row;
@@ -754,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
     for (int g = 0; g < NG; ++g) row_off[(2 * g + half) * kRows + row] = off[g];
     __syncthreads();
     l += row_max[(1 - half) * kRows + row];
-    const bool whole = cur.c0 == 0 && cur.c1 == cur.s.steps;
+    const bool whole = cur.c0 == 0 && cur.c1 == cur.steps;
     const float g = aside_ref == ref ? 1.f : ex2(aside_ref - ref);  // (neither has one yet: 1)
     const int i = min(row0 + row, end), token = i / per;
     const long long o_at = (long long)(cur.s.first + token) * p.o_stride + (long long)(cur.head * per + i - token * per) * D +
@@ -787,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
       num[1] = l;
     }
     if (!whole && cur.c0 == 0 && tid == 0)
-      parts[blockIdx.x] = Part{cur.s.first, rows, cur.head, (int)((at + cur.s.steps - 1) / r.length - blockIdx.x + 1), row0,
+      parts[blockIdx.x] = Part{cur.s.first, rows, cur.head, (int)((at + cur.steps - 1) / r.length - blockIdx.x + 1), row0,
                                slot, 0, 0};
     at += cur.c1 - cur.c0;
     if (at >= r.stop) break;
@@ -903,7 +903,7 @@ bool kv4_prompt_takes(const Kv4AttentionParams& p, int dtype) {
   const bool wide = dtype == kTypeF32, large = p.cache.head_dim == 256;
   const long long rows = (long long)p.tokens * (p.q_heads / p.cache.kv_heads);
   const long long tiles = (rows / kRows + p.batch) * p.cache.kv_heads;
-  const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost<kRows>;
+  const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost;
   const long long few = (wide ? 256 : 160) / (large ? 2 : 1), many = wide ? 64 : 48;
   return rows >= few * p.batch || (rows >= many * p.batch && tiles * steps >= 600);
 }
