@@ -428,8 +428,8 @@ int tk_kv4_gather_async(tk_device *dev, const tk_kv4_cache *cache, const int32_t
  * largest magnitude, the weights with 22 bits, sums are f32 and do not depend on the run (fixed
  * order).  Scores have to fit f32; a query row that holds an infinity or a NaN gives NaN.
  * tokens * q_heads at most 2^30.
- * workspace: tk_kv4_attention_workspace bytes of device memory on a 16-byte boundary, not
- * initialised, for calls that do not run at the same time. */
+ * workspace: tk_kv4_attention_workspace bytes of device memory (20 to 40 MB) on a 16-byte boundary,
+ * not initialised, for calls that do not run at the same time. */
 int tk_kv4_attention_workspace(tk_device *dev, const tk_kv4_cache *cache, uint32_t q_heads,
                                size_t *bytes);
 int tk_kv4_attention(tk_device *dev, const tk_kv4_cache *cache, const void *q,
