@@ -18,10 +18,14 @@
 // computing while the other's products run.  Warps wait for products, the two of a row for each other,
 // and one, which issues the products, for all.  The next step's codes travel meanwhile: those of keys
 // into the operand's own rows, whose products have completed.
-//   The tensor core's sums round toward zero: O is set aside into the CTA's slot of the workspace, in
-// f32 additions, every 2048 tokens (512 of f32 queries, whose outputs would show it).  S has eight
-// products a row, sixteen of f32 queries: 2.9e-6 of the result against 1.4e-6 of f32 sums in torch (2 x
-// 256 tokens over 1500 to 4000 positions); the exact integers of smaller tiles give 0.4 to 1.2e-6.
+//   The tensor core's sums round toward zero: O is set aside into the CTA's slot of the workspace every
+// 2048 tokens (512 of f32 queries, whose outputs would show it), and l and off with it, each a sum of the
+// steps' sums until then.  Those additions are compensated: what one drops begins the next interval, O's in
+// tensor memory.  So an error does not grow with the length: equal tokens and weights, f32, 2048 positions in
+// one CTA 0.3e-6 of the result, 131072 0.3e-6 (as plain running sums 8e-6 and 325e-6; the chunk below 1 %
+// faster, 256 dimensions 2 % slower than those).  S has eight products a row, sixteen of f32 queries: 2.9e-6 of the result
+// against 1.4e-6 of f32 sums in torch (2 x 256 tokens over 1500 to 4000 positions); the exact integers of
+// smaller tiles give 0.4 to 1.2e-6.
 //
 // What bounds it (B200; those 2 x 256 tokens, 40 + 8 heads of 128, bf16): 110 us, 295 TFLOP/s with one
 // product each (the second part of the weights is a third one); tiles of eight rows on mma.sync take 299.
@@ -156,6 +160,14 @@ __device__ __forceinline__ void add_scaled(float4& x, const float4& y, float f) 
   x.y = fmaf(y.y, f, x.y);
   x.z = fmaf(y.z, f, x.z);
   x.w = fmaf(y.w, f, x.w);
+}
+// kept = kept * g + x, or x where nothing is kept yet.  Returns what its rounding drops, so that a long row of
+// such sums is off by no more than a short one (compensated summation).
+__device__ __forceinline__ float keep(bool any, float& kept, float g, float x) {
+  if (!any) kept = 0.f;
+  const float sum = fmaf(kept, g, x), drop = x + fmaf(kept, g, -sum);
+  kept = sum;
+  return drop;
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pack_out(float a, float b) {
@@ -361,6 +373,9 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
     const int slot = at == r.start ? 0 : 1;
     // where the half's dimensions c .. c + 3 are set aside: (half * D / 8 + c / 4) * kRows + row
     float4* set_aside = reinterpret_cast<float4*>(sums + ((size_t)blockIdx.x * 2 + slot) * kSlot) + half * (D / 8) * kRows + row;
+    // l goes where the row's reference and l are left at the tile's end, off where its parts meet there
+    auto aside_l = [&]() -> float& { return sums[((size_t)blockIdx.x * 2 + slot) * kSlot + kRows * D + 2 * row + half]; };
+    auto aside_off = [&](int y) -> float& { return row_off[(2 * y + half) * kRows + row]; };
     const int* table = p.block_tables + (size_t)cur.b * p.max_blocks;
 
     // ---- the loads of a step ----
@@ -539,22 +554,30 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
       fence_proxy_async_smem();
       if (pending) wait_products();
       if (since == M::kFlush) {
+        // the sums so far, of another reference perhaps; what rounding drops of them begins the next ones
+        const float g = aside_ref == ref ? 1.f : ex2(aside_ref - ref);  // (neither has one yet: 1)
+        l = keep(aside, aside_l(), g, l);
+#pragma unroll
+        for (int y = 0; y < NG; ++y) off[y] = keep(aside, aside_off(y), g, off[y]);
 #pragma unroll 1
         for (int c = 0; c < D / 2; c += 16) {
           uint32_t o[16];
           tmem_load16(t_o + c, o);
-          const float g = aside_ref == ref ? 1.f : ex2(aside_ref - ref);  // (neither has one yet: 1)
 #pragma unroll
           for (int k = 0; k < 16; k += 4) {
-            float4 x = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
-                                   __uint_as_float(o[k + 3]));
             float4* kept = set_aside + (c + k) / 4 * kRows;
-            if (aside) add_scaled(x, *kept, g);
+            float4 x = *kept;
+            o[k] = __float_as_uint(keep(aside, x.x, g, __uint_as_float(o[k])));
+            o[k + 1] = __float_as_uint(keep(aside, x.y, g, __uint_as_float(o[k + 1])));
+            o[k + 2] = __float_as_uint(keep(aside, x.z, g, __uint_as_float(o[k + 2])));
+            o[k + 3] = __float_as_uint(keep(aside, x.w, g, __uint_as_float(o[k + 3])));
             *kept = x;
           }
+          tmem_store16(t_o + c, o);
         }
+        tmem_st_wait();
         aside_ref = ref;
-        aside = fresh = true;
+        aside = true;
         since = 0;
       }
       arrive(&keys_bar);
@@ -673,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
         const Pair r2 = pair_of(r0, r0);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          Pair l2 = pair_of(l, 0.f), off2 = pair_of(off[g], 0.f);
+          Pair l2 = pair_of(0.f, 0.f), off2 = l2;  // of the step
 #pragma unroll
           for (int c = 0; c < T2 / 32; ++c) {
             uint32_t hi[16], lo[16];
@@ -713,8 +736,8 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
             tmem_store16(t_p + g * TOK + T2 + c * 16, lo);
           }
           const float2 a = values_of(l2), b = values_of(off2);
-          if (g == 0) l = a.x + a.y;
-          off[g] = b.x + b.y;
+          if (g == 0) l += a.x + a.y;
+          off[g] += b.x + b.y;
         }
       };
       if (masked)
@@ -749,13 +772,14 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
     if (pending) wait_products();
 
     // ---- the tile's end ----
+    const float g = aside_ref == ref ? 1.f : ex2(aside_ref - ref);  // (neither has one yet: 1)
+    if (aside) l = fmaf(aside_l(), g, l);
     row_max[half * kRows + row] = l;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) row_off[(2 * g + half) * kRows + row] = off[g];
+    for (int y = 0; y < NG; ++y) aside_off(y) = aside ? fmaf(aside_off(y), g, off[y]) : off[y];
     __syncthreads();
     l += row_max[(1 - half) * kRows + row];
     const bool whole = cur.c0 == 0 && cur.c1 == cur.steps;
-    const float g = aside_ref == ref ? 1.f : ex2(aside_ref - ref);  // (neither has one yet: 1)
     const int i = min(row0 + row, end), token = i / per;
     const long long o_at = (long long)(cur.s.first + token) * p.o_stride + (long long)(cur.head * per + i - token * per) * D +
                            half * (D / 2);
