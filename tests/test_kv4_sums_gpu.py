@@ -81,3 +81,15 @@ def test_long_prompts(torch_cuda, tkdev, dim, group, alike, scale):
     ctas = tkdev.sm_count() * (1 if dim == 256 else 2)
     got = repeated_page(torch_cuda, tkdev, dim + group, alike, 131072, 64, 1, 8, dim, group, scale, 2 * ctas)
     check(*got, 64 + 2 * 22 + 3 * 2)
+
+
+@pytest.mark.parametrize("alike,scale", [(True, 0.0), (False, 0.0), (False, 0.01)])
+@pytest.mark.parametrize("queries", [1, 2])
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 64), (128, 128), (256, 64), (256, 128)])
+def test_long_contexts_of_few_rows(torch_cuda, tkdev, dim, group, queries, alike, scale):
+    """Four rows (one token) and eight a tile.  Numerator: two products for each 16 tokens of a warp, 512 at
+    most before they are set aside: 64.  The offsets' sum and the denominator: 64 additions in a row in a lane,
+    5 of lanes, 4 of warps, each off by half of 2^-23: 37 each.  Sums of intervals are compensated: 2 more each."""
+    ctas = tkdev.sm_count() * (2 if dim == 256 else 3)
+    got = repeated_page(torch_cuda, tkdev, dim + group, alike, 524288, queries, 4, 8, dim, group, scale, 2 * ctas)
+    check(*got, 64 + 2 * 37 + 3 * 2)

@@ -365,8 +365,20 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
       float o[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      // Sums set aside, in the warp's place for the join: O with off_sum in it, and l behind it
       bool flushed = false;
-      int since = 0;  // steps since the sums were set aside
+      int since = 0;  // steps since then
+      auto aside_l = [&](int row) -> float& { return joint[(my_row + row) * M::kJoint + D]; };
+      auto sum_lanes = [&] {  // of a row, what they have of l and off_sum
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int off = kFour ? 2 : 4; off < 32; off <<= 1) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+#pragma unroll
+            for (int y = 0; y < NG; ++y) off_sum[y][i] += __shfl_xor_sync(0xffffffffu, off_sum[y][i], off);
+          }
+      };
 
       // ---- the steps ----
       int stage = 0;
@@ -518,6 +530,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
             for (int i = 0; i < NT; ++i)
 #pragma unroll
               for (int k = 0; k < 4; ++k) kept(i, k) *= k & 1 ? f1 : f0;
+            if (g == 0 && !low) {
+              aside_l(0) *= f0;
+              aside_l(1) *= f1;
+            }
           }
         }
         const float base[2] = {ref[0] == -INFINITY ? 0.f : 10.f - ref[0], ref[1] == -INFINITY ? 0.f : 10.f - ref[1]};
@@ -586,18 +602,26 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
           step_of(std::true_type{});
         else
           step_of(std::false_type{});
-        // The tensor core drops what lies under the last bit of a sum, always towards 0: its sums are
-        // set aside, in the warp's place for the join, before that adds up (f32 outputs over 8192 positions
-        // of one CTA: 2.8e-6 off without it).
+        // The tensor core drops what lies under the last bit of a sum, always towards 0, and f32 additions of
+        // equal weights round the same way each time: the sums are set aside before that adds up, each time
+        // starting with what the addition dropped (f32 outputs of one CTA, 8192 positions: 2.8e-6 off without it;
+        // 131072 equal tokens: 24e-6 with l and off_sum as running sums, now 1e-6, as over 2048; costs 2 %).
         if (++since == kFlush) {
           since = 0;
+          sum_lanes();
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              kept(i, k) = flushed ? kept(i, k) + o[i][k] : o[i][k];
-              o[i][k] = 0.f;
+              const float x = low ? o[i][k] * kCodes : fmaf(o[i][k], kCodes, off_sum[i / (G / 16)][k & 1]);
+              o[i][k] = keep(flushed, kept(i, k), 1.f, x) * (1.f / kCodes);
             }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            l[i] = g == 0 && !low ? keep(flushed, aside_l(i), 1.f, l[i]) : 0.f;
+#pragma unroll
+            for (int y = 0; y < NG; ++y) off_sum[y][i] = 0.f;
+          }
           flushed = true;
         }
       }
@@ -605,28 +629,21 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
       __syncwarp();
 
       // ---- join the four warps ----
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int off = kFour ? 2 : 4; off < 32; off <<= 1) {
-          l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
-#pragma unroll
-          for (int y = 0; y < NG; ++y) off_sum[y][i] += __shfl_xor_sync(0xffffffffu, off_sum[y][i], off);
-        }
+      sum_lanes();
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          float x = o[i][k];
+          float x = low ? o[i][k] * kCodes : fmaf(o[i][k], kCodes, off_sum[i / (G / 16)][k & 1]);
           if (flushed) x += kept(i, k);
           if (kFour) x += __shfl_xor_sync(0xffffffffu, x, 2);  // both parts
-          if (!low) kept(i, k) = fmaf(x, kCodes, off_sum[i / (G / 16)][k & 1]);
+          if (!low) kept(i, k) = x;
         }
       if (g == 0 && !low) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           joint[kCols * M::kJoint + 2 * (my_row + i)] = ref[i];
-          joint[kCols * M::kJoint + 2 * (my_row + i) + 1] = l[i];
+          joint[kCols * M::kJoint + 2 * (my_row + i) + 1] = flushed ? l[i] + aside_l(i) : l[i];
         }
       }
 

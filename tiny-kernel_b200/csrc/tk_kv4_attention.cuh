@@ -92,6 +92,15 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
   lo = pack_f16(a - half_lo(hi), b - half_hi(hi));
 }
 
+// kept = kept * g + x, or x where nothing is kept yet.  Returns what its rounding drops, so that a long row of
+// such sums is off by no more than a short one (compensated summation).
+__device__ __forceinline__ float keep(bool any, float& kept, float g, float x) {
+  if (!any) kept = 0.f;
+  const float sum = fmaf(kept, g, x), drop = x + fmaf(kept, g, -sum);
+  kept = sum;
+  return drop;
+}
+
 struct Sequence {
   int first, n;     // query tokens
   int kv;           // visible positions, at most the table's reach

@@ -161,14 +161,6 @@ __device__ __forceinline__ void add_scaled(float4& x, const float4& y, float f) 
   x.z = fmaf(y.z, f, x.z);
   x.w = fmaf(y.w, f, x.w);
 }
-// kept = kept * g + x, or x where nothing is kept yet.  Returns what its rounding drops, so that a long row of
-// such sums is off by no more than a short one (compensated summation).
-__device__ __forceinline__ float keep(bool any, float& kept, float g, float x) {
-  if (!any) kept = 0.f;
-  const float sum = fmaf(kept, g, x), drop = x + fmaf(kept, g, -sum);
-  kept = sum;
-  return drop;
-}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack_out(float a, float b) {
   if constexpr (!BF) return pack_f16(a, b);
