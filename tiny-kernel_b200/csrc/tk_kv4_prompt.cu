@@ -19,17 +19,18 @@
 // and one, which issues the products, for all.  The next step's codes travel meanwhile: those of keys
 // into the operand's own rows, whose products have completed.
 //   The tensor core's sums round toward zero: O is set aside into the CTA's slot of the workspace every
-// 2048 tokens (512 of f32 queries, whose outputs would show it), and l and off with it, each a sum of the
+// 2048 tokens (256 of f32 queries, whose outputs would show it), and l and off with it, each a sum of the
 // steps' sums until then.  Those additions are compensated: what one drops begins the next interval, O's in
 // tensor memory.  So an error does not grow with the length: equal tokens and weights, f32, 2048 positions in
-// one CTA 0.3e-6 of the result, 131072 0.3e-6 (as plain running sums 8e-6 and 325e-6; the chunk below 1 %
-// faster, 256 dimensions 2 % slower than those).  S has eight products a row, sixteen of f32 queries: 2.9e-6 of the result
-// against 1.4e-6 of f32 sums in torch (2 x 256 tokens over 1500 to 4000 positions); the exact integers of
-// smaller tiles give 0.4 to 1.2e-6.
+// one CTA 0.3e-6 of the result, 131072 0.3e-6 (as plain running sums 8e-6 and 325e-6).  S has eight products a
+// row; of f32 queries the low part's eight go first, whose sum has little to drop.  2 x 256 tokens over 1500 to
+// 4000 positions, f32: 1.36e-6 of the result, 1.44e-6 in f32 torch operations (the high part first, every 512
+// tokens: 2.84e-6 and 149 us instead of 157; the low part first alone 1.78e-6); the exact integers of smaller tiles give 0.4
+// to 1.2e-6.
 //
-// What bounds it (B200; those 2 x 256 tokens, 40 + 8 heads of 128, bf16): 110 us, 295 TFLOP/s with one
+// What bounds it (B200; those 2 x 256 tokens, 40 + 8 heads of 128, bf16): 109 us, 298 TFLOP/s with one
 // product each (the second part of the weights is a third one); tiles of eight rows on mma.sync take 299.
-// f32: 150 and 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
+// f32: 157 and 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
 // cycle and scheduler, four warps a scheduler (128 registers, most of them scores), tensor pipe 24 %
 // busy.  When a call took 118 us, numbers of tokens for eight instead of four columns at a time made it
 // 125 (spilled); when it took 112, one f16 part of a weight instead of two 102, with 11 bits.
@@ -246,7 +247,7 @@ struct Form {
   static constexpr int kTokens = kGroups == 1 && !(kF32 && D == 128) ? 128 : 64;
   static constexpr int kCtas = D == 256 ? 1 : 2;  // of an SM
   static constexpr uint32_t kTmem = 512 / kCtas, kTmemO = kTmem / 2;
-  static constexpr int kFlush = (kF32 ? 512 : 2048) / kTokens;
+  static constexpr int kFlush = (kF32 ? 256 : 2048) / kTokens;
   static constexpr int kLoaders = kThreads / kTokens;      // threads of a token
   static constexpr int kWords = D / kLoaders / 8;          // of codes, eight each, a thread
   // per token and group a, b, log2 |s_v| less the groups' largest, (m_v + 8 s_v) / |s_v|; per token the
@@ -581,12 +582,12 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int q = 0; q < (F32 ? 2 : 1); ++q)
+            for (int q = F32 ? 1 : 0; q >= 0; --q)  // the low part first
 #pragma unroll
               for (int i = 0; i < G / 16; ++i) {
                 const int kk = g * (G / 16) + i;
                 umma_f16(tmem + g * TOK, a + ((q * M::kQPart + (kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4),
-                         b + (((kk >> 2) * (TOK * 128) + (kk & 3) * 32) >> 4), idesc, q > 0 || i > 0);
+                         b + (((kk >> 2) * (TOK * 128) + (kk & 3) * 32) >> 4), idesc, q < (F32 ? 1 : 0) || i > 0);
               }
           umma_commit(&bar);
         }
