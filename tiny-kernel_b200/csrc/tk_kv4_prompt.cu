@@ -46,7 +46,7 @@ namespace tk {
 namespace {
 
 constexpr int kRows = kManyRows, kThreads = 256;
-constexpr unsigned kErrWait = 4u;  // a product never completed
+constexpr unsigned kErrPromptWait = 64u;  // a product, or a warp, of a prompt never completed
 
 // Waits, a warp together, for the phase of `bar`; gives up, for good, after timeout_ns.
 __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t phase, bool& dead, const Kv4AttentionParams& p) {
@@ -54,7 +54,7 @@ __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t phase, bool& 
     const uint64_t t0 = global_timer_ns();
     while (!mbar_try_wait(bar, phase))
       if (global_timer_ns() - t0 > p.timeout_ns) {
-        atomicOr(p.err, kErrWait);
+        atomicOr(p.err, kErrPromptWait);
         dead = true;
         break;
       }
