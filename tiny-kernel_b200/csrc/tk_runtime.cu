@@ -55,7 +55,7 @@ int fail(int status, const char* fmt, ...) {
 // A kernel launch on a device: counted (tk_device_launch_count), then checked.
 #define TK_LAUNCH(dev, expr) \
   do {                       \
-    ++(dev)->launches;       \
+    (dev)->launches.fetch_add(1, std::memory_order_relaxed); \
     TK_CUDA_TRY(expr);       \
   } while (0)
 
@@ -132,7 +132,7 @@ struct tk_device {
   unsigned scratch_gen = 0;  // bumped whenever a scratch buffer is reallocated
   std::vector<struct FfnGraph> ffn_graphs;  // synchronous TK_FFN_HOST_IO calls, recorded
   unsigned long long* trace = nullptr;  // [sm_count][kTraceEvents] when tracing is enabled
-  unsigned long long launches = 0;      // kernels enqueued through this device
+  std::atomic<unsigned long long> launches{0};  // kernels enqueued through this device, by any thread
   // timed-out peer-memory exchanges seen by tk_device_check_error: a tk_tp group created before
   // the latest one is out of step with its peers and refuses further exchanges
   unsigned p2p_timeouts = 0;
@@ -1111,7 +1111,7 @@ void tk_device_destroy(tk_device* d) {
 
 const char* tk_device_name(tk_device* d) { return d ? d->name : ""; }
 int tk_device_sm_count(tk_device* d) { return d ? d->sm_count : 0; }
-uint64_t tk_device_launch_count(tk_device* d) { return d ? d->launches : 0; }
+uint64_t tk_device_launch_count(tk_device* d) { return d ? d->launches.load(std::memory_order_relaxed) : 0; }
 void* tk_device_stream(tk_device* d) { return d ? static_cast<void*>(d->stream) : nullptr; }
 
 int tk_device_synchronize(tk_device* d) {
@@ -1589,7 +1589,7 @@ int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* 
   p.scale = scale;
   p.err = d->err;
   p.timeout_ns = d->timeout_ns;
-  ++d->launches;  // two kernels
+  d->launches.fetch_add(1, std::memory_order_relaxed);  // two kernels
   TK_LAUNCH(d, launch_kv4_attention(p, dtype, d->sm_count, pick_stream(d, stream)));
   return TK_OK;
 }
