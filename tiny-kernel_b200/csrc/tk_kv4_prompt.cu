@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
   constexpr uint32_t kO = M::kTmemO;
   extern __shared__ uint8_t dynamic[];
   __shared__ uint64_t bar, keys_bar, weights_bar;  // products complete; all warps' keys, weights written
+  __shared__ uint64_t all_bar;                     // (after a wait gave up) all products complete
   __shared__ uint32_t tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -297,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
   float *row_max = row_sum + NG * kRows, *row_off = row_max + 2 * kRows, *row_undo = row_off + 2 * NG * kRows;
   if (tid == 0) {
     mbar_init(&bar, 1);
+    mbar_init(&all_bar, 1);
     mbar_init(&keys_bar, kThreads / 32);
     mbar_init(&weights_bar, kThreads / 32);
     fence_mbar_init();
@@ -811,6 +813,16 @@ __global__ void __launch_bounds__(kThreads, Form<D, G, TYPE>::kCtas) kv4_prompt_
     next_tile<kRows>(p, per, at, r.stop, cur);
     tcgen05_fence_before();
     __syncthreads();  // the rows' numbers have been read
+  }
+  // After a wait that gave up products may be under way.  They read this block's shared memory and write its
+  // tensor memory, which is another's next: they are waited for, a millisecond at least.
+  if (warp == 0 && __any_sync(0xffffffffu, dead)) {
+    if (elect_one()) umma_commit(&all_bar);  // of all that this lane has issued
+    __syncwarp();
+    const uint64_t t0 = global_timer_ns(), most = p.timeout_ns > 1000000ull ? p.timeout_ns : 1000000ull;
+    while (!mbar_try_wait(&all_bar, 0) && global_timer_ns() - t0 < most) {
+    }
+    __syncwarp();
   }
   tcgen05_fence_before();
   __syncthreads();
