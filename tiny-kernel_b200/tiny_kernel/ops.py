@@ -12,16 +12,24 @@ from . import _lib
 from ._lib import Int4MatrixC, Kv4CacheC, check
 
 
+_NO_PTR = object()
+_tensors = set()  # kinds of objects that have a data_ptr() and no ptr
+
+
 def _ptr(v) -> int:
-    if type(v) is int or v is None:
+    kind = type(v)
+    if kind is int or v is None:
         return v
-    try:
+    if kind in _tensors:
         return v.data_ptr()
-    except AttributeError:
-        pass
-    if hasattr(v, "ptr"):
-        return v.ptr
-    return int(v)
+    ptr = getattr(v, "ptr", _NO_PTR)  # a Buffer's; no error where there is none
+    if ptr is not _NO_PTR:
+        return ptr
+    if not hasattr(v, "data_ptr"):
+        return int(v)
+    if hasattr(kind, "data_ptr"):
+        _tensors.add(kind)
+    return v.data_ptr()
 
 
 def _dev(device) -> int:
