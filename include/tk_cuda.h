@@ -319,6 +319,7 @@ int tk_paged_attention_async(tk_device *dev, const float *q, const float *k_cach
  * Every length, page and slot is read on the device, so a step captured into a CUDA graph is
  * replayed with other lengths: capture it with as many rows (max_tokens, tokens) as a step may
  * have; the rows behind the last token carry position -1 and slot -1 and are left as they were.
+ * A call of no tokens does nothing; its rows' pointers may be NULL.
  * No call keeps state, allocates or waits: calls on different streams or from different threads
  * are independent as long as they share no output and no workspace.  The _async forms take the
  * stream as all others do; cudaStreamLegacy ((void *)1) names the legacy default stream.

@@ -1416,7 +1416,7 @@ int tk_qk_norm_rope_async(tk_device* d, const void* q, const void* k, const floa
   int st = check_dtype(dtype);
   if (st != TK_OK) return st;
   if (flags & ~TK_ROPE_INTERLEAVED) return fail(TK_ERR_ARG, "unknown flags 0x%x", flags);
-  if ((q_heads && (!q || !q_out)) || (kv_heads && (!k || !k_out)) || !positions ||
+  if ((tokens && ((q_heads && (!q || !q_out)) || (kv_heads && (!k || !k_out)) || !positions)) ||
       (rot_dim && (!cos_cache || !sin_cache)))
     return fail(TK_ERR_ARG, "NULL argument");
   if (head_dim == 0 || head_dim % 2 || head_dim > 1024 || rot_dim % 2 || rot_dim > head_dim)
@@ -1437,10 +1437,10 @@ int tk_qk_norm_rope_async(tk_device* d, const void* q, const void* k, const floa
     if ((st = check_stride(name, out[i], width, &p.out_stride[i])) != TK_OK) return st;
     if (p.heads[i] && (!aligned_for(p.x[i], dtype) || !aligned_for(p.out[i], dtype)))
       return fail(TK_ERR_ARG, "%s is not aligned to its type", name);
-    if (p.heads[i] && p.x[i] == p.out[i] && p.in_stride[i] != p.out_stride[i])
+    if (tokens && p.heads[i] && p.x[i] == p.out[i] && p.in_stride[i] != p.out_stride[i])
       return fail(TK_ERR_ARG, "%s in place needs the same stride in and out", name);
   }
-  if (q_heads && kv_heads && q_out == k_out) return fail(TK_ERR_ARG, "two outputs are the same");
+  if (tokens && q_heads && kv_heads && q_out == k_out) return fail(TK_ERR_ARG, "two outputs are the same");
   DeviceScope scope;
   if ((st = scope.enter(d)) != TK_OK) return st;
   if (tokens == 0) return TK_OK;
@@ -1468,7 +1468,7 @@ int check_rows(const tk_kv4_cache* cache, Kv4View* view, const void* k, const vo
   int st = check_cache(cache, view);
   if (st != TK_OK) return st;
   if ((st = check_dtype(dtype)) != TK_OK) return st;
-  if (!k || !v || !slots) return fail(TK_ERR_ARG, "NULL argument");
+  if (tokens && (!k || !v || !slots)) return fail(TK_ERR_ARG, "NULL argument");
   if (!aligned_for(k, dtype) || !aligned_for(v, dtype)) return fail(TK_ERR_ARG, "k or v is not aligned to its type");
   if ((uint64_t)tokens * cache->kv_heads > (1u << 30))
     return fail(TK_ERR_ARG, "%u tokens of %u heads are too many for one call", tokens, cache->kv_heads);
@@ -1507,7 +1507,7 @@ int tk_kv4_gather_async(tk_device* d, const tk_kv4_cache* cache, const int32_t* 
   long long ks = 0, vs = 0;
   int st = check_rows(cache, &view, k, v, slots, tokens, k_stride, v_stride, dtype, &ks, &vs);
   if (st != TK_OK) return st;
-  if (k == v) return fail(TK_ERR_ARG, "two outputs are the same");
+  if (tokens && k == v) return fail(TK_ERR_ARG, "two outputs are the same");
   DeviceScope scope;
   if ((st = scope.enter(d)) != TK_OK) return st;
   if (tokens == 0) return TK_OK;
@@ -1554,7 +1554,7 @@ int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* 
   if (st != TK_OK) return st;
   if ((st = check_heads(p.cache, q_heads)) != TK_OK) return st;
   if ((st = check_dtype(dtype)) != TK_OK) return st;
-  if (!q || !block_tables || !kv_lens || !o || !workspace) return fail(TK_ERR_ARG, "NULL argument");
+  if ((tokens && (!q || !o)) || !block_tables || !kv_lens || !workspace) return fail(TK_ERR_ARG, "NULL argument");
   if (!aligned_for(q, dtype) || !aligned_for(o, dtype)) return fail(TK_ERR_ARG, "q or o is not aligned to its type");
   if (!aligned16(workspace)) return fail(TK_ERR_ARG, "the workspace must be on a 16-byte boundary");
   if (batch == 0 || batch > (1u << 24) || max_blocks == 0 || max_blocks > kMaxCount || tokens > kMaxCount ||
@@ -1569,7 +1569,7 @@ int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* 
   const uint64_t width = (uint64_t)q_heads * cache->head_dim;
   if ((st = check_stride("q", q_stride, width, &p.q_stride)) != TK_OK) return st;
   if ((st = check_stride("o", o_stride, width, &p.o_stride)) != TK_OK) return st;
-  if (q == o && p.q_stride != p.o_stride) return fail(TK_ERR_ARG, "in place needs the same stride in and out");
+  if (tokens && q == o && p.q_stride != p.o_stride) return fail(TK_ERR_ARG, "in place needs the same stride in and out");
   DeviceScope scope;
   if ((st = scope.enter(d)) != TK_OK) return st;
   const size_t need = kv4_attention_workspace(p.cache.head_dim, d->sm_count);
