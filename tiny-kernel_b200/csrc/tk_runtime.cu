@@ -18,6 +18,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -1329,6 +1330,13 @@ bool aligned_for(const void* p, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) & (dtype == TK_F32 ? 3u : 1u)) == 0;
 }
 
+// int32 and f32 arrays that a kernel reads or writes by elements.
+int check_words(std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(TK_ERR_ARG, "an int32 or f32 array is not aligned to its type");
+  return TK_OK;
+}
+
 // A stride of rows of `width` values: 0 is packed.
 int check_stride(const char* name, uint32_t stride, uint64_t width, long long* out) {
   if (stride != 0 && stride < width)
@@ -1383,9 +1391,11 @@ int tk_paged_slots_async(tk_device* d, const int32_t* context_lens, const int32_
       (uint64_t)num_blocks * block_size > kMaxCount || max_tokens == 0 || max_tokens > kMaxCount - 8)
     return fail(TK_ERR_ARG, "batch %u, max_blocks %u, num_blocks %u or max_tokens %u is out of range", batch,
                 max_blocks, num_blocks, max_tokens);
-  DeviceScope scope;
-  int st = scope.enter(d);
+  int st = check_words({context_lens, query_lens, free_blocks, free_range, block_tables, kv_lens, query_start, positions,
+                        slots, counts});
   if (st != TK_OK) return st;
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
   int shift = 0;
   while ((1u << shift) < block_size) ++shift;
   const SlotsParams p{context_lens, query_lens, free_blocks, free_range, block_tables, kv_lens, query_start,
@@ -1440,6 +1450,7 @@ int tk_qk_norm_rope_async(tk_device* d, const void* q, const void* k, const floa
     if (tokens && p.heads[i] && p.x[i] == p.out[i] && p.in_stride[i] != p.out_stride[i])
       return fail(TK_ERR_ARG, "%s in place needs the same stride in and out", name);
   }
+  if ((st = check_words({positions, q_weight, k_weight, cos_cache, sin_cache})) != TK_OK) return st;
   if (tokens && q_heads && kv_heads && q_out == k_out) return fail(TK_ERR_ARG, "two outputs are the same");
   DeviceScope scope;
   if ((st = scope.enter(d)) != TK_OK) return st;
@@ -1470,6 +1481,7 @@ int check_rows(const tk_kv4_cache* cache, Kv4View* view, const void* k, const vo
   if ((st = check_dtype(dtype)) != TK_OK) return st;
   if (tokens && (!k || !v || !slots)) return fail(TK_ERR_ARG, "NULL argument");
   if (!aligned_for(k, dtype) || !aligned_for(v, dtype)) return fail(TK_ERR_ARG, "k or v is not aligned to its type");
+  if ((st = check_words({slots})) != TK_OK) return st;
   if ((uint64_t)tokens * cache->kv_heads > (1u << 30))
     return fail(TK_ERR_ARG, "%u tokens of %u heads are too many for one call", tokens, cache->kv_heads);
   const uint64_t width = (uint64_t)cache->kv_heads * cache->head_dim;
@@ -1556,6 +1568,7 @@ int tk_kv4_attention_async(tk_device* d, const tk_kv4_cache* cache, const void* 
   if ((st = check_dtype(dtype)) != TK_OK) return st;
   if ((tokens && (!q || !o)) || !block_tables || !kv_lens || !workspace) return fail(TK_ERR_ARG, "NULL argument");
   if (!aligned_for(q, dtype) || !aligned_for(o, dtype)) return fail(TK_ERR_ARG, "q or o is not aligned to its type");
+  if ((st = check_words({block_tables, kv_lens, query_start})) != TK_OK) return st;
   if (!aligned16(workspace)) return fail(TK_ERR_ARG, "the workspace must be on a 16-byte boundary");
   if (batch == 0 || batch > (1u << 24) || max_blocks == 0 || max_blocks > kMaxCount || tokens > kMaxCount ||
       (uint64_t)tokens * q_heads > (1u << 30))
