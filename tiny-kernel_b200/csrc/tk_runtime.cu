@@ -168,6 +168,23 @@ int set_device(tk_device* d) {
   return TK_OK;
 }
 
+// The device's for a while; then the calling thread's current one is as it was.
+struct DeviceScope {
+  int previous = -1;
+  int enter(tk_device* d) {
+    if (!d) return fail(TK_ERR_ARG, "device is NULL");
+    int now = -1;
+    TK_CUDA_TRY(cudaGetDevice(&now));
+    if (now == d->ordinal) return TK_OK;
+    TK_CUDA_TRY(cudaSetDevice(d->ordinal));
+    previous = now;
+    return TK_OK;
+  }
+  ~DeviceScope() {
+    if (previous >= 0) cudaSetDevice(previous);
+  }
+};
+
 cudaStream_t pick_stream(tk_device* d, void* stream) {
   return stream ? static_cast<cudaStream_t>(stream) : d->stream;
 }
@@ -1123,7 +1140,9 @@ int tk_device_synchronize(tk_device* d) {
 }
 
 int tk_device_check_error(tk_device* d) {
-  if (!d) return fail(TK_ERR_ARG, "device is NULL");
+  DeviceScope scope;
+  int st = scope.enter(d);
+  if (st != TK_OK) return st;
   unsigned h = 0;
   TK_CUDA_TRY(cudaMemcpy(&h, d->err, sizeof(h), cudaMemcpyDeviceToHost));
   if (h == 0) return TK_OK;
@@ -1302,22 +1321,6 @@ int tk_paged_attention(tk_device* d, const float* q, const float* kc, const floa
 // leave the calling thread's current device as they found it.
 
 namespace {
-
-struct DeviceScope {
-  int previous = -1;
-  int enter(tk_device* d) {
-    if (!d) return fail(TK_ERR_ARG, "device is NULL");
-    int now = -1;
-    TK_CUDA_TRY(cudaGetDevice(&now));
-    if (now == d->ordinal) return TK_OK;
-    TK_CUDA_TRY(cudaSetDevice(d->ordinal));
-    previous = now;
-    return TK_OK;
-  }
-  ~DeviceScope() {
-    if (previous >= 0) cudaSetDevice(previous);
-  }
-};
 
 constexpr uint32_t kMaxCount = 0x7fffffffu;
 
