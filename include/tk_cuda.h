@@ -398,10 +398,10 @@ int tk_qk_norm_rope_async(tk_device *dev, const void *q, const void *k, const fl
 /* Writes the keys and values of `tokens` tokens into their slots, quantised per group of
  * group_size dimensions: offset = f16(min), scale = f16((max - min) / 15), code = the integer
  * nearest to (x - offset) / scale (ties to even), in 0..15; a group of one value has scale 0.
- * Finite values past the f16 range saturate; a group that holds an infinity or a NaN reads back as
- * NaN.  k and v: rows of kv_heads * head_dim of type dtype, strides as above.  A token whose slot
- * is outside the cache (-1) is not written.  The slots of a call must differ: of two tokens in one
- * slot, parts of either may remain. */
+ * Of finite values past the f16 range the offset and the scale saturate; a group that holds an
+ * infinity or a NaN reads back as NaN.  k and v: rows of kv_heads * head_dim of type dtype, strides
+ * as above.  A token whose slot is outside the cache (-1) is not written.  The slots of a call must
+ * differ: of two tokens in one slot, parts of either may remain. */
 int tk_kv4_append(tk_device *dev, const tk_kv4_cache *cache, const void *k, const void *v,
                   const int32_t *slots, uint32_t tokens, uint32_t k_stride, uint32_t v_stride,
                   int dtype);
@@ -409,7 +409,9 @@ int tk_kv4_append_async(tk_device *dev, const tk_kv4_cache *cache, const void *k
                         const int32_t *slots, uint32_t tokens, uint32_t k_stride,
                         uint32_t v_stride, int dtype, void *stream);
 /* Reads the keys and values of `tokens` slots back (code * scale + offset, rounded once to dtype);
- * the rows of slots outside the cache stay as they were. */
+ * the rows of slots outside the cache stay as they were.  In f16 a value past its range is an
+ * infinity, although what was appended may have been finite: of a group from -65504 to 65504 the
+ * scale is 8736 and the largest value 15 * 8736 - 65504 = 65536.  f32 and bf16 hold it. */
 int tk_kv4_gather(tk_device *dev, const tk_kv4_cache *cache, const int32_t *slots, void *k,
                   void *v, uint32_t tokens, uint32_t k_stride, uint32_t v_stride, int dtype);
 int tk_kv4_gather_async(tk_device *dev, const tk_kv4_cache *cache, const int32_t *slots, void *k,
