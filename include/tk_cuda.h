@@ -321,8 +321,11 @@ int tk_paged_attention_async(tk_device *dev, const float *q, const float *k_cach
  * have; the rows behind the last token carry position -1 and slot -1 and are left as they were.
  * A call of no tokens does nothing; its rows' pointers may be NULL.
  * No call keeps state, allocates or waits: calls on different streams or from different threads
- * are independent as long as they share no output and no workspace.  The _async forms take the
- * stream as all others do; cudaStreamLegacy ((void *)1) names the legacy default stream.
+ * are independent as long as they share no output and no workspace.  (A wait in the attention of
+ * prompts that gives up sets the device's error word, which all calls of the device share: the
+ * next synchronous call or tk_device_check_error reports TK_ERR_TIMEOUT and clears it.)  The
+ * _async forms take the stream as all others do; cudaStreamLegacy ((void *)1) names the legacy
+ * default stream.
  *
  * The cache:  codes u8 [block][kv_head][block_size][head_dim/2], even dimension in the low nibble,
  *             scales f16 [block][kv_head][block_size][head_dim/group_size][2], (scale, offset);
@@ -351,11 +354,11 @@ typedef struct tk_kv4_cache {
  *   query_start[b]  index of the request's first token among the step's; query_start[batch]: all
  *   positions[t], slots[t]  of the step's token t; -1, -1 from the last token to max_tokens
  *   counts[4]       tokens of the step; pages it needs; tokens without a slot; free_range[0] plus
- *                   the pages taken
+ *                   the pages that the list had of them
  * A page that the list does not have, or whose id is outside [0, num_blocks), enters the table as
  * -1 and its tokens get slot -1, as do tokens past max_blocks pages; counts[2] counts them.
  * Tokens past max_tokens are cut off from the last requests (kv_lens and query_start go by what
- * remains).  The inputs are not changed: the caller moves free_range on by counts[1].  The outputs
+ * remains).  The inputs are not changed: counts[3] is the next step's free_range[0].  The outputs
  * must not be the inputs.  int32 throughout. */
 int tk_paged_slots(tk_device *dev, const int32_t *context_lens, const int32_t *query_lens,
                    const int32_t *free_blocks, const int32_t *free_range, int32_t *block_tables,
@@ -426,11 +429,16 @@ int tk_kv4_gather_async(tk_device *dev, const tk_kv4_cache *cache, const int32_t
  * q_heads * head_dim of type dtype, strides in elements (0: packed); o may be q.  The sequences'
  * ranges must not overlap; rows of no sequence are left as they were, and what the cache holds at
  * positions that a query does not see does not matter.  A query that sees nothing gives zeros.
- * kv_lens past max_blocks * block_size (below 2^31 - 1024) is cut there; a page whose id is outside
- * [0, num_blocks) counts as absent.  For every dtype the queries enter with 22 bits of their row's
- * largest magnitude, the weights with 22 bits, sums are f32 and do not depend on the run (fixed
- * order).  Scores have to fit f32; a query row that holds an infinity or a NaN gives NaN.
- * tokens * q_heads at most 2^30.
+ * Positions from max_blocks * block_size (below 2^31 - 1024) on count as absent, as do those of a
+ * page whose id is outside [0, num_blocks).  The queries enter with 22 bits of their row's largest
+ * magnitude (16-bit ones of prompts as they are), the weights with 22 bits; sums are f32, their order
+ * is fixed (the same bits from run to run), and their error does not grow with the length: f32
+ * outputs are about as far from 64 bits as the same formula in f32 operations.  Scores have to fit
+ * f32; a query row that holds an infinity or a NaN gives NaN.  tokens * q_heads at most 2^30.
+ * Speed: a call takes one kernel for all its sequences, for few or for many rows a sequence (query
+ * tokens * q_heads / kv_heads) on the mean, tokens / batch.  Single tokens beside a prompt, or in a
+ * step captured with rows for prompts, may take several times as long as in a call of their own
+ * with batch tokens and no query_start.
  * workspace: tk_kv4_attention_workspace bytes of device memory (20 to 40 MB) on a 16-byte boundary,
  * not initialised, for calls that do not run at the same time. */
 int tk_kv4_attention_workspace(tk_device *dev, const tk_kv4_cache *cache, uint32_t q_heads,
