@@ -27,7 +27,7 @@
 // What bounds it (B200, four heads a group, head dimension 128, group 128): 524288 positions take 128 us,
 // 4.5 TB/s of the 6.5 that a copy reaches.  Without its loads the same arithmetic runs at 6.4 TB/s of
 // codes, the loads without arithmetic at 5.3, and 12 warps on an SM overlap them only in part; 16 warps
-// of 128 registers spill (48 x 4096: 65 us instead of 58).  A short call is 9 us of waits one after the
+// of 128 registers spill (48 x 4096: 65 us, when 12 took 58; they take 59 now).  A short call is 9 us of waits one after the
 // other: lengths, block table, first pages, the end of the tile, the second kernel.
 //
 // Softmax in base 2 with a running reference per row: w = 2^(s - r) s_v must fit f16, so r follows
@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) kv4_attention_kernel(K
 }
 
 // Rows of a tile: four where a sequence has as many on the mean (its own query tokens are not known
-// here), eight otherwise: with four heads a group, 48 x 4096 58 us instead of 68, 524288 128 instead of
+// here), eight otherwise: with four heads a group, 48 x 4096 59 us instead of 68, 524288 128 instead of
 // 146; with eight, four-row tiles would read the cache twice.
 int attention_rows(const Kv4AttentionParams& p) {
   const long long per = p.q_heads / p.cache.kv_heads;

@@ -12,9 +12,9 @@ namespace tk {
 namespace {
 
 constexpr int kStep = 128;  // tokens of a step
-// Steps that a tile costs beside its own: queries, first loads, join (48 sequences of 64 to 8192: 65.3 us
-// with 1, 61.6 with 2, 60.6 with 3; 32 of 512: 15.2, 15.5, 17.5.  Prompts: 2 x 256 tokens over 1500 to
-// 4000 positions 113, 110, 116; 2048 tokens over themselves 140, 133, 133; 2 x 256 of them 34.5, 35.7, 39.4).
+// Steps that a tile costs beside its own: queries, first loads, join (48 sequences of 64 to 8192: 65.9 us
+// with 1, 62.7 with 2, 61.2 with 3; 32 of 512: 15.4, 15.7, 17.8.  Prompts: 2 x 256 tokens over 1500 to
+// 4000 positions 111, 109, 116; 2048 tokens over themselves 139, 132, 132; 512 of them 33.1, 34.1, 39.1).
 constexpr int kTileCost = 2;
 
 // Work is (sequence, key head, row tile, step of 128 tokens) in this order, cut into equal runs, one
@@ -109,7 +109,7 @@ struct Sequence {
   int steps;        // of a tile that sees all of it, its cost among them
 };
 // Tiles of many rows count the steps that their own rows see (32 + 8 heads of 128, 2048 tokens over
-// themselves: 133 us instead of 194, 8192: 1.44 ms instead of 2.55), smaller ones all of the sequence's.
+// themselves: 132 us instead of 194, 8192: 1.43 ms instead of 2.55), smaller ones all of the sequence's.
 constexpr int kManyRows = 128;
 __device__ __forceinline__ PromptTiles prompt_of(const Sequence& s, int per) {
   return prompt_tiles(s.tiles, per, kTileCost, s.last, s.kv);

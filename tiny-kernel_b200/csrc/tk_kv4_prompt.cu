@@ -29,8 +29,8 @@
 // to 1.2e-6.
 //
 // What bounds it (B200; those 2 x 256 tokens, 40 + 8 heads of 128, bf16): 109 us, 298 TFLOP/s with one
-// product each (the second part of the weights is a third one); tiles of eight rows on mma.sync take 299.
-// f32: 157 and 299.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
+// product each (the second part of the weights is a third one); tiles of eight rows on mma.sync take 301.
+// f32: 157 and 301.  Instruction issue and its latencies: 1400 instructions a warp and step at 0.47 a
 // cycle and scheduler, four warps a scheduler (128 registers, most of them scores), tensor pipe 24 %
 // busy.  When a call took 118 us, numbers of tokens for eight instead of four columns at a time made it
 // 125 (spilled); when it took 112, one f16 part of a weight instead of two 102, with 11 bits.
@@ -923,17 +923,18 @@ cudaError_t launch(const Kv4AttentionParams& p, int dtype, int sm_count, cudaStr
 }  // namespace
 
 // On the mean enough rows a sequence.  Against tiles of eight rows, four heads a group of 128, 16 x 2000
-// positions with 32 rows take 64 us instead of 53, with 48 65 instead of 73, with 128 70 instead of 168
-// (f32: 82 and 52, 83 and 73, 94 and 168; 256 dimensions, two groups: 141 and 99, 142 and 140); 60000
-// positions 110 and 75, 111 and 106, 114 and 255.  A step is long, so little work in all wants more rows:
-// one sequence of 3000, by the table's reach, with 128 rows 32 us instead of 28, with 256 33 instead of 40
-// (f32: 41 and 28, 43 and 43; 256 dimensions: 34 and 44 with 128, 33 and 29 with 64).
+// positions with 32 rows take 63 us instead of 52, with 48 64 instead of 73, with 128 69 instead of 168
+// (f32: 86 and 52, 64 rows 90 and 91, 98 and 168; 256 dimensions in two groups: 142 and 105, 143 and 148;
+// of f32 with 64 rows 196 and 194); 60000 positions 108 and 76, 108 and 106, 112 and 257.  A step is long, so little
+// work in all wants more rows: one sequence of 3000, by the table's reach, with 128 rows 33 us instead of 27, with
+// 256 33 instead of 40 (f32: 41 and 27, 43 and 40; 256 dimensions: 35 and 45 with 128, 34 and 29 with 64; f32 of them
+// 45 and 45 with 128).
 bool kv4_prompt_takes(const Kv4AttentionParams& p, int dtype) {
   const bool wide = dtype == kTypeF32, large = p.cache.head_dim == 256;
   const long long rows = (long long)p.tokens * (p.q_heads / p.cache.kv_heads);
   const long long tiles = (rows / kRows + p.batch) * p.cache.kv_heads;
   const long long steps = (((long long)p.max_blocks << p.cache.shift) + kStep - 1) / kStep + kTileCost;
-  const long long few = (wide ? 256 : 160) / (large ? 2 : 1), many = wide ? 64 : 48;
+  const long long few = (wide ? 288 : 160) / (large ? 2 : 1), many = wide ? 64 : 48;
   return rows >= few * p.batch || (rows >= many * p.batch && tiles * steps >= 600);
 }
 
