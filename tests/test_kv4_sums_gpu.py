@@ -16,9 +16,9 @@ pytestmark = pytest.mark.gpu
 PAGE = 16
 
 
-def repeated_page(torch, dev, seed, alike, positions, queries, per, hk, dim, group, scale, tiles):
+def repeated_page(torch, dev, seed, alike, positions, queries, per, hk, dim, group, scale, tiles, absent=0):
     """(outputs, what they should be, the size of the sums, the size of the scores) of sequences of `positions`
-    tokens; alike: the tokens' keys and values are all the same."""
+    tokens; alike: the tokens' keys and values are all the same; absent: so many of the first positions have no page."""
     rng = np.random.default_rng(seed)
     shape = (1, hk, PAGE, dim)
     parts = []
@@ -36,6 +36,7 @@ def repeated_page(torch, dev, seed, alike, positions, queries, per, hk, dim, gro
     batch, hq, width = -(-tiles // hk), hk * per, positions // PAGE
     i32 = dict(dtype=torch.int32, device="cuda")
     tables, lens = torch.zeros((batch, width), **i32), torch.full((batch,), positions, **i32)
+    tables[:, :absent // PAGE] = -1
     start = torch.arange(0, batch * queries + 1, queries, **i32)
     q1 = rng.standard_normal((queries, hq, dim)).astype(np.float32)
     q = torch.from_numpy(q1).cuda().repeat(batch, 1, 1).contiguous()
@@ -52,13 +53,13 @@ def repeated_page(torch, dev, seed, alike, positions, queries, per, hk, dim, gro
     k_size = oracle4.values_f64(kc, ks, np.abs(f64(km)))[0]
     want, sums, most = (np.zeros(q1.shape) for _ in range(3))
     for i in range(queries):
-        count = (positions - queries + i + 1 - np.arange(PAGE) + PAGE - 1) // PAGE  # of each token of the page
+        count = (positions - absent - queries + i + 1 - np.arange(PAGE) + PAGE - 1) // PAGE  # of each token of the page
         for h in range(hq):
             score = scale * (k[h // per] @ f64(q1[i, h]))
             w = count * np.exp(score - score.max())
             w /= w.sum()
             want[i, h], sums[i, h] = w @ v[h // per], w @ centre[h // per]
-            most[i, h] = scale * (k_size[h // per] @ np.abs(f64(q1[i, h]))).max()
+            most[i, h] = abs(scale) * (k_size[h // per] @ np.abs(f64(q1[i, h]))).max()
     return o.double().cpu().numpy().reshape(batch, queries, hq, dim), want, sums, most
 
 
@@ -93,3 +94,15 @@ def test_long_contexts_of_few_rows(torch_cuda, tkdev, dim, group, queries, alike
     ctas = tkdev.sm_count() * (2 if dim == 256 else 3)
     got = repeated_page(torch_cuda, tkdev, dim + group, alike, 524288, queries, 4, 8, dim, group, scale, 2 * ctas)
     check(*got, 64 + 2 * 37 + 3 * 2)
+
+
+@pytest.mark.parametrize("rows", ["many", "few"])
+@pytest.mark.parametrize("scale,absent", [(3.0, 0), (-3.0, 0), (0.0, 8192), (0.01, 8192), (-3.0, 8192)])
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 64), (128, 128), (256, 128)])
+def test_scores_far_from_zero_and_nothing_to_see_at_first(torch_cuda, tkdev, dim, group, scale, absent, rows):
+    """Rows whose scores are all far below zero (or above), and rows that have seen nothing when the sums are set
+    aside for the first time.  All tokens are alike: whatever the scores, the outputs are the values."""
+    queries, per, ctas = (64, 1, 1 if dim == 256 else 2) if rows == "many" else (2, 4, 2 if dim == 256 else 3)
+    got, want, sums, _ = repeated_page(torch_cuda, tkdev, dim + group, True, 16384, queries, per, 8, dim, group, scale,
+                                       2 * ctas * tkdev.sm_count(), absent)
+    check(got, want, sums, np.zeros_like(sums), 64 + 2 * 37 + 3 * 2)

@@ -95,7 +95,10 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
 // kept = kept * g + x, or x where nothing is kept yet.  Returns what its rounding drops, so that a long row of
 // such sums is off by no more than a short one (compensated summation).
 __device__ __forceinline__ float keep(bool any, float& kept, float g, float x) {
-  if (!any) kept = 0.f;
+  if (!any) {  // (g may be anything)
+    kept = x;
+    return 0.f;
+  }
   const float sum = fmaf(kept, g, x), drop = x + fmaf(kept, g, -sum);
   kept = sum;
   return drop;
