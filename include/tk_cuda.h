@@ -455,6 +455,56 @@ int tk_kv4_attention_async(tk_device *dev, const tk_kv4_cache *cache, const void
                            uint32_t q_heads, uint32_t max_blocks, uint32_t q_stride,
                            uint32_t o_stride, float scale, int dtype, void *stream);
 
+/* ---- projections in 8-bit floating point ----------------------------------------------------
+ * No counterpart in the reference (its matrices are f32 or 4 bits).  What stands between the serving
+ * step's calls and its sampler: the attention's output quantised (tk_fp8_quantize), projected
+ * (tk_fp8_matmul), added to the residual stream, normalised and quantised (tk_add_rmsnorm_fp8),
+ * projected again, at the end to logits (tk_sample_tokens).
+ *
+ * A matrix of rows [rows][dim]:
+ *   codes   u8 [rows][dim], e4m3 (4 bits of exponent, 3 of mantissa, up to 448; 0x7f and 0xff NaN)
+ *   scales  f32 [rows][ceil(dim/128)] of activations, [ceil(rows/128)][ceil(dim/128)] of weights
+ *   value = code * scale,  scale = max(largest magnitude of the group / 448, 2^-126), code the nearest
+ *   to value / scale (ties to even).  A group with an infinity or a NaN gets the scale NaN and codes 0.
+ * Strides of rows are in elements, 0: packed.  No call keeps state, allocates or waits, and all can be
+ * captured; calls on different streams or from different threads are independent as long as they share
+ * no output.  (A wait of the product that gives up sets the device's error word, as above.)  A call of no rows does nothing; its rows'
+ * pointers may be NULL. */
+
+/* s = x + residual (residual NULL: x), in f32;  sum_out = s rounded to dtype (NULL: not written; may be x
+ * or residual, same stride, else must not overlap them);  y = s * rsqrt(mean(s^2) + eps) * weight (weight
+ * NULL: ones);  codes and scales of y in groups of 128 of a row.  x, residual and sum_out of type dtype;
+ * the squares' sum has to fit f32.  dim at most 32768. */
+int tk_add_rmsnorm_fp8(tk_device *dev, const void *x, const void *residual, const float *weight,
+                       void *sum_out, uint8_t *codes, float *scales, uint32_t rows, uint32_t dim,
+                       uint32_t x_stride, uint32_t residual_stride, uint32_t sum_stride,
+                       uint32_t codes_stride, float eps, int dtype);
+int tk_add_rmsnorm_fp8_async(tk_device *dev, const void *x, const void *residual,
+                             const float *weight, void *sum_out, uint8_t *codes, float *scales,
+                             uint32_t rows, uint32_t dim, uint32_t x_stride,
+                             uint32_t residual_stride, uint32_t sum_stride, uint32_t codes_stride,
+                             float eps, int dtype, void *stream);
+
+/* Codes and scales of x (of type dtype) as it is: block_rows 1 for activations, 128 for weights. */
+int tk_fp8_quantize(tk_device *dev, const void *x, uint8_t *codes, float *scales, uint32_t rows,
+                    uint32_t dim, uint32_t block_rows, uint32_t x_stride, uint32_t codes_stride,
+                    int dtype);
+int tk_fp8_quantize_async(tk_device *dev, const void *x, uint8_t *codes, float *scales,
+                          uint32_t rows, uint32_t dim, uint32_t block_rows, uint32_t x_stride,
+                          uint32_t codes_stride, int dtype, void *stream);
+
+/* out[m][n] = sum_k a[m][k] * w[n][k] of the values that the codes stand for: a activations [m][k], w a
+ * weight [n][k] (out_dim, in_dim).  Sums over a block of 128 on the tensor cores, over the blocks in f32;
+ * rounded once to dtype.  The order of the sums is fixed (the same bits from run to run).  m, k, n of
+ * any size; the rows of a and w on 16-byte boundaries (pointers, and strides of multiples of 16). */
+int tk_fp8_matmul(tk_device *dev, const uint8_t *a, const float *a_scales, const uint8_t *w,
+                  const float *w_scales, void *out, uint32_t m, uint32_t k, uint32_t n,
+                  uint32_t a_stride, uint32_t w_stride, uint32_t out_stride, int dtype);
+int tk_fp8_matmul_async(tk_device *dev, const uint8_t *a, const float *a_scales, const uint8_t *w,
+                        const float *w_scales, void *out, uint32_t m, uint32_t k, uint32_t n,
+                        uint32_t a_stride, uint32_t w_stride, uint32_t out_stride, int dtype,
+                        void *stream);
+
 /* ---- sampler ----------------------------------------------------------------------------
  * Replaces the argmax shader (src/kernels/shaders.zig:889-943; the host loop of
  * src/model/llama.zig:290-303): out[0] = index of the largest of x[0..n).  Ties go to the smallest
@@ -470,6 +520,29 @@ int tk_softmax_sample(tk_device *dev, const float *logits, float *probs, uint32_
                       uint32_t vocab, float temperature, float random_val);
 int tk_softmax_sample_async(tk_device *dev, const float *logits, float *probs, uint32_t *sampled,
                             uint32_t vocab, float temperature, float random_val, void *stream);
+
+/* A token of each of `rows` rows of logits (of type dtype, rows of vocab values, stride in elements, 0:
+ * packed), each with its own temperature, filters and random number; one launch, no workspace, can be
+ * captured; calls that share no output are independent.  With w = exp((l - largest l) / temperature),
+ * tokens ranked by logit, equal ones by index, lowest first:
+ *   top_k   the first top_k are kept          (0 and below, or NULL: all)
+ *   top_p   of these the shortest prefix whose sum of w is at least top_p times their sum, one token at
+ *           the least                         (1 and above, NaN, or NULL: all)
+ *   min_p   of these those with w >= min_p    (0 and below, NaN, or NULL: all; above 1 counts as 1)
+ * tokens[row] = the first kept token, by index, at which the running sum of w exceeds random[row] times
+ * the sum of all kept; random in [0, 1) (below, or NaN, counts as 0; from 1 on the last one is taken).
+ * kept[row] (kept may be NULL) = how many are kept.  temperature NULL: 1; 0 and below, or NaN: the largest
+ * logit, filters aside, of equals the lowest index.  -inf and NaN logits are never kept; where there are
+ * +inf, they alone count; a row with nothing else than -inf and NaN gives token -1 and kept 0.  Weights
+ * below 2^-1022 count as 0.  Weights and sums are f64, in a fixed order.  vocab at most 393216. */
+int tk_sample_tokens(tk_device *dev, const void *logits, const float *temperature,
+                     const int32_t *top_k, const float *top_p, const float *min_p,
+                     const float *random, int32_t *tokens, int32_t *kept, uint32_t rows,
+                     uint32_t vocab, uint32_t stride, int dtype);
+int tk_sample_tokens_async(tk_device *dev, const void *logits, const float *temperature,
+                           const int32_t *top_k, const float *top_p, const float *min_p,
+                           const float *random, int32_t *tokens, int32_t *kept, uint32_t rows,
+                           uint32_t vocab, uint32_t stride, int dtype, void *stream);
 
 /* Test hook (bit-exactness of dequantisation, shaders.zig:474-495):
  * out f32 [k][n] = float(scale[g][n]) * (float(q[k][n]) - float(zero[g][n])). */

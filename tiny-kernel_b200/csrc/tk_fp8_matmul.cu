@@ -1,0 +1,353 @@
+// tk_fp8_matmul.cu -- rows of e4m3 codes times a weight of e4m3 codes, a scale for each block of 128 of k:
+//
+//   out[m][n] = sum over blocks b of  a_scales[m][b] w_scales[n / 128][b]  sum of a[m][k] w[n][k] in b
+//
+// The inner sums are products of 8-bit numbers on tcgen05, a block of k at a time into an accumulator of its own
+// in tensor memory; the outer sum, with the scales, is f32 in registers.
+#include <algorithm>
+#include <atomic>
+
+#include "tk_elements.cuh"
+#include "tk_fp8.h"
+#include "tk_internal.h"
+#include "tk_kv4.h"
+#include "tk_ptx.cuh"
+
+namespace tk {
+namespace {
+
+constexpr unsigned kErrFp8Wait = 128u;  // a copy or a product never completed
+
+// Waits for the phase of `bar`; gives up, for good, after timeout_ns.
+__device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t phase, bool& dead, const Fp8MatmulParams& p) {
+  if (dead || mbar_try_wait(bar, phase)) return;
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, phase))
+    if (global_timer_ns() - t0 > p.timeout_ns) {
+      atomicOr(p.err, kErrFp8Wait);
+      dead = true;
+      return;
+    }
+}
+
+// D[tmem] (+)= A[smem] x B[smem], e4m3, f32 sums, 32 of k.  The instruction's word is that of f16: type 0 is e4m3 here.
+__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
+}
+
+#define TK_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+// 16 consecutive columns of the warp's 32 lanes; complete after tmem_ld_wait.
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : TK_R4(r, 0), TK_R4(r, 4), TK_R4(r, 8), TK_R4(r, 12)
+      : "r"(at));
+}
+#undef TK_R4
+
+// Two f32 at once.
+__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
+  unsigned long long y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float2 values_of(unsigned long long p) {
+  float2 y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(p));
+  return y;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+
+__device__ __forceinline__ void store_out(const Fp8MatmulParams& p, long long at, float v) {
+  if (p.dtype == kTypeF32)
+    static_cast<float*>(p.out)[at] = v;
+  else if (p.dtype == kTypeBF16)
+    static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+  else
+    static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------
+//
+// The weight's rows are the product's 128 rows, the activations its NT columns.  The CTAs of a cluster share a
+// tile's blocks of k and add their sums through shared memory, in the order of their ranks.
+
+constexpr int kFewThreads = 192;  // a warp of copies, one of products, four of sums
+constexpr int kMaxStages = 8;
+
+template <int NT>
+struct Few {
+  static constexpr int kStep = NT == 128 ? 1 : 2;  // blocks of k between two waits
+  static constexpr int kBlockBytes = (128 + NT) * kFp8Block, kStageBytes = kStep * kBlockBytes;
+  static constexpr uint32_t kColumns = 2 * kStep * NT;  // of tensor memory: two steps
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const __grid_constant__ CUtensorMap a_map,
+                                                              const __grid_constant__ CUtensorMap w_map,
+                                                              Fp8MatmulParams p, int split, int stages) {
+  using M = Few<NT>;
+  constexpr int KS = M::kStep;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], sums_full[2], sums_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(16) float factors[4][2][KS][NT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
+  const int tile = blockIdx.x / split, rank = blockIdx.x % split, token0 = blockIdx.y * NT;
+  const int blocks = (p.k + kFp8Block - 1) / kFp8Block;
+  const int b0 = (int)((long long)blocks * rank / split), b1 = (int)((long long)blocks * (rank + 1) / split);
+  const int steps = (b1 - b0 + KS - 1) / KS;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 4);
+    mbar_init(&drained, 1);
+    fence_mbar_init();
+  }
+  after_previous();
+  if (warp == 1) tmem_alloc(&tmem_slot, M::kColumns);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+  bool dead = false;
+  int issued = 0;
+  unsigned long long acc[NT / 2];
+  if (warp == 0) {
+    const uint64_t once = l2_evict_first(), often = l2_evict_last();
+    for (int s = 0; s < steps; ++s) {
+      const int stage = s % stages;
+      if (s >= stages) wait_phase(&empty[stage], (s / stages - 1) & 1, dead, p);
+      if (__any_sync(0xffffffffu, dead)) {
+        dead = true;
+        break;
+      }
+      const int n = min(KS, b1 - b0 - s * KS);
+      if (elect_one()) {
+        uint8_t* to = smem + stage * M::kStageBytes;
+        mbar_arrive_expect_tx(&full[stage], n * M::kBlockBytes);
+        for (int i = 0; i < n; ++i) {
+          const int x = (b0 + s * KS + i) * kFp8Block;
+          tma_load_2d(to + i * 16384, &w_map, &full[stage], x, tile * 128, once);
+          tma_load_2d(to + KS * 16384 + i * NT * kFp8Block, &a_map, &full[stage], x, token0, often);
+        }
+      }
+      __syncwarp();
+      issued = s + 1;
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = umma_idesc_f16(128, NT);
+    for (int s = 0; s < steps; ++s) {
+      const int stage = s % stages, d = s & 1;
+      if (s >= 2) wait_phase(&sums_empty[d], (s / 2 - 1) & 1, dead, p);
+      wait_phase(&full[stage], (s / stages) & 1, dead, p);
+      if (__any_sync(0xffffffffu, dead)) {
+        dead = true;
+        break;
+      }
+      tcgen05_fence_after();
+      const int n = min(KS, b1 - b0 - s * KS);
+      if (elect_one()) {
+        const uint32_t at = smem_addr(smem) + stage * M::kStageBytes;
+        for (int i = 0; i < n; ++i) {
+          const uint64_t w = umma_smem_desc(at + i * 16384, 16, 1024, 2);
+          const uint64_t a = umma_smem_desc(at + KS * 16384 + i * NT * kFp8Block, 16, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_e4m3(tmem + (d * KS + i) * NT, w + 2 * k, a + 2 * k, idesc, k > 0);
+        }
+        umma_commit(&empty[stage]);
+        umma_commit(&sums_full[d]);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int quarter = warp & 3, at = warp - 2;
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+    for (int j = 0; j < NT / 2; ++j) acc[j] = 0;
+    constexpr int kEach = (NT + 31) / 32;
+    float next[KS][kEach];
+    auto fetch = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int b = b0 + s * KS + i;
+        const float w = b < b1 ? p.w_scales[(long long)tile * blocks + b] : 0.f;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const int j = e * 32 + lane, token = token0 + j;
+          next[i][e] = b < b1 && j < NT && token < p.m ? p.a_scales[(long long)token * blocks + b] * w : 0.f;
+        }
+      }
+    };
+    fetch(0);
+    for (int s = 0; s < steps; ++s) {
+      const int d = s & 1;
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+          if (e * 32 + lane < NT) factors[at][d][i][e * 32 + lane] = next[i][e];
+      if (s + 1 < steps) fetch(s + 1);
+      __syncwarp();
+      wait_phase(&sums_full[d], (s / 2) & 1, dead, p);
+      if (__any_sync(0xffffffffu, dead)) {
+        dead = true;
+        break;
+      }
+      tcgen05_fence_after();
+      const int n = min(KS, b1 - b0 - s * KS);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        if (i >= n) break;
+#pragma unroll
+        for (int c = 0; c < NT; c += 16) {
+          uint32_t t[16];
+          tmem_ld16(from + (d * KS + i) * NT + c, t);
+          tmem_ld_wait();
+          const float4* f = reinterpret_cast<const float4*>(&factors[at][d][i][c]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 g = f[j];
+            unsigned long long* to = &acc[c / 2 + 2 * j];
+            to[0] = fma2(pair_of(__uint_as_float(t[4 * j]), __uint_as_float(t[4 * j + 1])), pair_of(g.x, g.y), to[0]);
+            to[1] = fma2(pair_of(__uint_as_float(t[4 * j + 2]), __uint_as_float(t[4 * j + 3])), pair_of(g.z, g.w), to[1]);
+          }
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sums_empty[d]);
+    }
+  }
+  // After a wait that gave up: what is in flight completes before its memory is given back.
+  if (__syncthreads_or(dead)) {
+    bool late = false;
+    if (warp == 0)
+      for (int s = max(0, issued - stages); s < issued; ++s) wait_phase(&full[s % stages], (s / stages) & 1, late, p);
+    if (warp == 1) {
+      if (elect_one()) umma_commit(&drained);
+      __syncwarp();
+      wait_phase(&drained, 0, late, p);
+    }
+    dead = true;
+    __syncthreads();
+  }
+  const int row = (warp & 3) * 32 + lane, out_row = tile * 128 + row;
+  if (split == 1) {
+    if (warp >= 2 && !dead && out_row < p.n) {
+#pragma unroll
+      for (int j = 0; j < NT / 2; ++j) {
+        const float2 v = values_of(acc[j]);
+        const int token = token0 + 2 * j;
+        if (token < p.m) store_out(p, token * p.out_stride + out_row, v.x);
+        if (token + 1 < p.m) store_out(p, (token + 1) * p.out_stride + out_row, v.y);
+      }
+    }
+  } else {
+    float* mine = reinterpret_cast<float*>(smem);  // [NT][128]
+    if (warp >= 2) {
+#pragma unroll
+      for (int j = 0; j < NT / 2; ++j) {
+        const float2 v = values_of(acc[j]);
+        mine[2 * j * 128 + row] = v.x;
+        mine[(2 * j + 1) * 128 + row] = v.y;
+      }
+    }
+    cluster_sync();
+    if (warp >= 2 && !dead && out_row < p.n) {
+      const int j1 = min(NT * (rank + 1) / split, p.m - token0);
+      for (int j = NT * rank / split; j < j1; ++j) {
+        float sum = 0.f;
+        for (int r = 0; r < split; ++r) sum += ld_peer(smem_addr(mine + j * 128 + row), r);
+        store_out(p, (token0 + j) * p.out_stride + out_row, sum);
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+  }
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem, M::kColumns);
+  }
+}
+
+template <int NT>
+cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
+                       const CUtensorMap& w_map, cudaStream_t st) {
+  using M = Few<NT>;
+  constexpr int kMaxDevices = 64;
+  static std::atomic<unsigned> asked[kMaxDevices];
+  const int stages = std::min(kMaxStages, (NT <= 32 ? 112 * 1024 : 222 * 1024) / M::kStageBytes);
+  const int smem = std::max(stages * M::kStageBytes, NT * 512) + 1024;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned gen = attr_generation(dev) + 1;
+  if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
+    e = cudaFuncSetAttribute(fp8_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
+  }
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)plan.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((p.n + 127) / 128 * plan.split), (unsigned)((p.m + NT - 1) / NT));
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = plan.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, fp8_few_kernel<NT>, a_map, w_map, p, plan.split, stages);
+}
+
+}  // namespace
+
+Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count) {
+  Fp8MatmulPlan plan;
+  plan.tile = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  const long long tiles = (long long)((n + 127) / 128) * ((m + plan.tile - 1) / plan.tile);
+  const int blocks = (k + kFp8Block - 1) / kFp8Block;
+  plan.split = 1;
+  while (plan.split < 8 && tiles * plan.split * 2 <= sm_count * 2 && plan.split * 4 <= blocks) plan.split *= 2;
+  return plan;
+}
+
+void fp8_box_rows(const Fp8MatmulPlan& plan, int* a_rows, int* w_rows) {
+  *a_rows = plan.tile;
+  *w_rows = 128;
+}
+
+cudaError_t launch_fp8_matmul(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
+                              const CUtensorMap& w_map, int sm_count, cudaStream_t st) {
+  if (plan.tile == 16) return launch_few<16>(p, plan, a_map, w_map, st);
+  if (plan.tile == 32) return launch_few<32>(p, plan, a_map, w_map, st);
+  if (plan.tile == 64) return launch_few<64>(p, plan, a_map, w_map, st);
+  return launch_few<128>(p, plan, a_map, w_map, st);
+}
+
+}  // namespace tk

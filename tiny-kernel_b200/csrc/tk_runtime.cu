@@ -26,8 +26,10 @@
 #include "../../include/tk_cuda.h"
 #include "tk_decode.h"
 #include "tk_engine.h"
+#include "tk_fp8.h"
 #include "tk_internal.h"
 #include "tk_kv4.h"
+#include "tk_sample.h"
 
 using namespace tk;
 
@@ -1620,6 +1622,140 @@ int tk_kv4_attention(tk_device* d, const tk_kv4_cache* cache, const void* q, con
   return sync_and_check(d, d->stream);
 }
 
+namespace {
+
+// Rows of 8-bit codes for the product: boxes of 128 bytes of k, zeros past k and past the last row.
+int codes_tmap(const void* base, uint64_t k, uint64_t rows, uint64_t stride, int box_rows, CUtensorMap* out) {
+  int st = get_encoder();
+  if (st != TK_OK) return st;
+  cuuint64_t dims[2] = {k, rows};
+  cuuint64_t strides[1] = {stride};
+  cuuint32_t box[2] = {(cuuint32_t)kFp8Block, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = g_encode_tiled(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TK_ERR_CUDA, "cuTensorMapEncodeTiled (codes) failed (%d)", (int)r);
+  return TK_OK;
+}
+
+uint64_t fp8_blocks(uint64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+}  // namespace
+
+int tk_add_rmsnorm_fp8_async(tk_device* d, const void* x, const void* residual, const float* weight, void* sum_out,
+                             uint8_t* codes, float* scales, uint32_t rows, uint32_t dim, uint32_t x_stride,
+                             uint32_t residual_stride, uint32_t sum_stride, uint32_t codes_stride, float eps, int dtype,
+                             void* stream) {
+  int st = check_dtype(dtype);
+  if (st != TK_OK) return st;
+  if (rows && (!x || !codes || !scales)) return fail(TK_ERR_ARG, "NULL argument");
+  if (dim == 0 || dim > kFp8MaxDim) return fail(TK_ERR_ARG, "dim=%u is not in 1..%d", dim, kFp8MaxDim);
+  if (rows > kMaxCount || rows * fp8_blocks(dim) > kMaxCount)
+    return fail(TK_ERR_ARG, "%u rows of %u are too many for one call", rows, dim);
+  if (!std::isfinite(eps) || eps < 0.f) return fail(TK_ERR_ARG, "eps must be finite and not negative");
+  Fp8RowsParams p{x, residual, weight, sum_out, codes, scales, 0, 0, 0, 0, (int)rows, (int)dim, eps};
+  if ((st = check_stride("x", x_stride, dim, &p.x_stride)) != TK_OK) return st;
+  if ((st = check_stride("residual", residual_stride, dim, &p.residual_stride)) != TK_OK) return st;
+  if ((st = check_stride("sum", sum_stride, dim, &p.sum_stride)) != TK_OK) return st;
+  if ((st = check_stride("codes", codes_stride, dim, &p.codes_stride)) != TK_OK) return st;
+  if (!aligned_for(x, dtype) || !aligned_for(residual, dtype) || !aligned_for(sum_out, dtype))
+    return fail(TK_ERR_ARG, "x, residual or sum_out is not aligned to its type");
+  if ((st = check_words({weight, scales})) != TK_OK) return st;
+  if (rows && sum_out &&
+      ((sum_out == x && p.sum_stride != p.x_stride) || (sum_out == residual && p.sum_stride != p.residual_stride)))
+    return fail(TK_ERR_ARG, "in place needs the same stride in and out");
+  if (rows && (codes == x || codes == residual || codes == sum_out || (const void*)scales == x ||
+               (const void*)scales == residual || (const void*)scales == sum_out || (const void*)scales == codes ||
+               (const void*)codes == weight || scales == weight || (weight && sum_out == weight)))
+    return fail(TK_ERR_ARG, "an output is an input, or two outputs are the same");
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
+  if (rows == 0) return TK_OK;
+  TK_LAUNCH(d, launch_add_rmsnorm_fp8(p, dtype, d->sm_count, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_add_rmsnorm_fp8(tk_device* d, const void* x, const void* residual, const float* weight, void* sum_out,
+                       uint8_t* codes, float* scales, uint32_t rows, uint32_t dim, uint32_t x_stride,
+                       uint32_t residual_stride, uint32_t sum_stride, uint32_t codes_stride, float eps, int dtype) {
+  int st = tk_add_rmsnorm_fp8_async(d, x, residual, weight, sum_out, codes, scales, rows, dim, x_stride, residual_stride,
+                                    sum_stride, codes_stride, eps, dtype, nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
+int tk_fp8_quantize_async(tk_device* d, const void* x, uint8_t* codes, float* scales, uint32_t rows, uint32_t dim,
+                          uint32_t block_rows, uint32_t x_stride, uint32_t codes_stride, int dtype, void* stream) {
+  int st = check_dtype(dtype);
+  if (st != TK_OK) return st;
+  if (rows && (!x || !codes || !scales)) return fail(TK_ERR_ARG, "NULL argument");
+  if (block_rows != 1 && block_rows != kFp8Block) return fail(TK_ERR_ARG, "block_rows=%u is not 1 or 128", block_rows);
+  if (dim == 0 || dim > kMaxCount - kFp8Block || rows > kMaxCount || rows * fp8_blocks(dim) > kMaxCount)
+    return fail(TK_ERR_ARG, "%u rows of %u are out of range", rows, dim);
+  Fp8RowsParams p{x, nullptr, nullptr, nullptr, codes, scales, 0, 0, 0, 0, (int)rows, (int)dim, 0.f};
+  if ((st = check_stride("x", x_stride, dim, &p.x_stride)) != TK_OK) return st;
+  if ((st = check_stride("codes", codes_stride, dim, &p.codes_stride)) != TK_OK) return st;
+  if (!aligned_for(x, dtype)) return fail(TK_ERR_ARG, "x is not aligned to its type");
+  if ((st = check_words({scales})) != TK_OK) return st;
+  if (rows && (codes == x || (const void*)scales == x || (const void*)scales == codes))
+    return fail(TK_ERR_ARG, "an output is an input, or two outputs are the same");
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
+  if (rows == 0) return TK_OK;
+  TK_LAUNCH(d, launch_fp8_quantize(p, (int)block_rows, dtype, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_fp8_quantize(tk_device* d, const void* x, uint8_t* codes, float* scales, uint32_t rows, uint32_t dim,
+                    uint32_t block_rows, uint32_t x_stride, uint32_t codes_stride, int dtype) {
+  int st = tk_fp8_quantize_async(d, x, codes, scales, rows, dim, block_rows, x_stride, codes_stride, dtype, nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
+int tk_fp8_matmul_async(tk_device* d, const uint8_t* a, const float* a_scales, const uint8_t* w, const float* w_scales,
+                        void* out, uint32_t m, uint32_t k, uint32_t n, uint32_t a_stride, uint32_t w_stride,
+                        uint32_t out_stride, int dtype, void* stream) {
+  int st = check_dtype(dtype);
+  if (st != TK_OK) return st;
+  if ((m && (!a || !a_scales || !out)) || !w || !w_scales) return fail(TK_ERR_ARG, "NULL argument");
+  if (k == 0 || n == 0 || m > kMaxCount - 256 || k > kMaxCount - 256 || n > kMaxCount - 256 ||
+      (uint64_t)m * fp8_blocks(n) > kMaxCount)
+    return fail(TK_ERR_ARG, "product of %u x %u x %u is out of range", m, k, n);
+  long long as = 0, ws = 0;
+  Fp8MatmulParams p{a_scales, w_scales, out, 0, (int)m, (int)k, (int)n, dtype};
+  if ((st = check_stride("a", a_stride, k, &as)) != TK_OK) return st;
+  if ((st = check_stride("w", w_stride, k, &ws)) != TK_OK) return st;
+  if ((st = check_stride("out", out_stride, n, &p.out_stride)) != TK_OK) return st;
+  if (!aligned16(a) || !aligned16(w) || as % 16 || ws % 16)
+    return fail(TK_ERR_ARG, "the rows of a and w must be on 16-byte boundaries (strides %lld, %lld)", as, ws);
+  if (!aligned_for(out, dtype)) return fail(TK_ERR_ARG, "out is not aligned to its type");
+  if ((st = check_words({a_scales, w_scales})) != TK_OK) return st;
+  if (m && (out == a || out == w || out == a_scales || out == w_scales)) return fail(TK_ERR_ARG, "an output is an input");
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
+  if (m == 0) return TK_OK;
+  p.err = d->err;
+  p.timeout_ns = d->timeout_ns;
+  const Fp8MatmulPlan plan = fp8_matmul_plan((int)m, (int)k, (int)n, d->sm_count);
+  int a_rows = 0, w_rows = 0;
+  fp8_box_rows(plan, &a_rows, &w_rows);
+  CUtensorMap a_map, w_map;
+  if ((st = codes_tmap(a, k, m, (uint64_t)as, a_rows, &a_map)) != TK_OK) return st;
+  if ((st = codes_tmap(w, k, n, (uint64_t)ws, w_rows, &w_map)) != TK_OK) return st;
+  TK_LAUNCH(d, launch_fp8_matmul(p, plan, a_map, w_map, d->sm_count, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_fp8_matmul(tk_device* d, const uint8_t* a, const float* a_scales, const uint8_t* w, const float* w_scales,
+                  void* out, uint32_t m, uint32_t k, uint32_t n, uint32_t a_stride, uint32_t w_stride,
+                  uint32_t out_stride, int dtype) {
+  int st = tk_fp8_matmul_async(d, a, a_scales, w, w_scales, out, m, k, n, a_stride, w_stride, out_stride, dtype, nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
 int tk_argmax_async(tk_device* d, const float* x, uint32_t n, uint32_t* out, void* stream) {
   if (!d || !x || !out) return fail(TK_ERR_ARG, "NULL argument");
   if (n == 0 || n > (1u << 30)) return fail(TK_ERR_ARG, "argmax length %u out of range", n);
@@ -1650,6 +1786,38 @@ int tk_softmax_sample_async(tk_device* d, const float* logits, float* probs, uin
 int tk_softmax_sample(tk_device* d, const float* logits, float* probs, uint32_t* sampled,
                       uint32_t vocab, float temperature, float random_val) {
   int st = tk_softmax_sample_async(d, logits, probs, sampled, vocab, temperature, random_val, nullptr);
+  if (st != TK_OK) return st;
+  return sync_and_check(d, d->stream);
+}
+
+int tk_sample_tokens_async(tk_device* d, const void* logits, const float* temperature, const int32_t* top_k,
+                           const float* top_p, const float* min_p, const float* random, int32_t* tokens, int32_t* kept,
+                           uint32_t rows, uint32_t vocab, uint32_t stride, int dtype, void* stream) {
+  int st = check_dtype(dtype);
+  if (st != TK_OK) return st;
+  if (rows && (!logits || !random || !tokens)) return fail(TK_ERR_ARG, "NULL argument");
+  if (vocab == 0 || vocab > kSampleMaxVocab || rows > (1u << 24))
+    return fail(TK_ERR_ARG, "%u rows of %u logits are out of range", rows, vocab);
+  SampleParams p{logits, temperature, top_k, top_p, min_p, random, tokens, kept, 0, (int)rows, (int)vocab};
+  if ((st = check_stride("logits", stride, vocab, &p.stride)) != TK_OK) return st;
+  if (!aligned_for(logits, dtype)) return fail(TK_ERR_ARG, "logits is not aligned to its type");
+  if ((st = check_words({temperature, top_k, top_p, min_p, random, tokens, kept})) != TK_OK) return st;
+  const void* in[] = {logits, temperature, top_k, top_p, min_p, random};
+  for (const void* i : in)
+    if (rows && i && (i == tokens || i == kept)) return fail(TK_ERR_ARG, "an output is an input");
+  if (rows && tokens == kept) return fail(TK_ERR_ARG, "two outputs are the same");
+  DeviceScope scope;
+  if ((st = scope.enter(d)) != TK_OK) return st;
+  if (rows == 0) return TK_OK;
+  TK_LAUNCH(d, launch_sample_tokens(p, dtype, d->sm_count, pick_stream(d, stream)));
+  return TK_OK;
+}
+
+int tk_sample_tokens(tk_device* d, const void* logits, const float* temperature, const int32_t* top_k,
+                     const float* top_p, const float* min_p, const float* random, int32_t* tokens, int32_t* kept,
+                     uint32_t rows, uint32_t vocab, uint32_t stride, int dtype) {
+  int st = tk_sample_tokens_async(d, logits, temperature, top_k, top_p, min_p, random, tokens, kept, rows, vocab, stride,
+                                  dtype, nullptr);
   if (st != TK_OK) return st;
   return sync_and_check(d, d->stream);
 }

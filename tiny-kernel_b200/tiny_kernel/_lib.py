@@ -109,10 +109,18 @@ SIGNATURES = {
                          + [f32, i32]),
     "tk_kv4_attention_async": (i32, [vp, C.POINTER(Kv4CacheC)] + [vp] * 6 + [C.c_size_t] + [u32] * 6
                                + [f32, i32, vp]),
+    "tk_add_rmsnorm_fp8": (i32, [vp] * 7 + [u32] * 6 + [f32, i32]),
+    "tk_add_rmsnorm_fp8_async": (i32, [vp] * 7 + [u32] * 6 + [f32, i32, vp]),
+    "tk_fp8_quantize": (i32, [vp] * 4 + [u32] * 5 + [i32]),
+    "tk_fp8_quantize_async": (i32, [vp] * 4 + [u32] * 5 + [i32, vp]),
+    "tk_fp8_matmul": (i32, [vp] * 6 + [u32] * 6 + [i32]),
+    "tk_fp8_matmul_async": (i32, [vp] * 6 + [u32] * 6 + [i32, vp]),
     "tk_argmax": (i32, [vp, vp, u32, vp]),
     "tk_argmax_async": (i32, [vp, vp, u32, vp, vp]),
     "tk_softmax_sample": (i32, [vp, vp, vp, vp, u32, f32, f32]),
     "tk_softmax_sample_async": (i32, [vp, vp, vp, vp, u32, f32, f32, vp]),
+    "tk_sample_tokens": (i32, [vp] * 9 + [u32] * 3 + [i32]),
+    "tk_sample_tokens_async": (i32, [vp] * 9 + [u32] * 3 + [i32, vp]),
     "tk_tp_unique_id": (i32, [vp]),
     "tk_tp_create": (i32, [vp, i32, i32, vp, C.POINTER(vp)]),
     "tk_tp_destroy": (None, [vp]),

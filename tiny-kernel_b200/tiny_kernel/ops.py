@@ -253,6 +253,33 @@ def kv4_attention(device, cache, q, block_tables, kv_lens, query_start, o, works
            _dtype(dtype)), stream, sync)
 
 
+def add_rmsnorm_fp8(device, x, residual, weight, sum_out, codes, scales, rows, dim, eps, dtype="f32",
+                    x_stride=0, residual_stride=0, sum_stride=0, codes_stride=0, stream=None, sync=True):
+    """x + residual (None: x alone), its RMS norm (a None weight: ones) as e4m3 codes and scales per
+    group of 128, and the sum itself (a None sum_out: not written)."""
+    _call("tk_add_rmsnorm_fp8",
+          (_dev(device), _ptr(x), _ptr(residual), _ptr(weight), _ptr(sum_out), _ptr(codes), _ptr(scales),
+           rows, dim, x_stride, residual_stride, sum_stride, codes_stride, eps, _dtype(dtype)),
+          stream, sync)
+
+
+def fp8_quantize(device, x, codes, scales, rows, dim, block_rows=1, dtype="f32", x_stride=0,
+                 codes_stride=0, stream=None, sync=True):
+    """e4m3 codes and scales of x: per group of 128 of a row (block_rows 1, activations) or per block of
+    128 x 128 (block_rows 128, weights)."""
+    _call("tk_fp8_quantize",
+          (_dev(device), _ptr(x), _ptr(codes), _ptr(scales), rows, dim, block_rows, x_stride, codes_stride,
+           _dtype(dtype)), stream, sync)
+
+
+def fp8_matmul(device, a, a_scales, w, w_scales, out, m, k, n, dtype="f32", a_stride=0, w_stride=0,
+               out_stride=0, stream=None, sync=True):
+    """out [m][n] = a w^T of e4m3 activations [m][k] and an e4m3 weight [n][k] with their scales."""
+    _call("tk_fp8_matmul",
+          (_dev(device), _ptr(a), _ptr(a_scales), _ptr(w), _ptr(w_scales), _ptr(out), m, k, n, a_stride,
+           w_stride, out_stride, _dtype(dtype)), stream, sync)
+
+
 def argmax(device, x, n, out):
     """out[0] = index of the largest of x[0..n) (ties: the smallest index)."""
     check(_lib.lib().tk_argmax(_dev(device), _ptr(x), int(n), _ptr(out)))
@@ -263,6 +290,15 @@ def softmax_sample(device, logits, probs, sampled, vocab, temperature, random_va
     probability exceeds random_val (shaders.zig:826-887)."""
     check(_lib.lib().tk_softmax_sample(_dev(device), _ptr(logits), _ptr(probs), _ptr(sampled),
                                        int(vocab), float(temperature), float(random_val)))
+
+
+def sample_tokens(device, logits, temperature, top_k, top_p, min_p, random, tokens, kept, rows, vocab,
+                  dtype="f32", stride=0, stream=None, sync=True):
+    """tokens[row] of each row of logits, by its temperature, top_k, top_p and min_p (each an array of
+    rows, or None) and its random number; kept[row] (or None) = tokens that the filters leave."""
+    _call("tk_sample_tokens",
+          (_dev(device), _ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+           _ptr(random), _ptr(tokens), _ptr(kept), rows, vocab, stride, _dtype(dtype)), stream, sync)
 
 
 def dequant_int4(device, w_packed, scales, zeros, out, k, n, group_size):
