@@ -1,0 +1,154 @@
+"""GPU parity of tk_sample_tokens against the f64 oracle: tokens and counts are equal.  A row where the oracle's own
+comparisons come within 1e-9 of going the other way (the kernel's sums are within 1e-11 or so) is not asked; that is
+one row in ten thousand at the most."""
+import numpy as np
+import pytest
+
+import fp8
+from test_kv4_gpu import kind
+from tiny_kernel import ops
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = float("nan"), float("inf")
+
+
+def run(torch, dev, logits, dtype="f32", temperature=None, top_k=None, top_p=None, min_p=None, random=None, gap=0, offset=0):
+    """(tokens, kept) of rows of logits; parameters: None, a number for all rows, or one a row."""
+    logits = np.asarray(logits, np.float32)
+    rows, vocab = logits.shape
+
+    def each(v, t):
+        return None if v is None else torch.tensor(np.broadcast_to(np.asarray(v), (rows,)).copy(), dtype=t, device="cuda")
+
+    held = torch.full((offset + rows * (vocab + gap),), 99.0, dtype=kind(torch, dtype), device="cuda")
+    x = held[offset:].view(rows, vocab + gap)
+    x[:, :vocab] = torch.from_numpy(logits).cuda()
+    f = torch.float32
+    args = [each(temperature, f), each(top_k, torch.int32), each(top_p, f), each(min_p, f), each(random, f)]
+    tokens, kept = (torch.full((rows + 1,), -7, dtype=torch.int32, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    ops.sample_tokens(dev, x, *args, tokens, kept, rows, vocab, dtype, stride=vocab + gap)
+    assert tokens[rows] == -7 and kept[rows] == -7
+    host = [None if a is None else a.cpu().numpy() for a in args]
+    seen = x[:, :vocab].double().cpu().numpy()  # as rounded to their type
+    near = 0
+    for r in range(rows):
+        token, count, slack = fp8.sample(seen[r], *(None if a is None else a[r] for a in host))
+        if 0 < slack < 1e-9:  # 0: sums of equal weights, which are exact
+            near += 1
+            continue
+        assert (tokens[r].item(), kept[r].item()) == (token, count), (r, slack, [None if a is None else a[r] for a in host])
+    assert near <= max(1, rows // 100)
+    return tokens[:rows].cpu().numpy(), kept[:rows].cpu().numpy()
+
+
+def logits_of(seed, rows, vocab, width=2.0):
+    rng = np.random.default_rng(seed)
+    l = rng.normal(size=(rows, vocab)) * width - 2
+    l[np.arange(rows)[:, None], rng.integers(0, vocab, (rows, min(20, vocab)))] += rng.uniform(2, 12, (rows, min(20, vocab)))
+    return l, rng
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 100, 511, 1000, 4099, 32000, 50257, 128256])
+@pytest.mark.parametrize("rows,gap,offset", [(1, 0, 0), (12, 0, 0), (5, 3, 1)])
+def test_all_filters(torch_cuda, tkdev, vocab, dtype, rows, gap, offset):
+    l, rng = logits_of(vocab, rows, vocab)
+    l[rng.random(l.shape) < 0.02] = -INF
+    l[:, 0] = 1.0
+    run(torch_cuda, tkdev, l, dtype, rng.uniform(0.3, 2, rows), rng.integers(-1, 300, rows), rng.uniform(0.3, 1.1, rows),
+        np.where(rng.random(rows) < 0.5, 0, rng.uniform(0, 0.2, rows)), rng.random(rows), gap, offset)
+
+
+FILTERS = [dict(), dict(temperature=0.7), dict(top_k=1), dict(top_k=50), dict(top_k=3000), dict(top_p=0.5), dict(top_p=0.95),
+           dict(top_p=0.9999), dict(min_p=0.05), dict(min_p=1e-6), dict(top_k=100, top_p=0.8), dict(top_p=0.9, min_p=0.01),
+           dict(top_k=700, top_p=0.99, min_p=0.001, temperature=1.5)]
+
+
+@pytest.mark.parametrize("filters", FILTERS, ids=lambda f: "-".join(f"{k}{v}" for k, v in f.items()) or "none")
+@pytest.mark.parametrize("width", [0.01, 1.0, 6.0])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_each_filter(torch_cuda, tkdev, filters, width, dtype):
+    """Flat rows, whose filters keep most of a vocabulary, and peaked ones; 16-bit rows have thousands of equal values."""
+    rng = np.random.default_rng(3)
+    l = rng.normal(size=(40, 20011)) * width
+    run(torch_cuda, tkdev, l, dtype, random=rng.random(40), **filters)
+
+
+@pytest.mark.parametrize("vocab", [5, 600, 40000])
+def test_equal_logits(torch_cuda, tkdev, vocab):
+    """Of equal ones the lowest indexes are kept; the token is the one at random times their number."""
+    u = np.array([0.0, 0.125, 0.5, 0.75, 0.99])
+    l = np.full((5, vocab), -3.25)
+    tokens, kept = run(torch_cuda, tkdev, l, "f16", top_k=4, random=u)
+    assert (kept == 4).all() and tokens.tolist() == [0, 0, 2, 3, 3]
+    half = vocab // 2
+    l[:, :half] = -4.0
+    tokens, kept = run(torch_cuda, tkdev, l, "bf16", temperature=0.01, top_k=2, random=u)
+    assert tokens.tolist() == [half, half, half + 1, half + 1, half + 1]
+
+
+def test_special_rows(torch_cuda, tkdev):
+    l = np.zeros((14, 300), np.float32)
+    l[0] = -INF
+    l[1] = NAN
+    l[2, :] = -INF
+    l[2, 77] = -1e38
+    l[3, 10] = l[3, 200] = INF
+    l[4, ::2] = NAN
+    l[5] = -INF
+    l[5, [3, 4]] = INF
+    l[6, 1::2] = -INF
+    l[7] = 3.4e38
+    l[7, 5] = -3.4e38
+    l[8] = -0.0
+    l[8, 9] = 0.0
+    l[9] = np.linspace(-3e38, 3e38, 300)
+    l[10] = -1e30
+    l[11] = 1e-40
+    l[12] = np.arange(300) * 1e-45
+    u = np.linspace(0, 0.99, 14)
+    for more in (dict(), dict(top_k=3), dict(top_p=0.4), dict(min_p=0.5), dict(top_k=20, top_p=0.5, min_p=1.0), dict(temperature=0.0)):
+        tokens, kept = run(torch_cuda, tkdev, l, random=u, **more)
+        assert tokens[0] == tokens[1] == -1 and kept[0] == kept[1] == 0 and tokens[2] == 77 and kept[2] == 1
+        assert tokens[3] in (10, 200) and kept[3] <= 2
+        assert tokens[8] >= 0 and (more or kept[8] == 300)
+
+
+def test_parameters_at_their_ends(torch_cuda, tkdev):
+    l, rng = logits_of(8, 9, 3001)
+    ends = {"temperature": [0.0, -1.0, NAN, 1e-30, 1e-3, 1e30, INF, 1e-45, 1.0], "top_k": [0, -5, 3000, 3001, 3002, 2**31 - 1, 1, 2, -2**31],
+            "top_p": [0.0, -1.0, NAN, 1.0, 2.0, INF, -INF, 1e-30, 0.99999994], "min_p": [0.0, -1.0, NAN, 1.0, 2.0, INF, -INF, 1e-30, 0.99999994]}
+    for name, values in ends.items():
+        run(torch_cuda, tkdev, l, random=rng.random(9), **{name: values})
+    run(torch_cuda, tkdev, l, random=[0.0, -0.5, NAN, 1.0, 2.0, INF, -INF, 1e-30, 0.99999994])
+    run(torch_cuda, tkdev, l, random=[0.0, -0.5, NAN, 1.0, 2.0, INF, -INF, 1e-30, 0.99999994], top_k=20, top_p=0.9)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(1, 393216), (3, 262145), (160, 32000), (300, 257), (70, 100000)])
+def test_sizes(torch_cuda, tkdev, rows, vocab, dtype):
+    """The largest vocabulary, and as many rows as take one, two or more CTAs each."""
+    l, rng = logits_of(rows, rows, vocab)
+    run(torch_cuda, tkdev, l, dtype, top_k=rng.integers(0, 60, rows), top_p=0.9, random=rng.random(rows))
+    run(torch_cuda, tkdev, l, dtype, random=rng.random(rows))
+
+
+def test_random_numbers_give_the_distribution(torch_cuda, tkdev):
+    """Evenly spread numbers give each token as often as its probability says."""
+    n = 4096
+    p = np.array([0.5, 0.125, 0.25, 0.125])
+    l = np.broadcast_to(np.log(p), (n, 4))
+    tokens, _ = run(torch_cuda, tkdev, l, random=(np.arange(n) + 0.5) / n)
+    assert np.abs(np.bincount(tokens, minlength=4) / n - p).max() < 1e-3
+
+
+def test_rows_do_not_depend_on_others(torch_cuda, tkdev):
+    """A row alone and in a batch gives the same token: whatever the number of CTAs that share it."""
+    l, rng = logits_of(4, 100, 30000)
+    u, k = rng.random(100), rng.integers(0, 200, 100)
+    tokens, kept = run(torch_cuda, tkdev, l, top_k=k, top_p=0.95, random=u)
+    for r in (0, 50, 99):
+        one = run(torch_cuda, tkdev, l[r:r + 1], top_k=k[r:r + 1], top_p=0.95, random=u[r:r + 1])
+        assert one[0][0] == tokens[r] and one[1][0] == kept[r]

@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
       cut = cut_at(true, max(1ull, min(base, wanted + ((double)wanted < share))), true);
     }
   }
-  const double least = min_p > 0.f ? log2((double)fminf(min_p, 1.f)) : -INFINITY;
+  const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
 
   // Warps own runs of the row, so that the runs' sums stand in the order of the tokens.
   const int run = (slice + kWarps * 32 - 1) / (kWarps * 32) * 32;
@@ -306,9 +306,9 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     const uint32_t key = key_of(mine[i]);
     is = l > kNone && (!endless || l == most) && (key > cut.key || (key == cut.key && first + i <= last));
     if (!is) return 0.0;
-    const double t = exponent(l);
-    is = t >= least;
-    return is ? weight(t) : 0.0;
+    const double w = weight(exponent(l));
+    is = w >= least;
+    return is ? w : 0.0;
   };
   double sum = 0.0;
   int count = 0;
