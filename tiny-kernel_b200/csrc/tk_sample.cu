@@ -6,11 +6,17 @@
 //   of these w_i >= min_p.  The token is the first kept one, by index, at which the running sum of w passes
 //   random times the sum of all kept.
 //
-// The answer is a whole number that goes by where one sum passes another, so weights and sums are f64: tokens differ
-// from those of exact sums where the random number lies within about 1e-13 of a border, instead of within 1e-7,
+// The answer is a whole number that goes by where one sum passes another, so weights and sums are f64: a token differs
+// from that of exact sums where the random number lies within about 1e-13 of a border, instead of within 1e-7,
 // which in a row of 128256 tokens is one row in a hundred.  All sums have a fixed order, or are sums of integers.
 //
-// A row lies in the shared memory of a cluster's CTAs and is read from memory once.
+// A row lies in the shared memory of a cluster's CTAs and is read from memory once.  Then, by what the row asks for:
+//   top-k (few)       a level that at least top_k tokens reach, from the threads' largest; those tokens, some twice
+//                     top_k, are sorted by one CTA, which does the rest on its own
+//   top-p             sums of w by 64ths of an octave of w (integers, so that atomic additions give the same sums
+//                     in any order); the tokens of the part in which the sum passes its goal are sorted
+//   either, with more equal values than a list holds, or many top-k: the keys' digits one after the other
+// and, but for the first, a last pass with the sums of what is kept.
 #include <algorithm>
 #include <atomic>
 
@@ -22,10 +28,12 @@
 namespace tk {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
-constexpr int kBins = 2048;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8, kMaxWarps = kMaxCluster * kWarps;
+constexpr int kBins = 2048, kList = 1024, kFew = 400;
+constexpr int kParts = 64;           // of an octave of weights
 constexpr float kNone = -INFINITY;
 constexpr double kUnit = 17592186044416.0;  // 2^44: weights as integers, whose sums fit 64 bits
+constexpr double kWhole = 4503599627370496.0, kRound = 1.5 * kWhole;  // 2^52: added, a value's units are whole
 
 __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
@@ -39,21 +47,9 @@ __device__ __forceinline__ V* of_rank(V* mine, int rank) {
   return reinterpret_cast<V*>(at);
 }
 
-// Order of values as that of whole numbers.
+// Order of values as that of whole numbers; 16-bit types have keys of 16 bits.
 template <class T>
-struct Key;
-template <>
-struct Key<float> {
-  static constexpr int kBits = 32;
-};
-template <>
-struct Key<__half> {
-  static constexpr int kBits = 16;
-};
-template <>
-struct Key<__nv_bfloat16> {
-  static constexpr int kBits = 16;
-};
+constexpr int kKeyBits = sizeof(T) * 8;
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t b = __float_as_uint(v);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -68,17 +64,32 @@ __device__ __forceinline__ uint32_t key_of(__nv_bfloat16 v) {
 }
 
 struct Shared {
-  uint32_t count[kBins];
-  unsigned long long mass[kBins];
-  // read by the other CTAs
-  double warp_sum[kWarps];
-  int warp_count[kWarps];
-  float warp_max[kWarps];
-  // written by another CTA
-  int index;
+  union {
+    struct {
+      union {
+        struct {
+          uint32_t low[kBins], high[kBins];  // words of a bin's sum
+        };
+        unsigned long long sorted[2][kList];  // (key, ~index) of all CTAs' lists
+      };
+      unsigned long long list[kList];  // found here
+    };
+    struct {
+      uint32_t count[kBins];
+      unsigned long long mass[kBins];
+    } digits;
+  };
+  double table[kParts];  // 2^(i / 64)
+  // of all CTAs' warps, written by each into every CTA's
+  float all_most[kMaxWarps], all_level[kMaxWarps];
+  int all_valid[kMaxWarps], all_equal[kMaxWarps], all_count[kMaxWarps];
+  double all_sum[kMaxWarps];
+  int all_listed[kMaxCluster];
+  uint32_t cut_key;
+  int cut_index;
   // own
-  double all_sum[kMaxCluster * kWarps];
-  int all_count[kMaxCluster * kWarps];
+  int listed, first_equal;
+  float level;
   double scan[kWarps];
   unsigned long long scan_mass[kWarps];
   uint32_t scan_count[kWarps];
@@ -88,258 +99,602 @@ struct Shared {
   unsigned long long bin_mass;
 };
 
-// Where the kept ones end: all of a key above, and the first `ties` of that key.
-struct Cut {
-  uint32_t key;
-  unsigned long long ties, equal;  // kept of, and all with that key
-  unsigned long long mass;         // of the kept ones
-};
+// Sums of all threads before this one, and of all.
+__device__ __forceinline__ double scan_threads(double v, double* part, double* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double inc = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const double o = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += o;
+  }
+  __syncthreads();
+  if (lane == 31) part[warp] = inc;
+  __syncthreads();
+  double before = 0.0, all = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) before = all;
+    all += part[w];
+  }
+  *total = all;
+  return before + inc - v;
+}
+
+// Bitonic: V values a thread (of place tid + i * kThreads), n of them, a power of two up to V * kThreads; largest first
+// or smallest first.  buf: twice n.
+template <bool LARGEST_FIRST, int V, class U>
+__device__ __forceinline__ void sort_threads(U (&v)[V], int n, U* buf) {
+  const int tid = threadIdx.x;
+  int turn = 0;
+  for (int k = 2; k <= n; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (V > 1 && j == kThreads) {
+        if constexpr (V == 2) {
+          const bool swap = LARGEST_FIRST ? v[0] < v[1] : v[0] > v[1];  // k == 2 * kThreads: one direction
+          if (swap) {
+            const U t = v[0];
+            v[0] = v[1], v[1] = t;
+          }
+        }
+        continue;
+      }
+      U* at = buf + (turn & 1) * n;
+      if (j >= 32) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (tid + i * kThreads < n) at[tid + i * kThreads] = v[i];
+        __syncthreads();
+        ++turn;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int place = tid + i * kThreads;
+        U o;
+        if (j >= 32)
+          o = place < n ? at[place ^ j] : v[i];
+        else
+          o = __shfl_xor_sync(0xffffffffu, v[i], j);
+        const bool large = ((place & j) == 0) == ((place & k) == 0) ? LARGEST_FIRST : !LARGEST_FIRST;
+        if (large ? o > v[i] : o < v[i]) v[i] = o;
+      }
+    }
+}
 
 template <class T>
 __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p, int cluster, int slice) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   Shared& sh = *reinterpret_cast<Shared*>(dynamic);
   T* mine = reinterpret_cast<T*>(dynamic + (sizeof(Shared) + 15) / 16 * 16);
+  constexpr int kVec = 16 / sizeof(T);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = blockIdx.x % cluster;
+  const int rank = blockIdx.x % cluster, warps = cluster * kWarps;
   const long long row = blockIdx.x / cluster;
   const int first = rank * slice, n = max(0, min(slice, p.vocab - first));
+  if (tid < kParts) sh.table[tid] = exp2((double)tid / kParts);
+  if (tid == 0) sh.listed = 0, sh.first_equal = 0x7fffffff;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   after_previous();
   const T* src = static_cast<const T*>(p.logits) + row * p.stride + first;
+  const float heat = p.temperature ? p.temperature[row] : 1.f;
+  const bool greedy = !(heat > 0.f);
+  const int k = greedy || !p.top_k ? 0 : p.top_k[row];
+  const float top_p = greedy || !p.top_p ? 1.f : p.top_p[row];
+  const float min_p = greedy || !p.min_p ? 0.f : p.min_p[row];
+  const float u = p.random[row];
 
   // The row into shared memory: NaN as -inf, -0 as 0; its largest, and how many there are.
   float most = kNone;
   int valid = 0;
-  auto take = [&](int i, float v) {
-    v = v != v ? kNone : v + 0.f;
-    mine[i] = from_f32<T>(v);
+  auto take = [&](float v) {
     most = fmaxf(most, v);
     valid += v > kNone;
   };
-  constexpr int kVec = 16 / sizeof(T);
+  auto put = [&](int i, float v) {
+    v = v != v ? kNone : v + 0.f;
+    mine[i] = from_f32<T>(v);
+    take(v);
+  };
+  int begin = 0;
   if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+    constexpr int kFlight = 4;
     const int vecs = n / kVec;
-    for (int i = tid; i < vecs; i += kThreads) {
-      const uint4 raw = reinterpret_cast<const uint4*>(src)[i];
-      const T* e = reinterpret_cast<const T*>(&raw);
+    for (int i0 = 0; i0 < vecs; i0 += kFlight * kThreads) {
+      uint4 raw[kFlight];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) take(i * kVec + j, to_f32(e[j]));
+      for (int f = 0; f < kFlight; ++f) {
+        const int i = i0 + f * kThreads + tid;
+        if (i < vecs) raw[f] = reinterpret_cast<const uint4*>(src)[i];
+      }
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        const int i = i0 + f * kThreads + tid;
+        if (i >= vecs) break;
+        const T* e = reinterpret_cast<const T*>(&raw[f]);
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const float v = to_f32(e[j]);
+          odd |= v != v || __float_as_uint(v) == 0x80000000u;
+        }
+        if (odd) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) put(i * kVec + j, to_f32(e[j]));
+        } else {
+          reinterpret_cast<uint4*>(mine)[i] = raw[f];
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) take(to_f32(e[j]));
+        }
+      }
     }
-    for (int i = vecs * kVec + tid; i < n; i += kThreads) take(i, to_f32(src[i]));
-  } else {
-    for (int i = tid; i < n; i += kThreads) take(i, to_f32(src[i]));
+    begin = vecs * kVec;
+  }
+  for (int i = begin + tid; i < n; i += kThreads) put(i, to_f32(src[i]));
+  // what lies behind, up to a whole vector
+  const int padded = (n + kVec - 1) / kVec * kVec;
+  if (tid < padded - n) mine[n + tid] = from_f32<T>(kNone);
+
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all CTAs run: they may be written to
+  // For few top-k: each warp's each-th largest of its threads', which half of the warps reach at the least.
+  const bool few = k > 0 && k <= min(kFew, kWarps / 2 * 32 * cluster);
+  const int each = few ? (k + warps / 2 - 1) / (warps / 2) : 0;
+  if (few) {
+    float s = most;
+#pragma unroll
+    for (int kk = 2; kk <= 32; kk <<= 1)
+#pragma unroll
+      for (int j = kk >> 1; j > 0; j >>= 1) {
+        const float o = __shfl_xor_sync(0xffffffffu, s, j);
+        s = ((lane & j) == 0) == ((lane & kk) == 0) ? fmaxf(s, o) : fminf(s, o);
+      }
+    if (lane == each - 1)
+      for (int r = 0; r < cluster; ++r) *of_rank(&sh.all_level[rank * kWarps + warp], r) = s;
   }
 #pragma unroll
-  for (int off = 16; off; off >>= 1) {
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-    valid += __shfl_xor_sync(0xffffffffu, valid, off);
+  for (int off = 16; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+  valid = __reduce_add_sync(0xffffffffu, valid);
+  if (lane < cluster) {
+    *of_rank(&sh.all_most[rank * kWarps + warp], lane) = most;
+    *of_rank(&sh.all_valid[rank * kWarps + warp], lane) = valid;
   }
-  if (lane == 0) sh.warp_max[warp] = most, sh.warp_count[warp] = valid;
   cluster_sync();
   most = kNone;
   valid = 0;
-  for (int i = lane; i < cluster * kWarps; i += 32) {
-    most = fmaxf(most, of_rank(sh.warp_max, i / kWarps)[i % kWarps]);
-    valid += of_rank(sh.warp_count, i / kWarps)[i % kWarps];
+  for (int i = lane; i < warps; i += 32) {
+    most = fmaxf(most, sh.all_most[i]);
+    valid += sh.all_valid[i];
   }
 #pragma unroll
-  for (int off = 16; off; off >>= 1) {
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-    valid += __shfl_xor_sync(0xffffffffu, valid, off);
-  }
-  cluster_sync();  // warp_max and warp_count are free again
-
-  const float heat = p.temperature ? p.temperature[row] : 1.f;
-  const bool greedy = !(heat > 0.f);
-  const double slope = greedy ? 0.0 : 1.4426950408889634 / (double)heat;  // log2 e / T
-  const bool endless = most == INFINITY;
-  // log2 of a weight; what is not there is at -inf.  Where the largest is infinite only its equals are there.
-  auto exponent = [&](float l) -> double {
-    if (l == most) return 0.0;
-    if (endless || l == kNone) return -INFINITY;
-    return ((double)l - (double)most) * slope;
-  };
-  auto weight = [&](double t) -> double { return t < -1022.0 ? 0.0 : exp2(t); };
-  auto value = [&](int i) -> float { return to_f32(mine[i]); };
-
-  // By descending digits of the keys: the cut after `wanted` tokens, or after a sum of `wanted`.
-  auto cut_at = [&](bool by_mass, unsigned long long wanted, bool masses) -> Cut {
-    Cut cut{0, 0, 0, 0};
-    uint32_t known = 0;
-    unsigned long long above = 0, above_mass = 0, equal_mass = 0;
-    constexpr int kBits = Key<T>::kBits;
-    for (int high = kBits; high > 0;) {
-      const int digit = min(11, high), shift = high - digit;
-      for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0, sh.mass[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kThreads) {
-        const float l = value(i);
-        const uint32_t key = key_of(mine[i]);
-        if (l > kNone && (key & known) == cut.key) {
-          const uint32_t bin = key >> shift & ((1u << digit) - 1u);
-          atomicAdd(&sh.count[bin], 1u);
-          if (masses) atomicAdd(&sh.mass[bin], (unsigned long long)(weight(exponent(l)) * kUnit + 0.5));
-        }
-      }
-      cluster_sync();
-      // thread t sums four bins over the CTAs, from the top down
-      constexpr int kEach = kBins / kThreads;
-      uint32_t c[kEach], my_count = 0;
-      unsigned long long m[kEach], my_mass = 0;
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        const int bin = kBins - 1 - (tid * kEach + j);
-        c[j] = 0, m[j] = 0;
-        for (int r = 0; r < cluster; ++r) c[j] += of_rank(sh.count, r)[bin], m[j] += of_rank(sh.mass, r)[bin];
-        my_count += c[j], my_mass += m[j];
-      }
-      uint32_t inc = my_count;
-      unsigned long long inc_mass = my_mass;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const uint32_t o = __shfl_up_sync(0xffffffffu, inc, off);
-        const unsigned long long om = __shfl_up_sync(0xffffffffu, inc_mass, off);
-        if (lane >= off) inc += o, inc_mass += om;
-      }
-      if (lane == 31) sh.scan_count[warp] = inc, sh.scan_mass[warp] = inc_mass;
-      __syncthreads();
-      unsigned long long at = above + inc - my_count, at_mass = above_mass + inc_mass - my_mass;
-      for (int w = 0; w < warp; ++w) at += sh.scan_count[w], at_mass += sh.scan_mass[w];
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        const bool here = by_mass ? at_mass < wanted && wanted <= at_mass + m[j] : at < wanted && wanted <= at + c[j];
-        if (here) {
-          sh.bin = kBins - 1 - (tid * kEach + j);
-          sh.above_count = (uint32_t)at, sh.above_mass = at_mass;
-          sh.bin_count = c[j], sh.bin_mass = m[j];
-        }
-        at += c[j], at_mass += m[j];
-      }
-      cluster_sync();
-      above = sh.above_count, above_mass = sh.above_mass;
-      cut.equal = sh.bin_count, equal_mass = sh.bin_mass;
-      cut.key |= sh.bin << shift;
-      known |= ((1u << digit) - 1u) << shift;
-      high = shift;
-      __syncthreads();
-    }
-    const unsigned long long each = equal_mass / cut.equal;
-    if (!by_mass)
-      cut.ties = wanted - above;
-    else
-      cut.ties = each ? min(cut.equal, (wanted - above_mass + each - 1) / each) : cut.equal;
-    cut.mass = above_mass + cut.ties * each;
-    return cut;
-  };
-
+  for (int off = 16; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+  valid = __reduce_add_sync(0xffffffffu, valid);
   if (most == kNone) {
     if (rank == 0 && tid == 0) {
       p.tokens[row] = -1;
       if (p.kept) p.kept[row] = 0;
     }
-    cluster_sync();
     return;
   }
-  const int k = greedy || !p.top_k ? 0 : p.top_k[row];
-  const float top_p = greedy || !p.top_p ? 1.f : p.top_p[row];
-  const float min_p = greedy || !p.min_p ? 0.f : p.min_p[row];
-  Cut cut{0, 0, 0, 0};
-  const uint32_t top_key = key_of(from_f32<T>(most));
+  // Vectors of the CTA's slice, by threads; f(index in the slice, value).
+  auto for_all = [&](int from, int to, int start, int step, auto f) {
+    for (int i = from / kVec + start; i < (to + kVec - 1) / kVec; i += step) {
+      const uint4 raw = reinterpret_cast<const uint4*>(mine)[i];
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) f(i * kVec + j, e[j]);
+    }
+  };
+
   if (greedy) {
-    cut.key = top_key, cut.ties = 1, cut.equal = 2;
-  } else {
-    const bool by_k = k > 0 && k < valid, by_p = top_p < 1.f;
-    if (by_k) cut = cut_at(false, (unsigned long long)k, by_p);
+    for_all(0, n, tid, kThreads, [&](int i, T e) {
+      if (to_f32(e) == most) atomicMin(&sh.first_equal, i);
+    });
+    __syncthreads();
+    if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.first_equal;
+    cluster_sync();
+    if (rank == 0 && tid == 0) {
+      int r = 0;
+      while (sh.all_listed[r] == 0x7fffffff) ++r;
+      p.tokens[row] = r * slice + sh.all_listed[r];
+      if (p.kept) p.kept[row] = 1;
+    }
+    return;
+  }
+
+  const bool endless = most == INFINITY;
+  const double slope = kParts * 1.4426950408889634 / (double)heat;  // 64 log2 e / T
+  const double top = -(double)most * slope;
+  // 64 log2 of a weight; what is not there is at -inf.  Where the largest is infinite only its equals are there.
+  auto level_of = [&](float l) -> double {
+    const double y = fma((double)l, slope, top);
+    return l == most ? 0.0 : endless || l == kNone ? -INFINITY : y;
+  };
+  // 2^(y/64) = 2^a 2^(b/64) e^z with whole a and b and |z| <= ln 2 / 128: 1 + z + z^2/2 + z^3/6 + z^4/24 is within 4e-14.
+  auto weight = [&](double y) -> double {
+    if (!(y >= -1000.0 * kParts)) return 0.0;
+    const double shifted = y + kRound;
+    const int whole = __double2loint(shifted);
+    const double r = y - (shifted - kRound);
+    constexpr double c = 0.6931471805599453 / kParts;
+    double z = fma(r, c * c * c * c / 24, c * c * c / 6);
+    z = fma(r, z, c * c / 2);
+    z = fma(r, z, c);
+    const double t = sh.table[whole & (kParts - 1)];
+    const double w = fma(t, z * r, t);
+    return __hiloint2double(__double2hiint(w) + ((whole >> 6) << 20), __double2loint(w));
+  };
+  auto units = [&](double w) -> unsigned long long {  // to the nearest
+    return (unsigned long long)__double_as_longlong(fma(w, kUnit, kWhole)) & ((1ull << 52) - 1);
+  };
+  auto entry = [&](T e, int i) -> unsigned long long {
+    return (unsigned long long)key_of(e) << 32 | (0xffffffffu - (uint32_t)(first + i));
+  };
+  auto value_of = [&](uint32_t key) -> float {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    } else {
+      const unsigned short b = (unsigned short)(key & 0x8000u ? key & 0x7fffu : ~key);
+      T v;
+      memcpy(&v, &b, 2);
+      return to_f32(v);
+    }
+  };
+  // Those of all CTAs' lists, one after the other, of place tid + i * kThreads; 0 behind the last.
+  auto gather_lists = [&](unsigned long long (&v)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int at = tid + i * kThreads, r = 0;
+      while (r < cluster && at >= sh.all_listed[r]) at -= sh.all_listed[r++];
+      v[i] = r < cluster ? of_rank(sh.list, r)[at] : 0;
+    }
+  };
+  auto list = [&](T e, int i) {
+    const int at = atomicAdd(&sh.listed, 1);
+    if (at < kList) sh.list[at] = entry(e, i);
+  };
+  const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
+  const double goal_share = u > 0.f ? (double)fminf(u, 1.f) : 0.0;
+  const bool by_k = k > 0 && k < valid, by_p = top_p < 1.f;
+
+  bool listed = false;  // the lists held what they had to
+  if (by_k && few) {
+    if (warp == 0) {
+      // the least of the groups' medians: half of each group's warps reach it
+      float low = INFINITY;
+      for (int g = 0; g < warps; g += 32) {
+        float s = g + lane < warps ? sh.all_level[g + lane] : kNone;
+#pragma unroll
+        for (int kk = 2; kk <= 32; kk <<= 1)
+#pragma unroll
+          for (int j = kk >> 1; j > 0; j >>= 1) {
+            const float o = __shfl_xor_sync(0xffffffffu, s, j);
+            s = ((lane & j) == 0) == ((lane & kk) == 0) ? fmaxf(s, o) : fminf(s, o);
+          }
+        low = fminf(low, __shfl_sync(0xffffffffu, s, min(32, warps) / 2 - 1));
+      }
+      if (lane == 0) sh.level = low;
+    }
+    __syncthreads();
+    const float level = sh.level;
+    for_all(0, n, tid, kThreads, [&](int i, T e) {
+      const float l = to_f32(e);
+      if (l >= level && l > kNone) list(e, i);
+    });
+    __syncthreads();
+    if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
+    cluster_sync();
+    int count = 0;
+    bool fits = true;
+    for (int r = 0; r < cluster; ++r) count += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
+    listed = fits && count <= kList;
+    if (listed) {
+      unsigned long long v[2] = {0, 0};
+      if (rank == 0) gather_lists(v);
+      cluster_sync();  // no CTA reads another's after this
+      if (rank != 0) return;
+      int size = 32;
+      while (size < count) size <<= 1;
+      sort_threads<true, 2>(v, size, &sh.sorted[0][0]);
+      // thread t: the token of rank t
+      const bool ranked = tid < k;
+      const int index = (int)(0xffffffffu - (uint32_t)v[0]);
+      const double w = ranked ? weight(level_of(value_of((uint32_t)(v[0] >> 32)))) : 0.0;
+      double total;
+      const double before = scan_threads(w, sh.scan, &total);
+      bool is = ranked && w >= least && (!endless || w > 0.0);
+      if (by_p) is = is && (tid == 0 || before < (double)top_p * total);
+      const int kept = __syncthreads_count(is);  // a prefix
+      if (tid == 0 && p.kept) p.kept[row] = kept;
+      // by index; the ranks lead to the weights
+      double* weights = reinterpret_cast<double*>(&sh.sorted[0][0]);
+      uint32_t* buf = reinterpret_cast<uint32_t*>(&sh.sorted[1][0]);
+      weights[tid] = w;
+      size = 32;
+      while (size < kept) size <<= 1;
+      uint32_t by_index[1] = {is ? (uint32_t)index << 9 | (uint32_t)tid : 0xffffffffu};
+      __syncthreads();
+      sort_threads<false, 1>(by_index, size, buf);
+      const double x = tid < kept ? weights[by_index[0] & 511u] : 0.0;
+      const double at = scan_threads(x, sh.scan, &total);
+      const double goal = goal_share * total;
+      // the first whose end passes the goal, or the last with a weight
+      if (tid == 0) sh.first_equal = 0x7fffffff, sh.listed = 0;
+      __syncthreads();
+      if (x > 0.0) {
+        atomicMax(&sh.listed, tid);
+        if (at + x > goal) atomicMin(&sh.first_equal, tid);
+      }
+      __syncthreads();
+      if (tid == min(sh.first_equal, sh.listed)) p.tokens[row] = (int)(by_index[0] >> 9);
+      return;
+    }
+    __syncthreads();
+  }
+
+  // Where the kept ones end: a key, and the last index of it.
+  uint32_t cut_key = 0;
+  int cut_index = 0x7fffffff;
+  if (by_p && !by_k) {
+    for (int i = tid; i < kBins; i += kThreads) sh.low[i] = sh.high[i] = 0;
+    __syncthreads();
+    for_all(0, n, tid, kThreads, [&](int i, T e) {
+      const double y = level_of(to_f32(e));
+      const unsigned long long m = units(weight(y));
+      if (m) {
+        const int bin = min(kBins - 1, -__double2loint(y + kRound));
+        const uint32_t low = (uint32_t)m, old = atomicAdd(&sh.low[bin], low);
+        const uint32_t high = (uint32_t)(m >> 32) + (old + low < old);
+        if (high) atomicAdd(&sh.high[bin], high);
+      }
+    });
+    cluster_sync();
+    // each CTA sums some of the bins over all, in the place of its own, which no other reads before that
+    const int per = kBins / cluster;
+    for (int bin = rank * per + tid; bin < (rank + 1) * per; bin += kThreads) {
+      unsigned long long m = 0;
+      for (int r = 0; r < cluster; ++r)
+        m += of_rank(sh.low, r)[bin] + ((unsigned long long)of_rank(sh.high, r)[bin] << 32);
+      sh.low[bin] = (uint32_t)m, sh.high[bin] = (uint32_t)(m >> 32);
+    }
+    cluster_sync();
+    constexpr int kEach = kBins / kThreads;
+    unsigned long long m[kEach], mass = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int b = tid * kEach + j, r = b / per;
+      mass += m[j] = of_rank(sh.low, r)[b] + ((unsigned long long)of_rank(sh.high, r)[b] << 32);
+    }
+    unsigned long long inc = mass;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const unsigned long long o = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += o;
+    }
+    if (lane == 31) sh.scan_mass[warp] = inc;
+    __syncthreads();
+    unsigned long long at = inc - mass, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) at += sh.scan_mass[w];
+      all += sh.scan_mass[w];
+    }
+    const double share = (double)fmaxf(top_p, 0.f) * (double)all;
+    unsigned long long wanted = (unsigned long long)share;
+    wanted = max(1ull, min(all, wanted + ((double)wanted < share)));
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if (at < wanted && wanted <= at + m[j]) sh.bin = (uint32_t)(tid * kEach + j), sh.above_mass = at;
+      at += m[j];
+    }
+    __syncthreads();
+    const int bin = (int)sh.bin;
+    for_all(0, n, tid, kThreads, [&](int i, T e) {
+      const double y = level_of(to_f32(e));
+      if (y >= -1000.0 * kParts && min(kBins - 1, -__double2loint(y + kRound)) == bin) list(e, i);
+    });
+    __syncthreads();
+    if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
+    cluster_sync();
+    int count = 0;
+    bool fits = true;
+    for (int r = 0; r < cluster; ++r) count += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
+    listed = fits && count <= kList;
+    if (listed) {
+      if (rank == 0) {
+        unsigned long long v[2];
+        gather_lists(v);
+        int size = 32;
+        while (size < count) size <<= 1;
+        sort_threads<true, 2>(v, size, &sh.sorted[0][0]);
+        // thread t: ranks 2 t and 2 t + 1
+        unsigned long long* sorted = &sh.sorted[0][0];
+        __syncthreads();
+        sorted[tid] = v[0], sorted[tid + kThreads] = v[1];
+        if (tid == 0) sh.first_equal = count - 1;
+        __syncthreads();
+        unsigned long long own[2], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          v[i] = sorted[2 * tid + i];
+          own[i] = 2 * tid + i < count ? units(weight(level_of(value_of((uint32_t)(v[i] >> 32))))) : 0;
+          sum += own[i];
+        }
+        inc = sum;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const unsigned long long o = __shfl_up_sync(0xffffffffu, inc, off);
+          if (lane >= off) inc += o;
+        }
+        if (lane == 31) sh.scan_mass[warp] = inc;
+        __syncthreads();
+        unsigned long long passed = sh.above_mass + inc - sum;
+        for (int w = 0; w < warp; ++w) passed += sh.scan_mass[w];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          passed += own[i];
+          if (2 * tid + i < count && passed >= wanted) atomicMin(&sh.first_equal, 2 * tid + i);
+        }
+        __syncthreads();
+        if (tid < cluster) {
+          const unsigned long long last = sorted[sh.first_equal];
+          *of_rank(&sh.cut_key, tid) = (uint32_t)(last >> 32);
+          *of_rank(&sh.cut_index, tid) = (int)(0xffffffffu - (uint32_t)last);
+        }
+      }
+      cluster_sync();
+      cut_key = sh.cut_key, cut_index = sh.cut_index;
+    }
+  }
+
+  const int run = (slice + kWarps * 32 * kVec - 1) / (kWarps * 32 * kVec) * (32 * kVec);
+  const int r0 = min(padded, warp * run), r1 = min(padded, r0 + run);
+  if ((by_k || by_p) && !listed) {
+    // By descending digits of the keys: the cut after `wanted` tokens, or after a sum of `wanted`.
+    unsigned long long ties = 0, equal = 0, kept_mass = 0;
+    auto cut_at = [&](bool by_mass, unsigned long long wanted, bool masses) {
+      uint32_t known = 0;
+      unsigned long long above = 0, above_mass = 0, equal_mass = 0;
+      cut_key = 0;
+      for (int high = kKeyBits<T>; high > 0;) {
+        const int digit = min(11, high), shift = high - digit;
+        for (int i = tid; i < kBins; i += kThreads) sh.digits.count[i] = 0, sh.digits.mass[i] = 0;
+        __syncthreads();
+        for_all(0, n, tid, kThreads, [&](int, T e) {
+          const float l = to_f32(e);
+          const uint32_t key = key_of(e);
+          if (l > kNone && (key & known) == cut_key) {
+            const uint32_t bin = key >> shift & ((1u << digit) - 1u);
+            atomicAdd(&sh.digits.count[bin], 1u);
+            if (masses) atomicAdd(&sh.digits.mass[bin], units(weight(level_of(l))));
+          }
+        });
+        cluster_sync();
+        // thread t sums four bins over the CTAs, from the top down
+        constexpr int kEach = kBins / kThreads;
+        uint32_t c[kEach], my_count = 0;
+        unsigned long long m[kEach], my_mass = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          const int bin = kBins - 1 - (tid * kEach + j);
+          c[j] = 0, m[j] = 0;
+          for (int r = 0; r < cluster; ++r) c[j] += of_rank(sh.digits.count, r)[bin], m[j] += of_rank(sh.digits.mass, r)[bin];
+          my_count += c[j], my_mass += m[j];
+        }
+        uint32_t inc = my_count;
+        unsigned long long inc_mass = my_mass;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const uint32_t o = __shfl_up_sync(0xffffffffu, inc, off);
+          const unsigned long long om = __shfl_up_sync(0xffffffffu, inc_mass, off);
+          if (lane >= off) inc += o, inc_mass += om;
+        }
+        if (lane == 31) sh.scan_count[warp] = inc, sh.scan_mass[warp] = inc_mass;
+        __syncthreads();
+        unsigned long long at = above + inc - my_count, at_mass = above_mass + inc_mass - my_mass;
+        for (int w = 0; w < warp; ++w) at += sh.scan_count[w], at_mass += sh.scan_mass[w];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          const bool here = by_mass ? at_mass < wanted && wanted <= at_mass + m[j] : at < wanted && wanted <= at + c[j];
+          if (here) {
+            sh.bin = kBins - 1 - (tid * kEach + j);
+            sh.above_count = (uint32_t)at, sh.above_mass = at_mass;
+            sh.bin_count = c[j], sh.bin_mass = m[j];
+          }
+          at += c[j], at_mass += m[j];
+        }
+        cluster_sync();
+        above = sh.above_count, above_mass = sh.above_mass;
+        equal = sh.bin_count, equal_mass = sh.bin_mass;
+        cut_key |= sh.bin << shift;
+        known |= ((1u << digit) - 1u) << shift;
+        high = shift;
+        __syncthreads();
+      }
+      const unsigned long long one = equal_mass / equal;
+      if (!by_mass)
+        ties = wanted - above;
+      else
+        ties = one ? min(equal, (wanted - above_mass + one - 1) / one) : equal;
+      kept_mass = above_mass + ties * one;
+    };
+    cluster_sync();  // what lay there has been read
+    if (by_k) cut_at(false, (unsigned long long)k, by_p);
     if (by_p) {
-      unsigned long long base = cut.mass;
+      unsigned long long base = kept_mass;
       if (!by_k) {  // the sum of all
         unsigned long long sum = 0;
-        for (int i = tid; i < n; i += kThreads) sum += (unsigned long long)(weight(exponent(value(i))) * kUnit + 0.5);
+        for_all(0, n, tid, kThreads, [&](int, T e) { sum += units(weight(level_of(to_f32(e)))); });
 #pragma unroll
         for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (lane == 0) sh.mass[warp] = sum;
+        if (lane == 0) sh.digits.mass[warp] = sum;
         cluster_sync();
         base = 0;
-        for (int i = 0; i < cluster * kWarps; ++i) base += of_rank(sh.mass, i / kWarps)[i % kWarps];
+        for (int i = 0; i < warps; ++i) base += of_rank(sh.digits.mass, i / kWarps)[i % kWarps];
         cluster_sync();
       }
       const double share = (double)fmaxf(top_p, 0.f) * (double)base;
       const unsigned long long wanted = (unsigned long long)share;
-      cut = cut_at(true, max(1ull, min(base, wanted + ((double)wanted < share))), true);
+      cut_at(true, max(1ull, min(base, wanted + ((double)wanted < share))), true);
     }
-  }
-  const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
-
-  // Warps own runs of the row, so that the runs' sums stand in the order of the tokens.
-  const int run = (slice + kWarps * 32 - 1) / (kWarps * 32) * 32;
-  const int r0 = min(n, warp * run), r1 = min(n, r0 + run);
-  // The first kept ones of a key, by index.
-  int last = 0x7fffffff;
-  if (cut.ties < cut.equal) {
-    int equal = 0;
-    for (int i = r0 + lane; i < r1; i += 32) equal += key_of(mine[i]) == cut.key;
-#pragma unroll
-    for (int off = 16; off; off >>= 1) equal += __shfl_xor_sync(0xffffffffu, equal, off);
-    if (lane == 0) sh.warp_count[warp] = equal;
-    cluster_sync();
-    unsigned long long before = 0;
-    for (int i = 0; i < rank * kWarps + warp; ++i) before += of_rank(sh.warp_count, i / kWarps)[i % kWarps];
-    if (before < cut.ties && cut.ties <= before + equal) {
-      for (int i0 = r0; i0 < r1; i0 += 32) {
-        const bool is = i0 + lane < r1 && key_of(mine[i0 + lane]) == cut.key;
-        const uint32_t votes = __ballot_sync(0xffffffffu, is);
-        if (before + __popc(votes) >= cut.ties) {
-          const int nth = (int)(cut.ties - before);
-          if (is && __popc(votes & (0xffffffffu >> (31 - lane))) == nth)
-            for (int r = 0; r < cluster; ++r) *of_rank(&sh.index, r) = first + i0 + lane;
-          break;
+    if (ties < equal) {  // the first of that key, by index
+      int same = 0;
+      for (int i = r0 + lane; i < min(r1, n); i += 32) same += key_of(mine[i]) == cut_key;
+      same = __reduce_add_sync(0xffffffffu, same);
+      if (lane < cluster) *of_rank(&sh.all_equal[rank * kWarps + warp], lane) = same;
+      cluster_sync();
+      unsigned long long before = 0;
+      for (int i = 0; i < rank * kWarps + warp; ++i) before += sh.all_equal[i];
+      if (before < ties && ties <= before + same) {
+        for (int i0 = r0; i0 < min(r1, n); i0 += 32) {
+          const bool is = i0 + lane < min(r1, n) && key_of(mine[i0 + lane]) == cut_key;
+          const uint32_t votes = __ballot_sync(0xffffffffu, is);
+          if (before + __popc(votes) >= ties) {
+            if (is && __popc(votes & (0xffffffffu >> (31 - lane))) == (int)(ties - before))
+              for (int r = 0; r < cluster; ++r) *of_rank(&sh.cut_index, r) = first + i0 + lane;
+            break;
+          }
+          before += __popc(votes);
         }
-        before += __popc(votes);
       }
+      cluster_sync();
+      cut_index = sh.cut_index;
     }
-    cluster_sync();
-    last = sh.index;
   }
+
   // 0 where the token is not kept
-  auto kept_weight = [&](int i, bool& is) -> double {
-    const float l = value(i);
-    const uint32_t key = key_of(mine[i]);
-    is = l > kNone && (!endless || l == most) && (key > cut.key || (key == cut.key && first + i <= last));
+  auto kept_weight = [&](int i, T e, bool& is) -> double {
+    const float l = to_f32(e);
+    const uint32_t key = key_of(e);
+    is = l > kNone && (!endless || l == most) && (key > cut_key || (key == cut_key && first + i <= cut_index));
     if (!is) return 0.0;
-    const double w = weight(exponent(l));
+    const double w = weight(level_of(l));
     is = w >= least;
     return is ? w : 0.0;
   };
+  // Warps own runs of the row, so that the runs' sums stand in the order of the tokens.
   double sum = 0.0;
   int count = 0;
-  for (int i = r0 + lane; i < r1; i += 32) {
+  for_all(r0, r1, lane, 32, [&](int i, T e) {
     bool is;
-    sum += kept_weight(i, is);
+    sum += kept_weight(i, e, is);
     count += is;
-  }
+  });
 #pragma unroll
-  for (int off = 16; off; off >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    count += __shfl_xor_sync(0xffffffffu, count, off);
+  for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  count = __reduce_add_sync(0xffffffffu, count);
+  if (lane < cluster) {
+    *of_rank(&sh.all_sum[rank * kWarps + warp], lane) = sum;
+    *of_rank(&sh.all_count[rank * kWarps + warp], lane) = count;
   }
-  __syncthreads();
-  if (lane == 0) sh.warp_sum[warp] = sum, sh.warp_count[warp] = count;
-  cluster_sync();
-  for (int i = tid; i < cluster * kWarps; i += kThreads) {
-    sh.all_sum[i] = of_rank(sh.warp_sum, i / kWarps)[i % kWarps];
-    sh.all_count[i] = of_rank(sh.warp_count, i / kWarps)[i % kWarps];
-  }
-  cluster_sync();  // no CTA reads another's after this
+  cluster_sync();  // no CTA reads or writes another's after this
   double total = 0.0;
   int all = 0;
-  for (int i = 0; i < cluster * kWarps; ++i) total += sh.all_sum[i], all += sh.all_count[i];
+  for (int i = 0; i < warps; ++i) total += sh.all_sum[i], all += sh.all_count[i];
   if (rank == 0 && tid == 0 && p.kept) p.kept[row] = all;
-  const float u = p.random[row];
-  const double goal = (u > 0.f ? (double)fminf(u, 1.f) : 0.0) * total;
+  const double goal = goal_share * total;
   // the run in which the sum passes the goal; the last with a sum where rounding keeps it from that
   double before = 0.0, at = 0.0;
   int owner = -1;
-  for (int i = 0; i < cluster * kWarps; ++i) {
+  for (int i = 0; i < warps; ++i) {
     const double s = sh.all_sum[i];
     if (s > 0.0) {
       owner = i, before = at;
@@ -349,33 +704,24 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
   }
   if (owner / kWarps != rank) return;
   // All threads on that run, consecutive tokens each.
-  const int w0 = min(n, owner % kWarps * run), w1 = min(n, w0 + run), each = (run + kThreads - 1) / kThreads;
-  const int i0 = min(w1, w0 + tid * each), i1 = min(w1, i0 + each);
-  double part = 0.0;
+  const int w0 = min(n, owner % kWarps * run), w1 = min(n, w0 + run), share = (run + kThreads - 1) / kThreads;
+  const int i0 = min(w1, w0 + tid * share), i1 = min(w1, i0 + share);
+  double part = 0.0, ignored;
   bool is;
-  for (int i = i0; i < i1; ++i) part += kept_weight(i, is);
-  double inc = part;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const double o = __shfl_up_sync(0xffffffffu, inc, off);
-    if (lane >= off) inc += o;
-  }
-  if (lane == 31) sh.scan[warp] = inc;
-  if (tid == 0) sh.index = -1, sh.bin = 0;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) before += sh.scan[w];
+  for (int i = i0; i < i1; ++i) part += kept_weight(i, mine[i], is);
+  if (tid == 0) sh.first_equal = 0x7fffffff, sh.listed = -1;
+  const double lo = before + scan_threads(part, sh.scan, &ignored);
   // the first thread whose end passes the goal, or the last with a sum
-  const double lo = before + inc - part;
-  const bool passes = part > 0.0 && before + inc > goal;
-  if (passes) atomicMax(&sh.bin, (uint32_t)(kThreads - tid));
-  if (part > 0.0) atomicMax(&sh.index, tid);
+  if (part > 0.0) {
+    atomicMax(&sh.listed, tid);
+    if (lo + part > goal) atomicMin(&sh.first_equal, tid);
+  }
   __syncthreads();
-  const int winner = sh.bin ? kThreads - (int)sh.bin : sh.index;
-  if (tid == winner) {
+  if (tid == min(sh.first_equal, sh.listed)) {
     double running = lo;
     int token = -1;
     for (int i = i0; i < i1; ++i) {
-      const double w = kept_weight(i, is);
+      const double w = kept_weight(i, mine[i], is);
       if (w > 0.0) {
         token = first + i;
         running += w;
@@ -392,7 +738,7 @@ cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) 
   static std::atomic<unsigned> asked[kMaxDevices];
   int cluster = 1;
   while (cluster < kMaxCluster && ((long long)p.rows * cluster * 2 <= sm_count ||
-                                   kHead + ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > kMaxBytes))
+                                   ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > 32 * 1024))
     cluster *= 2;
   const int slice = ((p.vocab + cluster - 1) / cluster + 7) / 8 * 8, smem = kHead + slice * (int)sizeof(T);
   int dev = 0;
