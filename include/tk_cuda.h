@@ -534,7 +534,7 @@ int tk_softmax_sample_async(tk_device *dev, const float *logits, float *probs, u
  * kept[row] (kept may be NULL) = how many are kept.  temperature NULL: 1; 0 and below, or NaN: the largest
  * logit, filters aside, of equals the lowest index.  -inf and NaN logits are never kept; where there are
  * +inf, they alone count; a row with nothing else than -inf and NaN gives token -1 and kept 0.  Weights
- * below 2^-1000 count as 0.  Weights and sums are f64, in a fixed order.  vocab at most 393216. */
+ * below about 2^-1000 count as 0.  Weights and sums are f64, in a fixed order.  vocab at most 393216. */
 int tk_sample_tokens(tk_device *dev, const void *logits, const float *temperature,
                      const int32_t *top_k, const float *top_p, const float *min_p,
                      const float *random, int32_t *tokens, int32_t *kept, uint32_t rows,

@@ -68,7 +68,7 @@ def sample(logits, temperature, top_k, top_p, min_p, random):
         order = order[:top_k]
     top = l[order[0]]
     t = np.where(l[order] == top, 0.0, (l[order] - top) / heat) if np.isfinite(top) else np.zeros(len(order))
-    w = np.where(t * np.log2(np.e) < -1000, 0.0, np.exp(t))
+    w = np.where(t * np.log2(np.e) < -999.8, 0.0, np.exp(t))
     count, slack = len(order), 1.0
     if top_p is not None and top_p < 1:
         goal, passed = max(float(top_p), 0.0) * w.sum(), np.cumsum(w)

@@ -190,11 +190,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     most = fmaxf(most, v);
     valid += v > kNone;
   };
-  auto put = [&](int i, float v) {
-    v = v != v ? kNone : v + 0.f;
-    mine[i] = from_f32<T>(v);
-    take(v);
-  };
+  auto clean = [](float v) { return fmaxf(v + 0.f, kNone); };
   int begin = 0;
   if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
     constexpr int kFlight = 4;
@@ -210,26 +206,23 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
       for (int f = 0; f < kFlight; ++f) {
         const int i = i0 + f * kThreads + tid;
         if (i >= vecs) break;
-        const T* e = reinterpret_cast<const T*>(&raw[f]);
-        bool odd = false;
+        T* e = reinterpret_cast<T*>(&raw[f]);
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
-          const float v = to_f32(e[j]);
-          odd |= v != v || __float_as_uint(v) == 0x80000000u;
+          const float v = clean(to_f32(e[j]));
+          take(v);
+          e[j] = from_f32<T>(v);
         }
-        if (odd) {
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) put(i * kVec + j, to_f32(e[j]));
-        } else {
-          reinterpret_cast<uint4*>(mine)[i] = raw[f];
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) take(to_f32(e[j]));
-        }
+        reinterpret_cast<uint4*>(mine)[i] = raw[f];
       }
     }
     begin = vecs * kVec;
   }
-  for (int i = begin + tid; i < n; i += kThreads) put(i, to_f32(src[i]));
+  for (int i = begin + tid; i < n; i += kThreads) {
+    const float v = clean(to_f32(src[i]));
+    take(v);
+    mine[i] = from_f32<T>(v);
+  }
   // what lies behind, up to a whole vector
   const int padded = (n + kVec - 1) / kVec * kVec;
   if (tid < padded - n) mine[n + tid] = from_f32<T>(kNone);
@@ -303,15 +296,16 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
 
   const bool endless = most == INFINITY;
   const double slope = kParts * 1.4426950408889634 / (double)heat;  // 64 log2 e / T
-  const double top = -(double)most * slope;
-  // 64 log2 of a weight; what is not there is at -inf.  Where the largest is infinite only its equals are there.
+  // 64 log2 of a weight; what is not there is at -inf or (of an infinite temperature) NaN.  Where the largest is
+  // infinite only its equals are there.
   auto level_of = [&](float l) -> double {
-    const double y = fma((double)l, slope, top);
-    return l == most ? 0.0 : endless || l == kNone ? -INFINITY : y;
+    if (endless) return l == most ? 0.0 : -INFINITY;
+    return ((double)l - (double)most) * slope;
   };
+  // Below it weights, of less than 2^-999.7, count as 0; rounded so that none of less than 2^-1000 is above it.
+  const float least_level = endless ? kNone : __fsub_ru(most, __fmul_rd(693.f, heat));
   // 2^(y/64) = 2^a 2^(b/64) e^z with whole a and b and |z| <= ln 2 / 128: 1 + z + z^2/2 + z^3/6 + z^4/24 is within 4e-14.
-  auto weight = [&](double y) -> double {
-    if (!(y >= -1000.0 * kParts)) return 0.0;
+  auto weight_at = [&](double y) -> double {
     const double shifted = y + kRound;
     const int whole = __double2loint(shifted);
     const double r = y - (shifted - kRound);
@@ -322,6 +316,11 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     const double t = sh.table[whole & (kParts - 1)];
     const double w = fma(t, z * r, t);
     return __hiloint2double(__double2hiint(w) + ((whole >> 6) << 20), __double2loint(w));
+  };
+  auto weight = [&](float l) -> double {
+    if (endless) return l == most ? 1.0 : 0.0;
+    const double w = weight_at(((double)l - (double)most) * slope);
+    return l >= least_level && l > kNone ? w : 0.0;
   };
   auto units = [&](double w) -> unsigned long long {  // to the nearest
     return (unsigned long long)__double_as_longlong(fma(w, kUnit, kWhole)) & ((1ull << 52) - 1);
@@ -398,7 +397,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
       // thread t: the token of rank t
       const bool ranked = tid < k;
       const int index = (int)(0xffffffffu - (uint32_t)v[0]);
-      const double w = ranked ? weight(level_of(value_of((uint32_t)(v[0] >> 32)))) : 0.0;
+      const double w = ranked ? weight(value_of((uint32_t)(v[0] >> 32))) : 0.0;
       double total;
       const double before = scan_threads(w, sh.scan, &total);
       bool is = ranked && w >= least && (!endless || w > 0.0);
@@ -438,10 +437,10 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     for (int i = tid; i < kBins; i += kThreads) sh.low[i] = sh.high[i] = 0;
     __syncthreads();
     for_all(0, n, tid, kThreads, [&](int i, T e) {
-      const double y = level_of(to_f32(e));
-      const unsigned long long m = units(weight(y));
+      const float l = to_f32(e);
+      const unsigned long long m = units(weight(l));
       if (m) {
-        const int bin = min(kBins - 1, -__double2loint(y + kRound));
+        const int bin = min(kBins - 1, -__double2loint(level_of(l) + kRound));
         const uint32_t low = (uint32_t)m, old = atomicAdd(&sh.low[bin], low);
         const uint32_t high = (uint32_t)(m >> 32) + (old + low < old);
         if (high) atomicAdd(&sh.high[bin], high);
@@ -488,8 +487,8 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     __syncthreads();
     const int bin = (int)sh.bin;
     for_all(0, n, tid, kThreads, [&](int i, T e) {
-      const double y = level_of(to_f32(e));
-      if (y >= -1000.0 * kParts && min(kBins - 1, -__double2loint(y + kRound)) == bin) list(e, i);
+      const float l = to_f32(e);
+      if (l >= least_level && l > kNone && min(kBins - 1, -__double2loint(level_of(l) + kRound)) == bin) list(e, i);
     });
     __syncthreads();
     if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
@@ -515,7 +514,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           v[i] = sorted[2 * tid + i];
-          own[i] = 2 * tid + i < count ? units(weight(level_of(value_of((uint32_t)(v[i] >> 32))))) : 0;
+          own[i] = 2 * tid + i < count ? units(weight(value_of((uint32_t)(v[i] >> 32)))) : 0;
           sum += own[i];
         }
         inc = sum;
@@ -564,7 +563,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
           if (l > kNone && (key & known) == cut_key) {
             const uint32_t bin = key >> shift & ((1u << digit) - 1u);
             atomicAdd(&sh.digits.count[bin], 1u);
-            if (masses) atomicAdd(&sh.digits.mass[bin], units(weight(level_of(l))));
+            if (masses) atomicAdd(&sh.digits.mass[bin], units(weight(l)));
           }
         });
         cluster_sync();
@@ -622,7 +621,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
       unsigned long long base = kept_mass;
       if (!by_k) {  // the sum of all
         unsigned long long sum = 0;
-        for_all(0, n, tid, kThreads, [&](int, T e) { sum += units(weight(level_of(to_f32(e)))); });
+        for_all(0, n, tid, kThreads, [&](int, T e) { sum += units(weight(to_f32(e))); });
 #pragma unroll
         for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         if (lane == 0) sh.digits.mass[warp] = sum;
@@ -660,24 +659,31 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     }
   }
 
+  float cut_value = kNone;
+  if (by_k || by_p) cut_value = value_of(cut_key);
+  if (endless && cut_value < most) cut_value = 3.4028235e38f, cut_index = -1;
+  if (cut_value == kNone) cut_index = -1;
   // 0 where the token is not kept
-  auto kept_weight = [&](int i, T e, bool& is) -> double {
-    const float l = to_f32(e);
-    const uint32_t key = key_of(e);
-    is = l > kNone && (!endless || l == most) && (key > cut_key || (key == cut_key && first + i <= cut_index));
+  auto kept_weight = [&](int i, float l, bool& is) -> double {
+    is = l > cut_value || (l == cut_value && first + i <= cut_index);
     if (!is) return 0.0;
-    const double w = weight(level_of(l));
+    const double w = weight(l);
     is = w >= least;
     return is ? w : 0.0;
   };
   // Warps own runs of the row, so that the runs' sums stand in the order of the tokens.
   double sum = 0.0;
   int count = 0;
-  for_all(r0, r1, lane, 32, [&](int i, T e) {
-    bool is;
-    sum += kept_weight(i, e, is);
-    count += is;
-  });
+  const bool plain = !by_k && !by_p && least == 0.0 && !endless;  // all that are there
+  if (plain) {
+    for_all(r0, r1, lane, 32, [&](int, T e) { sum += weight(to_f32(e)); });
+  } else {
+    for_all(r0, r1, lane, 32, [&](int i, T e) {
+      bool is;
+      sum += kept_weight(i, to_f32(e), is);
+      count += is;
+    });
+  }
 #pragma unroll
   for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   count = __reduce_add_sync(0xffffffffu, count);
@@ -686,29 +692,47 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     *of_rank(&sh.all_count[rank * kWarps + warp], lane) = count;
   }
   cluster_sync();  // no CTA reads or writes another's after this
-  double total = 0.0;
+  // The run in which the sum passes the goal; the last with a sum where rounding keeps it from that.
+  constexpr int kEachRun = kMaxWarps / 32;
+  double sums[kEachRun], mine_sum = 0.0;
   int all = 0;
-  for (int i = 0; i < warps; ++i) total += sh.all_sum[i], all += sh.all_count[i];
-  if (rank == 0 && tid == 0 && p.kept) p.kept[row] = all;
-  const double goal = goal_share * total;
-  // the run in which the sum passes the goal; the last with a sum where rounding keeps it from that
-  double before = 0.0, at = 0.0;
-  int owner = -1;
-  for (int i = 0; i < warps; ++i) {
-    const double s = sh.all_sum[i];
-    if (s > 0.0) {
-      owner = i, before = at;
-      if (at + s > goal) break;
-    }
-    at += s;
+#pragma unroll
+  for (int j = 0; j < kEachRun; ++j) {
+    const int i = lane * kEachRun + j;
+    sums[j] = i < warps ? sh.all_sum[i] : 0.0;
+    mine_sum += sums[j];
+    all += i < warps ? sh.all_count[i] : 0;
   }
+  double upto = mine_sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const double o = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += o;
+  }
+  const double goal = goal_share * __shfl_sync(0xffffffffu, upto, 31);
+  int owner = -1, last_run = -1;
+  double before = upto - mine_sum, last_before = 0.0, owner_before = 0.0;
+#pragma unroll
+  for (int j = 0; j < kEachRun; ++j) {
+    if (sums[j] > 0.0) {
+      last_run = lane * kEachRun + j, last_before = before;
+      if (owner < 0 && before + sums[j] > goal) owner = last_run, owner_before = before;
+    }
+    before += sums[j];
+  }
+  const uint32_t passing = __ballot_sync(0xffffffffu, owner >= 0), any = __ballot_sync(0xffffffffu, last_run >= 0);
+  const int from = passing ? __ffs(passing) - 1 : 31 - __clz(any);
+  owner = __shfl_sync(0xffffffffu, passing ? owner : last_run, from);
+  before = __shfl_sync(0xffffffffu, passing ? owner_before : last_before, from);
+  all = __reduce_add_sync(0xffffffffu, all);
+  if (rank == 0 && tid == 0 && p.kept) p.kept[row] = plain ? valid : all;
   if (owner / kWarps != rank) return;
   // All threads on that run, consecutive tokens each.
   const int w0 = min(n, owner % kWarps * run), w1 = min(n, w0 + run), share = (run + kThreads - 1) / kThreads;
   const int i0 = min(w1, w0 + tid * share), i1 = min(w1, i0 + share);
   double part = 0.0, ignored;
   bool is;
-  for (int i = i0; i < i1; ++i) part += kept_weight(i, mine[i], is);
+  for (int i = i0; i < i1; ++i) part += kept_weight(i, to_f32(mine[i]), is);
   if (tid == 0) sh.first_equal = 0x7fffffff, sh.listed = -1;
   const double lo = before + scan_threads(part, sh.scan, &ignored);
   // the first thread whose end passes the goal, or the last with a sum
@@ -721,7 +745,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     double running = lo;
     int token = -1;
     for (int i = i0; i < i1; ++i) {
-      const double w = kept_weight(i, mine[i], is);
+      const double w = kept_weight(i, to_f32(mine[i]), is);
       if (w > 0.0) {
         token = first + i;
         running += w;
