@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8, kMaxWarps = kMaxCluster * kWarps;
 constexpr int kBins = 2048, kList = 1024, kFew = 400;
-constexpr int kParts = 64;           // of an octave of weights
+constexpr int kParts = 512, kPerBin = 8;  // of an octave of weights: in the table, and of these in a bin
 constexpr float kNone = -INFINITY;
 constexpr double kUnit = 17592186044416.0;  // 2^44: weights as integers, whose sums fit 64 bits
 constexpr double kWhole = 4503599627370496.0, kRound = 1.5 * kWhole;  // 2^52: added, a value's units are whole
@@ -63,7 +63,8 @@ __device__ __forceinline__ uint32_t key_of(__nv_bfloat16 v) {
   return (b & 0x8000u ? ~b : b | 0x8000u) & 0xffffu;
 }
 
-struct Shared {
+// What ranks need.
+struct Ranked {
   union {
     struct {
       union {
@@ -79,17 +80,19 @@ struct Shared {
       unsigned long long mass[kBins];
     } digits;
   };
-  double table[kParts];  // 2^(i / 64)
+};
+struct Shared {
+  double table[kParts];  // 2^(i / kParts)
   // of all CTAs' warps, written by each into every CTA's
+  double all_sum[kMaxWarps];
   float all_most[kMaxWarps], all_level[kMaxWarps];
   int all_valid[kMaxWarps], all_equal[kMaxWarps], all_count[kMaxWarps];
-  double all_sum[kMaxWarps];
   int all_listed[kMaxCluster];
   uint32_t cut_key;
   int cut_index;
   // own
   int listed, first_equal;
-  float level;
+  float level[kMaxWarps / 32];
   double scan[kWarps];
   unsigned long long scan_mass[kWarps];
   uint32_t scan_count[kWarps];
@@ -121,65 +124,86 @@ __device__ __forceinline__ double scan_threads(double v, double* part, double* t
   return before + inc - v;
 }
 
-// Bitonic: V values a thread (of place tid + i * kThreads), n of them, a power of two up to V * kThreads; largest first
-// or smallest first.  buf: twice n.
-template <bool LARGEST_FIRST, int V, class U>
-__device__ __forceinline__ void sort_threads(U (&v)[V], int n, U* buf) {
-  const int tid = threadIdx.x;
-  int turn = 0;
-  for (int k = 2; k <= n; k <<= 1)
+template <bool LARGEST_FIRST, class U>
+__device__ __forceinline__ bool precedes(U a, U b) {
+  return LARGEST_FIRST ? a > b : a < b;
+}
+// A value of each lane, in order.
+template <bool LARGEST_FIRST, class U>
+__device__ __forceinline__ U sort_warp(U v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
     for (int j = k >> 1; j > 0; j >>= 1) {
-      if (V > 1 && j == kThreads) {
-        if constexpr (V == 2) {
-          const bool swap = LARGEST_FIRST ? v[0] < v[1] : v[0] > v[1];  // k == 2 * kThreads: one direction
-          if (swap) {
-            const U t = v[0];
-            v[0] = v[1], v[1] = t;
-          }
-        }
-        continue;
-      }
-      U* at = buf + (turn & 1) * n;
-      if (j >= 32) {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (tid + i * kThreads < n) at[tid + i * kThreads] = v[i];
-        __syncthreads();
-        ++turn;
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int place = tid + i * kThreads;
-        U o;
-        if (j >= 32)
-          o = place < n ? at[place ^ j] : v[i];
-        else
-          o = __shfl_xor_sync(0xffffffffu, v[i], j);
-        const bool large = ((place & j) == 0) == ((place & k) == 0) ? LARGEST_FIRST : !LARGEST_FIRST;
-        if (large ? o > v[i] : o < v[i]) v[i] = o;
-      }
+      const U o = __shfl_xor_sync(0xffffffffu, v, j);
+      const bool early = ((lane & j) == 0) == ((lane & k) == 0);
+      if (precedes<LARGEST_FIRST>(o, v) == early) v = o;
     }
+  return v;
+}
+// V values a thread (of place tid + i * kThreads), n of them, a power of two from 32 on; they lie in order in
+// the returned half of buf (twice n).  Warps sort 32 each; of two sorted runs, a value's place in both is its place in
+// its own and how many of the other's precede it.
+template <bool LARGEST_FIRST, int V, class U>
+__device__ __forceinline__ U* sort_threads(U (&v)[V], int n, U* buf) {
+  const int tid = threadIdx.x;
+  int at[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    at[i] = tid + i * kThreads;
+    if (at[i] < n) buf[at[i]] = v[i] = sort_warp<LARGEST_FIRST>(v[i]);
+  }
+  __syncthreads();
+  U *from = buf, *to = buf + n;
+  for (int run = 32; run < n; run <<= 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (at[i] >= n) continue;
+      const U* other = from + ((at[i] & ~(run - 1)) ^ run);
+      const bool right = at[i] & run;  // of equal ones the left run's come first
+      int before = 0;
+      for (int s = run >> 1; s > 0; s >>= 1) {
+        const U o = other[before + s - 1];
+        if (precedes<LARGEST_FIRST>(o, v[i]) || (right && o == v[i])) before += s;
+      }
+      const U o = other[before];
+      before += precedes<LARGEST_FIRST>(o, v[i]) || (right && o == v[i]);
+      at[i] = (at[i] & ~(2 * run - 1)) + (at[i] & (run - 1)) + before;
+      to[at[i]] = v[i];
+    }
+    __syncthreads();
+    U* t = from;
+    from = to, to = t;
+  }
+  return from;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p, int cluster, int slice) {
+template <bool RANKS>
+constexpr int kHead = (sizeof(Shared) + (RANKS ? sizeof(Ranked) : 0) + 15) / 16 * 16;
+
+// RANKS: some row may have top-k or top-p.
+template <class T, bool RANKS>
+__global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(SampleParams p, int cluster, int slice) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   Shared& sh = *reinterpret_cast<Shared*>(dynamic);
-  T* mine = reinterpret_cast<T*>(dynamic + (sizeof(Shared) + 15) / 16 * 16);
+  Ranked& rs = *reinterpret_cast<Ranked*>(dynamic + sizeof(Shared));
+  T* mine = reinterpret_cast<T*>(dynamic + kHead<RANKS>);
   constexpr int kVec = 16 / sizeof(T);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x % cluster, warps = cluster * kWarps;
   const long long row = blockIdx.x / cluster;
   const int first = rank * slice, n = max(0, min(slice, p.vocab - first));
-  if (tid < kParts) sh.table[tid] = exp2((double)tid / kParts);
+  sh.table[tid] = exp2((double)tid / kParts);
+  static_assert(kThreads == kParts, "");
   if (tid == 0) sh.listed = 0, sh.first_equal = 0x7fffffff;
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   after_previous();
   const T* src = static_cast<const T*>(p.logits) + row * p.stride + first;
   const float heat = p.temperature ? p.temperature[row] : 1.f;
   const bool greedy = !(heat > 0.f);
-  const int k = greedy || !p.top_k ? 0 : p.top_k[row];
-  const float top_p = greedy || !p.top_p ? 1.f : p.top_p[row];
+  const int k = !RANKS || greedy || !p.top_k ? 0 : p.top_k[row];
+  const float top_p = !RANKS || greedy || !p.top_p ? 1.f : p.top_p[row];
   const float min_p = greedy || !p.min_p ? 0.f : p.min_p[row];
   const float u = p.random[row];
 
@@ -232,15 +256,8 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
   // For few top-k: each warp's each-th largest of its threads', which half of the warps reach at the least.
   const bool few = k > 0 && k <= min(kFew, kWarps / 2 * 32 * cluster);
   const int each = few ? (k + warps / 2 - 1) / (warps / 2) : 0;
-  if (few) {
-    float s = most;
-#pragma unroll
-    for (int kk = 2; kk <= 32; kk <<= 1)
-#pragma unroll
-      for (int j = kk >> 1; j > 0; j >>= 1) {
-        const float o = __shfl_xor_sync(0xffffffffu, s, j);
-        s = ((lane & j) == 0) == ((lane & kk) == 0) ? fmaxf(s, o) : fminf(s, o);
-      }
+  if (RANKS && few) {
+    const float s = sort_warp<true>(most);
     if (lane == each - 1)
       for (int r = 0; r < cluster; ++r) *of_rank(&sh.all_level[rank * kWarps + warp], r) = s;
   }
@@ -295,33 +312,33 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
   }
 
   const bool endless = most == INFINITY;
-  const double slope = kParts * 1.4426950408889634 / (double)heat;  // 64 log2 e / T
-  // 64 log2 of a weight; what is not there is at -inf or (of an infinite temperature) NaN.  Where the largest is
-  // infinite only its equals are there.
-  auto level_of = [&](float l) -> double {
-    if (endless) return l == most ? 0.0 : -INFINITY;
-    return ((double)l - (double)most) * slope;
-  };
-  // Below it weights, of less than 2^-999.7, count as 0; rounded so that none of less than 2^-1000 is above it.
-  const float least_level = endless ? kNone : __fsub_ru(most, __fmul_rd(693.f, heat));
-  // 2^(y/64) = 2^a 2^(b/64) e^z with whole a and b and |z| <= ln 2 / 128: 1 + z + z^2/2 + z^3/6 + z^4/24 is within 4e-14.
-  auto weight_at = [&](double y) -> double {
+  const double slope = kParts * 1.4426950408889634 / (double)heat;  // 512 log2 e / T
+  // 512 log2 of a weight, and the weight: 2^(y/512) = 2^a 2^(b/512) e^z with whole a and b and |z| <= ln 2 / 1024, for
+  // which 1 + z + z^2/2 + z^3/6 is within 9e-15.
+  auto level_of = [&](float l) -> double { return ((double)l - (double)most) * slope; };
+  auto weight_at = [&](double y, int& whole) -> double {
     const double shifted = y + kRound;
-    const int whole = __double2loint(shifted);
+    whole = __double2loint(shifted);
     const double r = y - (shifted - kRound);
     constexpr double c = 0.6931471805599453 / kParts;
-    double z = fma(r, c * c * c * c / 24, c * c * c / 6);
-    z = fma(r, z, c * c / 2);
-    z = fma(r, z, c);
+    const double z = fma(r, fma(r, c * c * c / 6, c * c / 2), c);
     const double t = sh.table[whole & (kParts - 1)];
     const double w = fma(t, z * r, t);
-    return __hiloint2double(__double2hiint(w) + ((whole >> 6) << 20), __double2loint(w));
+    return __hiloint2double(__double2hiint(w) + (whole >> 9 << 20), __double2loint(w));
   };
+  static_assert(kParts == 512, "");
+  // Below it weights, of less than 2^-999.7, count as 0; rounded so that none of less than 2^-1000 is above it.  Where
+  // the largest is infinite only its equals are there.
+  const float least_level = endless ? INFINITY : fmaxf(__fsub_ru(most, __fmul_rd(693.f, heat)), -3.4028235e38f);
   auto weight = [&](float l) -> double {
     if (endless) return l == most ? 1.0 : 0.0;
-    const double w = weight_at(((double)l - (double)most) * slope);
-    return l >= least_level && l > kNone ? w : 0.0;
+    int whole;
+    const double w = weight_at(level_of(l), whole);
+    return l >= least_level ? w : 0.0;
   };
+  // 64ths of an octave below the largest's
+  auto bin_of = [&](int whole) { return min(kBins - 1, -(whole >> 3)); };
+  static_assert(kPerBin == 8, "");
   auto units = [&](double w) -> unsigned long long {  // to the nearest
     return (unsigned long long)__double_as_longlong(fma(w, kUnit, kWhole)) & ((1ull << 52) - 1);
   };
@@ -344,37 +361,28 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     for (int i = 0; i < 2; ++i) {
       int at = tid + i * kThreads, r = 0;
       while (r < cluster && at >= sh.all_listed[r]) at -= sh.all_listed[r++];
-      v[i] = r < cluster ? of_rank(sh.list, r)[at] : 0;
+      v[i] = r < cluster ? of_rank(rs.list, r)[at] : 0;
     }
   };
   auto list = [&](T e, int i) {
     const int at = atomicAdd(&sh.listed, 1);
-    if (at < kList) sh.list[at] = entry(e, i);
+    if (at < kList) rs.list[at] = entry(e, i);
   };
   const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
   const double goal_share = u > 0.f ? (double)fminf(u, 1.f) : 0.0;
   const bool by_k = k > 0 && k < valid, by_p = top_p < 1.f;
 
   bool listed = false;  // the lists held what they had to
-  if (by_k && few) {
-    if (warp == 0) {
-      // the least of the groups' medians: half of each group's warps reach it
-      float low = INFINITY;
-      for (int g = 0; g < warps; g += 32) {
-        float s = g + lane < warps ? sh.all_level[g + lane] : kNone;
-#pragma unroll
-        for (int kk = 2; kk <= 32; kk <<= 1)
-#pragma unroll
-          for (int j = kk >> 1; j > 0; j >>= 1) {
-            const float o = __shfl_xor_sync(0xffffffffu, s, j);
-            s = ((lane & j) == 0) == ((lane & kk) == 0) ? fmaxf(s, o) : fminf(s, o);
-          }
-        low = fminf(low, __shfl_sync(0xffffffffu, s, min(32, warps) / 2 - 1));
-      }
-      if (lane == 0) sh.level = low;
+  if (RANKS && by_k && few) {
+    // the least of the groups' medians: half of each group's warps reach it
+    const int groups = (warps + 31) / 32;
+    if (warp < groups) {
+      const float s = sort_warp<true>(lane < warps ? sh.all_level[warp * 32 + lane] : kNone);
+      if (lane == min(32, warps) / 2 - 1) sh.level[warp] = s;
     }
     __syncthreads();
-    const float level = sh.level;
+    float level = sh.level[0];
+    for (int g = 1; g < groups; ++g) level = fminf(level, sh.level[g]);
     for_all(0, n, tid, kThreads, [&](int i, T e) {
       const float l = to_f32(e);
       if (l >= level && l > kNone) list(e, i);
@@ -393,11 +401,12 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
       if (rank != 0) return;
       int size = 32;
       while (size < count) size <<= 1;
-      sort_threads<true, 2>(v, size, &sh.sorted[0][0]);
+      const unsigned long long* sorted = sort_threads<true, 2>(v, size, &rs.sorted[0][0]);
       // thread t: the token of rank t
       const bool ranked = tid < k;
-      const int index = (int)(0xffffffffu - (uint32_t)v[0]);
-      const double w = ranked ? weight(value_of((uint32_t)(v[0] >> 32))) : 0.0;
+      const unsigned long long mine_of = ranked ? sorted[tid] : 0;
+      const int index = (int)(0xffffffffu - (uint32_t)mine_of);
+      const double w = ranked ? weight(value_of((uint32_t)(mine_of >> 32))) : 0.0;
       double total;
       const double before = scan_threads(w, sh.scan, &total);
       bool is = ranked && w >= least && (!endless || w > 0.0);
@@ -405,15 +414,16 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
       const int kept = __syncthreads_count(is);  // a prefix
       if (tid == 0 && p.kept) p.kept[row] = kept;
       // by index; the ranks lead to the weights
-      double* weights = reinterpret_cast<double*>(&sh.sorted[0][0]);
-      uint32_t* buf = reinterpret_cast<uint32_t*>(&sh.sorted[1][0]);
+      double* weights = reinterpret_cast<double*>(&rs.sorted[0][0]);
+      uint32_t* buf = reinterpret_cast<uint32_t*>(&rs.sorted[1][0]);
       weights[tid] = w;
       size = 32;
       while (size < kept) size <<= 1;
       uint32_t by_index[1] = {is ? (uint32_t)index << 9 | (uint32_t)tid : 0xffffffffu};
       __syncthreads();
-      sort_threads<false, 1>(by_index, size, buf);
-      const double x = tid < kept ? weights[by_index[0] & 511u] : 0.0;
+      const uint32_t* in_order = sort_threads<false, 1>(by_index, size, buf);
+      const uint32_t here = tid < kept ? in_order[tid] : 0;
+      const double x = tid < kept ? weights[here & 511u] : 0.0;
       const double at = scan_threads(x, sh.scan, &total);
       const double goal = goal_share * total;
       // the first whose end passes the goal, or the last with a weight
@@ -424,7 +434,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
         if (at + x > goal) atomicMin(&sh.first_equal, tid);
       }
       __syncthreads();
-      if (tid == min(sh.first_equal, sh.listed)) p.tokens[row] = (int)(by_index[0] >> 9);
+      if (tid == min(sh.first_equal, sh.listed)) p.tokens[row] = (int)(here >> 9);
       return;
     }
     __syncthreads();
@@ -433,17 +443,19 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
   // Where the kept ones end: a key, and the last index of it.
   uint32_t cut_key = 0;
   int cut_index = 0x7fffffff;
-  if (by_p && !by_k) {
-    for (int i = tid; i < kBins; i += kThreads) sh.low[i] = sh.high[i] = 0;
+  if (RANKS && by_p && !by_k) {
+    for (int i = tid; i < kBins; i += kThreads) rs.low[i] = rs.high[i] = 0;
     __syncthreads();
-    for_all(0, n, tid, kThreads, [&](int i, T e) {
+    for_all(0, n, tid, kThreads, [&](int, T e) {
       const float l = to_f32(e);
-      const unsigned long long m = units(weight(l));
+      if (l < least_level) return;
+      int whole = 0;
+      const unsigned long long m = units(endless ? 1.0 : weight_at(level_of(l), whole));
       if (m) {
-        const int bin = min(kBins - 1, -__double2loint(level_of(l) + kRound));
-        const uint32_t low = (uint32_t)m, old = atomicAdd(&sh.low[bin], low);
+        const int bin = bin_of(whole);
+        const uint32_t low = (uint32_t)m, old = atomicAdd(&rs.low[bin], low);
         const uint32_t high = (uint32_t)(m >> 32) + (old + low < old);
-        if (high) atomicAdd(&sh.high[bin], high);
+        if (high) atomicAdd(&rs.high[bin], high);
       }
     });
     cluster_sync();
@@ -452,8 +464,8 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     for (int bin = rank * per + tid; bin < (rank + 1) * per; bin += kThreads) {
       unsigned long long m = 0;
       for (int r = 0; r < cluster; ++r)
-        m += of_rank(sh.low, r)[bin] + ((unsigned long long)of_rank(sh.high, r)[bin] << 32);
-      sh.low[bin] = (uint32_t)m, sh.high[bin] = (uint32_t)(m >> 32);
+        m += of_rank(rs.low, r)[bin] + ((unsigned long long)of_rank(rs.high, r)[bin] << 32);
+      rs.low[bin] = (uint32_t)m, rs.high[bin] = (uint32_t)(m >> 32);
     }
     cluster_sync();
     constexpr int kEach = kBins / kThreads;
@@ -461,7 +473,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       const int b = tid * kEach + j, r = b / per;
-      mass += m[j] = of_rank(sh.low, r)[b] + ((unsigned long long)of_rank(sh.high, r)[b] << 32);
+      mass += m[j] = of_rank(rs.low, r)[b] + ((unsigned long long)of_rank(rs.high, r)[b] << 32);
     }
     unsigned long long inc = mass;
 #pragma unroll
@@ -488,7 +500,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
     const int bin = (int)sh.bin;
     for_all(0, n, tid, kThreads, [&](int i, T e) {
       const float l = to_f32(e);
-      if (l >= least_level && l > kNone && min(kBins - 1, -__double2loint(level_of(l) + kRound)) == bin) list(e, i);
+      if (l >= least_level && (endless ? 0 : bin_of(__double2loint(level_of(l) + kRound))) == bin) list(e, i);
     });
     __syncthreads();
     if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
@@ -503,17 +515,14 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
         gather_lists(v);
         int size = 32;
         while (size < count) size <<= 1;
-        sort_threads<true, 2>(v, size, &sh.sorted[0][0]);
         // thread t: ranks 2 t and 2 t + 1
-        unsigned long long* sorted = &sh.sorted[0][0];
-        __syncthreads();
-        sorted[tid] = v[0], sorted[tid + kThreads] = v[1];
+        const unsigned long long* sorted = sort_threads<true, 2>(v, size, &rs.sorted[0][0]);
         if (tid == 0) sh.first_equal = count - 1;
         __syncthreads();
         unsigned long long own[2], sum = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          v[i] = sorted[2 * tid + i];
+          v[i] = 2 * tid + i < count ? sorted[2 * tid + i] : 0;
           own[i] = 2 * tid + i < count ? units(weight(value_of((uint32_t)(v[i] >> 32)))) : 0;
           sum += own[i];
         }
@@ -546,7 +555,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
 
   const int run = (slice + kWarps * 32 * kVec - 1) / (kWarps * 32 * kVec) * (32 * kVec);
   const int r0 = min(padded, warp * run), r1 = min(padded, r0 + run);
-  if ((by_k || by_p) && !listed) {
+  if (RANKS && (by_k || by_p) && !listed) {
     // By descending digits of the keys: the cut after `wanted` tokens, or after a sum of `wanted`.
     unsigned long long ties = 0, equal = 0, kept_mass = 0;
     auto cut_at = [&](bool by_mass, unsigned long long wanted, bool masses) {
@@ -555,15 +564,15 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
       cut_key = 0;
       for (int high = kKeyBits<T>; high > 0;) {
         const int digit = min(11, high), shift = high - digit;
-        for (int i = tid; i < kBins; i += kThreads) sh.digits.count[i] = 0, sh.digits.mass[i] = 0;
+        for (int i = tid; i < kBins; i += kThreads) rs.digits.count[i] = 0, rs.digits.mass[i] = 0;
         __syncthreads();
         for_all(0, n, tid, kThreads, [&](int, T e) {
           const float l = to_f32(e);
           const uint32_t key = key_of(e);
           if (l > kNone && (key & known) == cut_key) {
             const uint32_t bin = key >> shift & ((1u << digit) - 1u);
-            atomicAdd(&sh.digits.count[bin], 1u);
-            if (masses) atomicAdd(&sh.digits.mass[bin], units(weight(l)));
+            atomicAdd(&rs.digits.count[bin], 1u);
+            if (masses) atomicAdd(&rs.digits.mass[bin], units(weight(l)));
           }
         });
         cluster_sync();
@@ -575,7 +584,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
         for (int j = 0; j < kEach; ++j) {
           const int bin = kBins - 1 - (tid * kEach + j);
           c[j] = 0, m[j] = 0;
-          for (int r = 0; r < cluster; ++r) c[j] += of_rank(sh.digits.count, r)[bin], m[j] += of_rank(sh.digits.mass, r)[bin];
+          for (int r = 0; r < cluster; ++r) c[j] += of_rank(rs.digits.count, r)[bin], m[j] += of_rank(rs.digits.mass, r)[bin];
           my_count += c[j], my_mass += m[j];
         }
         uint32_t inc = my_count;
@@ -624,10 +633,10 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
         for_all(0, n, tid, kThreads, [&](int, T e) { sum += units(weight(to_f32(e))); });
 #pragma unroll
         for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (lane == 0) sh.digits.mass[warp] = sum;
+        if (lane == 0) rs.digits.mass[warp] = sum;
         cluster_sync();
         base = 0;
-        for (int i = 0; i < warps; ++i) base += of_rank(sh.digits.mass, i / kWarps)[i % kWarps];
+        for (int i = 0; i < warps; ++i) base += of_rank(rs.digits.mass, i / kWarps)[i % kWarps];
         cluster_sync();
       }
       const double share = (double)fmaxf(top_p, 0.f) * (double)base;
@@ -756,21 +765,22 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p,
   }
 }
 
-template <class T>
+template <class T, bool RANKS>
 cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) {
-  constexpr int kMaxDevices = 64, kHead = (sizeof(Shared) + 15) / 16 * 16, kMaxBytes = 227 * 1024;
+  constexpr int kMaxDevices = 64, kMaxBytes = 227 * 1024;
+  static_assert(kHead<RANKS> + kSampleMaxVocab / kMaxCluster * (int)sizeof(T) <= kMaxBytes, "");
   static std::atomic<unsigned> asked[kMaxDevices];
   int cluster = 1;
   while (cluster < kMaxCluster && ((long long)p.rows * cluster * 2 <= sm_count ||
                                    ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > 32 * 1024))
     cluster *= 2;
-  const int slice = ((p.vocab + cluster - 1) / cluster + 7) / 8 * 8, smem = kHead + slice * (int)sizeof(T);
+  const int slice = ((p.vocab + cluster - 1) / cluster + 7) / 8 * 8, smem = kHead<RANKS> + slice * (int)sizeof(T);
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned gen = attr_generation(dev) + 1;
   if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
-    e = cudaFuncSetAttribute(sample_tokens_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBytes);
+    e = cudaFuncSetAttribute(sample_tokens_kernel<T, RANKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBytes);
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
   }
@@ -787,7 +797,12 @@ cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) 
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T>, p, cluster, slice);
+  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, RANKS>, p, cluster, slice);
+}
+
+template <class T>
+cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) {
+  return p.top_k || p.top_p ? launch_sample<T, true>(p, sm_count, st) : launch_sample<T, false>(p, sm_count, st);
 }
 
 }  // namespace
