@@ -31,7 +31,7 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8, kMaxWarps = kMaxCluster * kWarps;
 constexpr int kBins = 2048, kList = 1024, kFew = 400;
 constexpr int kParts = 512, kPerBin = 8;  // of an octave of weights: in the table, and of these in a bin
-constexpr float kNone = -INFINITY;
+constexpr float kNone = -INFINITY, kHuge = 3.4028235e38f;
 constexpr double kUnit = 17592186044416.0;  // 2^44: weights as integers, whose sums fit 64 bits
 constexpr double kWhole = 4503599627370496.0, kRound = 1.5 * kWhole;  // 2^52: added, a value's units are whole
 
@@ -95,10 +95,9 @@ struct Shared {
   float level[kMaxWarps / 32];
   double scan[kWarps];
   unsigned long long scan_mass[kWarps];
-  uint32_t scan_count[kWarps];
   uint32_t bin;
   unsigned long long above_mass;
-  uint32_t above_count, bin_count;
+  uint32_t bin_count;
   unsigned long long bin_mass;
 };
 
@@ -285,19 +284,27 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     }
     return;
   }
-  // Vectors of the CTA's slice, by threads; f(index in the slice, value).
-  auto for_all = [&](int from, int to, int start, int step, auto f) {
+  // Vectors of the CTA's slice, by threads: f(index in the slice, values), or of each f(index, value).
+  auto for_vectors = [&](int from, int to, int start, int step, auto f) {
     for (int i = from / kVec + start; i < (to + kVec - 1) / kVec; i += step) {
       const uint4 raw = reinterpret_cast<const uint4*>(mine)[i];
       const T* e = reinterpret_cast<const T*>(&raw);
+      float l[kVec];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) f(i * kVec + j, e[j]);
+      for (int j = 0; j < kVec; ++j) l[j] = to_f32(e[j]);
+      f(i * kVec, l);
     }
+  };
+  auto for_all = [&](int from, int to, int start, int step, auto f) {
+    for_vectors(from, to, start, step, [&](int i, const float(&l)[kVec]) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) f(i + j, l[j]);
+    });
   };
 
   if (greedy) {
-    for_all(0, n, tid, kThreads, [&](int i, T e) {
-      if (to_f32(e) == most) atomicMin(&sh.first_equal, i);
+    for_all(0, n, tid, kThreads, [&](int i, float l) {
+      if (l == most) atomicMin(&sh.first_equal, i);
     });
     __syncthreads();
     if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.first_equal;
@@ -315,7 +322,9 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   const double slope = kParts * 1.4426950408889634 / (double)heat;  // 512 log2 e / T
   // 512 log2 of a weight, and the weight: 2^(y/512) = 2^a 2^(b/512) e^z with whole a and b and |z| <= ln 2 / 1024, for
   // which 1 + z + z^2/2 + z^3/6 is within 9e-15.
-  auto level_of = [&](float l) -> double { return ((double)l - (double)most) * slope; };
+  // Where the largest is infinite only its equals are there, taken as the largest f32.
+  const float ref = endless ? kHuge : most;
+  auto level_of = [&](float l) -> double { return ((double)fminf(l, ref) - (double)ref) * slope; };
   auto weight_at = [&](double y, int& whole) -> double {
     const double shifted = y + kRound;
     whole = __double2loint(shifted);
@@ -327,11 +336,9 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     return __hiloint2double(__double2hiint(w) + (whole >> 9 << 20), __double2loint(w));
   };
   static_assert(kParts == 512, "");
-  // Below it weights, of less than 2^-999.7, count as 0; rounded so that none of less than 2^-1000 is above it.  Where
-  // the largest is infinite only its equals are there.
-  const float least_level = endless ? INFINITY : fmaxf(__fsub_ru(most, __fmul_rd(693.f, heat)), -3.4028235e38f);
+  // Below it weights, of less than 2^-999.7, count as 0; rounded so that none of less than 2^-1000 is above it.
+  const float least_level = endless ? INFINITY : fmaxf(__fsub_ru(most, __fmul_rd(693.f, heat)), -kHuge);
   auto weight = [&](float l) -> double {
-    if (endless) return l == most ? 1.0 : 0.0;
     int whole;
     const double w = weight_at(level_of(l), whole);
     return l >= least_level ? w : 0.0;
@@ -342,8 +349,8 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   auto units = [&](double w) -> unsigned long long {  // to the nearest
     return (unsigned long long)__double_as_longlong(fma(w, kUnit, kWhole)) & ((1ull << 52) - 1);
   };
-  auto entry = [&](T e, int i) -> unsigned long long {
-    return (unsigned long long)key_of(e) << 32 | (0xffffffffu - (uint32_t)(first + i));
+  auto entry = [&](float l, int i) -> unsigned long long {
+    return (unsigned long long)key_of(from_f32<T>(l)) << 32 | (0xffffffffu - (uint32_t)(first + i));
   };
   auto value_of = [&](uint32_t key) -> float {
     if constexpr (sizeof(T) == 4) {
@@ -364,15 +371,14 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
       v[i] = r < cluster ? of_rank(rs.list, r)[at] : 0;
     }
   };
-  auto list = [&](T e, int i) {
+  auto list = [&](float l, int i) {
     const int at = atomicAdd(&sh.listed, 1);
-    if (at < kList) rs.list[at] = entry(e, i);
+    if (at < kList) rs.list[at] = entry(l, i);
   };
   const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
   const double goal_share = u > 0.f ? (double)fminf(u, 1.f) : 0.0;
   const bool by_k = k > 0 && k < valid, by_p = top_p < 1.f;
 
-  bool listed = false;  // the lists held what they had to
   if (RANKS && by_k && few) {
     // the least of the groups' medians: half of each group's warps reach it
     const int groups = (warps + 31) / 32;
@@ -383,9 +389,9 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     __syncthreads();
     float level = sh.level[0];
     for (int g = 1; g < groups; ++g) level = fminf(level, sh.level[g]);
-    for_all(0, n, tid, kThreads, [&](int i, T e) {
-      const float l = to_f32(e);
-      if (l >= level && l > kNone) list(e, i);
+    const float bar = fmaxf(level, -kHuge);
+    for_all(0, n, tid, kThreads, [&](int i, float l) {
+      if (l >= bar) list(l, i);
     });
     __syncthreads();
     if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
@@ -393,8 +399,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     int count = 0;
     bool fits = true;
     for (int r = 0; r < cluster; ++r) count += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
-    listed = fits && count <= kList;
-    if (listed) {
+    if (fits && count <= kList) {
       unsigned long long v[2] = {0, 0};
       if (rank == 0) gather_lists(v);
       cluster_sync();  // no CTA reads another's after this
@@ -440,21 +445,33 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     __syncthreads();
   }
 
-  // Where the kept ones end: a key, and the last index of it.
-  uint32_t cut_key = 0;
-  int cut_index = 0x7fffffff;
-  if (RANKS && by_p && !by_k) {
+  const int run = (slice + kWarps * 32 * kVec - 1) / (kWarps * 32 * kVec) * (32 * kVec);
+  const int r0 = min(padded, warp * run), r1 = min(padded, r0 + run);
+  // Where the kept ones end: a value, and the last index of it.
+  float cut_value = endless ? kHuge : kNone;
+  int cut_index = -1;
+  auto above_cut = [&](int i, float l) { return l > cut_value || (l == cut_value && first + i <= cut_index); };
+  // Moves the cut up: of what is kept so far, the first `share` tokens, or those up to that share of their sum.
+  auto narrow = [&](bool by_mass, double share) {
     for (int i = tid; i < kBins; i += kThreads) rs.low[i] = rs.high[i] = 0;
+    if (tid == 0) sh.listed = 0;
     __syncthreads();
-    for_all(0, n, tid, kThreads, [&](int, T e) {
-      const float l = to_f32(e);
-      if (l < least_level) return;
-      int whole = 0;
-      const unsigned long long m = units(endless ? 1.0 : weight_at(level_of(l), whole));
-      if (m) {
-        const int bin = bin_of(whole);
-        const uint32_t low = (uint32_t)m, old = atomicAdd(&rs.low[bin], low);
-        const uint32_t high = (uint32_t)(m >> 32) + (old + low < old);
+    for_vectors(0, n, tid, kThreads, [&](int i, const float(&l)[kVec]) {
+      unsigned long long m[kVec];
+      int whole[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {  // all, before the first waits for another thread's addition
+        m[j] = units(weight_at(level_of(l[j]), whole[j]));
+        whole[j] = l[j] >= least_level ? whole[j] : kParts * -1000;
+        m[j] = by_mass && l[j] >= least_level ? m[j] : 0;
+        m[j] = above_cut(i + j, l[j]) ? (by_mass ? m[j] : 1) : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        if (m[j] == 0) continue;
+        const int bin = bin_of(whole[j]);
+        const uint32_t low = (uint32_t)m[j], old = atomicAdd(&rs.low[bin], low);
+        const uint32_t high = (uint32_t)(m[j] >> 32) + (old + low < old);
         if (high) atomicAdd(&rs.high[bin], high);
       }
     });
@@ -488,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
       if (w < warp) at += sh.scan_mass[w];
       all += sh.scan_mass[w];
     }
-    const double share = (double)fmaxf(top_p, 0.f) * (double)all;
+    if (by_mass) share *= (double)all;
     unsigned long long wanted = (unsigned long long)share;
     wanted = max(1ull, min(all, wanted + ((double)wanted < share)));
 #pragma unroll
@@ -498,9 +515,18 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     }
     __syncthreads();
     const int bin = (int)sh.bin;
-    for_all(0, n, tid, kThreads, [&](int i, T e) {
-      const float l = to_f32(e);
-      if (l >= least_level && (endless ? 0 : bin_of(__double2loint(level_of(l) + kRound))) == bin) list(e, i);
+    const unsigned long long above = sh.above_mass;
+    auto in_bin = [&](int i, float l) {
+      const int whole = l >= least_level ? __double2loint(level_of(l) + kRound) : kParts * -1000;
+      return bin_of(whole) == bin && above_cut(i, l);
+    };
+    for_vectors(0, n, tid, kThreads, [&](int i, const float(&l)[kVec]) {
+      bool is[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) is[j] = in_bin(i + j, l[j]);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (is[j]) list(l[j], i + j);
     });
     __syncthreads();
     if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
@@ -508,8 +534,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     int count = 0;
     bool fits = true;
     for (int r = 0; r < cluster; ++r) count += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
-    listed = fits && count <= kList;
-    if (listed) {
+    if (fits && count <= kList) {
       if (rank == 0) {
         unsigned long long v[2];
         gather_lists(v);
@@ -523,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           v[i] = 2 * tid + i < count ? sorted[2 * tid + i] : 0;
-          own[i] = 2 * tid + i < count ? units(weight(value_of((uint32_t)(v[i] >> 32)))) : 0;
+          own[i] = 2 * tid + i >= count ? 0 : by_mass ? units(weight(value_of((uint32_t)(v[i] >> 32)))) : 1;
           sum += own[i];
         }
         inc = sum;
@@ -534,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
         }
         if (lane == 31) sh.scan_mass[warp] = inc;
         __syncthreads();
-        unsigned long long passed = sh.above_mass + inc - sum;
+        unsigned long long passed = above + inc - sum;
         for (int w = 0; w < warp; ++w) passed += sh.scan_mass[w];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -549,148 +574,131 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
         }
       }
       cluster_sync();
-      cut_key = sh.cut_key, cut_index = sh.cut_index;
+      cut_value = value_of(sh.cut_key), cut_index = sh.cut_index;
+      return;
     }
-  }
-
-  const int run = (slice + kWarps * 32 * kVec - 1) / (kWarps * 32 * kVec) * (32 * kVec);
-  const int r0 = min(padded, warp * run), r1 = min(padded, r0 + run);
-  if (RANKS && (by_k || by_p) && !listed) {
-    // By descending digits of the keys: the cut after `wanted` tokens, or after a sum of `wanted`.
-    unsigned long long ties = 0, equal = 0, kept_mass = 0;
-    auto cut_at = [&](bool by_mass, unsigned long long wanted, bool masses) {
-      uint32_t known = 0;
-      unsigned long long above = 0, above_mass = 0, equal_mass = 0;
-      cut_key = 0;
-      for (int high = kKeyBits<T>; high > 0;) {
-        const int digit = min(11, high), shift = high - digit;
-        for (int i = tid; i < kBins; i += kThreads) rs.digits.count[i] = 0, rs.digits.mass[i] = 0;
-        __syncthreads();
-        for_all(0, n, tid, kThreads, [&](int, T e) {
-          const float l = to_f32(e);
-          const uint32_t key = key_of(e);
-          if (l > kNone && (key & known) == cut_key) {
-            const uint32_t bin = key >> shift & ((1u << digit) - 1u);
-            atomicAdd(&rs.digits.count[bin], 1u);
-            if (masses) atomicAdd(&rs.digits.mass[bin], units(weight(l)));
-          }
-        });
-        cluster_sync();
-        // thread t sums four bins over the CTAs, from the top down
-        constexpr int kEach = kBins / kThreads;
-        uint32_t c[kEach], my_count = 0;
-        unsigned long long m[kEach], my_mass = 0;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          const int bin = kBins - 1 - (tid * kEach + j);
-          c[j] = 0, m[j] = 0;
-          for (int r = 0; r < cluster; ++r) c[j] += of_rank(rs.digits.count, r)[bin], m[j] += of_rank(rs.digits.mass, r)[bin];
-          my_count += c[j], my_mass += m[j];
+    // More of nearly one value than a list holds: by descending digits of their keys.
+    uint32_t known = 0, key_so_far = 0;
+    unsigned long long before = above, equal = 0, equal_mass = 0;
+    for (int high = kKeyBits<T>; high > 0;) {
+      const int digit = min(11, high), shift = high - digit;
+      for (int i = tid; i < kBins; i += kThreads) rs.digits.count[i] = 0, rs.digits.mass[i] = 0;
+      __syncthreads();
+      for_all(0, n, tid, kThreads, [&](int i, float l) {
+        const uint32_t key = key_of(from_f32<T>(l));
+        if ((key & known) == key_so_far && in_bin(i, l)) {
+          const uint32_t b = key >> shift & ((1u << digit) - 1u);
+          atomicAdd(&rs.digits.count[b], 1u);
+          if (by_mass) atomicAdd(&rs.digits.mass[b], units(weight(l)));
         }
-        uint32_t inc = my_count;
-        unsigned long long inc_mass = my_mass;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const uint32_t o = __shfl_up_sync(0xffffffffu, inc, off);
-          const unsigned long long om = __shfl_up_sync(0xffffffffu, inc_mass, off);
-          if (lane >= off) inc += o, inc_mass += om;
-        }
-        if (lane == 31) sh.scan_count[warp] = inc, sh.scan_mass[warp] = inc_mass;
-        __syncthreads();
-        unsigned long long at = above + inc - my_count, at_mass = above_mass + inc_mass - my_mass;
-        for (int w = 0; w < warp; ++w) at += sh.scan_count[w], at_mass += sh.scan_mass[w];
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          const bool here = by_mass ? at_mass < wanted && wanted <= at_mass + m[j] : at < wanted && wanted <= at + c[j];
-          if (here) {
-            sh.bin = kBins - 1 - (tid * kEach + j);
-            sh.above_count = (uint32_t)at, sh.above_mass = at_mass;
-            sh.bin_count = c[j], sh.bin_mass = m[j];
-          }
-          at += c[j], at_mass += m[j];
-        }
-        cluster_sync();
-        above = sh.above_count, above_mass = sh.above_mass;
-        equal = sh.bin_count, equal_mass = sh.bin_mass;
-        cut_key |= sh.bin << shift;
-        known |= ((1u << digit) - 1u) << shift;
-        high = shift;
-        __syncthreads();
-      }
-      const unsigned long long one = equal_mass / equal;
-      if (!by_mass)
-        ties = wanted - above;
-      else
-        ties = one ? min(equal, (wanted - above_mass + one - 1) / one) : equal;
-      kept_mass = above_mass + ties * one;
-    };
-    cluster_sync();  // what lay there has been read
-    if (by_k) cut_at(false, (unsigned long long)k, by_p);
-    if (by_p) {
-      unsigned long long base = kept_mass;
-      if (!by_k) {  // the sum of all
-        unsigned long long sum = 0;
-        for_all(0, n, tid, kThreads, [&](int, T e) { sum += units(weight(to_f32(e))); });
-#pragma unroll
-        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (lane == 0) rs.digits.mass[warp] = sum;
-        cluster_sync();
-        base = 0;
-        for (int i = 0; i < warps; ++i) base += of_rank(rs.digits.mass, i / kWarps)[i % kWarps];
-        cluster_sync();
-      }
-      const double share = (double)fmaxf(top_p, 0.f) * (double)base;
-      const unsigned long long wanted = (unsigned long long)share;
-      cut_at(true, max(1ull, min(base, wanted + ((double)wanted < share))), true);
-    }
-    if (ties < equal) {  // the first of that key, by index
-      int same = 0;
-      for (int i = r0 + lane; i < min(r1, n); i += 32) same += key_of(mine[i]) == cut_key;
-      same = __reduce_add_sync(0xffffffffu, same);
-      if (lane < cluster) *of_rank(&sh.all_equal[rank * kWarps + warp], lane) = same;
+      });
       cluster_sync();
-      unsigned long long before = 0;
-      for (int i = 0; i < rank * kWarps + warp; ++i) before += sh.all_equal[i];
-      if (before < ties && ties <= before + same) {
-        for (int i0 = r0; i0 < min(r1, n); i0 += 32) {
-          const bool is = i0 + lane < min(r1, n) && key_of(mine[i0 + lane]) == cut_key;
-          const uint32_t votes = __ballot_sync(0xffffffffu, is);
-          if (before + __popc(votes) >= ties) {
-            if (is && __popc(votes & (0xffffffffu >> (31 - lane))) == (int)(ties - before))
-              for (int r = 0; r < cluster; ++r) *of_rank(&sh.cut_index, r) = first + i0 + lane;
-            break;
-          }
-          before += __popc(votes);
+      // thread t sums four bins over the CTAs, from the top down
+      uint32_t c[kEach];
+      mass = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const int b = kBins - 1 - (tid * kEach + j);
+        c[j] = 0, m[j] = 0;
+        for (int r = 0; r < cluster; ++r) c[j] += of_rank(rs.digits.count, r)[b], m[j] += of_rank(rs.digits.mass, r)[b];
+        if (!by_mass) m[j] = c[j];
+        mass += m[j];
+      }
+      inc = mass;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const unsigned long long o = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += o;
+      }
+      if (lane == 31) sh.scan_mass[warp] = inc;
+      __syncthreads();
+      at = before + inc - mass;
+      for (int w = 0; w < warp; ++w) at += sh.scan_mass[w];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (at < wanted && wanted <= at + m[j]) {
+          sh.bin = kBins - 1 - (tid * kEach + j);
+          sh.above_mass = at, sh.bin_mass = m[j], sh.bin_count = c[j];
         }
+        at += m[j];
       }
       cluster_sync();
-      cut_index = sh.cut_index;
+      before = sh.above_mass, equal = sh.bin_count, equal_mass = sh.bin_mass;
+      key_so_far |= sh.bin << shift;
+      known |= ((1u << digit) - 1u) << shift;
+      high = shift;
+      __syncthreads();
     }
+    // Of those with that key the first, by index.
+    const unsigned long long one = equal_mass / equal, ties = min(equal, (wanted - before + one - 1) / one);
+    const float cut = value_of(key_so_far);
+    int same = 0;
+    for (int i = r0 + lane; i < min(r1, n); i += 32) same += to_f32(mine[i]) == cut && above_cut(i, cut);
+    same = __reduce_add_sync(0xffffffffu, same);
+    if (lane < cluster) *of_rank(&sh.all_equal[rank * kWarps + warp], lane) = same;
+    cluster_sync();
+    unsigned long long earlier = 0;
+    for (int i = 0; i < rank * kWarps + warp; ++i) earlier += sh.all_equal[i];
+    if (earlier < ties && ties <= earlier + same) {
+      for (int i0 = r0; i0 < min(r1, n); i0 += 32) {
+        const int i = i0 + lane;
+        const bool is = i < min(r1, n) && to_f32(mine[i]) == cut && above_cut(i, cut);
+        const uint32_t votes = __ballot_sync(0xffffffffu, is);
+        if (earlier + __popc(votes) >= ties) {
+          if (is && __popc(votes & (0xffffffffu >> (31 - lane))) == (int)(ties - earlier))
+            for (int r = 0; r < cluster; ++r) *of_rank(&sh.cut_index, r) = first + i;
+          break;
+        }
+        earlier += __popc(votes);
+      }
+    }
+    cluster_sync();
+    cut_value = cut, cut_index = sh.cut_index;
+  };
+  if (RANKS) {
+#pragma unroll 1
+    for (int mass = by_k ? 0 : 1; mass <= (by_p ? 1 : 0); ++mass) narrow(mass != 0, mass ? (double)fmaxf(top_p, 0.f) : (double)k);
   }
 
-  float cut_value = kNone;
-  if (by_k || by_p) cut_value = value_of(cut_key);
-  if (endless && cut_value < most) cut_value = 3.4028235e38f, cut_index = -1;
-  if (cut_value == kNone) cut_index = -1;
   // 0 where the token is not kept
-  auto kept_weight = [&](int i, float l, bool& is) -> double {
-    is = l > cut_value || (l == cut_value && first + i <= cut_index);
-    if (!is) return 0.0;
+  auto kept_weight = [&](int i, float l) -> double {
     const double w = weight(l);
-    is = w >= least;
-    return is ? w : 0.0;
+    return above_cut(i, l) && w >= least ? w : 0.0;
   };
   // Warps own runs of the row, so that the runs' sums stand in the order of the tokens.
   double sum = 0.0;
   int count = 0;
   const bool plain = !by_k && !by_p && least == 0.0 && !endless;  // all that are there
   if (plain) {
-    for_all(r0, r1, lane, 32, [&](int, T e) { sum += weight(to_f32(e)); });
+    for_vectors(r0, r1, lane, 32, [&](int, const float(&l)[kVec]) {
+      double w[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) w[j] = weight(l[j]);
+#pragma unroll
+      for (int j = 1; j < kVec; j <<= 1)
+#pragma unroll
+        for (int i = 0; i < kVec; i += 2 * j) w[i] += w[i + j];
+      sum += w[0];
+    });
   } else {
-    for_all(r0, r1, lane, 32, [&](int i, T e) {
-      bool is;
-      sum += kept_weight(i, to_f32(e), is);
-      count += is;
+    for_vectors(r0, r1, lane, 32, [&](int i, const float(&l)[kVec]) {
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) any |= above_cut(i + j, l[j]);
+      if (!any) return;
+      double w[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        w[j] = weight(l[j]);
+        const bool is = above_cut(i + j, l[j]) && w[j] >= least;
+        w[j] = is ? w[j] : 0.0;
+        count += is;
+      }
+#pragma unroll
+      for (int j = 1; j < kVec; j <<= 1)
+#pragma unroll
+        for (int k = 0; k < kVec; k += 2 * j) w[k] += w[k + j];
+      sum += w[0];
     });
   }
 #pragma unroll
@@ -740,8 +748,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   const int w0 = min(n, owner % kWarps * run), w1 = min(n, w0 + run), share = (run + kThreads - 1) / kThreads;
   const int i0 = min(w1, w0 + tid * share), i1 = min(w1, i0 + share);
   double part = 0.0, ignored;
-  bool is;
-  for (int i = i0; i < i1; ++i) part += kept_weight(i, to_f32(mine[i]), is);
+  for (int i = i0; i < i1; ++i) part += kept_weight(i, to_f32(mine[i]));
   if (tid == 0) sh.first_equal = 0x7fffffff, sh.listed = -1;
   const double lo = before + scan_threads(part, sh.scan, &ignored);
   // the first thread whose end passes the goal, or the last with a sum
@@ -754,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     double running = lo;
     int token = -1;
     for (int i = i0; i < i1; ++i) {
-      const double w = kept_weight(i, to_f32(mine[i]), is);
+      const double w = kept_weight(i, to_f32(mine[i]));
       if (w > 0.0) {
         token = first + i;
         running += w;
@@ -770,9 +777,13 @@ cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) 
   constexpr int kMaxDevices = 64, kMaxBytes = 227 * 1024;
   static_assert(kHead<RANKS> + kSampleMaxVocab / kMaxCluster * (int)sizeof(T) <= kMaxBytes, "");
   static std::atomic<unsigned> asked[kMaxDevices];
+  // CTAs of a row: those that its size needs, and then, where the row may need its sums by bins (a pass of twice the
+  // others' work), while the launch stays within four a SM; without ranks, until there is about one a SM.  us with 2, 4, 8:
+  // 64 x 128256 bf16, top-p and others 88, 70, 62, plain 20, 26, 26; 256 x 32000 f32, all filters 31, 44, 77, plain 25, 30, 51.
   int cluster = 1;
-  while (cluster < kMaxCluster && ((long long)p.rows * cluster * 2 <= sm_count ||
-                                   ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > 32 * 1024))
+  while (cluster < kMaxCluster &&
+         ((RANKS ? (long long)p.rows * cluster * 2 <= 4 * sm_count : (long long)p.rows * cluster * 10 < 8 * sm_count) ||
+          kHead<RANKS> + ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > 112 * 1024))
     cluster *= 2;
   const int slice = ((p.vocab + cluster - 1) / cluster + 7) / 8 * 8, smem = kHead<RANKS> + slice * (int)sizeof(T);
   int dev = 0;
