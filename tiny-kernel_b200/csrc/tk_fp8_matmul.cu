@@ -325,10 +325,216 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
   return cudaLaunchKernelEx(&cfg, fp8_few_kernel<NT>, a_map, w_map, p, plan.split, stages);
 }
 
+// ---- many rows -----------------------------------------------------------------------------------------
+//
+// The activations are the product's 128 rows, 256 rows of the weight its columns.  A thread adds a row's half in
+// registers, so that its scale is one number a block: sum += scale * product.  Two accumulators of 256 columns fill
+// tensor memory: one is added up while the other's products run.  CTAs walk over the tiles, one an SM.
+
+constexpr int kManyThreads = 320;  // a warp of copies, one of products, eight of sums
+constexpr int kManyCols = 256, kManyStages = 4, kManyStageBytes = (128 + kManyCols) * kFp8Block;
+constexpr int kManyGroup = 16;  // tiles of rows that share the weight's tiles at a time, for L2
+constexpr int kPatch = 32 * 33 * 4;  // bytes of a warp's corner of shared memory, for rows off their 32-byte boundary
+
+struct ManyTile {
+  int m, n;
+};
+__device__ __forceinline__ ManyTile many_tile(int t, int tiles_m, int tiles_n) {
+  const int group = t / (kManyGroup * tiles_n), first = group * kManyGroup, rows = min(kManyGroup, tiles_m - first);
+  const int r = t - group * kManyGroup * tiles_n;
+  return {first + r % rows, r / rows};
+}
+
+// 32 values of a row.
+template <class T>
+__device__ __forceinline__ void store_32(T* dst, const float (&v)[32]) {
+  constexpr int kWords = 32 * sizeof(T) / 32;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) {
+    uint32_t y[8];
+    T* e = reinterpret_cast<T*>(y);
+#pragma unroll
+    for (int j = 0; j < 32 / (int)sizeof(T); ++j) e[j] = from_f32<T>(v[w * (32 / sizeof(T)) + j]);
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + w * (32 / sizeof(T))), "r"(y[0]), "r"(y[1]),
+                 "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+                 : "memory");
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_constant__ CUtensorMap a_map,
+                                                                   const __grid_constant__ CUtensorMap w_map,
+                                                                   Fp8MatmulParams p, int tiles_m, int tiles_n, int wide) {
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t full[kManyStages], empty[kManyStages], sums_full[2], sums_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
+  const int blocks = (p.k + kFp8Block - 1) / kFp8Block, tiles = tiles_m * tiles_n;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kManyStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 8);
+    mbar_init(&drained, 1);
+    fence_mbar_init();
+  }
+  after_previous();
+  if (warp == 1) tmem_alloc(&tmem_slot, 2 * kManyCols);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+  bool dead = false;
+  int issued = 0;
+  if (warp == 0) {
+    const uint64_t often = l2_evict_last();
+    for (int t = blockIdx.x; t < tiles && !dead; t += gridDim.x) {
+      const ManyTile tile = many_tile(t, tiles_m, tiles_n);
+      for (int b = 0; b < blocks; ++b, ++issued) {
+        const int stage = issued % kManyStages;
+        if (issued >= kManyStages) wait_phase(&empty[stage], (issued / kManyStages - 1) & 1, dead, p);
+        if (__any_sync(0xffffffffu, dead)) {
+          dead = true;
+          break;
+        }
+        if (elect_one()) {
+          uint8_t* to = smem + stage * kManyStageBytes;
+          mbar_arrive_expect_tx(&full[stage], kManyStageBytes);
+          tma_load_2d(to, &a_map, &full[stage], b * kFp8Block, tile.m * 128, often);
+          tma_load_2d(to + 128 * kFp8Block, &w_map, &full[stage], b * kFp8Block, tile.n * kManyCols, often);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = umma_idesc_f16(128, kManyCols);
+    int s = 0;
+    for (int t = blockIdx.x; t < tiles && !dead; t += gridDim.x)
+      for (int b = 0; b < blocks; ++b, ++s) {
+        const int stage = s % kManyStages, d = s & 1;
+        if (s >= 2) wait_phase(&sums_empty[d], (s / 2 - 1) & 1, dead, p);
+        wait_phase(&full[stage], (s / kManyStages) & 1, dead, p);
+        if (__any_sync(0xffffffffu, dead)) {
+          dead = true;
+          break;
+        }
+        tcgen05_fence_after();
+        if (elect_one()) {
+          const uint32_t at = smem_addr(smem) + stage * kManyStageBytes;
+          const uint64_t a = umma_smem_desc(at, 16, 1024, 2), w = umma_smem_desc(at + 128 * kFp8Block, 16, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_e4m3(tmem + d * kManyCols, a + 2 * k, w + 2 * k, idesc, k > 0);
+          umma_commit(&empty[stage]);
+          umma_commit(&sums_full[d]);
+        }
+        __syncwarp();
+      }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
+    float* patch = reinterpret_cast<float*>(smem + kManyStages * kManyStageBytes + (warp - 2) * kPatch);
+    int s = 0;
+    for (int t = blockIdx.x; t < tiles && !dead; t += gridDim.x) {
+      const ManyTile tile = many_tile(t, tiles_m, tiles_n);
+      const int row = tile.m * 128 + quarter * 32 + lane, col = tile.n * kManyCols + half * 128;
+      const float* a_scale = p.a_scales + (long long)min(row, p.m - 1) * blocks;
+      const float* w_scale = p.w_scales + (long long)min(col / kFp8Block, (p.n - 1) / kFp8Block) * blocks;
+      unsigned long long acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0;
+      float next = a_scale[0] * w_scale[0];
+      for (int b = 0; b < blocks; ++b, ++s) {
+        const int d = s & 1;
+        const unsigned long long f = pair_of(next, next);
+        if (b + 1 < blocks) next = a_scale[b + 1] * w_scale[b + 1];
+        wait_phase(&sums_full[d], (s / 2) & 1, dead, p);
+        if (__any_sync(0xffffffffu, dead)) {
+          dead = true;
+          break;
+        }
+        tcgen05_fence_after();
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t v[32];
+          tmem_ld16(from + d * kManyCols + c, v);
+          tmem_ld16(from + d * kManyCols + c + 16, v + 16);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            acc[c / 2 + j] = fma2(pair_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), f, acc[c / 2 + j]);
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sums_empty[d]);
+      }
+      if (dead) break;
+      T* out = static_cast<T*>(p.out) + row * p.out_stride + col;
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) {
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float2 y = values_of(acc[c / 2 + j]);
+          v[2 * j] = y.x, v[2 * j + 1] = y.y;
+        }
+        if (wide && col + c + 32 <= p.n) {
+          if (row < p.m) store_32(out + c, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) patch[lane * 33 + j] = v[j];
+          __syncwarp();
+          const int rows = min(32, p.m - (row - lane));
+          T* corner = static_cast<T*>(p.out) + (long long)(row - lane) * p.out_stride + col + c + lane;
+          if (col + c + lane < p.n)
+            for (int r = 0; r < rows; ++r) corner[r * p.out_stride] = from_f32<T>(patch[r * 33 + lane]);
+          __syncwarp();
+        }
+      }
+    }
+  }
+  // After a wait that gave up: what is in flight completes before its memory is given back.
+  if (__syncthreads_or(dead)) {
+    bool late = false;
+    if (warp == 0)
+      for (int s = max(0, issued - kManyStages); s < issued; ++s)
+        wait_phase(&full[s % kManyStages], (s / kManyStages) & 1, late, p);
+    if (warp == 1) {
+      if (elect_one()) umma_commit(&drained);
+      __syncwarp();
+      wait_phase(&drained, 0, late, p);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem, 2 * kManyCols);
+  }
+}
+
+template <class T>
+cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, const CUtensorMap& w_map, int sm_count,
+                        cudaStream_t st) {
+  constexpr int kMaxDevices = 64, smem = kManyStages * kManyStageBytes + 8 * kPatch + 1024;
+  static std::atomic<unsigned> asked[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned gen = attr_generation(dev) + 1;
+  if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
+    e = cudaFuncSetAttribute(fp8_many_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
+  }
+  const int tiles_m = (p.m + 127) / 128, tiles_n = (p.n + kManyCols - 1) / kManyCols;
+  const int wide = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_stride * (long long)sizeof(T))) % 32 == 0;
+  return launch(fp8_many_kernel<T>, dim3((unsigned)std::min(sm_count, tiles_m * tiles_n)), kManyThreads, smem, st, a_map,
+                w_map, p, tiles_m, tiles_n, wide);
+}
+
 }  // namespace
 
 Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count) {
   Fp8MatmulPlan plan;
+  if (m > 256) return {kManyCols, 1};
   plan.tile = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
   const long long tiles = (long long)((n + 127) / 128) * ((m + plan.tile - 1) / plan.tile);
   const int blocks = (k + kFp8Block - 1) / kFp8Block;
@@ -338,12 +544,17 @@ Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count) {
 }
 
 void fp8_box_rows(const Fp8MatmulPlan& plan, int* a_rows, int* w_rows) {
-  *a_rows = plan.tile;
-  *w_rows = 128;
+  *a_rows = std::min(plan.tile, 128);
+  *w_rows = plan.tile == kManyCols ? kManyCols : 128;
 }
 
 cudaError_t launch_fp8_matmul(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
                               const CUtensorMap& w_map, int sm_count, cudaStream_t st) {
+  if (plan.tile == kManyCols) {
+    if (p.dtype == kTypeF32) return launch_many<float>(p, a_map, w_map, sm_count, st);
+    return p.dtype == kTypeBF16 ? launch_many<__nv_bfloat16>(p, a_map, w_map, sm_count, st)
+                                : launch_many<__half>(p, a_map, w_map, sm_count, st);
+  }
   if (plan.tile == 16) return launch_few<16>(p, plan, a_map, w_map, st);
   if (plan.tile == 32) return launch_few<32>(p, plan, a_map, w_map, st);
   if (plan.tile == 64) return launch_few<64>(p, plan, a_map, w_map, st);
