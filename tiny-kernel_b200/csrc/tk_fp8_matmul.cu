@@ -187,16 +187,16 @@ __global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const __grid_const
 #pragma unroll
     for (int j = 0; j < NT / 2; ++j) acc[j] = 0;
     constexpr int kEach = (NT + 31) / 32;
-    float next[KS][kEach];
+    float next[KS][kEach], next_w[KS];  // multiplied when they are needed: not waited for before that
     auto fetch = [&](int s) {
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         const int b = b0 + s * KS + i;
-        const float w = b < b1 ? p.w_scales[(long long)tile * blocks + b] : 0.f;
+        next_w[i] = b < b1 ? p.w_scales[(long long)tile * blocks + b] : 0.f;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
           const int j = e * 32 + lane, token = token0 + j;
-          next[i][e] = b < b1 && j < NT && token < p.m ? p.a_scales[(long long)token * blocks + b] * w : 0.f;
+          next[i][e] = b < b1 && j < NT && token < p.m ? p.a_scales[(long long)token * blocks + b] : 0.f;
         }
       }
     };
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const __grid_const
       for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
-          if (e * 32 + lane < NT) factors[at][d][i][e * 32 + lane] = next[i][e];
+          if (e * 32 + lane < NT) factors[at][d][i][e * 32 + lane] = next[i][e] * next_w[i];
       if (s + 1 < steps) fetch(s + 1);
       __syncwarp();
       wait_phase(&sums_full[d], (s / 2) & 1, dead, p);
@@ -327,14 +327,59 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
 
 // ---- many rows -----------------------------------------------------------------------------------------
 //
-// The activations are the product's 128 rows, 256 rows of the weight its columns.  A thread adds a row's half in
-// registers, so that its scale is one number a block: sum += scale * product.  Two accumulators of 256 columns fill
-// tensor memory: one is added up while the other's products run.  CTAs walk over the tiles, one an SM.
+// The activations are the product's rows, 256 rows of the weight its columns.  Two CTAs share a product of 256 x 256:
+// each brings its 128 rows and half of the columns' weight, and has its rows' sums in its tensor memory.  (Alone, a
+// CTA would bring 48 KB a block to its 128 x 256 products, and writing and reading them would take shared memory
+// longer than the products take.)  A thread adds half of a row in registers, so that its scale is one number a block:
+// sum += scale * product.  Two accumulators of 256 columns fill tensor memory: one is added up while the other's
+// products run.  Pairs of CTAs walk over the tiles.
 
 constexpr int kManyThreads = 320;  // a warp of copies, one of products, eight of sums
-constexpr int kManyCols = 256, kManyStages = 4, kManyStageBytes = (128 + kManyCols) * kFp8Block;
-constexpr int kManyGroup = 16;  // tiles of rows that share the weight's tiles at a time, for L2
+constexpr int kManyRows = 256, kManyCols = 256, kManyStages = 6, kManyStageBytes = 2 * 128 * kFp8Block;  // a CTA's part
+constexpr int kManyGroup = 8;  // tiles of rows that share the weight's tiles at a time, for L2
 constexpr int kPatch = 32 * 33 * 4;  // bytes of a warp's corner of shared memory, for rows off their 32-byte boundary
+
+// The products of a pair, issued by its first CTA.
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
+}
+// Arrives on that barrier of both CTAs when every product issued so far by this thread completes.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ uint32_t of_first(const void* mine) {  // shared memory of the pair's first CTA
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_addr(mine)));
+  return at;
+}
+// A box into this CTA's shared memory, counted by a barrier of the first one's.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y,
+                                              uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 
 struct ManyTile {
   int m, n;
@@ -369,25 +414,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
   __shared__ uint64_t full[kManyStages], empty[kManyStages], sums_full[2], sums_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   uint8_t* smem = dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
   const int blocks = (p.k + kFp8Block - 1) / kFp8Block, tiles = tiles_m * tiles_n;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kManyStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-    for (int s = 0; s < 2; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 8);
+    for (int s = 0; s < 2; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 16);
     mbar_init(&drained, 1);
     fence_mbar_init();
   }
   after_previous();
-  if (warp == 1) tmem_alloc(&tmem_slot, 2 * kManyCols);
+  if (warp == 1) tmem_alloc_pair(&tmem_slot, 2 * kManyCols);
   tcgen05_fence_before();
   __syncthreads();
+  cluster_sync();
   tcgen05_fence_after();
   const uint32_t tmem = tmem_slot;
   bool dead = false;
   int issued = 0;
   if (warp == 0) {
     const uint64_t often = l2_evict_last();
-    for (int t = blockIdx.x; t < tiles && !dead; t += gridDim.x) {
+    for (int t = pair; t < tiles && !dead; t += pairs) {
       const ManyTile tile = many_tile(t, tiles_m, tiles_n);
       for (int b = 0; b < blocks; ++b, ++issued) {
         const int stage = issued % kManyStages;
@@ -398,17 +445,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
         }
         if (elect_one()) {
           uint8_t* to = smem + stage * kManyStageBytes;
-          mbar_arrive_expect_tx(&full[stage], kManyStageBytes);
-          tma_load_2d(to, &a_map, &full[stage], b * kFp8Block, tile.m * 128, often);
-          tma_load_2d(to + 128 * kFp8Block, &w_map, &full[stage], b * kFp8Block, tile.n * kManyCols, often);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kManyStageBytes);  // of both CTAs
+          const uint32_t bar = of_first(&full[stage]);
+          tma_load_pair(to, &a_map, bar, b * kFp8Block, tile.m * kManyRows + rank * 128, often);
+          tma_load_pair(to + 128 * kFp8Block, &w_map, bar, b * kFp8Block, tile.n * kManyCols + rank * 128, often);
         }
         __syncwarp();
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc = umma_idesc_f16(128, kManyCols);
+    constexpr uint32_t idesc = umma_idesc_f16(kManyRows, kManyCols);
     int s = 0;
-    for (int t = blockIdx.x; t < tiles && !dead; t += gridDim.x)
+    for (int t = pair; rank == 0 && t < tiles && !dead; t += pairs)
       for (int b = 0; b < blocks; ++b, ++s) {
         const int stage = s % kManyStages, d = s & 1;
         if (s >= 2) wait_phase(&sums_empty[d], (s / 2 - 1) & 1, dead, p);
@@ -422,9 +470,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
           const uint32_t at = smem_addr(smem) + stage * kManyStageBytes;
           const uint64_t a = umma_smem_desc(at, 16, 1024, 2), w = umma_smem_desc(at + 128 * kFp8Block, 16, 1024, 2);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_e4m3(tmem + d * kManyCols, a + 2 * k, w + 2 * k, idesc, k > 0);
-          umma_commit(&empty[stage]);
-          umma_commit(&sums_full[d]);
+          for (int k = 0; k < 4; ++k) umma_e4m3_pair(tmem + d * kManyCols, a + 2 * k, w + 2 * k, idesc, k > 0);
+          umma_commit_pair(&empty[stage]);
+          umma_commit_pair(&sums_full[d]);
         }
         __syncwarp();
       }
@@ -432,20 +480,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
     float* patch = reinterpret_cast<float*>(smem + kManyStages * kManyStageBytes + (warp - 2) * kPatch);
+    const uint32_t summed[2] = {of_first(&sums_empty[0]), of_first(&sums_empty[1])};
     int s = 0;
-    for (int t = blockIdx.x; t < tiles && !dead; t += gridDim.x) {
+    for (int t = pair; t < tiles && !dead; t += pairs) {
       const ManyTile tile = many_tile(t, tiles_m, tiles_n);
-      const int row = tile.m * 128 + quarter * 32 + lane, col = tile.n * kManyCols + half * 128;
+      const int row = tile.m * kManyRows + rank * 128 + quarter * 32 + lane, col = tile.n * kManyCols + half * 128;
       const float* a_scale = p.a_scales + (long long)min(row, p.m - 1) * blocks;
       const float* w_scale = p.w_scales + (long long)min(col / kFp8Block, (p.n - 1) / kFp8Block) * blocks;
       unsigned long long acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0;
-      float next = a_scale[0] * w_scale[0];
+      // (multiplied when they are needed: not waited for before that)
+      float next_a = a_scale[0], next_w = w_scale[0];
       for (int b = 0; b < blocks; ++b, ++s) {
         const int d = s & 1;
-        const unsigned long long f = pair_of(next, next);
-        if (b + 1 < blocks) next = a_scale[b + 1] * w_scale[b + 1];
+        const float scale = next_a * next_w;
+        const unsigned long long f = pair_of(scale, scale);
+        if (b + 1 < blocks) next_a = a_scale[b + 1], next_w = w_scale[b + 1];
         wait_phase(&sums_full[d], (s / 2) & 1, dead, p);
         if (__any_sync(0xffffffffu, dead)) {
           dead = true;
@@ -464,7 +515,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
         }
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sums_empty[d]);
+        if (lane == 0) arrive_at(summed[d]);
       }
       if (dead) break;
       T* out = static_cast<T*>(p.out) + row * p.out_stride + col;
@@ -494,19 +545,21 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
   // After a wait that gave up: what is in flight completes before its memory is given back.
   if (__syncthreads_or(dead)) {
     bool late = false;
-    if (warp == 0)
+    if (warp == 0 && rank == 0)
       for (int s = max(0, issued - kManyStages); s < issued; ++s)
         wait_phase(&full[s % kManyStages], (s / kManyStages) & 1, late, p);
-    if (warp == 1) {
-      if (elect_one()) umma_commit(&drained);
+    if (warp == 1 && rank == 0) {
+      if (elect_one()) umma_commit_pair(&drained);
       __syncwarp();
       wait_phase(&drained, 0, late, p);
     }
     __syncthreads();
   }
+  tcgen05_fence_before();
+  cluster_sync();  // neither CTA's memory goes while the other may use it
   if (warp == 1) {
     tcgen05_fence_after();
-    tmem_dealloc(tmem, 2 * kManyCols);
+    tmem_dealloc_pair(tmem, 2 * kManyCols);
   }
 }
 
@@ -524,10 +577,22 @@ cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, cons
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
   }
-  const int tiles_m = (p.m + 127) / 128, tiles_n = (p.n + kManyCols - 1) / kManyCols;
+  const int tiles_m = (p.m + kManyRows - 1) / kManyRows, tiles_n = (p.n + kManyCols - 1) / kManyCols;
   const int wide = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_stride * (long long)sizeof(T))) % 32 == 0;
-  return launch(fp8_many_kernel<T>, dim3((unsigned)std::min(sm_count, tiles_m * tiles_n)), kManyThreads, smem, st, a_map,
-                w_map, p, tiles_m, tiles_n, wide);
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(2 * std::min(sm_count / 2, tiles_m * tiles_n)));
+  cfg.blockDim = dim3(kManyThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, fp8_many_kernel<T>, a_map, w_map, p, tiles_m, tiles_n, wide);
 }
 
 }  // namespace
@@ -545,7 +610,7 @@ Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count) {
 
 void fp8_box_rows(const Fp8MatmulPlan& plan, int* a_rows, int* w_rows) {
   *a_rows = std::min(plan.tile, 128);
-  *w_rows = plan.tile == kManyCols ? kManyCols : 128;
+  *w_rows = 128;
 }
 
 cudaError_t launch_fp8_matmul(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
