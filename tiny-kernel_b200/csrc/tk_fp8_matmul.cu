@@ -18,16 +18,24 @@ namespace {
 
 constexpr unsigned kErrFp8Wait = 128u;  // a copy or a product never completed
 
-// Waits for the phase of `bar`; gives up, for good, after timeout_ns.
+// Waits for the phase of `bar`; gives up, for good, after timeout_ns.  The timer is read once in many tries, since a read
+// takes longer than a phase should be noticed late, and the phase is looked at once more after the last read: lanes of a
+// warp that wait for one phase agree.
 __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t phase, bool& dead, const Fp8MatmulParams& p) {
   if (dead || mbar_try_wait(bar, phase)) return;
-  const uint64_t t0 = global_timer_ns();
-  while (!mbar_try_wait(bar, phase))
-    if (global_timer_ns() - t0 > p.timeout_ns) {
+  uint64_t t0 = 0;
+  bool late = false;
+  for (uint32_t tries = 1; !mbar_try_wait(bar, phase); ++tries) {
+    if (late) {
       atomicOr(p.err, kErrFp8Wait);
       dead = true;
       return;
     }
+    if (tries % 64 != 0) continue;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    late = now - t0 > p.timeout_ns;
+  }
 }
 
 // D[tmem] (+)= A[smem] x B[smem], e4m3, f32 sums, 32 of k.  The instruction's word is that of f16: type 0 is e4m3 here.
@@ -434,15 +442,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
   int issued = 0;
   if (warp == 0) {
     const uint64_t often = l2_evict_last();
+    int stage = 0;
+    uint32_t phase = 1;  // a barrier's phase before its first counts as complete
     for (int t = pair; t < tiles && !dead; t += pairs) {
       const ManyTile tile = many_tile(t, tiles_m, tiles_n);
-      for (int b = 0; b < blocks; ++b, ++issued) {
-        const int stage = issued % kManyStages;
-        if (issued >= kManyStages) wait_phase(&empty[stage], (issued / kManyStages - 1) & 1, dead, p);
-        if (__any_sync(0xffffffffu, dead)) {
-          dead = true;
-          break;
-        }
+      for (int b = 0; b < blocks; ++b) {
+        wait_phase(&empty[stage], phase, dead, p);
+        __syncwarp();
+        if (dead) break;
         if (elect_one()) {
           uint8_t* to = smem + stage * kManyStageBytes;
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kManyStageBytes);  // of both CTAs
@@ -451,37 +458,44 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
           tma_load_pair(to + 128 * kFp8Block, &w_map, bar, b * kFp8Block, tile.n * kManyCols + rank * 128, often);
         }
         __syncwarp();
+        ++issued;
+        if (++stage == kManyStages) stage = 0, phase ^= 1;
       }
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc = umma_idesc_f16(kManyRows, kManyCols);
-    int s = 0;
+    const uint64_t a0 = umma_smem_desc(smem_addr(smem), 16, 1024, 2);
+    const uint64_t w0 = umma_smem_desc(smem_addr(smem) + 128 * kFp8Block, 16, 1024, 2);
+    int stage = 0, d = 0;
+    uint32_t phase = 0, sums_phase = 1;
     for (int t = pair; rank == 0 && t < tiles && !dead; t += pairs)
-      for (int b = 0; b < blocks; ++b, ++s) {
-        const int stage = s % kManyStages, d = s & 1;
-        if (s >= 2) wait_phase(&sums_empty[d], (s / 2 - 1) & 1, dead, p);
-        wait_phase(&full[stage], (s / kManyStages) & 1, dead, p);
-        if (__any_sync(0xffffffffu, dead)) {
-          dead = true;
-          break;
-        }
+      for (int b = 0; b < blocks; ++b) {
+        // (what is there earlier first: from the sums' word on there is little to do)
+        const uint64_t a = a0 + stage * (kManyStageBytes >> 4), w = w0 + stage * (kManyStageBytes >> 4);
+        const uint32_t to = tmem + d * kManyCols;
+        wait_phase(&full[stage], phase, dead, p);
+        wait_phase(&sums_empty[d], sums_phase, dead, p);
+        __syncwarp();
+        if (dead) break;
         tcgen05_fence_after();
         if (elect_one()) {
-          const uint32_t at = smem_addr(smem) + stage * kManyStageBytes;
-          const uint64_t a = umma_smem_desc(at, 16, 1024, 2), w = umma_smem_desc(at + 128 * kFp8Block, 16, 1024, 2);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_e4m3_pair(tmem + d * kManyCols, a + 2 * k, w + 2 * k, idesc, k > 0);
-          umma_commit_pair(&empty[stage]);
+          for (int k = 0; k < 4; ++k) umma_e4m3_pair(to, a + 2 * k, w + 2 * k, idesc, k > 0);
           umma_commit_pair(&sums_full[d]);
+          umma_commit_pair(&empty[stage]);
         }
         __syncwarp();
+        if (++stage == kManyStages) stage = 0, phase ^= 1;
+        sums_phase ^= d;
+        d ^= 1;
       }
   } else {
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
     float* patch = reinterpret_cast<float*>(smem + kManyStages * kManyStageBytes + (warp - 2) * kPatch);
-    const uint32_t summed[2] = {of_first(&sums_empty[0]), of_first(&sums_empty[1])};
-    int s = 0;
+    const uint32_t summed0 = of_first(&sums_empty[0]);
+    int d = 0;
+    uint32_t phase = 0;
     for (int t = pair; t < tiles && !dead; t += pairs) {
       const ManyTile tile = many_tile(t, tiles_m, tiles_n);
       const int row = tile.m * kManyRows + rank * 128 + quarter * 32 + lane, col = tile.n * kManyCols + half * 128;
@@ -492,30 +506,32 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
       for (int j = 0; j < 64; ++j) acc[j] = 0;
       // (multiplied when they are needed: not waited for before that)
       float next_a = a_scale[0], next_w = w_scale[0];
-      for (int b = 0; b < blocks; ++b, ++s) {
-        const int d = s & 1;
+      for (int b = 0; b < blocks; ++b) {
         const float scale = next_a * next_w;
         const unsigned long long f = pair_of(scale, scale);
         if (b + 1 < blocks) next_a = a_scale[b + 1], next_w = w_scale[b + 1];
-        wait_phase(&sums_full[d], (s / 2) & 1, dead, p);
-        if (__any_sync(0xffffffffu, dead)) {
-          dead = true;
-          break;
-        }
+        const uint32_t at = from + d * kManyCols;
+        wait_phase(&sums_full[d], phase, dead, p);
+        __syncwarp();
+        if (dead) break;
         tcgen05_fence_after();
 #pragma unroll
         for (int c = 0; c < 128; c += 32) {
           uint32_t v[32];
-          tmem_ld16(from + d * kManyCols + c, v);
-          tmem_ld16(from + d * kManyCols + c + 16, v + 16);
+          tmem_ld16(at + c, v);
+          tmem_ld16(at + c + 16, v + 16);
           tmem_ld_wait();
+          if (c == 96) {  // all read: the accumulator is free, whatever is still to be added
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(summed0 + d * (uint32_t)sizeof(uint64_t));
+          }
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             acc[c / 2 + j] = fma2(pair_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), f, acc[c / 2 + j]);
         }
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_at(summed[d]);
+        phase ^= d;
+        d ^= 1;
       }
       if (dead) break;
       T* out = static_cast<T*>(p.out) + row * p.out_stride + col;
