@@ -342,7 +342,10 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
 // sum += scale * product.  Two accumulators of 256 columns fill tensor memory: one is added up while the other's
 // products run.  Pairs of CTAs walk over the tiles.
 
-constexpr int kManyThreads = 320;  // a warp of copies, one of products, eight of sums
+// A warpgroup with a warp of copies and one of products, two of sums.  A thread of the sums holds 128 of them: the
+// registers of the launch, 168 for each thread, are handed from the first group to the others, 40 and 2 x 232 of 3 x 168.
+constexpr int kManyThreads = 384, kManyRegs = 168, kManyFewRegs = 40, kManyMoreRegs = 232;
+static_assert(kManyFewRegs + 2 * kManyMoreRegs <= 3 * kManyRegs, "the groups' shares");
 constexpr int kManyRows = 256, kManyCols = 256, kManyStages = 6, kManyStageBytes = 2 * 128 * kFp8Block;  // a CTA's part
 constexpr int kManyGroup = 8;  // tiles of rows that share the weight's tiles at a time, for L2
 constexpr int kPatch = 32 * 33 * 4;  // bytes of a warp's corner of shared memory, for rows off their 32-byte boundary
@@ -440,6 +443,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
   const uint32_t tmem = tmem_slot;
   bool dead = false;
   int issued = 0;
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyFewRegs));
   if (warp == 0) {
     const uint64_t often = l2_evict_last();
     int stage = 0;
@@ -489,10 +493,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
         sums_phase ^= d;
         d ^= 1;
       }
-  } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+  } else if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyMoreRegs));
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
-    float* patch = reinterpret_cast<float*>(smem + kManyStages * kManyStageBytes + (warp - 2) * kPatch);
+    float* patch = reinterpret_cast<float*>(smem + kManyStages * kManyStageBytes + (warp - 4) * kPatch);
     const uint32_t summed0 = of_first(&sums_empty[0]);
     int d = 0;
     uint32_t phase = 0;
@@ -589,6 +594,9 @@ cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, cons
   if (e != cudaSuccess) return e;
   const unsigned gen = attr_generation(dev) + 1;
   if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
+    cudaFuncAttributes has{};
+    if ((e = cudaFuncGetAttributes(&has, fp8_many_kernel<T>)) != cudaSuccess) return e;
+    if (has.numRegs < kManyRegs) return cudaErrorInvalidKernelImage;  // the sums would wait for registers for good
     e = cudaFuncSetAttribute(fp8_many_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
