@@ -84,14 +84,42 @@ __device__ __forceinline__ void store_out(const Fp8MatmulParams& p, long long at
     static_cast<__half*>(p.out)[at] = __float2half_rn(v);
 }
 
+// n of four values of a row, on the boundary of four of them or not.
+template <class T>
+__device__ __forceinline__ void store_four(T* dst, int n, const float4& v) {
+  const float e[4] = {v.x, v.y, v.z, v.w};
+  if (n >= 4 && reinterpret_cast<uintptr_t>(dst) % (4 * sizeof(T)) == 0) {
+    struct alignas(4 * sizeof(T)) Four {
+      T e[4];
+    } y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y.e[i] = from_f32<T>(e[i]);
+    *reinterpret_cast<Four*>(dst) = y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) dst[i] = from_f32<T>(e[i]);
+  }
+}
+__device__ __forceinline__ void store_four(const Fp8MatmulParams& p, long long at, int n, const float4& v) {
+  if (p.dtype == kTypeF32)
+    store_four(static_cast<float*>(p.out) + at, n, v);
+  else if (p.dtype == kTypeBF16)
+    store_four(static_cast<__nv_bfloat16*>(p.out) + at, n, v);
+  else
+    store_four(static_cast<__half*>(p.out) + at, n, v);
+}
+
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
+// Four values of a CTA of the cluster.  (Not ordered by the compiler among others: several travel at once; the barrier
+// before them and the one after are.)
+__device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
   uint32_t at;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  float4 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
   return v;
 }
 
@@ -101,7 +129,7 @@ __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
 // tile's blocks of k and add their sums through shared memory, in the order of their ranks.
 
 constexpr int kFewThreads = 192;  // a warp of copies, one of products, four of sums
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 8, kMaxSplit = 8;
 
 template <int NT>
 struct Few {
@@ -283,13 +311,21 @@ __global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const __grid_const
       }
     }
     cluster_sync();
-    if (warp >= 2 && !dead && out_row < p.n) {
-      const int j1 = min(NT * (rank + 1) / split, p.m - token0);
-      for (int j = NT * rank / split; j < j1; ++j) {
-        float sum = 0.f;
-        for (int r = 0; r < split; ++r) sum += ld_peer(smem_addr(mine + j * 128 + row), r);
-        store_out(p, (token0 + j) * p.out_stride + out_row, sum);
-      }
+    // the tokens' columns over the CTAs, four rows a thread, all CTAs' values at once
+    const int tokens = min(NT, p.m - token0), j0 = tokens * rank / split, j1 = tokens * (rank + 1) / split;
+    for (int i = threadIdx.x; !dead && i < (j1 - j0) * 32; i += kFewThreads) {
+      const int j = j0 + i / 32, row4 = i % 32 * 4, n = tile * 128 + row4;
+      if (n >= p.n) continue;
+      const uint32_t from = smem_addr(mine + j * 128 + row4);
+      float4 v[kMaxSplit];
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r)
+        if (r < split) v[r] = ld_peer(from, r);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r)
+        if (r < split) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+      store_four(p, (token0 + j) * p.out_stride + n, p.n - n, sum);
     }
     __syncwarp();
     cluster_sync();
@@ -342,7 +378,7 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
 // sum += scale * product.  Two accumulators of 256 columns fill tensor memory: one is added up while the other's
 // products run.  Pairs of CTAs walk over the tiles.
 
-// A warpgroup with a warp of copies and one of products, two of sums.  A thread of the sums holds 128 of them: the
+// A warpgroup with a warp of copies and two of products, two warpgroups of sums.  A thread of the sums holds 128 of them: the
 // registers of the launch, 168 for each thread, are handed from the first group to the others, 40 and 2 x 232 of 3 x 168.
 constexpr int kManyThreads = 384, kManyRegs = 168, kManyFewRegs = 40, kManyMoreRegs = 232;
 static_assert(kManyFewRegs + 2 * kManyMoreRegs <= 3 * kManyRegs, "the groups' shares");
@@ -431,7 +467,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
   if (threadIdx.x == 0) {
     for (int s = 0; s < kManyStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
     for (int s = 0; s < 2; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 16);
-    mbar_init(&drained, 1);
+    mbar_init(&drained, 2);
     fence_mbar_init();
   }
   after_previous();
@@ -466,7 +502,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
         if (++stage == kManyStages) stage = 0, phase ^= 1;
       }
     }
-  } else if (warp == 1) {
+  } else if (warp < 3) {  // an accumulator each: one waits for its sums while the other issues
     constexpr uint32_t idesc = umma_idesc_f16(kManyRows, kManyCols);
     const uint64_t a0 = umma_smem_desc(smem_addr(smem), 16, 1024, 2);
     const uint64_t w0 = umma_smem_desc(smem_addr(smem) + 128 * kFp8Block, 16, 1024, 2);
@@ -475,6 +511,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
     for (int t = pair; rank == 0 && t < tiles && !dead; t += pairs)
       for (int b = 0; b < blocks; ++b) {
         // (what is there earlier first: from the sums' word on there is little to do)
+        if (d != warp - 1) {
+          if (++stage == kManyStages) stage = 0, phase ^= 1;
+          sums_phase ^= d;
+          d ^= 1;
+          continue;
+        }
         const uint64_t a = a0 + stage * (kManyStageBytes >> 4), w = w0 + stage * (kManyStageBytes >> 4);
         const uint32_t to = tmem + d * kManyCols;
         wait_phase(&full[stage], phase, dead, p);
@@ -569,7 +611,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
     if (warp == 0 && rank == 0)
       for (int s = max(0, issued - kManyStages); s < issued; ++s)
         wait_phase(&full[s % kManyStages], (s / kManyStages) & 1, late, p);
-    if (warp == 1 && rank == 0) {
+    if ((warp == 1 || warp == 2) && rank == 0) {
       if (elect_one()) umma_commit_pair(&drained);
       __syncwarp();
       wait_phase(&drained, 0, late, p);
