@@ -125,38 +125,45 @@ __device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
 
 // ---- few rows ------------------------------------------------------------------------------------------
 //
-// The weight's rows are the product's 128 rows, the activations its NT columns.  The CTAs of a cluster share a
-// tile's blocks of k and add their sums through shared memory, in the order of their ranks.
+// The weight's rows are the product's 128 rows, the activations its NT columns: the weight is read once, by as many
+// CTAs as keep memory busy, two a SM.  Where there are fewer tiles than that, the CTAs of a cluster share a tile's blocks
+// of k and add their sums through shared memory, in the order of their ranks; where there are more, a CTA walks over
+// its tiles and its copies go on through their ends.
 
-constexpr int kFewThreads = 192;  // a warp of copies, one of products, four of sums
 constexpr int kMaxStages = 8, kMaxSplit = 8;
 
 template <int NT>
 struct Few {
-  static constexpr int kStep = NT == 128 ? 1 : 2;  // blocks of k between two waits
+  static constexpr int kStep = NT <= 32 ? 2 : 1;       // blocks of k between two waits
+  static constexpr int kGroups = NT >= 64 ? 2 : 1;     // warpgroups of sums, half of the columns each
+  static constexpr int kCols = NT / kGroups, kChunk = kCols < 32 ? kCols : 32;
+  static constexpr int kCtas = 2;                      // of an SM
+  static constexpr int kThreads = 64 + 128 * kGroups;  // a warp of copies, one of products, those of sums
+  static constexpr int kSums = 4;                      // steps in tensor memory
+  static constexpr uint32_t kColumns = kSums * kStep * NT;
   static constexpr int kBlockBytes = (128 + NT) * kFp8Block, kStageBytes = kStep * kBlockBytes;
-  static constexpr uint32_t kColumns = 2 * kStep * NT;  // of tensor memory: two steps
+  static constexpr int kStages = 220 * 1024 / kCtas / kStageBytes, kBytes = kStages * kStageBytes + 1024;
+  static_assert(kStages <= kMaxStages && NT * 512 <= kStages * kStageBytes, "shared memory");
 };
 
 template <int NT>
-__global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const __grid_constant__ CUtensorMap a_map,
-                                                              const __grid_constant__ CUtensorMap w_map,
-                                                              Fp8MatmulParams p, int split, int stages) {
+__global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_kernel(const __grid_constant__ CUtensorMap a_map,
+                                                                       const __grid_constant__ CUtensorMap w_map,
+                                                                       Fp8MatmulParams p, int split, int tiles_m, int tiles) {
   using M = Few<NT>;
-  constexpr int KS = M::kStep;
+  constexpr int KS = M::kStep, NC = M::kCols, CH = M::kChunk;
   extern __shared__ uint8_t dynamic[];
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], sums_full[2], sums_empty[2], drained;
+  __shared__ uint64_t full[M::kStages], empty[M::kStages], sums_full[M::kSums], sums_empty[M::kSums], drained;
   __shared__ uint32_t tmem_slot;
-  __shared__ __align__(16) float factors[4][2][KS][NT];
+  __shared__ __align__(16) float factors[4 * M::kGroups][2][KS][NC];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* smem = dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
-  const int tile = blockIdx.x / split, rank = blockIdx.x % split, token0 = blockIdx.y * NT;
+  const int rank = blockIdx.x % split, first = blockIdx.x / split, stride = gridDim.x / split;  // of tiles
   const int blocks = (p.k + kFp8Block - 1) / kFp8Block;
   const int b0 = (int)((long long)blocks * rank / split), b1 = (int)((long long)blocks * (rank + 1) / split);
-  const int steps = (b1 - b0 + KS - 1) / KS;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-    for (int s = 0; s < 2; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 4);
+    for (int s = 0; s < M::kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    for (int s = 0; s < M::kSums; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 4 * M::kGroups);
     mbar_init(&drained, 1);
     fence_mbar_init();
   }
@@ -168,119 +175,146 @@ __global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const __grid_const
   const uint32_t tmem = tmem_slot;
   bool dead = false;
   int issued = 0;
-  unsigned long long acc[NT / 2];
+  unsigned long long acc[NC / 2];
+  const int quarter = warp & 3, group = (warp - 2) >> 2, row = quarter * 32 + lane;
   if (warp == 0) {
-    const uint64_t once = l2_evict_first(), often = l2_evict_last();
-    for (int s = 0; s < steps; ++s) {
-      const int stage = s % stages;
-      if (s >= stages) wait_phase(&empty[stage], (s / stages - 1) & 1, dead, p);
-      if (__any_sync(0xffffffffu, dead)) {
-        dead = true;
-        break;
-      }
-      const int n = min(KS, b1 - b0 - s * KS);
-      if (elect_one()) {
-        uint8_t* to = smem + stage * M::kStageBytes;
-        mbar_arrive_expect_tx(&full[stage], n * M::kBlockBytes);
-        for (int i = 0; i < n; ++i) {
-          const int x = (b0 + s * KS + i) * kFp8Block;
-          tma_load_2d(to + i * 16384, &w_map, &full[stage], x, tile * 128, once);
-          tma_load_2d(to + KS * 16384 + i * NT * kFp8Block, &a_map, &full[stage], x, token0, often);
+    // the weight is read once, unless tiles of other tokens follow
+    const uint64_t once = tiles_m == 1 ? l2_evict_first() : l2_evict_last(), often = l2_evict_last();
+    int stage = 0;
+    uint32_t phase = 1;  // a barrier's phase before its first counts as complete
+    for (int t = first; t < tiles && !dead; t += stride) {
+      const int n0 = t / tiles_m * 128, token0 = t % tiles_m * NT;
+      for (int b = b0; b < b1; b += KS) {
+        wait_phase(&empty[stage], phase, dead, p);
+        __syncwarp();
+        if (dead) break;
+        const int n = min(KS, b1 - b);
+        if (elect_one()) {
+          uint8_t* to = smem + stage * M::kStageBytes;
+          mbar_arrive_expect_tx(&full[stage], n * M::kBlockBytes);
+          for (int i = 0; i < n; ++i) {
+            tma_load_2d(to + i * 16384, &w_map, &full[stage], (b + i) * kFp8Block, n0, once);
+            tma_load_2d(to + KS * 16384 + i * NT * kFp8Block, &a_map, &full[stage], (b + i) * kFp8Block, token0, often);
+          }
         }
+        __syncwarp();
+        ++issued;
+        if (++stage == M::kStages) stage = 0, phase ^= 1;
       }
-      __syncwarp();
-      issued = s + 1;
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc = umma_idesc_f16(128, NT);
-    for (int s = 0; s < steps; ++s) {
-      const int stage = s % stages, d = s & 1;
-      if (s >= 2) wait_phase(&sums_empty[d], (s / 2 - 1) & 1, dead, p);
-      wait_phase(&full[stage], (s / stages) & 1, dead, p);
-      if (__any_sync(0xffffffffu, dead)) {
-        dead = true;
-        break;
-      }
-      tcgen05_fence_after();
-      const int n = min(KS, b1 - b0 - s * KS);
-      if (elect_one()) {
-        const uint32_t at = smem_addr(smem) + stage * M::kStageBytes;
-        for (int i = 0; i < n; ++i) {
-          const uint64_t w = umma_smem_desc(at + i * 16384, 16, 1024, 2);
-          const uint64_t a = umma_smem_desc(at + KS * 16384 + i * NT * kFp8Block, 16, 1024, 2);
+    const uint64_t w0 = umma_smem_desc(smem_addr(smem), 16, 1024, 2);
+    const uint64_t a0 = umma_smem_desc(smem_addr(smem) + KS * 16384, 16, 1024, 2);
+    int stage = 0, d = 0;
+    uint32_t phase = 0, sums_phase = 1;
+    for (int t = first; t < tiles && !dead; t += stride)
+      for (int b = b0; b < b1; b += KS) {
+        const int n = min(KS, b1 - b);
+        wait_phase(&full[stage], phase, dead, p);
+        wait_phase(&sums_empty[d], sums_phase, dead, p);
+        __syncwarp();
+        if (dead) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_e4m3(tmem + (d * KS + i) * NT, w + 2 * k, a + 2 * k, idesc, k > 0);
+          for (int i = 0; i < KS; ++i) {
+            if (i >= n) break;
+            const uint64_t w = w0 + ((stage * M::kStageBytes + i * 16384) >> 4);
+            const uint64_t a = a0 + ((stage * M::kStageBytes + i * NT * kFp8Block) >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_e4m3(tmem + (d * KS + i) * NT, w + 2 * k, a + 2 * k, idesc, k > 0);
+          }
+          umma_commit(&sums_full[d]);
+          umma_commit(&empty[stage]);
         }
-        umma_commit(&empty[stage]);
-        umma_commit(&sums_full[d]);
+        __syncwarp();
+        if (++stage == M::kStages) stage = 0, phase ^= 1;
+        if (++d == M::kSums) d = 0, sums_phase ^= 1;
       }
-      __syncwarp();
-    }
   } else {
-    const int quarter = warp & 3, at = warp - 2;
-    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + group * NC;
+    float(&mine)[2][KS][NC] = factors[warp - 2];
+    constexpr int kEach = (NC + 31) / 32;
+    int d = 0, turn = 0;
+    uint32_t phase = 0;
+    for (int t = first; t < tiles && !dead; t += stride) {
+      const int n0 = t / tiles_m * 128, token0 = t % tiles_m * NT + group * NC;
+      const float* w_scale = p.w_scales + (long long)(t / tiles_m) * blocks;
 #pragma unroll
-    for (int j = 0; j < NT / 2; ++j) acc[j] = 0;
-    constexpr int kEach = (NT + 31) / 32;
-    float next[KS][kEach], next_w[KS];  // multiplied when they are needed: not waited for before that
-    auto fetch = [&](int s) {
+      for (int j = 0; j < NC / 2; ++j) acc[j] = 0;
+      float next[KS][kEach], next_w[KS];  // multiplied when they are needed: not waited for before that
+      auto fetch = [&](int b) {
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const int b = b0 + s * KS + i;
-        next_w[i] = b < b1 ? p.w_scales[(long long)tile * blocks + b] : 0.f;
+        for (int i = 0; i < KS; ++i) {
+          next_w[i] = b + i < b1 ? w_scale[b + i] : 0.f;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const int j = e * 32 + lane, token = token0 + j;
-          next[i][e] = b < b1 && j < NT && token < p.m ? p.a_scales[(long long)token * blocks + b] : 0.f;
-        }
-      }
-    };
-    fetch(0);
-    for (int s = 0; s < steps; ++s) {
-      const int d = s & 1;
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int e = 0; e < kEach; ++e)
-          if (e * 32 + lane < NT) factors[at][d][i][e * 32 + lane] = next[i][e] * next_w[i];
-      if (s + 1 < steps) fetch(s + 1);
-      __syncwarp();
-      wait_phase(&sums_full[d], (s / 2) & 1, dead, p);
-      if (__any_sync(0xffffffffu, dead)) {
-        dead = true;
-        break;
-      }
-      tcgen05_fence_after();
-      const int n = min(KS, b1 - b0 - s * KS);
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        if (i >= n) break;
-#pragma unroll
-        for (int c = 0; c < NT; c += 16) {
-          uint32_t t[16];
-          tmem_ld16(from + (d * KS + i) * NT + c, t);
-          tmem_ld_wait();
-          const float4* f = reinterpret_cast<const float4*>(&factors[at][d][i][c]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 g = f[j];
-            unsigned long long* to = &acc[c / 2 + 2 * j];
-            to[0] = fma2(pair_of(__uint_as_float(t[4 * j]), __uint_as_float(t[4 * j + 1])), pair_of(g.x, g.y), to[0]);
-            to[1] = fma2(pair_of(__uint_as_float(t[4 * j + 2]), __uint_as_float(t[4 * j + 3])), pair_of(g.z, g.w), to[1]);
+          for (int e = 0; e < kEach; ++e) {
+            const int j = e * 32 + lane, token = token0 + j;
+            next[i][e] = b + i < b1 && j < NC && token < p.m ? p.a_scales[(long long)token * blocks + b + i] : 0.f;
           }
         }
+      };
+      fetch(b0);
+      for (int b = b0; b < b1; b += KS) {
+        float(&now)[KS][NC] = mine[turn];
+        turn ^= 1;
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int e = 0; e < kEach; ++e)
+            if (e * 32 + lane < NC) now[i][e * 32 + lane] = next[i][e] * next_w[i];
+        if (b + KS < b1) fetch(b + KS);
+        const int n = min(KS, b1 - b);
+        wait_phase(&sums_full[d], phase, dead, p);
+        __syncwarp();
+        if (dead) break;
+        tcgen05_fence_after();
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          if (i >= n) break;
+#pragma unroll
+          for (int c = 0; c < NC; c += CH) {
+            uint32_t v[CH];
+#pragma unroll
+            for (int x = 0; x < CH; x += 16) tmem_ld16(from + (d * KS + i) * NT + c + x, v + x);
+            tmem_ld_wait();
+            if (c + CH == NC && i + 1 == n) {  // all read: the accumulators are free
+              tcgen05_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sums_empty[d]);
+            }
+            const float4* f = reinterpret_cast<const float4*>(&now[i][c]);
+#pragma unroll
+            for (int j = 0; j < CH / 4; ++j) {
+              const float4 g = f[j];
+              unsigned long long* to = &acc[c / 2 + 2 * j];
+              to[0] = fma2(pair_of(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), pair_of(g.x, g.y), to[0]);
+              to[1] = fma2(pair_of(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), pair_of(g.z, g.w), to[1]);
+            }
+          }
+        }
+        if (++d == M::kSums) d = 0, phase ^= 1;
       }
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sums_empty[d]);
+      if (split > 1 || dead) break;  // one tile a cluster
+      const int n = n0 + row;
+      if (n < p.n) {
+#pragma unroll
+        for (int j = 0; j < NC / 2; ++j) {
+          const float2 v = values_of(acc[j]);
+          const int token = token0 + 2 * j;
+          if (token < p.m) store_out(p, token * p.out_stride + n, v.x);
+          if (token + 1 < p.m) store_out(p, (token + 1) * p.out_stride + n, v.y);
+        }
+      }
     }
   }
   // After a wait that gave up: what is in flight completes before its memory is given back.
   if (__syncthreads_or(dead)) {
     bool late = false;
     if (warp == 0)
-      for (int s = max(0, issued - stages); s < issued; ++s) wait_phase(&full[s % stages], (s / stages) & 1, late, p);
+      for (int s = max(0, issued - M::kStages); s < issued; ++s)
+        wait_phase(&full[s % M::kStages], (s / M::kStages) & 1, late, p);
     if (warp == 1) {
       if (elect_one()) umma_commit(&drained);
       __syncwarp();
@@ -289,34 +323,24 @@ __global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const __grid_const
     dead = true;
     __syncthreads();
   }
-  const int row = (warp & 3) * 32 + lane, out_row = tile * 128 + row;
-  if (split == 1) {
-    if (warp >= 2 && !dead && out_row < p.n) {
-#pragma unroll
-      for (int j = 0; j < NT / 2; ++j) {
-        const float2 v = values_of(acc[j]);
-        const int token = token0 + 2 * j;
-        if (token < p.m) store_out(p, token * p.out_stride + out_row, v.x);
-        if (token + 1 < p.m) store_out(p, (token + 1) * p.out_stride + out_row, v.y);
-      }
-    }
-  } else {
-    float* mine = reinterpret_cast<float*>(smem);  // [NT][128]
+  if (split > 1) {
+    const int n0 = first / tiles_m * 128, token0 = first % tiles_m * NT;
+    float* sums = reinterpret_cast<float*>(smem);  // [NT][128]
     if (warp >= 2) {
 #pragma unroll
-      for (int j = 0; j < NT / 2; ++j) {
+      for (int j = 0; j < NC / 2; ++j) {
         const float2 v = values_of(acc[j]);
-        mine[2 * j * 128 + row] = v.x;
-        mine[(2 * j + 1) * 128 + row] = v.y;
+        sums[(group * NC + 2 * j) * 128 + row] = v.x;
+        sums[(group * NC + 2 * j + 1) * 128 + row] = v.y;
       }
     }
     cluster_sync();
     // the tokens' columns over the CTAs, four rows a thread, all CTAs' values at once
     const int tokens = min(NT, p.m - token0), j0 = tokens * rank / split, j1 = tokens * (rank + 1) / split;
-    for (int i = threadIdx.x; !dead && i < (j1 - j0) * 32; i += kFewThreads) {
-      const int j = j0 + i / 32, row4 = i % 32 * 4, n = tile * 128 + row4;
+    for (int i = threadIdx.x; !dead && i < (j1 - j0) * 32; i += M::kThreads) {
+      const int j = j0 + i / 32, row4 = i % 32 * 4, n = n0 + row4;
       if (n >= p.n) continue;
-      const uint32_t from = smem_addr(mine + j * 128 + row4);
+      const uint32_t from = smem_addr(sums + j * 128 + row4);
       float4 v[kMaxSplit];
 #pragma unroll
       for (int r = 0; r < kMaxSplit; ++r)
@@ -338,21 +362,20 @@ __global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const __grid_const
 
 template <int NT>
 cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
-                       const CUtensorMap& w_map, cudaStream_t st) {
+                       const CUtensorMap& w_map, int sm_count, cudaStream_t st) {
   using M = Few<NT>;
   constexpr int kMaxDevices = 64;
   static std::atomic<unsigned> asked[kMaxDevices];
-  const int stages = std::min(kMaxStages, (NT <= 32 ? 112 * 1024 : 222 * 1024) / M::kStageBytes);
-  const int smem = std::max(stages * M::kStageBytes, NT * 512) + 1024;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned gen = attr_generation(dev) + 1;
   if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
-    e = cudaFuncSetAttribute(fp8_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(fp8_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kBytes);
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
   }
+  const int tiles_m = (p.m + NT - 1) / NT, tiles = (p.n + 127) / 128 * tiles_m;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -360,13 +383,279 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
   attr[1].val.clusterDim.x = (unsigned)plan.split;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((p.n + 127) / 128 * plan.split), (unsigned)((p.m + NT - 1) / NT));
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.gridDim = dim3((unsigned)(plan.split > 1 ? tiles * plan.split : std::min(tiles, M::kCtas * sm_count)));
+  cfg.blockDim = dim3(M::kThreads);
+  cfg.dynamicSmemBytes = M::kBytes;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = plan.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, fp8_few_kernel<NT>, a_map, w_map, p, plan.split, stages);
+  return cudaLaunchKernelEx(&cfg, fp8_few_kernel<NT>, a_map, w_map, p, plan.split, tiles_m, tiles);
+}
+
+// ---- tiles with the activations as rows ------------------------------------------------------------------
+
+constexpr int kTileGroup = 8;  // tiles of rows that share the weight's tiles at a time, for L2
+constexpr int kPatch = 32 * 33 * 4;  // bytes of a warp's corner of shared memory, for rows off their 32-byte boundary
+
+struct Tile {
+  int m, n;
+};
+__device__ __forceinline__ Tile tile_of(int t, int tiles_m, int tiles_n) {
+  const int group = t / (kTileGroup * tiles_n), first = group * kTileGroup, rows = min(kTileGroup, tiles_m - first);
+  const int r = t - group * kTileGroup * tiles_n;
+  return {first + r % rows, r / rows};
+}
+
+// 32 values of a row.
+template <class T>
+__device__ __forceinline__ void store_32(T* dst, const float (&v)[32]) {
+  constexpr int kWords = 32 * sizeof(T) / 32;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) {
+    uint32_t y[8];
+    T* e = reinterpret_cast<T*>(y);
+#pragma unroll
+    for (int j = 0; j < 32 / (int)sizeof(T); ++j) e[j] = from_f32<T>(v[w * (32 / sizeof(T)) + j]);
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + w * (32 / sizeof(T))), "r"(y[0]), "r"(y[1]),
+                 "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+                 : "memory");
+  }
+}
+// 32 consecutive values of a row a lane, from column `at` on: whole sectors, or through the warp's corner of shared
+// memory where rows are off their boundary.
+template <class T>
+__device__ __forceinline__ void store_rows(const Fp8MatmulParams& p, int row, int at, bool wide, float* patch,
+                                           const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  if (wide && at + 32 <= p.n) {
+    if (row < p.m) store_32(static_cast<T*>(p.out) + row * p.out_stride + at, v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) patch[lane * 33 + j] = v[j];
+  __syncwarp();
+  const int rows = min(32, p.m - (row - lane));
+  T* corner = static_cast<T*>(p.out) + (long long)(row - lane) * p.out_stride + at + lane;
+  if (at + lane < p.n)
+    for (int r = 0; r < rows; ++r) corner[r * p.out_stride] = from_f32<T>(patch[r * 33 + lane]);
+  __syncwarp();
+}
+
+// ---- some rows -----------------------------------------------------------------------------------------
+//
+// Tiles of 128 rows by 128 of the weight's: a thread adds half of a row, whose scale is one number a block (in the form
+// for few rows it is one for each column, read from shared memory for each product).  Four accumulators.  CTAs of a
+// cluster share a tile's k, or walk over tiles, as above.
+
+constexpr int kSomeThreads = 320;  // a warp of copies, one of products, eight of sums
+constexpr int kSomeStages = 6, kSomeStageBytes = 2 * 128 * kFp8Block, kSomeSums = 4;
+constexpr int kSomePitch = 132;  // floats of a row of the exchange
+static_assert(128 * kSomePitch * 4 <= kSomeStages * kSomeStageBytes, "shared memory");
+
+template <class T>
+__global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_constant__ CUtensorMap a_map,
+                                                                   const __grid_constant__ CUtensorMap w_map,
+                                                                   Fp8MatmulParams p, int split, int tiles_m, int tiles_n,
+                                                                   int wide) {
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t full[kSomeStages], empty[kSomeStages], sums_full[kSomeSums], sums_empty[kSomeSums], drained;
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
+  const int rank = blockIdx.x % split, first = blockIdx.x / split, stride = gridDim.x / split, tiles = tiles_m * tiles_n;
+  const int blocks = (p.k + kFp8Block - 1) / kFp8Block;
+  const int b0 = (int)((long long)blocks * rank / split), b1 = (int)((long long)blocks * (rank + 1) / split);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSomeStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    for (int s = 0; s < kSomeSums; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 8);
+    mbar_init(&drained, 1);
+    fence_mbar_init();
+  }
+  after_previous();
+  if (warp == 1) tmem_alloc(&tmem_slot, kSomeSums * 128);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+  bool dead = false;
+  int issued = 0;
+  unsigned long long acc[32];
+  const int quarter = warp & 3, half = (warp - 2) >> 2;
+  if (warp == 0) {
+    const uint64_t once = tiles_m == 1 ? l2_evict_first() : l2_evict_last(), often = l2_evict_last();
+    int stage = 0;
+    uint32_t phase = 1;  // a barrier's phase before its first counts as complete
+    for (int t = first; t < tiles && !dead; t += stride) {
+      const Tile tile = tile_of(t, tiles_m, tiles_n);
+      for (int b = b0; b < b1; ++b) {
+        wait_phase(&empty[stage], phase, dead, p);
+        __syncwarp();
+        if (dead) break;
+        if (elect_one()) {
+          uint8_t* to = smem + stage * kSomeStageBytes;
+          mbar_arrive_expect_tx(&full[stage], kSomeStageBytes);
+          tma_load_2d(to, &a_map, &full[stage], b * kFp8Block, tile.m * 128, often);
+          tma_load_2d(to + 128 * kFp8Block, &w_map, &full[stage], b * kFp8Block, tile.n * 128, once);
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == kSomeStages) stage = 0, phase ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = umma_idesc_f16(128, 128);
+    const uint64_t a0 = umma_smem_desc(smem_addr(smem), 16, 1024, 2);
+    const uint64_t w0 = umma_smem_desc(smem_addr(smem) + 128 * kFp8Block, 16, 1024, 2);
+    int stage = 0, d = 0;
+    uint32_t phase = 0, sums_phase = 1;
+    for (int t = first; t < tiles && !dead; t += stride)
+      for (int b = b0; b < b1; ++b) {
+        const uint64_t a = a0 + stage * (kSomeStageBytes >> 4), w = w0 + stage * (kSomeStageBytes >> 4);
+        const uint32_t to = tmem + d * 128;
+        wait_phase(&full[stage], phase, dead, p);
+        wait_phase(&sums_empty[d], sums_phase, dead, p);
+        __syncwarp();
+        if (dead) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_e4m3(to, a + 2 * k, w + 2 * k, idesc, k > 0);
+          umma_commit(&sums_full[d]);
+          umma_commit(&empty[stage]);
+        }
+        __syncwarp();
+        if (++stage == kSomeStages) stage = 0, phase ^= 1;
+        if (++d == kSomeSums) d = 0, sums_phase ^= 1;
+      }
+  } else {
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * 64;
+    float* patch = reinterpret_cast<float*>(smem + kSomeStages * kSomeStageBytes + (warp - 2) * kPatch);
+    int d = 0;
+    uint32_t phase = 0;
+    for (int t = first; t < tiles && !dead; t += stride) {
+      const Tile tile = tile_of(t, tiles_m, tiles_n);
+      const int row = tile.m * 128 + quarter * 32 + lane, col = tile.n * 128 + half * 64;
+      const float* a_scale = p.a_scales + (long long)min(row, p.m - 1) * blocks;
+      const float* w_scale = p.w_scales + (long long)tile.n * blocks;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) acc[j] = 0;
+      // (multiplied when they are needed: not waited for before that)
+      float next_a = a_scale[b0], next_w = w_scale[b0];
+      for (int b = b0; b < b1; ++b) {
+        const float scale = next_a * next_w;
+        const unsigned long long f = pair_of(scale, scale);
+        if (b + 1 < b1) next_a = a_scale[b + 1], next_w = w_scale[b + 1];
+        const uint32_t at = from + d * 128;
+        wait_phase(&sums_full[d], phase, dead, p);
+        __syncwarp();
+        if (dead) break;
+        tcgen05_fence_after();
+        uint32_t v[64];
+#pragma unroll
+        for (int c = 0; c < 64; c += 16) tmem_ld16(at + c, v + c);
+        tmem_ld_wait();
+        tcgen05_fence_before();  // all read: the accumulator is free, whatever is still to be added
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sums_empty[d]);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          acc[j] = fma2(pair_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), f, acc[j]);
+        if (++d == kSomeSums) d = 0, phase ^= 1;
+      }
+      if (split > 1 || dead) break;  // one tile a cluster
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float2 y = values_of(acc[c / 2 + j]);
+          v[2 * j] = y.x, v[2 * j + 1] = y.y;
+        }
+        store_rows<T>(p, row, col + c, wide, patch, v);
+      }
+    }
+  }
+  // After a wait that gave up: what is in flight completes before its memory is given back.
+  if (__syncthreads_or(dead)) {
+    bool late = false;
+    if (warp == 0)
+      for (int s = max(0, issued - kSomeStages); s < issued; ++s)
+        wait_phase(&full[s % kSomeStages], (s / kSomeStages) & 1, late, p);
+    if (warp == 1) {
+      if (elect_one()) umma_commit(&drained);
+      __syncwarp();
+      wait_phase(&drained, 0, late, p);
+    }
+    dead = true;
+    __syncthreads();
+  }
+  if (split > 1) {
+    const Tile tile = tile_of(first, tiles_m, tiles_n);
+    float* sums = reinterpret_cast<float*>(smem);  // [128][pitch]
+    if (warp >= 2) {
+      float* mine = sums + (quarter * 32 + lane) * kSomePitch + half * 64;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 x = values_of(acc[2 * j]), y = values_of(acc[2 * j + 1]);
+        reinterpret_cast<float4*>(mine)[j] = make_float4(x.x, x.y, y.x, y.y);
+      }
+    }
+    cluster_sync();
+    // the rows over the CTAs, four columns a thread, all CTAs' values at once
+    const int rows = min(128, p.m - tile.m * 128), r0 = rows * rank / split, r1 = rows * (rank + 1) / split;
+    for (int i = threadIdx.x; !dead && i < (r1 - r0) * 32; i += kSomeThreads) {
+      const int r = r0 + i / 32, n = tile.n * 128 + i % 32 * 4;
+      if (n >= p.n) continue;
+      const uint32_t from = smem_addr(sums + r * kSomePitch + i % 32 * 4);
+      float4 v[kMaxSplit];
+#pragma unroll
+      for (int q = 0; q < kMaxSplit; ++q)
+        if (q < split) v[q] = ld_peer(from, q);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int q = 0; q < kMaxSplit; ++q)
+        if (q < split) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
+      store_four(static_cast<T*>(p.out) + (tile.m * 128 + r) * p.out_stride + n, p.n - n, sum);
+    }
+    __syncwarp();
+    cluster_sync();
+  }
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem, kSomeSums * 128);
+  }
+}
+
+template <class T>
+cudaError_t launch_some(const Fp8MatmulParams& p, int split, const CUtensorMap& a_map, const CUtensorMap& w_map,
+                        int sm_count, cudaStream_t st) {
+  constexpr int kMaxDevices = 64, smem = kSomeStages * kSomeStageBytes + 8 * kPatch + 1024;
+  static std::atomic<unsigned> asked[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned gen = attr_generation(dev) + 1;
+  if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
+    e = cudaFuncSetAttribute(fp8_some_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
+  }
+  const int tiles_m = (p.m + 127) / 128, tiles_n = (p.n + 127) / 128, tiles = tiles_m * tiles_n;
+  const int wide = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_stride * (long long)sizeof(T))) % 32 == 0;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : std::min(tiles, sm_count)));
+  cfg.blockDim = dim3(kSomeThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, fp8_some_kernel<T>, a_map, w_map, p, split, tiles_m, tiles_n, wide);
 }
 
 // ---- many rows -----------------------------------------------------------------------------------------
@@ -383,8 +672,6 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
 constexpr int kManyThreads = 384, kManyRegs = 168, kManyFewRegs = 40, kManyMoreRegs = 232;
 static_assert(kManyFewRegs + 2 * kManyMoreRegs <= 3 * kManyRegs, "the groups' shares");
 constexpr int kManyRows = 256, kManyCols = 256, kManyStages = 6, kManyStageBytes = 2 * 128 * kFp8Block;  // a CTA's part
-constexpr int kManyGroup = 8;  // tiles of rows that share the weight's tiles at a time, for L2
-constexpr int kPatch = 32 * 33 * 4;  // bytes of a warp's corner of shared memory, for rows off their 32-byte boundary
 
 // The products of a pair, issued by its first CTA.
 __device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -428,31 +715,6 @@ __device__ __forceinline__ void arrive_at(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-struct ManyTile {
-  int m, n;
-};
-__device__ __forceinline__ ManyTile many_tile(int t, int tiles_m, int tiles_n) {
-  const int group = t / (kManyGroup * tiles_n), first = group * kManyGroup, rows = min(kManyGroup, tiles_m - first);
-  const int r = t - group * kManyGroup * tiles_n;
-  return {first + r % rows, r / rows};
-}
-
-// 32 values of a row.
-template <class T>
-__device__ __forceinline__ void store_32(T* dst, const float (&v)[32]) {
-  constexpr int kWords = 32 * sizeof(T) / 32;
-#pragma unroll
-  for (int w = 0; w < kWords; ++w) {
-    uint32_t y[8];
-    T* e = reinterpret_cast<T*>(y);
-#pragma unroll
-    for (int j = 0; j < 32 / (int)sizeof(T); ++j) e[j] = from_f32<T>(v[w * (32 / sizeof(T)) + j]);
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + w * (32 / sizeof(T))), "r"(y[0]), "r"(y[1]),
-                 "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
-                 : "memory");
-  }
-}
-
 template <class T>
 __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_constant__ CUtensorMap a_map,
                                                                    const __grid_constant__ CUtensorMap w_map,
@@ -485,7 +747,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
     int stage = 0;
     uint32_t phase = 1;  // a barrier's phase before its first counts as complete
     for (int t = pair; t < tiles && !dead; t += pairs) {
-      const ManyTile tile = many_tile(t, tiles_m, tiles_n);
+      const Tile tile = tile_of(t, tiles_m, tiles_n);
       for (int b = 0; b < blocks; ++b) {
         wait_phase(&empty[stage], phase, dead, p);
         __syncwarp();
@@ -544,7 +806,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
     int d = 0;
     uint32_t phase = 0;
     for (int t = pair; t < tiles && !dead; t += pairs) {
-      const ManyTile tile = many_tile(t, tiles_m, tiles_n);
+      const Tile tile = tile_of(t, tiles_m, tiles_n);
       const int row = tile.m * kManyRows + rank * 128 + quarter * 32 + lane, col = tile.n * kManyCols + half * 128;
       const float* a_scale = p.a_scales + (long long)min(row, p.m - 1) * blocks;
       const float* w_scale = p.w_scales + (long long)min(col / kFp8Block, (p.n - 1) / kFp8Block) * blocks;
@@ -581,7 +843,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
         d ^= 1;
       }
       if (dead) break;
-      T* out = static_cast<T*>(p.out) + row * p.out_stride + col;
 #pragma unroll
       for (int c = 0; c < 128; c += 32) {
         float v[32];
@@ -590,18 +851,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
           const float2 y = values_of(acc[c / 2 + j]);
           v[2 * j] = y.x, v[2 * j + 1] = y.y;
         }
-        if (wide && col + c + 32 <= p.n) {
-          if (row < p.m) store_32(out + c, v);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) patch[lane * 33 + j] = v[j];
-          __syncwarp();
-          const int rows = min(32, p.m - (row - lane));
-          T* corner = static_cast<T*>(p.out) + (long long)(row - lane) * p.out_stride + col + c + lane;
-          if (col + c + lane < p.n)
-            for (int r = 0; r < rows; ++r) corner[r * p.out_stride] = from_f32<T>(patch[r * 33 + lane]);
-          __syncwarp();
-        }
+        store_rows<T>(p, row, col + c, wide, patch, v);
       }
     }
   }
@@ -663,15 +913,29 @@ cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, cons
 
 }  // namespace
 
+// Up to 64 rows the weight's rows are the product's, and a tile's k is split while a SM has no CTA (us with 1, 2, 4, 8 parts:
+// 1 x 4096 x 14336 12.4, 13.3, 16.4, 22.5; 1 x 4096 x 4096 9.6, 7.2, 5.7, 6.3; 64 x 14336 x 4096 43, 25, 16, 17).
+// Above, what is expected to take least: a block of k takes a tile of 128 x 128 0.4 us, one of 256 x 256 0.48, tiles go
+// round by round over the SMs or their pairs, and a split costs 3 us (128 x 4096 x 4096 15.5, 12.4, 10.0 in tiles of
+// 128, 18.0 of 256; 128 x 4096 x 14336 16.9 and 20.2; 256 x 4096 x 14336 29.7 and 20.7).
 Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count) {
-  Fp8MatmulPlan plan;
-  if (m > 256) return {kManyCols, 1};
-  plan.tile = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-  const long long tiles = (long long)((n + 127) / 128) * ((m + plan.tile - 1) / plan.tile);
   const int blocks = (k + kFp8Block - 1) / kFp8Block;
-  plan.split = 1;
-  while (plan.split < 8 && tiles * plan.split * 2 <= sm_count * 2 && plan.split * 4 <= blocks) plan.split *= 2;
-  return plan;
+  const long long tiles_n = (n + 127) / 128;
+  if (m <= 64) {
+    Fp8MatmulPlan plan{m <= 16 ? 16 : m <= 32 ? 32 : 64, 1};
+    while (plan.split < kMaxSplit && tiles_n * plan.split * 2 <= sm_count && plan.split * 8 <= blocks) plan.split *= 2;
+    return plan;
+  }
+  const auto rounds = [](long long tiles, int places) { return (double)((tiles + places - 1) / places); };
+  Fp8MatmulPlan best{kManyCols, 1};
+  double least = 4.5 + rounds((long long)((m + 255) / 256) * ((n + 255) / 256), sm_count / 2) * blocks * 0.48;
+  for (int split = 1; split <= kMaxSplit / 2 && (split == 1 || split * 4 <= blocks); split *= 2) {
+    const long long tiles = (m + 127) / 128 * tiles_n;
+    if (split > 1 && tiles * split > sm_count) break;
+    const double us = 3.0 + rounds(tiles * split, sm_count) * ((blocks + split - 1) / split) * 0.4 + (split > 1 ? 3.0 : 0.0);
+    if (us < least) least = us, best = {128, split};
+  }
+  return best;
 }
 
 void fp8_box_rows(const Fp8MatmulPlan& plan, int* a_rows, int* w_rows) {
@@ -686,10 +950,14 @@ cudaError_t launch_fp8_matmul(const Fp8MatmulParams& p, const Fp8MatmulPlan& pla
     return p.dtype == kTypeBF16 ? launch_many<__nv_bfloat16>(p, a_map, w_map, sm_count, st)
                                 : launch_many<__half>(p, a_map, w_map, sm_count, st);
   }
-  if (plan.tile == 16) return launch_few<16>(p, plan, a_map, w_map, st);
-  if (plan.tile == 32) return launch_few<32>(p, plan, a_map, w_map, st);
-  if (plan.tile == 64) return launch_few<64>(p, plan, a_map, w_map, st);
-  return launch_few<128>(p, plan, a_map, w_map, st);
+  if (plan.tile == 128) {
+    if (p.dtype == kTypeF32) return launch_some<float>(p, plan.split, a_map, w_map, sm_count, st);
+    return p.dtype == kTypeBF16 ? launch_some<__nv_bfloat16>(p, plan.split, a_map, w_map, sm_count, st)
+                                : launch_some<__half>(p, plan.split, a_map, w_map, sm_count, st);
+  }
+  if (plan.tile == 16) return launch_few<16>(p, plan, a_map, w_map, sm_count, st);
+  if (plan.tile == 32) return launch_few<32>(p, plan, a_map, w_map, sm_count, st);
+  return launch_few<64>(p, plan, a_map, w_map, sm_count, st);
 }
 
 }  // namespace tk
