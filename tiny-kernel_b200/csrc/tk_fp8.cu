@@ -23,27 +23,61 @@ namespace {
 constexpr int kE = 8;  // values of a thread's chunk: 16 bytes of 16-bit types, 8 bytes of codes
 constexpr float kLargest = 448.f, kLeastScale = 1.17549435e-38f;  // of e4m3; 2^-126
 
-// 16-byte loads and stores of every row: 0 by elements, 1 by 16 bytes, 2 by 32.
+// Whether every row of values lies on a boundary of 16 bytes.
 template <class T>
-int wide(const void* base, long long stride) {
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(base) | (uintptr_t)(stride * (long long)sizeof(T));
-  if (sizeof(T) == 4 && bits % 32 == 0) return 2;
-  return bits % 16 == 0 ? 1 : 0;
+bool even(const void* base, long long stride) {
+  return (reinterpret_cast<uintptr_t>(base) | (uintptr_t)(stride * (long long)sizeof(T))) % 16 == 0;
 }
 
-template <class T>
-__device__ __forceinline__ void load_chunk(const T* src, int n, int vec, float (&v)[kE]) {
-  if (n >= kE) {
-    load_f32<T, kE>(src, vec, v);
-  } else {
+// A thread's chunk as it lies in memory.  FAST: rows on 16-byte boundaries and of whole chunks, so that a load is 16 or 32
+// bytes; all of a thread's are on their way before the first is looked at (loads that were converted one after the
+// other took bf16 rows longer than f32 ones).  Otherwise by elements.
+template <class T, bool FAST>
+struct Chunk {
+  uint4 raw[FAST ? sizeof(T) * kE / 16 : 1];
+  T e[FAST ? 1 : kE];
+  __device__ __forceinline__ void load(const T* src, int n) {
+    if constexpr (FAST) {
+      if (n <= 0) {
 #pragma unroll
-    for (int i = 0; i < kE; ++i) v[i] = i < n ? to_f32(src[i]) : 0.f;
+        for (int w = 0; w < (int)sizeof(T) * kE / 16; ++w) raw[w] = make_uint4(0, 0, 0, 0);
+      } else if constexpr (sizeof(T) == 4) {
+        raw[0] = reinterpret_cast<const uint4*>(src)[0];
+        raw[1] = reinterpret_cast<const uint4*>(src)[1];
+      } else {
+        raw[0] = *reinterpret_cast<const uint4*>(src);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i) e[i] = i < n ? src[i] : from_f32<T>(0.f);
+    }
   }
-}
-template <class T>
-__device__ __forceinline__ void store_chunk(T* dst, int n, int vec, const float (&v)[kE]) {
-  if (n >= kE) {
-    store_f32<T, kE>(dst, vec, v);
+  __device__ __forceinline__ void values(float (&v)[kE]) const {
+    if constexpr (!FAST) {
+#pragma unroll
+      for (int i = 0; i < kE; ++i) v[i] = to_f32(e[i]);
+    } else if constexpr (sizeof(T) == 4) {
+      const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+      for (int i = 0; i < kE; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+      const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = y.x, v[2 * i + 1] = y.y;
+        } else {
+          v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      }
+    }
+  }
+};
+template <class T, bool FAST>
+__device__ __forceinline__ void store_chunk(T* dst, int n, const float (&v)[kE]) {
+  if constexpr (FAST) {
+    store_f32<T, kE>(dst, 1, v);
   } else {
 #pragma unroll
     for (int i = 0; i < kE; ++i)
@@ -74,14 +108,15 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return lo | (uint32_t)hi << 16;
 }
-// vec: dst is on an 8-byte boundary.
-__device__ __forceinline__ void store_codes(uint8_t* dst, int n, bool vec, const float (&v)[kE], const GroupScale& g) {
+// FAST: dst is on an 8-byte boundary.
+template <bool FAST>
+__device__ __forceinline__ void store_codes(uint8_t* dst, int n, const float (&v)[kE], const GroupScale& g) {
   uint2 y = make_uint2(0, 0);
   if (g.over != 0.f) {
     y.x = codes4(v[0] * g.over, v[1] * g.over, v[2] * g.over, v[3] * g.over);
     y.y = codes4(v[4] * g.over, v[5] * g.over, v[6] * g.over, v[7] * g.over);
   }
-  if (vec && n >= kE) {
+  if (FAST) {
     *reinterpret_cast<uint2*>(dst) = y;
   } else {
 #pragma unroll
@@ -92,38 +127,35 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, int n, bool vec, const
 
 // ---- norm ------------------------------------------------------------------------------------------
 
-struct RowVecs {
-  int x, residual, sum, weight, codes;
-};
-
 // `warps` warps a row, V chunks a thread; a block has as many rows as its warps make.
-template <class T, int V>
-__global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(Fp8RowsParams p, int warps, RowVecs vec) {
+template <class T, int V, int THREADS, bool FAST>
+__global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(Fp8RowsParams p, int warps) {
   __shared__ float part[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = warp / warps * warps;
   const long long row = (long long)blockIdx.x * (blockDim.x / 32 / warps) + warp / warps;
   const bool live = row < p.rows;
   const int at = ((warp - first) * 32 + lane) * kE, step = warps * 32 * kE;
   after_previous();
+  Chunk<T, FAST> x[V], r[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = at + i * step, n = live ? p.dim - e : 0;
+    x[i].load(static_cast<const T*>(p.x) + row * p.x_stride + e, n);
+    if (p.residual) r[i].load(static_cast<const T*>(p.residual) + row * p.residual_stride + e, n);
+  }
   float v[V][kE];
   float squares = 0.f;
-  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-  const T* res = static_cast<const T*>(p.residual) + row * p.residual_stride;
-  float r[V][kE];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = at + i * step, n = live ? p.dim - e : 0;
-    load_chunk(x + e, n, vec.x, v[i]);
-    if (p.residual) load_chunk(res + e, n, vec.residual, r[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = at + i * step, n = live ? p.dim - e : 0;
+    x[i].values(v[i]);
     if (p.residual) {
+      float y[kE];
+      r[i].values(y);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) v[i][j] += r[i][j];
+      for (int j = 0; j < kE; ++j) v[i][j] += y[j];
     }
-    if (p.sum) store_chunk(static_cast<T*>(p.sum) + row * p.sum_stride + e, n, vec.sum, v[i]);
+    if (p.sum && n > 0) store_chunk<T, FAST>(static_cast<T*>(p.sum) + row * p.sum_stride + e, n, v[i]);
 #pragma unroll
     for (int j = 0; j < kE; ++j) squares = fmaf(v[i][j], v[i][j], squares);
   }
@@ -139,11 +171,13 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(Fp8RowsParams p, 
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = at + i * step, n = live ? p.dim - e : 0;
-    float w[kE];
     if (p.weight) {
-      load_chunk(p.weight + e, n, vec.weight, w);
+      Chunk<float, FAST> w;
+      float y[kE];
+      w.load(p.weight + e, n);
+      w.values(y);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) v[i][j] = v[i][j] * rms * w[j];
+      for (int j = 0; j < kE; ++j) v[i][j] = v[i][j] * rms * y[j];
     } else {
 #pragma unroll
       for (int j = 0; j < kE; ++j) v[i][j] *= rms;
@@ -153,23 +187,28 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(Fp8RowsParams p, 
     for (int off = 8; off; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
     const GroupScale g = group_scale(most);
     if (n > 0) {
-      store_codes(p.codes + row * p.codes_stride + e, n, vec.codes, v[i], g);
+      store_codes<FAST>(p.codes + row * p.codes_stride + e, n, v[i], g);
       if (lane % 16 == 0) p.scales[row * ((p.dim + kFp8Block - 1) / kFp8Block) + e / kFp8Block] = g.scale;
     }
   }
 }
 
-template <class T, int V>
-cudaError_t launch_norm(const Fp8RowsParams& p, int warps, int block_rows, const RowVecs& vec, cudaStream_t st) {
-  return launch(add_rmsnorm_fp8_kernel<T, V>, dim3((unsigned)((p.rows + block_rows - 1) / block_rows)),
-                block_rows * warps * 32, 0, st, p, warps, vec);
+template <class T, int V, int THREADS>
+cudaError_t launch_norm(const Fp8RowsParams& p, bool fast, int warps, int block_rows, cudaStream_t st) {
+  const dim3 blocks((unsigned)((p.rows + block_rows - 1) / block_rows));
+  const int threads = block_rows * warps * 32;
+  if (fast) return launch(add_rmsnorm_fp8_kernel<T, V, THREADS, true>, blocks, threads, 0, st, p, warps);
+  return launch(add_rmsnorm_fp8_kernel<T, V, THREADS, false>, blocks, threads, 0, st, p, warps);
+}
+
+bool even_codes(const Fp8RowsParams& p) {
+  return p.dim % kE == 0 && (reinterpret_cast<uintptr_t>(p.codes) | (uintptr_t)p.codes_stride) % 8 == 0;
 }
 
 template <class T>
 cudaError_t launch_norm(const Fp8RowsParams& p, int sm_count, cudaStream_t st) {
-  RowVecs vec{wide<T>(p.x, p.x_stride), wide<T>(p.residual, p.residual_stride), wide<T>(p.sum, p.sum_stride),
-              wide<float>(p.weight, 0), 0};
-  vec.codes = (reinterpret_cast<uintptr_t>(p.codes) | (uintptr_t)p.codes_stride) % 8 == 0;
+  const bool fast = even<T>(p.x, p.x_stride) && (!p.residual || even<T>(p.residual, p.residual_stride)) &&
+                    (!p.sum || even<T>(p.sum, p.sum_stride)) && even<float>(p.weight, 0) && even_codes(p);
   const int chunks = (p.dim + kE - 1) / kE;
   // Few rows: as many threads as a row has chunks.  Many: four chunks a thread.
   int v = p.rows < 2 * sm_count ? 1 : 4;
@@ -177,9 +216,10 @@ cudaError_t launch_norm(const Fp8RowsParams& p, int sm_count, cudaStream_t st) {
   while ((chunks + v * 32 - 1) / (v * 32) > 32) v *= 2;
   const int warps = (chunks + v * 32 - 1) / (v * 32);
   const int block_rows = p.rows < 2 * sm_count ? 1 : std::max(1, 4 / warps);
-  if (v == 1) return launch_norm<T, 1>(p, warps, block_rows, vec, st);
-  if (v == 2) return launch_norm<T, 2>(p, warps, block_rows, vec, st);
-  return launch_norm<T, 4>(p, warps, block_rows, vec, st);
+  if (v == 1) return launch_norm<T, 1, 1024>(p, fast, warps, block_rows, st);
+  if (v == 2) return launch_norm<T, 2, 1024>(p, fast, warps, block_rows, st);
+  if (warps > 8) return launch_norm<T, 4, 1024>(p, fast, warps, block_rows, st);
+  return launch_norm<T, 4, 256>(p, fast, warps, block_rows, st);
 }
 
 // ---- rows and blocks as they are -----------------------------------------------------------------------
@@ -187,13 +227,12 @@ cudaError_t launch_norm(const Fp8RowsParams& p, int sm_count, cudaStream_t st) {
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;  // groups of a half warp, all loaded before the first is used
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) fp8_quantize_rows_kernel(Fp8RowsParams p, unsigned groups, unsigned total,
-                                                                      int vec, int vec_codes) {
+template <class T, bool FAST>
+__global__ void __launch_bounds__(kThreads) fp8_quantize_rows_kernel(Fp8RowsParams p, unsigned groups, unsigned total) {
   after_previous();
   const unsigned half = (blockIdx.x * kThreads + threadIdx.x) / 16;
   const int lane = threadIdx.x % 16;
-  float v[kUnroll][kE];
+  Chunk<T, FAST> x[kUnroll];
   long long row[kUnroll];
   int at[kUnroll], n[kUnroll];
 #pragma unroll
@@ -202,39 +241,44 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_rows_kernel(Fp8RowsPara
     row[u] = g / groups;
     at[u] = (int)(g % groups) * kFp8Block + lane * kE;
     n[u] = g < total ? p.dim - at[u] : 0;
-    load_chunk(static_cast<const T*>(p.x) + row[u] * p.x_stride + at[u], n[u], vec, v[u]);
+    x[u].load(static_cast<const T*>(p.x) + row[u] * p.x_stride + at[u], n[u]);
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    uint32_t most = largest_bits(v[u]);
+    float v[kE];
+    x[u].values(v);
+    uint32_t most = largest_bits(v);
 #pragma unroll
     for (int off = 8; off; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
     const GroupScale g = group_scale(most);
     if (n[u] > 0) {
-      store_codes(p.codes + row[u] * p.codes_stride + at[u], n[u], vec_codes, v[u], g);
+      store_codes<FAST>(p.codes + row[u] * p.codes_stride + at[u], n[u], v, g);
       if (lane == 0) p.scales[row[u] * groups + at[u] / kFp8Block] = g.scale;
     }
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) fp8_quantize_blocks_kernel(Fp8RowsParams p, unsigned groups, int vec,
-                                                                        int vec_codes) {
+template <class T, bool FAST>
+__global__ void __launch_bounds__(kThreads) fp8_quantize_blocks_kernel(Fp8RowsParams p, unsigned groups) {
   __shared__ uint32_t part[kThreads / 32];
   after_previous();
   constexpr int kRows = kThreads / 16, kTurns = kFp8Block / kRows;
   const long long block = blockIdx.x / groups;
   const int at = (int)(blockIdx.x % groups) * kFp8Block + threadIdx.x % 16 * kE;
-  float v[kTurns][kE];
+  Chunk<T, FAST> x[kTurns];
   uint32_t most = 0;
   const long long row0 = block * kFp8Block + threadIdx.x / 16;
 #pragma unroll
   for (int t = 0; t < kTurns; ++t) {
     const long long row = row0 + t * kRows;
-    load_chunk(static_cast<const T*>(p.x) + row * p.x_stride + at, row < p.rows ? p.dim - at : 0, vec, v[t]);
+    x[t].load(static_cast<const T*>(p.x) + row * p.x_stride + at, row < p.rows ? p.dim - at : 0);
   }
+  float v[kTurns][kE];
 #pragma unroll
-  for (int t = 0; t < kTurns; ++t) most = max(most, largest_bits(v[t]));
+  for (int t = 0; t < kTurns; ++t) {
+    x[t].values(v[t]);
+    most = max(most, largest_bits(v[t]));
+  }
   most = __reduce_max_sync(0xffffffffu, most);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = most;
   __syncthreads();
@@ -244,24 +288,25 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_blocks_kernel(Fp8RowsPa
 #pragma unroll
   for (int t = 0; t < kTurns; ++t) {
     const long long row = row0 + t * kRows;
-    if (row < p.rows) store_codes(p.codes + row * p.codes_stride + at, p.dim - at, vec_codes, v[t], g);
+    if (row < p.rows && at < p.dim) store_codes<FAST>(p.codes + row * p.codes_stride + at, p.dim - at, v[t], g);
   }
   if (threadIdx.x == 0) p.scales[blockIdx.x] = g.scale;
 }
 
 template <class T>
 cudaError_t launch_quantize(const Fp8RowsParams& p, int block_rows, cudaStream_t st) {
-  const int vec = wide<T>(p.x, p.x_stride);
-  const int vec_codes = (reinterpret_cast<uintptr_t>(p.codes) | (uintptr_t)p.codes_stride) % 8 == 0;
+  const bool fast = even<T>(p.x, p.x_stride) && even_codes(p);
   const unsigned groups = (unsigned)((p.dim + kFp8Block - 1) / kFp8Block);
   if (block_rows == 1) {
     const unsigned total = groups * (unsigned)p.rows;
     constexpr unsigned kEach = kThreads / 16 * kUnroll;
-    return launch(fp8_quantize_rows_kernel<T>, dim3((total + kEach - 1) / kEach), kThreads, 0, st, p, groups, total, vec,
-                  vec_codes);
+    const dim3 blocks((total + kEach - 1) / kEach);
+    if (fast) return launch(fp8_quantize_rows_kernel<T, true>, blocks, kThreads, 0, st, p, groups, total);
+    return launch(fp8_quantize_rows_kernel<T, false>, blocks, kThreads, 0, st, p, groups, total);
   }
-  const unsigned blocks = groups * (unsigned)(((long long)p.rows + kFp8Block - 1) / kFp8Block);
-  return launch(fp8_quantize_blocks_kernel<T>, dim3(blocks), kThreads, 0, st, p, groups, vec, vec_codes);
+  const dim3 blocks(groups * (unsigned)(((long long)p.rows + kFp8Block - 1) / kFp8Block));
+  if (fast) return launch(fp8_quantize_blocks_kernel<T, true>, blocks, kThreads, 0, st, p, groups);
+  return launch(fp8_quantize_blocks_kernel<T, false>, blocks, kThreads, 0, st, p, groups);
 }
 
 }  // namespace

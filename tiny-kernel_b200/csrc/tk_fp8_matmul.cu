@@ -130,7 +130,7 @@ __device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
 // of k and add their sums through shared memory, in the order of their ranks; where there are more, a CTA walks over
 // its tiles and its copies go on through their ends.
 
-constexpr int kMaxStages = 8, kMaxSplit = 8;
+constexpr int kMaxSplit = 8;
 
 template <int NT>
 struct Few {
@@ -142,8 +142,10 @@ struct Few {
   static constexpr int kSums = 4;                      // steps in tensor memory
   static constexpr uint32_t kColumns = kSums * kStep * NT;
   static constexpr int kBlockBytes = (128 + NT) * kFp8Block, kStageBytes = kStep * kBlockBytes;
-  static constexpr int kStages = 220 * 1024 / kCtas / kStageBytes, kBytes = kStages * kStageBytes + 1024;
-  static_assert(kStages <= kMaxStages && NT * 512 <= kStages * kStageBytes, "shared memory");
+  // Half of a SM's shared memory, also where there is a CTA for each only: the next launch's are set up beside them
+  // (with all of it, 1 x 4096 x 14336 and 16 x 4096 x 4096 12.8 and 6.3 us instead of 12.4 and 6.0).
+  static constexpr int kStages = 110 * 1024 / kStageBytes, kBytes = kStages * kStageBytes + 1024;
+  static_assert(NT * 512 <= kStages * kStageBytes, "shared memory");
 };
 
 template <int NT>
@@ -383,7 +385,8 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
   attr[1].val.clusterDim.x = (unsigned)plan.split;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(plan.split > 1 ? tiles * plan.split : std::min(tiles, M::kCtas * sm_count)));
+  const int ctas = plan.split > 1 ? tiles * plan.split : std::min(tiles, M::kCtas * sm_count);
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(M::kThreads);
   cfg.dynamicSmemBytes = M::kBytes;
   cfg.stream = st;
@@ -913,8 +916,9 @@ cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, cons
 
 }  // namespace
 
-// Up to 64 rows the weight's rows are the product's, and a tile's k is split while a SM has no CTA (us with 1, 2, 4, 8 parts:
-// 1 x 4096 x 14336 12.4, 13.3, 16.4, 22.5; 1 x 4096 x 4096 9.6, 7.2, 5.7, 6.3; 64 x 14336 x 4096 43, 25, 16, 17).
+// Up to 64 rows the weight's rows are the product's, and a tile's k is split while a SM has no CTA, or, split already and
+// long, has one (us with 1, 2, 4, 8 parts: 1 x 4096 x 14336 12.4, 13.3, 16.4, 22.5; 16 x 4096 x 4096 10.0, 7.6, 6.3, 6.6;
+// 16 x 14336 x 4096 27, 17, 14.3, 13.0; 16 x 2048 x 1024 6.2, 5.5, 4.6, 4.4).
 // Above, what is expected to take least: a block of k takes a tile of 128 x 128 0.4 us, one of 256 x 256 0.48, tiles go
 // round by round over the SMs or their pairs, and a split costs 3 us (128 x 4096 x 4096 15.5, 12.4, 10.0 in tiles of
 // 128, 18.0 of 256; 128 x 4096 x 14336 16.9 and 20.2; 256 x 4096 x 14336 29.7 and 20.7).
@@ -923,7 +927,9 @@ Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count) {
   const long long tiles_n = (n + 127) / 128;
   if (m <= 64) {
     Fp8MatmulPlan plan{m <= 16 ? 16 : m <= 32 ? 32 : 64, 1};
-    while (plan.split < kMaxSplit && tiles_n * plan.split * 2 <= sm_count && plan.split * 8 <= blocks) plan.split *= 2;
+    while (plan.split < kMaxSplit && blocks >= 8 && plan.split * 4 <= blocks &&
+           tiles_n * plan.split * 2 <= (plan.split > 1 && plan.split * 16 <= blocks ? 2 : 1) * sm_count)
+      plan.split *= 2;
     return plan;
   }
   const auto rounds = [](long long tiles, int places) { return (double)((tiles + places - 1) / places); };
