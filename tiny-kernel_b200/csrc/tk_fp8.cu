@@ -9,8 +9,10 @@
 // infinity or a NaN gets the scale NaN: it reads back as NaN, and so does every sum over it.
 //
 // Bound by memory: one pass, every value is read once into registers and stays there between the sum of squares,
-// the groups' maxima and the codes.  A thread has eight consecutive values of a group, so 16 lanes share it.
+// the groups' maxima and the codes.  A thread has 32 bytes of consecutive values of a group, so 16 lanes share it, of 16-bit
+// types 8.
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
 #include "tk_elements.cuh"
@@ -20,7 +22,8 @@
 namespace tk {
 namespace {
 
-constexpr int kE = 8;  // values of a thread's chunk: 16 bytes of 16-bit types, 8 bytes of codes
+template <class T>
+constexpr int kChunk = 32 / sizeof(T);  // values of a thread's chunk
 constexpr float kLargest = 448.f, kLeastScale = 1.17549435e-38f;  // of e4m3; 2^-126
 
 // Whether every row of values lies on a boundary of 16 bytes.
@@ -29,67 +32,90 @@ bool even(const void* base, long long stride) {
   return (reinterpret_cast<uintptr_t>(base) | (uintptr_t)(stride * (long long)sizeof(T))) % 16 == 0;
 }
 
-// A thread's chunk as it lies in memory.  FAST: rows on 16-byte boundaries and of whole chunks, so that a load is 16 or 32
+// A thread's chunk as it lies in memory.  FAST: rows on 16-byte boundaries and of whole chunks, so that loads are of 16
 // bytes; all of a thread's are on their way before the first is looked at (loads that were converted one after the
 // other took bf16 rows longer than f32 ones).  Otherwise by elements.
-template <class T, bool FAST>
+template <class T, int E, bool FAST>
 struct Chunk {
-  uint4 raw[FAST ? sizeof(T) * kE / 16 : 1];
-  T e[FAST ? 1 : kE];
+  static constexpr int kLoads = FAST ? (int)sizeof(T) * E / 16 : 1;
+  uint4 raw[kLoads];
+  T e[FAST ? 1 : E];
   __device__ __forceinline__ void load(const T* src, int n) {
     if constexpr (FAST) {
-      if (n <= 0) {
 #pragma unroll
-        for (int w = 0; w < (int)sizeof(T) * kE / 16; ++w) raw[w] = make_uint4(0, 0, 0, 0);
-      } else if constexpr (sizeof(T) == 4) {
-        raw[0] = reinterpret_cast<const uint4*>(src)[0];
-        raw[1] = reinterpret_cast<const uint4*>(src)[1];
-      } else {
-        raw[0] = *reinterpret_cast<const uint4*>(src);
-      }
+      for (int w = 0; w < kLoads; ++w) raw[w] = n <= 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(src)[w];
     } else {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) e[i] = i < n ? src[i] : from_f32<T>(0.f);
+      for (int i = 0; i < E; ++i) e[i] = i < n ? src[i] : from_f32<T>(0.f);
     }
   }
-  __device__ __forceinline__ void values(float (&v)[kE]) const {
+  __device__ __forceinline__ void values(float (&v)[E]) const {
     if constexpr (!FAST) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) v[i] = to_f32(e[i]);
-    } else if constexpr (sizeof(T) == 4) {
-      const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-#pragma unroll
-      for (int i = 0; i < kE; ++i) v[i] = __uint_as_float(w[i]);
+      for (int i = 0; i < E; ++i) v[i] = to_f32(e[i]);
     } else {
-      const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same<T, __half>::value) {
-          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          v[2 * i] = y.x, v[2 * i + 1] = y.y;
-        } else {
-          v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int l = 0; l < kLoads; ++l) {
+        const uint32_t w[4] = {raw[l].x, raw[l].y, raw[l].z, raw[l].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (sizeof(T) == 4) {
+            v[4 * l + i] = __uint_as_float(w[i]);
+          } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[8 * l + 2 * i] = y.x, v[8 * l + 2 * i + 1] = y.y;
+          } else {
+            v[8 * l + 2 * i] = __uint_as_float(w[i] << 16), v[8 * l + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+          }
         }
       }
     }
   }
 };
-template <class T, bool FAST>
-__device__ __forceinline__ void store_chunk(T* dst, int n, const float (&v)[kE]) {
+template <class T, int E, bool FAST>
+__device__ __forceinline__ void store_chunk(T* dst, int n, const float (&v)[E]) {
   if constexpr (FAST) {
-    store_f32<T, kE>(dst, 1, v);
+    store_f32<T, E>(dst, 1, v);
   } else {
 #pragma unroll
-    for (int i = 0; i < kE; ++i)
+    for (int i = 0; i < E; ++i)
       if (i < n) dst[i] = from_f32<T>(v[i]);
   }
 }
 
 // Largest magnitude as bits: those of infinities and NaNs are above all others'.
-__device__ __forceinline__ uint32_t largest_bits(const float (&v)[kE]) {
+template <int E>
+__device__ __forceinline__ uint32_t largest_bits(const float (&v)[E]) {
   uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < kE; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 0; i < E; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+  return most;
+}
+// The same of a chunk as it lies in memory: of 16-bit types two at once, whose magnitudes are in the order of their bits.
+template <class T, int E, bool FAST>
+__device__ __forceinline__ uint32_t largest_bits(const Chunk<T, E, FAST>& x, const float (&v)[E]) {
+  if constexpr (FAST && sizeof(T) == 2) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int l = 0; l < Chunk<T, E, FAST>::kLoads; ++l) {
+      most = __vmaxu2(most, x.raw[l].x & 0x7fff7fffu);
+      most = __vmaxu2(most, x.raw[l].y & 0x7fff7fffu);
+      most = __vmaxu2(most, x.raw[l].z & 0x7fff7fffu);
+      most = __vmaxu2(most, x.raw[l].w & 0x7fff7fffu);
+    }
+    const uint16_t bits = (uint16_t)max(most & 0xffffu, most >> 16);
+    T y;
+    memcpy(&y, &bits, 2);
+    return __float_as_uint(to_f32(y));
+  } else {
+    return largest_bits(v);
+  }
+}
+// Of the lanes that share a group.
+template <int LANES>
+__device__ __forceinline__ uint32_t of_group(uint32_t most) {
+#pragma unroll
+  for (int off = LANES / 2; off; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
   return most;
 }
 
@@ -98,8 +124,10 @@ struct GroupScale {
 };
 __device__ __forceinline__ GroupScale group_scale(uint32_t most) {
   if (most >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f};
-  const float s = fmaxf(__uint_as_float(most) / kLargest, kLeastScale);
-  return {s, 1.f / s};
+  const float s = fmaxf(__uint_as_float(most) * (1.f / kLargest), kLeastScale);
+  float over;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over) : "f"(s));  // within 2^-23: a code is of 4 bits
+  return {s, over};
 }
 
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
@@ -108,20 +136,23 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return lo | (uint32_t)hi << 16;
 }
-// FAST: dst is on an 8-byte boundary.
-template <bool FAST>
-__device__ __forceinline__ void store_codes(uint8_t* dst, int n, const float (&v)[kE], const GroupScale& g) {
-  uint2 y = make_uint2(0, 0);
-  if (g.over != 0.f) {
-    y.x = codes4(v[0] * g.over, v[1] * g.over, v[2] * g.over, v[3] * g.over);
-    y.y = codes4(v[4] * g.over, v[5] * g.over, v[6] * g.over, v[7] * g.over);
-  }
-  if (FAST) {
-    *reinterpret_cast<uint2*>(dst) = y;
-  } else {
+// FAST: dst is on a boundary of E bytes.
+template <int E, bool FAST>
+__device__ __forceinline__ void store_codes(uint8_t* dst, int n, const float (&v)[E], const GroupScale& g) {
+  uint32_t y[E / 4];
 #pragma unroll
-    for (int i = 0; i < kE; ++i)
-      if (i < n) dst[i] = (uint8_t)((i < 4 ? y.x : y.y) >> (i % 4 * 8));
+  for (int i = 0; i < E / 4; ++i) {
+    y[i] = codes4(v[4 * i] * g.over, v[4 * i + 1] * g.over, v[4 * i + 2] * g.over, v[4 * i + 3] * g.over);
+    if (g.over == 0.f) y[i] = 0;
+  }
+  if constexpr (!FAST) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < n) dst[i] = (uint8_t)(y[i / 4] >> (i % 4 * 8));
+  } else if constexpr (E == 8) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(y[0], y[1]);
+  } else {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(y[0], y[1], y[2], y[3]);
   }
 }
 
@@ -130,13 +161,14 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, int n, const float (&v
 // `warps` warps a row, V chunks a thread; a block has as many rows as its warps make.
 template <class T, int V, int THREADS, bool FAST>
 __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(Fp8RowsParams p, int warps) {
+  constexpr int kE = kChunk<T>, kLanes = kFp8Block / kE;
   __shared__ float part[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = warp / warps * warps;
   const long long row = (long long)blockIdx.x * (blockDim.x / 32 / warps) + warp / warps;
   const bool live = row < p.rows;
   const int at = ((warp - first) * 32 + lane) * kE, step = warps * 32 * kE;
   after_previous();
-  Chunk<T, FAST> x[V], r[V];
+  Chunk<T, kE, FAST> x[V], r[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = at + i * step, n = live ? p.dim - e : 0;
@@ -155,7 +187,7 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(Fp8RowsParams 
 #pragma unroll
       for (int j = 0; j < kE; ++j) v[i][j] += y[j];
     }
-    if (p.sum && n > 0) store_chunk<T, FAST>(static_cast<T*>(p.sum) + row * p.sum_stride + e, n, v[i]);
+    if (p.sum && n > 0) store_chunk<T, kE, FAST>(static_cast<T*>(p.sum) + row * p.sum_stride + e, n, v[i]);
 #pragma unroll
     for (int j = 0; j < kE; ++j) squares = fmaf(v[i][j], v[i][j], squares);
   }
@@ -172,7 +204,7 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(Fp8RowsParams 
   for (int i = 0; i < V; ++i) {
     const int e = at + i * step, n = live ? p.dim - e : 0;
     if (p.weight) {
-      Chunk<float, FAST> w;
+      Chunk<float, kE, FAST> w;
       float y[kE];
       w.load(p.weight + e, n);
       w.values(y);
@@ -182,13 +214,10 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(Fp8RowsParams 
 #pragma unroll
       for (int j = 0; j < kE; ++j) v[i][j] *= rms;
     }
-    uint32_t most = largest_bits(v[i]);
-#pragma unroll
-    for (int off = 8; off; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-    const GroupScale g = group_scale(most);
+    const GroupScale g = group_scale(of_group<kLanes>(largest_bits(v[i])));
     if (n > 0) {
-      store_codes<FAST>(p.codes + row * p.codes_stride + e, n, v[i], g);
-      if (lane % 16 == 0) p.scales[row * ((p.dim + kFp8Block - 1) / kFp8Block) + e / kFp8Block] = g.scale;
+      store_codes<kE, FAST>(p.codes + row * p.codes_stride + e, n, v[i], g);
+      if (lane % kLanes == 0) p.scales[row * ((p.dim + kFp8Block - 1) / kFp8Block) + e / kFp8Block] = g.scale;
     }
   }
 }
@@ -201,83 +230,72 @@ cudaError_t launch_norm(const Fp8RowsParams& p, bool fast, int warps, int block_
   return launch(add_rmsnorm_fp8_kernel<T, V, THREADS, false>, blocks, threads, 0, st, p, warps);
 }
 
+template <class T>
 bool even_codes(const Fp8RowsParams& p) {
-  return p.dim % kE == 0 && (reinterpret_cast<uintptr_t>(p.codes) | (uintptr_t)p.codes_stride) % 8 == 0;
+  return p.dim % kChunk<T> == 0 && (reinterpret_cast<uintptr_t>(p.codes) | (uintptr_t)p.codes_stride) % kChunk<T> == 0;
 }
 
 template <class T>
 cudaError_t launch_norm(const Fp8RowsParams& p, int sm_count, cudaStream_t st) {
   const bool fast = even<T>(p.x, p.x_stride) && (!p.residual || even<T>(p.residual, p.residual_stride)) &&
-                    (!p.sum || even<T>(p.sum, p.sum_stride)) && even<float>(p.weight, 0) && even_codes(p);
-  const int chunks = (p.dim + kE - 1) / kE;
-  // Few rows: as many threads as a row has chunks.  Many: four chunks a thread.
-  int v = p.rows < 2 * sm_count ? 1 : 4;
+                    (!p.sum || even<T>(p.sum, p.sum_stride)) && even<float>(p.weight, 0) && even_codes<T>(p);
+  const int chunks = (p.dim + kChunk<T> - 1) / kChunk<T>;
+  // Few rows: as many threads as a row has chunks.  Many: 128 bytes of f32, 64 of 16-bit types a thread.
+  constexpr int kMost = sizeof(T) == 4 ? 4 : 2;
+  int v = p.rows < 2 * sm_count ? 1 : kMost;
   while (v > 1 && chunks <= 32 * (v / 2)) v /= 2;
   while ((chunks + v * 32 - 1) / (v * 32) > 32) v *= 2;
   const int warps = (chunks + v * 32 - 1) / (v * 32);
   const int block_rows = p.rows < 2 * sm_count ? 1 : std::max(1, 4 / warps);
   if (v == 1) return launch_norm<T, 1, 1024>(p, fast, warps, block_rows, st);
+  if (v == kMost && warps <= 8) return launch_norm<T, kMost, 256>(p, fast, warps, block_rows, st);
   if (v == 2) return launch_norm<T, 2, 1024>(p, fast, warps, block_rows, st);
-  if (warps > 8) return launch_norm<T, 4, 1024>(p, fast, warps, block_rows, st);
-  return launch_norm<T, 4, 256>(p, fast, warps, block_rows, st);
+  return launch_norm<T, kMost, 1024>(p, fast, warps, block_rows, st);
 }
 
 // ---- rows and blocks as they are -----------------------------------------------------------------------
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // groups of a half warp, all loaded before the first is used
 
 template <class T, bool FAST>
 __global__ void __launch_bounds__(kThreads) fp8_quantize_rows_kernel(Fp8RowsParams p, unsigned groups, unsigned total) {
+  constexpr int kE = kChunk<T>, kLanes = kFp8Block / kE;
   after_previous();
-  const unsigned half = (blockIdx.x * kThreads + threadIdx.x) / 16;
-  const int lane = threadIdx.x % 16;
-  Chunk<T, FAST> x[kUnroll];
-  long long row[kUnroll];
-  int at[kUnroll], n[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const unsigned g = half + u * gridDim.x * (kThreads / 16);
-    row[u] = g / groups;
-    at[u] = (int)(g % groups) * kFp8Block + lane * kE;
-    n[u] = g < total ? p.dim - at[u] : 0;
-    x[u].load(static_cast<const T*>(p.x) + row[u] * p.x_stride + at[u], n[u]);
-  }
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    float v[kE];
-    x[u].values(v);
-    uint32_t most = largest_bits(v);
-#pragma unroll
-    for (int off = 8; off; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-    const GroupScale g = group_scale(most);
-    if (n[u] > 0) {
-      store_codes<FAST>(p.codes + row[u] * p.codes_stride + at[u], n[u], v, g);
-      if (lane == 0) p.scales[row[u] * groups + at[u] / kFp8Block] = g.scale;
-    }
-  }
+  // (a thread with two or four groups is slower: 2048 x 14336 bf16 14.7 and 16.4 us instead of 14.3)
+  const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / kLanes;
+  const int lane = threadIdx.x % kLanes, at = (int)(group % groups) * kFp8Block + lane * kE;
+  const long long row = group / groups;
+  const int n = group < total ? p.dim - at : 0;
+  Chunk<T, kE, FAST> x;
+  x.load(static_cast<const T*>(p.x) + row * p.x_stride + at, n);
+  float v[kE];
+  x.values(v);
+  const GroupScale g = group_scale(of_group<kLanes>(largest_bits(x, v)));
+  if (n <= 0) return;
+  store_codes<kE, FAST>(p.codes + row * p.codes_stride + at, n, v, g);
+  if (lane == 0) p.scales[group] = g.scale;
 }
 
 template <class T, bool FAST>
 __global__ void __launch_bounds__(kThreads) fp8_quantize_blocks_kernel(Fp8RowsParams p, unsigned groups) {
+  constexpr int kE = kChunk<T>, kLanes = kFp8Block / kE, kRows = kThreads / kLanes, kTurns = kFp8Block / kRows;
   __shared__ uint32_t part[kThreads / 32];
   after_previous();
-  constexpr int kRows = kThreads / 16, kTurns = kFp8Block / kRows;
   const long long block = blockIdx.x / groups;
-  const int at = (int)(blockIdx.x % groups) * kFp8Block + threadIdx.x % 16 * kE;
-  Chunk<T, FAST> x[kTurns];
+  const int at = (int)(blockIdx.x % groups) * kFp8Block + threadIdx.x % kLanes * kE;
+  Chunk<T, kE, FAST> x[kTurns];
   uint32_t most = 0;
-  const long long row0 = block * kFp8Block + threadIdx.x / 16;
+  const long long row0 = block * kFp8Block + threadIdx.x / kLanes;
 #pragma unroll
   for (int t = 0; t < kTurns; ++t) {
     const long long row = row0 + t * kRows;
     x[t].load(static_cast<const T*>(p.x) + row * p.x_stride + at, row < p.rows ? p.dim - at : 0);
   }
-  float v[kTurns][kE];
+  float v[kE];
 #pragma unroll
   for (int t = 0; t < kTurns; ++t) {
-    x[t].values(v[t]);
-    most = max(most, largest_bits(v[t]));
+    x[t].values(v);
+    most = max(most, largest_bits(x[t], v));
   }
   most = __reduce_max_sync(0xffffffffu, most);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = most;
@@ -288,18 +306,21 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_blocks_kernel(Fp8RowsPa
 #pragma unroll
   for (int t = 0; t < kTurns; ++t) {
     const long long row = row0 + t * kRows;
-    if (row < p.rows && at < p.dim) store_codes<FAST>(p.codes + row * p.codes_stride + at, p.dim - at, v[t], g);
+    if (row < p.rows && at < p.dim) {
+      x[t].values(v);
+      store_codes<kE, FAST>(p.codes + row * p.codes_stride + at, p.dim - at, v, g);
+    }
   }
   if (threadIdx.x == 0) p.scales[blockIdx.x] = g.scale;
 }
 
 template <class T>
 cudaError_t launch_quantize(const Fp8RowsParams& p, int block_rows, cudaStream_t st) {
-  const bool fast = even<T>(p.x, p.x_stride) && even_codes(p);
+  const bool fast = even<T>(p.x, p.x_stride) && even_codes<T>(p);
   const unsigned groups = (unsigned)((p.dim + kFp8Block - 1) / kFp8Block);
   if (block_rows == 1) {
     const unsigned total = groups * (unsigned)p.rows;
-    constexpr unsigned kEach = kThreads / 16 * kUnroll;
+    constexpr unsigned kEach = kThreads * kChunk<T> / kFp8Block;
     const dim3 blocks((total + kEach - 1) / kEach);
     if (fast) return launch(fp8_quantize_rows_kernel<T, true>, blocks, kThreads, 0, st, p, groups, total);
     return launch(fp8_quantize_rows_kernel<T, false>, blocks, kThreads, 0, st, p, groups, total);
