@@ -37,13 +37,14 @@ struct Fp8MatmulParams {
   unsigned* err;  // the device's error word, and how long a wait of a kernel may take
   unsigned long long timeout_ns;
 };
-// How a call's work is cut: rows of a that a tile takes, CTAs of a cluster that share a tile's k.
+// How a call's work is cut: rows of a and of w that a tile takes, CTAs of a cluster that share a tile's k; and the
+// boxes of 128 bytes x box_a, box_w rows, 128-byte swizzle, that a_map and w_map, of codes [rows][k], are made of.
 struct Fp8MatmulPlan {
-  int tile, split;
+  int rows, cols, split;
+  int box_a() const { return rows < 128 ? rows : 128; }
+  int box_w() const { return rows == 128 ? cols : 128; }
 };
 Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count);
-// a_map, w_map: of codes [rows][k], boxes of 128 bytes x fp8_box_rows() rows, 128-byte swizzle.
-void fp8_box_rows(const Fp8MatmulPlan& plan, int* a_rows, int* w_rows);
 cudaError_t launch_fp8_matmul(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
                               const CUtensorMap& w_map, int sm_count, cudaStream_t st);
 

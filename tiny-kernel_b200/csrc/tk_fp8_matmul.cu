@@ -446,22 +446,33 @@ __device__ __forceinline__ void store_rows(const Fp8MatmulParams& p, int row, in
 
 // ---- some rows -----------------------------------------------------------------------------------------
 //
-// Tiles of 128 rows by 128 of the weight's: a thread adds half of a row, whose scale is one number a block (in the form
-// for few rows it is one for each column, read from shared memory for each product).  Four accumulators.  CTAs of a
-// cluster share a tile's k, or walk over tiles, as above.
+// Tiles of 128 rows by 128 or 256 of the weight's: a thread adds half of a row, whose scale is one number a block (in the
+// form for few rows it is one for each column, read from shared memory for each product).  Accumulators fill tensor
+// memory.  CTAs of a cluster share a tile's k (of 128 columns), or walk over tiles, as above.
 
-constexpr int kSomeThreads = 320;  // a warp of copies, one of products, eight of sums
-constexpr int kSomeStages = 6, kSomeStageBytes = 2 * 128 * kFp8Block, kSomeSums = 4;
+// The registers of a launch of three warpgroups, 168 for each thread, are handed from the first group, of copies and
+// products, to the two of sums, where a thread holds 128 of them: 40 and 2 x 232 of 3 x 168.
+constexpr int kEvenRegs = 168, kFewRegs = 40, kMoreRegs = 232;
+static_assert(kFewRegs + 2 * kMoreRegs <= 3 * kEvenRegs, "the groups' shares");
+
+template <int COLS>
+struct Some {
+  static constexpr int kFirst = COLS == 256 ? 4 : 2;     // warps before those of sums: of copies, of products
+  static constexpr int kThreads = kFirst * 32 + 256, kHalf = COLS / 2, kSums = 512 / COLS;
+  static constexpr int kStageBytes = (128 + COLS) * kFp8Block, kStages = 192 * 1024 / kStageBytes;
+  static constexpr int kBytes = kStages * kStageBytes + 8 * kPatch + 1024;
+};
 constexpr int kSomePitch = 132;  // floats of a row of the exchange
-static_assert(128 * kSomePitch * 4 <= kSomeStages * kSomeStageBytes, "shared memory");
+static_assert(128 * kSomePitch * 4 <= Some<128>::kStages * Some<128>::kStageBytes, "shared memory");
 
-template <class T>
-__global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_constant__ CUtensorMap a_map,
-                                                                   const __grid_constant__ CUtensorMap w_map,
-                                                                   Fp8MatmulParams p, int split, int tiles_m, int tiles_n,
-                                                                   int wide) {
+template <class T, int COLS>
+__global__ void __launch_bounds__(Some<COLS>::kThreads, 1) fp8_some_kernel(const __grid_constant__ CUtensorMap a_map,
+                                                                           const __grid_constant__ CUtensorMap w_map,
+                                                                           Fp8MatmulParams p, int split, int tiles_m,
+                                                                           int tiles_n, int wide) {
+  using M = Some<COLS>;
   extern __shared__ uint8_t dynamic[];
-  __shared__ uint64_t full[kSomeStages], empty[kSomeStages], sums_full[kSomeSums], sums_empty[kSomeSums], drained;
+  __shared__ uint64_t full[M::kStages], empty[M::kStages], sums_full[M::kSums], sums_empty[M::kSums], drained;
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* smem = dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
@@ -469,21 +480,22 @@ __global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_
   const int blocks = (p.k + kFp8Block - 1) / kFp8Block;
   const int b0 = (int)((long long)blocks * rank / split), b1 = (int)((long long)blocks * (rank + 1) / split);
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSomeStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-    for (int s = 0; s < kSomeSums; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 8);
+    for (int s = 0; s < M::kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    for (int s = 0; s < M::kSums; ++s) mbar_init(&sums_full[s], 1), mbar_init(&sums_empty[s], 8);
     mbar_init(&drained, 1);
     fence_mbar_init();
   }
   after_previous();
-  if (warp == 1) tmem_alloc(&tmem_slot, kSomeSums * 128);
+  if (warp == 1) tmem_alloc(&tmem_slot, 512);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = tmem_slot;
   bool dead = false;
   int issued = 0;
-  unsigned long long acc[32];
-  const int quarter = warp & 3, half = (warp - 2) >> 2;
+  unsigned long long acc[M::kHalf / 2];
+  const int quarter = warp & 3, half = (warp - M::kFirst) >> 2;
+  if (COLS == 256 && warp < M::kFirst) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
   if (warp == 0) {
     const uint64_t once = tiles_m == 1 ? l2_evict_first() : l2_evict_last(), often = l2_evict_last();
     int stage = 0;
@@ -495,26 +507,26 @@ __global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_
         __syncwarp();
         if (dead) break;
         if (elect_one()) {
-          uint8_t* to = smem + stage * kSomeStageBytes;
-          mbar_arrive_expect_tx(&full[stage], kSomeStageBytes);
+          uint8_t* to = smem + stage * M::kStageBytes;
+          mbar_arrive_expect_tx(&full[stage], M::kStageBytes);
           tma_load_2d(to, &a_map, &full[stage], b * kFp8Block, tile.m * 128, often);
-          tma_load_2d(to + 128 * kFp8Block, &w_map, &full[stage], b * kFp8Block, tile.n * 128, once);
+          tma_load_2d(to + 128 * kFp8Block, &w_map, &full[stage], b * kFp8Block, tile.n * COLS, once);
         }
         __syncwarp();
         ++issued;
-        if (++stage == kSomeStages) stage = 0, phase ^= 1;
+        if (++stage == M::kStages) stage = 0, phase ^= 1;
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc = umma_idesc_f16(128, 128);
+    constexpr uint32_t idesc = umma_idesc_f16(128, COLS);
     const uint64_t a0 = umma_smem_desc(smem_addr(smem), 16, 1024, 2);
     const uint64_t w0 = umma_smem_desc(smem_addr(smem) + 128 * kFp8Block, 16, 1024, 2);
     int stage = 0, d = 0;
     uint32_t phase = 0, sums_phase = 1;
     for (int t = first; t < tiles && !dead; t += stride)
       for (int b = b0; b < b1; ++b) {
-        const uint64_t a = a0 + stage * (kSomeStageBytes >> 4), w = w0 + stage * (kSomeStageBytes >> 4);
-        const uint32_t to = tmem + d * 128;
+        const uint64_t a = a0 + stage * (M::kStageBytes >> 4), w = w0 + stage * (M::kStageBytes >> 4);
+        const uint32_t to = tmem + d * COLS;
         wait_phase(&full[stage], phase, dead, p);
         wait_phase(&sums_empty[d], sums_phase, dead, p);
         __syncwarp();
@@ -527,47 +539,53 @@ __global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_
           umma_commit(&empty[stage]);
         }
         __syncwarp();
-        if (++stage == kSomeStages) stage = 0, phase ^= 1;
-        if (++d == kSomeSums) d = 0, sums_phase ^= 1;
+        if (++stage == M::kStages) stage = 0, phase ^= 1;
+        if (++d == M::kSums) d = 0, sums_phase ^= 1;
       }
-  } else {
-    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * 64;
-    float* patch = reinterpret_cast<float*>(smem + kSomeStages * kSomeStageBytes + (warp - 2) * kPatch);
+  } else if (warp >= M::kFirst) {
+    if (COLS == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMoreRegs));
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * M::kHalf;
+    float* patch = reinterpret_cast<float*>(smem + M::kStages * M::kStageBytes + (warp - M::kFirst) * kPatch);
     int d = 0;
     uint32_t phase = 0;
     for (int t = first; t < tiles && !dead; t += stride) {
       const Tile tile = tile_of(t, tiles_m, tiles_n);
-      const int row = tile.m * 128 + quarter * 32 + lane, col = tile.n * 128 + half * 64;
+      const int row = tile.m * 128 + quarter * 32 + lane, col = tile.n * COLS + half * M::kHalf;
       const float* a_scale = p.a_scales + (long long)min(row, p.m - 1) * blocks;
-      const float* w_scale = p.w_scales + (long long)tile.n * blocks;
+      const float* w_scale = p.w_scales + (long long)min(col / kFp8Block, (p.n - 1) / kFp8Block) * blocks;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) acc[j] = 0;
+      for (int j = 0; j < M::kHalf / 2; ++j) acc[j] = 0;
       // (multiplied when they are needed: not waited for before that)
       float next_a = a_scale[b0], next_w = w_scale[b0];
       for (int b = b0; b < b1; ++b) {
         const float scale = next_a * next_w;
         const unsigned long long f = pair_of(scale, scale);
         if (b + 1 < b1) next_a = a_scale[b + 1], next_w = w_scale[b + 1];
-        const uint32_t at = from + d * 128;
+        const uint32_t at = from + d * COLS;
         wait_phase(&sums_full[d], phase, dead, p);
         __syncwarp();
         if (dead) break;
         tcgen05_fence_after();
-        uint32_t v[64];
 #pragma unroll
-        for (int c = 0; c < 64; c += 16) tmem_ld16(at + c, v + c);
-        tmem_ld_wait();
-        tcgen05_fence_before();  // all read: the accumulator is free, whatever is still to be added
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sums_empty[d]);
+        for (int c = 0; c < M::kHalf; c += 64) {
+          uint32_t v[64];
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          acc[j] = fma2(pair_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), f, acc[j]);
-        if (++d == kSomeSums) d = 0, phase ^= 1;
+          for (int x = 0; x < 64; x += 16) tmem_ld16(at + c + x, v + x);
+          tmem_ld_wait();
+          if (c + 64 == M::kHalf) {  // all read: the accumulator is free, whatever is still to be added
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sums_empty[d]);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            acc[c / 2 + j] = fma2(pair_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), f, acc[c / 2 + j]);
+        }
+        if (++d == M::kSums) d = 0, phase ^= 1;
       }
       if (split > 1 || dead) break;  // one tile a cluster
 #pragma unroll
-      for (int c = 0; c < 64; c += 32) {
+      for (int c = 0; c < M::kHalf; c += 32) {
         float v[32];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -582,8 +600,8 @@ __global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_
   if (__syncthreads_or(dead)) {
     bool late = false;
     if (warp == 0)
-      for (int s = max(0, issued - kSomeStages); s < issued; ++s)
-        wait_phase(&full[s % kSomeStages], (s / kSomeStages) & 1, late, p);
+      for (int s = max(0, issued - M::kStages); s < issued; ++s)
+        wait_phase(&full[s % M::kStages], (s / M::kStages) & 1, late, p);
     if (warp == 1) {
       if (elect_one()) umma_commit(&drained);
       __syncwarp();
@@ -592,10 +610,10 @@ __global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_
     dead = true;
     __syncthreads();
   }
-  if (split > 1) {
+  if (COLS == 128 && split > 1) {
     const Tile tile = tile_of(first, tiles_m, tiles_n);
     float* sums = reinterpret_cast<float*>(smem);  // [128][pitch]
-    if (warp >= 2) {
+    if (warp >= M::kFirst) {
       float* mine = sums + (quarter * 32 + lane) * kSomePitch + half * 64;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -606,7 +624,7 @@ __global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_
     cluster_sync();
     // the rows over the CTAs, four columns a thread, all CTAs' values at once
     const int rows = min(128, p.m - tile.m * 128), r0 = rows * rank / split, r1 = rows * (rank + 1) / split;
-    for (int i = threadIdx.x; !dead && i < (r1 - r0) * 32; i += kSomeThreads) {
+    for (int i = threadIdx.x; !dead && i < (r1 - r0) * 32; i += M::kThreads) {
       const int r = r0 + i / 32, n = tile.n * 128 + i % 32 * 4;
       if (n >= p.n) continue;
       const uint32_t from = smem_addr(sums + r * kSomePitch + i % 32 * 4);
@@ -625,25 +643,35 @@ __global__ void __launch_bounds__(kSomeThreads, 1) fp8_some_kernel(const __grid_
   }
   if (warp == 1) {
     tcgen05_fence_after();
-    tmem_dealloc(tmem, kSomeSums * 128);
+    tmem_dealloc(tmem, 512);
   }
 }
 
-template <class T>
+// A launch whose groups share out other registers than the kernel has would wait for them for good.
+template <class K>
+cudaError_t has_even_regs(K kernel) {
+  cudaFuncAttributes has{};
+  const cudaError_t e = cudaFuncGetAttributes(&has, kernel);
+  return e != cudaSuccess ? e : has.numRegs < kEvenRegs ? cudaErrorInvalidKernelImage : cudaSuccess;
+}
+
+template <class T, int COLS>
 cudaError_t launch_some(const Fp8MatmulParams& p, int split, const CUtensorMap& a_map, const CUtensorMap& w_map,
                         int sm_count, cudaStream_t st) {
-  constexpr int kMaxDevices = 64, smem = kSomeStages * kSomeStageBytes + 8 * kPatch + 1024;
+  using M = Some<COLS>;
+  constexpr int kMaxDevices = 64;
   static std::atomic<unsigned> asked[kMaxDevices];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned gen = attr_generation(dev) + 1;
   if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
-    e = cudaFuncSetAttribute(fp8_some_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (COLS == 256 && (e = has_even_regs(fp8_some_kernel<T, COLS>)) != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(fp8_some_kernel<T, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kBytes);
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
   }
-  const int tiles_m = (p.m + 127) / 128, tiles_n = (p.n + 127) / 128, tiles = tiles_m * tiles_n;
+  const int tiles_m = (p.m + 127) / 128, tiles_n = (p.n + COLS - 1) / COLS, tiles = tiles_m * tiles_n;
   const int wide = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_stride * (long long)sizeof(T))) % 32 == 0;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -653,12 +681,12 @@ cudaError_t launch_some(const Fp8MatmulParams& p, int split, const CUtensorMap& 
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : std::min(tiles, sm_count)));
-  cfg.blockDim = dim3(kSomeThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(M::kThreads);
+  cfg.dynamicSmemBytes = M::kBytes;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, fp8_some_kernel<T>, a_map, w_map, p, split, tiles_m, tiles_n, wide);
+  return cudaLaunchKernelEx(&cfg, fp8_some_kernel<T, COLS>, a_map, w_map, p, split, tiles_m, tiles_n, wide);
 }
 
 // ---- many rows -----------------------------------------------------------------------------------------
@@ -670,10 +698,7 @@ cudaError_t launch_some(const Fp8MatmulParams& p, int split, const CUtensorMap& 
 // sum += scale * product.  Two accumulators of 256 columns fill tensor memory: one is added up while the other's
 // products run.  Pairs of CTAs walk over the tiles.
 
-// A warpgroup with a warp of copies and two of products, two warpgroups of sums.  A thread of the sums holds 128 of them: the
-// registers of the launch, 168 for each thread, are handed from the first group to the others, 40 and 2 x 232 of 3 x 168.
-constexpr int kManyThreads = 384, kManyRegs = 168, kManyFewRegs = 40, kManyMoreRegs = 232;
-static_assert(kManyFewRegs + 2 * kManyMoreRegs <= 3 * kManyRegs, "the groups' shares");
+constexpr int kManyThreads = 384;  // a warpgroup with a warp of copies and two of products, two warpgroups of sums
 constexpr int kManyRows = 256, kManyCols = 256, kManyStages = 6, kManyStageBytes = 2 * 128 * kFp8Block;  // a CTA's part
 
 // The products of a pair, issued by its first CTA.
@@ -744,7 +769,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
   const uint32_t tmem = tmem_slot;
   bool dead = false;
   int issued = 0;
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyFewRegs));
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
   if (warp == 0) {
     const uint64_t often = l2_evict_last();
     int stage = 0;
@@ -801,7 +826,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
         d ^= 1;
       }
   } else if (warp >= 4) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyMoreRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMoreRegs));
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
     float* patch = reinterpret_cast<float*>(smem + kManyStages * kManyStageBytes + (warp - 4) * kPatch);
@@ -889,9 +914,7 @@ cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, cons
   if (e != cudaSuccess) return e;
   const unsigned gen = attr_generation(dev) + 1;
   if (dev >= kMaxDevices || asked[dev].load(std::memory_order_acquire) != gen) {
-    cudaFuncAttributes has{};
-    if ((e = cudaFuncGetAttributes(&has, fp8_many_kernel<T>)) != cudaSuccess) return e;
-    if (has.numRegs < kManyRegs) return cudaErrorInvalidKernelImage;  // the sums would wait for registers for good
+    if ((e = has_even_regs(fp8_many_kernel<T>)) != cudaSuccess) return e;
     e = cudaFuncSetAttribute(fp8_many_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
@@ -914,6 +937,14 @@ cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, cons
   return cudaLaunchKernelEx(&cfg, fp8_many_kernel<T>, a_map, w_map, p, tiles_m, tiles_n, wide);
 }
 
+template <class T>
+cudaError_t launch_rows(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
+                        const CUtensorMap& w_map, int sm_count, cudaStream_t st) {
+  if (plan.rows == kManyRows) return launch_many<T>(p, a_map, w_map, sm_count, st);
+  if (plan.cols == 256) return launch_some<T, 256>(p, 1, a_map, w_map, sm_count, st);
+  return launch_some<T, 128>(p, plan.split, a_map, w_map, sm_count, st);
+}
+
 }  // namespace
 
 // Up to 64 rows the weight's rows are the product's, and a tile's k is split while a SM has no CTA, or, split already and
@@ -926,44 +957,37 @@ Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count) {
   const int blocks = (k + kFp8Block - 1) / kFp8Block;
   const long long tiles_n = (n + 127) / 128;
   if (m <= 64) {
-    Fp8MatmulPlan plan{m <= 16 ? 16 : m <= 32 ? 32 : 64, 1};
+    Fp8MatmulPlan plan{m <= 16 ? 16 : m <= 32 ? 32 : 64, 128, 1};
     while (plan.split < kMaxSplit && blocks >= 8 && plan.split * 4 <= blocks &&
            tiles_n * plan.split * 2 <= (plan.split > 1 && plan.split * 16 <= blocks ? 2 : 1) * sm_count)
       plan.split *= 2;
     return plan;
   }
-  const auto rounds = [](long long tiles, int places) { return (double)((tiles + places - 1) / places); };
-  Fp8MatmulPlan best{kManyCols, 1};
-  double least = 4.5 + rounds((long long)((m + 255) / 256) * ((n + 255) / 256), sm_count / 2) * blocks * 0.48;
-  for (int split = 1; split <= kMaxSplit / 2 && (split == 1 || split * 4 <= blocks); split *= 2) {
-    const long long tiles = (m + 127) / 128 * tiles_n;
-    if (split > 1 && tiles * split > sm_count) break;
-    const double us = 3.0 + rounds(tiles * split, sm_count) * ((blocks + split - 1) / split) * 0.4 + (split > 1 ? 3.0 : 0.0);
-    if (us < least) least = us, best = {128, split};
-  }
+  Fp8MatmulPlan best{};
+  double least = 0.0;
+  const auto consider = [&](int rows, int cols, int split, int places, double fixed, double block) {
+    const long long tiles = (long long)((m + rows - 1) / rows) * ((n + cols - 1) / cols) * split;
+    const double us = fixed + (double)((tiles + places - 1) / places) * ((blocks + split - 1) / split) * block;
+    if (best.rows == 0 || us < least) least = us, best = {rows, cols, split};
+  };
+  consider(kManyRows, kManyCols, 1, sm_count / 2, 4.5, 0.48);
+  consider(128, 256, 1, sm_count, 3.5, 0.5);
+  consider(128, 128, 1, sm_count, 3.0, 0.4);
+  for (int split = 2; split <= kMaxSplit / 2 && split * 4 <= blocks; split *= 2)
+    if ((m + 127) / 128 * tiles_n * split <= sm_count) consider(128, 128, split, sm_count, 6.0, 0.4);
   return best;
-}
-
-void fp8_box_rows(const Fp8MatmulPlan& plan, int* a_rows, int* w_rows) {
-  *a_rows = std::min(plan.tile, 128);
-  *w_rows = 128;
 }
 
 cudaError_t launch_fp8_matmul(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
                               const CUtensorMap& w_map, int sm_count, cudaStream_t st) {
-  if (plan.tile == kManyCols) {
-    if (p.dtype == kTypeF32) return launch_many<float>(p, a_map, w_map, sm_count, st);
-    return p.dtype == kTypeBF16 ? launch_many<__nv_bfloat16>(p, a_map, w_map, sm_count, st)
-                                : launch_many<__half>(p, a_map, w_map, sm_count, st);
+  if (plan.rows < 128) {
+    if (plan.rows == 16) return launch_few<16>(p, plan, a_map, w_map, sm_count, st);
+    if (plan.rows == 32) return launch_few<32>(p, plan, a_map, w_map, sm_count, st);
+    return launch_few<64>(p, plan, a_map, w_map, sm_count, st);
   }
-  if (plan.tile == 128) {
-    if (p.dtype == kTypeF32) return launch_some<float>(p, plan.split, a_map, w_map, sm_count, st);
-    return p.dtype == kTypeBF16 ? launch_some<__nv_bfloat16>(p, plan.split, a_map, w_map, sm_count, st)
-                                : launch_some<__half>(p, plan.split, a_map, w_map, sm_count, st);
-  }
-  if (plan.tile == 16) return launch_few<16>(p, plan, a_map, w_map, sm_count, st);
-  if (plan.tile == 32) return launch_few<32>(p, plan, a_map, w_map, sm_count, st);
-  return launch_few<64>(p, plan, a_map, w_map, sm_count, st);
+  if (p.dtype == kTypeF32) return launch_rows<float>(p, plan, a_map, w_map, sm_count, st);
+  return p.dtype == kTypeBF16 ? launch_rows<__nv_bfloat16>(p, plan, a_map, w_map, sm_count, st)
+                              : launch_rows<__half>(p, plan, a_map, w_map, sm_count, st);
 }
 
 }  // namespace tk

@@ -1739,11 +1739,9 @@ int tk_fp8_matmul_async(tk_device* d, const uint8_t* a, const float* a_scales, c
   p.err = d->err;
   p.timeout_ns = d->timeout_ns;
   const Fp8MatmulPlan plan = fp8_matmul_plan((int)m, (int)k, (int)n, d->sm_count);
-  int a_rows = 0, w_rows = 0;
-  fp8_box_rows(plan, &a_rows, &w_rows);
   CUtensorMap a_map, w_map;
-  if ((st = codes_tmap(a, k, m, (uint64_t)as, a_rows, &a_map)) != TK_OK) return st;
-  if ((st = codes_tmap(w, k, n, (uint64_t)ws, w_rows, &w_map)) != TK_OK) return st;
+  if ((st = codes_tmap(a, k, m, (uint64_t)as, plan.box_a(), &a_map)) != TK_OK) return st;
+  if ((st = codes_tmap(w, k, n, (uint64_t)ws, plan.box_w(), &w_map)) != TK_OK) return st;
   TK_LAUNCH(d, launch_fp8_matmul(p, plan, a_map, w_map, d->sm_count, pick_stream(d, stream)));
   return TK_OK;
 }

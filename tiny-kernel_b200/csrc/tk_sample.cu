@@ -29,7 +29,7 @@ namespace tk {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8, kMaxWarps = kMaxCluster * kWarps;
-constexpr int kBins = 2048, kList = 1024, kFew = 400;
+constexpr int kBins = 2048, kList = 1024, kPer = kList / kThreads, kFew = 400, kReach = 192;
 constexpr int kParts = 512, kPerBin = 8;  // of an octave of weights: in the table, and of these in a bin
 constexpr float kNone = -INFINITY, kHuge = 3.4028235e38f;
 constexpr double kUnit = 17592186044416.0;  // 2^44: weights as integers, whose sums fit 64 bits
@@ -84,14 +84,16 @@ struct Ranked {
 struct Shared {
   double table[kParts];  // 2^(i / kParts)
   // of all CTAs' warps, written by each into every CTA's
-  double all_sum[kMaxWarps];
+  double all_sum[kMaxWarps], all_head[kMaxWarps];
   float all_most[kMaxWarps], all_level[kMaxWarps];
-  int all_valid[kMaxWarps], all_equal[kMaxWarps], all_count[kMaxWarps];
+  int all_equal[kMaxWarps], all_count[kMaxWarps];
   int all_listed[kMaxCluster];
   uint32_t cut_key;
   int cut_index;
   // own
   int listed, first_equal;
+  unsigned long long extra[kWarps];
+  int extra_count[kWarps];
   float level[kMaxWarps / 32];
   double scan[kWarps];
   unsigned long long scan_mass[kWarps];
@@ -183,7 +185,7 @@ constexpr int kHead = (sizeof(Shared) + (RANKS ? sizeof(Ranked) : 0) + 15) / 16 
 
 // RANKS: some row may have top-k or top-p.
 template <class T, bool RANKS>
-__global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(SampleParams p, int cluster, int slice) {
+__global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams p, int cluster, int slice) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   Shared& sh = *reinterpret_cast<Shared*>(dynamic);
   Ranked& rs = *reinterpret_cast<Ranked*>(dynamic + sizeof(Shared));
@@ -193,8 +195,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   const int rank = blockIdx.x % cluster, warps = cluster * kWarps;
   const long long row = blockIdx.x / cluster;
   const int first = rank * slice, n = max(0, min(slice, p.vocab - first));
-  sh.table[tid] = exp2((double)tid / kParts);
-  static_assert(kThreads == kParts, "");
+  for (int i = tid; i < kParts; i += kThreads) sh.table[i] = exp2((double)i / kParts);
   if (tid == 0) sh.listed = 0, sh.first_equal = 0x7fffffff;
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   after_previous();
@@ -206,13 +207,8 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   const float min_p = greedy || !p.min_p ? 0.f : p.min_p[row];
   const float u = p.random[row];
 
-  // The row into shared memory: NaN as -inf, -0 as 0; its largest, and how many there are.
+  // The row into shared memory: NaN as -inf, -0 as 0; its largest.
   float most = kNone;
-  int valid = 0;
-  auto take = [&](float v) {
-    most = fmaxf(most, v);
-    valid += v > kNone;
-  };
   auto clean = [](float v) { return fmaxf(v + 0.f, kNone); };
   int begin = 0;
   if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
@@ -233,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
           const float v = clean(to_f32(e[j]));
-          take(v);
+          most = fmaxf(most, v);
           e[j] = from_f32<T>(v);
         }
         reinterpret_cast<uint4*>(mine)[i] = raw[f];
@@ -243,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   }
   for (int i = begin + tid; i < n; i += kThreads) {
     const float v = clean(to_f32(src[i]));
-    take(v);
+    most = fmaxf(most, v);
     mine[i] = from_f32<T>(v);
   }
   // what lies behind, up to a whole vector
@@ -252,31 +248,25 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
 
   __syncwarp();
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all CTAs run: they may be written to
-  // For few top-k: each warp's each-th largest of its threads', which half of the warps reach at the least.
-  const bool few = k > 0 && k <= min(kFew, kWarps / 2 * 32 * cluster);
-  const int each = few ? (k + warps / 2 - 1) / (warps / 2) : 0;
-  if (RANKS && few) {
+  // For a list of the row's largest: each warp's each-th largest of its threads', which half of the warps reach at the
+  // least.  Few top-k, or, of top-p alone, as many as mostly do.
+  const bool by_k = k > 0 && k < p.vocab, by_p = top_p < 1.f;
+  const int reach = by_k ? k : by_p ? kReach : 0;
+  const bool quick = RANKS && reach > 0 && reach <= min(kFew, kWarps / 2 * 32 * cluster);
+  const int each = (reach + warps / 2 - 1) / (warps / 2);
+  if (quick) {
     const float s = sort_warp<true>(most);
     if (lane == each - 1)
       for (int r = 0; r < cluster; ++r) *of_rank(&sh.all_level[rank * kWarps + warp], r) = s;
   }
 #pragma unroll
   for (int off = 16; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-  valid = __reduce_add_sync(0xffffffffu, valid);
-  if (lane < cluster) {
-    *of_rank(&sh.all_most[rank * kWarps + warp], lane) = most;
-    *of_rank(&sh.all_valid[rank * kWarps + warp], lane) = valid;
-  }
+  if (lane < cluster) *of_rank(&sh.all_most[rank * kWarps + warp], lane) = most;
   cluster_sync();
   most = kNone;
-  valid = 0;
-  for (int i = lane; i < warps; i += 32) {
-    most = fmaxf(most, sh.all_most[i]);
-    valid += sh.all_valid[i];
-  }
+  for (int i = lane; i < warps; i += 32) most = fmaxf(most, sh.all_most[i]);
 #pragma unroll
   for (int off = 16; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-  valid = __reduce_add_sync(0xffffffffu, valid);
   if (most == kNone) {
     if (rank == 0 && tid == 0) {
       p.tokens[row] = -1;
@@ -294,6 +284,15 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
       for (int j = 0; j < kVec; ++j) l[j] = to_f32(e[j]);
       f(i * kVec, l);
     }
+  };
+  auto for_fours = [&](int from, int to, int start, int step, auto f) {
+    for_vectors(from, to, start, step, [&](int i, const float(&l)[kVec]) {
+#pragma unroll
+      for (int j = 0; j < kVec; j += 4) {
+        const float four[4] = {l[j], l[j + 1], l[j + 2], l[j + 3]};
+        f(i + j, four);
+      }
+    });
   };
   auto for_all = [&](int from, int to, int start, int step, auto f) {
     for_vectors(from, to, start, step, [&](int i, const float(&l)[kVec]) {
@@ -319,12 +318,11 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   }
 
   const bool endless = most == INFINITY;
-  const double slope = kParts * 1.4426950408889634 / (double)heat;  // 512 log2 e / T
-  // 512 log2 of a weight, and the weight: 2^(y/512) = 2^a 2^(b/512) e^z with whole a and b and |z| <= ln 2 / 1024, for
-  // which 1 + z + z^2/2 + z^3/6 is within 9e-15.
-  // Where the largest is infinite only its equals are there, taken as the largest f32.
-  const float ref = endless ? kHuge : most;
-  auto level_of = [&](float l) -> double { return ((double)fminf(l, ref) - (double)ref) * slope; };
+  // 512 log2 of a weight, from the exact difference.  Where the largest is infinite only its equals are there, at 0.
+  const double slope = endless ? 0.0 : kParts * 1.4426950408889634 / (double)heat, top = endless ? kHuge : most;
+  auto level_of = [&](float l) -> double { return ((double)l - top) * slope; };  // of a finite l
+  // The weight: 2^(y/512) = 2^a 2^(b/512) e^z with whole a and b and |z| <= ln 2 / 1024, for which
+  // 1 + z + z^2/2 + z^3/6 is within 9e-15.
   auto weight_at = [&](double y, int& whole) -> double {
     const double shifted = y + kRound;
     whole = __double2loint(shifted);
@@ -333,14 +331,15 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     const double z = fma(r, fma(r, c * c * c / 6, c * c / 2), c);
     const double t = sh.table[whole & (kParts - 1)];
     const double w = fma(t, z * r, t);
-    return __hiloint2double(__double2hiint(w) + (whole >> 9 << 20), __double2loint(w));
+    return __hiloint2double(__double2hiint(w) + ((whole & -kParts) << 11), __double2loint(w));
   };
   static_assert(kParts == 512, "");
   // Below it weights, of less than 2^-999.7, count as 0; rounded so that none of less than 2^-1000 is above it.
   const float least_level = endless ? INFINITY : fmaxf(__fsub_ru(most, __fmul_rd(693.f, heat)), -kHuge);
+  auto bounded = [&](float l) { return fminf(fmaxf(l, least_level), kHuge); };
   auto weight = [&](float l) -> double {
     int whole;
-    const double w = weight_at(level_of(l), whole);
+    const double w = weight_at(level_of(bounded(l)), whole);
     return l >= least_level ? w : 0.0;
   };
   // 64ths of an octave below the largest's
@@ -363,9 +362,9 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     }
   };
   // Those of all CTAs' lists, one after the other, of place tid + i * kThreads; 0 behind the last.
-  auto gather_lists = [&](unsigned long long (&v)[2]) {
+  auto gather_lists = [&](unsigned long long (&v)[kPer]) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPer; ++i) {
       int at = tid + i * kThreads, r = 0;
       while (r < cluster && at >= sh.all_listed[r]) at -= sh.all_listed[r++];
       v[i] = r < cluster ? of_rank(rs.list, r)[at] : 0;
@@ -377,9 +376,8 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   };
   const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
   const double goal_share = u > 0.f ? (double)fminf(u, 1.f) : 0.0;
-  const bool by_k = k > 0 && k < valid, by_p = top_p < 1.f;
 
-  if (RANKS && by_k && few) {
+  if (quick) {
     // the least of the groups' medians: half of each group's warps reach it
     const int groups = (warps + 31) / 32;
     if (warp < groups) {
@@ -390,32 +388,73 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     float level = sh.level[0];
     for (int g = 1; g < groups; ++g) level = fminf(level, sh.level[g]);
     const float bar = fmaxf(level, -kHuge);
-    for_all(0, n, tid, kThreads, [&](int i, float l) {
-      if (l >= bar) list(l, i);
-    });
+    double mass = 0.0, head = 0.0;  // (top-p alone) of all, and of those listed
+    if (by_k) {
+      for_all(0, n, tid, kThreads, [&](int i, float l) {
+        if (l >= bar) list(l, i);
+      });
+    } else {
+      for_fours(0, n, tid, kThreads, [&](int i, const float(&l)[4]) {
+        double w[4];
+        int whole;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[j] = weight_at(level_of(bounded(l[j])), whole);
+          w[j] = l[j] >= least_level ? w[j] : 0.0;
+        }
+        mass += (w[0] + w[1]) + (w[2] + w[3]);
+        if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) < bar) return;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (l[j] >= bar) {
+            list(l[j], i + j);
+            head += w[j];
+          }
+      });
+#pragma unroll
+      for (int off = 16; off; off >>= 1) {
+        mass += __shfl_xor_sync(0xffffffffu, mass, off);
+        head += __shfl_xor_sync(0xffffffffu, head, off);
+      }
+      if (lane < cluster) {
+        *of_rank(&sh.all_sum[rank * kWarps + warp], lane) = mass;
+        *of_rank(&sh.all_head[rank * kWarps + warp], lane) = head;
+      }
+    }
     __syncthreads();
     if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
     cluster_sync();
     int count = 0;
     bool fits = true;
     for (int r = 0; r < cluster; ++r) count += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
-    if (fits && count <= kList) {
-      unsigned long long v[2] = {0, 0};
+    fits = fits && count <= (by_k ? kList : kThreads);
+    if (!by_k) {  // the list reaches the sum that is wanted, or min_p ends within it, or it holds all
+      mass = head = 0.0;
+      for (int i = lane; i < warps; i += 32) mass += sh.all_sum[i], head += sh.all_head[i];
+#pragma unroll
+      for (int off = 16; off; off >>= 1) {
+        mass += __shfl_xor_sync(0xffffffffu, mass, off);
+        head += __shfl_xor_sync(0xffffffffu, head, off);
+      }
+      fits = fits && (head >= (double)top_p * mass || weight(bar) < least || bar == -kHuge);
+    }
+    if (fits) {
+      unsigned long long v[kPer] = {};
       if (rank == 0) gather_lists(v);
       cluster_sync();  // no CTA reads another's after this
       if (rank != 0) return;
       int size = 32;
       while (size < count) size <<= 1;
-      const unsigned long long* sorted = sort_threads<true, 2>(v, size, &rs.sorted[0][0]);
+      const unsigned long long* sorted = sort_threads<true, kPer>(v, size, &rs.sorted[0][0]);
       // thread t: the token of rank t
-      const bool ranked = tid < k;
+      const bool ranked = tid < (by_k ? min(k, count) : count);
       const unsigned long long mine_of = ranked ? sorted[tid] : 0;
       const int index = (int)(0xffffffffu - (uint32_t)mine_of);
       const double w = ranked ? weight(value_of((uint32_t)(mine_of >> 32))) : 0.0;
       double total;
       const double before = scan_threads(w, sh.scan, &total);
       bool is = ranked && w >= least && (!endless || w > 0.0);
-      if (by_p) is = is && (tid == 0 || before < (double)top_p * total);
+      if (by_p) is = is && (tid == 0 || before < (double)top_p * (by_k ? total : mass));
       const int kept = __syncthreads_count(is);  // a prefix
       if (tid == 0 && p.kept) p.kept[row] = kept;
       // by index; the ranks lead to the weights
@@ -445,36 +484,52 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     __syncthreads();
   }
 
+  // Warps own runs of the row, so that the runs' sums stand in the order of the tokens.
   const int run = (slice + kWarps * 32 * kVec - 1) / (kWarps * 32 * kVec) * (32 * kVec);
   const int r0 = min(padded, warp * run), r1 = min(padded, r0 + run);
+  double sum = 0.0;  // of the weights of what is kept of the warp's run, over the lanes
+  int count = 0;
+  bool summed = false;
   // Where the kept ones end: a value, and the last index of it.
   float cut_value = endless ? kHuge : kNone;
   int cut_index = -1;
   auto above_cut = [&](int i, float l) { return l > cut_value || (l == cut_value && first + i <= cut_index); };
-  // Moves the cut up: of what is kept so far, the first `share` tokens, or those up to that share of their sum.
+  // Moves the cut up: of what is kept so far, the first `share` tokens, or those up to that share of their sum.  The
+  // latter, which is the last filter by rank, also sums what is kept.
   auto narrow = [&](bool by_mass, double share) {
     for (int i = tid; i < kBins; i += kThreads) rs.low[i] = rs.high[i] = 0;
     if (tid == 0) sh.listed = 0;
+    if (tid < kWarps) sh.extra[tid] = 0, sh.extra_count[tid] = 0;
     __syncthreads();
-    for_vectors(0, n, tid, kThreads, [&](int i, const float(&l)[kVec]) {
-      unsigned long long m[kVec];
-      int whole[kVec];
+    auto add = [&](int whole, unsigned long long m) {
+      const int bin = bin_of(whole);
+      const uint32_t low = (uint32_t)m, old = atomicAdd(&rs.low[bin], low);
+      const uint32_t high = (uint32_t)(m >> 32) + (old + low < old);
+      if (high) atomicAdd(&rs.high[bin], high);
+    };
+    if (by_mass && cut_value == kNone) {  // of all
+      for_fours(0, n, tid, kThreads, [&](int, const float(&l)[4]) {
+        unsigned long long m[4];
+        int whole[4];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {  // all, before the first waits for another thread's addition
-        m[j] = units(weight_at(level_of(l[j]), whole[j]));
-        whole[j] = l[j] >= least_level ? whole[j] : kParts * -1000;
-        m[j] = by_mass && l[j] >= least_level ? m[j] : 0;
-        m[j] = above_cut(i + j, l[j]) ? (by_mass ? m[j] : 1) : 0;
-      }
+        for (int j = 0; j < 4; ++j) m[j] = units(weight_at(level_of(fmaxf(l[j], least_level)), whole[j]));
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        if (m[j] == 0) continue;
-        const int bin = bin_of(whole[j]);
-        const uint32_t low = (uint32_t)m[j], old = atomicAdd(&rs.low[bin], low);
-        const uint32_t high = (uint32_t)(m[j] >> 32) + (old + low < old);
-        if (high) atomicAdd(&rs.high[bin], high);
-      }
-    });
+        for (int j = 0; j < 4; ++j)  // all weights, before the first waits for another thread's addition
+          if (l[j] >= least_level && m[j]) add(whole[j], m[j]);
+      });
+    } else {
+      for_all(0, n, tid, kThreads, [&](int i, float l) {
+        int whole;
+        const unsigned long long m = units(weight_at(level_of(bounded(l)), whole));
+        if (!above_cut(i, l)) return;
+        if (l < least_level)
+          by_mass ? void() : add(-kParts * 1000, 1);
+        else if (!by_mass)
+          add(whole, 1);
+        else if (m)
+          add(whole, m);
+      });
+    }
     cluster_sync();
     // each CTA sums some of the bins over all, in the place of its own, which no other reads before that
     const int per = kBins / cluster;
@@ -516,39 +571,54 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     __syncthreads();
     const int bin = (int)sh.bin;
     const unsigned long long above = sh.above_mass;
-    auto in_bin = [&](int i, float l) {
-      const int whole = l >= least_level ? __double2loint(level_of(l) + kRound) : kParts * -1000;
-      return bin_of(whole) == bin && above_cut(i, l);
+    auto whole_of = [&](float l) {
+      return l >= least_level ? __double2loint(level_of(fminf(l, kHuge)) + kRound) : kParts * -1000;
     };
-    for_vectors(0, n, tid, kThreads, [&](int i, const float(&l)[kVec]) {
-      bool is[kVec];
+    auto in_bin = [&](int i, float l) { return bin_of(whole_of(l)) == bin && above_cut(i, l); };
+    if (by_mass) {  // what is above the bin is kept, what is in it is listed
+      const bool all = cut_value == kNone;
+      for_fours(r0, r1, lane, 32, [&](int i, const float(&l)[4]) {
+        double w[4];
+        int whole[4];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) is[j] = in_bin(i + j, l[j]);
+        for (int j = 0; j < 4; ++j) w[j] = weight_at(level_of(bounded(l[j])), whole[j]);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        if (is[j]) list(l[j], i + j);
-    });
+        for (int j = 0; j < 4; ++j) {
+          const int b = bin_of(whole[j]);
+          const bool there = l[j] >= least_level && (all || above_cut(i + j, l[j]));
+          if (there && b == bin) list(l[j], i + j);
+          const bool kept = there && b < bin && w[j] >= least;
+          w[j] = kept ? w[j] : 0.0;
+          count += kept;
+        }
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+      });
+    } else {
+      for_all(0, n, tid, kThreads, [&](int i, float l) {
+        if (in_bin(i, l)) list(l, i);
+      });
+    }
     __syncthreads();
     if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
     cluster_sync();
-    int count = 0;
+    int entries = 0;
     bool fits = true;
-    for (int r = 0; r < cluster; ++r) count += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
-    if (fits && count <= kList) {
+    for (int r = 0; r < cluster; ++r) entries += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
+    if (fits && entries <= kList) {
       if (rank == 0) {
-        unsigned long long v[2];
+        unsigned long long v[kPer];
         gather_lists(v);
         int size = 32;
-        while (size < count) size <<= 1;
-        // thread t: ranks 2 t and 2 t + 1
-        const unsigned long long* sorted = sort_threads<true, 2>(v, size, &rs.sorted[0][0]);
-        if (tid == 0) sh.first_equal = count - 1;
+        while (size < entries) size <<= 1;
+        // thread t: ranks from kPer t on
+        const unsigned long long* sorted = sort_threads<true, kPer>(v, size, &rs.sorted[0][0]);
+        if (tid == 0) sh.first_equal = entries - 1;
         __syncthreads();
-        unsigned long long own[2], sum = 0;
+        unsigned long long own[kPer], sum = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          v[i] = 2 * tid + i < count ? sorted[2 * tid + i] : 0;
-          own[i] = 2 * tid + i >= count ? 0 : by_mass ? units(weight(value_of((uint32_t)(v[i] >> 32)))) : 1;
+        for (int i = 0; i < kPer; ++i) {
+          v[i] = kPer * tid + i < entries ? sorted[kPer * tid + i] : 0;
+          own[i] = kPer * tid + i >= entries ? 0 : by_mass ? units(weight(value_of((uint32_t)(v[i] >> 32)))) : 1;
           sum += own[i];
         }
         inc = sum;
@@ -562,9 +632,9 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
         unsigned long long passed = above + inc - sum;
         for (int w = 0; w < warp; ++w) passed += sh.scan_mass[w];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kPer; ++i) {
           passed += own[i];
-          if (2 * tid + i < count && passed >= wanted) atomicMin(&sh.first_equal, 2 * tid + i);
+          if (kPer * tid + i < entries && passed >= wanted) atomicMin(&sh.first_equal, kPer * tid + i);
         }
         __syncthreads();
         if (tid < cluster) {
@@ -575,9 +645,26 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
       }
       cluster_sync();
       cut_value = value_of(sh.cut_key), cut_index = sh.cut_index;
+      if (by_mass) {
+        // the kept of the bin, in whole units: listed in any order, their sums are the same
+        for (int i = tid; i < sh.listed; i += kThreads) {
+          const unsigned long long v = rs.list[i];
+          const int at = (int)(0xffffffffu - (uint32_t)v) - first;
+          const float l = value_of((uint32_t)(v >> 32));
+          const double w = weight(l);
+          if (above_cut(at, l) && w >= least) {
+            atomicAdd(&sh.extra[at / run], units(w));
+            atomicAdd(&sh.extra_count[at / run], 1);
+          }
+        }
+        __syncthreads();
+        if (lane == 0) sum += (double)sh.extra[warp] * (1.0 / kUnit), count += sh.extra_count[warp];
+        summed = true;
+      }
       return;
     }
     // More of nearly one value than a list holds: by descending digits of their keys.
+    sum = 0.0, count = 0;
     uint32_t known = 0, key_so_far = 0;
     unsigned long long before = above, equal = 0, equal_mass = 0;
     for (int high = kKeyBits<T>; high > 0;) {
@@ -665,40 +752,29 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
     const double w = weight(l);
     return above_cut(i, l) && w >= least ? w : 0.0;
   };
-  // Warps own runs of the row, so that the runs' sums stand in the order of the tokens.
-  double sum = 0.0;
-  int count = 0;
-  const bool plain = !by_k && !by_p && least == 0.0 && !endless;  // all that are there
-  if (plain) {
-    for_vectors(r0, r1, lane, 32, [&](int, const float(&l)[kVec]) {
-      double w[kVec];
+  if (!summed) {
+    const bool plain = !by_k && !by_p && least == 0.0 && !endless;  // all that are there
+    for_fours(r0, r1, lane, 32, [&](int i, const float(&l)[4]) {
+      bool is[4];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) w[j] = weight(l[j]);
+      for (int j = 0; j < 4; ++j) is[j] = plain ? l[j] > kNone : above_cut(i + j, l[j]);
+      if (!(is[0] | is[1] | is[2] | is[3])) return;
+      double w[4];
+      int whole;
 #pragma unroll
-      for (int j = 1; j < kVec; j <<= 1)
-#pragma unroll
-        for (int i = 0; i < kVec; i += 2 * j) w[i] += w[i + j];
-      sum += w[0];
-    });
-  } else {
-    for_vectors(r0, r1, lane, 32, [&](int i, const float(&l)[kVec]) {
-      bool any = false;
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) any |= above_cut(i + j, l[j]);
-      if (!any) return;
-      double w[kVec];
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        w[j] = weight(l[j]);
-        const bool is = above_cut(i + j, l[j]) && w[j] >= least;
-        w[j] = is ? w[j] : 0.0;
-        count += is;
+      for (int j = 0; j < 4; ++j) {
+        w[j] = weight_at(level_of(bounded(l[j])), whole);
+        w[j] = is[j] && l[j] >= least_level ? w[j] : 0.0;
       }
 #pragma unroll
-      for (int j = 1; j < kVec; j <<= 1)
-#pragma unroll
-        for (int k = 0; k < kVec; k += 2 * j) w[k] += w[k + j];
-      sum += w[0];
+      for (int j = 0; j < 4; ++j) {
+        if (!plain) {
+          is[j] = is[j] && w[j] >= least;
+          w[j] = is[j] ? w[j] : 0.0;
+        }
+        count += is[j];
+      }
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
     });
   }
 #pragma unroll
@@ -742,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
   owner = __shfl_sync(0xffffffffu, passing ? owner : last_run, from);
   before = __shfl_sync(0xffffffffu, passing ? owner_before : last_before, from);
   all = __reduce_add_sync(0xffffffffu, all);
-  if (rank == 0 && tid == 0 && p.kept) p.kept[row] = plain ? valid : all;
+  if (rank == 0 && tid == 0 && p.kept) p.kept[row] = all;
   if (owner / kWarps != rank) return;
   // All threads on that run, consecutive tokens each.
   const int w0 = min(n, owner % kWarps * run), w1 = min(n, w0 + run), share = (run + kThreads - 1) / kThreads;
@@ -773,18 +849,10 @@ __global__ void __launch_bounds__(kThreads, RANKS ? 2 : 3) sample_tokens_kernel(
 }
 
 template <class T, bool RANKS>
-cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) {
+cudaError_t launch_sample(const SampleParams& p, int cluster, cudaStream_t st) {
   constexpr int kMaxDevices = 64, kMaxBytes = 227 * 1024;
   static_assert(kHead<RANKS> + kSampleMaxVocab / kMaxCluster * (int)sizeof(T) <= kMaxBytes, "");
   static std::atomic<unsigned> asked[kMaxDevices];
-  // CTAs of a row: those that its size needs, and then, where the row may need its sums by bins (a pass of twice the
-  // others' work), while the launch stays within four a SM; without ranks, until there is about one a SM.  us with 2, 4, 8:
-  // 64 x 128256 bf16, top-p and others 88, 70, 62, plain 20, 26, 26; 256 x 32000 f32, all filters 31, 44, 77, plain 25, 30, 51.
-  int cluster = 1;
-  while (cluster < kMaxCluster &&
-         ((RANKS ? (long long)p.rows * cluster * 2 <= 4 * sm_count : (long long)p.rows * cluster * 10 < 8 * sm_count) ||
-          kHead<RANKS> + ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > 112 * 1024))
-    cluster *= 2;
   const int slice = ((p.vocab + cluster - 1) / cluster + 7) / 8 * 8, smem = kHead<RANKS> + slice * (int)sizeof(T);
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -813,7 +881,18 @@ cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) 
 
 template <class T>
 cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) {
-  return p.top_k || p.top_p ? launch_sample<T, true>(p, sm_count, st) : launch_sample<T, false>(p, sm_count, st);
+  const bool ranks = p.top_k || p.top_p;
+  const int head = ranks ? kHead<true> : kHead<false>;
+  // CTAs of a row: as its size needs them where two share a SM; where the row may need its sums by bins, a pass over it
+  // more, while the launch stays within four a SM; without ranks, until there is about one a SM.  us with 2, 4, 8:
+  // 64 x 128256 bf16, some rows with top-k, some with top-p 67, 59, 57, plain 23, 23, 29; with 1, 2, 4: 256 x 32000 f32,
+  // all filters 35, 31, 43, plain 30, 27, 36.
+  int cluster = 1;
+  while (cluster < kMaxCluster &&
+         ((ranks ? (long long)p.rows * cluster * 2 <= 4 * sm_count : (long long)p.rows * cluster * 10 < 8 * sm_count) ||
+          head + ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > 112 * 1024))
+    cluster *= 2;
+  return ranks ? launch_sample<T, true>(p, cluster, st) : launch_sample<T, false>(p, cluster, st);
 }
 
 }  // namespace
