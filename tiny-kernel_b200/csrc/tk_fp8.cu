@@ -124,17 +124,25 @@ struct GroupScale {
 };
 __device__ __forceinline__ GroupScale group_scale(uint32_t most) {
   if (most >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f};
-  const float s = fmaxf(__uint_as_float(most) * (1.f / kLargest), kLeastScale);
-  float over;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over) : "f"(s));  // within 2^-23: a code is of 4 bits
-  return {s, over};
+  const float s = fmaxf(__fdiv_rn(__uint_as_float(most), kLargest), kLeastScale);
+  return {s, __frcp_rn(s)};
 }
 
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
-  uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-  return lo | (uint32_t)hi << 16;
+// Codes of v[0] / scale .. v[3] / scale.  A product with the reciprocal alone would round some quotients to the wrong side
+// of a tie, of which 16-bit values over their largest make many (7 codes in 10000, bf16); it is corrected by its
+// remainder, after which it is the nearest f32 (Markstein, 1990).  (With divisions 22 us instead of 15: 2048 x 14336 bf16.)
+__device__ __forceinline__ uint32_t codes4(const float* v, const GroupScale& g) {
+  const unsigned long long over = pair_of(g.over, g.over), less = pair_of(-g.scale, -g.scale);
+  uint32_t y = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const unsigned long long x = pair_of(v[i], v[i + 1]), q = mul2(x, over);
+    const float2 r = values_of(fma2(fma2(q, less, x), over, q));
+    uint16_t two;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(r.y), "f"(r.x));
+    y |= (uint32_t)two << (8 * i);
+  }
+  return y;
 }
 // FAST: dst is on a boundary of E bytes.
 template <int E, bool FAST>
@@ -142,7 +150,7 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, int n, const float (&v
   uint32_t y[E / 4];
 #pragma unroll
   for (int i = 0; i < E / 4; ++i) {
-    y[i] = codes4(v[4 * i] * g.over, v[4 * i + 1] * g.over, v[4 * i + 2] * g.over, v[4 * i + 3] * g.over);
+    y[i] = codes4(&v[4 * i], g);
     if (g.over == 0.f) y[i] = 0;
   }
   if constexpr (!FAST) {
