@@ -342,3 +342,56 @@ def test_calls_leave_the_current_device_and_count_their_launches(torch_cuda, tkd
     b.step(1)
     torch_cuda.cuda.synchronize()
     assert tkdev.launch_count() == before + 5 and torch_cuda.cuda.current_device() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("block", [1, 128])
+def test_codes_are_the_nearest_of_the_quotient(torch_cuda, tkdev, block, dtype):
+    """Scales are the largest over 448 and codes the conversion of value / scale, bit by bit: 16-bit values over their
+    largest lie on ties often."""
+    torch = torch_cuda
+    x = rows_of(torch, 77, 256, 4096, dtype, 0)
+    codes, scales = torch.zeros((256, 4096), dtype=torch.uint8, device="cuda"), torch.zeros((256 // block, 32), device="cuda")
+    torch.cuda.synchronize()
+    ops.fp8_quantize(tkdev, x, codes, scales, 256, 4096, block, dtype)
+    v, s = x.float().cpu(), scales.cpu()
+    tiles = v.view(256 // block, block, 32, 128)
+    want = tiles.abs().amax((1, 3)) / torch.tensor(448.0)
+    assert torch.equal(s, want)
+    nearest = (tiles / want[:, None, :, None]).view(256, 4096).to(torch.float8_e4m3fn)
+    assert torch.equal(codes.cpu(), nearest.view(torch.uint8))
+
+
+def test_classes(torch_cuda, tkdev):
+    """The objects of kernels.fp8 and kernels.sampler over the framework's own buffers: an odd k, whose rows of codes
+    the weight pads."""
+    import tiny_kernel as tk
+    rng = np.random.default_rng(5)
+    m, k, n = 4, 300, 500
+    x, r, weight = rng.normal(size=(m, k)), rng.normal(size=(m, k)), 1 + 0.1 * rng.normal(size=k)
+    w = rng.normal(size=(n, k)) * k**-0.5
+    buf = lambda a: tkdev.create_buffer_with_data("f32", np.asarray(a, np.float32))
+    new = lambda t, c: tkdev.create_buffer(t, c)
+    fp = tk.kernels.fp8
+    linear = fp.LinearFP8.init(tkdev, n, k)
+    linear.load(buf(w))
+    total, codes, scales = new("f32", m * k), new("u8", m * k), new("f32", m * fp.blocks(k))
+    fp.AddRMSNormFP8.init(tkdev).forward(buf(x), buf(r), buf(weight), total, codes, scales, k, 1e-5)
+    want_sum, y = fp8.add_rmsnorm(x.astype(np.float32), r.astype(np.float32), weight.astype(np.float32), 1e-5)
+    check_codes(y, codes.read().reshape(m, k), scales.read().reshape(m, -1).astype(np.float64), fp8.group_scales(y, 1), 1, NORM_ERROR)
+    assert np.abs(total.read().reshape(m, k) - want_sum).max() <= 2.0**-23 * np.abs(want_sum).max()
+    again, scales2 = new("u8", m * k), new("f32", m * fp.blocks(k))
+    fp.QuantizeFP8.init(tkdev).forward(total, again, scales2, k)
+    padded = tkdev.create_buffer_with_data("u8", np.pad(again.read().reshape(m, k), ((0, 0), (0, linear.row - k))))
+    logits = new("f32", m * n)
+    linear.forward(padded, scales2, logits, m, a_stride=linear.row)
+    want, size = fp8.matmul(again.read().reshape(m, k), scales2.read().reshape(m, -1), linear.codes.read().reshape(n, -1)[:, :k],
+                            linear.scales.read().reshape(fp.blocks(n), -1))
+    assert (np.abs(logits.read().reshape(m, n) - want) <= 140 * 2.0**-23 * size).all()
+    tokens, kept = new("i32", m), new("i32", m)
+    u = np.array([0.1, 0.4, 0.6, 0.9], np.float32)
+    tk.kernels.sampler.SampleTokens.init(tkdev).forward(logits, None, None, buf([0.9] * m), None, buf(u), tokens, kept)
+    for i, l in enumerate(logits.read().reshape(m, n)):
+        token, count, slack = fp8.sample(l, None, None, np.float32(0.9), None, u[i])
+        assert slack < 1e-9 or (token, count) == (tokens.read()[i], kept.read()[i])
+    linear.deinit()

@@ -6,6 +6,8 @@ pub const quantized = @import("kernels/quantized.zig");
 pub const fused = @import("kernels/fused.zig");
 pub const rmsnorm = @import("kernels/rmsnorm.zig");
 pub const kv4 = @import("kernels/kv4.zig");
+pub const fp8 = @import("kernels/fp8.zig");
+pub const sampler = @import("kernels/sampler.zig");
 
 pub const Device = cuda.Device;
 pub const Buffer = cuda.Buffer;
