@@ -395,3 +395,22 @@ def test_classes(torch_cuda, tkdev):
         token, count, slack = fp8.sample(l, None, None, np.float32(0.9), None, u[i])
         assert slack < 1e-9 or (token, count) == (tokens.read()[i], kept.read()[i])
     linear.deinit()
+
+
+def test_as_many_rows_as_a_call_takes(torch_cuda, tkdev):
+    """Rows of one value, each a group of its own: more groups than 2^32 threads have, and the largest number of rows."""
+    torch = torch_cuda
+    rows = 2**28 + 37
+    x = torch.arange(rows, dtype=torch.float32, device="cuda") % 97 + 1
+    codes, scales = torch.zeros(rows, dtype=torch.uint8, device="cuda"), torch.zeros(rows, device="cuda")
+    torch.cuda.synchronize()
+    ops.fp8_quantize(tkdev, x, codes, scales, rows, 1)
+    assert (codes == 0x7E).all() and torch.equal(scales, x / torch.tensor(448.0, device="cuda"))
+    del x, codes, scales
+    rows = 2**31 - 1
+    x = torch.full((rows,), -3.0, dtype=torch.bfloat16, device="cuda")
+    codes, scales = torch.zeros(rows, dtype=torch.uint8, device="cuda"), torch.zeros(rows, device="cuda")
+    torch.cuda.synchronize()
+    ops.add_rmsnorm_fp8(tkdev, x, None, None, None, codes, scales, rows, 1, 0.0, "bf16")
+    assert codes.min().item() == codes.max().item() == 0xFE
+    assert abs(scales.min().item() * 448 - 1) < 1e-6 and abs(scales.max().item() * 448 - 1) < 1e-6

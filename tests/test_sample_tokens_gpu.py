@@ -152,3 +152,78 @@ def test_rows_do_not_depend_on_others(torch_cuda, tkdev):
     for r in (0, 50, 99):
         one = run(torch_cuda, tkdev, l[r:r + 1], top_k=k[r:r + 1], top_p=0.95, random=u[r:r + 1])
         assert one[0][0] == tokens[r] and one[1][0] == kept[r]
+
+
+@pytest.mark.parametrize("top_k", [255, 256, 257, 399, 400, 401, 511, 512, 513, 1023, 1024, 1025, 2048])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_top_k_around_the_lists(torch_cuda, tkdev, top_k, dtype):
+    """One CTA a row and several; 16-bit rows have more equal values at the cut than a list holds."""
+    rng = np.random.default_rng(top_k)
+    for rows, vocab in [(6, 3001), (6, 60000)]:
+        l = rng.normal(size=(rows, vocab))
+        l[1] = np.sort(l[1])
+        l[2] = np.sort(l[2])[::-1]
+        l[3] = np.round(l[3])
+        l[4] = np.where(np.arange(vocab) % 2 == 0, 1.0, -1.0)
+        for more in (dict(), dict(top_p=0.7), dict(top_p=0.999, min_p=0.1)):
+            run(torch_cuda, tkdev, l, dtype, top_k=top_k, random=rng.random(rows), **more)
+
+
+@pytest.mark.parametrize("top_p", [1e-6, 0.3, 0.5, 0.75, 0.999, 0.99999994])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_top_p_of_equal_and_spread_values(torch_cuda, tkdev, top_p, dtype):
+    """The goal lies among thousands of equal values, in a few values of very different size, in a list's last value,
+    in values of no more than 2^-40 of the largest's weight."""
+    rng = np.random.default_rng(1)
+    vocab = 50000
+    l = np.full((8, vocab), -2.5)
+    l[1, rng.integers(0, vocab, 3000)] = 0.0
+    l[2] = np.round(rng.normal(size=vocab))
+    l[3] = -np.arange(vocab) * 0.5
+    l[4] = -np.arange(vocab) * 0.5
+    l[4, 1:] -= 25.0
+    l[5] = -60.0
+    l[5, 33] = 0.0
+    l[6] = -28.0
+    l[6, 44] = 0.0
+    l[7] = rng.permutation(vocab) / vocab
+    for more in (dict(), dict(min_p=0.3), dict(temperature=0.25)):
+        run(torch_cuda, tkdev, l, dtype, top_p=top_p, random=rng.random(8), **more)
+
+
+def test_streams_and_graphs(torch_cuda, tkdev):
+    """Two calls at once on two streams, over and over, and a captured call replayed with other rows, parameters and
+    numbers, give what calls one by one give."""
+    torch = torch_cuda
+    l, rng = logits_of(77, 96, 32003)
+    x = [torch.tensor(l[i * 48:(i + 1) * 48], dtype=torch.float32, device="cuda") for i in (0, 1)]
+    k = [torch.tensor(rng.integers(0, 600, 48), dtype=torch.int32, device="cuda") for _ in (0, 1)]
+    q = [torch.tensor(rng.uniform(0.3, 1.1, 48), dtype=torch.float32, device="cuda") for _ in (0, 1)]
+    u = [torch.tensor(rng.random(48), dtype=torch.float32, device="cuda") for _ in (0, 1)]
+    out = [torch.zeros((2, 48), dtype=torch.int32, device="cuda") for _ in (0, 1)]
+    want = [torch.zeros((2, 48), dtype=torch.int32, device="cuda") for _ in (0, 1)]
+    torch.cuda.synchronize()
+
+    def call(i, to, stream=None):
+        ops.sample_tokens(tkdev, x[i], None, k[i], q[i], None, u[i], to[0], to[1], 48, 32003, stream=stream)
+
+    for i in (0, 1):
+        call(i, want[i])
+    streams = [torch.cuda.Stream() for _ in (0, 1)]
+    for _ in range(30):
+        for i in (0, 1):
+            call(i, out[i], streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(0, out[0], torch.cuda.current_stream().cuda_stream)
+    for i in (0, 1, 0):
+        first = [a[0].clone() for a in (x, k, q, u)]
+        for a in (x, k, q, u):
+            a[0].copy_(a[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[i])
+        for a, b in zip((x, k, q, u), first):
+            a[0].copy_(b)

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(Fp8RowsParams 
 
 template <class T, int V, int THREADS>
 cudaError_t launch_norm(const Fp8RowsParams& p, bool fast, int warps, int block_rows, cudaStream_t st) {
-  const dim3 blocks((unsigned)((p.rows + block_rows - 1) / block_rows));
+  const dim3 blocks(((unsigned)p.rows + block_rows - 1) / block_rows);
   const int threads = block_rows * warps * 32;
   if (fast) return launch(add_rmsnorm_fp8_kernel<T, V, THREADS, true>, blocks, threads, 0, st, p, warps);
   return launch(add_rmsnorm_fp8_kernel<T, V, THREADS, false>, blocks, threads, 0, st, p, warps);
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_rows_kernel(Fp8RowsPara
   constexpr int kE = kChunk<T>, kLanes = kFp8Block / kE;
   after_previous();
   // (a thread with two or four groups is slower: 2048 x 14336 bf16 14.7 and 16.4 us instead of 14.3)
-  const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / kLanes;
+  const unsigned group = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;  // (threads may be more than 2^32)
   const int lane = threadIdx.x % kLanes, at = (int)(group % groups) * kFp8Block + lane * kE;
   const long long row = group / groups;
   const int n = group < total ? p.dim - at : 0;
