@@ -101,6 +101,7 @@ struct Shared {
   unsigned long long above_mass;
   uint32_t bin_count;
   unsigned long long bin_mass;
+  int long_rows[kWarps], chosen;
 };
 
 // Sums of all threads before this one, and of all.
@@ -185,7 +186,7 @@ constexpr int kHead = (sizeof(Shared) + (RANKS ? sizeof(Ranked) : 0) + 15) / 16 
 
 // RANKS: some row may have top-k or top-p.
 template <class T, bool RANKS>
-__global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams p, int cluster, int slice) {
+__global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams p, int cluster, int slice, int sorted_rows) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   Shared& sh = *reinterpret_cast<Shared*>(dynamic);
   Ranked& rs = *reinterpret_cast<Ranked*>(dynamic + sizeof(Shared));
@@ -193,12 +194,31 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
   constexpr int kVec = 16 / sizeof(T);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x % cluster, warps = cluster * kWarps;
-  const long long row = blockIdx.x / cluster;
+  long long row = blockIdx.x / cluster;
   const int first = rank * slice, n = max(0, min(slice, p.vocab - first));
   for (int i = tid; i < kParts; i += kThreads) sh.table[i] = exp2((double)i / kParts);
   if (tid == 0) sh.listed = 0, sh.first_equal = 0x7fffffff;
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   after_previous();
+  if (RANKS && sorted_rows) {  // the rows that may take long, then the others
+    bool may = false;
+    if (tid < p.rows) {
+      const int k = p.top_k ? p.top_k[tid] : 0;
+      may = (!p.temperature || p.temperature[tid] > 0.f) && (k > 0 && k < p.vocab ? k > kFew : p.top_p && p.top_p[tid] < 1.f);
+    }
+    const uint32_t votes = __ballot_sync(0xffffffffu, may);
+    if (lane == 0) sh.long_rows[warp] = __popc(votes);
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) before = all;
+      all += sh.long_rows[w];
+    }
+    before += __popc(votes & ((1u << lane) - 1u));
+    if (tid < p.rows && (may ? before : all + tid - before) == row) sh.chosen = tid;
+    __syncthreads();
+    row = sh.chosen;
+  }
   const T* src = static_cast<const T*>(p.logits) + row * p.stride + first;
   const float heat = p.temperature ? p.temperature[row] : 1.f;
   const bool greedy = !(heat > 0.f);
@@ -849,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
 }
 
 template <class T, bool RANKS>
-cudaError_t launch_sample(const SampleParams& p, int cluster, cudaStream_t st) {
+cudaError_t launch_sample(const SampleParams& p, int cluster, int sm_count, cudaStream_t st) {
   constexpr int kMaxDevices = 64, kMaxBytes = 227 * 1024;
   static_assert(kHead<RANKS> + kSampleMaxVocab / kMaxCluster * (int)sizeof(T) <= kMaxBytes, "");
   static std::atomic<unsigned> asked[kMaxDevices];
@@ -876,7 +896,9 @@ cudaError_t launch_sample(const SampleParams& p, int cluster, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, RANKS>, p, cluster, slice);
+  // More CTAs than run at once: the last to start should not be those that take longest.
+  const int sorted_rows = p.rows <= kThreads && (long long)p.rows * cluster > 2 * sm_count;
+  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, RANKS>, p, cluster, slice, sorted_rows);
 }
 
 template <class T>
@@ -892,7 +914,7 @@ cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) 
          ((ranks ? (long long)p.rows * cluster * 2 <= 4 * sm_count : (long long)p.rows * cluster * 10 < 8 * sm_count) ||
           head + ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > 112 * 1024))
     cluster *= 2;
-  return ranks ? launch_sample<T, true>(p, cluster, st) : launch_sample<T, false>(p, cluster, st);
+  return ranks ? launch_sample<T, true>(p, cluster, sm_count, st) : launch_sample<T, false>(p, cluster, sm_count, st);
 }
 
 }  // namespace
