@@ -85,7 +85,7 @@ struct Shared {
   double table[kParts];  // 2^(i / kParts)
   // of all CTAs' warps, written by each into every CTA's
   double all_sum[kMaxWarps], all_head[kMaxWarps];
-  float all_most[kMaxWarps], all_level[kMaxWarps];
+  float all_most[kMaxWarps], all_level[kMaxWarps], all_few[kMaxWarps], all_sample[kMaxWarps];
   int all_equal[kMaxWarps], all_count[kMaxWarps];
   int all_listed[kMaxCluster];
   uint32_t cut_key;
@@ -201,11 +201,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   after_previous();
   if (RANKS && sorted_rows) {  // the rows that may take long, then the others
-    bool may = false;
-    if (tid < p.rows) {
-      const int k = p.top_k ? p.top_k[tid] : 0;
-      may = (!p.temperature || p.temperature[tid] > 0.f) && (k > 0 && k < p.vocab ? k > kFew : p.top_p && p.top_p[tid] < 1.f);
-    }
+    const bool there = tid < p.rows;
+    const float heat = there && p.temperature ? p.temperature[tid] : 1.f, top_p = there && p.top_p ? p.top_p[tid] : 1.f;
+    const int k = there && p.top_k ? p.top_k[tid] : 0;
+    const bool may = (heat > 0.f) & (k > 0 && k < p.vocab ? k > kFew : top_p < 1.f);
     const uint32_t votes = __ballot_sync(0xffffffffu, may);
     if (lane == 0) sh.long_rows[warp] = __popc(votes);
     __syncthreads();
@@ -215,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
       all += sh.long_rows[w];
     }
     before += __popc(votes & ((1u << lane) - 1u));
-    if (tid < p.rows && (may ? before : all + tid - before) == row) sh.chosen = tid;
+    if (there && (may ? before : all + tid - before) == row) sh.chosen = tid;
     __syncthreads();
     row = sh.chosen;
   }
@@ -272,21 +271,61 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
   // least.  Few top-k, or, of top-p alone, as many as mostly do.
   const bool by_k = k > 0 && k < p.vocab, by_p = top_p < 1.f;
   const int reach = by_k ? k : by_p ? kReach : 0;
-  const bool quick = RANKS && reach > 0 && reach <= min(kFew, kWarps / 2 * 32 * cluster);
+  bool quick = RANKS && reach > 0 && reach <= min(kFew, kWarps / 2 * 32 * cluster);
   const int each = (reach + warps / 2 - 1) / (warps / 2);
+  float s = kNone;
   if (quick) {
-    const float s = sort_warp<true>(most);
+    s = sort_warp<true>(most);
     if (lane == each - 1)
       for (int r = 0; r < cluster; ++r) *of_rank(&sh.all_level[rank * kWarps + warp], r) = s;
   }
 #pragma unroll
   for (int off = 16; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+  // Of top-p alone, whether that list is likely to do, by the weights of the warp's largest and of a sample of the others, a
+  // vector of each thread's: a flat row is spared the pass that would show that it does not.
+  const bool guess = quick && !by_k && begin > 0 && !(min_p > 0.f);
+  const float per_unit = 1.44269504f / heat;
+  if (guess) {
+    const float level = __shfl_sync(0xffffffffu, s, each - 1);
+    float few = lane < each ? exp2f((s - most) * per_unit) : 0.f, sample = 0.f;
+    const int own = (n / kVec - tid + kThreads - 1) / kThreads;
+    if (own > 0) {
+      const uint4 raw = reinterpret_cast<const uint4*>(mine)[tid + warp % own * kThreads];
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) sample += to_f32(e[j]) < level ? exp2f((to_f32(e[j]) - most) * per_unit) : 0.f;
+      sample *= (float)own;
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+      few += __shfl_xor_sync(0xffffffffu, few, off);
+      sample += __shfl_xor_sync(0xffffffffu, sample, off);
+    }
+    if (lane < cluster) {
+      *of_rank(&sh.all_few[rank * kWarps + warp], lane) = few;
+      *of_rank(&sh.all_sample[rank * kWarps + warp], lane) = sample;
+    }
+  }
   if (lane < cluster) *of_rank(&sh.all_most[rank * kWarps + warp], lane) = most;
   cluster_sync();
   most = kNone;
   for (int i = lane; i < warps; i += 32) most = fmaxf(most, sh.all_most[i]);
 #pragma unroll
   for (int off = 16; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+  if (guess) {
+    float few = 0.f, sample = 0.f;
+    for (int i = lane; i < warps; i += 32) {
+      const float scale = sh.all_most[i] == kNone ? 0.f : exp2f((sh.all_most[i] - most) * per_unit);
+      few += scale > 0.f ? scale * sh.all_few[i] : 0.f;
+      sample += scale > 0.f ? scale * sh.all_sample[i] : 0.f;
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+      few += __shfl_xor_sync(0xffffffffu, few, off);
+      sample += __shfl_xor_sync(0xffffffffu, sample, off);
+    }
+    quick = !(1.1f * few < top_p * (few + sample));
+  }
   if (most == kNone) {
     if (rank == 0 && tid == 0) {
       p.tokens[row] = -1;
