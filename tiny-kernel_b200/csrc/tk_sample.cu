@@ -30,7 +30,9 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8, kMaxWarps = kMaxCluster * kWarps;
 constexpr int kBins = 2048, kList = 1024, kPer = kList / kThreads, kFew = 400, kReach = 192;
-constexpr int kParts = 512, kPerBin = 8;  // of an octave of weights: in the table, and of these in a bin
+constexpr int kParts = 512;  // of an octave of weights, in the table
+constexpr float kBinUnit = 65536.f;  // of a bin's sum: its largest weight
+constexpr int kMostBytes = 112 * 1024;  // of a CTA, unless no cluster is large enough for that
 constexpr float kNone = -INFINITY, kHuge = 3.4028235e38f;
 constexpr double kUnit = 17592186044416.0;  // 2^44: weights as integers, whose sums fit 64 bits
 constexpr double kWhole = 4503599627370496.0, kRound = 1.5 * kWhole;  // 2^52: added, a value's units are whole
@@ -68,9 +70,7 @@ struct Ranked {
   union {
     struct {
       union {
-        struct {
-          uint32_t low[kBins], high[kBins];  // words of a bin's sum
-        };
+        uint32_t sums[kBins];
         unsigned long long sorted[2][kList];  // (key, ~index) of all CTAs' lists
       };
       unsigned long long list[kList];  // found here
@@ -84,7 +84,7 @@ struct Ranked {
 struct Shared {
   double table[kParts];  // 2^(i / kParts)
   // of all CTAs' warps, written by each into every CTA's
-  double all_sum[kMaxWarps], all_head[kMaxWarps];
+  double all_sum[kMaxWarps], all_head[kMaxWarps], all_mass[kMaxWarps];
   float all_most[kMaxWarps], all_level[kMaxWarps], all_few[kMaxWarps], all_sample[kMaxWarps];
   int all_equal[kMaxWarps], all_count[kMaxWarps];
   int all_listed[kMaxCluster];
@@ -401,9 +401,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
     const double w = weight_at(level_of(bounded(l)), whole);
     return l >= least_level ? w : 0.0;
   };
-  // 64ths of an octave below the largest's
-  auto bin_of = [&](int whole) { return min(kBins - 1, -(whole >> 3)); };
-  static_assert(kPerBin == 8, "");
+  // 64ths of an octave below the largest, in f32: in the order of the values, which is all that is asked of it.  The last
+  // bin has whatever is smaller.
+  const float per_bin = endless ? 0.f : fmaxf(-64.f * 1.44269504f / heat, -kHuge);
+  auto place_of = [&](float l) -> float { return fminf(fmaxf(l - most, -kHuge) * per_bin, kBins - 1.f); };
+  auto bin_of = [&](float l) -> int { return (int)place_of(l); };
   auto units = [&](double w) -> unsigned long long {  // to the nearest
     return (unsigned long long)__double_as_longlong(fma(w, kUnit, kWhole)) & ((1ull << 52) - 1);
   };
@@ -556,55 +558,41 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
   // Moves the cut up: of what is kept so far, the first `share` tokens, or those up to that share of their sum.  The
   // latter, which is the last filter by rank, also sums what is kept.
   auto narrow = [&](bool by_mass, double share) {
-    for (int i = tid; i < kBins; i += kThreads) rs.low[i] = rs.high[i] = 0;
+    for (int i = tid; i < kBins; i += kThreads) rs.sums[i] = 0;
     if (tid == 0) sh.listed = 0;
     if (tid < kWarps) sh.extra[tid] = 0, sh.extra_count[tid] = 0;
     __syncthreads();
-    auto add = [&](int whole, unsigned long long m) {
-      const int bin = bin_of(whole);
-      const uint32_t low = (uint32_t)m, old = atomicAdd(&rs.low[bin], low);
-      const uint32_t high = (uint32_t)(m >> 32) + (old + low < old);
-      if (high) atomicAdd(&rs.high[bin], high);
-    };
-    if (by_mass && cut_value == kNone) {  // of all
-      for_fours(0, n, tid, kThreads, [&](int, const float(&l)[4]) {
-        unsigned long long m[4];
-        int whole[4];
+    const bool all_there = cut_value == kNone;
+    // Sums of weights are in a bin's own unit, within 1e-5: enough to find the bin, nearly always, and a pass with the exact
+    // sums follows anyway.
+    for_fours(0, n, tid, kThreads, [&](int i, const float(&l)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = units(weight_at(level_of(fmaxf(l[j], least_level)), whole[j]));
-#pragma unroll
-        for (int j = 0; j < 4; ++j)  // all weights, before the first waits for another thread's addition
-          if (l[j] >= least_level && m[j]) add(whole[j], m[j]);
-      });
-    } else {
-      for_all(0, n, tid, kThreads, [&](int i, float l) {
-        int whole;
-        const unsigned long long m = units(weight_at(level_of(bounded(l)), whole));
-        if (!above_cut(i, l)) return;
-        if (l < least_level)
-          by_mass ? void() : add(-kParts * 1000, 1);
-        else if (!by_mass)
-          add(whole, 1);
-        else if (m)
-          add(whole, m);
-      });
-    }
+      for (int j = 0; j < 4; ++j) {
+        if (!(all_there ? l[j] > kNone : above_cut(i + j, l[j]))) continue;
+        const float place = place_of(l[j]);
+        const int bin = (int)place;
+        if (!by_mass)
+          atomicAdd(&rs.sums[bin], 1u);
+        else if (bin < kBins - 1)
+          atomicAdd(&rs.sums[bin], (uint32_t)fmaf(place - (float)bin, -kBinUnit * 0.01077f, kBinUnit));
+      }
+    });
     cluster_sync();
     // each CTA sums some of the bins over all, in the place of its own, which no other reads before that
     const int per = kBins / cluster;
     for (int bin = rank * per + tid; bin < (rank + 1) * per; bin += kThreads) {
       unsigned long long m = 0;
-      for (int r = 0; r < cluster; ++r)
-        m += of_rank(rs.low, r)[bin] + ((unsigned long long)of_rank(rs.high, r)[bin] << 32);
-      rs.low[bin] = (uint32_t)m, rs.high[bin] = (uint32_t)(m >> 32);
+      for (int r = 0; r < cluster; ++r) m += of_rank(rs.sums, r)[bin];
+      rs.sums[bin] = by_mass ? __float_as_uint((float)m * exp2f(bin * (-1.f / 64.f))) : (uint32_t)m;
     }
     cluster_sync();
     constexpr int kEach = kBins / kThreads;
     unsigned long long m[kEach], mass = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int b = tid * kEach + j, r = b / per;
-      mass += m[j] = of_rank(rs.low, r)[b] + ((unsigned long long)of_rank(rs.high, r)[b] << 32);
+      const int b = tid * kEach + j;
+      const uint32_t v = of_rank(rs.sums, b / per)[b];
+      mass += m[j] = by_mass ? (unsigned long long)(__uint_as_float(v) * kBinUnit) : v;
     }
     unsigned long long inc = mass;
 #pragma unroll
@@ -619,47 +607,92 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
       if (w < warp) at += sh.scan_mass[w];
       all += sh.scan_mass[w];
     }
-    if (by_mass) share *= (double)all;
-    unsigned long long wanted = (unsigned long long)share;
-    wanted = max(1ull, min(all, wanted + ((double)wanted < share)));
+    const double about = by_mass ? share * (double)all : share;
+    unsigned long long wanted = (unsigned long long)about;
+    wanted = max(1ull, min(all, wanted + ((double)wanted < about)));
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       if (at < wanted && wanted <= at + m[j]) sh.bin = (uint32_t)(tid * kEach + j), sh.above_mass = at;
       at += m[j];
     }
     __syncthreads();
-    const int bin = (int)sh.bin;
-    const unsigned long long above = sh.above_mass;
-    auto whole_of = [&](float l) {
-      return l >= least_level ? __double2loint(level_of(fminf(l, kHuge)) + kRound) : kParts * -1000;
-    };
-    auto in_bin = [&](int i, float l) { return bin_of(whole_of(l)) == bin && above_cut(i, l); };
-    if (by_mass) {  // what is above the bin is kept, what is in it is listed
-      const bool all = cut_value == kNone;
-      for_fours(r0, r1, lane, 32, [&](int i, const float(&l)[4]) {
-        double w[4];
-        int whole[4];
+    int bin = (int)sh.bin;
+    unsigned long long above = sh.above_mass;
+    auto in_bin = [&](int i, float l) { return l > kNone && bin_of(l) == bin && above_cut(i, l); };
+    if (by_mass) {
+      // What is above the bin is kept, what is in it is listed.  Where the exact sums say that the goal is in another bin, that
+      // one, in growing steps until they have it between them.
+      int low = 0, high = kBins - 1;
+      for (int step = 1;; step *= 2) {
+        double mass = 0.0, head = 0.0;
+        sum = 0.0, count = 0;
+        for_fours(r0, r1, lane, 32, [&](int i, const float(&l)[4]) {
+          double w[4];
+          int whole;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = weight_at(level_of(bounded(l[j])), whole[j]);
+          for (int j = 0; j < 4; ++j) w[j] = weight_at(level_of(bounded(l[j])), whole);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int b = bin_of(whole[j]);
-          const bool there = l[j] >= least_level && (all || above_cut(i + j, l[j]));
-          if (there && b == bin) list(l[j], i + j);
-          const bool kept = there && b < bin && w[j] >= least;
-          w[j] = kept ? w[j] : 0.0;
-          count += kept;
+          for (int j = 0; j < 4; ++j) {
+            const int b = bin_of(l[j]);
+            const bool there = l[j] >= least_level && (all_there || above_cut(i + j, l[j]));
+            if (there && b == bin) {
+              list(l[j], i + j);
+              head += w[j];
+            }
+            w[j] = there ? w[j] : 0.0;
+            mass += w[j];
+            count += there && b < bin;
+            sum += there && b < bin ? w[j] : 0.0;
+          }
+        });
+        double above = sum;
+#pragma unroll
+        for (int off = 16; off; off >>= 1) {
+          mass += __shfl_xor_sync(0xffffffffu, mass, off);
+          head += __shfl_xor_sync(0xffffffffu, head, off);
+          above += __shfl_xor_sync(0xffffffffu, above, off);
         }
-        sum += (w[0] + w[1]) + (w[2] + w[3]);
-      });
+        if (lane < cluster) {
+          *of_rank(&sh.all_mass[rank * kWarps + warp], lane) = mass;
+          *of_rank(&sh.all_head[rank * kWarps + warp], lane) = head;
+          *of_rank(&sh.all_sum[rank * kWarps + warp], lane) = above;
+        }
+        __syncthreads();
+        if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
+        cluster_sync();
+        mass = head = above = 0.0;
+        for (int i = lane; i < warps; i += 32) mass += sh.all_mass[i], head += sh.all_head[i], above += sh.all_sum[i];
+#pragma unroll
+        for (int off = 16; off; off >>= 1) {
+          mass += __shfl_xor_sync(0xffffffffu, mass, off);
+          head += __shfl_xor_sync(0xffffffffu, head, off);
+          above += __shfl_xor_sync(0xffffffffu, above, off);
+        }
+        const double goal = share * mass;
+        const bool before = above >= goal && bin > 0, behind = above + head < goal;
+        if (before) high = bin - 1;
+        if (behind) low = bin + 1;
+        if (!(before || behind) || low > high) {
+          const double rest = (goal - above) * kUnit;  // in units, of what the bin has
+          wanted = rest > 1.0 ? (unsigned long long)rest : 1;
+          wanted += (double)wanted < rest;
+          break;
+        }
+        bin = before ? max(low, bin - step) : min(high, bin + step);
+        if (low > 0 && high < kBins - 1) bin = (low + high) / 2;
+        cluster_sync();  // all have read what the next pass writes
+        if (tid == 0) sh.listed = 0;
+        __syncthreads();
+      }
+      above = 0;
     } else {
       for_all(0, n, tid, kThreads, [&](int i, float l) {
         if (in_bin(i, l)) list(l, i);
       });
+      __syncthreads();
+      if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
+      cluster_sync();
     }
-    __syncthreads();
-    if (tid < cluster) *of_rank(&sh.all_listed[rank], tid) = sh.listed;
-    cluster_sync();
     int entries = 0;
     bool fits = true;
     for (int r = 0; r < cluster; ++r) entries += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
@@ -704,15 +737,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
       }
       cluster_sync();
       cut_value = value_of(sh.cut_key), cut_index = sh.cut_index;
-      if (by_mass) {
+      if (by_mass && least == 0.0) {
         // the kept of the bin, in whole units: listed in any order, their sums are the same
         for (int i = tid; i < sh.listed; i += kThreads) {
           const unsigned long long v = rs.list[i];
           const int at = (int)(0xffffffffu - (uint32_t)v) - first;
           const float l = value_of((uint32_t)(v >> 32));
-          const double w = weight(l);
-          if (above_cut(at, l) && w >= least) {
-            atomicAdd(&sh.extra[at / run], units(w));
+          if (above_cut(at, l)) {
+            atomicAdd(&sh.extra[at / run], units(weight(l)));
             atomicAdd(&sh.extra_count[at / run], 1);
           }
         }
@@ -720,6 +752,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
         if (lane == 0) sum += (double)sh.extra[warp] * (1.0 / kUnit), count += sh.extra_count[warp];
         summed = true;
       }
+      if (!summed) sum = 0.0, count = 0;
       return;
     }
     // More of nearly one value than a list holds: by descending digits of their keys.
@@ -758,8 +791,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
       }
       if (lane == 31) sh.scan_mass[warp] = inc;
       __syncthreads();
-      at = before + inc - mass;
-      for (int w = 0; w < warp; ++w) at += sh.scan_mass[w];
+      at = before + inc - mass, all = before;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) at += sh.scan_mass[w];
+        all += sh.scan_mass[w];
+      }
+      if (by_mass && known == 0) wanted = min(wanted, all);  // (rounded otherwise than the sums of weights)
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
         if (at < wanted && wanted <= at + m[j]) {
@@ -910,6 +947,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
 template <class T, bool RANKS>
 cudaError_t launch_sample(const SampleParams& p, int cluster, int sm_count, cudaStream_t st) {
   constexpr int kMaxDevices = 64, kMaxBytes = 227 * 1024;
+  static_assert(kSampleMaxVocab / kMaxCluster * (double)kBinUnit < 4294967296.0 && kMostBytes / 2 * (double)kBinUnit < 4294967296.0, "a CTA's bins");
   static_assert(kHead<RANKS> + kSampleMaxVocab / kMaxCluster * (int)sizeof(T) <= kMaxBytes, "");
   static std::atomic<unsigned> asked[kMaxDevices];
   const int slice = ((p.vocab + cluster - 1) / cluster + 7) / 8 * 8, smem = kHead<RANKS> + slice * (int)sizeof(T);
@@ -951,7 +989,7 @@ cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) 
   int cluster = 1;
   while (cluster < kMaxCluster &&
          ((ranks ? (long long)p.rows * cluster * 2 <= 4 * sm_count : (long long)p.rows * cluster * 10 < 8 * sm_count) ||
-          head + ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > 112 * 1024))
+          head + ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > kMostBytes))
     cluster *= 2;
   return ranks ? launch_sample<T, true>(p, cluster, sm_count, st) : launch_sample<T, false>(p, cluster, sm_count, st);
 }
