@@ -7,16 +7,23 @@
 //   random times the sum of all kept.
 //
 // The answer is a whole number that goes by where one sum passes another, so weights and sums are f64: a token differs
-// from that of exact sums where the random number lies within about 1e-13 of a border, instead of within 1e-7,
+// from that of exact sums where the random number lies within about 1e-12 of a border, instead of within 1e-7,
 // which in a row of 128256 tokens is one row in a hundred.  All sums have a fixed order, or are sums of integers.
 //
 // A row lies in the shared memory of a cluster's CTAs and is read from memory once.  Then, by what the row asks for:
 //   top-k (few)       a level that at least top_k tokens reach, from the threads' largest; those tokens, some twice
 //                     top_k, are sorted by one CTA, which does the rest on its own
-//   top-p             sums of w by 64ths of an octave of w (integers, so that atomic additions give the same sums
-//                     in any order); the tokens of the part in which the sum passes its goal are sorted
+//   top-p             the same with a list of some 200 to 400, where these are likely to hold the sum; otherwise sums of w by
+//                     64ths of an octave of w, then a pass with exact sums in which the tokens of the part where the sum
+//                     passes its goal are listed; those are sorted
 //   either, with more equal values than a list holds, or many top-k: the keys' digits one after the other
-// and, but for the first, a last pass with the sums of what is kept.
+// and, where that pass has not done it, a last one with the sums of what is kept.
+//
+// Bound by the passes' instructions (a weight is some 25, half of them f64; issue slots are half busy) and, of a row,
+// by the steps between them, which wait for one another: barriers of a cluster at 0.7 us, a sort at 4.  us: 1 x 128256
+// f32, top-k, 12; a row alone whose top-p keeps half of its tokens 25; 64 x 128256 bf16, plain 22.5, top-k 20.6, flat rows with
+// top-p 60, a mixture 44; 256 x 32000 f32, plain 27.4.  (CTAs of 256 threads are not faster, nor is the entry of a list found by
+// parts of its range instead of by sorting it: equal values meet in one counter.)
 #include <algorithm>
 #include <atomic>
 
@@ -34,6 +41,7 @@ constexpr int kParts = 512;  // of an octave of weights, in the table
 constexpr float kBinUnit = 65536.f;  // of a bin's sum: its largest weight
 constexpr int kMostBytes = 112 * 1024;  // of a CTA, unless no cluster is large enough for that
 constexpr float kNone = -INFINITY, kHuge = 3.4028235e38f;
+constexpr double kNear = 1e-13;  // more than the rounding of a row's sums, of which it is a share
 constexpr double kUnit = 17592186044416.0;  // 2^44: weights as integers, whose sums fit 64 bits
 constexpr double kWhole = 4503599627370496.0, kRound = 1.5 * kWhole;  // 2^52: added, a value's units are whole
 
@@ -669,7 +677,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
           above += __shfl_xor_sync(0xffffffffu, above, off);
         }
         const double goal = share * mass;
-        const bool before = above >= goal && bin > 0, behind = above + head < goal;
+        // (a goal on a bin's border, within rounding, is in either)
+        const double near = head > 0.0 ? kNear * mass : 0.0;
+        const bool before = above >= goal + near && bin > 0, behind = !before && above + head < goal - near;
         if (before) high = bin - 1;
         if (behind) low = bin + 1;
         if (!(before || behind) || low > high) {
@@ -730,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
         }
         __syncthreads();
         if (tid < cluster) {
-          const unsigned long long last = sorted[sh.first_equal];
+          const unsigned long long last = entries > 0 ? sorted[sh.first_equal] : entry(most, 0x7fffffff - first);
           *of_rank(&sh.cut_key, tid) = (uint32_t)(last >> 32);
           *of_rank(&sh.cut_index, tid) = (int)(0xffffffffu - (uint32_t)last);
         }
@@ -973,7 +983,8 @@ cudaError_t launch_sample(const SampleParams& p, int cluster, int sm_count, cuda
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  // More CTAs than run at once: the last to start should not be those that take longest.
+  // More CTAs than run at once: the last to start should not be those that take longest (the mixture above 55 us as they come;
+  // it costs 1 where no row takes long).
   const int sorted_rows = p.rows <= kThreads && (long long)p.rows * cluster > 2 * sm_count;
   return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, RANKS>, p, cluster, slice, sorted_rows);
 }
@@ -982,13 +993,14 @@ template <class T>
 cudaError_t launch_sample(const SampleParams& p, int sm_count, cudaStream_t st) {
   const bool ranks = p.top_k || p.top_p;
   const int head = ranks ? kHead<true> : kHead<false>;
-  // CTAs of a row: as its size needs them where two share a SM; where the row may need its sums by bins, a pass over it
-  // more, while the launch stays within four a SM; without ranks, until there is about one a SM.  us with 2, 4, 8:
-  // 64 x 128256 bf16, some rows with top-k, some with top-p 67, 59, 57, plain 23, 23, 29; with 1, 2, 4: 256 x 32000 f32,
-  // all filters 35, 31, 43, plain 30, 27, 36.
+  // CTAs of a row: as its size needs them where two share a SM; more, without ranks, until there is about one a SM; with
+  // them until there are two, and with both top-k and top-p, where rows that go without top-k may take long, until there
+  // are four, of which two run at once.  us with 2, 4, 8: 64 x 128256 bf16, plain 23, 22.5, 29; top-k of all rows -, 20.6, 31.9; flat
+  // rows with top-p alone 101, 60, 75; a mixture 72, 56, 44, though 20, 19.5, 31 where all its rows have top-k.  With 1, 2, 4:
+  // 256 x 32000 f32, all filters 36, 33, 46, plain 30, 27, 36.
   int cluster = 1;
   while (cluster < kMaxCluster &&
-         ((ranks ? (long long)p.rows * cluster * 2 <= 4 * sm_count : (long long)p.rows * cluster * 10 < 8 * sm_count) ||
+         ((ranks ? (long long)p.rows * cluster * 2 <= (p.top_k && p.top_p ? 4 : 2) * sm_count : (long long)p.rows * cluster * 10 < 8 * sm_count) ||
           head + ((p.vocab + cluster - 1) / cluster + 8) * (int)sizeof(T) > kMostBytes))
     cluster *= 2;
   return ranks ? launch_sample<T, true>(p, cluster, sm_count, st) : launch_sample<T, false>(p, cluster, sm_count, st);
