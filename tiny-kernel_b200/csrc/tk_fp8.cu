@@ -9,9 +9,9 @@
 // infinity or a NaN gets the scale NaN: it reads back as NaN, and so does every sum over it.
 //
 // Bound by memory: one pass, every value is read once into registers and stays there between the sum of squares,
-// the groups' maxima and the codes.  A thread has 32 bytes of consecutive values of a group, so 16 lanes share it, of 16-bit
-// types 8.  us, and the bytes at the rate of a copy: norm 8192 x 4096 bf16 43.2, 36.5; rows 2048 x 14336 bf16 14.9, 13.8;
-// weight 14336 x 4096 f32 44.4, 45.5; norm 4 x 4096 f32 2.5, which is a launch's way through the SMs.
+// the groups' maxima and the codes.  A thread has 32 bytes of consecutive values of a group, so 16 lanes share it, of
+// 16-bit types 8.  us, and the bytes at the rate of a copy: norm 8192 x 4096 bf16 43.2, 36.5; rows 2048 x 14336 bf16
+// 14.9, 13.8; weight 14336 x 4096 f32 44.4, 45.5; norm 4 x 4096 f32 2.5, which is a launch's way through the SMs.
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
@@ -129,10 +129,10 @@ __device__ __forceinline__ GroupScale group_scale(uint32_t most) {
   return {s, __frcp_rn(s)};
 }
 
-// Codes of v[0] / scale .. v[3] / scale.  A product with the reciprocal alone would round some quotients to the wrong side
-// of a tie, of which 16-bit values over their largest make many (7 codes in 10000, bf16); it is corrected by its
-// remainder, after which it is the nearest f32 (Markstein, 1990), unless the remainder is below the least f32: values below
-// about 1e-30.  (With divisions 22 us instead of 15: 2048 x 14336 bf16.)
+// Codes of v[0] / scale .. v[3] / scale.  A product with the reciprocal alone would round some quotients to the wrong
+// side of a tie, of which 16-bit values over their largest make many (7 codes in 10000, bf16); it is corrected by its
+// remainder, after which it is the nearest f32 (Markstein, 1990), unless the remainder is below the least f32: values
+// below about 1e-30.  (With divisions 22 us instead of 15: 2048 x 14336 bf16.)
 __device__ __forceinline__ uint32_t codes4(const float* v, const GroupScale& g) {
   const unsigned long long over = pair_of(g.over, g.over), less = pair_of(-g.scale, -g.scale);
   uint32_t y = 0;
