@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
   float most = kNone;
   auto clean = [](float v) { return fmaxf(v + 0.f, kNone); };
   int begin = 0;
-  if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+  const bool even = reinterpret_cast<uintptr_t>(src) % 16 == 0;  // of all of the row's CTAs: slices are whole vectors
+  if (even) {
     constexpr int kFlight = 4;
     const int vecs = n / kVec;
     for (int i0 = 0; i0 < vecs; i0 += kFlight * kThreads) {
@@ -290,8 +291,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
 #pragma unroll
   for (int off = 16; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
   // Of top-p alone, whether that list is likely to do, by the weights of the warp's largest and of a sample of the others, a
-  // vector of each thread's: a flat row is spared the pass that would show that it does not.
-  const bool guess = quick && !by_k && begin > 0 && !(min_p > 0.f);
+  // vector of each thread's: a flat row is spared the pass that would show that it does not.  (All CTAs have to come to one
+  // answer, or their barriers part: it goes by what they share, and a slice without a vector has an empty sample.)
+  const bool guess = quick && !by_k && even && !(min_p > 0.f);
   const float per_unit = 1.44269504f / heat;
   if (guess) {
     const float level = __shfl_sync(0xffffffffu, s, each - 1);
