@@ -18,9 +18,9 @@ namespace {
 
 constexpr unsigned kErrFp8Wait = 128u;  // a copy or a product never completed
 
-// Waits for the phase of `bar`; gives up, for good, after timeout_ns.  The timer is read once in many tries, since a read
-// takes longer than a phase should be noticed late, and the phase is looked at once more after the last read: lanes of a
-// warp that wait for one phase agree.
+// Waits, all lanes of a warp, for the phase of `bar`; gives up, for good, after timeout_ns.  The timer is read once in many
+// tries, since a read takes longer than a phase should be noticed late.  A lane may give up where another, that read the timer
+// earlier or later, sees the phase complete: what they do next goes by agreed().
 __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t phase, bool& dead, const Fp8MatmulParams& p) {
   if (dead || mbar_try_wait(bar, phase)) return;
   uint64_t t0 = 0;
@@ -37,6 +37,8 @@ __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t phase, bool& 
     late = now - t0 > p.timeout_ns;
   }
 }
+// Whether a lane of the warp gave up: then all do, since instructions of whole warps follow.
+__device__ __forceinline__ bool agreed(bool dead) { return __any_sync(0xffffffffu, dead); }
 
 // D[tmem] (+)= A[smem] x B[smem], e4m3, f32 sums, 32 of k.  The instruction's word is that of f16: type 0 is e4m3 here.
 __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
       const int n0 = t / tiles_m * 128, token0 = t % tiles_m * NT;
       for (int b = b0; b < b1; b += KS) {
         wait_phase(&empty[stage], phase, dead, p);
-        __syncwarp();
+        dead = agreed(dead);
         if (dead) break;
         const int n = min(KS, b1 - b);
         if (elect_one()) {
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
         const int n = min(KS, b1 - b);
         wait_phase(&full[stage], phase, dead, p);
         wait_phase(&sums_empty[d], sums_phase, dead, p);
-        __syncwarp();
+        dead = agreed(dead);
         if (dead) break;
         tcgen05_fence_after();
         if (elect_one()) {
@@ -257,7 +259,8 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
         if (b + KS < b1) fetch(b + KS);
         const int n = min(KS, b1 - b);
         wait_phase(&sums_full[d], phase, dead, p);
-        __syncwarp();
+        __syncwarp();  // (the factors, too)
+        dead = agreed(dead);
         if (dead) break;
         tcgen05_fence_after();
 #pragma unroll
@@ -310,6 +313,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
       __syncwarp();
       wait_phase(&drained, 0, late, p);
     }
+    __syncwarp();
     dead = true;
     __syncthreads();
   }
@@ -494,7 +498,7 @@ __global__ void __launch_bounds__(Some<COLS>::kThreads, 1) fp8_some_kernel(const
       const Tile tile = tile_of(t, tiles_m, tiles_n);
       for (int b = b0; b < b1; ++b) {
         wait_phase(&empty[stage], phase, dead, p);
-        __syncwarp();
+        dead = agreed(dead);
         if (dead) break;
         if (elect_one()) {
           uint8_t* to = smem + stage * M::kStageBytes;
@@ -519,7 +523,7 @@ __global__ void __launch_bounds__(Some<COLS>::kThreads, 1) fp8_some_kernel(const
         const uint32_t to = tmem + d * COLS;
         wait_phase(&full[stage], phase, dead, p);
         wait_phase(&sums_empty[d], sums_phase, dead, p);
-        __syncwarp();
+        dead = agreed(dead);
         if (dead) break;
         tcgen05_fence_after();
         if (elect_one()) {
@@ -553,7 +557,7 @@ __global__ void __launch_bounds__(Some<COLS>::kThreads, 1) fp8_some_kernel(const
         if (b + 1 < b1) next_a = a_scale[b + 1], next_w = w_scale[b + 1];
         const uint32_t at = from + d * COLS;
         wait_phase(&sums_full[d], phase, dead, p);
-        __syncwarp();
+        dead = agreed(dead);
         if (dead) break;
         tcgen05_fence_after();
 #pragma unroll
@@ -597,6 +601,7 @@ __global__ void __launch_bounds__(Some<COLS>::kThreads, 1) fp8_some_kernel(const
       __syncwarp();
       wait_phase(&drained, 0, late, p);
     }
+    __syncwarp();
     dead = true;
     __syncthreads();
   }
@@ -770,7 +775,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
       const Tile tile = tile_of(t, tiles_m, tiles_n);
       for (int b = 0; b < blocks; ++b) {
         wait_phase(&empty[stage], phase, dead, p);
-        __syncwarp();
+        dead = agreed(dead);
         if (dead) break;
         if (elect_one()) {
           uint8_t* to = smem + stage * kManyStageBytes;
@@ -803,7 +808,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
         const uint32_t to = tmem + d * kManyCols;
         wait_phase(&full[stage], phase, dead, p);
         wait_phase(&sums_empty[d], sums_phase, dead, p);
-        __syncwarp();
+        dead = agreed(dead);
         if (dead) break;
         tcgen05_fence_after();
         if (elect_one()) {
@@ -841,7 +846,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
         if (b + 1 < blocks) next_a = a_scale[b + 1], next_w = w_scale[b + 1];
         const uint32_t at = from + d * kManyCols;
         wait_phase(&sums_full[d], phase, dead, p);
-        __syncwarp();
+        dead = agreed(dead);
         if (dead) break;
         tcgen05_fence_after();
 #pragma unroll
@@ -886,6 +891,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
       __syncwarp();
       wait_phase(&drained, 0, late, p);
     }
+    __syncwarp();
     __syncthreads();
   }
   tcgen05_fence_before();
