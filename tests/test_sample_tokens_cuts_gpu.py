@@ -65,7 +65,7 @@ def test_tails_of_one_weight(torch_cuda, tkdev, vocab, low, top_p, rows, dtype):
     for top_k in (None, vocab - 1):  # the latter leaves out the last of the tail
         want, margin, w = tail(vocab if top_k is None else top_k, low, top_p)
         assert margin > off_by(vocab, 4 if vocab > 300000 else 1) / w + vocab * 2.0**-44
-        last = np.where(at < want, want - 1, want - 2)  # of the kept ones, by index
+        last = np.maximum(at, want - 1)  # of the kept ones, by index: the first of the tail, and the one above it
         for u, token in ((1.0, last), (0.0, np.zeros(rows)), (0.5, at)):
             tokens, kept = sample(torch_cuda, tkdev, l, dtype, top_p, u, top_k)
             assert (kept == want).all() and (tokens == token).all()

@@ -7,8 +7,9 @@
 //   random times the sum of all kept.
 //
 // The answer is a whole number that goes by where one sum passes another, so weights and sums are f64: a token differs
-// from that of exact sums where the random number lies within about 1e-12 of a border, instead of within 1e-7,
-// which in a row of 128256 tokens is one row in a hundred.  All sums have a fixed order, or are sums of integers.
+// from that of exact sums where the random number lies within about 1e-13 of a border, instead of within 1e-7,
+// which in a row of 128256 tokens is one row in a hundred.  All sums have a fixed order, or are sums of integers: in units of
+// their bin, so that a goal among 128255 tokens of a weight of 2^-39 is found to the token.
 //
 // A row lies in the shared memory of a cluster's CTAs and is read from memory once.  Then, by what the row asks for:
 //   top-k (few)       a level that at least top_k tokens reach, from the threads' largest; those tokens, some twice
@@ -41,8 +42,9 @@ constexpr int kParts = 512;  // of an octave of weights, in the table
 constexpr float kBinUnit = 65536.f;  // of a bin's sum: its largest weight
 constexpr int kMostBytes = 112 * 1024;  // of a CTA, unless no cluster is large enough for that
 constexpr float kNone = -INFINITY, kHuge = 3.4028235e38f;
-constexpr double kNear = 1e-13;  // more than the rounding of a row's sums, of which it is a share
-constexpr double kUnit = 17592186044416.0;  // 2^44: weights as integers, whose sums fit 64 bits
+// Weights of one bin as whole numbers, whose sums are the same in any order: in a list, and among any number of tokens, the bin's
+// largest has up to 2^51 and 2^44 units, so that 64 bits hold the sums.
+constexpr int kListBits = 51, kRowBits = 44;
 constexpr double kWhole = 4503599627370496.0, kRound = 1.5 * kWhole;  // 2^52: added, a value's units are whole
 
 __device__ __forceinline__ void cluster_sync() {
@@ -99,6 +101,8 @@ struct Shared {
   uint32_t cut_key;
   int cut_index;
   // own
+  double rest;  // of the goal, for that bin
+  int rest_bin;
   int listed, first_equal;
   unsigned long long extra[kWarps];
   int extra_count[kWarps];
@@ -416,8 +420,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
   const float per_bin = endless ? 0.f : fmaxf(-64.f * 1.44269504f / heat, -kHuge);
   auto place_of = [&](float l) -> float { return fminf(fmaxf(l - most, -kHuge) * per_bin, kBins - 1.f); };
   auto bin_of = [&](float l) -> int { return (int)place_of(l); };
-  auto units = [&](double w) -> unsigned long long {  // to the nearest
-    return (unsigned long long)__double_as_longlong(fma(w, kUnit, kWhole)) & ((1ull << 52) - 1);
+  // A power of two: units of weight 1 that give the largest weight of a bin, of 2^(-bin / 64), up to 2^bits.  (Those of weight
+  // 1 itself would leave few to a weight of 2^-39, of which a vocabulary may hold the goal.  The last bin's are those of its
+  // upper end, 2^-32: a weight that is too small for them is too small for a sum of f64 that the row's largest is in.)
+  auto units_of_one = [](int bits, int bin) -> double { return __hiloint2double((1023 + bits + bin / 64) << 20, 0); };
+  auto units = [&](double w, double one) -> unsigned long long {  // to the nearest
+    return (unsigned long long)__double_as_longlong(fma(w, one, kWhole)) & ((1ull << 52) - 1);
+  };
+  auto units_up = [](double v) -> unsigned long long {  // the least whole number that is not below v, 1 at the least
+    const unsigned long long whole = v > 1.0 ? (unsigned long long)v : 1;
+    return whole + ((double)whole < v);
   };
   auto entry = [&](float l, int i) -> unsigned long long {
     return (unsigned long long)key_of(from_f32<T>(l)) << 32 | (0xffffffffu - (uint32_t)(first + i));
@@ -679,19 +691,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
           above += __shfl_xor_sync(0xffffffffu, above, off);
         }
         const double goal = share * mass;
-        // (a goal on a bin's border, within rounding, is in either)
-        const double near = head > 0.0 ? kNear * mass : 0.0;
-        const bool before = above >= goal + near && bin > 0, behind = !before && above + head < goal - near;
+        const bool before = above >= goal && bin > 0, behind = !before && above + head < goal;
         if (before) high = bin - 1;
         if (behind) low = bin + 1;
-        if (!(before || behind) || low > high) {
-          const double rest = (goal - above) * kUnit;  // in units, of what the bin has
-          wanted = rest > 1.0 ? (unsigned long long)rest : 1;
-          wanted += (double)wanted < rest;
+        if (!(before || behind) || step == 0 || (behind && low > high)) {
+          if (tid == 0) sh.rest = goal - above, sh.rest_bin = bin;
           break;
         }
-        bin = before ? max(low, bin - step) : min(high, bin + step);
-        if (low > 0 && high < kBins - 1) bin = (low + high) / 2;
+        if (low > high) {  // on a border, where the sums of its sides, added up in different ways, differ: what lies before it
+          bin = high;
+          step = 0;
+        } else {
+          bin = before ? max(low, bin - step) : min(high, bin + step);
+          if (low > 0 && high < kBins - 1) bin = (low + high) / 2;
+        }
         cluster_sync();  // all have read what the next pass writes
         if (tid == 0) sh.listed = 0;
         __syncthreads();
@@ -708,7 +721,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
     int entries = 0;
     bool fits = true;
     for (int r = 0; r < cluster; ++r) entries += sh.all_listed[r], fits &= sh.all_listed[r] <= kList;
-    if (fits && entries <= kList) {
+    fits = fits && entries <= kList;
+    if (fits) {
       if (rank == 0) {
         unsigned long long v[kPer];
         gather_lists(v);
@@ -718,11 +732,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
         const unsigned long long* sorted = sort_threads<true, kPer>(v, size, &rs.sorted[0][0]);
         if (tid == 0) sh.first_equal = entries - 1;
         __syncthreads();
+        const double one = units_of_one(kListBits, sh.rest_bin);
+        if (by_mass) wanted = units_up(sh.rest * one);
         unsigned long long own[kPer], sum = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           v[i] = kPer * tid + i < entries ? sorted[kPer * tid + i] : 0;
-          own[i] = kPer * tid + i >= entries ? 0 : by_mass ? units(weight(value_of((uint32_t)(v[i] >> 32)))) : 1;
+          own[i] = kPer * tid + i >= entries ? 0 : by_mass ? units(weight(value_of((uint32_t)(v[i] >> 32))), one) : 1;
           sum += own[i];
         }
         inc = sum;
@@ -751,17 +767,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
       cut_value = value_of(sh.cut_key), cut_index = sh.cut_index;
       if (by_mass && least == 0.0) {
         // the kept of the bin, in whole units: listed in any order, their sums are the same
+        const double one = units_of_one(kListBits, sh.rest_bin);
         for (int i = tid; i < sh.listed; i += kThreads) {
           const unsigned long long v = rs.list[i];
           const int at = (int)(0xffffffffu - (uint32_t)v) - first;
           const float l = value_of((uint32_t)(v >> 32));
           if (above_cut(at, l)) {
-            atomicAdd(&sh.extra[at / run], units(weight(l)));
+            atomicAdd(&sh.extra[at / run], units(weight(l), one));
             atomicAdd(&sh.extra_count[at / run], 1);
           }
         }
         __syncthreads();
-        if (lane == 0) sum += (double)sh.extra[warp] * (1.0 / kUnit), count += sh.extra_count[warp];
+        if (lane == 0) sum += (double)sh.extra[warp] / one, count += sh.extra_count[warp];
         summed = true;
       }
       if (!summed) sum = 0.0, count = 0;
@@ -780,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
         if ((key & known) == key_so_far && in_bin(i, l)) {
           const uint32_t b = key >> shift & ((1u << digit) - 1u);
           atomicAdd(&rs.digits.count[b], 1u);
-          if (by_mass) atomicAdd(&rs.digits.mass[b], units(weight(l)));
+          if (by_mass) atomicAdd(&rs.digits.mass[b], units(weight(l), units_of_one(kRowBits, sh.rest_bin)));
         }
       });
       cluster_sync();
@@ -808,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
         if (w < warp) at += sh.scan_mass[w];
         all += sh.scan_mass[w];
       }
-      if (by_mass && known == 0) wanted = min(wanted, all);  // (rounded otherwise than the sums of weights)
+      if (by_mass && known == 0) wanted = min(units_up(sh.rest * units_of_one(kRowBits, sh.rest_bin)), all);  // (rounded otherwise than the sums of weights)
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
         if (at < wanted && wanted <= at + m[j]) {
@@ -825,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
       __syncthreads();
     }
     // Of those with that key the first, by index.
-    const unsigned long long one = equal_mass / equal, ties = min(equal, (wanted - before + one - 1) / one);
+    const unsigned long long a_tie = equal_mass / equal, ties = min(equal, (wanted - before + a_tie - 1) / a_tie);
     const float cut = value_of(key_so_far);
     int same = 0;
     for (int i = r0 + lane; i < min(r1, n); i += 32) same += to_f32(mine[i]) == cut && above_cut(i, cut);
