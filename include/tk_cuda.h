@@ -610,6 +610,11 @@ int tk_qmatmul_int4_path(uint32_t m, uint32_t k, uint32_t n, uint32_t group_size
 /* The same for tk_int4_ffn over [m][hidden] with an intermediate size inter. */
 int tk_int4_ffn_path(uint32_t m, uint32_t hidden, uint32_t inter, uint32_t group_size);
 
+/* How tk_fp8_matmul cuts a product on a device of sm_count SMs (a B200 has 148): plan[0] rows of a (16,
+ * 32, 64: with the weight's rows as the product's; 128; 256: tiles of pairs of CTAs) and plan[1] rows of w
+ * of a tile, plan[2] parts of its k, plan[3] parts of tiles that are worked on at once. */
+int tk_fp8_matmul_plan(uint32_t m, uint32_t k, uint32_t n, uint32_t sm_count, uint32_t plan[4]);
+
 #ifdef __cplusplus
 }
 #endif

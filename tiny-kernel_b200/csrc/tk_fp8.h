@@ -45,6 +45,8 @@ struct Fp8MatmulPlan {
   int box_w() const { return rows == 128 ? cols : 128; }
 };
 Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count);
+// Parts of tiles that are worked on at once, by a CTA each (a pair, of 256 rows): the others follow.
+int fp8_matmul_places(const Fp8MatmulPlan& plan, int m, int n, int sm_count);
 cudaError_t launch_fp8_matmul(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
                               const CUtensorMap& w_map, int sm_count, cudaStream_t st);
 

@@ -377,8 +377,7 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
   attr[1].val.clusterDim.x = (unsigned)plan.split;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  const int ctas = plan.split > 1 ? tiles * plan.split : std::min(tiles, M::kCtas * sm_count);
-  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.gridDim = dim3((unsigned)fp8_matmul_places(plan, p.m, p.n, sm_count));
   cfg.blockDim = dim3(M::kThreads);
   cfg.dynamicSmemBytes = M::kBytes;
   cfg.stream = st;
@@ -651,8 +650,8 @@ cudaError_t has_even_regs(K kernel) {
 }
 
 template <class T, int COLS>
-cudaError_t launch_some(const Fp8MatmulParams& p, int split, const CUtensorMap& a_map, const CUtensorMap& w_map,
-                        int sm_count, cudaStream_t st) {
+cudaError_t launch_some(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
+                        const CUtensorMap& w_map, int sm_count, cudaStream_t st) {
   using M = Some<COLS>;
   constexpr int kMaxDevices = 64;
   static std::atomic<unsigned> asked[kMaxDevices];
@@ -666,22 +665,22 @@ cudaError_t launch_some(const Fp8MatmulParams& p, int split, const CUtensorMap& 
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
   }
-  const int tiles_m = (p.m + 127) / 128, tiles_n = (p.n + COLS - 1) / COLS, tiles = tiles_m * tiles_n;
+  const int tiles_m = (p.m + 127) / 128, tiles_n = (p.n + COLS - 1) / COLS;
   const int wide = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_stride * (long long)sizeof(T))) % 32 == 0;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)split;
+  attr[1].val.clusterDim.x = (unsigned)plan.split;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : std::min(tiles, sm_count)));
+  cfg.gridDim = dim3((unsigned)fp8_matmul_places(plan, p.m, p.n, sm_count));
   cfg.blockDim = dim3(M::kThreads);
   cfg.dynamicSmemBytes = M::kBytes;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, fp8_some_kernel<T, COLS>, a_map, w_map, p, split, tiles_m, tiles_n, wide);
+  cfg.numAttrs = plan.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, fp8_some_kernel<T, COLS>, a_map, w_map, p, plan.split, tiles_m, tiles_n, wide);
 }
 
 // ---- many rows -----------------------------------------------------------------------------------------
@@ -903,8 +902,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp8_many_kernel(const __grid_
 }
 
 template <class T>
-cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, const CUtensorMap& w_map, int sm_count,
-                        cudaStream_t st) {
+cudaError_t launch_many(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
+                        const CUtensorMap& w_map, int sm_count, cudaStream_t st) {
   constexpr int kMaxDevices = 64, smem = kManyStages * kManyStageBytes + 8 * kPatch + 1024;
   static std::atomic<unsigned> asked[kMaxDevices];
   int dev = 0;
@@ -926,7 +925,7 @@ cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, cons
   attr[1].val.clusterDim.x = 2;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(2 * std::min(sm_count / 2, tiles_m * tiles_n)));
+  cfg.gridDim = dim3((unsigned)(2 * fp8_matmul_places(plan, p.m, p.n, sm_count)));
   cfg.blockDim = dim3(kManyThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -938,9 +937,9 @@ cudaError_t launch_many(const Fp8MatmulParams& p, const CUtensorMap& a_map, cons
 template <class T>
 cudaError_t launch_rows(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,
                         const CUtensorMap& w_map, int sm_count, cudaStream_t st) {
-  if (plan.rows == kManyRows) return launch_many<T>(p, a_map, w_map, sm_count, st);
-  if (plan.cols == 256) return launch_some<T, 256>(p, 1, a_map, w_map, sm_count, st);
-  return launch_some<T, 128>(p, plan.split, a_map, w_map, sm_count, st);
+  if (plan.rows == kManyRows) return launch_many<T>(p, plan, a_map, w_map, sm_count, st);
+  if (plan.cols == 256) return launch_some<T, 256>(p, plan, a_map, w_map, sm_count, st);
+  return launch_some<T, 128>(p, plan, a_map, w_map, sm_count, st);
 }
 
 }  // namespace
@@ -974,6 +973,12 @@ Fp8MatmulPlan fp8_matmul_plan(int m, int k, int n, int sm_count) {
   for (int split = 2; split <= kMaxSplit / 2 && split * 4 <= blocks; split *= 2)
     if ((m + 127) / 128 * tiles_n * split <= sm_count) consider(128, 128, split, sm_count, 6.0, 0.4);
   return best;
+}
+
+int fp8_matmul_places(const Fp8MatmulPlan& plan, int m, int n, int sm_count) {
+  const long long parts = (long long)((m + plan.rows - 1) / plan.rows) * ((n + plan.cols - 1) / plan.cols) * plan.split;
+  const int most = plan.rows < 128 ? Few<64>::kCtas * sm_count : plan.rows == kManyRows ? sm_count / 2 : sm_count;
+  return (int)(plan.split > 1 ? parts : std::min<long long>(parts, most));
 }
 
 cudaError_t launch_fp8_matmul(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, const CUtensorMap& a_map,

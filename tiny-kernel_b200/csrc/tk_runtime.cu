@@ -1641,6 +1641,11 @@ int codes_tmap(const void* base, uint64_t k, uint64_t rows, uint64_t stride, int
 
 uint64_t fp8_blocks(uint64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 
+bool fp8_product_in_range(uint32_t m, uint32_t k, uint32_t n) {
+  return k > 0 && n > 0 && m <= kMaxCount - 256 && k <= kMaxCount - 256 && n <= kMaxCount - 256 &&
+         m * fp8_blocks(n) <= kMaxCount;
+}
+
 }  // namespace
 
 int tk_add_rmsnorm_fp8_async(tk_device* d, const void* x, const void* residual, const float* weight, void* sum_out,
@@ -1720,9 +1725,7 @@ int tk_fp8_matmul_async(tk_device* d, const uint8_t* a, const float* a_scales, c
   int st = check_dtype(dtype);
   if (st != TK_OK) return st;
   if ((m && (!a || !a_scales || !out)) || !w || !w_scales) return fail(TK_ERR_ARG, "NULL argument");
-  if (k == 0 || n == 0 || m > kMaxCount - 256 || k > kMaxCount - 256 || n > kMaxCount - 256 ||
-      (uint64_t)m * fp8_blocks(n) > kMaxCount)
-    return fail(TK_ERR_ARG, "product of %u x %u x %u is out of range", m, k, n);
+  if (!fp8_product_in_range(m, k, n)) return fail(TK_ERR_ARG, "product of %u x %u x %u is out of range", m, k, n);
   long long as = 0, ws = 0;
   Fp8MatmulParams p{a_scales, w_scales, out, 0, (int)m, (int)k, (int)n, dtype};
   if ((st = check_stride("a", a_stride, k, &as)) != TK_OK) return st;
@@ -1752,6 +1755,16 @@ int tk_fp8_matmul(tk_device* d, const uint8_t* a, const float* a_scales, const u
   int st = tk_fp8_matmul_async(d, a, a_scales, w, w_scales, out, m, k, n, a_stride, w_stride, out_stride, dtype, nullptr);
   if (st != TK_OK) return st;
   return sync_and_check(d, d->stream);
+}
+
+int tk_fp8_matmul_plan(uint32_t m, uint32_t k, uint32_t n, uint32_t sm_count, uint32_t plan[4]) {
+  if (!plan) return fail(TK_ERR_ARG, "NULL argument");
+  if (m == 0 || !fp8_product_in_range(m, k, n) || sm_count < 2 || sm_count > 4096)
+    return fail(TK_ERR_ARG, "product of %u x %u x %u on %u SMs is out of range", m, k, n, sm_count);
+  const Fp8MatmulPlan p = fp8_matmul_plan((int)m, (int)k, (int)n, (int)sm_count);
+  plan[0] = (uint32_t)p.rows, plan[1] = (uint32_t)p.cols, plan[2] = (uint32_t)p.split;
+  plan[3] = (uint32_t)fp8_matmul_places(p, (int)m, (int)n, (int)sm_count);
+  return TK_OK;
 }
 
 int tk_argmax_async(tk_device* d, const float* x, uint32_t n, uint32_t* out, void* stream) {

@@ -115,6 +115,7 @@ SIGNATURES = {
     "tk_fp8_quantize_async": (i32, [vp] * 4 + [u32] * 5 + [i32, vp]),
     "tk_fp8_matmul": (i32, [vp] * 6 + [u32] * 6 + [i32]),
     "tk_fp8_matmul_async": (i32, [vp] * 6 + [u32] * 6 + [i32, vp]),
+    "tk_fp8_matmul_plan": (i32, [u32, u32, u32, u32, C.POINTER(u32)]),
     "tk_argmax": (i32, [vp, vp, u32, vp]),
     "tk_argmax_async": (i32, [vp, vp, u32, vp, vp]),
     "tk_softmax_sample": (i32, [vp, vp, vp, vp, u32, f32, f32]),

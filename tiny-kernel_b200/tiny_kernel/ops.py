@@ -315,3 +315,11 @@ def path(m, k, n, group_size) -> int:
 def ffn_path(m, hidden, inter, group_size) -> int:
     """int4_ffn's path, with the same codes as path()."""
     return _lib.lib().tk_int4_ffn_path(int(m), int(hidden), int(inter), int(group_size))
+
+
+def fp8_matmul_plan(m, k, n, sm_count=148) -> tuple:
+    """How fp8_matmul cuts a product on that many SMs: (rows of a, rows of w, parts of k) of a tile, and
+    parts of tiles worked on at once."""
+    plan = (_lib.u32 * 4)()
+    check(_lib.lib().tk_fp8_matmul_plan(int(m), int(k), int(n), int(sm_count), plan))
+    return tuple(plan)
