@@ -19,8 +19,20 @@ pub fn blocks(n: u32) u32 {
     return (n + 127) / 128;
 }
 
+/// Bytes from one row of k codes to the next that the product takes: on 16-byte boundaries.
+pub fn rowOf(k: u32) u32 {
+    return (k + 15) / 16 * 16;
+}
+
+/// Whether a buffer holds rows of dim elements, stride apart.
+fn holds(count: usize, rows: u32, stride: u32, dim: u32) bool {
+    return rows == 0 or count >= (@as(usize, rows) - 1) * stride + dim;
+}
+
 /// x + residual (null: x alone), its RMS norm as e4m3 codes [rows][dim] and scales
-/// [rows][blocks(dim)], and the sum itself (a null sum_out: not written).
+/// [rows][blocks(dim)], and the sum itself (a null sum_out: not written).  forward() takes as many
+/// packed rows as codes hold, forwardRows() rows of codes that lie codes_stride bytes apart (0: dim;
+/// LinearFP8 takes rowOf(k)).
 pub const AddRMSNormFP8 = struct {
     device: *cuda.Device,
 
@@ -40,15 +52,38 @@ pub const AddRMSNormFP8 = struct {
         dim: u32,
         eps: f32,
     ) !void {
-        const rows: u32 = @intCast(codes.count / dim);
+        try self.forwardRows(T, x, residual, weight, sum_out, codes, scales, dim, eps,
+            @intCast(codes.count / dim), 0);
+    }
+
+    pub fn forwardRows(
+        self: *AddRMSNormFP8,
+        comptime T: type,
+        x: *cuda.Buffer(T),
+        residual: ?*cuda.Buffer(T),
+        weight: ?*cuda.Buffer(f32),
+        sum_out: ?*cuda.Buffer(T),
+        codes: *cuda.Buffer(u8),
+        scales: *cuda.Buffer(f32),
+        dim: u32,
+        eps: f32,
+        rows: u32,
+        codes_stride: u32,
+    ) !void {
+        const stride = if (codes_stride == 0) dim else codes_stride;
+        if (!holds(x.count, rows, dim, dim) or !holds(codes.count, rows, stride, dim) or
+            !holds(scales.count, rows, blocks(dim), blocks(dim))) return error.InvalidArgument;
+        if (residual) |r| if (!holds(r.count, rows, dim, dim)) return error.InvalidArgument;
+        if (sum_out) |t| if (!holds(t.count, rows, dim, dim)) return error.InvalidArgument;
+        if (weight) |w| if (w.count < dim) return error.InvalidArgument;
         try cuda.check(c.tk_add_rmsnorm_fp8(self.device.ctx, x.handle,
             if (residual) |r| r.handle else null, if (weight) |w| w.handle else null,
-            if (sum_out) |s| s.handle else null, codes.handle, scales.handle, rows, dim, 0, 0, 0, 0,
-            eps, typeOf(T)));
+            if (sum_out) |t| t.handle else null, codes.handle, scales.handle, rows, dim, 0, 0, 0,
+            stride, eps, typeOf(T)));
     }
 };
 
-/// Codes and scales of activations that no norm precedes.
+/// Codes and scales of activations that no norm precedes; forward() and forwardRows() as above.
 pub const QuantizeFP8 = struct {
     device: *cuda.Device,
 
@@ -64,9 +99,24 @@ pub const QuantizeFP8 = struct {
         scales: *cuda.Buffer(f32),
         dim: u32,
     ) !void {
-        const rows: u32 = @intCast(codes.count / dim);
+        try self.forwardRows(T, x, codes, scales, dim, @intCast(codes.count / dim), 0);
+    }
+
+    pub fn forwardRows(
+        self: *QuantizeFP8,
+        comptime T: type,
+        x: *cuda.Buffer(T),
+        codes: *cuda.Buffer(u8),
+        scales: *cuda.Buffer(f32),
+        dim: u32,
+        rows: u32,
+        codes_stride: u32,
+    ) !void {
+        const stride = if (codes_stride == 0) dim else codes_stride;
+        if (!holds(x.count, rows, dim, dim) or !holds(codes.count, rows, stride, dim) or
+            !holds(scales.count, rows, blocks(dim), blocks(dim))) return error.InvalidArgument;
         try cuda.check(c.tk_fp8_quantize(self.device.ctx, x.handle, codes.handle, scales.handle, rows,
-            dim, 1, 0, 0, typeOf(T)));
+            dim, 1, 0, stride, typeOf(T)));
     }
 };
 
@@ -81,7 +131,7 @@ pub const LinearFP8 = struct {
     scales: cuda.Buffer(f32),
 
     pub fn init(device: *cuda.Device, n: u32, k: u32) !LinearFP8 {
-        const row = (k + 15) / 16 * 16;
+        const row = rowOf(k);
         var codes = try cuda.Buffer(u8).initKind(device, @as(usize, n) * row, c.TK_MEM_DEVICE);
         errdefer codes.deinit();
         return .{
@@ -101,6 +151,7 @@ pub const LinearFP8 = struct {
 
     /// Quantises weight, n rows of k values.
     pub fn load(self: *LinearFP8, comptime T: type, weight: *cuda.Buffer(T)) !void {
+        if (!holds(weight.count, self.n, self.k, self.k)) return error.InvalidArgument;
         try cuda.check(c.tk_fp8_quantize(self.device.ctx, weight.handle, self.codes.handle,
             self.scales.handle, self.n, self.k, 128, 0, self.row, typeOf(T)));
     }
@@ -115,7 +166,10 @@ pub const LinearFP8 = struct {
         m: u32,
         a_stride: u32,
     ) !void {
+        const stride = if (a_stride == 0) self.k else a_stride;
+        if (!holds(codes.count, m, stride, self.k) or !holds(scales.count, m, blocks(self.k), blocks(self.k)) or
+            !holds(out.count, m, self.n, self.n)) return error.InvalidArgument;
         try cuda.check(c.tk_fp8_matmul(self.device.ctx, codes.handle, scales.handle, self.codes.handle,
-            self.scales.handle, out.handle, m, self.k, self.n, a_stride, self.row, 0, typeOf(T)));
+            self.scales.handle, out.handle, m, self.k, self.n, stride, self.row, 0, typeOf(T)));
     }
 };
