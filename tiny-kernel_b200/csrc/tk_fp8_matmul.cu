@@ -110,7 +110,7 @@ __device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
 
 // ---- few rows ------------------------------------------------------------------------------------------
 //
-// The weight's rows are the product's 128 rows, the activations its NT columns: the weight is read once, by as many
+// The weight's rows are the product's 128 rows, the activations, NT at the most, its columns: the weight is read once, by as many
 // CTAs as keep memory busy, two a SM.  Where there are fewer tiles than that, the CTAs of a cluster share a tile's blocks
 // of k and add their sums through shared memory, in the order of their ranks; where there are more, a CTA walks over
 // its tiles and its copies go on through their ends.  Bound by memory, and below some 60 MB by the way to the first
@@ -141,7 +141,7 @@ struct Few {
 template <int NT>
 __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_kernel(const __grid_constant__ CUtensorMap a_map,
                                                                        const __grid_constant__ CUtensorMap w_map,
-                                                                       Fp8MatmulParams p, int split, int tiles_m, int tiles) {
+                                                                       Fp8MatmulParams p, int split, int tiles) {
   using M = Few<NT>;
   constexpr int KS = M::kStep, NC = M::kCols, CH = M::kChunk;
   extern __shared__ uint8_t dynamic[];
@@ -170,12 +170,10 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
   unsigned long long acc[NC / 2];
   const int quarter = warp & 3, group = (warp - 2) >> 2, row = quarter * 32 + lane;
   if (warp == 0) {
-    // the weight is read once, unless tiles of other tokens follow
-    const uint64_t once = tiles_m == 1 ? l2_evict_first() : l2_evict_last(), often = l2_evict_last();
+    const uint64_t once = l2_evict_first(), often = l2_evict_last();
     int stage = 0;
     uint32_t phase = 1;  // a barrier's phase before its first counts as complete
     for (int t = first; t < tiles && !dead; t += stride) {
-      const int n0 = t / tiles_m * 128, token0 = t % tiles_m * NT;
       for (int b = b0; b < b1; b += KS) {
         wait_phase(&empty[stage], phase, dead, p);
         dead = agreed(dead);
@@ -185,8 +183,8 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
           uint8_t* to = smem + stage * M::kStageBytes;
           mbar_arrive_expect_tx(&full[stage], n * M::kBlockBytes);
           for (int i = 0; i < n; ++i) {
-            tma_load_2d(to + i * 16384, &w_map, &full[stage], (b + i) * kFp8Block, n0, once);
-            tma_load_2d(to + KS * 16384 + i * NT * kFp8Block, &a_map, &full[stage], (b + i) * kFp8Block, token0, often);
+            tma_load_2d(to + i * 16384, &w_map, &full[stage], (b + i) * kFp8Block, t * 128, once);
+            tma_load_2d(to + KS * 16384 + i * NT * kFp8Block, &a_map, &full[stage], (b + i) * kFp8Block, 0, often);
           }
         }
         __syncwarp();
@@ -231,8 +229,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
     int d = 0, turn = 0;
     uint32_t phase = 0;
     for (int t = first; t < tiles && !dead; t += stride) {
-      const int n0 = t / tiles_m * 128, token0 = t % tiles_m * NT + group * NC;
-      const float* w_scale = p.w_scales + (long long)(t / tiles_m) * blocks;
+      const float* w_scale = p.w_scales + (long long)t * blocks;
 #pragma unroll
       for (int j = 0; j < NC / 2; ++j) acc[j] = 0;
       float next[KS][kEach], next_w[KS];  // multiplied when they are needed: not waited for before that
@@ -242,7 +239,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
           next_w[i] = b + i < b1 ? w_scale[b + i] : 0.f;
 #pragma unroll
           for (int e = 0; e < kEach; ++e) {
-            const int j = e * 32 + lane, token = token0 + j;
+            const int j = e * 32 + lane, token = group * NC + j;
             next[i][e] = b + i < b1 && j < NC && token < p.m ? p.a_scales[(long long)token * blocks + b + i] : 0.f;
           }
         }
@@ -290,12 +287,12 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
         if (++d == M::kSums) d = 0, phase ^= 1;
       }
       if (split > 1 || dead) break;  // one tile a cluster
-      const int n = n0 + row;
+      const int n = t * 128 + row;
       if (n < p.n) {
 #pragma unroll
         for (int j = 0; j < NC / 2; ++j) {
           const float2 v = values_of(acc[j]);
-          const int token = token0 + 2 * j;
+          const int token = group * NC + 2 * j;
           if (token < p.m) store_out(p, token * p.out_stride + n, v.x);
           if (token + 1 < p.m) store_out(p, (token + 1) * p.out_stride + n, v.y);
         }
@@ -318,7 +315,6 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
     __syncthreads();
   }
   if (split > 1) {
-    const int n0 = first / tiles_m * 128, token0 = first % tiles_m * NT;
     float* sums = reinterpret_cast<float*>(smem);  // [NT][128]
     if (warp >= 2) {
 #pragma unroll
@@ -330,9 +326,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
     }
     cluster_sync();
     // the tokens' columns over the CTAs, four rows a thread, all CTAs' values at once
-    const int tokens = min(NT, p.m - token0), j0 = tokens * rank / split, j1 = tokens * (rank + 1) / split;
+    const int j0 = p.m * rank / split, j1 = p.m * (rank + 1) / split;
     for (int i = threadIdx.x; !dead && i < (j1 - j0) * 32; i += M::kThreads) {
-      const int j = j0 + i / 32, row4 = i % 32 * 4, n = n0 + row4;
+      const int j = j0 + i / 32, row4 = i % 32 * 4, n = first * 128 + row4;
       if (n >= p.n) continue;
       const uint32_t from = smem_addr(sums + j * 128 + row4);
       float4 v[kMaxSplit];
@@ -343,7 +339,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, Few<NT>::kCtas) fp8_few_ker
 #pragma unroll
       for (int r = 0; r < kMaxSplit; ++r)
         if (r < split) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
-      store_four(p, (token0 + j) * p.out_stride + n, p.n - n, sum);
+      store_four(p, j * p.out_stride + n, p.n - n, sum);
     }
     __syncwarp();
     cluster_sync();
@@ -369,7 +365,6 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) asked[dev].store(gen, std::memory_order_release);
   }
-  const int tiles_m = (p.m + NT - 1) / NT, tiles = (p.n + 127) / 128 * tiles_m;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -383,7 +378,7 @@ cudaError_t launch_few(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, cons
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = plan.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, fp8_few_kernel<NT>, a_map, w_map, p, plan.split, tiles_m, tiles);
+  return cudaLaunchKernelEx(&cfg, fp8_few_kernel<NT>, a_map, w_map, p, plan.split, (p.n + 127) / 128);
 }
 
 // ---- tiles with the activations as rows ------------------------------------------------------------------
