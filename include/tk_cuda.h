@@ -465,11 +465,11 @@ int tk_kv4_attention_async(tk_device *dev, const tk_kv4_cache *cache, const void
  *   codes   u8 [rows][dim], e4m3 (4 bits of exponent, 3 of mantissa, up to 448; 0x7f and 0xff NaN)
  *   scales  f32 [rows][ceil(dim/128)] of activations, [ceil(rows/128)][ceil(dim/128)] of weights
  *   value = code * scale,  scale = max(largest magnitude of the group / 448, 2^-126), code the nearest
- *   to value / scale (ties to even).  A group with an infinity or a NaN gets the scale NaN and codes 0.
+ *   to value / scale in f32 (ties to even).  A group with an infinity or a NaN gets the scale NaN and codes 0.
  * Strides of rows are in elements, 0: packed.  No call keeps state, allocates or waits, and all can be
  * captured; calls on different streams or from different threads are independent as long as they share
- * no output.  (A wait of the product that gives up sets the device's error word, as above.)  A call of no rows does nothing; its rows'
- * pointers may be NULL. */
+ * no output.  (A wait of the product that gives up sets the device's error word, as above.)  A call of no
+ * rows does nothing; its rows' pointers may be NULL. */
 
 /* s = x + residual (residual NULL: x), in f32;  sum_out = s rounded to dtype (NULL: not written; may be x
  * or residual, same stride, else must not overlap them);  y = s * rsqrt(mean(s^2) + eps) * weight (weight
@@ -495,8 +495,10 @@ int tk_fp8_quantize_async(tk_device *dev, const void *x, uint8_t *codes, float *
 
 /* out[m][n] = sum_k a[m][k] * w[n][k] of the values that the codes stand for: a activations [m][k], w a
  * weight [n][k] (out_dim, in_dim).  Sums over a block of 128 on the tensor cores, over the blocks in f32;
- * rounded once to dtype.  The order of the sums is fixed (the same bits from run to run).  m, k, n of
- * any size; the rows of a and w on 16-byte boundaries (pointers, and strides of multiples of 16). */
+ * rounded once to dtype.  The two scales of a block are multiplied first, in f32: where that is above the
+ * largest f32 (scales of 1e19 on both sides, of values of 1e21) outputs are infinite or NaN; where it is
+ * below 2^-126 it is a multiple of 2^-149.  The order of the sums is fixed (the same bits from run to run).
+ * m, k, n of any size; the rows of a and w on 16-byte boundaries (pointers, and strides of multiples of 16). */
 int tk_fp8_matmul(tk_device *dev, const uint8_t *a, const float *a_scales, const uint8_t *w,
                   const float *w_scales, void *out, uint32_t m, uint32_t k, uint32_t n,
                   uint32_t a_stride, uint32_t w_stride, uint32_t out_stride, int dtype);

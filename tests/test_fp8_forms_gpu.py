@@ -64,6 +64,22 @@ def test_nan_stays_in_its_rows_and_columns(torch_cuda, tkdev, shape):
 
 
 @named
+def test_scales_as_far_as_their_product_fits(torch_cuda, tkdev, shape):
+    """Blocks whose scales multiply to 2^127, 2^-126 and, below that, a multiple of 2^-149, over sums of 0, 1 and -1: exact."""
+    torch, (m, k, n) = torch_cuda, shape
+    stride, blocks = -(-k // 16) * 16, -(-k // 128)
+    for a_scale, w_scale in ((2.0**100, 2.0**27), (2.0**-120, 2.0**-6), (2.0**-126, 2.0**-20), (1.0, 2.0**127)):
+        a, w = (torch.zeros((r, stride), dtype=torch.uint8, device="cuda") for r in (m, n))
+        a[:, 0] = 0x38                         # 1 in the first place of every row,
+        w[::3, 0], w[1::3, 0] = 0x38, 0xB8     # 1, -1 and 0 in that of the columns
+        scales = [torch.full((r, blocks), s, device="cuda") for r, s in ((m, a_scale), (-(-n // 128), w_scale))]
+        got = product(torch, tkdev, [a, scales[0], w, scales[1]], m, k, n, "f32")
+        want = torch.zeros(n, device="cuda")
+        want[::3], want[1::3] = a_scale * w_scale, -a_scale * w_scale
+        assert torch.equal(got, want.expand(m, n))
+
+
+@named
 def test_the_same_bits_whenever_it_runs(torch_cuda, tkdev, shape):
     """Again, on two streams at once with another product's operands, and captured and replayed over other operands."""
     torch, (m, k, n) = torch_cuda, shape
