@@ -10,8 +10,11 @@
 //
 // Bound by memory: one pass, every value is read once into registers and stays there between the sum of squares,
 // the groups' maxima and the codes.  A thread has 32 bytes of consecutive values of a group, so 16 lanes share it, of
-// 16-bit types 8.  us, and the bytes at the rate of a copy: norm 8192 x 4096 bf16 43.2, 36.5; rows 2048 x 14336 bf16
-// 14.9, 13.8; weight 14336 x 4096 f32 44.4, 45.5; norm 4 x 4096 f32 2.5, which is a launch's way through the SMs.
+// 16-bit types 8.  us, and the bytes at the rate of a copy: norm 8192 x 4096 bf16 45.8, 36.5; rows 2048 x 14336 bf16
+// 15.4, 13.8; weight 14336 x 4096 f32 45.9, 45.5; norm 4 x 4096 f32 2.6, which is a launch's way through the SMs.  Rows that
+// are not whole chunks, or off their boundary, go by elements, 8 or 16 neighbours a thread, which is several times as
+// long: 8192 x 2000 and 2008 bf16 26 and 145, as rows alone 9.7 and 47.  f32 rows wider than 8192 have four chunks a
+// thread in 64 registers and spill some: 2048 x 8192 and 16384 f32 43 and 94, for 34 and 68.
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
@@ -271,7 +274,7 @@ template <class T, bool FAST>
 __global__ void __launch_bounds__(kThreads) fp8_quantize_rows_kernel(Fp8RowsParams p, unsigned groups, unsigned total) {
   constexpr int kE = kChunk<T>, kLanes = kFp8Block / kE;
   after_previous();
-  // (a thread with two or four groups is slower: 2048 x 14336 bf16 14.7 and 16.4 us instead of 14.3)
+  // (a thread with two or four groups was slower by 3 and 15 %: 2048 x 14336 bf16)
   const unsigned group = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;  // (threads may be more than 2^32)
   const int lane = threadIdx.x % kLanes, at = (int)(group % groups) * kFp8Block + lane * kE;
   const long long row = group / groups;

@@ -110,11 +110,12 @@ __device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
 
 // ---- few rows ------------------------------------------------------------------------------------------
 //
-// The weight's rows are the product's 128 rows, the activations, NT at the most, its columns: the weight is read once, by as many
-// CTAs as keep memory busy, two a SM.  Where there are fewer tiles than that, the CTAs of a cluster share a tile's blocks
-// of k and add their sums through shared memory, in the order of their ranks; where there are more, a CTA walks over
+// The weight's rows are the product's 128 rows, the activations, NT at the most, its columns: the weight is read once, by
+// as many CTAs as keep memory busy, two a SM.  Where there are fewer tiles than that, the CTAs of a cluster share a tile's
+// blocks of k and add their sums through shared memory, in the order of their ranks; where there are more, a CTA walks over
 // its tiles and its copies go on through their ends.  Bound by memory, and below some 60 MB by the way to the first
-// product and from the last: 48 x 4096 x 128256 (525 MB) 5.3 TB/s, 1 x 4096 x 14336 (59 MB) 12.4 us, 4.7 TB/s.
+// product and from the last: 48 x 4096 x 128256 (525 MB of weight) 92 to 110 us, 4.8 to 5.7 TB/s; 1 x 4096 x 14336 (59 MB)
+// 12.6, 4.7 TB/s, with a CTA on 112 of 148 SMs; 32 x 14336 x 4096 14.0, 256 CTAs on 148 SMs.
 //
 // Waits of a cluster's CTAs for one another need all of them to get their tensor memory.  They do: two CTAs of this form
 // have the 512 columns of a SM at most and leave no shared memory for a third, those below fill a SM's shared memory
@@ -436,7 +437,7 @@ __device__ __forceinline__ void store_rows(const Fp8MatmulParams& p, int row, in
 // form for few rows it is one for each column, read from shared memory for each product).  Accumulators fill tensor
 // memory.  CTAs of a cluster share a tile's k (of 128 columns), or walk over tiles, as above.  Bound by the chain of one
 // block after the other (0.4 to 0.5 us: products, word, sums, word back) where a CTA has a tile or two: 777 x 2000 x 5003
-// 16.7 us, of which tiles take 8.
+// 17.2 us over the same buffers, of which tiles take 8, and 21.6 with operands and outputs in memory.
 
 // The registers of a launch of three warpgroups, 168 for each thread, are handed from the first group, of copies and
 // products, to the two of sums, where a thread holds 128 of them: 40 and 2 x 232 of 3 x 168.
@@ -685,7 +686,7 @@ cudaError_t launch_some(const Fp8MatmulParams& p, const Fp8MatmulPlan& plan, con
 // CTA would bring 48 KB a block to its 128 x 256 products, and writing and reading them would take shared memory
 // longer than the products take.)  A thread adds half of a row in registers, so that its scale is one number a block:
 // sum += scale * product.  Two accumulators of 256 columns fill tensor memory: one is added up while the other's
-// products run.  Pairs of CTAs walk over the tiles.  8192 x 4096 x 14336: 440 to 450 us in bursts (2.2 PFLOP/s), 500 to
+// products run.  Pairs of CTAs walk over the tiles.  8192 x 4096 x 14336: 425 to 450 us in bursts (2.2 PFLOP/s), 480 to
 // 520 in long runs, where power limits the clock; the tensor pipe is busy 55 % of the time, and waits for the sums of
 // the block before the last (a block's 128 x 256 values through registers take about as long as its products).
 

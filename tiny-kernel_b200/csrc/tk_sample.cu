@@ -20,10 +20,12 @@
 //   either, with more equal values than a list holds, or many top-k: the keys' digits one after the other
 // and, where that pass has not done it, a last one with the sums of what is kept.
 //
-// Bound by the passes' instructions (a weight is some 25, half of them f64; issue slots are half busy) and, of a row,
-// by the steps between them, which wait for one another: barriers of a cluster at 0.7 us, a sort at 4.  us: 1 x 128256
-// f32, top-k, 12; a row alone whose top-p keeps half of its tokens 25; 64 x 128256 bf16, plain 22.5, top-k 20.6, flat rows with
-// top-p 60, a mixture 44; 256 x 32000 f32, plain 27.4.  (CTAs of 256 threads are not faster, nor is the entry of a list found by
+// Bound by the passes' instructions (plain f32 rows: 67 a token in all, of which the weight is some 25, half of them f64; ALU the
+// busiest pipe at 45 %, issue slots 62 % busy) and, of a row, by the steps between them, which wait for one another:
+// barriers of a cluster at 0.7 us, a sort at 4.  us: 1 x 128256 f32, all filters, 11 over the same logits, 14 from memory; a
+// row alone whose top-p keeps half of its tokens 25; 64 x 128256 bf16, plain 23.5, top-k 16, flat rows with top-p 61, a
+// mixture 43.6; 256 x 32000 f32, plain 28.3.  Rows off their 16-byte boundary are read by elements: 64 x 50257 bf16 13.2, plain,
+// 33.8, mixed, and 50256 12.5 and 32.5.  (CTAs of 256 threads are not faster, nor is the entry of a list found by
 // parts of its range instead of by sorting it: equal values meet in one counter.)
 #include <algorithm>
 #include <atomic>
